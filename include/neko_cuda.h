@@ -8,7 +8,8 @@
  *                   parameter blocks the GLSL shaders take. nekochat_b200/csrc/cuda_compute.cpp wraps it as a
  *                   C++ ComputeBackend subclass so Model::startGpu (model.cpp:137-148) can pick it.
  *  2. neko_op_*     single operators on device pointers (weight codec, dequant matmul, norms, softmax,
- *                   attention), for the operator sweep and for callers that manage their own memory.
+ *                   attention; the paged cache), for the operator sweep and for callers that manage their own
+ *                   memory.
  *  3. neko_model_*  a native GPT-2 / Qwen3 runner built on the same kernels: fused decode steps replayed as
  *                   CUDA graphs, plus batched multi-sequence decode (which the single-sequence
  *                   Model::forward of app/architecture/shared/cpp/model.h:72 cannot express).
@@ -168,6 +169,89 @@ int neko_op_sample(float* logits, int rows, int V, const int* history, const int
  * Codes 0x7F / 0xFF decode to +-480 as in the reference's table. */
 int neko_op_fp8_block_dequant(const uint8_t* codes, int64_t rows, int64_t cols, const float* scales,
                               int64_t scale_rows, int64_t scale_cols, float* out, void* stream);
+
+/* ---- paged key/value cache (no counterpart in the engine, whose caches are one contiguous slot per sequence)
+ *
+ * Keys and values live in pools of pages; page p holds page_size tokens of every KV head, [n_kv][page_size][head_dim]
+ * contiguous, pages page_stride elements apart (so one pool may interleave K and V pages). table[s][i] is the page of
+ * sequence s's tokens [i * page_size, (i + 1) * page_size). An entry outside [0, num_pages), or past max_pages, is a
+ * page that is not resident: nothing is stored to it and its tokens are masked.
+ * NEKO_T_E4M3 pages hold 8-bit codes (cvt.rn.satfinite) and a scale for each (page, KV head), scale_stride floats
+ * between pages, n_kv contiguous: value = code * scale. The scales that the append writes are powers of two. */
+enum neko_type { NEKO_T_F32 = 0, NEKO_T_F16 = 1, NEKO_T_BF16 = 2, NEKO_T_E4M3 = 3 };
+typedef struct neko_paged_cache {
+    void* k_pages;          /* device; type NEKO_T_F16 or NEKO_T_E4M3, 16-byte aligned */
+    void* v_pages;
+    float* k_scale;         /* device; NEKO_T_E4M3 only */
+    float* v_scale;
+    const int32_t* table;   /* device [n_seq][table_stride] */
+    int64_t page_stride;    /* elements; page_stride * element size a multiple of 16 bytes */
+    int64_t scale_stride;
+    int64_t table_stride;
+    int32_t type;
+    int32_t n_seq;
+    int32_t max_pages;      /* table entries per sequence */
+    int32_t num_pages;
+    int32_t n_kv;
+    int32_t page_size;      /* 16, 32, 64 or 128 */
+    int32_t head_dim;       /* 32, 64 or 128 */
+    int32_t reserved;
+} neko_paged_cache;
+/* Appends keys and values: token i of sequence s (row q_start[s] + i of q, k, v; i < q_start[s + 1] - q_start[s], at
+ * most max_new; q_start NULL: one token per sequence) goes to position start[s] + i. On the way q and k get the
+ * per-head RMSNorm (x * rsqrt(mean x^2 + eps) * gain; gains NULL: none) and the rotation by the table cs
+ * [cs_rows][rot / 2] of (cos, sin) over the first rot of each head's head_dim values: pairs (j, j + rot / 2), or
+ * (2j, 2j + 1) when interleaved (rot a multiple of 8; 0: no rotation). k and v are rounded once, from f32.
+ * A sequence with start[s] < 0 is inactive: nothing is stored, its q rows come out as zeros. Positions at or past
+ * cs_rows are not stored either and report a device error.
+ * NEKO_T_E4M3: a (page, head) that gets tokens takes as scale the smallest power of two (at least 2^-100) with which
+ * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
+ * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new
+ * (exact, but for codes that become subnormal). Infinities are stored as +-448 * scale, NaN as NaN.
+ * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous. */
+typedef struct neko_paged_append_args {
+    neko_paged_cache cache;
+    const void *q, *k, *v;
+    void* q_out;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head; /* element strides */
+    const int32_t* start;   /* device [n_seq]: tokens the cache holds before the call */
+    const int32_t* q_start; /* device [n_seq + 1] or NULL */
+    const float* cs;
+    const float *q_gain, *k_gain; /* device [head_dim], both or neither (k_gain alone when q is NULL) */
+    int32_t type;           /* of q, k, v, q_out: NEKO_T_F32, NEKO_T_F16, NEKO_T_BF16 */
+    int32_t tokens;         /* rows of q, k, v */
+    int32_t n_head;
+    int32_t max_new;
+    int32_t rot, cs_rows, interleaved;
+    float eps;
+} neko_paged_append_args;
+int neko_op_paged_append(const neko_paged_append_args* args, void* stream);
+/* Attention over the cache. Row q_start[s] + i of q is at position pos = kv_len[s] - n + i of its sequence, n its
+ * new tokens (q_start NULL: one per sequence; they are in the cache already). Per query head h (KV head
+ * h / (n_head / n_kv)) and key j: z = scale * q . k_j; with softcap > 0, z = softcap * tanh(z / softcap); with slopes,
+ * z += slopes[h] * (j - pos). Key j is seen when its page is resident, j < kv_len[s], and j <= pos with (window == 0
+ * or pos - j < window), or j < prefix[s] (prefix NULL: none). out = sum_j softmax(z)_j v_j over the keys seen, zeros
+ * when there are none. A value that is not seen has no effect, whatever it holds. Sums, maxima and accumulators are f32;
+ * NEKO_T_F32 queries and weights enter the tensor cores as f16 hi + lo (22 bits), 16-bit ones as one f16.
+ * n_head a multiple of n_kv. out rows have type `type` and strides o_token, o_head. */
+typedef struct neko_paged_attention_args {
+    neko_paged_cache cache;
+    const void* q;
+    void* out;
+    int64_t q_token, q_head, o_token, o_head;
+    const int32_t* kv_len;  /* device [n_seq], new tokens included */
+    const int32_t* q_start; /* device [n_seq + 1] or NULL */
+    const float* slopes;    /* device [n_head] or NULL */
+    const int32_t* prefix;  /* device [n_seq] or NULL */
+    int32_t type;
+    int32_t tokens;
+    int32_t n_head;
+    int32_t max_new;
+    int32_t window;
+    float scale, softcap;
+    int32_t reserved;
+} neko_paged_attention_args;
+int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------------ 3. native model runner */
 

@@ -1,6 +1,7 @@
 """Single operators of the C ABI (``neko_op_*``) on torch CUDA tensors. torch is only the device allocator and
 stream here; the arithmetic is the library's."""
 import ctypes as C
+import struct
 
 from . import NekoError, check, lib
 
@@ -137,4 +138,185 @@ def attention(q, q_stride, k_cache, v_cache, T, n_head, n_kv, hd, pos0):
     out = torch.empty((T, n_head * hd), dtype=torch.float32, device=q.device)
     check(lib().neko_op_attention(_ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(out), T, n_head, n_kv, hd,
                                   pos0, _stream()), "attention")
+    return out
+
+
+# ------------------------------------------------------------------ paged key/value cache
+# neko_paged_cache, neko_paged_append_args and neko_paged_attention_args (include/neko_cuda.h)
+_CACHE = "5P3q8i"
+_APPEND = struct.Struct("@" + _CACHE + "4P8q5P7if")
+_ATTEND = struct.Struct("@" + _CACHE + "2P4q4P5i2fi")
+_types = {}
+
+
+def _type(t, what):
+    """neko_type of a tensor's dtype (uint8 and float8_e4m3fn both hold E4M3 codes)."""
+    if not _types:
+        import torch
+        _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.uint8: 3})
+    try:
+        return _types[t.dtype]
+    except KeyError:
+        raise NekoError(f"{what}: {t.dtype} is not supported") from None
+
+
+def _rows(t, what, type_, n, hd, dev):
+    """(pointer, token stride, head stride) of [tokens][heads][hd] rows."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or sh[2] != hd or sh[0] != n or (st[2] != 1 and hd > 1) or t.device != dev or _type(t, what) != type_:
+        raise NekoError(f"{what}: [tokens][heads][head_dim] rows on the cache's device, values contiguous, one type")
+    return t.data_ptr(), st[0], st[1]
+
+
+def _ints(t, what, n, dev):
+    if t is None:
+        return 0
+    if t.dtype.itemsize != 4 or t.dtype.is_floating_point or t.dim() != 1 or t.shape[0] != n or t.device != dev or \
+            (n > 1 and t.stride(0) != 1):
+        raise NekoError(f"{what}: {n} contiguous int32 on the cache's device")
+    return t.data_ptr()
+
+
+def _floats(t, what, n, dev):
+    if t is None:
+        return 0
+    if str(t.dtype) != "torch.float32" or t.numel() != n or t.device != dev or not t.is_contiguous():
+        raise NekoError(f"{what}: {n} contiguous float32 on the cache's device")
+    return t.data_ptr()
+
+
+def _cache(k_pages, v_pages, k_scale, v_scale, table):
+    """The fields of neko_paged_cache, (n_seq, n_kv, head dim, device)."""
+    dev, sh, st = k_pages.device, k_pages.shape, k_pages.stride()
+    if dev.type != "cuda" or len(sh) != 4 or v_pages.shape != sh or v_pages.stride() != st or v_pages.device != dev or \
+            v_pages.dtype != k_pages.dtype:
+        raise NekoError("paged cache: k_pages and v_pages are alike [pages][kv heads][page][head_dim] CUDA tensors")
+    pages, n_kv, ps, hd = sh
+    if st[3] != 1 or st[2] != hd or (st[1] != ps * hd and n_kv > 1):
+        raise NekoError("paged cache: a page is contiguous")
+    type_ = _type(k_pages, "paged cache")
+    ks = vs = sst = 0
+    if type_ == 3:
+        if k_scale is None or v_scale is None:
+            raise NekoError("paged cache: 8-bit pages need k_scale and v_scale")
+        sst = k_scale.stride(0)
+        for t in (k_scale, v_scale):
+            if t.shape != (pages, n_kv) or str(t.dtype) != "torch.float32" or t.device != dev or t.stride(0) != sst or \
+                    (n_kv > 1 and t.stride(1) != 1):
+                raise NekoError("paged cache: scales are alike [pages][kv heads] float32")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    if table.dim() != 2 or table.dtype.itemsize != 4 or table.dtype.is_floating_point or table.device != dev or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise NekoError("paged cache: the table is [sequences][pages] int32")
+    n_seq, width = table.shape
+    page_stride = st[0] if pages > 1 else n_kv * ps * hd
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), page_stride, sst,
+            table.stride(0) if n_seq > 1 else width, type_, n_seq, width, pages, n_kv, ps, hd, 0), n_seq, n_kv, hd, dev
+
+
+def _on(dev):
+    """The current stream of the tensors' device, which has to be the current one."""
+    import torch
+    if torch.cuda.current_device() != dev.index:
+        raise NekoError(f"paged cache: the tensors are on {dev}, the current device is {torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def rope_table(positions, rot, theta, scaling="none", factor=1.0, original=0, beta_fast=32.0, beta_slow=1.0,
+               device="cuda"):
+    """The (cos, sin) table [positions][rot / 2][2] of paged_append, computed in double like Qwen3Model::ropeTable
+    (qwen3_model.cpp) and rounded once. Pair j turns by pos * theta^(-2j / rot). Longer contexts (factor times the
+    `original` positions a model was trained on):
+      "linear" positions divided by factor;
+      "ntk"    theta raised to theta * factor^(rot / (rot - 2)), so the slowest pair is slowed by factor;
+      "yarn"   pairs that turn more than beta_fast times over `original` positions keep their speed, those below
+               beta_slow turns are slowed by factor, a linear ramp between, and cos and sin are multiplied by
+               0.1 ln(factor) + 1 (YaRN, Peng et al. 2023)."""
+    import math
+
+    import numpy as np
+    import torch
+    if rot <= 0 or rot % 8 or positions <= 0 or theta <= 0 or factor < 1:
+        raise NekoError("rope_table: rot a positive multiple of 8, positions and theta positive, factor >= 1")
+    half = rot // 2
+    j = np.arange(half, dtype=np.float64)
+    gain = 1.0
+    if scaling == "ntk":
+        theta = theta * factor ** (rot / (rot - 2))
+    freq = theta ** (-j / half)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if original <= 0:
+            raise NekoError("rope_table: yarn needs the original context length")
+        pair = lambda turns: half * math.log(original / (turns * 2 * math.pi)) / math.log(theta)  # noqa: E731
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), half - 1)
+        slow = np.clip((j - low) / max(high - low, 1e-3), 0, 1)
+        freq = freq * (1 - slow) + freq / factor * slow
+        gain = 0.1 * math.log(factor) + 1.0
+    elif scaling not in ("none", "ntk"):
+        raise NekoError(f"rope_table: unknown scaling {scaling!r}")
+    ang = np.arange(positions, dtype=np.float64)[:, None] * freq
+    return torch.from_numpy(np.stack([np.cos(ang) * gain, np.sin(ang) * gain], -1).astype(np.float32)).to(device)
+
+
+def paged_append(k, v, k_pages, v_pages, table, start, k_scale=None, v_scale=None, q_start=None, max_new=1, q=None,
+                 cs=None, interleaved=False, q_gain=None, k_gain=None, eps=1e-6, q_out=None):
+    """neko_op_paged_append: k, v [tokens][kv heads][hd] (any token and head stride) go to the pages, after the
+    per-head norm (k_gain) and the rotation by cs (rope_table) of k. Sequence s's rows are q_start[s] ..
+    q_start[s + 1] - 1 (q_start None: row s) and go to positions start[s], start[s] + 1, ..; at most max_new per
+    sequence. Returns q with its norm (q_gain) and rotation applied (into q_out, which may be q; a new tensor when
+    None), or None without q."""
+    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table)
+    type_ = _type(k, "paged_append k")
+    tokens = k.shape[0]
+    if k.shape[1] != n_kv or v.shape[1] != n_kv:
+        raise NekoError("paged_append: k and v have the cache's KV heads")
+    kp = _rows(k, "paged_append k", type_, tokens, hd, dev)
+    vp = _rows(v, "paged_append v", type_, tokens, hd, dev)
+    qp = op = (0, 0, 0)
+    heads = 0
+    if q is not None:
+        heads = q.shape[1]
+        qp = _rows(q, "paged_append q", type_, tokens, hd, dev)
+        if q_out is None:
+            q_out = q.new_empty((tokens, heads, hd))
+        elif q_out.shape != q.shape:
+            raise NekoError("paged_append: q_out is shaped like q")
+        op = _rows(q_out, "paged_append q_out", type_, tokens, hd, dev)
+    rot = rows = csp = 0
+    if cs is not None:
+        if cs.dim() != 3 or cs.shape[2] != 2:
+            raise NekoError("paged_append: cs is [positions][rot / 2][2]")
+        rows, rot = cs.shape[0], 2 * cs.shape[1]
+        csp = _floats(cs, "paged_append cs", rows * rot, dev)
+    args = _APPEND.pack(*fields, qp[0], kp[0], vp[0], op[0], *qp[1:], *kp[1:], *vp[1:], *op[1:],
+                        _ints(start, "paged_append start", n_seq, dev),
+                        _ints(q_start, "paged_append q_start", n_seq + 1, dev), csp,
+                        _floats(q_gain, "paged_append q_gain", hd, dev), _floats(k_gain, "paged_append k_gain", hd, dev),
+                        type_, tokens, heads, max_new, rot, rows, 1 if interleaved else 0, eps)
+    check(lib().neko_op_paged_append(args, _on(dev)), "paged_append")
+    return q_out if q is not None else None
+
+
+def paged_attention(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=None, q_start=None, max_new=1,
+                    scale=None, softcap=0.0, window=0, slopes=None, prefix=None, out=None):
+    """neko_op_paged_attention: q [tokens][heads][hd] over the cached keys and values; kv_len [sequences] counts the
+    new tokens, which are in the cache already. scale: 1 / sqrt(hd) when None; softcap, window, slopes [heads] and
+    prefix [sequences] as the header defines them. Returns out (shaped and typed like q)."""
+    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table)
+    type_ = _type(q, "paged_attention q")
+    tokens, heads = q.shape[0], q.shape[1]
+    qp = _rows(q, "paged_attention q", type_, tokens, hd, dev)
+    if out is None:
+        out = q.new_empty((tokens, heads, hd))
+    elif out.shape != q.shape:
+        raise NekoError("paged_attention: out is shaped like q")
+    op = _rows(out, "paged_attention out", type_, tokens, hd, dev)
+    args = _ATTEND.pack(*fields, qp[0], op[0], *qp[1:], *op[1:], _ints(kv_len, "paged_attention kv_len", n_seq, dev),
+                        _ints(q_start, "paged_attention q_start", n_seq + 1, dev),
+                        _floats(slopes, "paged_attention slopes", heads, dev),
+                        _ints(prefix, "paged_attention prefix", n_seq, dev), type_, tokens, heads, max_new, window,
+                        hd ** -0.5 if scale is None else scale, softcap, 0)
+    check(lib().neko_op_paged_attention(args, _on(dev)), "paged_attention")
     return out

@@ -177,7 +177,7 @@ int neko_op_fp8_block_dequant(const uint8_t* codes, int64_t rows, int64_t cols, 
  * sequence s's tokens [i * page_size, (i + 1) * page_size). An entry outside [0, num_pages), or past max_pages, is a
  * page that is not resident: nothing is stored to it and its tokens are masked.
  * NEKO_T_E4M3 pages hold 8-bit codes (cvt.rn.satfinite) and a scale for each (page, KV head), scale_stride floats
- * between pages, n_kv contiguous: value = code * scale. The scales that the append writes are powers of two. */
+ * between pages, n_kv contiguous: value = code * scale, the scale not negative. The append writes powers of two. */
 enum neko_type { NEKO_T_F32 = 0, NEKO_T_F16 = 1, NEKO_T_BF16 = 2, NEKO_T_E4M3 = 3 };
 typedef struct neko_paged_cache {
     void* k_pages;          /* device; type NEKO_T_F16 or NEKO_T_E4M3, 16-byte aligned */

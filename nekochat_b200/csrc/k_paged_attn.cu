@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "paged.cuh"
+#include "paged_math.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -26,15 +27,8 @@ namespace neko {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 8;
-constexpr int kNoRow = -(1 << 30);  // the position of a column without a row: it sees nothing
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -45,9 +39,6 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
     return d;
 }
-// tanh(x) = 1 - 2 / (1 + e^2x): absolute error of a few 2^-23, which the cap multiplies; large |x| saturate.
-__device__ __forceinline__ float tanh_abs(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(fminf(x * (2.0f * kLog2e), 64.0f))); }
-
 // Words (4 bytes) of one key row that a lane holds: K (a quarter of the row) and V (an eighth).
 template <int HD, bool Q8>
 struct Words {
@@ -159,16 +150,11 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
 #pragma unroll
             for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float m = fabsf(x[i][e]);
-                    if (m <= 3.402823466e38f) most = fmaxf(most, m);
-                }
+                for (int e = 0; e < 4; e++) most = fmaxf(most, finite_abs(x[i][e]));
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // the row's largest magnitude goes to [1, 2)
-        const int ex = most > 0.0f ? max(int(__float_as_uint(most) >> 23) - 127, -126) : 0;
-        const float up = __uint_as_float(uint32_t(min(127 - ex, 253)) << 23);
+        const float up = row_up(most);
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
@@ -528,6 +514,8 @@ cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st) {
+    const int64_t rows = int64_t(a.max_new) * (a.n_head / a.cache.n_kv);
+    if (rows > kPromptRows && a.cache.head_dim >= 64) return launch_paged_prompt(a, st);
     const bool q8 = a.cache.type == NEKO_T_E4M3;
     switch (a.cache.head_dim) {
         case 32: return q8 ? by_rows<32, true>(a, st) : by_rows<32, false>(a, st);

@@ -1,0 +1,722 @@
+// Attention of many query rows over a paged cache (neko_op_paged_attention): prompts and long continuations, on
+// tcgen05.
+//
+// The packed rows of a (sequence, KV head) are its new tokens times the G query heads that share the KV head. A CTA
+// takes two tiles of 128 rows (one when there are no more) and walks the keys in tiles of 128:
+//   S = Q K^T in TMEM, weights P back into TMEM over S (f16), O += P V in TMEM, all accumulation f32.
+// f32 queries are f16 hi + lo in shared memory (S = Qhi K^T + Qlo K^T) and their weights hi + lo in TMEM (P takes
+// exactly the 128 columns of its S); 16-bit queries are one exact f16 and their weights one f16. Rows are scaled by a
+// power of two into f16's range first. Roles:
+//  * warps 0..3 and 4..7: softmax of one row tile each, a thread per row, no shuffles. The reference maximum moves only
+//    when a score exceeds it by 2^8 (weights up to 2^8 are as exact as any in f16), so O is hardly ever rescaled, and
+//    the row's own thread does that; the tensor core works on the other row tile meanwhile.
+//  * warps 8..11: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
+//    serves K as a K-major and V as an MN-major operand: cp.async for f16 pages, registers and an exact conversion to
+//    f16 for 8-bit ones (fetched one tile ahead). Scales stay out of the operands: a block's key scale multiplies its
+//    scores and its value scale enters the weights' exponent (the sum takes it out again), 16 columns at a time.
+//  * warp 12, one lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
+// Masks only touch the key tiles that need them. Values that no row sees are zeroed by the loader; values that are not
+// finite in a tile that some row does not see whole are zeroed too and added by the threads of the rows that see them.
+// A cluster of CTAs splits the keys when there are few row tiles and joins over distributed shared memory in rank
+// order. Every wait is bounded and gives up once another role has failed.
+#include <cooperative_groups.h>
+
+#include "paged.cuh"
+#include "paged_math.cuh"
+#include "tc5_core.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace neko {
+
+namespace {
+
+constexpr int kRows = 128, kKeys = 128;  // of a tile
+constexpr int kThreads = 13 * 32;
+constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
+constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
+constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
+constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
+constexpr float kVNone = -126.0f;
+constexpr float kGone = -1.0f;
+
+struct PromptPlan {
+    int ranks;      // CTAs that share a (sequence, KV head, row tile pair): the cluster
+    int row_tiles;  // pairs of row tiles per (sequence, KV head)
+    int tiles_per;  // row tiles of a CTA: 1 or 2
+};
+
+template <int HD, bool Q8, bool HILO>
+struct PL {
+    static constexpr int kParts = HILO ? 2 : 1;
+    static constexpr int kHalf = kRows * 128;             // bytes of a 128-row, 64-wide f16 tile
+    static constexpr int kQTile = kHalf * (HD / 64);      // one part of one row tile
+    static constexpr int kStage = kHalf * (HD / 64);
+    static constexpr int kQBytes = 2 * kParts * kQTile;
+    static constexpr int kStages = HD == 64 ? 5 : HILO ? 3 : 5;
+    static constexpr int kStageOff = kQBytes;
+    static constexpr int kMiscOff = kStageOff + kStages * kStage;
+    static constexpr int kJoinPitch = HD + 4;             // floats of a row's state: values, maximum, sum
+    static constexpr int kSmem = kMiscOff + 1536 + 1024;  // + alignment
+    static_assert(2 * kRows * kJoinPitch * 4 <= kMiscOff, "the joined states take the operands' place");
+    static_assert(kStages <= 5, "the ring of scales");
+};
+
+// barriers and small arrays behind the operands
+struct Misc {
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain;
+    uint32_t tmem, fail;
+    float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
+    float vs[kRing][8];                // log2 of theirs of the values
+    uint32_t odd[5][4];                // per stage: keys with values that are not finite
+    float qdown[2 * kRows];            // scale / the row's power of two
+};
+static_assert(sizeof(Misc) <= 1536, "misc");
+
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
+    // MN-major, 128-byte swizzle: 64-value blocks 16 KB apart (LBO), groups of 8 keys 1024 bytes apart (SBO)
+    return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(16384 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc)
+        : "memory");
+}
+#define NEKO_R32(r)                                                                                                  \
+    "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),      \
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),       \
+        "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),      \
+        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+#define NEKO_REGS32                                                                                                  \
+    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"  \
+    "%29,%30,%31}"
+// 32 columns of this thread's TMEM lane; the values are there after ld_wait on the same registers.
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " NEKO_REGS32 ", [%32];" : NEKO_R32(r) : "r"(addr));
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : NEKO_R32(r)::"memory");
+}
+__device__ __forceinline__ void st32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " NEKO_REGS32 ";" : NEKO_R32(r) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Bounded wait that also ends once another role has failed; false: give up.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile uint32_t* fail) {
+    for (uint32_t i = 0; i < kMbarMaxTries; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 63 && *fail) return false;
+    }
+    *fail = 1;
+    set_device_error(kErrMbarTimeout);
+    return false;
+}
+// Whether the four 16-byte words hold f16 values that are not finite; those are zeroed.
+__device__ __forceinline__ bool drop_odd(uint4& x) {
+    bool odd = false;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if ((w[i] & 0x7c00u) == 0x7c00u) w[i] &= 0xffff0000u, odd = true;
+        if ((w[i] & 0x7c000000u) == 0x7c000000u) w[i] &= 0xffffu, odd = true;
+    }
+    return odd;
+}
+
+template <int HD, bool Q8, bool HILO>
+__global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_paged_attention_args a,
+                                                                  const PromptPlan plan) {
+    using L = PL<HD, Q8, HILO>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    Misc& ms = *reinterpret_cast<Misc*>(sm + L::kMiscOff);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const neko_paged_cache& c = a.cache;
+
+    // ---- the work of this CTA, the same for its whole cluster but for the rank
+    int b = blockIdx.x;
+    const int rank = b % plan.ranks;
+    b /= plan.ranks;
+    const int kvh = b % c.n_kv;
+    b /= c.n_kv;
+    const int s = b % c.n_seq;
+    const int tile = plan.row_tiles - 1 - b / c.n_seq;  // the longest rows first
+    const int G = a.n_head / c.n_kv;
+    const int row0 = a.q_start ? a.q_start[s] : s;
+    const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
+    const int held = max(a.kv_len[s], 0);
+    const int len = min(held, c.max_pages * c.page_size);
+    if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {
+        if (tid == 0) set_device_error(kErrBadIndex);
+        return;
+    }
+    const int r0 = tile * plan.tiles_per * kRows;
+    const int rows = min(n * G - r0, plan.tiles_per * kRows);
+    if (rows <= 0) return;
+    const int mt = rows > kRows ? 2 : 1;
+    const int pos_lo = held - n + r0 / G, pos_hi = held - n + (r0 + rows - 1) / G;
+    const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
+    const int hi = max(min(len, pos_hi + 1), 0);
+    const int lo = a.window ? min(max(pos_lo - a.window + 1, 0), hi) : 0;
+    const int t_lo = lo / kKeys, t_hi = (max(hi, prefix > lo ? prefix : 0) + kKeys - 1) / kKeys;
+    const int t_pre = min((prefix + kKeys - 1) / kKeys, t_lo);
+    const int nt_all = t_pre + max(t_hi - t_lo, 0);
+    const int i_begin = int(int64_t(nt_all) * rank / plan.ranks), i_end = int(int64_t(nt_all) * (rank + 1) / plan.ranks);
+    const int nt = i_end - i_begin;
+    auto key_of = [&](int i) { i += i_begin; return kKeys * (i < t_pre ? i : i - t_pre + t_lo); };
+    // every key of the tile is seen by every row between two positions
+    auto open = [&](int j0, int p_lo, int p_hi) {
+        return j0 + kKeys <= len && ((j0 + kKeys - 1 <= p_lo && (!a.window || p_hi - j0 < a.window)) || j0 + kKeys <= prefix);
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], 128), mbar_init(&ms.empty[i], 1);
+        for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 128), mbar_init(&ms.pv_done[h], 1);
+        mbar_init(&ms.drain, 1);
+        ms.fail = 0;
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // ---- queries: a warp per row, hd / 32 values a lane
+    if (warp < 8) {
+        constexpr int E = HD / 32;
+        for (int r = warp; r < mt * kRows; r += 8) {
+            const int pr = r0 + r;
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = 0.0f;
+            if (r < rows) {
+                const int64_t off = int64_t(row0 + pr / G) * a.q_token + int64_t(kvh * G + pr % G) * a.q_head + lane * E;
+                auto fetch = [&](auto* p) { load_row<E>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * E - 1)) == 0, x); };
+                if (a.type == kTF32) fetch(static_cast<const float*>(a.q) + off);
+                else if (a.type == kTF16) fetch(static_cast<const __half*>(a.q) + off);
+                else fetch(static_cast<const __nv_bfloat16*>(a.q) + off);
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) most = fmaxf(most, finite_abs(x[e]));
+            const float up = row_up(warp_max(most));
+            uint32_t h2[E / 2], l2[E / 2];
+#pragma unroll
+            for (int e = 0; e < E; e += 2) split_hilo(x[e] * up, x[e + 1] * up, h2[e / 2], l2[e / 2]);
+            const int d = lane * E, half = d / 64;
+            uint8_t* dst = sm + (r / kRows * L::kParts) * L::kQTile + half * L::kHalf + sw128_off(r % kRows, (d % 64) / 8) + (d % 8) * 2;
+            if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h2[0], h2[1]);
+            else *reinterpret_cast<uint32_t*>(dst) = h2[0];
+            if constexpr (HILO) {
+                dst += L::kQTile;
+                if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(l2[0], l2[1]);
+                else *reinterpret_cast<uint32_t*>(dst) = l2[0];
+            }
+            if (lane == 0) ms.qdown[r] = a.scale / up;
+        }
+        fence_proxy_async();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ms.tmem;
+    volatile uint32_t* fail = &ms.fail;
+
+    float row_max = -INFINITY, row_sum = 0.0f, vref = 0.0f;  // of a softmax thread's row; vref: log2 of O's unit
+    if (warp >= 8 && warp < 12) {
+        // ------------------------------------------------------------------ loader
+        const int lt = tid - 256;
+        const int32_t* table = c.table + int64_t(s) * c.table_stride;
+        const int ps_log = 31 - __clz(c.page_size);
+        const int64_t head_off = int64_t(kvh) * c.page_size * HD;
+        auto page_at = [&](int j) {  // page of the 16 keys from j, -1: none
+            const int slot = j >> ps_log;
+            const int p = j < len && slot < c.max_pages ? table[slot] : -1;
+            return p < c.num_pages ? p : -1;
+        };
+        constexpr int kB = Q8 ? 1 : 2;
+        constexpr int kRowChunks = HD * kB / 16;        // 16-byte pieces of a key row
+        constexpr int kPer = kKeys * kRowChunks / 128;  // pieces per thread
+        constexpr int kRowsAt = 128 / kRowChunks;       // key rows of one piece round (a multiple of the 16-key blocks or a part)
+        const int piece = lt % kRowChunks, row_in = lt / kRowChunks;
+        uint4 held_regs[Q8 ? kPer : 1];
+        int pages_k = -1, pages_next = -1;  // lane x < 8: page of block x of the tile
+        auto src = [&](bool v, int page, int j) {
+            const uint8_t* p = static_cast<const uint8_t*>(v ? c.v_pages : c.k_pages);
+            return p + (int64_t(page) * c.page_stride + head_off + int64_t(j & (c.page_size - 1)) * HD) * kB + piece * 16;
+        };
+        auto fetch8 = [&](bool v, int j0, int pages) {
+            if constexpr (Q8) {
+#pragma unroll
+                for (int x = 0; x < kPer; x++) {
+                    const int r = row_in + x * kRowsAt;
+                    const int page = __shfl_sync(0xffffffffu, pages, r >> 4);
+                    const bool ok = page >= 0 && j0 + r < len;
+                    held_regs[x] = ok ? ldg_stream(src(v, page, j0 + r)) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        const int total = 2 * nt;  // K0 V0 K1 V1 ..
+        if (nt > 0) {
+            pages_k = lane < 8 ? page_at(key_of(0) + 16 * lane) : -1;
+            fetch8(false, key_of(0), pages_k);
+        }
+        auto publish = [&](int x) {  // stage of item x is complete for this thread: odd values, then the barrier
+            const int st = x % L::kStages, i = x >> 1;
+            uint8_t* base = sm + L::kStageOff + st * L::kStage;
+            const int j0 = key_of(i);
+            if ((x & 1) && !open(j0, pos_lo, pos_hi)) {
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                // each thread looks through one key row
+                bool odd = false;
+                for (int h = 0; h < HD / 64; h++)
+                    for (int ch = 0; ch < 8; ch++) {
+                        uint4* p = reinterpret_cast<uint4*>(base + h * L::kHalf + sw128_off(lt, ch));
+                        uint4 v = *p;
+                        if (drop_odd(v)) *p = v, odd = true;
+                    }
+                const uint32_t m = __ballot_sync(0xffffffffu, odd);
+                if (lane == 0) ms.odd[st][warp - 8] = m;
+            }
+            fence_proxy_async();
+            mbar_arrive(&ms.full[st]);
+        };
+        bool ok = true;
+        for (int x = 0; x < total && ok; x++) {
+            const int st = x % L::kStages, i = x >> 1;
+            const bool v = x & 1;
+            const int j0 = key_of(i);
+            if (x >= L::kStages) ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
+            if (!ok) break;
+            uint8_t* base = sm + L::kStageOff + st * L::kStage;
+            if (!v && lt < 8) {  // the tile's scales (lanes 0..7 of the first loader warp hold its pages)
+                float ks = pages_k >= 0 ? 1.0f : kGone, vs = kVNone;
+                if (Q8 && pages_k >= 0) {
+                    ks = c.k_scale[int64_t(pages_k) * c.scale_stride + kvh];
+                    ks = fabsf(ks);  // scales are not negative: kGone stays apart
+                    vs = fmaxf(log2f(c.v_scale[int64_t(pages_k) * c.scale_stride + kvh]), kVNone);
+                }
+                ms.ks[i % kRing][lt] = ks;
+                ms.vs[i % kRing][lt] = vs;
+            }
+            if (!v && i + 1 < nt) pages_next = lane < 8 ? page_at(key_of(i + 1) + 16 * lane) : -1;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int y = 0; y < kPer; y++) {
+                    const int r = row_in + y * kRowsAt;
+                    const uint4 w = held_regs[y];
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                    uint32_t f[8];
+#pragma unroll
+                    for (int z = 0; z < 4; z++) f[2 * z] = e4m3x2_to_f16x2(uint16_t(ws[z])), f[2 * z + 1] = e4m3x2_to_f16x2(uint16_t(ws[z] >> 16));
+                    uint8_t* p = base + (piece * 16 / 64) * L::kHalf;
+                    const int ch = (piece * 2) % 8;
+                    uint4* p0 = reinterpret_cast<uint4*>(p + sw128_off(r, ch));
+                    uint4* p1 = reinterpret_cast<uint4*>(p + sw128_off(r, ch + 1));
+                    const uint4 v0 = make_uint4(f[0], f[1], f[2], f[3]), v1 = make_uint4(f[4], f[5], f[6], f[7]);
+                    // the two 64-wide halves take opposite pieces first: eight lanes, eight bank groups
+                    if (piece * 16 / 64) *p1 = v1, *p0 = v0;
+                    else *p0 = v0, *p1 = v1;
+                }
+                // the next item's pieces, while this one is used
+                if (x + 1 < total) {
+                    if (v) pages_k = pages_next;
+                    fetch8(!v, v ? key_of(i + 1) : j0, pages_k);
+                }
+                publish(x);
+            } else {
+#pragma unroll
+                for (int y = 0; y < kPer; y++) {
+                    const int r = row_in + y * kRowsAt;
+                    const int page = __shfl_sync(0xffffffffu, pages_k, r >> 4);
+                    const bool in = page >= 0 && j0 + r < len;
+                    cp16(base + (piece / 8) * L::kHalf + sw128_off(r, piece % 8),
+                         in ? src(v, page, j0 + r) : static_cast<const uint8_t*>(c.k_pages), in ? 16 : 0);
+                }
+                cp_commit();
+                if (v) pages_k = pages_next;
+                if (x > 0) {
+                    cp_wait<1>();
+                    publish(x - 1);
+                }
+            }
+        }
+        if constexpr (!Q8) {
+            cp_wait<0>();
+            if (ok && total > 0) publish(total - 1);
+        }
+    } else if (warp == 12) {
+        // ------------------------------------------------------------------ UMMA issue
+        if (lane == 0 && nt > 0) {
+            constexpr uint32_t idesc_s = f16_idesc(kRows, kKeys), idesc_o = f16_idesc(kRows, HD) | (1u << 16);
+            const uint32_t q_base = smem_u32(sm), st_base = smem_u32(sm + L::kStageOff);
+            auto issue_s = [&](int h, int st) {
+                const uint32_t kb = st_base + st * L::kStage;
+#pragma unroll
+                for (int part = 0; part < L::kParts; part++)
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint32_t off = (k / 4) * L::kHalf + (k % 4) * 32;
+                        umma_f16(tmem + h * 128, sw128_desc(q_base + (h * L::kParts + part) * L::kQTile + off), sw128_desc(kb + off),
+                                 idesc_s, part + k > 0 ? 1u : 0u);
+                    }
+            };
+            auto issue_pv = [&](int h, int st) {
+                const uint32_t vb = st_base + st * L::kStage;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; k++) {
+                    // weights of keys 16 k ..: f16 columns 8 k; hi + lo: 32-column groups of hi, lo (16 each)
+                    const uint32_t col = HILO ? uint32_t(32 * (k / 2) + 8 * (k % 2)) : uint32_t(8 * k);
+                    umma_ts(tmem + 256 + h * 128, tmem + h * 128 + col, v_desc(vb + k * 2048), idesc_o);
+                    if constexpr (HILO) umma_ts(tmem + 256 + h * 128, tmem + h * 128 + col + 16, v_desc(vb + k * 2048), idesc_o);
+                }
+            };
+            bool ok = wait_on(&ms.full[0], 0, fail);
+            if (ok) {
+                for (int h = 0; h < mt; h++) {
+                    issue_s(h, 0);
+                    umma_commit(&ms.s_full[h]);
+                }
+                umma_commit(&ms.empty[0]);
+            }
+            for (int i = 0; i < nt && ok; i++) {
+                const int xv = 2 * i + 1, xk = 2 * i + 2;
+                ok = wait_on(&ms.full[xv % L::kStages], (xv / L::kStages) & 1, fail);
+                for (int h = 0; h < mt && ok; h++) {
+                    ok = wait_on(&ms.p_full[h], i & 1, fail);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(h, xv % L::kStages);
+                    umma_commit(&ms.pv_done[h]);
+                    if (h == mt - 1) umma_commit(&ms.empty[xv % L::kStages]);
+                    if (i + 1 < nt) {
+                        if (h == 0) ok = wait_on(&ms.full[xk % L::kStages], (xk / L::kStages) & 1, fail);
+                        if (!ok) break;
+                        issue_s(h, xk % L::kStages);
+                        umma_commit(&ms.s_full[h]);
+                        if (h == mt - 1) umma_commit(&ms.empty[xk % L::kStages]);
+                    }
+                }
+            }
+            umma_commit(&ms.drain);  // nothing is in flight when the TMEM is freed, whatever happened
+            mbar_wait(&ms.drain, 0);
+        }
+        __syncwarp();
+    } else if (warp / 4 < mt) {
+        // ------------------------------------------------------------------ softmax, a thread per row
+        const int h = warp / 4;
+        const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + lanes + h * 128, to = tmem + lanes + 256 + h * 128;
+        const int r = h * kRows + (warp & 3) * 32 + lane, pr = r0 + r;
+        const bool real = r < rows;
+        const int qpos = real ? held - n + pr / G : kNoRow;
+        const float down = ms.qdown[r];
+        const float slope = a.slopes && real ? a.slopes[kvh * G + pr % G] * kLog2e : 0.0f;
+        const int h_lo = held - n + (r0 + h * kRows) / G, h_hi = held - n + (r0 + min(rows, (h + 1) * kRows) - 1) / G;
+        const bool shaped = a.softcap > 0.0f || a.slopes;
+        {
+            uint32_t z[32];
+#pragma unroll
+            for (int x = 0; x < 32; x++) z[x] = 0;
+#pragma unroll
+            for (int x = 0; x < HD; x += 32) st32(to + x, z);
+            st_wait();
+        }
+        bool ok = true;
+        for (int i = 0; i < nt && ok; i++) {
+            const int j0 = key_of(i);
+            ok = wait_on(&ms.s_full[h], i & 1, fail);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const float* ksp = ms.ks[i % kRing];
+            const float* vsp = ms.vs[i % kRing];
+            bool resident = true;
+            float vnow = kVNone;
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                resident &= ksp[x] != kGone;
+                if constexpr (Q8) vnow = fmaxf(vnow, vsp[x]);
+            }
+            const bool plain_mask = open(j0, h_lo, h_hi) && resident;
+            const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
+            // ---- the row's largest score (log2 units)
+            float top = -INFINITY;
+            {
+                uint32_t w[2][32];
+                ld32(ts, w[0]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    ld_wait(w[q & 1]);
+                    if (q < 3) ld32(ts + 32 * (q + 1), w[(q + 1) & 1]);
+                    uint32_t(&u)[32] = w[q & 1];
+                    if (!cooked) {
+#pragma unroll
+                        for (int g = 0; g < 2; g++) {
+                            float m0 = __uint_as_float(u[16 * g]), m1 = __uint_as_float(u[16 * g + 1]);
+#pragma unroll
+                            for (int x = 2; x < 16; x += 2) {
+                                m0 = fmaxf(m0, __uint_as_float(u[16 * g + x]));
+                                m1 = fmaxf(m1, __uint_as_float(u[16 * g + x + 1]));
+                            }
+                            const float f = Q8 ? down * ksp[2 * q + g] * kLog2e : down * kLog2e;
+                            top = fmaxf(top, fmaxf(m0, m1) * f);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            const int j = j0 + 32 * q + x;
+                            const float ks = ksp[2 * q + x / 16];
+                            float v = __uint_as_float(u[x]) * (down * ks);
+                            if (a.softcap > 0.0f) v = a.softcap * tanh_abs(__fdividef(v, a.softcap));
+                            v *= kLog2e;
+                            if (a.slopes) v += slope * float(j - qpos);
+                            const bool see = plain_mask ||
+                                             (ks != kGone && j < len && ((j <= qpos && (!a.window || qpos - j < a.window)) ||
+                                                                        (j < prefix && qpos != kNoRow)));
+                            v = see ? v : -INFINITY;
+                            top = fmaxf(top, v);
+                            u[x] = __float_as_uint(v);
+                        }
+                        st32(ts + 32 * q, u);
+                    }
+                }
+                if (cooked) st_wait();
+            }
+            // ---- the reference maximum and value scale
+            const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
+            const bool up = top > row_max + kLazy;  // also from -inf
+            bool odd_tile = false;
+            const int xv = 2 * i + 1, stv = xv % L::kStages;
+            if (!open(j0, pos_lo, pos_hi)) {
+                ok = wait_on(&ms.full[stv], (xv / L::kStages) & 1, fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                odd_tile = (ms.odd[stv][0] | ms.odd[stv][1] | ms.odd[stv][2] | ms.odd[stv][3]) != 0;
+            }
+            if (__any_sync(0xffffffffu, up || v_up || odd_tile)) {
+                float f = 1.0f;
+                if (up) {
+                    f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
+                    row_sum *= f;
+                    row_max = top;
+                }
+                if (v_up) {
+                    if (i > 0) f *= ex2(vref - vnow);
+                    vref = vnow;
+                }
+                if (i > 0) {
+                    ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                if (i > 0 || odd_tile) {
+#pragma unroll 1
+                    for (int x = 0; x < HD; x += 32) {
+                        uint32_t w[32];
+                        ld32(to + x, w);
+                        ld_wait(w);
+#pragma unroll
+                        for (int y = 0; y < 32; y++) w[y] = __float_as_uint(__uint_as_float(w[y]) * f);
+                        if (odd_tile) {
+#pragma unroll 1
+                            for (int key = 0; key < kKeys; key++) {
+                                if (!(ms.odd[stv][key >> 5] >> (key & 31) & 1)) continue;
+                                const int j = j0 + key, slot = j / c.page_size;
+                                if (j >= len || ksp[key >> 4] == kGone) continue;
+                                const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
+                                const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
+                                                   (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
+#pragma unroll
+                                for (int y = 0; y < 32; y++) {
+                                    float v;
+                                    if constexpr (Q8) {
+                                        v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
+                                    } else {
+                                        v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
+                                        if (fabsf(v) <= 65504.0f) v = 0.0f;
+                                    }
+                                    if (see) w[y] = __float_as_uint(__uint_as_float(w[y]) + v);
+                                }
+                            }
+                        }
+                        st32(to + x, w);
+                    }
+                    st_wait();
+                }
+            }
+            // ---- weights, their sum; P over S
+            const float ref = row_max == -INFINITY ? 0.0f : row_max;
+            {
+                uint32_t w[2][32];
+                ld32(ts, w[0]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    ld_wait(w[q & 1]);
+                    if (q < 3) ld32(ts + 32 * (q + 1), w[(q + 1) & 1]);
+                    uint32_t(&u)[32] = w[q & 1];
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const int blk = 2 * q + g;
+                        const float f = cooked ? 1.0f : Q8 ? down * ksp[blk] * kLog2e : down * kLog2e;
+                        float vr = 0.0f;
+                        if constexpr (Q8) vr = fmaxf(vsp[blk] - vref, kVMin);
+                        const float off = vr - ref;
+                        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 16; x += 2) {
+                            const float p0 = ex2(fmaf(__uint_as_float(u[16 * g + x]), f, off));
+                            const float p1 = ex2(fmaf(__uint_as_float(u[16 * g + x + 1]), f, off));
+                            sum0 += p0;
+                            sum1 += p1;
+                            u[16 * g + x] = __float_as_uint(p0);
+                            u[16 * g + x + 1] = __float_as_uint(p1);
+                        }
+                        row_sum += Q8 ? (sum0 + sum1) * ex2(-vr) : sum0 + sum1;
+                    }
+                    if constexpr (HILO) {
+                        uint32_t hl[32];
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
+                        st32(ts + 32 * q, hl);
+                    } else {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
+                        st16(ts + 16 * q, p);
+                    }
+                }
+                st_wait();
+            }
+            tc_fence_before();
+            mbar_arrive(&ms.p_full[h]);
+        }
+        if (ok && nt > 0) {
+            ok = wait_on(&ms.pv_done[h], (nt - 1) & 1, fail);
+            tc_fence_after();
+        }
+    }
+    // ---- the outputs: everything is read out of TMEM before the operands' memory is used again
+    __syncwarp();
+    __syncthreads();
+    const bool alone = plan.ranks == 1;
+    float* state = reinterpret_cast<float*>(sm);  // [row][values, maximum, sum]
+    if (warp < 8 && warp / 4 < mt) {
+        const int h = warp / 4, r = h * kRows + (warp & 3) * 32 + lane;
+        const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + h * 128;
+        float f = Q8 ? exp2f(vref) : 1.0f;
+        if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
+        float* mine = state + r * L::kJoinPitch;
+#pragma unroll
+        for (int x = 0; x < HD; x += 32) {
+            uint32_t w[32];
+            ld32(to + x, w);
+            ld_wait(w);
+#pragma unroll
+            for (int y = 0; y < 32; y += 4) {
+                float4 v = make_float4(__uint_as_float(w[y]) * f, __uint_as_float(w[y + 1]) * f, __uint_as_float(w[y + 2]) * f,
+                                       __uint_as_float(w[y + 3]) * f);
+                if (alone && row_sum == 0.0f) v = make_float4(0, 0, 0, 0);
+                *reinterpret_cast<float4*>(mine + x + y) = v;
+            }
+        }
+        mine[HD] = row_max;
+        mine[HD + 1] = row_sum;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    auto put = [&](int r, int d, float4 v) {
+        const int pr = r0 + r;
+        const int64_t off = int64_t(row0 + pr / G) * a.o_token + int64_t(kvh * G + pr % G) * a.o_head + d;
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        auto store = [&](auto* p) { store_row<4>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0, x); };
+        if (a.type == kTF32) store(static_cast<float*>(a.out) + off);
+        else if (a.type == kTF16) store(static_cast<__half*>(a.out) + off);
+        else store(static_cast<__nv_bfloat16*>(a.out) + off);
+    };
+    if (alone) {
+        for (int x = tid; x < rows * (HD / 4); x += kThreads) {
+            const int r = x / (HD / 4), d = x % (HD / 4) * 4;
+            put(r, d, *reinterpret_cast<const float4*>(state + r * L::kJoinPitch + d));
+        }
+        return;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int share = (rows * (HD / 4) + plan.ranks - 1) / plan.ranks;
+    for (int x = rank * share + tid; x < min(rows * (HD / 4), (rank + 1) * share); x += kThreads) {
+        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < plan.ranks; w++) top = fmaxf(top, cluster.map_shared_rank(state, w)[r * L::kJoinPitch + HD]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 v = make_float4(0, 0, 0, 0);
+        for (int w = 0; w < plan.ranks; w++) {
+            const float* st = cluster.map_shared_rank(state, w) + r * L::kJoinPitch;
+            const float f = ex2(st[HD] - ref);
+            const float4 o = *reinterpret_cast<const float4*>(st + d);
+            sum += f * st[HD + 1];
+            v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
+        }
+        const float f = 1.0f / sum;
+        put(r, d, sum == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    }
+    cluster.sync();  // no CTA leaves while another reads its state
+}
+
+template <int HD, bool Q8, bool HILO>
+cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
+    using L = PL<HD, Q8, HILO>;
+    const neko_paged_cache& c = a.cache;
+    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
+    PromptPlan p;
+    // two row tiles per CTA unless that leaves SMs without work
+    const int64_t tiles = (rows + kRows - 1) / kRows, heads = int64_t(c.n_seq) * c.n_kv;
+    p.tiles_per = tiles > 1 && heads * ((tiles + 1) / 2) * 2 > num_sms() ? 2 : 1;
+    p.row_tiles = int((tiles + p.tiles_per - 1) / p.tiles_per);
+    const int64_t items = heads * p.row_tiles, key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
+    p.ranks = 1;
+    while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
+    if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    auto* fn = paged_prompt_kernel<HD, Q8, HILO>;
+    if (cudaError_t e = ensure_dyn_smem(fn, L::kSmem); e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(items * p.ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = L::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(p.ranks);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.ranks > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, a, p);
+}
+
+template <int HD>
+cudaError_t by_type(const neko_paged_attention_args& a, cudaStream_t st) {
+    const bool q8 = a.cache.type == NEKO_T_E4M3, f32 = a.type == NEKO_T_F32;
+    if (q8) return f32 ? go<HD, true, true>(a, st) : go<HD, true, false>(a, st);
+    return f32 ? go<HD, false, true>(a, st) : go<HD, false, false>(a, st);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st) {
+    return a.cache.head_dim == 64 ? by_type<64>(a, st) : by_type<128>(a, st);
+}
+
+}  // namespace neko

@@ -14,6 +14,9 @@ constexpr int kScaleMinExp = -100;  // scale of a block of zeros: 2^-100
 
 cudaError_t launch_paged_append(const neko_paged_append_args& a, cudaStream_t st);
 cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st);
+// The tcgen05 kernel for more than kPromptRows packed rows (new tokens x query heads per KV head), head dim 64 or 128.
+cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st);
+constexpr int kPromptRows = 16;
 
 // Two e4m3 codes as exact f16 (0x7F / 0xFF: NaN).
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {

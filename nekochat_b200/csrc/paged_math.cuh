@@ -1,0 +1,29 @@
+// Arithmetic that the paged attention kernels share (k_paged_attn.cu, k_paged_prompt.cu).
+#pragma once
+#include "neko_common.cuh"
+
+namespace neko {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNoRow = -(1 << 30);  // the position of a place without a row: it sees nothing
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// tanh(x) = 1 - 2 / (1 + e^2x): absolute error of a few 2^-23, which the cap multiplies; large |x| saturate.
+__device__ __forceinline__ float tanh_abs(float x) {
+    return 1.0f - __fdividef(2.0f, 1.0f + ex2(fminf(x * (2.0f * kLog2e), 64.0f)));
+}
+__device__ __forceinline__ float finite_abs(float x) {
+    const float m = fabsf(x);
+    return m <= 3.402823466e38f ? m : 0.0f;
+}
+// The power of two that brings a row's largest magnitude to [1, 2).
+__device__ __forceinline__ float row_up(float most) {
+    const int ex = most > 0.0f ? max(int(__float_as_uint(most) >> 23) - 127, -126) : 0;
+    return __uint_as_float(uint32_t(min(127 - ex, 253)) << 23);
+}
+
+}  // namespace neko

@@ -408,3 +408,56 @@ def test_results_repeat(torch):
     table = torch.from_numpy(cache.table).cuda()
     outs = [ops.paged_attention(q, cache.k, cache.v, table, n, k_scale=cache.ks, v_scale=cache.vs) for _ in range(3)]
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd,heads,n_kv,ps", [(128, 16, 8, 16), (64, 12, 12, 64), (128, 8, 1, 128), (64, 6, 2, 32)])
+def test_prompts(torch, hd, heads, n_kv, ps, e4m3, dtype):
+    """Row tiles of 128 packed rows and their ragged ends, key tiles of 128 and theirs, earlier turns."""
+    rng = np.random.default_rng(hd + heads + ps + 3 * e4m3)
+    new = [130, 1, 64, 257, 0]
+    lens = [130, 77, 300, 400, 30]
+    cache = Cache(torch, rng, lens, n_kv, ps, hd, e4m3)
+    cache.fill(rng, lens)
+    attend(torch, cache, lens, new, heads, dtype, 52)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("opts", [dict(softcap=30.0), dict(window=1), dict(window=100),
+                                  dict(window=140, softcap=50.0, alibi=True), dict(alibi=True), dict(pre=True),
+                                  dict(pre=True, window=18), dict(scale=0.5), dict(scale=-0.1), dict(strided=True),
+                                  dict(gone=True), dict(odd=True), dict(odd=True, window=30)])
+def test_prompt_masks_and_biases(torch, opts, e4m3, dtype):
+    """Masks on whole tiles and inside them, pages that are not resident, NaN that only some rows see."""
+    opts = dict(opts)
+    rng = np.random.default_rng(len(opts) + e4m3)
+    new, lens = [200, 40, 150], [330, 600, 150]
+    if opts.pop("pre", False):
+        opts["prefix"] = [290, 40, 150]
+    cache = Cache(torch, rng, lens, 2, 16, 128, e4m3)
+    cache.fill(rng, lens)
+    if opts.pop("gone", False):
+        cache.table[0, 2:5] = -1
+        cache.table[0, 8:16] = 1 << 20
+        cache.table[2, :] = -1
+    if opts.pop("odd", False):
+        nan = 0x7F if e4m3 else float("nan")
+        for s, j in ((0, 250), (0, 140), (1, 570), (2, 0)):
+            cache.v[int(cache.table[s, j // 16]), s % 2, j % 16, 3:70] = nan
+        cache.k[int(cache.table[2, 6]), 1, 7, 5] = nan
+    attend(torch, cache, lens, new, 4, dtype, 53, **opts)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_prompt_of_blocks_of_very_different_scales(torch, dtype):
+    rng = np.random.default_rng(54)
+    lens = [500, 260]
+    cache = Cache(torch, rng, lens, 2, 16, 128, True)
+    cache.fill(rng, lens, exps=1)
+    cache.vs.copy_(torch.from_numpy((2.0 ** rng.integers(-8, 5, tuple(cache.vs.shape))).astype(np.float32)).cuda())
+    attend(torch, cache, lens, [60, 200], 4, dtype, 55)
+    cache.vs.copy_(torch.from_numpy(rng.uniform(0.01, 0.3, tuple(cache.vs.shape)).astype(np.float32)).cuda())
+    cache.ks.copy_(torch.from_numpy((rng.integers(0, 5, tuple(cache.ks.shape)) * 0.03).astype(np.float32)).cuda())
+    attend(torch, cache, lens, [60, 200], 4, dtype, 55)

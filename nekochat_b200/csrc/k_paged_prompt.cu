@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kRows = 128, kKeys = 128;  // of a tile
 constexpr int kThreads = 13 * 32;
+constexpr int kQBatch = 8;      // a multiple of it is 128: batches stay in one row tile
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
 constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
@@ -110,6 +111,23 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
         : "memory");
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
 // Bounded wait that also ends once another role has failed; false: give up.
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile uint32_t* fail) {
     for (uint32_t i = 0; i < kMbarMaxTries; i++) {
@@ -190,39 +208,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // ---- queries: a warp per row, hd / 32 values a lane
-    if (warp < 8) {
+    // ---- queries: a warp per row, hd / 32 values a lane, the loads of kQBatch rows in flight together
+    if (warp < 12) {
         constexpr int E = HD / 32;
-        for (int r = warp; r < mt * kRows; r += 8) {
-            const int pr = r0 + r;
-            float x[E];
+        const auto load_q = [&](auto* q) {
+#pragma unroll 1
+            for (int rb = warp * kQBatch; rb < mt * kRows; rb += 12 * kQBatch) {
+                float x[kQBatch][E];
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = 0.0f;
-            if (r < rows) {
-                const int64_t off = int64_t(row0 + pr / G) * a.q_token + int64_t(kvh * G + pr % G) * a.q_head + lane * E;
-                auto fetch = [&](auto* p) { load_row<E>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * E - 1)) == 0, x); };
-                if (a.type == kTF32) fetch(static_cast<const float*>(a.q) + off);
-                else if (a.type == kTF16) fetch(static_cast<const __half*>(a.q) + off);
-                else fetch(static_cast<const __nv_bfloat16*>(a.q) + off);
+                for (int y = 0; y < kQBatch; y++) {
+                    const int pr = r0 + rb + y;
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[y][e] = 0.0f;
+                    if (rb + y < rows) {
+                        const auto* p = q + int64_t(row0 + pr / G) * a.q_token + int64_t(kvh * G + pr % G) * a.q_head + lane * E;
+                        load_row<E>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * E - 1)) == 0, x[y]);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < kQBatch; y++) {
+                    const int r = rb + y;
+                    float most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; e++) most = fmaxf(most, finite_abs(x[y][e]));
+                    const float up = row_up(warp_max(most));
+                    uint32_t h2[E / 2], l2[E / 2];
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) split_hilo(x[y][e] * up, x[y][e + 1] * up, h2[e / 2], l2[e / 2]);
+                    const int d = lane * E, half = d / 64;
+                    uint8_t* dst = sm + (r / kRows * L::kParts) * L::kQTile + half * L::kHalf + sw128_off(r % kRows, (d % 64) / 8) + (d % 8) * 2;
+                    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h2[0], h2[1]);
+                    else *reinterpret_cast<uint32_t*>(dst) = h2[0];
+                    if constexpr (HILO) {
+                        dst += L::kQTile;
+                        if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(l2[0], l2[1]);
+                        else *reinterpret_cast<uint32_t*>(dst) = l2[0];
+                    }
+                    if (lane == 0) ms.qdown[r] = a.scale / up;
+                }
             }
-            float most = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; e++) most = fmaxf(most, finite_abs(x[e]));
-            const float up = row_up(warp_max(most));
-            uint32_t h2[E / 2], l2[E / 2];
-#pragma unroll
-            for (int e = 0; e < E; e += 2) split_hilo(x[e] * up, x[e + 1] * up, h2[e / 2], l2[e / 2]);
-            const int d = lane * E, half = d / 64;
-            uint8_t* dst = sm + (r / kRows * L::kParts) * L::kQTile + half * L::kHalf + sw128_off(r % kRows, (d % 64) / 8) + (d % 8) * 2;
-            if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h2[0], h2[1]);
-            else *reinterpret_cast<uint32_t*>(dst) = h2[0];
-            if constexpr (HILO) {
-                dst += L::kQTile;
-                if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(l2[0], l2[1]);
-                else *reinterpret_cast<uint32_t*>(dst) = l2[0];
-            }
-            if (lane == 0) ms.qdown[r] = a.scale / up;
-        }
+        };
+        if constexpr (HILO) load_q(static_cast<const float*>(a.q));
+        else if (a.type == kTF16) load_q(static_cast<const __half*>(a.q));
+        else load_q(static_cast<const __nv_bfloat16*>(a.q));
         fence_proxy_async();
     }
     tc_fence_before();
@@ -334,13 +362,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 publish(x);
             } else {
+                constexpr int kIn = 16 / kRowsAt;  // pieces of a thread per block of 16 keys
+#pragma unroll 2
+                for (int blk = 0; blk < 8; blk++) {
+                    const int page = __shfl_sync(0xffffffffu, pages_k, blk);
+                    const int r = 16 * blk + row_in;
+                    const uint8_t* p = page >= 0 ? src(v, page, j0 + r) : static_cast<const uint8_t*>(c.k_pages);
+                    uint8_t* dst = base + (piece / 8) * L::kHalf + sw128_off(r, piece % 8);
 #pragma unroll
-                for (int y = 0; y < kPer; y++) {
-                    const int r = row_in + y * kRowsAt;
-                    const int page = __shfl_sync(0xffffffffu, pages_k, r >> 4);
-                    const bool in = page >= 0 && j0 + r < len;
-                    cp16(base + (piece / 8) * L::kHalf + sw128_off(r, piece % 8),
-                         in ? src(v, page, j0 + r) : static_cast<const uint8_t*>(c.k_pages), in ? 16 : 0);
+                    for (int y = 0; y < kIn; y++) {
+                        const bool in = page >= 0 && j0 + r + y * kRowsAt < len;
+                        // rows kRowsAt (a multiple of 8) further on: the same place in the swizzle's pattern
+                        cp16(dst + y * kRowsAt * 128, in ? p + y * kRowsAt * HD * kB : p, in ? 16 : 0);
+                    }
                 }
                 cp_commit();
                 if (v) pages_k = pages_next;
@@ -423,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         const float slope = a.slopes && real ? a.slopes[kvh * G + pr % G] * kLog2e : 0.0f;
         const int h_lo = held - n + (r0 + h * kRows) / G, h_hi = held - n + (r0 + min(rows, (h + 1) * kRows) - 1) / G;
         const bool shaped = a.softcap > 0.0f || a.slopes;
+        const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
         {
             uint32_t z[32];
 #pragma unroll
@@ -449,48 +484,67 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             }
             const bool plain_mask = open(j0, h_lo, h_hi) && resident;
             const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
-            // ---- the row's largest score (log2 units)
+            // ---- the row's largest score (log2 units); loops are kept rolled: straight code of a few KB per pass was
+            // bound by instruction fetch
             float top = -INFINITY;
-            {
+            if (!cooked) {
                 uint32_t w[2][32];
                 ld32(ts, w[0]);
+#pragma unroll 1
+                for (int q = 0; q < 4; q += 2) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    ld_wait(w[q & 1]);
-                    if (q < 3) ld32(ts + 32 * (q + 1), w[(q + 1) & 1]);
-                    uint32_t(&u)[32] = w[q & 1];
-                    if (!cooked) {
+                    for (int y = 0; y < 2; y++) {
+                        ld_wait(w[y]);
+                        if (y == 0 || q == 0) ld32(ts + 32 * (q + y + 1), w[y ^ 1]);
 #pragma unroll
                         for (int g = 0; g < 2; g++) {
-                            float m0 = __uint_as_float(u[16 * g]), m1 = __uint_as_float(u[16 * g + 1]);
+                            float m0 = __uint_as_float(w[y][16 * g]), m1 = __uint_as_float(w[y][16 * g + 1]);
 #pragma unroll
                             for (int x = 2; x < 16; x += 2) {
-                                m0 = fmaxf(m0, __uint_as_float(u[16 * g + x]));
-                                m1 = fmaxf(m1, __uint_as_float(u[16 * g + x + 1]));
+                                m0 = fmaxf(m0, __uint_as_float(w[y][16 * g + x]));
+                                m1 = fmaxf(m1, __uint_as_float(w[y][16 * g + x + 1]));
                             }
-                            const float f = Q8 ? down * ksp[2 * q + g] * kLog2e : down * kLog2e;
-                            top = fmaxf(top, fmaxf(m0, m1) * f);
+                            m0 = fmaxf(m0, m1);
+                            top = fmaxf(top, Q8 ? m0 * ksp[2 * (q + y) + g] : m0);
                         }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 32; x++) {
-                            const int j = j0 + 32 * q + x;
-                            const float ks = ksp[2 * q + x / 16];
-                            float v = __uint_as_float(u[x]) * (down * ks);
-                            if (a.softcap > 0.0f) v = a.softcap * tanh_abs(__fdividef(v, a.softcap));
-                            v *= kLog2e;
-                            if (a.slopes) v += slope * float(j - qpos);
-                            const bool see = plain_mask ||
-                                             (ks != kGone && j < len && ((j <= qpos && (!a.window || qpos - j < a.window)) ||
-                                                                        (j < prefix && qpos != kNoRow)));
-                            v = see ? v : -INFINITY;
-                            top = fmaxf(top, v);
-                            u[x] = __float_as_uint(v);
-                        }
-                        st32(ts + 32 * q, u);
                     }
                 }
-                if (cooked) st_wait();
+                top *= down * kLog2e;
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < 4; q++) {
+                    uint32_t u[32];
+                    ld32(ts + 32 * q, u);
+                    ld_wait(u);
+                    const float ks0 = ksp[2 * q], ks1 = ksp[2 * q + 1];
+                    const int jq = j0 + 32 * q;
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        const float ks = x < 16 ? ks0 : ks1;
+                        float v = __uint_as_float(u[x]) * (down * ks);
+                        if (a.softcap > 0.0f) v = a.softcap * tanh_abs(v * inv_cap);
+                        u[x] = __float_as_uint(v * kLog2e);
+                    }
+                    if (a.slopes) {
+#pragma unroll
+                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x])));
+                    }
+                    if (!plain_mask) {
+                        // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
+                        const int see_hi = min(len, qpos + 1), see_lo = a.window ? qpos - a.window + 1 : 0;
+                        const int pre = real ? prefix : 0;
+#pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            const int j = jq + x;
+                            const bool see = ((j < see_hi && j >= see_lo) || j < pre) && (x < 16 ? ks0 : ks1) != kGone;
+                            if (!see) u[x] = __float_as_uint(-INFINITY);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(u[x]));
+                    st32(ts + 32 * q, u);
+                }
+                st_wait();
             }
             // ---- the reference maximum and value scale
             const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
@@ -558,45 +612,57 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             // ---- weights, their sum; P over S
             const float ref = row_max == -INFINITY ? 0.0f : row_max;
             {
+                const float f0 = cooked ? 1.0f : down * kLog2e;
+                uint64_t sums[2] = {0, 0};
                 uint32_t w[2][32];
                 ld32(ts, w[0]);
+#pragma unroll 1
+                for (int q = 0; q < 4; q += 2) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    ld_wait(w[q & 1]);
-                    if (q < 3) ld32(ts + 32 * (q + 1), w[(q + 1) & 1]);
-                    uint32_t(&u)[32] = w[q & 1];
+                    for (int y = 0; y < 2; y++) {
+                        ld_wait(w[y]);
+                        if (y == 0 || q == 0) ld32(ts + 32 * (q + y + 1), w[y ^ 1]);
+                        uint32_t(&u)[32] = w[y];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const int blk = 2 * q + g;
-                        const float f = cooked ? 1.0f : Q8 ? down * ksp[blk] * kLog2e : down * kLog2e;
-                        float vr = 0.0f;
-                        if constexpr (Q8) vr = fmaxf(vsp[blk] - vref, kVMin);
-                        const float off = vr - ref;
-                        float sum0 = 0.0f, sum1 = 0.0f;
+                        for (int g = 0; g < 2; g++) {
+                            const int blk = 2 * (q + y) + g;
+                            const float f = Q8 && !cooked ? f0 * ksp[blk] : f0;
+                            const float vr = Q8 ? fmaxf(vsp[blk] - vref, kVMin) : 0.0f;
+                            const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
+                            if (Q8) sums[0] = sums[1] = 0;
 #pragma unroll
-                        for (int x = 0; x < 16; x += 2) {
-                            const float p0 = ex2(fmaf(__uint_as_float(u[16 * g + x]), f, off));
-                            const float p1 = ex2(fmaf(__uint_as_float(u[16 * g + x + 1]), f, off));
-                            sum0 += p0;
-                            sum1 += p1;
-                            u[16 * g + x] = __float_as_uint(p0);
-                            u[16 * g + x + 1] = __float_as_uint(p1);
+                            for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                                float z0, z1;
+                                unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
+                                z0 = ex2(z0), z1 = ex2(z1);
+                                u[x] = __float_as_uint(z0), u[x + 1] = __float_as_uint(z1);
+                                sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
+                            }
+                            if (Q8) {  // the sum without the value scale
+                                float z0, z1;
+                                unpack2(add2(sums[0], sums[1]), z0, z1);
+                                row_sum = fmaf(z0 + z1, ex2(-vr), row_sum);
+                            }
                         }
-                        row_sum += Q8 ? (sum0 + sum1) * ex2(-vr) : sum0 + sum1;
-                    }
-                    if constexpr (HILO) {
-                        uint32_t hl[32];
+                        if constexpr (HILO) {
+                            uint32_t hl[32];
 #pragma unroll
-                        for (int x = 0; x < 16; x++)
-                            split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
-                        st32(ts + 32 * q, hl);
-                    } else {
-                        uint32_t p[16];
+                            for (int x = 0; x < 16; x++)
+                                split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
+                            st32(ts + 32 * (q + y), hl);
+                        } else {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int x = 0; x < 16; x++)
-                            p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
-                        st16(ts + 16 * q, p);
+                            for (int x = 0; x < 16; x++)
+                                p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
+                            st16(ts + 16 * (q + y), p);
+                        }
                     }
+                }
+                if (!Q8) {
+                    float z0, z1;
+                    unpack2(add2(sums[0], sums[1]), z0, z1);
+                    row_sum += z0 + z1;
                 }
                 st_wait();
             }

@@ -10,11 +10,11 @@
 //  * warps 0..3 and 4..7: softmax of one row tile each, a thread per row, no shuffles. The reference maximum moves only
 //    when a score exceeds it by 2^8 (weights up to 2^8 are as exact as any in f16), so O is hardly ever rescaled, and
 //    the row's own thread does that; the tensor core works on the other row tile meanwhile.
-//  * warps 8..11: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
+//  * warps 8..10: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
 //    serves K as a K-major and V as an MN-major operand: cp.async for f16 pages, registers and an exact conversion to
 //    f16 for 8-bit ones (fetched one tile ahead). Scales stay out of the operands: a block's key scale multiplies its
 //    scores and its value scale enters the weights' exponent (the sum takes it out again), 16 columns at a time.
-//  * warp 12, one lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
+//  * warp 11, one lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
 // Masks only touch the key tiles that need them. Values that no row sees are zeroed by the loader; values that are not
 // finite in a tile that some row does not see whole are zeroed too and added by the threads of the rows that see them.
 // A cluster of CTAs splits the keys when there are few row tiles and joins over distributed shared memory in rank
@@ -24,6 +24,7 @@
 #include "paged.cuh"
 #include "paged_math.cuh"
 #include "tc5_core.cuh"
+#include "tma_host.h"
 
 namespace cg = cooperative_groups;
 
@@ -32,9 +33,11 @@ namespace neko {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128;  // of a tile
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 12 * 32;  // 168 registers a thread: a row's 128 scores stay in them
+constexpr int kLoaders = 96;
 constexpr int kQBatch = 8;      // a multiple of it is 128: batches stay in one row tile
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
+constexpr int kOddRing = 8;     // and their keys with odd values
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
 constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
 constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
@@ -58,21 +61,21 @@ struct PL {
     static constexpr int kStageOff = kQBytes;
     static constexpr int kMiscOff = kStageOff + kStages * kStage;
     static constexpr int kJoinPitch = HD + 4;             // floats of a row's state: values, maximum, sum
-    static constexpr int kSmem = kMiscOff + 1536 + 1024;  // + alignment
+    static constexpr int kSmem = kMiscOff + 2048 + 1024;  // + alignment
     static_assert(2 * kRows * kJoinPitch * 4 <= kMiscOff, "the joined states take the operands' place");
     static_assert(kStages <= 5, "the ring of scales");
 };
 
 // barriers and small arrays behind the operands
 struct Misc {
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain;
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned;
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
-    uint32_t odd[5][4];                // per stage: keys with values that are not finite
+    uint32_t odd[kOddRing][4];         // of a key tile that needs masks: keys with values that are not finite
     float qdown[2 * kRows];            // scale / the row's power of two
 };
-static_assert(sizeof(Misc) <= 1536, "misc");
+static_assert(sizeof(Misc) <= 2048, "misc");
 
 __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
     // MN-major, 128-byte swizzle: 64-value blocks 16 KB apart (LBO), groups of 8 keys 1024 bytes apart (SBO)
@@ -150,9 +153,22 @@ __device__ __forceinline__ bool drop_odd(uint4& x) {
     return odd;
 }
 
+// The pools as [pages][kv heads * page][hd] f16, read in boxes of a page's tokens x 64 values (f16 pages only).
+struct PromptMaps {
+    CUtensorMap k, v;
+};
+__device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
 template <int HD, bool Q8, bool HILO>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_paged_attention_args a,
-                                                                  const PromptPlan plan) {
+                                                                  const PromptPlan plan,
+                                                                  const __grid_constant__ PromptMaps maps) {
     using L = PL<HD, Q8, HILO>;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -197,19 +213,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     };
 
     if (tid == 0) {
-        for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], 128), mbar_init(&ms.empty[i], 1);
+        for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], Q8 ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
         for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 128), mbar_init(&ms.pv_done[h], 1);
-        mbar_init(&ms.drain, 1);
+        mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders);
         ms.fail = 0;
+        for (int i = 0; i < 8; i++) ms.odd[i / 4][i % 4] = 0;  // tiles 0 and 1
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // ---- queries: a warp per row, hd / 32 values a lane, the loads of kQBatch rows in flight together
-    if (warp < 12) {
+    {
         constexpr int E = HD / 32;
         const auto load_q = [&](auto* q) {
 #pragma unroll 1
@@ -260,135 +277,176 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     volatile uint32_t* fail = &ms.fail;
 
     float row_max = -INFINITY, row_sum = 0.0f, vref = 0.0f;  // of a softmax thread's row; vref: log2 of O's unit
-    if (warp >= 8 && warp < 12) {
+    if (warp >= 8 && warp < 11) {
         // ------------------------------------------------------------------ loader
         const int lt = tid - 256;
         const int32_t* table = c.table + int64_t(s) * c.table_stride;
         const int ps_log = 31 - __clz(c.page_size);
-        const int64_t head_off = int64_t(kvh) * c.page_size * HD;
-        auto page_at = [&](int j) {  // page of the 16 keys from j, -1: none
-            const int slot = j >> ps_log;
-            const int p = j < len && slot < c.max_pages ? table[slot] : -1;
+        const int total = 2 * nt;  // items K0 V0 K1 V1 ..
+        // lane x < 8: page of the 16 keys from j0 + 16 x, -1: none
+        auto pages_of = [&](int j0) {
+            const int j = j0 + 16 * lane, slot = j >> ps_log;
+            const int p = lane < 8 && j < len && slot < c.max_pages ? table[slot] : -1;
             return p < c.num_pages ? p : -1;
         };
-        constexpr int kB = Q8 ? 1 : 2;
-        constexpr int kRowChunks = HD * kB / 16;        // 16-byte pieces of a key row
-        constexpr int kPer = kKeys * kRowChunks / 128;  // pieces per thread
-        constexpr int kRowsAt = 128 / kRowChunks;       // key rows of one piece round (a multiple of the 16-key blocks or a part)
-        const int piece = lt % kRowChunks, row_in = lt / kRowChunks;
-        uint4 held_regs[Q8 ? kPer : 1];
-        int pages_k = -1, pages_next = -1;  // lane x < 8: page of block x of the tile
-        auto src = [&](bool v, int page, int j) {
-            const uint8_t* p = static_cast<const uint8_t*>(v ? c.v_pages : c.k_pages);
-            return p + (int64_t(page) * c.page_stride + head_off + int64_t(j & (c.page_size - 1)) * HD) * kB + piece * 16;
-        };
-        auto fetch8 = [&](bool v, int j0, int pages) {
-            if constexpr (Q8) {
-#pragma unroll
-                for (int x = 0; x < kPer; x++) {
-                    const int r = row_in + x * kRowsAt;
-                    const int page = __shfl_sync(0xffffffffu, pages, r >> 4);
-                    const bool ok = page >= 0 && j0 + r < len;
-                    held_regs[x] = ok ? ldg_stream(src(v, page, j0 + r)) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        };
-        const int total = 2 * nt;  // K0 V0 K1 V1 ..
-        if (nt > 0) {
-            pages_k = lane < 8 ? page_at(key_of(0) + 16 * lane) : -1;
-            fetch8(false, key_of(0), pages_k);
-        }
-        auto publish = [&](int x) {  // stage of item x is complete for this thread: odd values, then the barrier
-            const int st = x % L::kStages, i = x >> 1;
-            uint8_t* base = sm + L::kStageOff + st * L::kStage;
-            const int j0 = key_of(i);
-            if ((x & 1) && !open(j0, pos_lo, pos_hi)) {
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                // each thread looks through one key row
-                bool odd = false;
-                for (int h = 0; h < HD / 64; h++)
-                    for (int ch = 0; ch < 8; ch++) {
-                        uint4* p = reinterpret_cast<uint4*>(base + h * L::kHalf + sw128_off(lt, ch));
-                        uint4 v = *p;
-                        if (drop_odd(v)) *p = v, odd = true;
-                    }
-                const uint32_t m = __ballot_sync(0xffffffffu, odd);
-                if (lane == 0) ms.odd[st][warp - 8] = m;
-            }
-            fence_proxy_async();
-            mbar_arrive(&ms.full[st]);
-        };
+        int pages = nt > 0 ? pages_of(key_of(0)) : -1, pages_next = -1;
         bool ok = true;
-        for (int x = 0; x < total && ok; x++) {
-            const int st = x % L::kStages, i = x >> 1;
-            const bool v = x & 1;
-            const int j0 = key_of(i);
-            if (x >= L::kStages) ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
-            if (!ok) break;
-            uint8_t* base = sm + L::kStageOff + st * L::kStage;
-            if (!v && lt < 8) {  // the tile's scales (lanes 0..7 of the first loader warp hold its pages)
-                float ks = pages_k >= 0 ? 1.0f : kGone, vs = kVNone;
-                if (Q8 && pages_k >= 0) {
-                    ks = c.k_scale[int64_t(pages_k) * c.scale_stride + kvh];
-                    ks = fabsf(ks);  // scales are not negative: kGone stays apart
-                    vs = fmaxf(log2f(c.v_scale[int64_t(pages_k) * c.scale_stride + kvh]), kVNone);
-                }
-                ms.ks[i % kRing][lt] = ks;
-                ms.vs[i % kRing][lt] = vs;
-            }
-            if (!v && i + 1 < nt) pages_next = lane < 8 ? page_at(key_of(i + 1) + 16 * lane) : -1;
-            if constexpr (Q8) {
+        if constexpr (Q8) {
+            constexpr int kRowChunks = HD / 16;             // 16-byte pieces of a key row
+            constexpr int kRowsAt = kLoaders / kRowChunks;  // key rows of one round of pieces: 12 or 24
+            constexpr int kPer = (kKeys + kRowsAt - 1) / kRowsAt;
+            const int piece = lt % kRowChunks, row_in = lt / kRowChunks;
+            const int64_t inner = int64_t(kvh) * c.page_size * HD + piece * 16;
+            uint4 got[kPer];
+            auto fetch = [&](const void* pool, int j0) {
+                const uint8_t* base = static_cast<const uint8_t*>(pool) + inner;
+                const int64_t at = pages >= 0 ? int64_t(pages) * c.page_stride : -1;
+                const int at_lo = int(uint32_t(at)), at_hi = int(at >> 32);
 #pragma unroll
                 for (int y = 0; y < kPer; y++) {
                     const int r = row_in + y * kRowsAt;
-                    const uint4 w = held_regs[y];
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                    const uint32_t o_lo = __shfl_sync(0xffffffffu, at_lo, r >> 4);  // rows past 128: lane 8, no page
+                    const int o_hi = __shfl_sync(0xffffffffu, at_hi, r >> 4);
+                    const uint8_t* p = base + (int64_t(o_hi) << 32 | o_lo) + (r & (c.page_size - 1)) * HD;
+                    got[y] = o_hi >= 0 && r < len - j0 ? ldg_stream(p) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            // Pieces of the second 64 values write their 16-byte halves in the other order: eight lanes, eight bank groups.
+            const bool second = piece >= 4;
+            const uint32_t place = second ? L::kHalf : 0;
+            const int ch0 = piece * 2 % 8 + second, ch1 = piece * 2 % 8 + !second;
+            float ks = 0.0f, vs = 0.0f;  // lt < 8: the scales of this thread's block of the tile
+            auto scales = [&]() {
+                if (lt < 8 && pages >= 0) {
+                    ks = c.k_scale[int64_t(pages) * c.scale_stride + kvh];
+                    vs = c.v_scale[int64_t(pages) * c.scale_stride + kvh];
+                }
+            };
+            if (nt > 0) {
+                scales();
+                fetch(c.k_pages, key_of(0));
+            }
+            for (int x = 0; x < total; x++) {
+                const int st = x % L::kStages, i = x >> 1;
+                const bool v = x & 1;
+                if (x >= L::kStages) {
+                    ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                uint8_t* base = sm + L::kStageOff + st * L::kStage + place;
+                if (!v) {
+                    if (lt < 8) {
+                        ms.ks[i % kRing][lt] = pages >= 0 ? fabsf(ks) : kGone;
+                        ms.vs[i % kRing][lt] = pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone;
+                    }
+                    // every loader thread is past item x - kStages (the wait above), so none has touched tile i + 2's yet
+                    if (lt >= 32 && lt < 36) ms.odd[(i + 2) % kOddRing][lt - 32] = 0;
+                    if (i + 1 < nt) pages_next = pages_of(key_of(i + 1));
+                } else if (!open(key_of(i), pos_lo, pos_hi)) {  // values that are not numbers leave the operand
+#pragma unroll
+                    for (int y = 0; y < kPer; y++) {
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&got[y]);
+                        bool odd = false;
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            // 0x80 of each byte whose low seven bits are all ones
+                            const uint32_t nan = ((w[z] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                            odd |= nan != 0;
+                            w[z] &= ~(nan | (nan - (nan >> 7)));
+                        }
+                        const int r = row_in + y * kRowsAt;
+                        if (odd) atomicOr(&ms.odd[i % kOddRing][r >> 5], 1u << (r & 31));  // r < 128: others are zeros
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < kPer; y++) {
+                    const uint32_t ws[4] = {got[y].x, got[y].y, got[y].z, got[y].w};
                     uint32_t f[8];
 #pragma unroll
                     for (int z = 0; z < 4; z++) f[2 * z] = e4m3x2_to_f16x2(uint16_t(ws[z])), f[2 * z + 1] = e4m3x2_to_f16x2(uint16_t(ws[z] >> 16));
-                    uint8_t* p = base + (piece * 16 / 64) * L::kHalf;
-                    const int ch = (piece * 2) % 8;
-                    uint4* p0 = reinterpret_cast<uint4*>(p + sw128_off(r, ch));
-                    uint4* p1 = reinterpret_cast<uint4*>(p + sw128_off(r, ch + 1));
-                    const uint4 v0 = make_uint4(f[0], f[1], f[2], f[3]), v1 = make_uint4(f[4], f[5], f[6], f[7]);
-                    // the two 64-wide halves take opposite pieces first: eight lanes, eight bank groups
-                    if (piece * 16 / 64) *p1 = v1, *p0 = v0;
-                    else *p0 = v0, *p1 = v1;
-                }
-                // the next item's pieces, while this one is used
-                if (x + 1 < total) {
-                    if (v) pages_k = pages_next;
-                    fetch8(!v, v ? key_of(i + 1) : j0, pages_k);
-                }
-                publish(x);
-            } else {
-                constexpr int kIn = 16 / kRowsAt;  // pieces of a thread per block of 16 keys
-#pragma unroll 2
-                for (int blk = 0; blk < 8; blk++) {
-                    const int page = __shfl_sync(0xffffffffu, pages_k, blk);
-                    const int r = 16 * blk + row_in;
-                    const uint8_t* p = page >= 0 ? src(v, page, j0 + r) : static_cast<const uint8_t*>(c.k_pages);
-                    uint8_t* dst = base + (piece / 8) * L::kHalf + sw128_off(r, piece % 8);
-#pragma unroll
-                    for (int y = 0; y < kIn; y++) {
-                        const bool in = page >= 0 && j0 + r + y * kRowsAt < len;
-                        // rows kRowsAt (a multiple of 8) further on: the same place in the swizzle's pattern
-                        cp16(dst + y * kRowsAt * 128, in ? p + y * kRowsAt * HD * kB : p, in ? 16 : 0);
+                    const uint4 a0 = make_uint4(f[0], f[1], f[2], f[3]), a1 = make_uint4(f[4], f[5], f[6], f[7]);
+                    const int r = row_in + y * kRowsAt;
+                    if ((y + 1) * kRowsAt <= kKeys || r < kKeys) {
+                        *reinterpret_cast<uint4*>(base + sw128_off(r, ch0)) = second ? a1 : a0;
+                        *reinterpret_cast<uint4*>(base + sw128_off(r, ch1)) = second ? a0 : a1;
                     }
                 }
-                cp_commit();
-                if (v) pages_k = pages_next;
-                if (x > 0) {
-                    cp_wait<1>();
-                    publish(x - 1);
+                fence_proxy_async();
+                mbar_arrive(&ms.full[st]);
+                if (x + 1 < total) {  // the next item's pieces fly while this one is used
+                    if (v) {
+                        pages = pages_next;
+                        scales();
+                    }
+                    fetch(v ? c.k_pages : c.v_pages, key_of((x + 1) >> 1));
                 }
             }
+        } else {
+            // one warp starts the tensor copies, a lane per page and 64 values; all four look through the tiles that need it
+            const int per_page = kKeys / c.page_size, box = lane >> (HD / 64 - 1), half = lane & (HD / 64 - 1);
+            const uint32_t box_bytes = uint32_t(c.page_size) * 128;
+            const bool carrier = box < per_page;  // at most 16 lanes (8 pages of 16 tokens, two halves)
+            int scans = 0;
+            for (int x = 0; x < total; x++) {
+                const int st = x % L::kStages, i = x >> 1;
+                const bool v = x & 1;
+                const int j0 = key_of(i);
+                uint8_t* base = sm + L::kStageOff + st * L::kStage;
+                const bool strict = !open(j0, pos_lo, pos_hi);
+                const bool scan = v && (strict || !__all_sync(0xffffffffu, lane >= 8 || pages >= 0));
+                if (warp == 8) {
+                    if (x >= L::kStages) {
+                        ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                    }
+                    if (!v && lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? 1.0f : kGone;
+                    if (!v && lane < 4) ms.odd[(i + 2) % kOddRing][lane] = 0;
+                    const int page = __shfl_sync(0xffffffffu, pages, carrier ? box << (ps_log - 4) : 31);
+                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                    uint64_t* bar = scan ? &ms.land : &ms.full[st];
+                    if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_bytes);
+                    __syncwarp();
+                    if (page >= 0)
+                        copy_box(base + half * L::kHalf + box * box_bytes, v ? &maps.v : &maps.k, half * 64, kvh * c.page_size, page, bar);
+                }
+                if (scan) {
+                    ok = wait_on(&ms.land, scans & 1, fail);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    // a thread per key row: rows that nobody holds are zeroed, values that are not finite taken out
+                    for (int r = lt; r < kKeys + 64; r += kLoaders) {  // whole warps: 96 rows, then 32 and nothing
+                        const bool dead = __shfl_sync(0xffffffffu, pages, (r >> 4) & 7) < 0 || j0 + r >= len;
+                        if (r >= kKeys) continue;
+                        bool odd = false;
+                        for (int h = 0; h < HD / 64; h++)
+                            for (int ch = 0; ch < 8; ch++) {
+                                uint4* p = reinterpret_cast<uint4*>(base + h * L::kHalf + sw128_off(r, ch));
+                                if (dead) {
+                                    *p = make_uint4(0, 0, 0, 0);
+                                } else if (strict) {
+                                    uint4 u = *p;
+                                    if (drop_odd(u)) *p = u, odd = true;
+                                }
+                            }
+                        if (odd) atomicOr(&ms.odd[i % kOddRing][r >> 5], 1u << (r & 31));
+                    }
+                    fence_proxy_async();
+                    mbar_arrive(&ms.scanned);
+                    if (warp == 8) {
+                        ok = wait_on(&ms.scanned, scans & 1, fail);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive(&ms.full[st]);
+                    }
+                    scans++;
+                }
+                if (!v && i + 1 < nt) pages_next = pages_of(key_of(i + 1));
+                if (v) pages = pages_next;
+            }
         }
-        if constexpr (!Q8) {
-            cp_wait<0>();
-            if (ok && total > 0) publish(total - 1);
-        }
-    } else if (warp == 12) {
+    } else if (warp == 11) {
         // ------------------------------------------------------------------ UMMA issue
         if (lane == 0 && nt > 0) {
             constexpr uint32_t idesc_s = f16_idesc(kRows, kKeys), idesc_o = f16_idesc(kRows, HD) | (1u << 16);
@@ -484,33 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             }
             const bool plain_mask = open(j0, h_lo, h_hi) && resident;
             const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
-            // ---- the row's largest score (log2 units); loops are kept rolled: straight code of a few KB per pass was
-            // bound by instruction fetch
-            float top = -INFINITY;
-            if (!cooked) {
-                uint32_t w[2][32];
-                ld32(ts, w[0]);
-#pragma unroll 1
-                for (int q = 0; q < 4; q += 2) {
-#pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        ld_wait(w[y]);
-                        if (y == 0 || q == 0) ld32(ts + 32 * (q + y + 1), w[y ^ 1]);
-#pragma unroll
-                        for (int g = 0; g < 2; g++) {
-                            float m0 = __uint_as_float(w[y][16 * g]), m1 = __uint_as_float(w[y][16 * g + 1]);
-#pragma unroll
-                            for (int x = 2; x < 16; x += 2) {
-                                m0 = fmaxf(m0, __uint_as_float(w[y][16 * g + x]));
-                                m1 = fmaxf(m1, __uint_as_float(w[y][16 * g + x + 1]));
-                            }
-                            m0 = fmaxf(m0, m1);
-                            top = fmaxf(top, Q8 ? m0 * ksp[2 * (q + y) + g] : m0);
-                        }
-                    }
-                }
-                top *= down * kLog2e;
-            } else {
+            // ---- the row's largest score (log2 units); the masking loop is
+            // kept rolled: as straight code it was bound by instruction fetch
+            if (cooked) {  // scale, cap, bias and masks, back into TMEM
 #pragma unroll 1
                 for (int q = 0; q < 4; q++) {
                     uint32_t u[32];
@@ -540,12 +574,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             if (!see) u[x] = __float_as_uint(-INFINITY);
                         }
                     }
-#pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(u[x]));
                     st32(ts + 32 * q, u);
                 }
                 st_wait();
             }
+            uint32_t w[4][32];  // the row's scores
+#pragma unroll
+            for (int q = 0; q < 4; q++) ld32(ts + 32 * q, w[q]);
+#pragma unroll
+            for (int q = 0; q < 4; q++) ld_wait(w[q]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const float* u = reinterpret_cast<const float*>(&w[q][16 * g]);
+                    float m0 = fmaxf(fmaxf(u[0], u[1]), u[2]), m1 = fmaxf(fmaxf(u[3], u[4]), u[5]);
+                    m0 = fmaxf(fmaxf(m0, u[6]), u[7]), m1 = fmaxf(fmaxf(m1, u[8]), u[9]);
+                    m0 = fmaxf(fmaxf(m0, u[10]), u[11]), m1 = fmaxf(fmaxf(m1, u[12]), u[13]);
+                    m0 = fmaxf(fmaxf(fmaxf(m0, u[14]), u[15]), m1);
+                    top = fmaxf(top, Q8 && !cooked ? m0 * ksp[2 * q + g] : m0);
+                }
+            if (!cooked) top *= down * kLog2e;
             // ---- the reference maximum and value scale
             const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
             const bool up = top > row_max + kLazy;  // also from -inf
@@ -555,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 ok = wait_on(&ms.full[stv], (xv / L::kStages) & 1, fail);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                odd_tile = (ms.odd[stv][0] | ms.odd[stv][1] | ms.odd[stv][2] | ms.odd[stv][3]) != 0;
+                const uint32_t* od = ms.odd[i % kOddRing];
+                odd_tile = (od[0] | od[1] | od[2] | od[3]) != 0;
             }
             if (__any_sync(0xffffffffu, up || v_up || odd_tile)) {
                 float f = 1.0f;
@@ -577,15 +628,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 if (i > 0 || odd_tile) {
 #pragma unroll 1
                     for (int x = 0; x < HD; x += 32) {
-                        uint32_t w[32];
-                        ld32(to + x, w);
-                        ld_wait(w);
+                        uint32_t o[32];
+                        ld32(to + x, o);
+                        ld_wait(o);
 #pragma unroll
-                        for (int y = 0; y < 32; y++) w[y] = __float_as_uint(__uint_as_float(w[y]) * f);
+                        for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
                         if (odd_tile) {
 #pragma unroll 1
                             for (int key = 0; key < kKeys; key++) {
-                                if (!(ms.odd[stv][key >> 5] >> (key & 31) & 1)) continue;
+                                if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
                                 const int j = j0 + key, slot = j / c.page_size;
                                 if (j >= len || ksp[key >> 4] == kGone) continue;
                                 const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
@@ -600,11 +651,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                                         v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
                                         if (fabsf(v) <= 65504.0f) v = 0.0f;
                                     }
-                                    if (see) w[y] = __float_as_uint(__uint_as_float(w[y]) + v);
+                                    if (see) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
                                 }
                             }
                         }
-                        st32(to + x, w);
+                        st32(to + x, o);
                     }
                     st_wait();
                 }
@@ -614,49 +665,42 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             {
                 const float f0 = cooked ? 1.0f : down * kLog2e;
                 uint64_t sums[2] = {0, 0};
-                uint32_t w[2][32];
-                ld32(ts, w[0]);
-#pragma unroll 1
-                for (int q = 0; q < 4; q += 2) {
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        ld_wait(w[y]);
-                        if (y == 0 || q == 0) ld32(ts + 32 * (q + y + 1), w[y ^ 1]);
-                        uint32_t(&u)[32] = w[y];
+                for (int q = 0; q < 4; q++) {
+                    uint32_t(&u)[32] = w[q];
 #pragma unroll
-                        for (int g = 0; g < 2; g++) {
-                            const int blk = 2 * (q + y) + g;
-                            const float f = Q8 && !cooked ? f0 * ksp[blk] : f0;
-                            const float vr = Q8 ? fmaxf(vsp[blk] - vref, kVMin) : 0.0f;
-                            const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
-                            if (Q8) sums[0] = sums[1] = 0;
+                    for (int g = 0; g < 2; g++) {
+                        const int blk = 2 * q + g;
+                        const float f = Q8 && !cooked ? f0 * ksp[blk] : f0;
+                        const float vr = Q8 ? fmaxf(vsp[blk] - vref, kVMin) : 0.0f;
+                        const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
+                        if (Q8) sums[0] = sums[1] = 0;
 #pragma unroll
-                            for (int x = 16 * g; x < 16 * g + 16; x += 2) {
-                                float z0, z1;
-                                unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
-                                z0 = ex2(z0), z1 = ex2(z1);
-                                u[x] = __float_as_uint(z0), u[x + 1] = __float_as_uint(z1);
-                                sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
-                            }
-                            if (Q8) {  // the sum without the value scale
-                                float z0, z1;
-                                unpack2(add2(sums[0], sums[1]), z0, z1);
-                                row_sum = fmaf(z0 + z1, ex2(-vr), row_sum);
-                            }
+                        for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                            float z0, z1;
+                            unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
+                            z0 = ex2(z0), z1 = ex2(z1);
+                            u[x] = __float_as_uint(z0), u[x + 1] = __float_as_uint(z1);
+                            sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
                         }
-                        if constexpr (HILO) {
-                            uint32_t hl[32];
-#pragma unroll
-                            for (int x = 0; x < 16; x++)
-                                split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
-                            st32(ts + 32 * (q + y), hl);
-                        } else {
-                            uint32_t p[16];
-#pragma unroll
-                            for (int x = 0; x < 16; x++)
-                                p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
-                            st16(ts + 16 * (q + y), p);
+                        if (Q8) {  // the sum without the value scale
+                            float z0, z1;
+                            unpack2(add2(sums[0], sums[1]), z0, z1);
+                            row_sum = fmaf(z0 + z1, ex2(-vr), row_sum);
                         }
+                    }
+                    if constexpr (HILO) {
+                        uint32_t hl[32];
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
+                        st32(ts + 32 * q, hl);
+                    } else {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++)
+                            p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
+                        st16(ts + 16 * q, p);
                     }
                 }
                 if (!Q8) {
@@ -703,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     auto put = [&](int r, int d, float4 v) {
         const int pr = r0 + r;
         const int64_t off = int64_t(row0 + pr / G) * a.o_token + int64_t(kvh * G + pr % G) * a.o_head + d;
@@ -769,7 +813,11 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.ranks > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, fn, a, p);
+    PromptMaps maps = {};
+    if (!Q8 && (!encode_f16_pages(&maps.k, c.k_pages, HD, c.n_kv * c.page_size, c.num_pages, c.page_stride * 2, c.page_size) ||
+                !encode_f16_pages(&maps.v, c.v_pages, HD, c.n_kv * c.page_size, c.num_pages, c.page_stride * 2, c.page_size)))
+        return cudaErrorNotSupported;
+    return cudaLaunchKernelEx(&cfg, fn, a, p, maps);
 }
 
 template <int HD>

@@ -66,4 +66,31 @@ inline bool encode_u8_2d(CUtensorMap* map, const void* base, uint64_t cols, uint
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// [pages][rows] x [cols] f16 (rows of a page contiguous, pages page_bytes apart) read in boxes of box_rows rows x 64
+// columns of one page, with the 128-byte swizzle. False as encode_f16_2d_sw128.
+inline bool encode_f16_pages(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pages,
+                             uint64_t page_bytes, uint32_t box_rows) {
+    using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Fn fn = []() -> Fn {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        return reinterpret_cast<Fn>(p);
+    }();
+    if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || page_bytes % 16 || box_rows > 256) return false;
+    const cuuint64_t dims[3] = {cols, rows, pages};
+    const cuuint64_t strides[2] = {cols * 2, page_bytes};
+    const cuuint32_t box[3] = {64u, box_rows, 1u};
+    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace neko

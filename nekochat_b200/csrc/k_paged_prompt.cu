@@ -72,6 +72,8 @@ struct Misc {
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
+    float vtop[kRing];                 // the largest of vs
+    uint32_t whole[kRing];             // every block is resident
     uint32_t odd[kOddRing][4];         // of a key tile that needs masks: keys with values that are not finite
     float qdown[2 * kRows];            // scale / the row's power of two
 };
@@ -113,6 +115,11 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Two f32 operations in one instruction.
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
@@ -130,6 +137,33 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+// 2^x of two numbers (at least 2^-126) off the special-function unit, which is what bounds the softmax: the integer part
+// by adding 1.5 * 2^23, a polynomial of degree 4 for the rest (least maximum relative error on [-1/2, 1/2]: 2.6e-6,
+// against 2.4e-4 of the f16 that the weight is rounded to).
+__device__ __forceinline__ void exp2_poly(float& x, float& y) {
+    const uint64_t magic = pack2(12582912.0f, 12582912.0f), less = pack2(-12582912.0f, -12582912.0f), neg = pack2(-1.0f, -1.0f);
+    const uint64_t z = pack2(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    const uint64_t r = add2(z, magic), f = fma2(add2(r, less), neg, z);
+    uint64_t p = pack2(0.009570086374878883f, 0.009570086374878883f);
+    p = fma2(p, f, pack2(0.055917900055646896f, 0.055917900055646896f));
+    p = fma2(p, f, pack2(0.2402474582195282f, 0.2402474582195282f));
+    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float r0, r1, p0, p1;
+    unpack2(r, r0, r1), unpack2(p, p0, p1);
+    x = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+    y = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
 }
 // Bounded wait that also ends once another role has failed; false: give up.
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile uint32_t* fail) {
@@ -336,9 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 uint8_t* base = sm + L::kStageOff + st * L::kStage + place;
                 if (!v) {
-                    if (lt < 8) {
-                        ms.ks[i % kRing][lt] = pages >= 0 ? fabsf(ks) : kGone;
-                        ms.vs[i % kRing][lt] = pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone;
+                    if (warp == 8) {
+                        const float vl = lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone, vt = warp_max(vl);
+                        const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0);
+                        if (lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? fabsf(ks) : kGone, ms.vs[i % kRing][lane] = vl;
+                        if (lane == 0) ms.vtop[i % kRing] = vt, ms.whole[i % kRing] = whole;
                     }
                     // every loader thread is past item x - kStages (the wait above), so none has touched tile i + 2's yet
                     if (lt >= 32 && lt < 36) ms.odd[(i + 2) % kOddRing][lt - 32] = 0;
@@ -394,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const int j0 = key_of(i);
                 uint8_t* base = sm + L::kStageOff + st * L::kStage;
                 const bool strict = !open(j0, pos_lo, pos_hi);
-                const bool scan = v && (strict || !__all_sync(0xffffffffu, lane >= 8 || pages >= 0));
+                const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0), scan = v && (strict || !whole);
                 if (warp == 8) {
                     if (x >= L::kStages) {
                         ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
@@ -403,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     if (!v && lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? 1.0f : kGone;
                     if (!v && lane < 4) ms.odd[(i + 2) % kOddRing][lane] = 0;
+                    if (!v && lane == 0) ms.whole[i % kRing] = whole;
                     const int page = __shfl_sync(0xffffffffu, pages, carrier ? box << (ps_log - 4) : 31);
                     const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
                     uint64_t* bar = scan ? &ms.land : &ms.full[st];
@@ -448,58 +485,74 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         }
     } else if (warp == 11) {
         // ------------------------------------------------------------------ UMMA issue
-        if (lane == 0 && nt > 0) {
+        // The whole warp walks the loop and one elected lane issues: with the role on a single lane of a divergent warp the
+        // operands' descriptors went through vector registers, about 70 cycles an UMMA.
+        if (nt > 0) {
             constexpr uint32_t idesc_s = f16_idesc(kRows, kKeys), idesc_o = f16_idesc(kRows, HD) | (1u << 16);
-            const uint32_t q_base = smem_u32(sm), st_base = smem_u32(sm + L::kStageOff);
+            const uint64_t q_desc = sw128_desc(smem_u32(sm)), k_desc = sw128_desc(smem_u32(sm + L::kStageOff)),
+                           vv_desc = v_desc(smem_u32(sm + L::kStageOff));
             auto issue_s = [&](int h, int st) {
-                const uint32_t kb = st_base + st * L::kStage;
+                const uint64_t qd = q_desc + uint64_t(h * L::kParts * (L::kQTile >> 4));
+                const uint64_t kd = k_desc + uint64_t(st * (L::kStage >> 4));
+                if (elect_one()) {
 #pragma unroll
-                for (int part = 0; part < L::kParts; part++)
+                    for (int part = 0; part < L::kParts; part++)
 #pragma unroll
-                    for (int k = 0; k < HD / 16; k++) {
-                        const uint32_t off = (k / 4) * L::kHalf + (k % 4) * 32;
-                        umma_f16(tmem + h * 128, sw128_desc(q_base + (h * L::kParts + part) * L::kQTile + off), sw128_desc(kb + off),
-                                 idesc_s, part + k > 0 ? 1u : 0u);
-                    }
-            };
-            auto issue_pv = [&](int h, int st) {
-                const uint32_t vb = st_base + st * L::kStage;
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; k++) {
-                    // weights of keys 16 k ..: f16 columns 8 k; hi + lo: 32-column groups of hi, lo (16 each)
-                    const uint32_t col = HILO ? uint32_t(32 * (k / 2) + 8 * (k % 2)) : uint32_t(8 * k);
-                    umma_ts(tmem + 256 + h * 128, tmem + h * 128 + col, v_desc(vb + k * 2048), idesc_o);
-                    if constexpr (HILO) umma_ts(tmem + 256 + h * 128, tmem + h * 128 + col + 16, v_desc(vb + k * 2048), idesc_o);
-                }
-            };
-            bool ok = wait_on(&ms.full[0], 0, fail);
-            if (ok) {
-                for (int h = 0; h < mt; h++) {
-                    issue_s(h, 0);
+                        for (int k = 0; k < HD / 16; k++) {
+                            const uint32_t off = ((k / 4) * L::kHalf + (k % 4) * 32) >> 4;
+                            umma_f16(tmem + h * 128, qd + part * (L::kQTile >> 4) + off, kd + off, idesc_s, part + k > 0);
+                        }
                     umma_commit(&ms.s_full[h]);
                 }
-                umma_commit(&ms.empty[0]);
+            };
+            auto issue_pv = [&](int h, int st) {
+                // weights of keys 16 k ..: f16 columns 8 k; hi + lo: 32-column groups of hi, lo (16 each)
+                const uint32_t p = tmem + h * 128, o = tmem + 256 + h * 128;
+                const uint64_t vd = vv_desc + uint64_t(st * (L::kStage >> 4));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; k++) {
+                        const uint32_t col = HILO ? 32 * (k / 2) + 8 * (k % 2) : 8 * k;
+                        umma_ts(o, p + col, vd + k * (2048 >> 4), idesc_o);
+                        if constexpr (HILO) umma_ts(o, p + col + 16, vd + k * (2048 >> 4), idesc_o);
+                    }
+                    umma_commit(&ms.pv_done[h]);
+                }
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (elect_one()) umma_commit(bar);
+            };
+            bool ok = wait_on(&ms.full[0], 0, fail);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                for (int h = 0; h < mt; h++) issue_s(h, 0);
+                commit(&ms.empty[0]);
             }
+            int sv = 1, pv = 0, sk = 2 % L::kStages, pk = 2 / L::kStages;  // stages and phases of V of this tile and K of the next
+            auto next = [&](int& st, int& ph) {
+                st += 2;
+                if (st >= L::kStages) st -= L::kStages, ph ^= 1;
+            };
             for (int i = 0; i < nt && ok; i++) {
-                const int xv = 2 * i + 1, xk = 2 * i + 2;
-                ok = wait_on(&ms.full[xv % L::kStages], (xv / L::kStages) & 1, fail);
+                ok = wait_on(&ms.full[sv], pv, fail);
                 for (int h = 0; h < mt && ok; h++) {
-                    ok = wait_on(&ms.p_full[h], i & 1, fail);
+                    ok = ok && wait_on(&ms.p_full[h], i & 1, fail);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(h, xv % L::kStages);
-                    umma_commit(&ms.pv_done[h]);
-                    if (h == mt - 1) umma_commit(&ms.empty[xv % L::kStages]);
+                    issue_pv(h, sv);
+                    if (h == mt - 1) commit(&ms.empty[sv]);
                     if (i + 1 < nt) {
-                        if (h == 0) ok = wait_on(&ms.full[xk % L::kStages], (xk / L::kStages) & 1, fail);
+                        if (h == 0) ok = wait_on(&ms.full[sk], pk, fail);
+                        ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
-                        issue_s(h, xk % L::kStages);
-                        umma_commit(&ms.s_full[h]);
-                        if (h == mt - 1) umma_commit(&ms.empty[xk % L::kStages]);
+                        issue_s(h, sk);
+                        if (h == mt - 1) commit(&ms.empty[sk]);
                     }
                 }
+                next(sv, pv), next(sk, pk);
             }
-            umma_commit(&ms.drain);  // nothing is in flight when the TMEM is freed, whatever happened
+            commit(&ms.drain);  // nothing is in flight when the TMEM is freed, whatever happened
             mbar_wait(&ms.drain, 0);
         }
         __syncwarp();
@@ -533,14 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             tc_fence_after();
             const float* ksp = ms.ks[i % kRing];
             const float* vsp = ms.vs[i % kRing];
-            bool resident = true;
-            float vnow = kVNone;
-#pragma unroll
-            for (int x = 0; x < 8; x++) {
-                resident &= ksp[x] != kGone;
-                if constexpr (Q8) vnow = fmaxf(vnow, vsp[x]);
-            }
-            const bool plain_mask = open(j0, h_lo, h_hi) && resident;
+            const bool plain_mask = open(j0, h_lo, h_hi) && ms.whole[i % kRing];
+            const float vnow = Q8 ? ms.vtop[i % kRing] : 0.0f;
             const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
             // ---- the row's largest score (log2 units); the masking loop is
             // kept rolled: as straight code it was bound by instruction fetch
@@ -589,13 +636,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
                     const float* u = reinterpret_cast<const float*>(&w[q][16 * g]);
-                    float m0 = fmaxf(fmaxf(u[0], u[1]), u[2]), m1 = fmaxf(fmaxf(u[3], u[4]), u[5]);
-                    m0 = fmaxf(fmaxf(m0, u[6]), u[7]), m1 = fmaxf(fmaxf(m1, u[8]), u[9]);
-                    m0 = fmaxf(fmaxf(m0, u[10]), u[11]), m1 = fmaxf(fmaxf(m1, u[12]), u[13]);
-                    m0 = fmaxf(fmaxf(fmaxf(m0, u[14]), u[15]), m1);
-                    top = fmaxf(top, Q8 && !cooked ? m0 * ksp[2 * q + g] : m0);
+                    float m[4] = {u[0], u[1], u[2], u[3]};
+#pragma unroll
+                    for (int x = 4; x < 16; x++) m[x & 3] = max_nan(m[x & 3], u[x]);
+                    const float m0 = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+                    top = max_nan(top, Q8 && !cooked ? m0 * ksp[2 * q + g] : m0);
                 }
             if (!cooked) top *= down * kLog2e;
+            if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
             // ---- the reference maximum and value scale
             const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
             const bool up = top > row_max + kLazy;  // also from -inf
@@ -679,9 +727,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                         for (int x = 16 * g; x < 16 * g + 16; x += 2) {
                             float z0, z1;
                             unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
-                            z0 = ex2(z0), z1 = ex2(z1);
+                            if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
+                            else z0 = ex2(z0), z1 = ex2(z1);
                             u[x] = __float_as_uint(z0), u[x + 1] = __float_as_uint(z1);
                             sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
+                        }
+                        if constexpr (HILO) {
+                            uint32_t hi8[8], lo8[8];
+#pragma unroll
+                            for (int x = 0; x < 8; x++)
+                                split_hilo(__uint_as_float(u[16 * g + 2 * x]), __uint_as_float(u[16 * g + 2 * x + 1]), hi8[x], lo8[x]);
+                            st8(ts + 32 * q + 8 * g, hi8);
+                            st8(ts + 32 * q + 16 + 8 * g, lo8);
                         }
                         if (Q8) {  // the sum without the value scale
                             float z0, z1;
@@ -689,13 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             row_sum = fmaf(z0 + z1, ex2(-vr), row_sum);
                         }
                     }
-                    if constexpr (HILO) {
-                        uint32_t hl[32];
-#pragma unroll
-                        for (int x = 0; x < 16; x++)
-                            split_hilo(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1]), hl[x], hl[16 + x]);
-                        st32(ts + 32 * q, hl);
-                    } else {
+                    if constexpr (!HILO) {
                         uint32_t p[16];
 #pragma unroll
                         for (int x = 0; x < 16; x++)

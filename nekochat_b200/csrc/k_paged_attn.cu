@@ -27,7 +27,6 @@ namespace neko {
 
 namespace {
 
-constexpr int kWarps = 8;
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
@@ -62,13 +61,17 @@ __device__ __forceinline__ void load_words(const uint8_t* p, int step, uint32_t 
     }
 }
 
+// CTAs of 8 warps per SM, by the registers that a key group in flight takes.
+template <int kWarps, int HD, bool Q8, int NT>
+constexpr int kCtas = kWarps == 16 ? 1 : NT == 1 && (Q8 || HD <= 64) ? 2 : 1;
+
 struct DecodePlan {
     int ranks;      // CTAs per (sequence, KV head, row tile): the cluster
     int row_tiles;  // tiles of packed rows
 };
 
 // Columns of an MMA: 8 rows (16-bit queries) or 4 (f32: hi and lo columns).
-template <int HD, bool Q8, bool HILO, int NT>
+template <int HD, bool Q8, bool HILO, int NT, int kWarps>
 struct Tile {
     static constexpr int kRowsPer = HILO ? 4 : 8;
     static constexpr int kRows = NT * kRowsPer;
@@ -79,10 +82,10 @@ struct Tile {
     static constexpr size_t kSmem = size_t(kWarps + 1) * kState * 4;
 };
 
-template <int HD, bool Q8, bool HILO, int NT>
-__global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_paged_attention_args a,
-                                                                  const DecodePlan plan) {
-    using TL = Tile<HD, Q8, HILO, NT>;
+template <int HD, bool Q8, bool HILO, int NT, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_decode_kernel(
+    const neko_paged_attention_args a, const DecodePlan plan) {
+    using TL = Tile<HD, Q8, HILO, NT, kWarps>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
     extern __shared__ __align__(16) float sm[];
@@ -228,22 +231,33 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
         }
     };
 
-    int k = k_begin + warp;
-    int page = page_of(k);
-    if (page >= 0) load_k(page, key_of(k));
-    for (; k < k_end; k += kWarps) {
-        const int next_page = page_of(k + kWarps);
-        const int j0 = key_of(k);
-        if (page < 0) {
-            page = next_page;
-            if (page >= 0) load_k(page, key_of(k + kWarps));
-            continue;
-        }
-        load_v(page, j0);
-        float ks = 1.0f, vs = 1.0f;
+    float ks = 1.0f, vs = 1.0f;
+    auto load_scales = [&](int page) {
         if constexpr (Q8) {
             ks = c.k_scale[int64_t(page) * c.scale_stride + kvh];
             vs = c.v_scale[int64_t(page) * c.scale_stride + kvh];
+        }
+    };
+    // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
+    // scores, V from the end of its P V.
+    int k = k_begin + warp;
+    int page = page_of(k), next_page = page_of(k + kWarps);
+    if (page >= 0) {
+        load_k(page, key_of(k));
+        load_scales(page);
+        load_v(page, key_of(k));
+    }
+    for (; k < k_end; k += kWarps) {
+        const int j0 = key_of(k), j1 = key_of(k + kWarps);
+        const int after = page_of(k + 2 * kWarps);
+        if (page < 0) {
+            page = next_page, next_page = after;
+            if (page >= 0) {
+                load_k(page, j1);
+                load_scales(page);
+                load_v(page, j1);
+            }
+            continue;
         }
         // ---- scores
         float sc[NT][4];
@@ -262,8 +276,12 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
                 else mma16816(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
             }
         }
-        page = next_page;
-        if (page >= 0) load_k(page, key_of(k + kWarps));  // overlaps the softmax and P V
+        const float ks_now = ks, vs_now = vs;
+        page = next_page, next_page = after;
+        if (page >= 0) {
+            load_k(page, j1);
+            load_scales(page);
+        }
         // ---- masks, running maximum, weights
         // free of masks: every key of the group is seen by every row of the tile
         const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= pos_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
@@ -280,7 +298,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
                 for (int h = 0; h < 2; h++) {
                     const float dot = HILO ? sc[nt][2 * h] + sc[nt][2 * h + 1] : sc[nt][2 * h + r];
                     const int j = j0 + g + 8 * h;
-                    float v = dot * (qscale[nt][r] * ks);
+                    float v = dot * (qscale[nt][r] * ks_now);
                     if (a.softcap > 0.0f) v = a.softcap * tanh_abs(__fdividef(v, a.softcap));
                     v = v * kLog2e;
                     if (a.slopes) v += slope[nt][r] * float(j - qpos[nt][r]);
@@ -370,7 +388,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const int r = HILO ? 0 : e & 1;
-                                if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e] * vs;
+                                if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e] * vs_now;
                             }
                         }
                     }
@@ -391,9 +409,10 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
                 mma16816_z(d, f, pf[nt][0], pf[nt][1]);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    acc[nt][i][e] = acc[nt][i][e] * alpha[nt][HILO ? 0 : e & 1] + d[e] * vs;
+                    acc[nt][i][e] = acc[nt][i][e] * alpha[nt][HILO ? 0 : e & 1] + d[e] * vs_now;
             }
         }
+        if (page >= 0) load_v(page, j1);
     }
 
     // ---- the warps' states to shared memory: [row](max, sum, values)
@@ -472,20 +491,17 @@ __global__ void __launch_bounds__(32 * kWarps) paged_decode_kernel(const neko_pa
     cluster.sync();  // no CTA leaves while another reads its state
 }
 
-template <int HD, bool Q8, bool HILO, int NT>
-cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
-    using TL = Tile<HD, Q8, HILO, NT>;
+template <int HD, bool Q8, bool HILO, int NT, int kWarps>
+cudaError_t go(const neko_paged_attention_args& a, int ranks, cudaStream_t st) {
+    using TL = Tile<HD, Q8, HILO, NT, kWarps>;
     const neko_paged_cache& c = a.cache;
     const int G = a.n_head / c.n_kv;
     DecodePlan p;
     p.row_tiles = int((int64_t(a.max_new) * G + TL::kRows - 1) / TL::kRows);
     const int64_t items = int64_t(c.n_seq) * c.n_kv * p.row_tiles;
-    // CTAs per item: enough for two on every SM, as long as each warp keeps two groups of 16 keys
-    const int64_t groups = int64_t(c.max_pages) * c.page_size / 16;
-    p.ranks = 1;
-    while (p.ranks < 16 && items * p.ranks < 2 * num_sms() && groups > 2 * kWarps * p.ranks) p.ranks *= 2;
+    p.ranks = ranks;
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT>;
+    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, kWarps>;
     cudaError_t e = ensure_dyn_smem(fn, TL::kSmem);
     if (e != cudaSuccess) return e;
     if (p.ranks > 8 && (e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
@@ -504,11 +520,26 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, fn, a, p);
 }
 
+// CTAs that share a (sequence, KV head, row tile): enough for two CTAs of 8 warps on every SM, as long as each warp
+// keeps two groups of 16 keys. Where 16 of them do not fill the GPU, CTAs of 16 warps.
+template <int HD, bool Q8, bool HILO, int NT>
+cudaError_t by_work(const neko_paged_attention_args& a, cudaStream_t st) {
+    const neko_paged_cache& c = a.cache;
+    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv), kRows = Tile<HD, Q8, HILO, NT, 8>::kRows;
+    const int64_t items = int64_t(c.n_seq) * c.n_kv * ((rows + kRows - 1) / kRows);
+    const int64_t groups = int64_t(c.max_pages) * c.page_size / 16;
+    int ranks = 1;
+    while (ranks < 16 && items * ranks < 2 * num_sms() && groups > 16 * ranks) ranks *= 2;
+    if (NT == 1 && ranks == 16 && items * 16 <= num_sms() && groups > 32 * ranks)
+        return go<HD, Q8, HILO, NT, NT == 1 ? 16 : 8>(a, ranks, st);
+    return go<HD, Q8, HILO, NT, 8>(a, ranks, st);
+}
+
 template <int HD, bool Q8>
 cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t rows = int64_t(a.max_new) * (a.n_head / a.cache.n_kv);
-    if (a.type == NEKO_T_F32) return rows <= 4 ? go<HD, Q8, true, 1>(a, st) : go<HD, Q8, true, 2>(a, st);
-    return rows <= 8 ? go<HD, Q8, false, 1>(a, st) : go<HD, Q8, false, 2>(a, st);
+    if (a.type == NEKO_T_F32) return rows <= 4 ? by_work<HD, Q8, true, 1>(a, st) : by_work<HD, Q8, true, 2>(a, st);
+    return rows <= 8 ? by_work<HD, Q8, false, 1>(a, st) : by_work<HD, Q8, false, 2>(a, st);
 }
 
 }  // namespace

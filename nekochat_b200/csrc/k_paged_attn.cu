@@ -38,6 +38,17 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
     return d;
 }
+// The bits of a word's values that are not finite (8-bit codes: NaN).
+template <bool Q8>
+__device__ __forceinline__ uint32_t odd_lanes(uint32_t w) {
+    if constexpr (Q8) {
+        const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        return nan | (nan - (nan >> 7));
+    } else {
+        return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+    }
+}
+
 // Words (4 bytes) of one key row that a lane holds: K (a quarter of the row) and V (an eighth).
 template <int HD, bool Q8>
 struct Words {
@@ -66,8 +77,11 @@ template <int kWarps, int HD, bool Q8, int NT>
 constexpr int kCtas = kWarps == 16 ? 1 : NT == 1 && (Q8 || HD <= 64) ? 2 : 1;
 
 struct DecodePlan {
-    int ranks;      // CTAs per (sequence, KV head, row tile): the cluster
-    int row_tiles;  // tiles of packed rows
+    int ranks_log;        // log2 of the CTAs per (sequence, KV head, row tile): the cluster
+    int group;            // query heads per KV head
+    uint64_t group_inv;   // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
+    uint32_t page_16;     // page stride in 16-byte units
+    int page_log;
 };
 
 // Columns of an MMA: 8 rows (16-bit queries) or 4 (f32: hi and lo columns).
@@ -91,19 +105,16 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
-    int b = blockIdx.x;
-    const int rank = b % plan.ranks;
-    b /= plan.ranks;
-    const int tile = b % plan.row_tiles;
-    b /= plan.row_tiles;
-    const int kvh = b % c.n_kv, s = b / c.n_kv;
-    const int G = a.n_head / c.n_kv;
+    const int ranks = 1 << plan.ranks_log;
+    const int rank = blockIdx.x & (ranks - 1), s = blockIdx.x >> plan.ranks_log, kvh = blockIdx.y, tile = blockIdx.z;
+    const int G = plan.group;
+    auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
 
     // the sequence: everything below is the same for all CTAs of the cluster
     const int row0 = a.q_start ? a.q_start[s] : s;
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
-    const int len = min(max(a.kv_len[s], 0), c.max_pages * c.page_size);
-    const int held = max(a.kv_len[s], 0);
+    const int held = max(a.kv_len[s], 0), len = min(held, c.max_pages << plan.page_log);
+    const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {
         if (tid == 0) set_device_error(kErrBadIndex);
         return;
@@ -111,21 +122,76 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     const int r0 = tile * TL::kRows;  // first packed row of this tile
     const int rows = min(n * G - r0, TL::kRows);
     if (rows <= 0) return;
-    const int pos_lo = held - n + r0 / G, pos_hi = held - n + (r0 + rows - 1) / G;
-    const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
+    const int pos_lo = held - n + over_g(r0), pos_hi = held - n + over_g(r0 + rows - 1);
     // keys some row of the tile sees: [0, pre) and [lo, hi), as groups of 16
     const int hi = max(min(len, pos_hi + 1), 0);
     const int lo = a.window ? min(max(pos_lo - a.window + 1, 0), hi) : 0;
     const int g_lo = lo / 16, g_hi = (max(hi, prefix > lo ? prefix : 0) + 15) / 16;
     const int g_pre = min((prefix + 15) / 16, g_lo);  // prefix groups before g_lo
     const int ng = g_pre + max(g_hi - g_lo, 0);
-    const int k_begin = int(int64_t(ng) * rank / plan.ranks), k_end = int(int64_t(ng) * (rank + 1) / plan.ranks);
+    const int k_begin = int(int64_t(ng) * rank >> plan.ranks_log), k_end = int(int64_t(ng) * (rank + 1) >> plan.ranks_log);
+
+    // ---- keys and values: fragments straight from the pages
+    const int32_t* table = c.table + int64_t(s) * c.table_stride;
+    constexpr int kB = Q8 ? 1 : 2;
+    const int in_page = (1 << plan.page_log) - 1;
+    const int64_t head_off = (int64_t(kvh) << plan.page_log) * HD * kB;
+    const uint8_t* kp = static_cast<const uint8_t*>(c.k_pages) + head_off + g * W::kRow + t * (W::kK >= 4 ? 16 : W::kK * 4);
+    const uint8_t* vp = static_cast<const uint8_t*>(c.v_pages) + head_off + 2 * t * W::kRow + g * (W::kV >= 4 ? 16 : W::kV * 4);
+    const float *ksp = c.k_scale + kvh, *vsp = c.v_scale + kvh;
+    auto key_of = [&](int k) { return 16 * (k < g_pre ? k : k - g_pre + g_lo); };  // first key of a group
+    auto page_of = [&](int k) {
+        const int slot = key_of(k) >> plan.page_log;
+        const int p = k < k_end && slot < c.max_pages ? table[slot] : -1;
+        return p < c.num_pages ? p : -1;
+    };
+    uint32_t kw[2][W::kK], vw[4][W::kV];
+    float ks = 1.0f, vs = 1.0f;
+    auto place = [&](int page, int j0) {
+        return (uint64_t(uint32_t(page)) * plan.page_16 << 4) + uint32_t((j0 & in_page) * W::kRow);
+    };
+    auto load_k = [&](int page, int j0) {
+        const uint8_t* p = kp + place(page, j0);
+        load_words(p, 64, kw[0]);
+        load_words(p + 8 * W::kRow, 64, kw[1]);
+        if constexpr (Q8) ks = ksp[int64_t(page) * c.scale_stride];
+    };
+    auto load_v = [&](int page, int j0) {
+        const uint8_t* p = vp + place(page, j0);
+        load_words(p, 128, vw[0]);
+        load_words(p + W::kRow, 128, vw[1]);
+        load_words(p + 8 * W::kRow, 128, vw[2]);
+        load_words(p + 9 * W::kRow, 128, vw[3]);
+        if constexpr (Q8) vs = vsp[int64_t(page) * c.scale_stride];
+    };
+    // the V^T fragments of dims' tiles: word w gives one (f16) or two (8-bit) tiles of 16 dims
+    auto v_frag = [&](int tile_i, uint32_t (&f)[4]) {
+        if constexpr (Q8) {
+            const int w = tile_i >> 1;
+            const uint32_t sel = tile_i & 1 ? 0x7362u : 0x5140u;
+            const uint32_t x = prmt(vw[0][w], vw[1][w], sel), y = prmt(vw[2][w], vw[3][w], sel);
+            f[0] = e4m3x2_to_f16x2(uint16_t(x)), f[1] = e4m3x2_to_f16x2(uint16_t(x >> 16));
+            f[2] = e4m3x2_to_f16x2(uint16_t(y)), f[3] = e4m3x2_to_f16x2(uint16_t(y >> 16));
+        } else {
+            f[0] = prmt(vw[0][tile_i], vw[1][tile_i], 0x5410u), f[1] = prmt(vw[0][tile_i], vw[1][tile_i], 0x7632u);
+            f[2] = prmt(vw[2][tile_i], vw[3][tile_i], 0x5410u), f[3] = prmt(vw[2][tile_i], vw[3][tile_i], 0x7632u);
+        }
+    };
+    // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
+    // scores, V from the end of its P V. The first group's fly while the queries are read.
+    int k = k_begin + warp;
+    int page = page_of(k), next_page = page_of(k + kWarps);
+    if (page >= 0) {
+        load_k(page, key_of(k));
+        load_v(page, key_of(k));
+    }
 
     // ---- queries as B fragments
     uint32_t qf[NT][kSteps][2];
-    float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two
+    float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two (* log2 e without a cap)
     int qpos[NT][TL::kLaneRows];
     float slope[NT][TL::kLaneRows];
+    const float unit = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int r = r0 + nt * TL::kRowsPer + (HILO ? g >> 1 : g);
@@ -136,7 +202,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
 #pragma unroll
             for (int e = 0; e < 4; e++) x[i][e] = 0.0f;
         if (r < n * G) {
-            const int64_t off = int64_t(row0 + r / G) * a.q_token + int64_t(kvh * G + r % G) * a.q_head;
+            const int rt = over_g(r);
+            const int64_t off = int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + r - rt * G) * a.q_head;
             auto fetch = [&](auto* p) {
                 const bool vec = (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0;
 #pragma unroll
@@ -147,7 +214,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
                     load_row<4>(p + d, vec, x[i]);
                 }
             };
-            if (a.type == kTF32) fetch(static_cast<const float*>(a.q) + off);
+            if constexpr (HILO) fetch(static_cast<const float*>(a.q) + off);
             else if (a.type == kTF16) fetch(static_cast<const __half*>(a.q) + off);
             else fetch(static_cast<const __nv_bfloat16*>(a.q) + off);
 #pragma unroll
@@ -166,19 +233,20 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
                 split_hilo(x[i][2 * h] * up, x[i][2 * h + 1] * up, hi2, lo2);
                 qf[nt][i][h] = HILO && (g & 1) ? lo2 : hi2;
             }
-        const float down = a.scale / up;
+        const float down = unit / up;
 #pragma unroll
-        for (int k = 0; k < TL::kLaneRows; k++) {
-            const int rr = HILO ? t : 2 * t + k;  // this lane's score row within the column tile
-            qscale[nt][k] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
-            const int pr = r0 + nt * TL::kRowsPer + rr;
-            qpos[nt][k] = pr < n * G ? held - n + pr / G : kNoRow;
-            slope[nt][k] = a.slopes && pr < n * G ? a.slopes[kvh * G + pr % G] * kLog2e : 0.0f;
+        for (int x2 = 0; x2 < TL::kLaneRows; x2++) {
+            const int rr = HILO ? t : 2 * t + x2;  // this lane's score row within the column tile
+            qscale[nt][x2] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
+            const int pr = r0 + nt * TL::kRowsPer + rr, rt = over_g(pr);
+            qpos[nt][x2] = pr < n * G ? held - n + rt : kNoRow;
+            slope[nt][x2] = a.slopes && pr < n * G ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
         }
     }
 
     float acc[NT][kSteps][4];
     float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];
+    float vref = 0.0f;  // the value scale that the accumulators are in units of
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -186,67 +254,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < TL::kLaneRows; k++) m[nt][k] = -INFINITY, l[nt][k] = 0.0f;
+        for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = -INFINITY, l[nt][r] = 0.0f;
     }
+    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
-    const int32_t* table = c.table + int64_t(s) * c.table_stride;
-    const int ps_log = 31 - __clz(c.page_size);
-    const int64_t head_off = int64_t(kvh) * c.page_size * HD;
-    constexpr int kB = Q8 ? 1 : 2;
-    const uint8_t* kp = static_cast<const uint8_t*>(c.k_pages);
-    const uint8_t* vp = static_cast<const uint8_t*>(c.v_pages);
-    // group index -> first key
-    auto key_of = [&](int k) { return 16 * (k < g_pre ? k : k - g_pre + g_lo); };
-    auto page_of = [&](int k) {
-        const int slot = key_of(k) >> ps_log;
-        const int p = k < k_end && slot < c.max_pages ? table[slot] : -1;
-        return p < c.num_pages ? p : -1;
-    };
-    uint32_t kw[2][W::kK], vw[4][W::kV];
-    auto load_k = [&](int page, int j0) {
-        const uint8_t* p = kp + (int64_t(page) * c.page_stride + head_off + int64_t((j0 & (c.page_size - 1)) + g) * HD) * kB +
-                           t * (W::kK >= 4 ? 16 : W::kK * 4);
-        load_words(p, 64, kw[0]);
-        load_words(p + 8 * W::kRow, 64, kw[1]);
-    };
-    auto load_v = [&](int page, int j0) {
-        const uint8_t* p = vp + (int64_t(page) * c.page_stride + head_off + int64_t((j0 & (c.page_size - 1)) + 2 * t) * HD) * kB +
-                           g * (W::kV >= 4 ? 16 : W::kV * 4);
-        load_words(p, 128, vw[0]);
-        load_words(p + W::kRow, 128, vw[1]);
-        load_words(p + 8 * W::kRow, 128, vw[2]);
-        load_words(p + 9 * W::kRow, 128, vw[3]);
-    };
-    // the V^T fragments of dims' tiles: word w gives one (f16) or two (8-bit) tiles of 16 dims
-    auto v_frag = [&](int tile_i, uint32_t (&f)[4]) {
-        if constexpr (Q8) {
-            const int w = tile_i >> 1;
-            const uint32_t sel = tile_i & 1 ? 0x7362u : 0x5140u;
-            const uint32_t x = prmt(vw[0][w], vw[1][w], sel), y = prmt(vw[2][w], vw[3][w], sel);
-            f[0] = e4m3x2_to_f16x2(uint16_t(x)), f[1] = e4m3x2_to_f16x2(uint16_t(x >> 16));
-            f[2] = e4m3x2_to_f16x2(uint16_t(y)), f[3] = e4m3x2_to_f16x2(uint16_t(y >> 16));
-        } else {
-            f[0] = prmt(vw[0][tile_i], vw[1][tile_i], 0x5410u), f[1] = prmt(vw[0][tile_i], vw[1][tile_i], 0x7632u);
-            f[2] = prmt(vw[2][tile_i], vw[3][tile_i], 0x5410u), f[3] = prmt(vw[2][tile_i], vw[3][tile_i], 0x7632u);
-        }
-    };
-
-    float ks = 1.0f, vs = 1.0f;
-    auto load_scales = [&](int page) {
-        if constexpr (Q8) {
-            ks = c.k_scale[int64_t(page) * c.scale_stride + kvh];
-            vs = c.v_scale[int64_t(page) * c.scale_stride + kvh];
-        }
-    };
-    // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
-    // scores, V from the end of its P V.
-    int k = k_begin + warp;
-    int page = page_of(k), next_page = page_of(k + kWarps);
-    if (page >= 0) {
-        load_k(page, key_of(k));
-        load_scales(page);
-        load_v(page, key_of(k));
-    }
     for (; k < k_end; k += kWarps) {
         const int j0 = key_of(k), j1 = key_of(k + kWarps);
         const int after = page_of(k + 2 * kWarps);
@@ -254,7 +265,6 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
             page = next_page, next_page = after;
             if (page >= 0) {
                 load_k(page, j1);
-                load_scales(page);
                 load_v(page, j1);
             }
             continue;
@@ -276,59 +286,113 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
                 else mma16816(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
             }
         }
-        const float ks_now = ks, vs_now = vs;
+        const float ks_now = ks;
         page = next_page, next_page = after;
-        if (page >= 0) {
-            load_k(page, j1);
-            load_scales(page);
-        }
-        // ---- masks, running maximum, weights
-        // free of masks: every key of the group is seen by every row of the tile
+        if (page >= 0) load_k(page, j1);
+        // ---- scale, cap, bias, masks
+        // open: every key of the group is seen by every row of the tile
         const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= pos_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
-        uint32_t pf[NT][2];
-        float alpha[NT][TL::kLaneRows];
         uint32_t seen_bits = 0;  // per lane: (nt, row, key) -> seen
+        float z[NT][TL::kLaneRows][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int r = 0; r < TL::kLaneRows; r++) {
+                const float f = qscale[nt][r] * ks_now;
+#pragma unroll
+                for (int h = 0; h < 2; h++) z[nt][r][h] = (HILO ? sc[nt][2 * h] + sc[nt][2 * h + 1] : sc[nt][2 * h + r]) * f;
+            }
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) z[nt][r][h] = a.softcap * kLog2e * tanh_abs(z[nt][r][h] * inv_cap);
+        }
+        if (a.slopes) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) z[nt][r][h] = fmaf(slope[nt][r], float(j0 + g + 8 * h - qpos[nt][r]), z[nt][r][h]);
+        }
+        if (!open) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int j = j0 + g + 8 * h, at = qpos[nt][r];
+                        const bool see = (j < len && j <= at && (!a.window || at - j < a.window)) || (j < prefix && at != kNoRow);
+                        if (see) seen_bits |= 1u << (nt * 4 + r * 2 + h);
+                        else z[nt][r][h] = -INFINITY;
+                    }
+        }
+        // ---- running maximum (moved only by more than 2^8: weights up to that are as exact) and value scale
+        const float vs_now = vs;
+        bool up = false;
+        float top[NT][TL::kLaneRows];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int r = 0; r < TL::kLaneRows; r++) {
+                float x = fmaxf(z[nt][r][0], z[nt][r][1]);
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                top[nt][r] = x;
+                up |= x > m[nt][r] + 8.0f;
+            }
+        const bool v_up = Q8 && vs_now > 16.0f * vref;
+        if (__any_sync(0xffffffffu, up) || v_up) {
+            float fv = 1.0f;
+            if (v_up) {
+                fv = __fdividef(vref, vs_now);
+                vref = vs_now;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float f[TL::kLaneRows];
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++) {
+                    f[r] = 1.0f;
+                    if (top[nt][r] > m[nt][r] + 8.0f) {
+                        f[r] = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
+                        m[nt][r] = top[nt][r];
+                        l[nt][r] *= f[r];
+                    }
+                    f[r] *= fv;
+                }
+#pragma unroll
+                for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[nt][i][e] *= f[HILO ? 0 : e & 1];
+            }
+        }
+        // ---- weights as B fragments, in units of the reference scale
+        uint32_t pf[NT][2];
+        const float ratio = Q8 ? (vref > 0.0f ? __fdividef(vs_now, vref) : 0.0f) : 1.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float p[2][TL::kLaneRows];
 #pragma unroll
             for (int r = 0; r < TL::kLaneRows; r++) {
-                float z[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float dot = HILO ? sc[nt][2 * h] + sc[nt][2 * h + 1] : sc[nt][2 * h + r];
-                    const int j = j0 + g + 8 * h;
-                    float v = dot * (qscale[nt][r] * ks_now);
-                    if (a.softcap > 0.0f) v = a.softcap * tanh_abs(__fdividef(v, a.softcap));
-                    v = v * kLog2e;
-                    if (a.slopes) v += slope[nt][r] * float(j - qpos[nt][r]);
-                    bool see = true;
-                    if (!open) {
-                        see = (j < len && j <= qpos[nt][r] && (!a.window || qpos[nt][r] - j < a.window)) ||
-                              (j < prefix && qpos[nt][r] != kNoRow);
-                        if (see) seen_bits |= 1u << (nt * 4 + r * 2 + h);
-                    }
-                    z[h] = see ? v : -INFINITY;
-                }
-                float top = fmaxf(z[0], z[1]);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                const float m_new = fmaxf(m[nt][r], top);
-                const float ref = m_new == -INFINITY ? 0.0f : m_new;
-                alpha[nt][r] = ex2(m[nt][r] - ref);
-                m[nt][r] = m_new;
-                p[0][r] = ex2(z[0] - ref), p[1][r] = ex2(z[1] - ref);
-                l[nt][r] = l[nt][r] * alpha[nt][r] + (p[0][r] + p[1][r]);
+                const float ref = m[nt][r] == -INFINITY ? 0.0f : m[nt][r];
+                p[0][r] = ex2(z[nt][r][0] - ref), p[1][r] = ex2(z[nt][r][1] - ref);
+                l[nt][r] += p[0][r] + p[1][r];
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t hl;
                 if constexpr (HILO) {
-                    const __half hi1 = __float2half_rn(p[h][0]);
-                    hl = h2u(__halves2half2(hi1, __float2half_rn(p[h][0] - __half2float(hi1))));
+                    const float x = p[h][0] * ratio;
+                    const __half hi1 = __float2half_rn(x);
+                    hl = h2u(__halves2half2(hi1, __float2half_rn(x - __half2float(hi1))));
                 } else {
-                    hl = h2u(__floats2half2_rn(p[h][0], p[h][1]));
+                    hl = h2u(__floats2half2_rn(p[h][0] * ratio, p[h][1] * ratio));
                 }
                 pf[nt][h] = movmatrix(hl);
             }
@@ -345,35 +409,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
 #pragma unroll
                 for (int w = 0; w < W::kV; w++) {
                     if (dead) vw[x][w] = 0;
-                    if constexpr (Q8) {
-#pragma unroll
-                        for (int y = 0; y < 4; y++) odd |= ((vw[x][w] >> (8 * y)) & 0x7f) == 0x7f;
-                    } else {
-                        odd |= (vw[x][w] & 0x7c00u) == 0x7c00u || (vw[x][w] & 0x7c000000u) == 0x7c000000u;
-                    }
+                    odd |= odd_lanes<Q8>(vw[x][w]) != 0;
                 }
             }
             if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
                 for (int key = 0; key < 16; key++) {
                     // who sees this key: the lanes that hold its scores say so
                     const uint32_t bits = __shfl_sync(0xffffffffu, seen_bits, (key & 7) * 4 + t) >> (key >> 3);
+                    const int mine = (key >> 3) * 2 + (key & 1);
+                    const bool here = (key & 7) >> 1 == t;
                     uint32_t keep[4][W::kV];
 #pragma unroll
                     for (int x = 0; x < 4; x++)
 #pragma unroll
                         for (int w = 0; w < W::kV; w++) {
                             keep[x][w] = vw[x][w];
-                            uint32_t mask = 0;
-                            if (2 * t + (x & 1) + 8 * (x >> 1) == key) {
-                                if constexpr (Q8) {
-#pragma unroll
-                                    for (int y = 0; y < 4; y++)
-                                        if (((vw[x][w] >> (8 * y)) & 0x7f) == 0x7f) mask |= 0xffu << (8 * y);
-                                } else {
-                                    if ((vw[x][w] & 0x7c00u) == 0x7c00u) mask |= 0xffffu;
-                                    if ((vw[x][w] & 0x7c000000u) == 0x7c000000u) mask |= 0xffff0000u;
-                                }
-                            }
+                            const uint32_t mask = here && x == mine ? odd_lanes<Q8>(vw[x][w]) : 0u;
                             vw[x][w] &= mask;
                             keep[x][w] &= ~mask;
                         }
@@ -388,7 +440,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const int r = HILO ? 0 : e & 1;
-                                if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e] * vs_now;
+                                if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e];
                             }
                         }
                     }
@@ -404,13 +456,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
             uint32_t f[4];
             v_frag(i, f);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float d[4];
-                mma16816_z(d, f, pf[nt][0], pf[nt][1]);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    acc[nt][i][e] = acc[nt][i][e] * alpha[nt][HILO ? 0 : e & 1] + d[e] * vs_now;
-            }
+            for (int nt = 0; nt < NT; nt++) mma16816(acc[nt][i], f, pf[nt][0], pf[nt][1]);
         }
         if (page >= 0) load_v(page, j1);
     }
@@ -432,7 +478,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
             for (int i = 0; i < kSteps; i++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float v = HILO ? acc[nt][i][2 * h] + acc[nt][i][2 * h + 1] : acc[nt][i][2 * h + r];
+                    const float v = (HILO ? acc[nt][i][2 * h] + acc[nt][i][2 * h + 1] : acc[nt][i][2 * h + r]) * (Q8 ? vref : 1.0f);
                     const int d = Q8 ? (HD / 8) * g + 2 * i + h
                                      : (W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) + h : 4 * g + 2 * i + h);
                     st[2 + d] = v;
@@ -441,11 +487,11 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     }
     __syncthreads();
     // ---- joined over the warps
-    const bool alone = plan.ranks == 1;
+    const bool alone = ranks == 1;
     float* cta = sm + kWarps * TL::kState;
     auto put = [&](int row, int d, float v) {
-        const int pr = r0 + row;
-        const int64_t off = int64_t(row0 + pr / G) * a.o_token + int64_t(kvh * G + pr % G) * a.o_head + d;
+        const int pr = r0 + row, rt = over_g(pr);
+        const int64_t off = int64_t(row0 + rt) * a.o_token + int64_t(kvh * G + pr - rt * G) * a.o_head + d;
         if (a.type == kTF32) static_cast<float*>(a.out)[off] = v;
         else if (a.type == kTF16) static_cast<__half*>(a.out)[off] = __float2half_rn(v);
         else static_cast<__nv_bfloat16*>(a.out)[off] = __float2bfloat16_rn(v);
@@ -480,11 +526,11 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     // ---- joined over the cluster, each CTA a share of the outputs
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    const int share = (rows * HD + plan.ranks - 1) / plan.ranks;
+    const int share = (rows * HD + ranks - 1) >> plan.ranks_log;
     for (int x = rank * share + tid; x < min(rows * HD, (rank + 1) * share); x += 32 * kWarps) {
         const int row = x / HD, d = x % HD;
         float top, sum;
-        const float v = join(row, d, plan.ranks,
+        const float v = join(row, d, ranks,
                              [&](int w) { return cluster.map_shared_rank(cta, w) + row * (TL::kPitch + 2); }, top, sum);
         put(row, d, sum == 0.0f ? 0.0f : v / sum);
     }
@@ -495,28 +541,30 @@ template <int HD, bool Q8, bool HILO, int NT, int kWarps>
 cudaError_t go(const neko_paged_attention_args& a, int ranks, cudaStream_t st) {
     using TL = Tile<HD, Q8, HILO, NT, kWarps>;
     const neko_paged_cache& c = a.cache;
-    const int G = a.n_head / c.n_kv;
     DecodePlan p;
-    p.row_tiles = int((int64_t(a.max_new) * G + TL::kRows - 1) / TL::kRows);
-    const int64_t items = int64_t(c.n_seq) * c.n_kv * p.row_tiles;
-    p.ranks = ranks;
-    if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    p.group = a.n_head / c.n_kv;
+    p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
+    p.ranks_log = 31 - __builtin_clz(ranks);
+    p.page_16 = uint32_t(c.page_stride * (Q8 ? 1 : 2) / 16);
+    p.page_log = 31 - __builtin_clz(c.page_size);
+    const int64_t row_tiles = (int64_t(a.max_new) * p.group + TL::kRows - 1) / TL::kRows;
+    if (row_tiles > 65535 || c.n_kv > 65535 || int64_t(c.n_seq) * ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, kWarps>;
     cudaError_t e = ensure_dyn_smem(fn, TL::kSmem);
     if (e != cudaSuccess) return e;
-    if (p.ranks > 8 && (e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
+    if (ranks > 8 && (e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
         return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(items * p.ranks));
+    cfg.gridDim = dim3(unsigned(c.n_seq * ranks), unsigned(c.n_kv), unsigned(row_tiles));
     cfg.blockDim = dim3(32 * kWarps);
     cfg.dynamicSmemBytes = TL::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(p.ranks);
+    attr[0].val.clusterDim.x = unsigned(ranks);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.ranks > 1 ? 1 : 0;
+    cfg.numAttrs = ranks > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, fn, a, p);
 }
 

@@ -25,6 +25,7 @@ const char* bad_cache(const neko_paged_cache& c) {
     if (c.page_stride < int64_t(c.n_kv) * c.page_size * c.head_dim) return "pages overlap";
     if (!aligned(c.k_pages, 16) || !aligned(c.v_pages, 16) || (c.page_stride * (q8 ? 1 : 2)) % 16)
         return "pages must be 16-byte aligned";
+    if (c.page_stride * (q8 ? 1 : 2) / 16 > 0xffffffffll) return "page stride of 64 GB or more";
     if (c.table_stride < c.max_pages) return "table stride below max_pages";
     if (q8 && c.scale_stride < c.n_kv) return "scale stride below n_kv";
     if (int64_t(c.max_pages) * c.page_size > (int64_t(1) << 30)) return "more than 2^30 positions per sequence";

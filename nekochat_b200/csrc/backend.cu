@@ -57,6 +57,34 @@ int num_sms() {
     return cache[dev];
 }
 
+// Stream-ordered scratch for operators called outside a model comes from the library's own memory pool on the
+// current device: it keeps what it has grown to (release threshold at its maximum), so after the first calls an
+// allocation maps no memory, and the default pool's settings stay the caller's.
+cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st) {
+    static std::mutex mu;
+    static cudaMemPool_t pools[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaMallocAsync(p, bytes, st);
+    cudaMemPool_t pool;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!pools[dev]) {
+            cudaMemPoolProps props = {};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.handleTypes = cudaMemHandleTypeNone;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = dev;
+            if ((e = cudaMemPoolCreate(&pools[dev], &props)) != cudaSuccess) return e;
+            uint64_t keep = UINT64_MAX;
+            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
+        }
+        pool = pools[dev];
+    }
+    return cudaMallocFromPoolAsync(p, bytes, pool, st);
+}
+
 namespace {
 struct DynSmem {
     int limit = -1;  // opt-in per-block limit less the kernel's static shared memory
@@ -155,34 +183,6 @@ struct DeviceGuard {
         if (prev >= 0 && cur != prev) cudaSetDevice(prev);
     }
 };
-
-// Stream-ordered scratch for operators called outside a model comes from the library's own memory pool on the
-// current device: it keeps what it has grown to (release threshold at its maximum), so after the first calls an
-// allocation maps no memory, and the default pool's settings stay the caller's.
-cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st) {
-    static std::mutex mu;
-    static cudaMemPool_t pools[64] = {};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaMallocAsync(p, bytes, st);
-    cudaMemPool_t pool;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (!pools[dev]) {
-            cudaMemPoolProps props = {};
-            props.allocType = cudaMemAllocationTypePinned;
-            props.handleTypes = cudaMemHandleTypeNone;
-            props.location.type = cudaMemLocationTypeDevice;
-            props.location.id = dev;
-            if ((e = cudaMemPoolCreate(&pools[dev], &props)) != cudaSuccess) return e;
-            uint64_t keep = UINT64_MAX;
-            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
-        }
-        pool = pools[dev];
-    }
-    return cudaMallocFromPoolAsync(p, bytes, pool, st);
-}
 
 // A matmul outside a model: a stream-ordered workspace for the tensor-core path's K splits and activation split,
 // allocated and freed around the call (both stream-ordered, so the call can be captured in a graph). Without the

@@ -11,17 +11,16 @@
 // the f32 accumulator. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
 // 16-bit queries one exact f16 column, weights one f16. Rows are scaled by a power of two into f16's range first.
-// Each warp keeps its own running maximum and sum; warps meet in shared memory at the end, and the CTAs that share a
-// (sequence, KV head) form a thread-block cluster and meet over distributed shared memory, in rank order, so no
-// scratch memory is needed and results do not depend on timing.
-#include <cooperative_groups.h>
-
+// All groups of all items, in order, are dealt out in equal shares to the warps that the GPU holds at a time, whatever
+// the lengths; each CTA adds up the sequences' groups itself (the lengths are on the device only). A warp goes through
+// its share item by item, its start-up hidden behind the other warps of its SM: nothing waits for a CTA's other warps
+// until all are done, when the parts of an item meet in shared memory. What several CTAs share is joined from their parts
+// by a second small kernel, in order, so results do not depend on timing.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.cuh"
 #include "paged_math.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace neko {
 
@@ -72,64 +71,148 @@ __device__ __forceinline__ void load_words(const uint8_t* p, int step, uint32_t 
     }
 }
 
-// CTAs of 8 warps per SM, by the registers that a key group in flight takes.
-template <int kWarps, int HD, bool Q8, int NT>
-constexpr int kCtas = kWarps == 16 ? 1 : NT == 1 && (Q8 || HD <= 64) ? 2 : 1;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+// CTAs per SM, by the registers that a key group in flight takes.
+template <int HD, bool Q8, int NT>
+constexpr int kCtas = NT == 1 && (Q8 || HD <= 64) ? 2 : 1;
 
 struct DecodePlan {
-    int ranks_log;        // log2 of the CTAs per (sequence, KV head, row tile): the cluster
     int group;            // query heads per KV head
     uint64_t group_inv;   // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
     uint32_t page_16;     // page stride in 16-byte units
     int page_log;
+    float* part;          // [row tile][2 * CTAs][rows][HD + 4]: values, maximum, sum
+    int4* desc;           // [row tile][CTAs]: an item that starts in the CTA and ends in a later one
 };
 
 // Columns of an MMA: 8 rows (16-bit queries) or 4 (f32: hi and lo columns).
-template <int HD, bool Q8, bool HILO, int NT, int kWarps>
+template <int HD, bool HILO, int NT>
 struct Tile {
     static constexpr int kRowsPer = HILO ? 4 : 8;
     static constexpr int kRows = NT * kRowsPer;
     static constexpr int kLaneRows = HILO ? 1 : 2;  // rows per lane and column tile
-    static constexpr int kPitch = HD + 4;
-    // dynamic shared memory (floats): per warp and row maximum, sum, accumulator; then the CTA's
-    static constexpr int kState = kRows * (kPitch + 2);
-    static constexpr size_t kSmem = size_t(kWarps + 1) * kState * 4;
+    static constexpr int kPitch = HD + 4;           // floats of a row's state: values, maximum, sum
+    static constexpr int kState = kRows * kPitch;
+    // dynamic shared memory: the warps' two states, what they are, warp totals, groups before each sequence
+    static constexpr int kMetaOff = 2 * kWarps * kState * 4;
+    static constexpr int kScanOff = kMetaOff + 2 * kWarps * 16;
+    static constexpr int kPreOff = kScanOff + 16 * 4;
+    static size_t smem(int n_seq) { return kPreOff + size_t(n_seq + 1) * 4; }
 };
 
-template <int HD, bool Q8, bool HILO, int NT, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_decode_kernel(
-    const neko_paged_attention_args a, const DecodePlan plan) {
-    using TL = Tile<HD, Q8, HILO, NT, kWarps>;
+// What a row tile of a sequence sees, the same for all its KV heads.
+struct Span {
+    int row0, n, held, len, prefix, rows, pos_lo, pos_hi, hi, lo, g_lo, g_pre, ng;
+};
+template <int kRows>
+__device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, const DecodePlan& plan, int s, int tile) {
+    Span v;
+    v.row0 = a.q_start ? a.q_start[s] : s;
+    v.n = a.q_start ? a.q_start[s + 1] - v.row0 : 1;
+    v.held = max(a.kv_len[s], 0);
+    v.len = min(v.held, a.cache.max_pages << plan.page_log);
+    v.prefix = a.prefix ? min(max(a.prefix[s], 0), v.len) : 0;
+    if (v.row0 < 0 || v.n < 0 || v.n > a.max_new || v.row0 + v.n > a.tokens) {
+        set_device_error(kErrBadIndex);
+        v.n = 0;
+    }
+    auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
+    const int r0 = tile * kRows;
+    v.rows = max(min(v.n * plan.group - r0, kRows), 0);
+    v.pos_lo = v.held - v.n + over_g(r0), v.pos_hi = v.held - v.n + over_g(r0 + max(v.rows, 1) - 1);
+    // keys some row of the tile sees: [0, pre) and [lo, hi), as groups of 16
+    v.hi = max(min(v.len, v.pos_hi + 1), 0);
+    v.lo = a.window ? min(max(v.pos_lo - a.window + 1, 0), v.hi) : 0;
+    const int g_hi = (max(v.hi, v.prefix > v.lo ? v.prefix : 0) + 15) / 16;
+    v.g_lo = v.lo / 16;
+    v.g_pre = min((v.prefix + 15) / 16, v.g_lo);  // prefix groups before g_lo
+    // rows that see nothing still get a group, without a page, so that some CTA writes their zeros
+    v.ng = v.rows > 0 ? max(v.g_pre + max(g_hi - v.g_lo, 0), 1) : 0;
+    return v;
+}
+
+// v / sum to four values of a packed row of the output.
+template <bool HILO>
+__device__ __forceinline__ void put_row(const neko_paged_attention_args& a, const DecodePlan& plan, int row0, int kvh, int pr, int d,
+                                        float4 v, float sum) {
+    const int rt = int(uint64_t(uint32_t(pr)) * plan.group_inv >> 32);
+    const int64_t off = int64_t(row0 + rt) * a.o_token + int64_t(kvh * plan.group + pr - rt * plan.group) * a.o_head + d;
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    auto store = [&](auto* p) { store_row<4>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0, x); };
+    if constexpr (HILO) store(static_cast<float*>(a.out) + off);
+    else if (a.type == kTF16) store(static_cast<__half*>(a.out) + off);
+    else store(static_cast<__nv_bfloat16*>(a.out) + off);
+}
+
+template <int HD, bool Q8, bool HILO, int NT>
+__global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kernel(const neko_paged_attention_args a,
+                                                                                const DecodePlan plan) {
+    using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
-    const int ranks = 1 << plan.ranks_log;
-    const int rank = blockIdx.x & (ranks - 1), s = blockIdx.x >> plan.ranks_log, kvh = blockIdx.y, tile = blockIdx.z;
-    const int G = plan.group;
+    const int tile = blockIdx.y, G = plan.group, n_kv = c.n_kv;
+    uint8_t* smb = reinterpret_cast<uint8_t*>(sm);
+    int4* meta = reinterpret_cast<int4*>(smb + TL::kMetaOff);  // item, 1 starts | 2 ends, row0, rows; item -1: none
+    int* totals = reinterpret_cast<int*>(smb + TL::kScanOff);
+    int* pre = reinterpret_cast<int*>(smb + TL::kPreOff);
     auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
 
-    // the sequence: everything below is the same for all CTAs of the cluster
-    const int row0 = a.q_start ? a.q_start[s] : s;
-    const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
-    const int held = max(a.kv_len[s], 0), len = min(held, c.max_pages << plan.page_log);
-    const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
-    if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {
-        if (tid == 0) set_device_error(kErrBadIndex);
-        return;
+    // ---- groups of 16 keys before each sequence
+    int carry = 0;
+    for (int base = 0; base < c.n_seq; base += kThreads) {
+        const int s = base + tid;
+        int x = s < c.n_seq ? span_of<TL::kRows>(a, plan, s, tile).ng : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) totals[warp] = x;
+        __syncthreads();
+        int before = carry;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < warp) before += totals[w];
+            carry += totals[w];
+        }
+        if (s < c.n_seq) pre[s + 1] = before + x;
+        __syncthreads();
     }
-    const int r0 = tile * TL::kRows;  // first packed row of this tile
-    const int rows = min(n * G - r0, TL::kRows);
-    if (rows <= 0) return;
-    const int pos_lo = held - n + over_g(r0), pos_hi = held - n + over_g(r0 + rows - 1);
-    // keys some row of the tile sees: [0, pre) and [lo, hi), as groups of 16
-    const int hi = max(min(len, pos_hi + 1), 0);
-    const int lo = a.window ? min(max(pos_lo - a.window + 1, 0), hi) : 0;
-    const int g_lo = lo / 16, g_hi = (max(hi, prefix > lo ? prefix : 0) + 15) / 16;
-    const int g_pre = min((prefix + 15) / 16, g_lo);  // prefix groups before g_lo
-    const int ng = g_pre + max(g_hi - g_lo, 0);
-    const int k_begin = int(int64_t(ng) * rank >> plan.ranks_log), k_end = int(int64_t(ng) * (rank + 1) >> plan.ranks_log);
+    if (tid == 0) pre[0] = 0;
+    __syncthreads();
+    // ---- this warp's equal share of all (sequence, KV head) items' groups, in order
+    const int64_t total = int64_t(carry) * n_kv;
+    const int64_t warps = max(min(int64_t(gridDim.x) * kWarps, total), int64_t(1));
+    const int cta = blockIdx.x, gw = cta * kWarps + warp;
+    int64_t x = gw < warps ? total * gw / warps : 0;
+    const int64_t x_end = gw < warps ? total * (gw + 1) / warps : 0;
+    if (lane < 2) meta[2 * warp + lane].x = -1;
+    __syncwarp();
+    int s = 0, kvh = 0, cnt = 1;
+    if (x < x_end) {
+        int a0 = 0, a1 = c.n_seq;  // pre[a0] * n_kv <= x < pre[a1] * n_kv
+        while (a1 - a0 > 1) {
+            const int mid = (a0 + a1) >> 1;
+            if (int64_t(pre[mid]) * n_kv <= x) a0 = mid;
+            else a1 = mid;
+        }
+        s = a0;
+        cnt = pre[s + 1] - pre[s];
+        kvh = int(uint32_t(x - int64_t(pre[s]) * n_kv) / uint32_t(cnt));
+    }
+    int starts_last = -1;  // the CTA where the item that starts in this warp and does not end in it does
+#pragma unroll 1
+    while (x < x_end) {
+    const int64_t item = int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
+    const int k_begin = int(x - item), k_end = int(min(int64_t(cnt), x_end - item));
+    const Span sp = span_of<TL::kRows>(a, plan, s, tile);
+    const int row0 = sp.row0, n = sp.n, held = sp.held, len = sp.len, prefix = sp.prefix, rows = sp.rows;
+    const int pos_lo = sp.pos_lo, pos_hi = sp.pos_hi, hi = sp.hi, lo = sp.lo, g_lo = sp.g_lo, g_pre = sp.g_pre;
+    const int r0 = tile * TL::kRows;
 
     // ---- keys and values: fragments straight from the pages
     const int32_t* table = c.table + int64_t(s) * c.table_stride;
@@ -179,14 +262,14 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     };
     // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
     // scores, V from the end of its P V. The first group's fly while the queries are read.
-    int k = k_begin + warp;
-    int page = page_of(k), next_page = page_of(k + kWarps);
+    int k = k_begin;
+    int page = page_of(k), next_page = page_of(k + 1);
     if (page >= 0) {
         load_k(page, key_of(k));
         load_v(page, key_of(k));
     }
 
-    // ---- queries as B fragments
+    // ---- queries as B fragments: for each step of 16 dims this lane's four of column g
     uint32_t qf[NT][kSteps][2];
     float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two (* log2 e without a cap)
     int qpos[NT][TL::kLaneRows];
@@ -194,24 +277,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     const float unit = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = r0 + nt * TL::kRowsPer + (HILO ? g >> 1 : g);
-        float x[kSteps][4];
+        const int r = nt * TL::kRowsPer + (HILO ? g >> 1 : g);
+        float q[kSteps][4];
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = 0.0f;
-        if (r < n * G) {
-            const int rt = over_g(r);
-            const int64_t off = int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + r - rt * G) * a.q_head;
+            for (int e = 0; e < 4; e++) q[i][e] = 0.0f;
+        if (r < rows) {
+            const int rt = over_g(r0 + r);
+            const int64_t off = int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + r0 + r - rt * G) * a.q_head;
             auto fetch = [&](auto* p) {
                 const bool vec = (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0;
 #pragma unroll
                 for (int i = 0; i < kSteps; i++) {
-                    // the four dims of step i: one word of an 8-bit row, two words of an f16 row
-                    const int d = Q8 ? (W::kK >= 4 ? 64 * (i / 4) + 16 * t + 4 * (i % 4) : 8 * t + 4 * i)
-                                     : 32 * (i / 2) + 8 * t + 4 * (i % 2);
-                    load_row<4>(p + d, vec, x[i]);
+                    // one word of an 8-bit row, two words of an f16 row
+                    const int d = Q8 ? (W::kK >= 4 ? 64 * (i / 4) + 16 * t + 4 * (i % 4) : 8 * t + 4 * i) : 32 * (i / 2) + 8 * t + 4 * (i % 2);
+                    load_row<4>(p + d, vec, q[i]);
                 }
             };
             if constexpr (HILO) fetch(static_cast<const float*>(a.q) + off);
@@ -220,7 +302,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
 #pragma unroll
             for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) most = fmaxf(most, finite_abs(x[i][e]));
+                for (int e = 0; e < 4; e++) most = fmaxf(most, finite_abs(q[i][e]));
         }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -229,18 +311,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
         for (int i = 0; i < kSteps; i++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                uint32_t hi2, lo2;
-                split_hilo(x[i][2 * h] * up, x[i][2 * h + 1] * up, hi2, lo2);
+                uint32_t hi2 = h2u(__floats2half2_rn(q[i][2 * h] * up, q[i][2 * h + 1] * up)), lo2 = 0;
+                if constexpr (HILO) split_hilo(q[i][2 * h] * up, q[i][2 * h + 1] * up, hi2, lo2);
                 qf[nt][i][h] = HILO && (g & 1) ? lo2 : hi2;
             }
         const float down = unit / up;
 #pragma unroll
-        for (int x2 = 0; x2 < TL::kLaneRows; x2++) {
-            const int rr = HILO ? t : 2 * t + x2;  // this lane's score row within the column tile
-            qscale[nt][x2] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
-            const int pr = r0 + nt * TL::kRowsPer + rr, rt = over_g(pr);
-            qpos[nt][x2] = pr < n * G ? held - n + rt : kNoRow;
-            slope[nt][x2] = a.slopes && pr < n * G ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
+        for (int y = 0; y < TL::kLaneRows; y++) {
+            const int rr = HILO ? t : 2 * t + y, r2 = nt * TL::kRowsPer + rr, rt = over_g(r0 + r2);
+            qscale[nt][y] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
+            qpos[nt][y] = r2 < rows ? held - n + rt : kNoRow;
+            slope[nt][y] = a.slopes && r2 < rows ? a.slopes[kvh * G + r0 + r2 - rt * G] * kLog2e : 0.0f;
         }
     }
 
@@ -258,9 +339,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
     }
     const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
-    for (; k < k_end; k += kWarps) {
-        const int j0 = key_of(k), j1 = key_of(k + kWarps);
-        const int after = page_of(k + 2 * kWarps);
+#pragma unroll 1
+    for (; k < k_end; k++) {
+        const int j0 = key_of(k), j1 = key_of(k + 1);
+        const int after = page_of(k + 2);
         if (page < 0) {
             page = next_page, next_page = after;
             if (page >= 0) {
@@ -461,8 +543,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
         if (page >= 0) load_v(page, j1);
     }
 
-    // ---- the warps' states to shared memory: [row](max, sum, values)
-    float* mine = sm + warp * TL::kState;
+    // ---- an item of this warp's own to the output, a part of one to shared memory
+    const bool first = k_begin == 0, ends = k_end == cnt;
+    float* st0 = sm + (2 * warp + first) * TL::kState;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -472,122 +555,169 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<kWarps, HD, Q8, NT>) paged_
             sum += __shfl_xor_sync(0xffffffffu, sum, 8);
             sum += __shfl_xor_sync(0xffffffffu, sum, 16);
             const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
-            float* st = mine + row * (TL::kPitch + 2);
-            if (g == 0) st[0] = m[nt][r], st[1] = sum;
+            float* st = st0 + row * TL::kPitch;
+            if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum;
 #pragma unroll
-            for (int i = 0; i < kSteps; i++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float v = (HILO ? acc[nt][i][2 * h] + acc[nt][i][2 * h + 1] : acc[nt][i][2 * h + r]) * (Q8 ? vref : 1.0f);
-                    const int d = Q8 ? (HD / 8) * g + 2 * i + h
-                                     : (W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) + h : 4 * g + 2 * i + h);
-                    st[2 + d] = v;
-                }
+            for (int i = 0; i < kSteps; i++) {
+                float2 v;
+                v.x = HILO ? acc[nt][i][0] + acc[nt][i][1] : acc[nt][i][r];
+                v.y = HILO ? acc[nt][i][2] + acc[nt][i][3] : acc[nt][i][2 + r];
+                if (Q8) v.x *= vref, v.y *= vref;
+                const int d = Q8 ? (HD / 8) * g + 2 * i : W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : 4 * g + 2 * i;
+                *reinterpret_cast<float2*>(st + d) = v;
+            }
         }
+    }
+    __syncwarp();
+    if (first && ends) {
+        for (int y = lane; y < rows * (HD / 4); y += 32) {
+            const int row = y / (HD / 4), d = y % (HD / 4) * 4;
+            const float* st = st0 + row * TL::kPitch;
+            put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d), st[HD + 1]);
+        }
+        __syncwarp();
+    } else if (lane == 0) {
+        meta[2 * warp + first] = make_int4(s * n_kv + kvh, (first ? 1 : 0) | (ends ? 2 : 0), row0, rows);
+    }
+    if (first && !ends) starts_last = int((((item + cnt) * warps - 1) / total) / kWarps);
+    x = item + k_end;
+    if (x < x_end && ++kvh == n_kv) {
+        kvh = 0;
+        do s++;
+        while (pre[s + 1] == pre[s]);
+        cnt = pre[s + 1] - pre[s];
+    }
     }
     __syncthreads();
-    // ---- joined over the warps
-    const bool alone = ranks == 1;
-    float* cta = sm + kWarps * TL::kState;
-    auto put = [&](int row, int d, float v) {
-        const int pr = r0 + row, rt = over_g(pr);
-        const int64_t off = int64_t(row0 + rt) * a.o_token + int64_t(kvh * G + pr - rt * G) * a.o_head + d;
-        if (a.type == kTF32) static_cast<float*>(a.out)[off] = v;
-        else if (a.type == kTF16) static_cast<__half*>(a.out)[off] = __float2half_rn(v);
-        else static_cast<__nv_bfloat16*>(a.out)[off] = __float2bfloat16_rn(v);
-    };
-    auto join = [&](int row, int d, int count, auto state, float& top, float& sum) {
-        top = -INFINITY;
-        for (int w = 0; w < count; w++) top = fmaxf(top, state(w)[0]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        sum = 0.0f;
-        float v = 0.0f;
-        for (int w = 0; w < count; w++) {
-            const float* st = state(w);
-            const float f = ex2(st[0] - ref);
-            sum += f * st[1];
-            v += f * st[2 + d];
+    // ---- parts of the same item joined over the warps: to the output, or as one of this CTA's (at most two) parts
+    if (starts_last > cta && lane == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(s, kvh, starts_last, meta[2 * warp + 1].z);
+    bool open_item = false;
+    for (int b = 0; b < 2 * kWarps;) {
+        const int4 mb = meta[b];
+        int e = b + 1;
+        if (mb.x < 0) {
+            b = e;
+            continue;
         }
-        return v;
-    };
-    for (int x = tid; x < rows * HD; x += 32 * kWarps) {
-        const int row = x / HD, d = x % HD;
-        float top, sum;
-        const float v = join(row, d, kWarps, [&](int w) { return sm + w * TL::kState + row * (TL::kPitch + 2); }, top, sum);
-        if (alone) {
-            put(row, d, sum == 0.0f ? 0.0f : v / sum);
-        } else {
-            float* st = cta + row * (TL::kPitch + 2);
-            if (d == 0) st[0] = top, st[1] = sum;
-            st[2 + d] = v;
+        int flags = mb.y;
+        while (e < 2 * kWarps && (meta[e].x == mb.x || meta[e].x < 0)) {
+            if (meta[e].x >= 0) flags |= meta[e].y;
+            e++;
         }
+        const int row0 = mb.z, rows = mb.w, kvh2 = mb.x % n_kv;
+        float* part = plan.part + ((int64_t(tile) * gridDim.x + cta) * 2 + (flags & 1)) * TL::kState;
+        open_item |= (flags & 3) == 1;
+        for (int y = tid; y < rows * (HD / 4); y += kThreads) {
+            const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
+            float top = -INFINITY, sum = 0.0f;
+            for (int i = b; i < e; i++)
+                if (meta[i].x >= 0) top = fmaxf(top, sm[i * TL::kState + at + HD]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float4 v = make_float4(0, 0, 0, 0);
+            for (int i = b; i < e; i++) {
+                if (meta[i].x < 0) continue;
+                const float* st = sm + i * TL::kState + at;
+                const float f = ex2(st[HD] - ref);
+                const float4 o = *reinterpret_cast<const float4*>(st + d);
+                sum = fmaf(f, st[HD + 1], sum);
+                v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
+            }
+            if (flags == 3) {
+                put_row<HILO>(a, plan, row0, kvh2, tile * TL::kRows + row, d, v, sum);
+            } else {
+                *reinterpret_cast<float4*>(part + at + d) = v;
+                if (d == 0) part[at + HD] = top, part[at + HD + 1] = sum;
+            }
+        }
+        b = e;
     }
-    if (alone) return;
-    // ---- joined over the cluster, each CTA a share of the outputs
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int share = (rows * HD + ranks - 1) >> plan.ranks_log;
-    for (int x = rank * share + tid; x < min(rows * HD, (rank + 1) * share); x += 32 * kWarps) {
-        const int row = x / HD, d = x % HD;
-        float top, sum;
-        const float v = join(row, d, ranks,
-                             [&](int w) { return cluster.map_shared_rank(cta, w) + row * (TL::kPitch + 2); }, top, sum);
-        put(row, d, sum == 0.0f ? 0.0f : v / sum);
-    }
-    cluster.sync();  // no CTA leaves while another reads its state
+    if (!open_item && tid == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(-1, 0, 0, 0);
+    pdl_trigger();
 }
 
-template <int HD, bool Q8, bool HILO, int NT, int kWarps>
-cudaError_t go(const neko_paged_attention_args& a, int ranks, cudaStream_t st) {
-    using TL = Tile<HD, Q8, HILO, NT, kWarps>;
+// Joins the parts of the items that several CTAs share, in their order: block x the item that starts in the decode
+// kernel's CTA x.
+template <int HD, bool HILO, int NT>
+__global__ void __launch_bounds__(128) paged_join_kernel(const neko_paged_attention_args a, const DecodePlan plan, int ctas) {
+    using TL = Tile<HD, HILO, NT>;
+    pdl_wait();
+    const int tile = blockIdx.y, cta = blockIdx.x;
+    const int4 d4 = plan.desc[int64_t(tile) * ctas + cta];
+    if (d4.x < 0) return;
+    const int s = d4.x, kvh = d4.y, last = d4.z, row0 = d4.w;
+    const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
+    const int rows = min(n * plan.group - tile * TL::kRows, TL::kRows);
+    const float* base = plan.part + (int64_t(tile) * ctas + cta) * 2 * TL::kState;
+    // part 0 is the CTA's second slot, the others the first slots of the CTAs after it
+    auto part = [&](int i) { return base + (i == 0 ? 1 : 2 * i) * int64_t(TL::kState); };
+    const int parts = last - cta + 1;
+    for (int y = threadIdx.x; y < rows * (HD / 4); y += 128) {
+        const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
+        float top = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0, 0, 0, 0);
+        for (int i0 = 0; i0 < parts; i0 += 8) {  // eight parts' loads in flight
+            float mw[8], lw[8];
+            float4 o[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool in = i0 + i < parts;
+                const float* p = part(in ? i0 + i : 0) + at;
+                mw[i] = in ? p[HD] : -INFINITY, lw[i] = in ? p[HD + 1] : 0.0f;
+                o[i] = in ? *reinterpret_cast<const float4*>(p + d) : make_float4(0, 0, 0, 0);
+            }
+            float now = top;
+#pragma unroll
+            for (int i = 0; i < 8; i++) now = fmaxf(now, mw[i]);
+            const float ref = now == -INFINITY ? 0.0f : now, old = ex2(top - ref);
+            top = now;
+            sum *= old, v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float f = ex2(mw[i] - ref);
+                sum = fmaf(f, lw[i], sum);
+                v.x = fmaf(f, o[i].x, v.x), v.y = fmaf(f, o[i].y, v.y), v.z = fmaf(f, o[i].z, v.z), v.w = fmaf(f, o[i].w, v.w);
+            }
+        }
+        put_row<HILO>(a, plan, row0, kvh, tile * TL::kRows + row, d, v, sum);
+    }
+}
+
+template <int HD, bool Q8, bool HILO, int NT>
+cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
+    using TL = Tile<HD, HILO, NT>;
     const neko_paged_cache& c = a.cache;
     DecodePlan p;
     p.group = a.n_head / c.n_kv;
     p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
-    p.ranks_log = 31 - __builtin_clz(ranks);
     p.page_16 = uint32_t(c.page_stride * (Q8 ? 1 : 2) / 16);
     p.page_log = 31 - __builtin_clz(c.page_size);
     const int64_t row_tiles = (int64_t(a.max_new) * p.group + TL::kRows - 1) / TL::kRows;
-    if (row_tiles > 65535 || c.n_kv > 65535 || int64_t(c.n_seq) * ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, kWarps>;
-    cudaError_t e = ensure_dyn_smem(fn, TL::kSmem);
+    if (row_tiles > 65535) return cudaErrorInvalidConfiguration;
+    // as many CTAs as the GPU holds at a time, or a group of 16 keys for each warp where the cache has room for fewer
+    const int64_t groups = int64_t(c.max_pages) * c.page_size / 16 * c.n_kv * c.n_seq;
+    const int64_t items = int64_t(c.n_kv) * c.n_seq;
+    const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(num_sms()) * kCtas<HD, Q8, NT>, std::max(groups, items) / kWarps)));
+    const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
+    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT>;
+    const size_t smem = TL::smem(c.n_seq);
+    cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;
-    if (ranks > 8 && (e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
-        return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(c.n_seq * ranks), unsigned(c.n_kv), unsigned(row_tiles));
-    cfg.blockDim = dim3(32 * kWarps);
-    cfg.dynamicSmemBytes = TL::kSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(ranks);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = ranks > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, fn, a, p);
-}
-
-// CTAs that share a (sequence, KV head, row tile): enough for two CTAs of 8 warps on every SM, as long as each warp
-// keeps two groups of 16 keys. Where 16 of them do not fill the GPU, CTAs of 16 warps.
-template <int HD, bool Q8, bool HILO, int NT>
-cudaError_t by_work(const neko_paged_attention_args& a, cudaStream_t st) {
-    const neko_paged_cache& c = a.cache;
-    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv), kRows = Tile<HD, Q8, HILO, NT, 8>::kRows;
-    const int64_t items = int64_t(c.n_seq) * c.n_kv * ((rows + kRows - 1) / kRows);
-    const int64_t groups = int64_t(c.max_pages) * c.page_size / 16;
-    int ranks = 1;
-    while (ranks < 16 && items * ranks < 2 * num_sms() && groups > 16 * ranks) ranks *= 2;
-    if (NT == 1 && ranks == 16 && items * 16 <= num_sms() && groups > 32 * ranks)
-        return go<HD, Q8, HILO, NT, NT == 1 ? 16 : 8>(a, ranks, st);
-    return go<HD, Q8, HILO, NT, 8>(a, ranks, st);
+    void* mem = nullptr;
+    if ((e = scratch_alloc(&mem, part_bytes + desc_bytes, st)) != cudaSuccess) return e;
+    p.part = static_cast<float*>(mem);
+    p.desc = reinterpret_cast<int4*>(static_cast<char*>(mem) + part_bytes);
+    e = launch_ex(fn, dim3(unsigned(ctas), unsigned(row_tiles)), dim3(kThreads), smem, st, false, a, p);
+    if (e == cudaSuccess)
+        e = launch_ex(paged_join_kernel<HD, HILO, NT>, dim3(unsigned(ctas), unsigned(row_tiles)), dim3(128), 0, st, true, a, p, ctas);
+    cudaFreeAsync(mem, st);
+    return e;
 }
 
 template <int HD, bool Q8>
 cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t rows = int64_t(a.max_new) * (a.n_head / a.cache.n_kv);
-    if (a.type == NEKO_T_F32) return rows <= 4 ? by_work<HD, Q8, true, 1>(a, st) : by_work<HD, Q8, true, 2>(a, st);
-    return rows <= 8 ? by_work<HD, Q8, false, 1>(a, st) : by_work<HD, Q8, false, 2>(a, st);
+    if (a.type == NEKO_T_F32) return rows <= 4 ? go<HD, Q8, true, 1>(a, st) : go<HD, Q8, true, 2>(a, st);
+    return rows <= 8 ? go<HD, Q8, false, 1>(a, st) : go<HD, Q8, false, 2>(a, st);
 }
 
 }  // namespace

@@ -43,6 +43,9 @@ inline int max_dyn_smem(F* fn) { return max_dyn_smem(reinterpret_cast<const void
 template <typename F>
 inline cudaError_t ensure_dyn_smem(F* fn, size_t bytes) { return ensure_dyn_smem(reinterpret_cast<const void*>(fn), bytes); }
 
+// Stream-ordered scratch from the library's own pool of the current device (backend.cu); freed with cudaFreeAsync.
+cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st);
+
 // ------------------------------------------------------------------ weight codec (k_quant.cu)
 cudaError_t launch_quantize(int fmt, const float* w, int rows, int cols, int64_t ld, int transpose, uint8_t* out,
                             cudaStream_t st);

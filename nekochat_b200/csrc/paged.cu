@@ -72,6 +72,7 @@ extern "C" int neko_op_paged_attention(const neko_paged_attention_args* a, void*
     if (!a->q || !a->out || !a->kv_len) return paged_fail(NEKO_ERR_ARG, op, "null pointer");
     if (!a->q_start && a->tokens != a->cache.n_seq)
         return paged_fail(NEKO_ERR_ARG, op, "without q_start there is one token per sequence");
+    if (a->cache.n_seq > 16384) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 16384 sequences");
     if (a->window < 0 || !(a->softcap >= 0.0f) || !(a->scale == a->scale))
         return paged_fail(NEKO_ERR_ARG, op, "window and softcap are not negative");
     return finish(op, launch_paged_attention(*a, static_cast<cudaStream_t>(stream)));

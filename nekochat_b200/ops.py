@@ -149,77 +149,67 @@ _ATTEND = struct.Struct("@" + _CACHE + "2P4q4P5i2fi")
 _types = {}
 
 
-def _type(t, what):
-    """neko_type of a tensor's dtype (uint8 and float8_e4m3fn both hold E4M3 codes)."""
-    if not _types:
-        import torch
-        _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.uint8: 3})
-    try:
-        return _types[t.dtype]
-    except KeyError:
-        raise NekoError(f"{what}: {t.dtype} is not supported") from None
+def _setup():
+    """neko_type of each dtype (uint8 and float8_e4m3fn both hold E4M3 codes) and the entries, on first use."""
+    import torch
+    l = lib()
+    _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.uint8: 3,
+                   "f32": torch.float32, "i32": torch.int32, "append": l.neko_op_paged_append,
+                   "attend": l.neko_op_paged_attention, "device": torch.cuda.current_device,
+                   "stream": getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+                   (lambda i: torch.cuda.current_stream(i).cuda_stream)})
+    return _types
 
 
-def _rows(t, what, type_, n, hd, dev):
+def _rows(t, what, dtype, shape, dev):
     """(pointer, token stride, head stride) of [tokens][heads][hd] rows."""
-    sh, st = t.shape, t.stride()
-    if len(sh) != 3 or sh[2] != hd or sh[0] != n or (st[2] != 1 and hd > 1) or t.device != dev or _type(t, what) != type_:
-        raise NekoError(f"{what}: [tokens][heads][head_dim] rows on the cache's device, values contiguous, one type")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        raise NekoError(f"{what}: {dtype} {list(shape)} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    st = t.stride()
+    if st[2] != 1:
+        raise NekoError(f"{what}: the last dimension is contiguous")
     return t.data_ptr(), st[0], st[1]
 
 
-def _ints(t, what, n, dev):
+def _vector(t, what, dtype, n, dev):
+    """Pointer of n contiguous numbers, NULL for None."""
     if t is None:
         return 0
-    if t.dtype.itemsize != 4 or t.dtype.is_floating_point or t.dim() != 1 or t.shape[0] != n or t.device != dev or \
-            (n > 1 and t.stride(0) != 1):
-        raise NekoError(f"{what}: {n} contiguous int32 on the cache's device")
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise NekoError(f"{what}: {n} contiguous {dtype} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _floats(t, what, n, dev):
-    if t is None:
-        return 0
-    if str(t.dtype) != "torch.float32" or t.numel() != n or t.device != dev or not t.is_contiguous():
-        raise NekoError(f"{what}: {n} contiguous float32 on the cache's device")
-    return t.data_ptr()
-
-
-def _cache(k_pages, v_pages, k_scale, v_scale, table):
-    """The fields of neko_paged_cache, (n_seq, n_kv, head dim, device)."""
-    dev, sh, st = k_pages.device, k_pages.shape, k_pages.stride()
-    if dev.type != "cuda" or len(sh) != 4 or v_pages.shape != sh or v_pages.stride() != st or v_pages.device != dev or \
-            v_pages.dtype != k_pages.dtype:
-        raise NekoError("paged cache: k_pages and v_pages are alike [pages][kv heads][page][head_dim] CUDA tensors")
+def _cache(k_pages, v_pages, k_scale, v_scale, table, types):
+    """The fields of neko_paged_cache, then n_seq, n_kv, head dim and device index."""
+    dev, sh, st, dt = k_pages.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype
+    if dev < 0 or len(sh) != 4 or v_pages.shape != sh or v_pages.stride() != st or v_pages.get_device() != dev or \
+            v_pages.dtype is not dt or dt not in types:
+        raise NekoError("paged cache: k_pages and v_pages are alike [pages][kv heads][page][head_dim] CUDA tensors "
+                        "(float16, float8_e4m3fn or uint8)")
     pages, n_kv, ps, hd = sh
     if st[3] != 1 or st[2] != hd or (st[1] != ps * hd and n_kv > 1):
         raise NekoError("paged cache: a page is contiguous")
-    type_ = _type(k_pages, "paged cache")
+    type_ = types[dt]
     ks = vs = sst = 0
     if type_ == 3:
         if k_scale is None or v_scale is None:
             raise NekoError("paged cache: 8-bit pages need k_scale and v_scale")
-        sst = k_scale.stride(0)
+        sst = k_scale.stride()[0]
         for t in (k_scale, v_scale):
-            if t.shape != (pages, n_kv) or str(t.dtype) != "torch.float32" or t.device != dev or t.stride(0) != sst or \
-                    (n_kv > 1 and t.stride(1) != 1):
+            s2 = t.stride()
+            if t.shape != (pages, n_kv) or t.dtype is not types["f32"] or t.get_device() != dev or s2[0] != sst or \
+                    (n_kv > 1 and s2[1] != 1):
                 raise NekoError("paged cache: scales are alike [pages][kv heads] float32")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-    if table.dim() != 2 or table.dtype.itemsize != 4 or table.dtype.is_floating_point or table.device != dev or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
+    tsh, tst = table.shape, table.stride()
+    if len(tsh) != 2 or table.dtype is not types["i32"] or table.get_device() != dev or (tsh[1] > 1 and tst[1] != 1):
         raise NekoError("paged cache: the table is [sequences][pages] int32")
-    n_seq, width = table.shape
-    page_stride = st[0] if pages > 1 else n_kv * ps * hd
-    return (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), page_stride, sst,
-            table.stride(0) if n_seq > 1 else width, type_, n_seq, width, pages, n_kv, ps, hd, 0), n_seq, n_kv, hd, dev
-
-
-def _on(dev):
-    """The current stream of the tensors' device, which has to be the current one."""
-    import torch
-    if torch.cuda.current_device() != dev.index:
-        raise NekoError(f"paged cache: the tensors are on {dev}, the current device is {torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
+    n_seq, width = tsh
+    if types["device"]() != dev:
+        raise NekoError(f"paged cache: the tensors are on cuda:{dev}, which is not the current device")
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), st[0] if pages > 1 else n_kv * ps * hd, sst,
+            tst[0] if n_seq > 1 else width, type_, n_seq, width, pages, n_kv, ps, hd, 0), n_seq, n_kv, hd, dev
 
 
 def rope_table(positions, rot, theta, scaling="none", factor=1.0, original=0, beta_fast=32.0, beta_slow=1.0,
@@ -267,35 +257,38 @@ def paged_append(k, v, k_pages, v_pages, table, start, k_scale=None, v_scale=Non
     q_start[s + 1] - 1 (q_start None: row s) and go to positions start[s], start[s] + 1, ..; at most max_new per
     sequence. Returns q with its norm (q_gain) and rotation applied (into q_out, which may be q; a new tensor when
     None), or None without q."""
-    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table)
-    type_ = _type(k, "paged_append k")
-    tokens = k.shape[0]
-    if k.shape[1] != n_kv or v.shape[1] != n_kv:
-        raise NekoError("paged_append: k and v have the cache's KV heads")
-    kp = _rows(k, "paged_append k", type_, tokens, hd, dev)
-    vp = _rows(v, "paged_append v", type_, tokens, hd, dev)
+    types = _types or _setup()
+    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table, types)
+    dt, tokens = k.dtype, k.shape[0]
+    shape = (tokens, n_kv, hd)
+    kp = _rows(k, "paged_append k", dt, shape, dev)
+    vp = _rows(v, "paged_append v", dt, shape, dev)
     qp = op = (0, 0, 0)
     heads = 0
     if q is not None:
         heads = q.shape[1]
-        qp = _rows(q, "paged_append q", type_, tokens, hd, dev)
+        shape = (tokens, heads, hd)
+        qp = _rows(q, "paged_append q", dt, shape, dev)
         if q_out is None:
-            q_out = q.new_empty((tokens, heads, hd))
-        elif q_out.shape != q.shape:
-            raise NekoError("paged_append: q_out is shaped like q")
-        op = _rows(q_out, "paged_append q_out", type_, tokens, hd, dev)
+            q_out = q.new_empty(shape)
+        op = _rows(q_out, "paged_append q_out", dt, shape, dev)
     rot = rows = csp = 0
     if cs is not None:
-        if cs.dim() != 3 or cs.shape[2] != 2:
+        rows, half, two = cs.shape
+        rot = 2 * half
+        if two != 2:
             raise NekoError("paged_append: cs is [positions][rot / 2][2]")
-        rows, rot = cs.shape[0], 2 * cs.shape[1]
-        csp = _floats(cs, "paged_append cs", rows * rot, dev)
+        csp = _vector(cs, "paged_append cs", types["f32"], rows * rot, dev)
+    i32, f32 = types["i32"], types["f32"]
     args = _APPEND.pack(*fields, qp[0], kp[0], vp[0], op[0], *qp[1:], *kp[1:], *vp[1:], *op[1:],
-                        _ints(start, "paged_append start", n_seq, dev),
-                        _ints(q_start, "paged_append q_start", n_seq + 1, dev), csp,
-                        _floats(q_gain, "paged_append q_gain", hd, dev), _floats(k_gain, "paged_append k_gain", hd, dev),
-                        type_, tokens, heads, max_new, rot, rows, 1 if interleaved else 0, eps)
-    check(lib().neko_op_paged_append(args, _on(dev)), "paged_append")
+                        _vector(start, "paged_append start", i32, n_seq, dev),
+                        _vector(q_start, "paged_append q_start", i32, n_seq + 1, dev), csp,
+                        _vector(q_gain, "paged_append q_gain", f32, hd, dev),
+                        _vector(k_gain, "paged_append k_gain", f32, hd, dev),
+                        types.get(dt, -1), tokens, heads, max_new, rot, rows, 1 if interleaved else 0, eps)
+    rc = types["append"](args, types["stream"](dev))
+    if rc:
+        check(rc, "paged_append")
     return q_out if q is not None else None
 
 
@@ -304,19 +297,22 @@ def paged_attention(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=No
     """neko_op_paged_attention: q [tokens][heads][hd] over the cached keys and values; kv_len [sequences] counts the
     new tokens, which are in the cache already. scale: 1 / sqrt(hd) when None; softcap, window, slopes [heads] and
     prefix [sequences] as the header defines them. Returns out (shaped and typed like q)."""
-    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table)
-    type_ = _type(q, "paged_attention q")
-    tokens, heads = q.shape[0], q.shape[1]
-    qp = _rows(q, "paged_attention q", type_, tokens, hd, dev)
+    types = _types or _setup()
+    fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table, types)
+    dt, shape = q.dtype, q.shape
+    if len(shape) != 3 or shape[2] != hd:
+        raise NekoError("paged_attention q: [tokens][heads][head_dim] rows")
+    qp = _rows(q, "paged_attention q", dt, shape, dev)
     if out is None:
-        out = q.new_empty((tokens, heads, hd))
-    elif out.shape != q.shape:
-        raise NekoError("paged_attention: out is shaped like q")
-    op = _rows(out, "paged_attention out", type_, tokens, hd, dev)
-    args = _ATTEND.pack(*fields, qp[0], op[0], *qp[1:], *op[1:], _ints(kv_len, "paged_attention kv_len", n_seq, dev),
-                        _ints(q_start, "paged_attention q_start", n_seq + 1, dev),
-                        _floats(slopes, "paged_attention slopes", heads, dev),
-                        _ints(prefix, "paged_attention prefix", n_seq, dev), type_, tokens, heads, max_new, window,
-                        hd ** -0.5 if scale is None else scale, softcap, 0)
-    check(lib().neko_op_paged_attention(args, _on(dev)), "paged_attention")
+        out = q.new_empty(shape)
+    op = _rows(out, "paged_attention out", dt, shape, dev)
+    i32 = types["i32"]
+    args = _ATTEND.pack(*fields, qp[0], op[0], *qp[1:], *op[1:], _vector(kv_len, "paged_attention kv_len", i32, n_seq, dev),
+                        _vector(q_start, "paged_attention q_start", i32, n_seq + 1, dev),
+                        _vector(slopes, "paged_attention slopes", types["f32"], shape[1], dev),
+                        _vector(prefix, "paged_attention prefix", i32, n_seq, dev), types.get(dt, -1), shape[0], shape[1],
+                        max_new, window, hd ** -0.5 if scale is None else scale, softcap, 0)
+    rc = types["attend"](args, types["stream"](dev))
+    if rc:
+        check(rc, "paged_attention")
     return out

@@ -35,7 +35,6 @@ namespace {
 constexpr int kRows = 128, kKeys = 128;  // of a tile
 constexpr int kThreads = 12 * 32;  // 168 registers a thread: a row's 128 scores stay in them
 constexpr int kLoaders = 96;
-constexpr int kQBatch = 8;      // a multiple of it is 128: batches stay in one row tile
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
@@ -48,6 +47,8 @@ struct PromptPlan {
     int ranks;      // CTAs that share a (sequence, KV head, row tile pair): the cluster
     int row_tiles;  // pairs of row tiles per (sequence, KV head)
     int tiles_per;  // row tiles of a CTA: 1 or 2
+    int group;      // query heads per KV head
+    uint64_t group_inv;  // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
 };
 
 template <int HD, bool Q8, bool HILO>
@@ -68,7 +69,7 @@ struct PL {
 
 // barriers and small arrays behind the operands
 struct Misc {
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned;
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full;
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
@@ -115,7 +116,7 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&v)[8]) {
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
@@ -201,7 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     b /= c.n_kv;
     const int s = b % c.n_seq;
     const int tile = plan.row_tiles - 1 - b / c.n_seq;  // the longest rows first
-    const int G = a.n_head / c.n_kv;
+    const int G = plan.group;
+    auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
     const int row0 = a.q_start ? a.q_start[s] : s;
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
     const int held = max(a.kv_len[s], 0);
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int rows = min(n * G - r0, plan.tiles_per * kRows);
     if (rows <= 0) return;
     const int mt = rows > kRows ? 2 : 1;
-    const int pos_lo = held - n + r0 / G, pos_hi = held - n + (r0 + rows - 1) / G;
+    const int pos_lo = held - n + over_g(r0), pos_hi = held - n + over_g(r0 + rows - 1);
     const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
     const int hi = max(min(len, pos_hi + 1), 0);
     const int lo = a.window ? min(max(pos_lo - a.window + 1, 0), hi) : 0;
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     if (tid == 0) {
         for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], Q8 ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
         for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 128), mbar_init(&ms.pv_done[h], 1);
-        mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders);
+        mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders), mbar_init(&ms.q_full, 256);
         ms.fail = 0;
         for (int i = 0; i < 8; i++) ms.odd[i / 4][i % 4] = 0;  // tiles 0 and 1
         fence_barrier_init();
@@ -241,51 +243,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    // ---- queries: a warp per row, hd / 32 values a lane, the loads of kQBatch rows in flight together
-    {
-        constexpr int E = HD / 32;
-        const auto load_q = [&](auto* q) {
-#pragma unroll 1
-            for (int rb = warp * kQBatch; rb < mt * kRows; rb += 12 * kQBatch) {
-                float x[kQBatch][E];
-#pragma unroll
-                for (int y = 0; y < kQBatch; y++) {
-                    const int pr = r0 + rb + y;
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[y][e] = 0.0f;
-                    if (rb + y < rows) {
-                        const auto* p = q + int64_t(row0 + pr / G) * a.q_token + int64_t(kvh * G + pr % G) * a.q_head + lane * E;
-                        load_row<E>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * E - 1)) == 0, x[y]);
-                    }
-                }
-#pragma unroll
-                for (int y = 0; y < kQBatch; y++) {
-                    const int r = rb + y;
-                    float most = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < E; e++) most = fmaxf(most, finite_abs(x[y][e]));
-                    const float up = row_up(warp_max(most));
-                    uint32_t h2[E / 2], l2[E / 2];
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) split_hilo(x[y][e] * up, x[y][e + 1] * up, h2[e / 2], l2[e / 2]);
-                    const int d = lane * E, half = d / 64;
-                    uint8_t* dst = sm + (r / kRows * L::kParts) * L::kQTile + half * L::kHalf + sw128_off(r % kRows, (d % 64) / 8) + (d % 8) * 2;
-                    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h2[0], h2[1]);
-                    else *reinterpret_cast<uint32_t*>(dst) = h2[0];
-                    if constexpr (HILO) {
-                        dst += L::kQTile;
-                        if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(l2[0], l2[1]);
-                        else *reinterpret_cast<uint32_t*>(dst) = l2[0];
-                    }
-                    if (lane == 0) ms.qdown[r] = a.scale / up;
-                }
-            }
-        };
-        if constexpr (HILO) load_q(static_cast<const float*>(a.q));
-        else if (a.type == kTF16) load_q(static_cast<const __half*>(a.q));
-        else load_q(static_cast<const __nv_bfloat16*>(a.q));
-        fence_proxy_async();
     }
     tc_fence_before();
     __syncthreads();
@@ -505,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             auto commit = [&](uint64_t* bar) {
                 if (elect_one()) umma_commit(bar);
             };
-            bool ok = wait_on(&ms.full[0], 0, fail);
+            bool ok = wait_on(&ms.q_full, 0, fail) && wait_on(&ms.full[0], 0, fail);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
                 for (int h = 0; h < mt; h++) issue_s(h, 0);
@@ -539,17 +496,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             mbar_wait(&ms.drain, 0);
         }
         __syncwarp();
-    } else if (warp / 4 < mt) {
+    } else {
+        // ------------------------------------------------------------------ queries: eight lanes a row, hd / 8 values each
+        constexpr int E = HD / 8;
+        const auto load_q = [&](auto* base) {
+#pragma unroll 2
+            for (int r = warp * 4 + (lane >> 3); r < mt * kRows; r += 32) {
+                float x[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) x[e] = 0.0f;
+                if (r < rows) {
+                    const int pr = r0 + r, rt = over_g(pr);
+                    const auto* p = base + int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + pr - rt * G) * a.q_head + (lane & 7) * E;
+                    const bool vec = (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0;
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) load_row<4>(p + e, vec, *reinterpret_cast<float(*)[4]>(&x[e]));
+                }
+                float most = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) most = fmaxf(most, finite_abs(x[e]));
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float up = row_up(most);
+                const int d = (lane & 7) * E;
+                uint8_t* dst = sm + (r / kRows * L::kParts) * L::kQTile + d / 64 * L::kHalf;
+#pragma unroll
+                for (int e = 0; e < E; e += 8) {
+                    uint32_t h2[4], l2[4];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) split_hilo(x[e + 2 * y] * up, x[e + 2 * y + 1] * up, h2[y], l2[y]);
+                    const uint32_t at = sw128_off(r % kRows, (d % 64 + e) / 8);
+                    *reinterpret_cast<uint4*>(dst + at) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
+                    if constexpr (HILO) *reinterpret_cast<uint4*>(dst + L::kQTile + at) = make_uint4(l2[0], l2[1], l2[2], l2[3]);
+                }
+                if ((lane & 7) == 0) ms.qdown[r] = a.scale / up;
+            }
+        };
+        if constexpr (HILO) load_q(static_cast<const float*>(a.q));
+        else if (a.type == kTF16) load_q(static_cast<const __half*>(a.q));
+        else load_q(static_cast<const __nv_bfloat16*>(a.q));
+        fence_proxy_async();
+        mbar_arrive(&ms.q_full);
+    }
+    if (warp < 8 && warp / 4 < mt) {
         // ------------------------------------------------------------------ softmax, a thread per row
         const int h = warp / 4;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + h * 128, to = tmem + lanes + 256 + h * 128;
         const int r = h * kRows + (warp & 3) * 32 + lane, pr = r0 + r;
         const bool real = r < rows;
-        const int qpos = real ? held - n + pr / G : kNoRow;
-        const float down = ms.qdown[r];
-        const float slope = a.slopes && real ? a.slopes[kvh * G + pr % G] * kLog2e : 0.0f;
-        const int h_lo = held - n + (r0 + h * kRows) / G, h_hi = held - n + (r0 + min(rows, (h + 1) * kRows) - 1) / G;
+        const int rt = over_g(pr), qpos = real ? held - n + rt : kNoRow;
+        const float slope = a.slopes && real ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
+        const int h_lo = held - n + over_g(r0 + h * kRows), h_hi = held - n + over_g(r0 + min(rows, (h + 1) * kRows) - 1);
         const bool shaped = a.softcap > 0.0f || a.slopes;
         const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
         {
@@ -560,7 +558,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             for (int x = 0; x < HD; x += 32) st32(to + x, z);
             st_wait();
         }
-        bool ok = true;
+        bool ok = __all_sync(0xffffffffu, wait_on(&ms.q_full, 0, fail));
+        const float down = ms.qdown[r];
         for (int i = 0; i < nt && ok; i++) {
             const int j0 = key_of(i);
             ok = wait_on(&ms.s_full[h], i & 1, fail);
@@ -572,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const bool plain_mask = open(j0, h_lo, h_hi) && ms.whole[i % kRing];
             const float vnow = Q8 ? ms.vtop[i % kRing] : 0.0f;
             const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
-            // ---- the row's largest score (log2 units); the masking loop is
-            // kept rolled: as straight code it was bound by instruction fetch
+            // ---- tiles that need more than the scale (the loop is kept rolled: as straight code it was bound by instruction
+            // fetch)
             if (cooked) {  // scale, cap, bias and masks, back into TMEM
 #pragma unroll 1
                 for (int q = 0; q < 4; q++) {
@@ -608,28 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 st_wait();
             }
-            uint32_t w[4][32];  // the row's scores
-#pragma unroll
-            for (int q = 0; q < 4; q++) ld32(ts + 32 * q, w[q]);
-#pragma unroll
-            for (int q = 0; q < 4; q++) ld_wait(w[q]);
-            float top = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const float* u = reinterpret_cast<const float*>(&w[q][16 * g]);
-                    float m[4] = {u[0], u[1], u[2], u[3]};
-#pragma unroll
-                    for (int x = 4; x < 16; x++) m[x & 3] = max_nan(m[x & 3], u[x]);
-                    const float m0 = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
-                    top = max_nan(top, Q8 && !cooked ? m0 * ksp[2 * q + g] : m0);
-                }
-            if (!cooked) top *= down * kLog2e;
-            if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
-            // ---- the reference maximum and value scale
+            // ---- the value scale's reference, and values that are not finite in this tile
             const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
-            const bool up = top > row_max + kLazy;  // also from -inf
             bool odd_tile = false;
             const int xv = 2 * i + 1, stv = xv % L::kStages;
             if (!open(j0, pos_lo, pos_hi)) {
@@ -639,65 +618,73 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const uint32_t* od = ms.odd[i % kOddRing];
                 odd_tile = (od[0] | od[1] | od[2] | od[3]) != 0;
             }
-            if (__any_sync(0xffffffffu, up || v_up || odd_tile)) {
-                float f = 1.0f;
-                if (up) {
-                    f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
-                    row_sum *= f;
-                    row_max = top;
-                }
-                if (v_up) {
-                    if (i > 0) f *= ex2(vref - vnow);
-                    vref = vnow;
-                }
-                if (i > 0) {
-                    ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                }
-                if (i > 0 || odd_tile) {
+            float f_o = 1.0f;  // what O has to be multiplied by
+            if (v_up) {
+                if (i > 0) f_o = ex2(vref - vnow);
+                vref = vnow;
+            }
+            bool fix = (v_up && i > 0) || odd_tile;
+            // ---- weights against the reference maximum so far; only where a score exceeds it by more than 2^8 (and in the
+            // first tile) it moves to the largest score, O follows, and the weights are taken again
+            uint32_t w[4][32];
+            float sum;
+            for (;;) {
+                if (fix) {  // the same for the whole warp
+                    if (i > 0) {
+                        ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if (i > 0 || odd_tile) {
 #pragma unroll 1
-                    for (int x = 0; x < HD; x += 32) {
-                        uint32_t o[32];
-                        ld32(to + x, o);
-                        ld_wait(o);
+                        for (int x = 0; x < HD; x += 32) {
+                            uint32_t o[32];
+                            ld32(to + x, o);
+                            ld_wait(o);
 #pragma unroll
-                        for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                        if (odd_tile) {
+                            for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f_o);
+                            if (odd_tile) {
 #pragma unroll 1
-                            for (int key = 0; key < kKeys; key++) {
-                                if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
-                                const int j = j0 + key, slot = j / c.page_size;
-                                if (j >= len || ksp[key >> 4] == kGone) continue;
-                                const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
-                                const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
-                                                   (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
+                                for (int key = 0; key < kKeys; key++) {
+                                    if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
+                                    const int j = j0 + key, slot = j / c.page_size;
+                                    if (j >= len || ksp[key >> 4] == kGone) continue;
+                                    const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
+                                    const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
+                                                       (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
 #pragma unroll
-                                for (int y = 0; y < 32; y++) {
-                                    float v;
-                                    if constexpr (Q8) {
-                                        v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
-                                    } else {
-                                        v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
-                                        if (fabsf(v) <= 65504.0f) v = 0.0f;
+                                    for (int y = 0; y < 32; y++) {
+                                        float v;
+                                        if constexpr (Q8) {
+                                            v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
+                                        } else {
+                                            v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
+                                            if (fabsf(v) <= 65504.0f) v = 0.0f;
+                                        }
+                                        if (see) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
                                     }
-                                    if (see) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
                                 }
                             }
+                            st32(to + x, o);
                         }
-                        st32(to + x, o);
+                        st_wait();
                     }
-                    st_wait();
+                    odd_tile = false;
                 }
-            }
-            // ---- weights, their sum; P over S
-            const float ref = row_max == -INFINITY ? 0.0f : row_max;
-            {
+                const float ref = row_max == -INFINITY ? 0.0f : row_max;
                 const float f0 = cooked ? 1.0f : down * kLog2e;
+                float top = -INFINITY;
+                sum = 0.0f;
                 uint64_t sums[2] = {0, 0};
+                ld32(ts, w[0]);
+                ld32(ts + 32, w[1]);
+                ld_wait(w[0]), ld_wait(w[1]);
+                ld32(ts + 64, w[2]);
+                ld32(ts + 96, w[3]);
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
+                    if (q == 2) ld_wait(w[2]), ld_wait(w[3]);
                     uint32_t(&u)[32] = w[q];
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
@@ -705,45 +692,65 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                         const float f = Q8 && !cooked ? f0 * ksp[blk] : f0;
                         const float vr = Q8 ? fmaxf(vsp[blk] - vref, kVMin) : 0.0f;
                         const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
+                        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         if (Q8) sums[0] = sums[1] = 0;
+                        [[maybe_unused]] uint32_t hl[8];
 #pragma unroll
                         for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                            const float s0 = __uint_as_float(u[x]), s1 = __uint_as_float(u[x + 1]);
+                            m[x & 2] = max_nan(m[x & 2], s0), m[(x & 2) + 1] = max_nan(m[(x & 2) + 1], s1);
                             float z0, z1;
-                            unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
+                            unpack2(fma2(pack2(s0, s1), ff, off), z0, z1);
                             if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
                             else z0 = ex2(z0), z1 = ex2(z1);
-                            u[x] = __float_as_uint(z0), u[x + 1] = __float_as_uint(z1);
                             sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
+                            // the weights as f16 in the scores' registers: columns x / 2, or hi and lo
+                            if constexpr (HILO) split_hilo(z0, z1, u[16 * g + (x & 15) / 2], hl[x / 2 & 7]);
+                            else u[x / 2] = h2u(__floats2half2_rn(z0, z1));
                         }
                         if constexpr (HILO) {
-                            uint32_t hi8[8], lo8[8];
 #pragma unroll
-                            for (int x = 0; x < 8; x++)
-                                split_hilo(__uint_as_float(u[16 * g + 2 * x]), __uint_as_float(u[16 * g + 2 * x + 1]), hi8[x], lo8[x]);
-                            st8(ts + 32 * q + 8 * g, hi8);
-                            st8(ts + 32 * q + 16 + 8 * g, lo8);
+                            for (int x = 0; x < 8; x++) u[16 * g + 8 + x] = hl[x];
                         }
+                        top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * f);
                         if (Q8) {  // the sum without the value scale
                             float z0, z1;
                             unpack2(add2(sums[0], sums[1]), z0, z1);
-                            row_sum = fmaf(z0 + z1, ex2(-vr), row_sum);
+                            sum = fmaf(z0 + z1, ex2(-vr), sum);
                         }
-                    }
-                    if constexpr (!HILO) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int x = 0; x < 16; x++)
-                            p[x] = h2u(__floats2half2_rn(__uint_as_float(u[2 * x]), __uint_as_float(u[2 * x + 1])));
-                        st16(ts + 16 * q, p);
                     }
                 }
                 if (!Q8) {
                     float z0, z1;
                     unpack2(add2(sums[0], sums[1]), z0, z1);
-                    row_sum += z0 + z1;
+                    sum = z0 + z1;
                 }
-                st_wait();
+                const bool up = top > row_max + kLazy;  // also from -inf
+                if (!(top < INFINITY)) sum = NAN;       // as exp(inf - inf) and exp(NaN) give, whatever computed the weights
+                fix = __any_sync(0xffffffffu, up && top < INFINITY);
+                if (!fix) break;
+                f_o = 1.0f;
+                if (up && top < INFINITY) {
+                    f_o = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
+                    row_sum *= f_o;
+                    row_max = top;
+                }
             }
+            if (!ok) break;
+            row_sum += sum;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (HILO) {  // 32-column groups: hi of 32 keys, lo of them
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        st8(ts + 32 * q + 8 * g, &w[q][16 * g]);
+                        st8(ts + 32 * q + 16 + 8 * g, &w[q][16 * g + 8]);
+                    }
+                } else {
+                    st16(ts + 16 * q, *reinterpret_cast<const uint32_t(*)[16]>(w[q]));
+                }
+            }
+            st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);
         }
@@ -784,7 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     auto put = [&](int r, int d, float4 v) {
         const int pr = r0 + r;
-        const int64_t off = int64_t(row0 + pr / G) * a.o_token + int64_t(kvh * G + pr % G) * a.o_head + d;
+        const int rt = over_g(pr);
+        const int64_t off = int64_t(row0 + rt) * a.o_token + int64_t(kvh * G + pr - rt * G) * a.o_head + d;
         const float x[4] = {v.x, v.y, v.z, v.w};
         auto store = [&](auto* p) { store_row<4>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0, x); };
         if (a.type == kTF32) store(static_cast<float*>(a.out) + off);
@@ -803,16 +811,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int share = (rows * (HD / 4) + plan.ranks - 1) / plan.ranks;
     for (int x = rank * share + tid; x < min(rows * (HD / 4), (rank + 1) * share); x += kThreads) {
         const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-        float top = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < plan.ranks; w++) top = fmaxf(top, cluster.map_shared_rank(state, w)[r * L::kJoinPitch + HD]);
+        float mw[8], lw[8], top = -INFINITY, sum = 0.0f;
+        float4 o[8];
+#pragma unroll
+        for (int w = 0; w < 8; w++) {  // all ranks' loads in flight
+            const float* st = cluster.map_shared_rank(state, w < plan.ranks ? w : 0) + r * L::kJoinPitch;
+            mw[w] = w < plan.ranks ? st[HD] : -INFINITY, lw[w] = st[HD + 1];
+            o[w] = *reinterpret_cast<const float4*>(st + d);
+        }
+#pragma unroll
+        for (int w = 0; w < 8; w++) top = fmaxf(top, mw[w]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float4 v = make_float4(0, 0, 0, 0);
-        for (int w = 0; w < plan.ranks; w++) {
-            const float* st = cluster.map_shared_rank(state, w) + r * L::kJoinPitch;
-            const float f = ex2(st[HD] - ref);
-            const float4 o = *reinterpret_cast<const float4*>(st + d);
-            sum += f * st[HD + 1];
-            v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            const float f = ex2(mw[w] - ref);
+            if (w < plan.ranks) sum = fmaf(f, lw[w], sum), v.x = fmaf(f, o[w].x, v.x), v.y = fmaf(f, o[w].y, v.y), v.z = fmaf(f, o[w].z, v.z), v.w = fmaf(f, o[w].w, v.w);
         }
         const float f = 1.0f / sum;
         put(r, d, sum == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
@@ -831,6 +845,8 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     p.tiles_per = tiles > 1 && heads * ((tiles + 1) / 2) * 2 > num_sms() ? 2 : 1;
     p.row_tiles = int((tiles + p.tiles_per - 1) / p.tiles_per);
     const int64_t items = heads * p.row_tiles, key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
+    p.group = a.n_head / c.n_kv;
+    p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
     p.ranks = 1;
     while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;

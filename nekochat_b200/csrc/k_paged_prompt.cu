@@ -35,6 +35,8 @@ namespace {
 constexpr int kRows = 128, kKeys = 128;  // of a tile
 constexpr int kThreads = 12 * 32;  // 168 registers a thread: a row's 128 scores stay in them
 constexpr int kLoaders = 96;
+constexpr int kCopyTiles = 3;
+constexpr int64_t kCopyBytes = int64_t(1) << 31;
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
@@ -42,6 +44,9 @@ constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
 constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
 constexpr float kVNone = -126.0f;
 constexpr float kGone = -1.0f;
+
+// What the key and value tiles come from: f16 pages, 8-bit pages converted by the loader, or f16 copies of 8-bit pages.
+enum Source : int { kF16Pages = 0, kCodes = 1, kCopies = 2 };
 
 struct PromptPlan {
     int ranks;      // CTAs that share a (sequence, KV head, row tile pair): the cluster
@@ -51,7 +56,7 @@ struct PromptPlan {
     uint64_t group_inv;  // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
 };
 
-template <int HD, bool Q8, bool HILO>
+template <int HD, bool HILO>
 struct PL {
     static constexpr int kParts = HILO ? 2 : 1;
     static constexpr int kHalf = kRows * 128;             // bytes of a 128-row, 64-wide f16 tile
@@ -116,11 +121,6 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
-                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -183,11 +183,12 @@ __device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-template <int HD, bool Q8, bool HILO>
+template <int HD, int SRC, bool HILO>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_paged_attention_args a,
                                                                   const PromptPlan plan,
                                                                   const __grid_constant__ PromptMaps maps) {
-    using L = PL<HD, Q8, HILO>;
+    constexpr bool kScaled = SRC != kF16Pages, kConvert = SRC == kCodes;
+    using L = PL<HD, HILO>;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     Misc& ms = *reinterpret_cast<Misc*>(sm + L::kMiscOff);
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     };
 
     if (tid == 0) {
-        for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], Q8 ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
+        for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], kConvert ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
         for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 128), mbar_init(&ms.pv_done[h], 1);
         mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders), mbar_init(&ms.q_full, 256);
         ms.fail = 0;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         };
         int pages = nt > 0 ? pages_of(key_of(0)) : -1, pages_next = -1;
         bool ok = true;
-        if constexpr (Q8) {
+        if constexpr (kConvert) {
             constexpr int kRowChunks = HD / 16;             // 16-byte pieces of a key row
             constexpr int kRowsAt = kLoaders / kRowChunks;  // key rows of one round of pieces: 12 or 24
             constexpr int kPer = (kKeys + kRowsAt - 1) / kRowsAt;
@@ -364,6 +365,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const uint32_t box_bytes = uint32_t(c.page_size) * 128;
             const bool carrier = box < per_page;  // at most 16 lanes (8 pages of 16 tokens, two halves)
             int scans = 0;
+            float ks = 0.0f, vs = 0.0f;
+            auto scales = [&]() {
+                if (SRC == kCopies && warp == 8 && pages >= 0) {
+                    ks = c.k_scale[int64_t(pages) * c.scale_stride + kvh];
+                    vs = c.v_scale[int64_t(pages) * c.scale_stride + kvh];
+                }
+            };
+            if (nt > 0) scales();
             for (int x = 0; x < total; x++) {
                 const int st = x % L::kStages, i = x >> 1;
                 const bool v = x & 1;
@@ -377,10 +386,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                     }
-                    if (!v && lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? 1.0f : kGone;
+                    if (!v) {
+                        const float vl = SRC == kCopies && lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone;
+                        const float vt = SRC == kCopies ? warp_max(vl) : 0.0f;
+                        if (lane < 8) ms.ks[i % kRing][lane] = pages < 0 ? kGone : SRC == kCopies ? fabsf(ks) : 1.0f, ms.vs[i % kRing][lane] = vl;
+                        if (lane == 0) ms.vtop[i % kRing] = vt;
+                    }
                     if (!v && lane < 4) ms.odd[(i + 2) % kOddRing][lane] = 0;
                     if (!v && lane == 0) ms.whole[i % kRing] = whole;
-                    const int page = __shfl_sync(0xffffffffu, pages, carrier ? box << (ps_log - 4) : 31);
+                    int page = __shfl_sync(0xffffffffu, pages, carrier ? box << (ps_log - 4) : 31);
+                    if (SRC == kCopies && page >= 0) page = s * c.max_pages + (j0 >> ps_log) + box;
                     const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
                     uint64_t* bar = scan ? &ms.land : &ms.full[st];
                     if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_bytes);
@@ -420,7 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     scans++;
                 }
                 if (!v && i + 1 < nt) pages_next = pages_of(key_of(i + 1));
-                if (v) pages = pages_next;
+                if (v) {
+                    pages = pages_next;
+                    scales();
+                }
             }
         }
     } else if (warp == 11) {
@@ -548,8 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         const int rt = over_g(pr), qpos = real ? held - n + rt : kNoRow;
         const float slope = a.slopes && real ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
         const int h_lo = held - n + over_g(r0 + h * kRows), h_hi = held - n + over_g(r0 + min(rows, (h + 1) * kRows) - 1);
-        const bool shaped = a.softcap > 0.0f || a.slopes;
-        const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+        const float cap = a.softcap * kLog2e;
         {
             uint32_t z[32];
 #pragma unroll
@@ -559,7 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             st_wait();
         }
         bool ok = __all_sync(0xffffffffu, wait_on(&ms.q_full, 0, fail));
-        const float down = ms.qdown[r];
+        // from the accumulator to log2 units, or with a cap to the tanh's argument
+        const float factor = a.softcap > 0.0f ? ms.qdown[r] / a.softcap : ms.qdown[r] * kLog2e;
         for (int i = 0; i < nt && ok; i++) {
             const int j0 = key_of(i);
             ok = wait_on(&ms.s_full[h], i & 1, fail);
@@ -569,48 +587,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const float* ksp = ms.ks[i % kRing];
             const float* vsp = ms.vs[i % kRing];
             const bool plain_mask = open(j0, h_lo, h_hi) && ms.whole[i % kRing];
-            const float vnow = Q8 ? ms.vtop[i % kRing] : 0.0f;
-            const bool cooked = shaped || !plain_mask || a.scale < 0.0f;  // one answer for the whole warp
-            // ---- tiles that need more than the scale (the loop is kept rolled: as straight code it was bound by instruction
-            // fetch)
-            if (cooked) {  // scale, cap, bias and masks, back into TMEM
-#pragma unroll 1
-                for (int q = 0; q < 4; q++) {
-                    uint32_t u[32];
-                    ld32(ts + 32 * q, u);
-                    ld_wait(u);
-                    const float ks0 = ksp[2 * q], ks1 = ksp[2 * q + 1];
-                    const int jq = j0 + 32 * q;
-#pragma unroll
-                    for (int x = 0; x < 32; x++) {
-                        const float ks = x < 16 ? ks0 : ks1;
-                        float v = __uint_as_float(u[x]) * (down * ks);
-                        if (a.softcap > 0.0f) v = a.softcap * tanh_abs(v * inv_cap);
-                        u[x] = __float_as_uint(v * kLog2e);
-                    }
-                    if (a.slopes) {
-#pragma unroll
-                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x])));
-                    }
-                    if (!plain_mask) {
-                        // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
-                        const int see_hi = min(len, qpos + 1), see_lo = a.window ? qpos - a.window + 1 : 0;
-                        const int pre = real ? prefix : 0;
-#pragma unroll
-                        for (int x = 0; x < 32; x++) {
-                            const int j = jq + x;
-                            const bool see = ((j < see_hi && j >= see_lo) || j < pre) && (x < 16 ? ks0 : ks1) != kGone;
-                            if (!see) u[x] = __float_as_uint(-INFINITY);
-                        }
-                    }
-                    st32(ts + 32 * q, u);
-                }
-                st_wait();
-            }
-            // ---- the value scale's reference, and values that are not finite in this tile
-            const bool v_up = Q8 && (i == 0 || vnow > vref + kVLazy);
-            bool odd_tile = false;
+            const float vnow = kScaled ? ms.vtop[i % kRing] : 0.0f;
             const int xv = 2 * i + 1, stv = xv % L::kStages;
+            bool odd_tile = false;
             if (!open(j0, pos_lo, pos_hi)) {
                 ok = wait_on(&ms.full[stv], (xv / L::kStages) & 1, fail);
                 ok = __all_sync(0xffffffffu, ok);
@@ -618,138 +597,187 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const uint32_t* od = ms.odd[i % kOddRing];
                 odd_tile = (od[0] | od[1] | od[2] | od[3]) != 0;
             }
-            float f_o = 1.0f;  // what O has to be multiplied by
-            if (v_up) {
-                if (i > 0) f_o = ex2(vref - vnow);
-                vref = vnow;
-            }
-            bool fix = (v_up && i > 0) || odd_tile;
-            // ---- weights against the reference maximum so far; only where a score exceeds it by more than 2^8 (and in the
-            // first tile) it moves to the largest score, O follows, and the weights are taken again
-            uint32_t w[4][32];
-            float sum;
-            for (;;) {
-                if (fix) {  // the same for the whole warp
-                    if (i > 0) {
-                        ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    if (i > 0 || odd_tile) {
+            // O times f for this thread's row, and this tile's values that are not finite
+            auto fix_o = [&](float f, bool odd) {
+                if (i > 0) {
+                    ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    tc_fence_after();
+                }
 #pragma unroll 1
-                        for (int x = 0; x < HD; x += 32) {
-                            uint32_t o[32];
-                            ld32(to + x, o);
-                            ld_wait(o);
+                for (int x = 0; x < HD; x += 32) {
+                    uint32_t o[32];
+                    ld32(to + x, o);
+                    ld_wait(o);
 #pragma unroll
-                            for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f_o);
-                            if (odd_tile) {
+                    for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                    if (odd) {
 #pragma unroll 1
-                                for (int key = 0; key < kKeys; key++) {
-                                    if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
-                                    const int j = j0 + key, slot = j / c.page_size;
-                                    if (j >= len || ksp[key >> 4] == kGone) continue;
-                                    const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
-                                    const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
-                                                       (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
+                        for (int key = 0; key < kKeys; key++) {
+                            if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
+                            const int j = j0 + key, slot = j / c.page_size;
+                            if (j >= len || ksp[key >> 4] == kGone) continue;
+                            const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
+                            const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
+                                               (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
 #pragma unroll
-                                    for (int y = 0; y < 32; y++) {
-                                        float v;
-                                        if constexpr (Q8) {
-                                            v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
-                                        } else {
-                                            v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
-                                            if (fabsf(v) <= 65504.0f) v = 0.0f;
-                                        }
-                                        if (see) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
-                                    }
+                            for (int y = 0; y < 32; y++) {
+                                float v;
+                                if constexpr (kScaled) {
+                                    v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
+                                } else {
+                                    v = __half2float(static_cast<const __half*>(c.v_pages)[at + y]);
+                                    if (fabsf(v) <= 65504.0f) v = 0.0f;
                                 }
+                                if (see) o[y] = __float_as_uint(__uint_as_float(o[y]) + v);
                             }
-                            st32(to + x, o);
                         }
-                        st_wait();
                     }
-                    odd_tile = false;
+                    st32(to + x, o);
                 }
+                st_wait();
+            };
+            {
+                const bool v_up = kScaled && (i == 0 || vnow > vref + kVLazy);
+                if (odd_tile || (v_up && i > 0)) fix_o(v_up && i > 0 ? ex2(vref - vnow) : 1.0f, odd_tile);
+                if (!ok) break;
+                if (v_up) vref = vnow;
+            }
+            // ---- 32 keys at a time, in a rolled loop (as straight code it was bound by instruction fetch)
+            uint32_t ahead[32];
+            ld32(ts, ahead);
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+                uint32_t u[32];
+                ld_wait(ahead);
+#pragma unroll
+                for (int x = 0; x < 32; x++) u[x] = ahead[x];
+                if (q < 3) ld32(ts + 32 * (q + 1), ahead);
+                float f0 = kScaled ? factor * ksp[2 * q] : factor, f1 = kScaled ? factor * ksp[2 * q + 1] : factor;
+                const float ks0 = ksp[2 * q], ks1 = ksp[2 * q + 1];
+                if (a.softcap > 0.0f) {  // y = score / cap
+                    float most = 0.0f;
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        u[x] = __float_as_uint(__uint_as_float(u[x]) * (x < 16 ? f0 : f1));
+                        most = max_nan(most, fabsf(__uint_as_float(u[x])));
+                    }
+                    if (__all_sync(0xffffffffu, most <= 0.5f)) {
+                        // an odd polynomial of degree 9 (least maximum error on [-1/2, 1/2]: 3e-9): two units of the
+                        // special functions less than below
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) {
+                            const uint64_t y = pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), y2 = mul2(y, y);
+                            uint64_t p = fma2(y2, pack2(0.016737453639507294f, 0.016737453639507294f), pack2(-0.05276207625865936f, -0.05276207625865936f));
+                            p = fma2(p, y2, pack2(0.13320569694042206f, 0.13320569694042206f));
+                            p = fma2(p, y2, pack2(-0.3333277702331543f, -0.3333277702331543f));
+                            p = fma2(p, y2, pack2(0.9999999403953552f, 0.9999999403953552f));
+                            p = mul2(mul2(p, y), pack2(cap, cap));
+                            float p0, p1;
+                            unpack2(p, p0, p1);
+                            u[x] = __float_as_uint(p0), u[x + 1] = __float_as_uint(p1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(cap * tanh_abs(__uint_as_float(u[x])));
+                    }
+                    f0 = f1 = 1.0f;
+                }
+                const int jq = j0 + 32 * q;
+                if (a.slopes) {
+#pragma unroll
+                    for (int x = 0; x < 32; x++)
+                        u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x]) * (x < 16 ? f0 : f1)));
+                    f0 = f1 = 1.0f;
+                }
+                if (!plain_mask || a.scale < 0.0f) {
+                    // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
+                    const int see_hi = plain_mask ? len : min(len, qpos + 1), see_lo = a.window && !plain_mask ? qpos - a.window + 1 : 0;
+                    const int pre = real ? prefix : 0;
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        const int j = jq + x;
+                        const bool see = ((j < see_hi && j >= see_lo) || j < pre) && (x < 16 ? ks0 : ks1) != kGone;
+                        u[x] = see ? __float_as_uint(__uint_as_float(u[x]) * (x < 16 ? f0 : f1)) : 0xff800000u;
+                    }
+                    f0 = f1 = 1.0f;
+                }
+                // the largest score in log2 units
+                float m[8];
+#pragma unroll
+                for (int x = 0; x < 32; x++) {
+                    const float v = __uint_as_float(u[x]);
+                    float& mm = m[(x & 3) + (x & 16) / 4];
+                    mm = (x & 15) < 4 ? v : max_nan(mm, v);
+                }
+                const float top = max_nan(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * f0,
+                                          max_nan(max_nan(m[4], m[5]), max_nan(m[6], m[7])) * f1);
+                if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
+                const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
+                if (__any_sync(0xffffffffu, up)) {
+                    // the reference maximum moves up to the next whole number: O, the sum and this tile's weights so far
+                    // follow, by a power of two
+                    float f = 1.0f;
+                    if (up) {
+                        const float to_max = ceilf(top);
+                        f = ex2(row_max - to_max);  // row_max = -inf: nothing there yet, 0
+                        row_max = to_max;
+                        row_sum *= f;
+                    }
+                    if (i > 0) fix_o(f, false);
+                    if (!ok) break;
+                    const __half2 fh = __float2half2_rn(f);
+                    for (int x = 0; x < (HILO ? q : q / 2 + q % 2); x++) {  // the columns that hold weights by now
+                        uint32_t o[32];
+                        ld32(ts + 32 * x, o);
+                        ld_wait(o);
+#pragma unroll
+                        for (int y = 0; y < 32; y++) {
+                            if (HILO || 32 * x + y < 16 * q) {
+                                const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&o[y]), fh);
+                                o[y] = *reinterpret_cast<const uint32_t*>(&v);
+                            }
+                        }
+                        if (HILO || 2 * x + 2 <= q) st32(ts + 32 * x, o);
+                        else st16(ts + 32 * x, *reinterpret_cast<const uint32_t(*)[16]>(o));
+                    }
+                    st_wait();
+                }
+                // weights, their sum; P over S
                 const float ref = row_max == -INFINITY ? 0.0f : row_max;
-                const float f0 = cooked ? 1.0f : down * kLog2e;
-                float top = -INFINITY;
-                sum = 0.0f;
                 uint64_t sums[2] = {0, 0};
-                ld32(ts, w[0]);
-                ld32(ts + 32, w[1]);
-                ld_wait(w[0]), ld_wait(w[1]);
-                ld32(ts + 64, w[2]);
-                ld32(ts + 96, w[3]);
+                uint32_t p_hi[16], p_lo[HILO ? 16 : 1];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (q == 2) ld_wait(w[2]), ld_wait(w[3]);
-                    uint32_t(&u)[32] = w[q];
+                for (int g = 0; g < 2; g++) {
+                    const float f = g ? f1 : f0;
+                    const float vr = kScaled ? fmaxf(vsp[2 * q + g] - vref, kVMin) : 0.0f;
+                    const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
+                    if (kScaled) sums[0] = sums[1] = 0;
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const int blk = 2 * q + g;
-                        const float f = Q8 && !cooked ? f0 * ksp[blk] : f0;
-                        const float vr = Q8 ? fmaxf(vsp[blk] - vref, kVMin) : 0.0f;
-                        const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
-                        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        if (Q8) sums[0] = sums[1] = 0;
-                        [[maybe_unused]] uint32_t hl[8];
-#pragma unroll
-                        for (int x = 16 * g; x < 16 * g + 16; x += 2) {
-                            const float s0 = __uint_as_float(u[x]), s1 = __uint_as_float(u[x + 1]);
-                            m[x & 2] = max_nan(m[x & 2], s0), m[(x & 2) + 1] = max_nan(m[(x & 2) + 1], s1);
-                            float z0, z1;
-                            unpack2(fma2(pack2(s0, s1), ff, off), z0, z1);
-                            if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
-                            else z0 = ex2(z0), z1 = ex2(z1);
-                            sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
-                            // the weights as f16 in the scores' registers: columns x / 2, or hi and lo
-                            if constexpr (HILO) split_hilo(z0, z1, u[16 * g + (x & 15) / 2], hl[x / 2 & 7]);
-                            else u[x / 2] = h2u(__floats2half2_rn(z0, z1));
-                        }
-                        if constexpr (HILO) {
-#pragma unroll
-                            for (int x = 0; x < 8; x++) u[16 * g + 8 + x] = hl[x];
-                        }
-                        top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * f);
-                        if (Q8) {  // the sum without the value scale
-                            float z0, z1;
-                            unpack2(add2(sums[0], sums[1]), z0, z1);
-                            sum = fmaf(z0 + z1, ex2(-vr), sum);
-                        }
+                    for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                        float z0, z1;
+                        unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
+                        if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
+                        else z0 = ex2(z0), z1 = ex2(z1);
+                        sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
+                        if constexpr (HILO) split_hilo(z0, z1, p_hi[x / 2], p_lo[x / 2]);
+                        else p_hi[x / 2] = h2u(__floats2half2_rn(z0, z1));
+                    }
+                    if (kScaled || g) {  // the sum without the value scale
+                        float z0, z1;
+                        unpack2(add2(sums[0], sums[1]), z0, z1);
+                        row_sum = kScaled ? fmaf(z0 + z1, ex2(-vr), row_sum) : row_sum + (z0 + z1);
                     }
                 }
-                if (!Q8) {
-                    float z0, z1;
-                    unpack2(add2(sums[0], sums[1]), z0, z1);
-                    sum = z0 + z1;
-                }
-                const bool up = top > row_max + kLazy;  // also from -inf
-                if (!(top < INFINITY)) sum = NAN;       // as exp(inf - inf) and exp(NaN) give, whatever computed the weights
-                fix = __any_sync(0xffffffffu, up && top < INFINITY);
-                if (!fix) break;
-                f_o = 1.0f;
-                if (up && top < INFINITY) {
-                    f_o = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
-                    row_sum *= f_o;
-                    row_max = top;
+                if constexpr (HILO) {
+                    st16(ts + 32 * q, p_hi);
+                    st16(ts + 32 * q + 16, p_lo);
+                } else {
+                    st16(ts + 16 * q, p_hi);
                 }
             }
             if (!ok) break;
-            row_sum += sum;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if constexpr (HILO) {  // 32-column groups: hi of 32 keys, lo of them
-#pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        st8(ts + 32 * q + 8 * g, &w[q][16 * g]);
-                        st8(ts + 32 * q + 16 + 8 * g, &w[q][16 * g + 8]);
-                    }
-                } else {
-                    st16(ts + 16 * q, *reinterpret_cast<const uint32_t(*)[16]>(w[q]));
-                }
-            }
             st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);
@@ -767,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     if (warp < 8 && warp / 4 < mt) {
         const int h = warp / 4, r = h * kRows + (warp & 3) * 32 + lane;
         const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + h * 128;
-        float f = Q8 ? exp2f(vref) : 1.0f;
+        float f = kScaled ? exp2f(vref) : 1.0f;
         if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
         float* mine = state + r * L::kJoinPitch;
 #pragma unroll
@@ -834,23 +862,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     cluster.sync();  // no CTA leaves while another reads its state
 }
 
-template <int HD, bool Q8, bool HILO>
-cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
-    using L = PL<HD, Q8, HILO>;
+// f16 copies of the 8-bit pages that the sequences hold: block (s, i) of the copies is page table[s][i], codes without
+// their scales (exact). A CTA per (sequence, page, K or V).
+__global__ void __launch_bounds__(256) paged_copies_kernel(const neko_paged_attention_args a, uint4* copies) {
     const neko_paged_cache& c = a.cache;
-    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
-    PromptPlan p;
-    // two row tiles per CTA unless that leaves SMs without work
-    const int64_t tiles = (rows + kRows - 1) / kRows, heads = int64_t(c.n_seq) * c.n_kv;
-    p.tiles_per = tiles > 1 && heads * ((tiles + 1) / 2) * 2 > num_sms() ? 2 : 1;
-    p.row_tiles = int((tiles + p.tiles_per - 1) / p.tiles_per);
-    const int64_t items = heads * p.row_tiles, key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
-    p.group = a.n_head / c.n_kv;
-    p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
-    p.ranks = 1;
-    while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
-    if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    auto* fn = paged_prompt_kernel<HD, Q8, HILO>;
+    const int slot = blockIdx.x, s = blockIdx.y, v = blockIdx.z;
+    const int page = c.table[int64_t(s) * c.table_stride + slot];
+    if (int64_t(slot) * c.page_size >= a.kv_len[s] || page < 0 || page >= c.num_pages) return;
+    const int pieces = c.n_kv * c.page_size * c.head_dim / 16;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(v ? c.v_pages : c.k_pages) + int64_t(page) * c.page_stride);
+    uint4* dst = copies + (int64_t(v) * c.n_seq * c.max_pages + int64_t(s) * c.max_pages + slot) * pieces * 2;
+    for (int i0 = threadIdx.x; i0 < pieces; i0 += 4 * 256) {
+        uint4 w[4];
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+            if (i0 + 256 * y < pieces) w[y] = ldg_stream(src + i0 + 256 * y);
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            if (i0 + 256 * y >= pieces) break;
+            const uint32_t ws[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
+            uint32_t f[8];
+#pragma unroll
+            for (int z = 0; z < 4; z++) f[2 * z] = e4m3x2_to_f16x2(uint16_t(ws[z])), f[2 * z + 1] = e4m3x2_to_f16x2(uint16_t(ws[z] >> 16));
+            dst[2 * (i0 + 256 * y)] = make_uint4(f[0], f[1], f[2], f[3]);
+            dst[2 * (i0 + 256 * y) + 1] = make_uint4(f[4], f[5], f[6], f[7]);
+        }
+    }
+}
+
+template <int HD, int SRC, bool HILO>
+cudaError_t go(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, const __half* copies, cudaStream_t st) {
+    using L = PL<HD, HILO>;
+    const neko_paged_cache& c = a.cache;
+    auto* fn = paged_prompt_kernel<HD, SRC, HILO>;
     if (cudaError_t e = ensure_dyn_smem(fn, L::kSmem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(items * p.ranks));
@@ -864,23 +908,54 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = p.ranks > 1 ? 1 : 0;
     PromptMaps maps = {};
-    if (!Q8 && (!encode_f16_pages(&maps.k, c.k_pages, HD, c.n_kv * c.page_size, c.num_pages, c.page_stride * 2, c.page_size) ||
-                !encode_f16_pages(&maps.v, c.v_pages, HD, c.n_kv * c.page_size, c.num_pages, c.page_stride * 2, c.page_size)))
-        return cudaErrorNotSupported;
+    if (SRC != kCodes) {
+        const int64_t rows = int64_t(c.n_kv) * c.page_size, own = rows * HD, pages = int64_t(c.n_seq) * c.max_pages;
+        const bool copy = SRC == kCopies;
+        if (!encode_f16_pages(&maps.k, copy ? copies : c.k_pages, HD, rows, copy ? pages : c.num_pages, (copy ? own : c.page_stride) * 2, c.page_size) ||
+            !encode_f16_pages(&maps.v, copy ? copies + pages * own : c.v_pages, HD, rows, copy ? pages : c.num_pages, (copy ? own : c.page_stride) * 2, c.page_size))
+            return cudaErrorNotSupported;
+    }
     return cudaLaunchKernelEx(&cfg, fn, a, p, maps);
 }
 
+template <int HD, int SRC>
+cudaError_t by_type(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, const __half* copies, cudaStream_t st) {
+    return a.type == NEKO_T_F32 ? go<HD, SRC, true>(a, p, items, copies, st) : go<HD, SRC, false>(a, p, items, copies, st);
+}
+
 template <int HD>
-cudaError_t by_type(const neko_paged_attention_args& a, cudaStream_t st) {
-    const bool q8 = a.cache.type == NEKO_T_E4M3, f32 = a.type == NEKO_T_F32;
-    if (q8) return f32 ? go<HD, true, true>(a, st) : go<HD, true, false>(a, st);
-    return f32 ? go<HD, false, true>(a, st) : go<HD, false, false>(a, st);
+cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
+    const neko_paged_cache& c = a.cache;
+    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
+    PromptPlan p;
+    // two row tiles per CTA unless that leaves SMs without work
+    const int64_t tiles = (rows + kRows - 1) / kRows, heads = int64_t(c.n_seq) * c.n_kv;
+    p.tiles_per = tiles > 1 && heads * ((tiles + 1) / 2) * 2 > num_sms() ? 2 : 1;
+    p.row_tiles = int((tiles + p.tiles_per - 1) / p.tiles_per);
+    const int64_t items = heads * p.row_tiles, key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
+    p.group = a.n_head / c.n_kv;
+    p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
+    p.ranks = 1;
+    while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
+    if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, p, items, nullptr, st);
+    // Each CTA would convert its keys again: from kCopyTiles CTAs per (sequence, KV head) on, they are converted once,
+    // if the copies stay below kCopyBytes.
+    const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
+    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes || c.n_seq > 65535) return by_type<HD, kCodes>(a, p, items, nullptr, st);
+    void* mem = nullptr;
+    if (cudaError_t e = scratch_alloc(&mem, size_t(bytes), st); e != cudaSuccess) return e;
+    cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
+                              static_cast<uint4*>(mem));
+    if (e == cudaSuccess) e = by_type<HD, kCopies>(a, p, items, static_cast<const __half*>(mem), st);
+    cudaFreeAsync(mem, st);
+    return e;
 }
 
 }  // namespace
 
 cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st) {
-    return a.cache.head_dim == 64 ? by_type<64>(a, st) : by_type<128>(a, st);
+    return a.cache.head_dim == 64 ? by_source<64>(a, st) : by_source<128>(a, st);
 }
 
 }  // namespace neko

@@ -7,14 +7,16 @@
 // f32 queries are f16 hi + lo in shared memory (S = Qhi K^T + Qlo K^T) and their weights hi + lo in TMEM (P takes
 // exactly the 128 columns of its S); 16-bit queries are one exact f16 and their weights one f16. Rows are scaled by a
 // power of two into f16's range first. Roles:
-//  * warps 0..3 and 4..7: softmax of one row tile each, a thread per row, no shuffles. The reference maximum moves only
+//  * warps 0..7 and 8..15: softmax of one row tile each, two threads per row (64 keys each; two warps more per scheduler
+//    hide each other's latencies), which tell each other their largest scores. The reference maximum moves only
 //    when a score exceeds it by 2^8 (weights up to 2^8 are as exact as any in f16), so O is hardly ever rescaled, and
-//    the row's own thread does that; the tensor core works on the other row tile meanwhile.
-//  * warps 8..10: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
-//    serves K as a K-major and V as an MN-major operand: cp.async for f16 pages, registers and an exact conversion to
+//    the row's own threads do that; the tensor core works on the other row tile meanwhile. A quarter of 16-bit queries'
+//    exponentials is computed on the FMA pipe: the special-function unit is what bounds this step.
+//  * warps 16..18: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
+//    serves K as a K-major and V as an MN-major operand: tensor copies for f16 pages, registers and an exact conversion to
 //    f16 for 8-bit ones (fetched one tile ahead). Scales stay out of the operands: a block's key scale multiplies its
 //    scores and its value scale enters the weights' exponent (the sum takes it out again), 16 columns at a time.
-//  * warp 11, one lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
+//  * warp 19, an elected lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
 // Masks only touch the key tiles that need them. Values that no row sees are zeroed by the loader; values that are not
 // finite in a tile that some row does not see whole are zeroed too and added by the threads of the rows that see them.
 // A cluster of CTAs splits the keys when there are few row tiles and joins over distributed shared memory in rank
@@ -33,7 +35,7 @@ namespace neko {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128;  // of a tile
-constexpr int kThreads = 12 * 32;  // 168 registers a thread: a row's 128 scores stay in them
+constexpr int kSoftWarps = 16, kLoadWarp = 16, kMmaWarp = 19, kThreads = 20 * 32;  // 96 registers a thread
 constexpr int kLoaders = 96;
 constexpr int kCopyTiles = 3;
 constexpr int64_t kCopyBytes = int64_t(1) << 31;
@@ -67,23 +69,25 @@ struct PL {
     static constexpr int kStageOff = kQBytes;
     static constexpr int kMiscOff = kStageOff + kStages * kStage;
     static constexpr int kJoinPitch = HD + 4;             // floats of a row's state: values, maximum, sum
-    static constexpr int kSmem = kMiscOff + 2048 + 1024;  // + alignment
+    static constexpr int kSmem = kMiscOff + 3072 - 128;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
     static_assert(2 * kRows * kJoinPitch * 4 <= kMiscOff, "the joined states take the operands' place");
     static_assert(kStages <= 5, "the ring of scales");
 };
 
 // barriers and small arrays behind the operands
 struct Misc {
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full;
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full, pair[8];
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
     float vtop[kRing];                 // the largest of vs
     uint32_t whole[kRing];             // every block is resident
     uint32_t odd[kOddRing][4];         // of a key tile that needs masks: keys with values that are not finite
-    float qdown[2 * kRows];            // scale / the row's power of two
+    float most[2][2 * kRows];          // by half of the key tile: the rows' largest scores, at the end their sums; before
+                                       // the first tile most[0] is scale / the row's power of two
 };
-static_assert(sizeof(Misc) <= 2048, "misc");
+static_assert(sizeof(Misc) <= 3072 - 128, "misc");
 
 __device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
     // MN-major, 128-byte swizzle: 64-value blocks 16 KB apart (LBO), groups of 8 keys 1024 bytes apart (SBO)
@@ -189,8 +193,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                                                                   const __grid_constant__ PromptMaps maps) {
     constexpr bool kScaled = SRC != kF16Pages, kConvert = SRC == kCodes;
     using L = PL<HD, HILO>;
-    extern __shared__ uint8_t raw[];
-    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t sm[];
+    if (smem_u32(sm) & 1023u) {  // the operands' swizzle goes by address bits
+        if (threadIdx.x == 0) set_device_error(kErrMisalignedSmem);
+        return;
+    }
     Misc& ms = *reinterpret_cast<Misc*>(sm + L::kMiscOff);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const neko_paged_cache& c = a.cache;
@@ -234,13 +241,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
 
     if (tid == 0) {
         for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], kConvert ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
-        for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 128), mbar_init(&ms.pv_done[h], 1);
-        mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders), mbar_init(&ms.q_full, 256);
+        for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 256), mbar_init(&ms.pv_done[h], 1);
+        mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders), mbar_init(&ms.q_full, 32 * kSoftWarps);
+        for (int i = 0; i < 8; i++) mbar_init(&ms.pair[i], 2);
         ms.fail = 0;
         for (int i = 0; i < 8; i++) ms.odd[i / 4][i % 4] = 0;  // tiles 0 and 1
         fence_barrier_init();
     }
-    if (warp == 11) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -252,9 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     volatile uint32_t* fail = &ms.fail;
 
     float row_max = -INFINITY, row_sum = 0.0f, vref = 0.0f;  // of a softmax thread's row; vref: log2 of O's unit
-    if (warp >= 8 && warp < 11) {
+    if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ------------------------------------------------------------------ loader
-        const int lt = tid - 256;
+        const int lt = tid - 32 * kLoadWarp;
         const int32_t* table = c.table + int64_t(s) * c.table_stride;
         const int ps_log = 31 - __clz(c.page_size);
         const int total = 2 * nt;  // items K0 V0 K1 V1 ..
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 uint8_t* base = sm + L::kStageOff + st * L::kStage + place;
                 if (!v) {
-                    if (warp == 8) {
+                    if (warp == kLoadWarp) {
                         const float vl = lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone, vt = warp_max(vl);
                         const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0);
                         if (lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? fabsf(ks) : kGone, ms.vs[i % kRing][lane] = vl;
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             int scans = 0;
             float ks = 0.0f, vs = 0.0f;
             auto scales = [&]() {
-                if (SRC == kCopies && warp == 8 && pages >= 0) {
+                if (SRC == kCopies && warp == kLoadWarp && pages >= 0) {
                     ks = c.k_scale[int64_t(pages) * c.scale_stride + kvh];
                     vs = c.v_scale[int64_t(pages) * c.scale_stride + kvh];
                 }
@@ -380,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 uint8_t* base = sm + L::kStageOff + st * L::kStage;
                 const bool strict = !open(j0, pos_lo, pos_hi);
                 const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0), scan = v && (strict || !whole);
-                if (warp == 8) {
+                if (warp == kLoadWarp) {
                     if (x >= L::kStages) {
                         ok = wait_on(&ms.empty[st], ((x / L::kStages) & 1) ^ 1, fail);
                         ok = __all_sync(0xffffffffu, ok);
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     fence_proxy_async();
                     mbar_arrive(&ms.scanned);
-                    if (warp == 8) {
+                    if (warp == kLoadWarp) {
                         ok = wait_on(&ms.scanned, scans & 1, fail);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
@@ -441,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
             }
         }
-    } else if (warp == 11) {
+    } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------------ UMMA issue
         // The whole warp walks the loop and one elected lane issues: with the role on a single lane of a divergent warp the
         // operands' descriptors went through vector registers, about 70 cycles an UMMA.
@@ -464,13 +472,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
             };
             auto issue_pv = [&](int h, int st) {
-                // weights of keys 16 k ..: f16 columns 8 k; hi + lo: 32-column groups of hi, lo (16 each)
+                // weights of keys 16 k ..: each thread's over its own scores; hi + lo: 32-column groups of hi, lo (16 each)
                 const uint32_t p = tmem + h * 128, o = tmem + 256 + h * 128;
                 const uint64_t vd = vv_desc + uint64_t(st * (L::kStage >> 4));
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; k++) {
-                        const uint32_t col = HILO ? 32 * (k / 2) + 8 * (k % 2) : 8 * k;
+                        const uint32_t col = HILO ? 32 * (k / 2) + 8 * (k % 2) : 64 * (k / 4) + 8 * (k % 4);
                         umma_ts(o, p + col, vd + k * (2048 >> 4), idesc_o);
                         if constexpr (HILO) umma_ts(o, p + col + 16, vd + k * (2048 >> 4), idesc_o);
                     }
@@ -519,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         constexpr int E = HD / 8;
         const auto load_q = [&](auto* base) {
 #pragma unroll 2
-            for (int r = warp * 4 + (lane >> 3); r < mt * kRows; r += 32) {
+            for (int r = warp * 4 + (lane >> 3); r < mt * kRows; r += 4 * kSoftWarps) {
                 float x[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) x[e] = 0.0f;
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     *reinterpret_cast<uint4*>(dst + at) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
                     if constexpr (HILO) *reinterpret_cast<uint4*>(dst + L::kQTile + at) = make_uint4(l2[0], l2[1], l2[2], l2[3]);
                 }
-                if ((lane & 7) == 0) ms.qdown[r] = a.scale / up;
+                if ((lane & 7) == 0) ms.most[0][r] = a.scale / up;
             }
         };
         if constexpr (HILO) load_q(static_cast<const float*>(a.q));
@@ -556,12 +564,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         fence_proxy_async();
         mbar_arrive(&ms.q_full);
     }
-    if (warp < 8 && warp / 4 < mt) {
-        // ------------------------------------------------------------------ softmax, a thread per row
-        const int h = warp / 4;
+    const int half_w = warp / 8, col_w = (warp >> 2) & 1;  // of a softmax warp: row tile and half of the key tile
+    const int row_w = half_w * kRows + (warp & 3) * 32 + lane;
+    if (warp < kSoftWarps && half_w < mt) {
+        // ------------------------------------------------------------------ softmax, two threads per row
+        const int h = half_w, r = row_w, pr = r0 + r;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + h * 128, to = tmem + lanes + 256 + h * 128;
-        const int r = h * kRows + (warp & 3) * 32 + lane, pr = r0 + r;
+        const uint32_t ts = tmem + lanes + h * 128, to = tmem + lanes + 256 + h * 128 + col_w * (HD / 2);
         const bool real = r < rows;
         const int rt = over_g(pr), qpos = real ? held - n + rt : kNoRow;
         const float slope = a.slopes && real ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
@@ -572,12 +581,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
 #pragma unroll
             for (int x = 0; x < 32; x++) z[x] = 0;
 #pragma unroll
-            for (int x = 0; x < HD; x += 32) st32(to + x, z);
+            for (int x = 0; x < HD / 2; x += 32) st32(to + x, z);
             st_wait();
         }
         bool ok = __all_sync(0xffffffffu, wait_on(&ms.q_full, 0, fail));
         // from the accumulator to log2 units, or with a cap to the tanh's argument
-        const float factor = a.softcap > 0.0f ? ms.qdown[r] / a.softcap : ms.qdown[r] * kLog2e;
+        const float factor = a.softcap > 0.0f ? ms.most[0][r] / a.softcap : ms.most[0][r] * kLog2e;
+        // both threads of a row have read it before either writes (a wait of its own for each exchange: phase 0)
+        uint64_t* pair = &ms.pair[4 * h + (warp & 3)];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        ok = __all_sync(0xffffffffu, ok && wait_on(pair, 0, fail));
         for (int i = 0; i < nt && ok; i++) {
             const int j0 = key_of(i);
             ok = wait_on(&ms.s_full[h], i & 1, fail);
@@ -597,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const uint32_t* od = ms.odd[i % kOddRing];
                 odd_tile = (od[0] | od[1] | od[2] | od[3]) != 0;
             }
-            // O times f for this thread's row, and this tile's values that are not finite
+            // this thread's half of its row of O times f, and this tile's values that are not finite
             auto fix_o = [&](float f, bool odd) {
                 if (i > 0) {
                     ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
@@ -606,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     tc_fence_after();
                 }
 #pragma unroll 1
-                for (int x = 0; x < HD; x += 32) {
+                for (int x = 0; x < HD / 2; x += 32) {
                     uint32_t o[32];
                     ld32(to + x, o);
                     ld_wait(o);
@@ -620,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             if (j >= len || ksp[key >> 4] == kGone) continue;
                             const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
                             const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
-                                               (int64_t(kvh) * c.page_size + j % c.page_size) * HD + x;
+                                               (int64_t(kvh) * c.page_size + j % c.page_size) * HD + col_w * (HD / 2) + x;
 #pragma unroll
                             for (int y = 0; y < 32; y++) {
                                 float v;
@@ -644,118 +658,113 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 if (!ok) break;
                 if (v_up) vref = vnow;
             }
-            // ---- 32 keys at a time, in a rolled loop (as straight code it was bound by instruction fetch)
-            uint32_t ahead[32];
-            ld32(ts, ahead);
+            // ---- this thread's 64 scores, 32 at a time in rolled loops: the largest; with a cap, a bias or masks, the scores
+            // in log2 units back into TMEM
+            const float *kb = ksp + 4 * col_w, *vb = vsp + 4 * col_w;  // of their blocks of 16
+            const uint32_t tc = ts + 64 * col_w;
+            const bool shaped = a.softcap > 0.0f || a.slopes || !plain_mask || a.scale < 0.0f;
+            float top = -INFINITY;
 #pragma unroll 1
-            for (int q = 0; q < 4; q++) {
+            for (int q = 0; q < 2; q++) {
                 uint32_t u[32];
-                ld_wait(ahead);
-#pragma unroll
-                for (int x = 0; x < 32; x++) u[x] = ahead[x];
-                if (q < 3) ld32(ts + 32 * (q + 1), ahead);
-                float f0 = kScaled ? factor * ksp[2 * q] : factor, f1 = kScaled ? factor * ksp[2 * q + 1] : factor;
-                const float ks0 = ksp[2 * q], ks1 = ksp[2 * q + 1];
-                if (a.softcap > 0.0f) {  // y = score / cap
+                ld32(tc + 32 * q, u);
+                const float f0 = kScaled ? factor * fabsf(kb[2 * q]) : factor, f1 = kScaled ? factor * fabsf(kb[2 * q + 1]) : factor;
+                ld_wait(u);
+                if (shaped) {
+                    const int jq = j0 + 64 * col_w + 32 * q;
                     float most = 0.0f;
 #pragma unroll
                     for (int x = 0; x < 32; x++) {
                         u[x] = __float_as_uint(__uint_as_float(u[x]) * (x < 16 ? f0 : f1));
                         most = max_nan(most, fabsf(__uint_as_float(u[x])));
                     }
-                    if (__all_sync(0xffffffffu, most <= 0.5f)) {
-                        // an odd polynomial of degree 9 (least maximum error on [-1/2, 1/2]: 3e-9): two units of the
-                        // special functions less than below
+                    if (a.softcap > 0.0f) {  // of score / cap
+                        if (__all_sync(0xffffffffu, most <= 0.5f)) {
+                            // an odd polynomial of degree 9 (least maximum error on [-1/2, 1/2]: 3e-9): two units of the
+                            // special functions less than below
 #pragma unroll
-                        for (int x = 0; x < 32; x += 2) {
-                            const uint64_t y = pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), y2 = mul2(y, y);
-                            uint64_t p = fma2(y2, pack2(0.016737453639507294f, 0.016737453639507294f), pack2(-0.05276207625865936f, -0.05276207625865936f));
-                            p = fma2(p, y2, pack2(0.13320569694042206f, 0.13320569694042206f));
-                            p = fma2(p, y2, pack2(-0.3333277702331543f, -0.3333277702331543f));
-                            p = fma2(p, y2, pack2(0.9999999403953552f, 0.9999999403953552f));
-                            p = mul2(mul2(p, y), pack2(cap, cap));
-                            float p0, p1;
-                            unpack2(p, p0, p1);
-                            u[x] = __float_as_uint(p0), u[x + 1] = __float_as_uint(p1);
-                        }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(cap * tanh_abs(__uint_as_float(u[x])));
-                    }
-                    f0 = f1 = 1.0f;
-                }
-                const int jq = j0 + 32 * q;
-                if (a.slopes) {
-#pragma unroll
-                    for (int x = 0; x < 32; x++)
-                        u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x]) * (x < 16 ? f0 : f1)));
-                    f0 = f1 = 1.0f;
-                }
-                if (!plain_mask || a.scale < 0.0f) {
-                    // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
-                    const int see_hi = plain_mask ? len : min(len, qpos + 1), see_lo = a.window && !plain_mask ? qpos - a.window + 1 : 0;
-                    const int pre = real ? prefix : 0;
-#pragma unroll
-                    for (int x = 0; x < 32; x++) {
-                        const int j = jq + x;
-                        const bool see = ((j < see_hi && j >= see_lo) || j < pre) && (x < 16 ? ks0 : ks1) != kGone;
-                        u[x] = see ? __float_as_uint(__uint_as_float(u[x]) * (x < 16 ? f0 : f1)) : 0xff800000u;
-                    }
-                    f0 = f1 = 1.0f;
-                }
-                // the largest score in log2 units
-                float m[8];
-#pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    const float v = __uint_as_float(u[x]);
-                    float& mm = m[(x & 3) + (x & 16) / 4];
-                    mm = (x & 15) < 4 ? v : max_nan(mm, v);
-                }
-                const float top = max_nan(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * f0,
-                                          max_nan(max_nan(m[4], m[5]), max_nan(m[6], m[7])) * f1);
-                if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
-                const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
-                if (__any_sync(0xffffffffu, up)) {
-                    // the reference maximum moves up to the next whole number: O, the sum and this tile's weights so far
-                    // follow, by a power of two
-                    float f = 1.0f;
-                    if (up) {
-                        const float to_max = ceilf(top);
-                        f = ex2(row_max - to_max);  // row_max = -inf: nothing there yet, 0
-                        row_max = to_max;
-                        row_sum *= f;
-                    }
-                    if (i > 0) fix_o(f, false);
-                    if (!ok) break;
-                    const __half2 fh = __float2half2_rn(f);
-                    for (int x = 0; x < (HILO ? q : q / 2 + q % 2); x++) {  // the columns that hold weights by now
-                        uint32_t o[32];
-                        ld32(ts + 32 * x, o);
-                        ld_wait(o);
-#pragma unroll
-                        for (int y = 0; y < 32; y++) {
-                            if (HILO || 32 * x + y < 16 * q) {
-                                const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&o[y]), fh);
-                                o[y] = *reinterpret_cast<const uint32_t*>(&v);
+                            for (int x = 0; x < 32; x += 2) {
+                                const uint64_t y = pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), y2 = mul2(y, y);
+                                uint64_t p = fma2(y2, pack2(0.016737453639507294f, 0.016737453639507294f), pack2(-0.05276207625865936f, -0.05276207625865936f));
+                                p = fma2(p, y2, pack2(0.13320569694042206f, 0.13320569694042206f));
+                                p = fma2(p, y2, pack2(-0.3333277702331543f, -0.3333277702331543f));
+                                p = fma2(p, y2, pack2(0.9999999403953552f, 0.9999999403953552f));
+                                p = mul2(mul2(p, y), pack2(cap, cap));
+                                float p0, p1;
+                                unpack2(p, p0, p1);
+                                u[x] = __float_as_uint(p0), u[x + 1] = __float_as_uint(p1);
                             }
-                        }
-                        if (HILO || 2 * x + 2 <= q) st32(ts + 32 * x, o);
-                        else st16(ts + 32 * x, *reinterpret_cast<const uint32_t(*)[16]>(o));
-                    }
-                    st_wait();
-                }
-                // weights, their sum; P over S
-                const float ref = row_max == -INFINITY ? 0.0f : row_max;
-                uint64_t sums[2] = {0, 0};
-                uint32_t p_hi[16], p_lo[HILO ? 16 : 1];
+                        } else {
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const float f = g ? f1 : f0;
-                    const float vr = kScaled ? fmaxf(vsp[2 * q + g] - vref, kVMin) : 0.0f;
-                    const uint64_t ff = pack2(f, f), off = pack2(vr - ref, vr - ref);
+                            for (int x = 0; x < 32; x++) u[x] = __float_as_uint(cap * tanh_abs(__uint_as_float(u[x])));
+                        }
+                    }
+                    if (a.slopes) {
+#pragma unroll
+                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x])));
+                    }
+                    if (!plain_mask) {
+                        // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
+                        const int see_hi = min(len, qpos + 1) - jq, see_lo = (a.window ? qpos - a.window + 1 : 0) - jq;
+                        const int pre = (real ? prefix : 0) - jq;
+                        const bool gone0 = kb[2 * q] == kGone, gone1 = kb[2 * q + 1] == kGone;
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (!((x < see_hi && x >= see_lo) || x < pre) || (x < 16 ? gone0 : gone1)) u[x] = 0xff800000u;
+                    }
+                    st32(tc + 32 * q, u);
+                }
+                float m[4];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const float v = __uint_as_float(u[16 * b + x]);
+                        m[x & 3] = x < 4 ? v : max_nan(m[x & 3], v);
+                    }
+                    top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * (shaped ? 1.0f : b ? f1 : f0));
+                }
+            }
+            if (shaped) st_wait();
+            // One buffer: this tile's scores exist, so the other thread has handed in its last weights and read this one's.
+            ms.most[col_w][r] = top;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pair);
+            ok = wait_on(pair, (i + 1) & 1, fail);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            top = max_nan(top, ms.most[col_w ^ 1][r]);
+            if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
+            // the reference moves only when a score exceeds it by more than 2^8 (the same decision in both warps of a row)
+            const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
+            if (__any_sync(0xffffffffu, up)) {
+                float f = 1.0f;
+                if (up) {
+                    f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
+                    row_max = top;
+                    row_sum *= f;
+                }
+                if (i > 0) fix_o(f, false);
+                if (!ok) break;
+            }
+            // ---- weights, their sum; P over this thread's scores
+            const float ref = row_max == -INFINITY ? 0.0f : row_max;
+#pragma unroll 1
+            for (int q = 0; q < 2; q++) {
+                uint32_t u[32], p_hi[16];
+                [[maybe_unused]] uint32_t p_lo[16];
+                ld32(tc + 32 * q, u);
+                uint64_t sums[2] = {0, 0};
+                const float f0 = shaped ? 1.0f : kScaled ? factor * kb[2 * q] : factor, f1 = shaped ? 1.0f : kScaled ? factor * kb[2 * q + 1] : factor;
+                const float v0 = kScaled ? fmaxf(vb[2 * q] - vref, kVMin) : 0.0f, v1 = kScaled ? fmaxf(vb[2 * q + 1] - vref, kVMin) : 0.0f;
+                ld_wait(u);
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const float vr = b ? v1 : v0;
+                    const uint64_t ff = b ? pack2(f1, f1) : pack2(f0, f0), off = pack2(vr - ref, vr - ref);
                     if (kScaled) sums[0] = sums[1] = 0;
 #pragma unroll
-                    for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                    for (int x = 16 * b; x < 16 * b + 16; x += 2) {
                         float z0, z1;
                         unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
                         if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
@@ -764,20 +773,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                         if constexpr (HILO) split_hilo(z0, z1, p_hi[x / 2], p_lo[x / 2]);
                         else p_hi[x / 2] = h2u(__floats2half2_rn(z0, z1));
                     }
-                    if (kScaled || g) {  // the sum without the value scale
+                    if (kScaled || b) {  // the sum without the value scale
                         float z0, z1;
                         unpack2(add2(sums[0], sums[1]), z0, z1);
                         row_sum = kScaled ? fmaf(z0 + z1, ex2(-vr), row_sum) : row_sum + (z0 + z1);
                     }
                 }
-                if constexpr (HILO) {
-                    st16(ts + 32 * q, p_hi);
-                    st16(ts + 32 * q + 16, p_lo);
-                } else {
-                    st16(ts + 16 * q, p_hi);
-                }
+                st16(tc + (HILO ? 32 : 16) * q, p_hi);
+                if constexpr (HILO) st16(tc + 32 * q + 16, p_lo);
             }
-            if (!ok) break;
             st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);
@@ -789,17 +793,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     }
     // ---- the outputs: everything is read out of TMEM before the operands' memory is used again
     __syncwarp();
+    if (warp < kSoftWarps && half_w < mt) ms.most[col_w][row_w] = row_sum;
     __syncthreads();
     const bool alone = plan.ranks == 1;
     float* state = reinterpret_cast<float*>(sm);  // [row][values, maximum, sum]
-    if (warp < 8 && warp / 4 < mt) {
-        const int h = warp / 4, r = h * kRows + (warp & 3) * 32 + lane;
-        const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + h * 128;
+    if (warp < kSoftWarps && half_w < mt) {
+        const int r = row_w;
+        const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + half_w * 128 + col_w * (HD / 2);
+        row_sum += ms.most[col_w ^ 1][r];
         float f = kScaled ? exp2f(vref) : 1.0f;
         if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
         float* mine = state + r * L::kJoinPitch;
 #pragma unroll
-        for (int x = 0; x < HD; x += 32) {
+        for (int x = 0; x < HD / 2; x += 32) {
             uint32_t w[32];
             ld32(to + x, w);
             ld_wait(w);
@@ -808,15 +814,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 float4 v = make_float4(__uint_as_float(w[y]) * f, __uint_as_float(w[y + 1]) * f, __uint_as_float(w[y + 2]) * f,
                                        __uint_as_float(w[y + 3]) * f);
                 if (alone && row_sum == 0.0f) v = make_float4(0, 0, 0, 0);
-                *reinterpret_cast<float4*>(mine + x + y) = v;
+                *reinterpret_cast<float4*>(mine + col_w * (HD / 2) + x + y) = v;
             }
         }
-        mine[HD] = row_max;
-        mine[HD + 1] = row_sum;
+        if (!col_w) mine[HD] = row_max, mine[HD + 1] = row_sum;
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     auto put = [&](int r, int d, float4 v) {
         const int pr = r0 + r;
         const int rt = over_g(pr);

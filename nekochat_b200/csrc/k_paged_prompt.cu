@@ -77,7 +77,7 @@ struct PL {
 
 // barriers and small arrays behind the operands
 struct Misc {
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full, pair[8];
+    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full;
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
@@ -125,6 +125,22 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&v)[16]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+#define NEKO_R16(r)                                                                                                  \
+    "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),      \
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : NEKO_R16(r)
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ld_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : NEKO_R16(r)::"memory");
+}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -157,7 +173,7 @@ __device__ __forceinline__ void exp2_poly(float& x, float& y) {
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile uint32_t* fail) {
     for (uint32_t i = 0; i < kMbarMaxTries; i++) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63) == 63 && *fail) return false;
+        if ((i & 7) == 7 && *fail) return false;
     }
     *fail = 1;
     set_device_error(kErrMbarTimeout);
@@ -243,7 +259,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         for (int i = 0; i < L::kStages; i++) mbar_init(&ms.full[i], kConvert ? kLoaders : 1), mbar_init(&ms.empty[i], 1);
         for (int h = 0; h < 2; h++) mbar_init(&ms.s_full[h], 1), mbar_init(&ms.p_full[h], 256), mbar_init(&ms.pv_done[h], 1);
         mbar_init(&ms.drain, 1), mbar_init(&ms.land, 1), mbar_init(&ms.scanned, kLoaders), mbar_init(&ms.q_full, 32 * kSoftWarps);
-        for (int i = 0; i < 8; i++) mbar_init(&ms.pair[i], 2);
         ms.fail = 0;
         for (int i = 0; i < 8; i++) ms.odd[i / 4][i % 4] = 0;  // tiles 0 and 1
         fence_barrier_init();
@@ -584,48 +599,45 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             for (int x = 0; x < HD / 2; x += 32) st32(to + x, z);
             st_wait();
         }
-        bool ok = __all_sync(0xffffffffu, wait_on(&ms.q_full, 0, fail));
+        wait_on(&ms.q_full, 0, fail);
+        __syncwarp();
         // from the accumulator to log2 units, or with a cap to the tanh's argument
         const float factor = a.softcap > 0.0f ? ms.most[0][r] / a.softcap : ms.most[0][r] * kLog2e;
-        // both threads of a row have read it before either writes (a wait of its own for each exchange: phase 0)
-        uint64_t* pair = &ms.pair[4 * h + (warp & 3)];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pair);
-        ok = __all_sync(0xffffffffu, ok && wait_on(pair, 0, fail));
-        for (int i = 0; i < nt && ok; i++) {
+        // The two warps of 32 rows meet at a named barrier of theirs: no wait of this role ends it early (a wait that gives up
+        // has set the fail flag, and every later one returns at once), so both always come to every meeting.
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * h + (warp & 3)) : "memory"); };
+        meet();  // both threads of a row have read its factor before either writes
+        for (int i = 0; i < nt; i++) {
             const int j0 = key_of(i);
-            ok = wait_on(&ms.s_full[h], i & 1, fail);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
+            const bool open_rows = open(j0, h_lo, h_hi), open_cta = open(j0, pos_lo, pos_hi);
             const float* ksp = ms.ks[i % kRing];
             const float* vsp = ms.vs[i % kRing];
-            const bool plain_mask = open(j0, h_lo, h_hi) && ms.whole[i % kRing];
-            const float vnow = kScaled ? ms.vtop[i % kRing] : 0.0f;
+            wait_on(&ms.s_full[h], i & 1, fail);
+            __syncwarp();
+            tc_fence_after();
+            const bool plain_mask = open_rows && ms.whole[i % kRing];
             const int xv = 2 * i + 1, stv = xv % L::kStages;
             bool odd_tile = false;
-            if (!open(j0, pos_lo, pos_hi)) {
-                ok = wait_on(&ms.full[stv], (xv / L::kStages) & 1, fail);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+            if (!open_cta) {
+                wait_on(&ms.full[stv], (xv / L::kStages) & 1, fail);
+                __syncwarp();
                 const uint32_t* od = ms.odd[i % kOddRing];
                 odd_tile = (od[0] | od[1] | od[2] | od[3]) != 0;
             }
             // this thread's half of its row of O times f, and this tile's values that are not finite
             auto fix_o = [&](float f, bool odd) {
                 if (i > 0) {
-                    ok = wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return;
+                    wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
+                    __syncwarp();
                     tc_fence_after();
                 }
 #pragma unroll 1
-                for (int x = 0; x < HD / 2; x += 32) {
-                    uint32_t o[32];
-                    ld32(to + x, o);
-                    ld_wait(o);
+                for (int x = 0; x < HD / 2; x += 16) {
+                    uint32_t o[16];
+                    ld16(to + x, o);
+                    ld_wait16(o);
 #pragma unroll
-                    for (int y = 0; y < 32; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                    for (int y = 0; y < 16; y++) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
                     if (odd) {
 #pragma unroll 1
                         for (int key = 0; key < kKeys; key++) {
@@ -636,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
                                                (int64_t(kvh) * c.page_size + j % c.page_size) * HD + col_w * (HD / 2) + x;
 #pragma unroll
-                            for (int y = 0; y < 32; y++) {
+                            for (int y = 0; y < 16; y++) {
                                 float v;
                                 if constexpr (kScaled) {
                                     v = (static_cast<const uint8_t*>(c.v_pages)[at + y] & 0x7f) == 0x7f ? NAN : 0.0f;
@@ -648,29 +660,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             }
                         }
                     }
-                    st32(to + x, o);
+                    st16(to + x, o);
                 }
                 st_wait();
             };
-            {
+            if (kScaled || odd_tile) {
+                const float vnow = kScaled ? ms.vtop[i % kRing] : 0.0f;
                 const bool v_up = kScaled && (i == 0 || vnow > vref + kVLazy);
                 if (odd_tile || (v_up && i > 0)) fix_o(v_up && i > 0 ? ex2(vref - vnow) : 1.0f, odd_tile);
-                if (!ok) break;
                 if (v_up) vref = vnow;
             }
-            // ---- this thread's 64 scores, 32 at a time in rolled loops: the largest; with a cap, a bias or masks, the scores
-            // in log2 units back into TMEM
-            const float *kb = ksp + 4 * col_w, *vb = vsp + 4 * col_w;  // of their blocks of 16
+            // ---- tiles that need more than the scale: a cap, a bias, masks; 32 scores at a time in a rolled loop, in log2 units
+            // back into TMEM
+            const float *kb = ksp + 4 * col_w, *vb = vsp + 4 * col_w;  // of this thread's blocks of 16 keys
             const uint32_t tc = ts + 64 * col_w;
             const bool shaped = a.softcap > 0.0f || a.slopes || !plain_mask || a.scale < 0.0f;
-            float top = -INFINITY;
+            if (shaped) {
 #pragma unroll 1
-            for (int q = 0; q < 2; q++) {
-                uint32_t u[32];
-                ld32(tc + 32 * q, u);
-                const float f0 = kScaled ? factor * fabsf(kb[2 * q]) : factor, f1 = kScaled ? factor * fabsf(kb[2 * q + 1]) : factor;
-                ld_wait(u);
-                if (shaped) {
+                for (int q = 0; q < 2; q++) {
+                    uint32_t u[32];
+                    ld32(tc + 32 * q, u);
+                    const float f0 = kScaled ? factor * fabsf(kb[2 * q]) : factor, f1 = kScaled ? factor * fabsf(kb[2 * q + 1]) : factor;
+                    ld_wait(u);
                     const int jq = j0 + 64 * col_w + 32 * q;
                     float most = 0.0f;
 #pragma unroll
@@ -714,25 +725,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     st32(tc + 32 * q, u);
                 }
+                st_wait();
+            }
+            // ---- this thread's 64 scores and the largest of them
+            uint32_t u[2][32];
+            ld32(tc, u[0]);
+            ld32(tc + 32, u[1]);
+            float fb[4];  // what brings them to log2 units
+#pragma unroll
+            for (int b = 0; b < 4; b++) fb[b] = shaped ? 1.0f : kScaled ? factor * kb[b] : factor;
+            ld_wait(u[0]), ld_wait(u[1]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
                 float m[4];
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float v = __uint_as_float(u[16 * b + x]);
-                        m[x & 3] = x < 4 ? v : max_nan(m[x & 3], v);
-                    }
-                    top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * (shaped ? 1.0f : b ? f1 : f0));
+                for (int x = 0; x < 16; x++) {
+                    const float v = __uint_as_float(u[b / 2][16 * (b & 1) + x]);
+                    m[x & 3] = x < 4 ? v : max_nan(m[x & 3], v);
                 }
+                top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * fb[b]);
             }
-            if (shaped) st_wait();
             // One buffer: this tile's scores exist, so the other thread has handed in its last weights and read this one's.
             ms.most[col_w][r] = top;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(pair);
-            ok = wait_on(pair, (i + 1) & 1, fail);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            meet();
             top = max_nan(top, ms.most[col_w ^ 1][r]);
             if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
             // the reference moves only when a score exceeds it by more than 2^8 (the same decision in both warps of a row)
@@ -745,49 +761,47 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     row_sum *= f;
                 }
                 if (i > 0) fix_o(f, false);
-                if (!ok) break;
             }
             // ---- weights, their sum; P over this thread's scores
             const float ref = row_max == -INFINITY ? 0.0f : row_max;
-#pragma unroll 1
-            for (int q = 0; q < 2; q++) {
-                uint32_t u[32], p_hi[16];
-                [[maybe_unused]] uint32_t p_lo[16];
-                ld32(tc + 32 * q, u);
-                uint64_t sums[2] = {0, 0};
-                const float f0 = shaped ? 1.0f : kScaled ? factor * kb[2 * q] : factor, f1 = shaped ? 1.0f : kScaled ? factor * kb[2 * q + 1] : factor;
-                const float v0 = kScaled ? fmaxf(vb[2 * q] - vref, kVMin) : 0.0f, v1 = kScaled ? fmaxf(vb[2 * q + 1] - vref, kVMin) : 0.0f;
-                ld_wait(u);
+            uint64_t sums[2] = {0, 0};
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const float vr = b ? v1 : v0;
-                    const uint64_t ff = b ? pack2(f1, f1) : pack2(f0, f0), off = pack2(vr - ref, vr - ref);
-                    if (kScaled) sums[0] = sums[1] = 0;
+            for (int b = 0; b < 4; b++) {
+                const int q = b / 2, g = b & 1;
+                const float vr = kScaled ? fmaxf(vb[b] - vref, kVMin) : 0.0f;
+                const uint64_t ff = pack2(fb[b], fb[b]), off = pack2(vr - ref, vr - ref);
+                if (kScaled) sums[0] = sums[1] = 0;
+                [[maybe_unused]] uint32_t lo8[8];
 #pragma unroll
-                    for (int x = 16 * b; x < 16 * b + 16; x += 2) {
-                        float z0, z1;
-                        unpack2(fma2(pack2(__uint_as_float(u[x]), __uint_as_float(u[x + 1])), ff, off), z0, z1);
-                        if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
-                        else z0 = ex2(z0), z1 = ex2(z1);
-                        sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
-                        if constexpr (HILO) split_hilo(z0, z1, p_hi[x / 2], p_lo[x / 2]);
-                        else p_hi[x / 2] = h2u(__floats2half2_rn(z0, z1));
-                    }
-                    if (kScaled || b) {  // the sum without the value scale
-                        float z0, z1;
-                        unpack2(add2(sums[0], sums[1]), z0, z1);
-                        row_sum = kScaled ? fmaf(z0 + z1, ex2(-vr), row_sum) : row_sum + (z0 + z1);
-                    }
+                for (int x = 16 * g; x < 16 * g + 16; x += 2) {
+                    float z0, z1;
+                    unpack2(fma2(pack2(__uint_as_float(u[q][x]), __uint_as_float(u[q][x + 1])), ff, off), z0, z1);
+                    if (!HILO && (x & 7) == 6) exp2_poly(z0, z1);
+                    else z0 = ex2(z0), z1 = ex2(z1);
+                    sums[x / 2 & 1] = add2(sums[x / 2 & 1], pack2(z0, z1));
+                    // f16 weights in the scores' registers
+                    if constexpr (HILO) split_hilo(z0, z1, u[q][16 * g + (x & 15) / 2], lo8[(x & 15) / 2]);
+                    else u[q][x / 2] = h2u(__floats2half2_rn(z0, z1));
                 }
-                st16(tc + (HILO ? 32 : 16) * q, p_hi);
-                if constexpr (HILO) st16(tc + 32 * q + 16, p_lo);
+                if constexpr (HILO) {
+                    st8(tc + 32 * q + 8 * g, &u[q][16 * g]);
+                    st8(tc + 32 * q + 16 + 8 * g, lo8);
+                } else if (g) {
+                    st16(tc + 16 * q, *reinterpret_cast<const uint32_t(*)[16]>(u[q]));
+                }
+                if (kScaled || b == 3) {  // the sum without the value scale
+                    float z0, z1;
+                    unpack2(add2(sums[0], sums[1]), z0, z1);
+                    row_sum = kScaled ? fmaf(z0 + z1, ex2(-vr), row_sum) : row_sum + (z0 + z1);
+                }
             }
             st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);
         }
-        if (ok && nt > 0) {
-            ok = wait_on(&ms.pv_done[h], (nt - 1) & 1, fail);
+        if (nt > 0) {
+            wait_on(&ms.pv_done[h], (nt - 1) & 1, fail);
+            __syncwarp();
             tc_fence_after();
         }
     }

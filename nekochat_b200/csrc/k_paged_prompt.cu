@@ -430,22 +430,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     ok = wait_on(&ms.land, scans & 1, fail);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    // a thread per key row: rows that nobody holds are zeroed, values that are not finite taken out
-                    for (int r = lt; r < kKeys + 64; r += kLoaders) {  // whole warps: 96 rows, then 32 and nothing
-                        const bool dead = __shfl_sync(0xffffffffu, pages, (r >> 4) & 7) < 0 || j0 + r >= len;
-                        if (r >= kKeys) continue;
-                        bool odd = false;
-                        for (int h = 0; h < HD / 64; h++)
-                            for (int ch = 0; ch < 8; ch++) {
-                                uint4* p = reinterpret_cast<uint4*>(base + h * L::kHalf + sw128_off(r, ch));
-                                if (dead) {
-                                    *p = make_uint4(0, 0, 0, 0);
-                                } else if (strict) {
-                                    uint4 u = *p;
-                                    if (drop_odd(u)) *p = u, odd = true;
-                                }
-                            }
-                        if (odd) atomicOr(&ms.odd[i % kOddRing][r >> 5], 1u << (r & 31));
+                    // rows that nobody holds are zeroed, values that are not finite taken out
+                    uint32_t held_rows = 0;  // lane x < 8: rows of block x that are held
+                    if (lane < 8 && pages >= 0) held_rows = uint32_t(min(max(len - j0 - 16 * lane, 0), 16));
+                    constexpr int kChunks = HD / 8;  // 16-byte pieces of a key row
+#pragma unroll 4
+                    for (int k = 0; k < (kKeys * kChunks + kLoaders - 1) / kLoaders; k++) {  // as often for every lane
+                        const int y = lt + k * kLoaders, r = y / kChunks, ch = y % kChunks;
+                        const uint32_t held16 = __shfl_sync(0xffffffffu, held_rows, (r >> 4) & 7);
+                        if (r < kKeys) {
+                            uint4* p = reinterpret_cast<uint4*>(base + ch / 8 * L::kHalf + sw128_off(r, ch % 8));
+                            uint4 u = (r & 15) < int(held16) ? *p : make_uint4(0, 0, 0, 0);
+                            const bool odd = strict && drop_odd(u);
+                            if (odd || (r & 15) >= int(held16)) *p = u;
+                            if (odd) atomicOr(&ms.odd[i % kOddRing][r >> 5], 1u << (r & 31));
+                        }
                     }
                     fence_proxy_async();
                     mbar_arrive(&ms.scanned);
@@ -805,19 +804,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             tc_fence_after();
         }
     }
-    // ---- the outputs: everything is read out of TMEM before the operands' memory is used again
+    // ---- the outputs. Alone: through shared memory, once the operands are used up. In a cluster each CTA owns a share of
+    // the rows: every CTA pushes its states of them into the owner's shared memory.
     __syncwarp();
     if (warp < kSoftWarps && half_w < mt) ms.most[col_w][row_w] = row_sum;
-    __syncthreads();
     const bool alone = plan.ranks == 1;
-    float* state = reinterpret_cast<float*>(sm);  // [row][values, maximum, sum]
+    cg::cluster_group cluster = cg::this_cluster();
+    if (alone) __syncthreads();
+    else cluster.sync();
+    float* state = reinterpret_cast<float*>(sm);  // [rank][row of the share][values, maximum, sum]
+    const int share = mt * kRows / plan.ranks;
     if (warp < kSoftWarps && half_w < mt) {
         const int r = row_w;
         const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + half_w * 128 + col_w * (HD / 2);
         row_sum += ms.most[col_w ^ 1][r];
         float f = kScaled ? exp2f(vref) : 1.0f;
         if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
-        float* mine = state + r * L::kJoinPitch;
+        float* mine = (alone ? state : cluster.map_shared_rank(state, r / share)) + (rank * share + r % share) * L::kJoinPitch;
 #pragma unroll
         for (int x = 0; x < HD / 2; x += 32) {
             uint32_t w[32];
@@ -834,7 +837,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         if (!col_w) mine[HD] = row_max, mine[HD + 1] = row_sum;
     }
     tc_fence_before();
-    __syncthreads();
+    if (alone) __syncthreads();
+    else cluster.sync();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     auto put = [&](int r, int d, float4 v) {
         const int pr = r0 + r;
@@ -853,32 +857,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         }
         return;
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int share = (rows * (HD / 4) + plan.ranks - 1) / plan.ranks;
-    for (int x = rank * share + tid; x < min(rows * (HD / 4), (rank + 1) * share); x += kThreads) {
+    const int mine = min(max(rows - rank * share, 0), share);  // rows that this CTA owns
+    for (int x = tid; x < mine * (HD / 4); x += kThreads) {
         const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-        float mw[8], lw[8], top = -INFINITY, sum = 0.0f;
-        float4 o[8];
-#pragma unroll
-        for (int w = 0; w < 8; w++) {  // all ranks' loads in flight
-            const float* st = cluster.map_shared_rank(state, w < plan.ranks ? w : 0) + r * L::kJoinPitch;
-            mw[w] = w < plan.ranks ? st[HD] : -INFINITY, lw[w] = st[HD + 1];
-            o[w] = *reinterpret_cast<const float4*>(st + d);
-        }
-#pragma unroll
-        for (int w = 0; w < 8; w++) top = fmaxf(top, mw[w]);
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < plan.ranks; w++) top = fmaxf(top, state[(w * share + r) * L::kJoinPitch + HD]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            const float f = ex2(mw[w] - ref);
-            if (w < plan.ranks) sum = fmaf(f, lw[w], sum), v.x = fmaf(f, o[w].x, v.x), v.y = fmaf(f, o[w].y, v.y), v.z = fmaf(f, o[w].z, v.z), v.w = fmaf(f, o[w].w, v.w);
+        for (int w = 0; w < plan.ranks; w++) {
+            const float* st = state + (w * share + r) * L::kJoinPitch;
+            const float f = ex2(st[HD] - ref);
+            const float4 o = *reinterpret_cast<const float4*>(st + d);
+            sum = fmaf(f, st[HD + 1], sum), v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
         }
         const float f = 1.0f / sum;
-        put(r, d, sum == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        put(rank * share + r, d, sum == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
     }
-    cluster.sync();  // no CTA leaves while another reads its state
 }
 
 // f16 copies of the 8-bit pages that the sequences hold: block (s, i) of the copies is page table[s][i], codes without

@@ -16,11 +16,15 @@
 // its share item by item, its start-up hidden behind the other warps of its SM: nothing waits for a CTA's other warps
 // until all are done, when the parts of an item meet in shared memory. What several CTAs share is joined from their parts
 // by a second small kernel, in order, so results do not depend on timing.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
 #include "paged.cuh"
 #include "paged_math.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace neko {
 
@@ -83,6 +87,7 @@ struct DecodePlan {
     int page_log;
     float* part;          // [row tile][2 * CTAs][rows][HD + 4]: values, maximum, sum
     int4* desc;           // [row tile][CTAs]: an item that starts in the CTA and ends in a later one
+    int ranks_log;        // of the clusters of the small variant
 };
 
 // Columns of an MMA: 8 rows (16-bit queries) or 4 (f32: hi and lo columns).
@@ -98,6 +103,7 @@ struct Tile {
     static constexpr int kScanOff = kMetaOff + 2 * kWarps * 16;
     static constexpr int kPreOff = kScanOff + 16 * 4;
     static size_t smem(int n_seq) { return kPreOff + size_t(n_seq + 1) * 4; }
+    static size_t smem_small() { return kPreOff + size_t(kState) * 4; }  // the CTA's part in place of the groups
 };
 
 // What a row tile of a sequence sees, the same for all its KV heads.
@@ -145,7 +151,7 @@ __device__ __forceinline__ void put_row(const neko_paged_attention_args& a, cons
     else store(static_cast<__nv_bfloat16*>(a.out) + off);
 }
 
-template <int HD, bool Q8, bool HILO, int NT>
+template <int HD, bool Q8, bool HILO, int NT, bool CL>
 __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kernel(const neko_paged_attention_args a,
                                                                                 const DecodePlan plan) {
     using TL = Tile<HD, HILO, NT>;
@@ -161,53 +167,63 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     int* pre = reinterpret_cast<int*>(smb + TL::kPreOff);
     auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
 
-    // ---- groups of 16 keys before each sequence
-    int carry = 0;
-    for (int base = 0; base < c.n_seq; base += kThreads) {
-        const int s = base + tid;
-        int x = s < c.n_seq ? span_of<TL::kRows>(a, plan, s, tile).ng : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) totals[warp] = x;
-        __syncthreads();
-        int before = carry;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            if (w < warp) before += totals[w];
-            carry += totals[w];
-        }
-        if (s < c.n_seq) pre[s + 1] = before + x;
-        __syncthreads();
-    }
-    if (tid == 0) pre[0] = 0;
-    __syncthreads();
-    // ---- this warp's equal share of all (sequence, KV head) items' groups, in order
-    const int64_t total = int64_t(carry) * n_kv;
-    const int64_t warps = max(min(int64_t(gridDim.x) * kWarps, total), int64_t(1));
-    const int cta = blockIdx.x, gw = cta * kWarps + warp;
-    int64_t x = gw < warps ? total * gw / warps : 0;
-    const int64_t x_end = gw < warps ? total * (gw + 1) / warps : 0;
+    // ---- this warp's equal share of the groups of 16 keys
+    const int cta = blockIdx.x;
+    int s = 0, kvh = 0, cnt = 1;
+    int64_t total, warps, x = 0, x_end = 0;
     if (lane < 2) meta[2 * warp + lane].x = -1;
     __syncwarp();
-    int s = 0, kvh = 0, cnt = 1;
-    if (x < x_end) {
-        int a0 = 0, a1 = c.n_seq;  // pre[a0] * n_kv <= x < pre[a1] * n_kv
-        while (a1 - a0 > 1) {
-            const int mid = (a0 + a1) >> 1;
-            if (int64_t(pre[mid]) * n_kv <= x) a0 = mid;
-            else a1 = mid;
+    if constexpr (CL) {
+        // of one item: the cluster's
+        s = blockIdx.x >> plan.ranks_log, kvh = blockIdx.z;
+        cnt = span_of<TL::kRows>(a, plan, s, tile).ng;
+        total = cnt, warps = min(int64_t(kWarps) << plan.ranks_log, total);
+        const int gw = (blockIdx.x & ((1 << plan.ranks_log) - 1)) * kWarps + warp;
+        if (gw < warps) x = total * gw / warps, x_end = total * (gw + 1) / warps;
+    } else {
+        // of all (sequence, KV head) items', in order: groups before each sequence, added up
+        int carry = 0;
+        for (int base = 0; base < c.n_seq; base += kThreads) {
+            const int sq = base + tid;
+            int y = sq < c.n_seq ? span_of<TL::kRows>(a, plan, sq, tile).ng : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int z = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) y += z;
+            }
+            if (lane == 31) totals[warp] = y;
+            __syncthreads();
+            int before = carry;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                if (w < warp) before += totals[w];
+                carry += totals[w];
+            }
+            if (sq < c.n_seq) pre[sq + 1] = before + y;
+            __syncthreads();
         }
-        s = a0;
-        cnt = pre[s + 1] - pre[s];
-        kvh = int(uint32_t(x - int64_t(pre[s]) * n_kv) / uint32_t(cnt));
+        if (tid == 0) pre[0] = 0;
+        __syncthreads();
+        total = int64_t(carry) * n_kv;
+        warps = max(min(int64_t(gridDim.x) * kWarps, total), int64_t(1));
+        const int gw = cta * kWarps + warp;
+        if (gw < warps) x = total * gw / warps, x_end = total * (gw + 1) / warps;
+        if (x < x_end) {
+            int a0 = 0, a1 = c.n_seq;  // pre[a0] * n_kv <= x < pre[a1] * n_kv
+            while (a1 - a0 > 1) {
+                const int mid = (a0 + a1) >> 1;
+                if (int64_t(pre[mid]) * n_kv <= x) a0 = mid;
+                else a1 = mid;
+            }
+            s = a0;
+            cnt = pre[s + 1] - pre[s];
+            kvh = int(uint32_t(x - int64_t(pre[s]) * n_kv) / uint32_t(cnt));
+        }
     }
     int starts_last = -1;  // the CTA where the item that starts in this warp and does not end in it does
 #pragma unroll 1
     while (x < x_end) {
-    const int64_t item = int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
+    const int64_t item = CL ? 0 : int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
     const int k_begin = int(x - item), k_end = int(min(int64_t(cnt), x_end - item));
     const Span sp = span_of<TL::kRows>(a, plan, s, tile);
     const int row0 = sp.row0, n = sp.n, held = sp.held, len = sp.len, prefix = sp.prefix, rows = sp.rows;
@@ -569,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         }
     }
     __syncwarp();
-    if (first && ends) {
+    if (!CL && first && ends) {
         for (int y = lane; y < rows * (HD / 4); y += 32) {
             const int row = y / (HD / 4), d = y % (HD / 4) * 4;
             const float* st = st0 + row * TL::kPitch;
@@ -581,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     }
     if (first && !ends) starts_last = int((((item + cnt) * warps - 1) / total) / kWarps);
     x = item + k_end;
-    if (x < x_end && ++kvh == n_kv) {
+    if (!CL && x < x_end && ++kvh == n_kv) {
         kvh = 0;
         do s++;
         while (pre[s + 1] == pre[s]);
@@ -589,6 +605,51 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     }
     }
     __syncthreads();
+    if constexpr (CL) {
+        // ---- the warps' parts joined in each CTA, the CTAs' over distributed shared memory, in order
+        cg::cluster_group cluster = cg::this_cluster();
+        const Span sp = span_of<TL::kRows>(a, plan, s, tile);
+        const int ranks = 1 << plan.ranks_log, rank = blockIdx.x & (ranks - 1);
+        float* mine = reinterpret_cast<float*>(smb + TL::kPreOff);
+        auto join = [&](int row, int d, int parts, auto part, float& top, float& sum) {
+            top = -INFINITY, sum = 0.0f;
+            for (int i = 0; i < parts; i++)
+                if (const float* st = part(i)) top = fmaxf(top, st[row * TL::kPitch + HD]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float4 v = make_float4(0, 0, 0, 0);
+            for (int i = 0; i < parts; i++) {
+                const float* st = part(i);
+                if (!st) continue;
+                st += row * TL::kPitch;
+                const float f = ex2(st[HD] - ref);
+                const float4 o = *reinterpret_cast<const float4*>(st + d);
+                sum = fmaf(f, st[HD + 1], sum);
+                v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
+            }
+            return v;
+        };
+        for (int y = tid; y < sp.rows * (HD / 4); y += kThreads) {
+            const int row = y / (HD / 4), d = y % (HD / 4) * 4;
+            float top, sum;
+            const float4 v = join(row, d, 2 * kWarps, [&](int i) { return meta[i].x >= 0 ? sm + i * TL::kState : nullptr; }, top, sum);
+            if (ranks == 1) {
+                put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, sum);
+            } else {
+                *reinterpret_cast<float4*>(mine + row * TL::kPitch + d) = v;
+                if (d == 0) mine[row * TL::kPitch + HD] = top, mine[row * TL::kPitch + HD + 1] = sum;
+            }
+        }
+        if (ranks == 1) return;
+        cluster.sync();
+        for (int y = rank * kThreads + tid; y < sp.rows * (HD / 4); y += kThreads * ranks) {
+            const int row = y / (HD / 4), d = y % (HD / 4) * 4;
+            float top, sum;
+            const float4 v = join(row, d, ranks, [&](int i) -> const float* { return cluster.map_shared_rank(mine, i); }, top, sum);
+            put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, sum);
+        }
+        cluster.sync();  // no CTA leaves while another reads its part
+        return;
+    }
     // ---- parts of the same item joined over the warps: to the output, or as one of this CTA's (at most two) parts
     if (starts_last > cta && lane == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(s, kvh, starts_last, meta[2 * warp + 1].z);
     bool open_item = false;
@@ -691,6 +752,7 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
     p.page_16 = uint32_t(c.page_stride * (Q8 ? 1 : 2) / 16);
     p.page_log = 31 - __builtin_clz(c.page_size);
+    p.ranks_log = 0;
     const int64_t row_tiles = (int64_t(a.max_new) * p.group + TL::kRows - 1) / TL::kRows;
     if (row_tiles > 65535) return cudaErrorInvalidConfiguration;
     // as many CTAs as the GPU holds at a time, or a group of 16 keys for each warp where the cache has room for fewer
@@ -698,7 +760,31 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t items = int64_t(c.n_kv) * c.n_seq;
     const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(num_sms()) * kCtas<HD, Q8, NT>, std::max(groups, items) / kWarps)));
     const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
-    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT>;
+    // Few items of few keys: a cluster of CTAs each, two groups for every warp, which need neither scratch memory nor the
+    // second kernel (one chat, 777 keys: 12 us a call, 8.4 on
+    // the GPU, against 16 and 10.4 of the variant below)
+    const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, room = int64_t(num_sms()) * kCtas<HD, Q8, NT>;
+    int ranks = 1;
+    while (ranks < 8 && per_item > 16 * ranks && items * row_tiles * ranks * 2 <= room) ranks *= 2;
+    if (items * row_tiles * ranks <= room && per_item <= 64 * ranks && c.n_kv <= 65535) {
+        auto* small = paged_decode_kernel<HD, Q8, HILO, NT, true>;
+        if (cudaError_t e = ensure_dyn_smem(small, TL::smem_small()); e != cudaSuccess) return e;
+        p.ranks_log = 31 - __builtin_clz(ranks);
+        p.part = nullptr, p.desc = nullptr;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(c.n_seq * ranks), unsigned(row_tiles), unsigned(c.n_kv));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = TL::smem_small();
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(ranks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = ranks > 1 ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, small, a, p);
+    }
+    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, false>;
     const size_t smem = TL::smem(c.n_seq);
     cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;

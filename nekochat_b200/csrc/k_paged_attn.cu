@@ -650,47 +650,59 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         cluster.sync();  // no CTA leaves while another reads its part
         return;
     }
-    // ---- parts of the same item joined over the warps: to the output, or as one of this CTA's (at most two) parts
+    // ---- parts of the same item joined over the warps, a warp per item: to the output, or as one of this CTA's (at most
+    // two) parts
     if (starts_last > cta && lane == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(s, kvh, starts_last, meta[2 * warp + 1].z);
+    const int4 mine = lane < 2 * kWarps ? meta[lane] : make_int4(-1, 0, 0, 0);
+    const uint32_t valid = __ballot_sync(0xffffffffu, mine.x >= 0);
+    // lanes that hold the first part of an item here: the part before theirs belongs to another
+    const uint32_t below = valid & ((1u << lane) - 1u);
+    const int item_before = __shfl_sync(0xffffffffu, mine.x, below ? 31 - __clz(below) : lane);
+    const uint32_t heads = __ballot_sync(0xffffffffu, mine.x >= 0 && (!below || item_before != mine.x));
     bool open_item = false;
-    for (int b = 0; b < 2 * kWarps;) {
-        const int4 mb = meta[b];
-        int e = b + 1;
-        if (mb.x < 0) {
-            b = e;
-            continue;
-        }
-        int flags = mb.y;
-        while (e < 2 * kWarps && (meta[e].x == mb.x || meta[e].x < 0)) {
-            if (meta[e].x >= 0) flags |= meta[e].y;
-            e++;
-        }
-        const int row0 = mb.z, rows = mb.w, kvh2 = mb.x % n_kv;
+    int run = 0;
+    for (uint32_t left = heads; left; left &= left - 1, run++) {  // the same in every warp
+        const int b = __ffs(left) - 1;
+        const uint32_t rest = left & (left - 1);
+        const uint32_t in = valid & ~((1u << b) - 1u) & (rest ? (rest & (0u - rest)) - 1u : 0xffffffffu);
+        const int last_part = 31 - __clz(in);
+        const int flags = (__shfl_sync(0xffffffffu, mine.y, b) & 1) | (__shfl_sync(0xffffffffu, mine.y, last_part) & 2);
+        open_item |= flags == 1;
+        const int item_id = __shfl_sync(0xffffffffu, mine.x, b), row0 = __shfl_sync(0xffffffffu, mine.z, b), rows = __shfl_sync(0xffffffffu, mine.w, b);
+        if (run % kWarps != warp) continue;
         float* part = plan.part + ((int64_t(tile) * gridDim.x + cta) * 2 + (flags & 1)) * TL::kState;
-        open_item |= (flags & 3) == 1;
-        for (int y = tid; y < rows * (HD / 4); y += kThreads) {
+        for (int y = lane; y < rows * (HD / 4); y += 32) {
             const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
             float top = -INFINITY, sum = 0.0f;
-            for (int i = b; i < e; i++)
-                if (meta[i].x >= 0) top = fmaxf(top, sm[i * TL::kState + at + HD]);
-            const float ref = top == -INFINITY ? 0.0f : top;
             float4 v = make_float4(0, 0, 0, 0);
-            for (int i = b; i < e; i++) {
-                if (meta[i].x < 0) continue;
-                const float* st = sm + i * TL::kState + at;
-                const float f = ex2(st[HD] - ref);
-                const float4 o = *reinterpret_cast<const float4*>(st + d);
-                sum = fmaf(f, st[HD + 1], sum);
-                v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
+            for (uint32_t w = in; w;) {  // four parts at a time
+                float mw[4], lw[4];
+                float4 o[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float* st = sm + (w ? __ffs(w) - 1 : b) * TL::kState + at;
+                    mw[i] = w ? st[HD] : -INFINITY, lw[i] = st[HD + 1];
+                    o[i] = *reinterpret_cast<const float4*>(st + d);
+                    w &= w - 1;
+                }
+                const float now = fmaxf(top, fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3])));
+                const float ref = now == -INFINITY ? 0.0f : now, was = ex2(top - ref);
+                top = now;
+                sum *= was, v.x *= was, v.y *= was, v.z *= was, v.w *= was;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float f = ex2(mw[i] - ref);
+                    sum = fmaf(f, lw[i], sum);
+                    v.x = fmaf(f, o[i].x, v.x), v.y = fmaf(f, o[i].y, v.y), v.z = fmaf(f, o[i].z, v.z), v.w = fmaf(f, o[i].w, v.w);
+                }
             }
             if (flags == 3) {
-                put_row<HILO>(a, plan, row0, kvh2, tile * TL::kRows + row, d, v, sum);
+                put_row<HILO>(a, plan, row0, item_id % n_kv, tile * TL::kRows + row, d, v, sum);
             } else {
                 *reinterpret_cast<float4*>(part + at + d) = v;
                 if (d == 0) part[at + HD] = top, part[at + HD + 1] = sum;
             }
         }
-        b = e;
     }
     if (!open_item && tid == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(-1, 0, 0, 0);
     pdl_trigger();

@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         cluster.sync();  // no CTA leaves while another reads its part
         return;
     }
-    // ---- parts of the same item joined over the warps, a warp per item: to the output, or as one of this CTA's (at most
+    // ---- parts of the same item joined over the warps, 32 pieces of four values a warp: to the output, or as one of this CTA's (at most
     // two) parts
     if (starts_last > cta && lane == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(s, kvh, starts_last, meta[2 * warp + 1].z);
     const int4 mine = lane < 2 * kWarps ? meta[lane] : make_int4(-1, 0, 0, 0);
@@ -660,8 +660,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     const int item_before = __shfl_sync(0xffffffffu, mine.x, below ? 31 - __clz(below) : lane);
     const uint32_t heads = __ballot_sync(0xffffffffu, mine.x >= 0 && (!below || item_before != mine.x));
     bool open_item = false;
-    int run = 0;
-    for (uint32_t left = heads; left; left &= left - 1, run++) {  // the same in every warp
+    int turn = 0;  // 32 output pieces at a time go round the warps
+    for (uint32_t left = heads; left; left &= left - 1) {  // the same in every warp
         const int b = __ffs(left) - 1;
         const uint32_t rest = left & (left - 1);
         const uint32_t in = valid & ~((1u << b) - 1u) & (rest ? (rest & (0u - rest)) - 1u : 0xffffffffu);
@@ -669,9 +669,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         const int flags = (__shfl_sync(0xffffffffu, mine.y, b) & 1) | (__shfl_sync(0xffffffffu, mine.y, last_part) & 2);
         open_item |= flags == 1;
         const int item_id = __shfl_sync(0xffffffffu, mine.x, b), row0 = __shfl_sync(0xffffffffu, mine.z, b), rows = __shfl_sync(0xffffffffu, mine.w, b);
-        if (run % kWarps != warp) continue;
         float* part = plan.part + ((int64_t(tile) * gridDim.x + cta) * 2 + (flags & 1)) * TL::kState;
-        for (int y = lane; y < rows * (HD / 4); y += 32) {
+        for (int y0 = 0; y0 < rows * (HD / 4); y0 += 32) {
+            const int y = y0 + lane;
+            if (turn++ % kWarps != warp || y >= rows * (HD / 4)) continue;
             const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
             float top = -INFINITY, sum = 0.0f;
             float4 v = make_float4(0, 0, 0, 0);

@@ -157,6 +157,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
+    // Weights are 2^(score - maximum + kLift) times a ratio of value scales up to kVLazy: at most 2^15, clear of f16's subnormals.
+    constexpr float kLazy = 8.0f, kVLazy = 16.0f, kLift = 3.0f;
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                         else z[nt][r][h] = -INFINITY;
                     }
         }
-        // ---- running maximum (moved only by more than 2^8: weights up to that are as exact) and value scale
+        // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact) and value scale
         const float vs_now = vs;
         bool up = false;
         float top[NT][TL::kLaneRows];
@@ -442,9 +444,9 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 top[nt][r] = x;
-                up |= x > m[nt][r] + 8.0f;
+                up |= x > m[nt][r] + kLazy;
             }
-        const bool v_up = Q8 && vs_now > 16.0f * vref;
+        const bool v_up = Q8 && vs_now > kVLazy * vref;
         if (__any_sync(0xffffffffu, up) || v_up) {
             float fv = 1.0f;
             if (v_up) {
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                 for (int r = 0; r < TL::kLaneRows; r++) {
                     f[r] = 1.0f;
-                    if (top[nt][r] > m[nt][r] + 8.0f) {
+                    if (top[nt][r] > m[nt][r] + kLazy) {
                         f[r] = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
                         m[nt][r] = top[nt][r];
                         l[nt][r] *= f[r];
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             float p[2][TL::kLaneRows];
 #pragma unroll
             for (int r = 0; r < TL::kLaneRows; r++) {
-                const float ref = m[nt][r] == -INFINITY ? 0.0f : m[nt][r];
+                const float ref = (m[nt][r] == -INFINITY ? 0.0f : m[nt][r]) - kLift;
                 p[0][r] = ex2(z[nt][r][0] - ref), p[1][r] = ex2(z[nt][r][1] - ref);
                 l[nt][r] += p[0][r] + p[1][r];
             }

@@ -9,7 +9,7 @@
 // power of two into f16's range first. Roles:
 //  * warps 0..7 and 8..15: softmax of one row tile each, two threads per row (64 keys each; two warps more per scheduler
 //    hide each other's latencies), which tell each other their largest scores. The reference maximum moves only
-//    when a score exceeds it by 2^8 (weights up to 2^8 are as exact as any in f16), so O is hardly ever rescaled, and
+//    when a score exceeds it by a factor of 2^8 (weights above 1 are as exact as any in f16), so O is hardly ever rescaled, and
 //    the row's own threads do that; the tensor core works on the other row tile meanwhile. A quarter of 16-bit queries'
 //    exponentials is computed on the FMA pipe: the special-function unit is what bounds this step.
 //  * warps 16..18: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
@@ -41,8 +41,18 @@ constexpr int kCopyTiles = 3;
 constexpr int64_t kCopyBytes = int64_t(1) << 31;
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
+// Weights are 2^(score - reference + kLift), in units of the reference value scale: at most 2^15, clear of f16's subnormals.
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
 constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
+constexpr float kLift = 15.0f - kLazy - kVLazy;
+// An UMMA's f32 accumulation truncates: each step takes a share off the sum, 3.2e-8 on average (measured on sums of 2,500
+// steps, whose common factor was 1 - 2.1e-5; half a unit in the last of 24 places is 4.3e-8 of a mantissa spread evenly over
+// the logarithm). What O held before a step loses as a whole, so the sum of the weights, which is rounded to nearest, is made
+// to lose as much and the quotient does not keep it. What is left differs from value to value, about 6e-9 a step: for f32
+// queries O leaves TMEM every kFlush key tiles for sums that are rounded to nearest.
+constexpr float kDrop = 3.2e-8f;
+constexpr int kFlush = 16;
+constexpr int64_t kFlushBytes = int64_t(1) << 30;
 constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
 constexpr float kVNone = -126.0f;
 constexpr float kGone = -1.0f;
@@ -56,6 +66,7 @@ struct PromptPlan {
     int tiles_per;  // row tiles of a CTA: 1 or 2
     int group;      // query heads per KV head
     uint64_t group_inv;  // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
+    float* flush;        // [CTA][HD][256 rows]: sums that have left TMEM (f32 queries; NULL: none do)
 };
 
 template <int HD, bool HILO>
@@ -275,6 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     volatile uint32_t* fail = &ms.fail;
 
     float row_max = -INFINITY, row_sum = 0.0f, vref = 0.0f;  // of a softmax thread's row; vref: log2 of O's unit
+    // f32 queries: this thread's first kept sum (256 floats between columns), and log2 of their unit, the reference maximum and
+    // value scale, which only grow
+    float* kept = nullptr;
+    float kept_ref = 0.0f, sum_kept = 0.0f;  // and the weights' sum that goes with them
     if (warp >= kLoadWarp && warp < kMmaWarp) {
         // ------------------------------------------------------------------ loader
         const int lt = tid - 32 * kLoadWarp;
@@ -476,11 +491,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const uint64_t kd = k_desc + uint64_t(st * (L::kStage >> 4));
                 if (elect_one()) {
 #pragma unroll
-                    for (int part = 0; part < L::kParts; part++)
+                    for (int part = L::kParts - 1; part >= 0; part--)  // the small products first: fewer steps truncate large sums
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++) {
                             const uint32_t off = ((k / 4) * L::kHalf + (k % 4) * 32) >> 4;
-                            umma_f16(tmem + h * 128, qd + part * (L::kQTile >> 4) + off, kd + off, idesc_s, part + k > 0);
+                            umma_f16(tmem + h * 128, qd + part * (L::kQTile >> 4) + off, kd + off, idesc_s, part < L::kParts - 1 || k > 0);
                         }
                     umma_commit(&ms.s_full[h]);
                 }
@@ -601,7 +616,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         wait_on(&ms.q_full, 0, fail);
         __syncwarp();
         // from the accumulator to log2 units, or with a cap to the tanh's argument
-        const float factor = a.softcap > 0.0f ? ms.most[0][r] / a.softcap : ms.most[0][r] * kLog2e;
+        // (and what the scores' own HD / 16 steps truncate)
+        const float whole_score = ms.most[0][r] * (1.0f + (HD / 16 + 1) / 2.0f * kDrop);
+        const float factor = a.softcap > 0.0f ? whole_score / a.softcap : whole_score * kLog2e;
         // The two warps of 32 rows meet at a named barrier of theirs: no wait of this role ends it early (a wait that gives up
         // has set the fail flag, and every later one returns at once), so both always come to every meeting.
         auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * h + (warp & 3)) : "memory"); };
@@ -614,6 +631,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             wait_on(&ms.s_full[h], i & 1, fail);
             __syncwarp();
             tc_fence_after();
+            if constexpr (HILO) {
+                if (i > 0 && i % kFlush == 0 && plan.flush) {
+                    wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
+                    __syncwarp();
+                    tc_fence_after();
+                    const bool again = kept != nullptr;
+                    kept = plan.flush + (int64_t(blockIdx.x) * HD + col_w * (HD / 2)) * (2 * kRows) + r;
+                    const float now = (row_max == -INFINITY ? 0.0f : row_max) + vref, f = ex2(fminf(kept_ref - now, 0.0f));
+                    kept_ref = now;
+                    sum_kept += row_sum;
+                    row_sum = 0.0f;
+#pragma unroll 1
+                    for (int x = 0; x < HD / 2; x += 16) {
+                        uint32_t o[16];
+                        ld16(to + x, o);
+                        float was[16];
+#pragma unroll
+                        for (int y = 0; y < 16; y++) was[y] = again ? kept[(x + y) * (2 * kRows)] : 0.0f;
+                        ld_wait16(o);
+#pragma unroll
+                        for (int y = 0; y < 16; y++) {
+                            kept[(x + y) * (2 * kRows)] = fmaf(was[y], f, __uint_as_float(o[y]));
+                            o[y] = 0;
+                        }
+                        st16(to + x, o);
+                    }
+                    st_wait();
+                }
+            }
             const bool plain_mask = open_rows && ms.whole[i % kRing];
             const int xv = 2 * i + 1, stv = xv % L::kStages;
             bool odd_tile = false;
@@ -750,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             meet();
             top = max_nan(top, ms.most[col_w ^ 1][r]);
             if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
-            // the reference moves only when a score exceeds it by more than 2^8 (the same decision in both warps of a row)
+            // the reference moves only when a score exceeds it by more than 2^kLazy (the same decision in both warps of a row)
             const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
             if (__any_sync(0xffffffffu, up)) {
                 float f = 1.0f;
@@ -758,11 +804,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
                     row_max = top;
                     row_sum *= f;
+                    if (HILO) sum_kept *= f;
                 }
                 if (i > 0) fix_o(f, false);
             }
             // ---- weights, their sum; P over this thread's scores
-            const float ref = row_max == -INFINITY ? 0.0f : row_max;
+            const float ref = (row_max == -INFINITY ? 0.0f : row_max) - kLift;
+            float sum = 0.0f;
             uint64_t sums[2] = {0, 0};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
@@ -791,9 +839,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 if (kScaled || b == 3) {  // the sum without the value scale
                     float z0, z1;
                     unpack2(add2(sums[0], sums[1]), z0, z1);
-                    row_sum = kScaled ? fmaf(z0 + z1, ex2(-vr), row_sum) : row_sum + (z0 + z1);
+                    sum = kScaled ? fmaf(z0 + z1, ex2(-vr), sum) : z0 + z1;
                 }
             }
+            constexpr float kSteps = kKeys / 16 * L::kParts;
+            row_sum = fmaf(row_sum, -kSteps * kDrop, row_sum) + fmaf(sum, -(kSteps + 1) / 2 * kDrop, sum);
             st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);
@@ -807,6 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     // ---- the outputs. Alone: through shared memory, once the operands are used up. In a cluster each CTA owns a share of
     // the rows: every CTA pushes its states of them into the owner's shared memory.
     __syncwarp();
+    if (HILO) row_sum += sum_kept;
     if (warp < kSoftWarps && half_w < mt) ms.most[col_w][row_w] = row_sum;
     const bool alone = plan.ranks == 1;
     cg::cluster_group cluster = cg::this_cluster();
@@ -820,12 +871,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         row_sum += ms.most[col_w ^ 1][r];
         float f = kScaled ? exp2f(vref) : 1.0f;
         if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
+        const float f_kept = ex2(fminf(kept_ref - (row_max == -INFINITY ? 0.0f : row_max) - vref, 0.0f));
         float* mine = (alone ? state : cluster.map_shared_rank(state, r / share)) + (rank * share + r % share) * L::kJoinPitch;
 #pragma unroll
         for (int x = 0; x < HD / 2; x += 32) {
             uint32_t w[32];
             ld32(to + x, w);
             ld_wait(w);
+            if (HILO && kept) {
+#pragma unroll
+                for (int y = 0; y < 32; y++) w[y] = __float_as_uint(fmaf(kept[(x + y) * (2 * kRows)], f_kept, __uint_as_float(w[y])));
+            }
 #pragma unroll
             for (int y = 0; y < 32; y += 4) {
                 float4 v = make_float4(__uint_as_float(w[y]) * f, __uint_as_float(w[y + 1]) * f, __uint_as_float(w[y + 2]) * f,
@@ -937,6 +993,23 @@ cudaError_t by_type(const neko_paged_attention_args& a, const PromptPlan& p, int
 }
 
 template <int HD>
+cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, cudaStream_t st) {
+    const neko_paged_cache& c = a.cache;
+    if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, p, items, nullptr, st);
+    // Each CTA would convert its keys again: from kCopyTiles CTAs per (sequence, KV head) on, they are converted once,
+    // if the copies stay below kCopyBytes.
+    const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
+    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes || c.n_seq > 65535) return by_type<HD, kCodes>(a, p, items, nullptr, st);
+    void* mem = nullptr;
+    if (cudaError_t e = scratch_alloc(&mem, size_t(bytes), st); e != cudaSuccess) return e;
+    cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
+                              static_cast<uint4*>(mem));
+    if (e == cudaSuccess) e = by_type<HD, kCopies>(a, p, items, static_cast<const __half*>(mem), st);
+    cudaFreeAsync(mem, st);
+    return e;
+}
+
+template <int HD>
 cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
     const neko_paged_cache& c = a.cache;
     const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
@@ -951,17 +1024,15 @@ cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
     p.ranks = 1;
     while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, p, items, nullptr, st);
-    // Each CTA would convert its keys again: from kCopyTiles CTAs per (sequence, KV head) on, they are converted once,
-    // if the copies stay below kCopyBytes.
-    const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
-    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes || c.n_seq > 65535) return by_type<HD, kCodes>(a, p, items, nullptr, st);
-    void* mem = nullptr;
-    if (cudaError_t e = scratch_alloc(&mem, size_t(bytes), st); e != cudaSuccess) return e;
-    cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
-                              static_cast<uint4*>(mem));
-    if (e == cudaSuccess) e = by_type<HD, kCopies>(a, p, items, static_cast<const __half*>(mem), st);
-    cudaFreeAsync(mem, st);
+    p.flush = nullptr;
+    void* flush = nullptr;
+    const int64_t flush_bytes = items * p.ranks * 2 * kRows * HD * 4;
+    if (a.type == NEKO_T_F32 && key_tiles > int64_t(p.ranks) * kFlush && flush_bytes <= kFlushBytes) {
+        if (cudaError_t e = scratch_alloc(&flush, size_t(flush_bytes), st); e != cudaSuccess) return e;
+        p.flush = static_cast<float*>(flush);
+    }
+    const cudaError_t e = by_pages<HD>(a, p, items, st);
+    if (flush) cudaFreeAsync(flush, st);
     return e;
 }
 

@@ -461,3 +461,25 @@ def test_prompt_of_blocks_of_very_different_scales(torch, dtype):
     cache.vs.copy_(torch.from_numpy(rng.uniform(0.01, 0.3, tuple(cache.vs.shape)).astype(np.float32)).cuda())
     cache.ks.copy_(torch.from_numpy((rng.integers(0, 5, tuple(cache.ks.shape)) * 0.03).astype(np.float32)).cuda())
     attend(torch, cache, lens, [60, 200], 4, dtype, 55)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new,ctx,heads,n_kv", [(300, 2900, 4, 2), (40, 5000, 8, 2), (1024, 1024, 16, 8)])
+def test_long_prompts_keep_f32_precision(torch, new, ctx, heads, n_kv, e4m3):
+    """Thousands of keys a row: the relative error (2-norm) of f32 results stays that of f32 sums. Half a unit of 2^-24 at
+    each of the 64 steps between two sums of the tensor core's accumulator and 22 bits of queries and weights: 3e-6."""
+    rng = np.random.default_rng(ctx)
+    cache = Cache(torch, rng, [new + ctx], n_kv, 64, 128, e4m3)
+    from nekochat_b200 import ops
+    cache.fill(rng, [new + ctx])
+    q = torch.randn((new, heads, 128), device="cuda", generator=torch.Generator("cuda").manual_seed(7))
+    i = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), i(new + ctx), k_scale=cache.ks,
+                              v_scale=cache.vs, q_start=i(0, new), max_new=new).double()
+    kv, vv = (torch.from_numpy(x).cuda()[torch.from_numpy(cache.table[0]).long().cuda()].transpose(0, 1).reshape(n_kv, -1, 128)[:, :new + ctx]
+              for x in cache.values())
+    see = torch.arange(new + ctx, device="cuda")[None] <= ctx + torch.arange(new, device="cuda")[:, None]
+    for h in range(heads):
+        z = torch.where(see, q[:, h].double() @ kv[h * n_kv // heads].T * 128 ** -0.5, -torch.inf)
+        want = torch.softmax(z, -1) @ vv[h * n_kv // heads]
+        assert (got[:, h] - want).norm() <= 3e-6 * want.norm()

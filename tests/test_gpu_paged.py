@@ -483,3 +483,20 @@ def test_long_prompts_keep_f32_precision(torch, new, ctx, heads, n_kv, e4m3):
         z = torch.where(see, q[:, h].double() @ kv[h * n_kv // heads].T * 128 ** -0.5, -torch.inf)
         want = torch.softmax(z, -1) @ vv[h * n_kv // heads]
         assert (got[:, h] - want).norm() <= 3e-6 * want.norm()
+
+
+@pytest.mark.parametrize("n,L,heads,n_kv,hd", [(48, 9000, 16, 8, 128), (1, 30000, 8, 2, 128), (60, 5000, 12, 12, 64)])
+def test_long_steps_keep_f32_precision(torch, n, L, heads, n_kv, hd):
+    """Single tokens over long contexts: 22-bit products and sums rounded to nearest, an error of 1.5e-6 (2-norm) at most."""
+    from nekochat_b200 import ops
+    g = torch.Generator("cuda").manual_seed(9)
+    P = -(-L // 64)
+    k, v = (torch.randn((n * P, n_kv, 64, hd), device="cuda", generator=g, dtype=torch.float16) for _ in range(2))
+    q = torch.randn((n, heads, hd), device="cuda", generator=g)
+    table = torch.randperm(n * P, device="cuda", generator=g).int().view(n, P)
+    got = ops.paged_attention(q, k, v, table, torch.full((n,), L, dtype=torch.int32, device="cuda")).double()
+    for s in (0, n // 2, n - 1):
+        kk, vv = (x[table[s].long()].double().transpose(0, 1).reshape(n_kv, -1, hd)[:, :L] for x in (k, v))
+        for h in range(heads):
+            want = torch.softmax(kk[h * n_kv // heads] @ q[s, h].double() * hd ** -0.5, -1) @ vv[h * n_kv // heads]
+            assert (got[s, h] - want).norm() <= 1.5e-6 * want.norm()

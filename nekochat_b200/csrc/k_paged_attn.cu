@@ -225,397 +225,408 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     int starts_last = -1;  // the CTA where the item that starts in this warp and does not end in it does
 #pragma unroll 1
     while (x < x_end) {
-    const int64_t item = CL ? 0 : int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
-    const int k_begin = int(x - item), k_end = int(min(int64_t(cnt), x_end - item));
-    const Span sp = span_of<TL::kRows>(a, plan, s, tile);
-    const int row0 = sp.row0, n = sp.n, held = sp.held, len = sp.len, prefix = sp.prefix, rows = sp.rows;
-    const int pos_lo = sp.pos_lo, pos_hi = sp.pos_hi, hi = sp.hi, lo = sp.lo, g_lo = sp.g_lo, g_pre = sp.g_pre;
-    const int r0 = tile * TL::kRows;
+        const int64_t item = CL ? 0 : int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
+        const int k_begin = int(x - item), k_end = int(min(int64_t(cnt), x_end - item));
+        const Span sp = span_of<TL::kRows>(a, plan, s, tile);
+        const int row0 = sp.row0, n = sp.n, held = sp.held, len = sp.len, prefix = sp.prefix, rows = sp.rows;
+        const int pos_lo = sp.pos_lo, pos_hi = sp.pos_hi, hi = sp.hi, lo = sp.lo, g_lo = sp.g_lo, g_pre = sp.g_pre;
+        const int r0 = tile * TL::kRows;
 
-    // ---- keys and values: fragments straight from the pages
-    const int32_t* table = c.table + int64_t(s) * c.table_stride;
-    constexpr int kB = Q8 ? 1 : 2;
-    const int in_page = (1 << plan.page_log) - 1;
-    const int64_t head_off = (int64_t(kvh) << plan.page_log) * HD * kB;
-    const uint8_t* kp = static_cast<const uint8_t*>(c.k_pages) + head_off + g * W::kRow + t * (W::kK >= 4 ? 16 : W::kK * 4);
-    const uint8_t* vp = static_cast<const uint8_t*>(c.v_pages) + head_off + 2 * t * W::kRow + g * (W::kV >= 4 ? 16 : W::kV * 4);
-    const float *ksp = c.k_scale + kvh, *vsp = c.v_scale + kvh;
-    auto key_of = [&](int k) { return 16 * (k < g_pre ? k : k - g_pre + g_lo); };  // first key of a group
-    auto page_of = [&](int k) {
-        const int slot = key_of(k) >> plan.page_log;
-        const int p = k < k_end && slot < c.max_pages ? table[slot] : -1;
-        return p < c.num_pages ? p : -1;
-    };
-    uint32_t kw[2][W::kK], vw[4][W::kV];
-    float ks = 1.0f, vs = 1.0f;
-    auto place = [&](int page, int j0) {
-        return (uint64_t(uint32_t(page)) * plan.page_16 << 4) + uint32_t((j0 & in_page) * W::kRow);
-    };
-    auto load_k = [&](int page, int j0) {
-        const uint8_t* p = kp + place(page, j0);
-        load_words(p, 64, kw[0]);
-        load_words(p + 8 * W::kRow, 64, kw[1]);
-        if constexpr (Q8) ks = ksp[int64_t(page) * c.scale_stride];
-    };
-    auto load_v = [&](int page, int j0) {
-        const uint8_t* p = vp + place(page, j0);
-        load_words(p, 128, vw[0]);
-        load_words(p + W::kRow, 128, vw[1]);
-        load_words(p + 8 * W::kRow, 128, vw[2]);
-        load_words(p + 9 * W::kRow, 128, vw[3]);
-        if constexpr (Q8) vs = vsp[int64_t(page) * c.scale_stride];
-    };
-    // the V^T fragments of dims' tiles: word w gives one (f16) or two (8-bit) tiles of 16 dims
-    auto v_frag = [&](int tile_i, uint32_t (&f)[4]) {
-        if constexpr (Q8) {
-            const int w = tile_i >> 1;
-            const uint32_t sel = tile_i & 1 ? 0x7362u : 0x5140u;
-            const uint32_t x = prmt(vw[0][w], vw[1][w], sel), y = prmt(vw[2][w], vw[3][w], sel);
-            f[0] = e4m3x2_to_f16x2(uint16_t(x)), f[1] = e4m3x2_to_f16x2(uint16_t(x >> 16));
-            f[2] = e4m3x2_to_f16x2(uint16_t(y)), f[3] = e4m3x2_to_f16x2(uint16_t(y >> 16));
-        } else {
-            f[0] = prmt(vw[0][tile_i], vw[1][tile_i], 0x5410u), f[1] = prmt(vw[0][tile_i], vw[1][tile_i], 0x7632u);
-            f[2] = prmt(vw[2][tile_i], vw[3][tile_i], 0x5410u), f[3] = prmt(vw[2][tile_i], vw[3][tile_i], 0x7632u);
+        // ---- keys and values: fragments straight from the pages
+        const int32_t* table = c.table + int64_t(s) * c.table_stride;
+        constexpr int kB = Q8 ? 1 : 2;
+        const int in_page = (1 << plan.page_log) - 1;
+        const int64_t head_off = (int64_t(kvh) << plan.page_log) * HD * kB;
+        const uint8_t* kp = static_cast<const uint8_t*>(c.k_pages) + head_off + g * W::kRow + t * (W::kK >= 4 ? 16 : W::kK * 4);
+        const uint8_t* vp = static_cast<const uint8_t*>(c.v_pages) + head_off + 2 * t * W::kRow + g * (W::kV >= 4 ? 16 : W::kV * 4);
+        const float *ksp = c.k_scale + kvh, *vsp = c.v_scale + kvh;
+        auto key_of = [&](int k) { return 16 * (k < g_pre ? k : k - g_pre + g_lo); };  // first key of a group
+        auto page_of = [&](int k) {
+            const int slot = key_of(k) >> plan.page_log;
+            const int p = k < k_end && slot < c.max_pages ? table[slot] : -1;
+            return p < c.num_pages ? p : -1;
+        };
+        uint32_t kw[2][W::kK], vw[4][W::kV];
+        float ks = 1.0f, vs = 1.0f;
+        auto place = [&](int page, int j0) {
+            return (uint64_t(uint32_t(page)) * plan.page_16 << 4) + uint32_t((j0 & in_page) * W::kRow);
+        };
+        auto load_k = [&](int page, int j0) {
+            const uint8_t* p = kp + place(page, j0);
+            load_words(p, 64, kw[0]);
+            load_words(p + 8 * W::kRow, 64, kw[1]);
+            if constexpr (Q8) ks = ksp[int64_t(page) * c.scale_stride];
+        };
+        auto load_v = [&](int page, int j0) {
+            const uint8_t* p = vp + place(page, j0);
+            load_words(p, 128, vw[0]);
+            load_words(p + W::kRow, 128, vw[1]);
+            load_words(p + 8 * W::kRow, 128, vw[2]);
+            load_words(p + 9 * W::kRow, 128, vw[3]);
+            if constexpr (Q8) vs = vsp[int64_t(page) * c.scale_stride];
+        };
+        // the V^T fragments of dims' tiles: word w gives one (f16) or two (8-bit) tiles of 16 dims
+        auto v_frag = [&](int tile_i, uint32_t (&f)[4]) {
+            if constexpr (Q8) {
+                const int w = tile_i >> 1;
+                const uint32_t sel = tile_i & 1 ? 0x7362u : 0x5140u;
+                const uint32_t x = prmt(vw[0][w], vw[1][w], sel), y = prmt(vw[2][w], vw[3][w], sel);
+                f[0] = e4m3x2_to_f16x2(uint16_t(x)), f[1] = e4m3x2_to_f16x2(uint16_t(x >> 16));
+                f[2] = e4m3x2_to_f16x2(uint16_t(y)), f[3] = e4m3x2_to_f16x2(uint16_t(y >> 16));
+            } else {
+                f[0] = prmt(vw[0][tile_i], vw[1][tile_i], 0x5410u), f[1] = prmt(vw[0][tile_i], vw[1][tile_i], 0x7632u);
+                f[2] = prmt(vw[2][tile_i], vw[3][tile_i], 0x5410u), f[3] = prmt(vw[2][tile_i], vw[3][tile_i], 0x7632u);
+            }
+        };
+        // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
+        // scores, V from the end of its P V. The first group's fly while the queries are read.
+        int k = k_begin;
+        int page = page_of(k), next_page = page_of(k + 1);
+        if (page >= 0) {
+            load_k(page, key_of(k));
+            load_v(page, key_of(k));
         }
-    };
-    // K and V of a group are in flight as soon as their registers are free: K of the next from the end of this one's
-    // scores, V from the end of its P V. The first group's fly while the queries are read.
-    int k = k_begin;
-    int page = page_of(k), next_page = page_of(k + 1);
-    if (page >= 0) {
-        load_k(page, key_of(k));
-        load_v(page, key_of(k));
-    }
 
-    // ---- queries as B fragments: for each step of 16 dims this lane's four of column g
-    uint32_t qf[NT][kSteps][2];
-    float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two (* log2 e without a cap)
-    int qpos[NT][TL::kLaneRows];
-    float slope[NT][TL::kLaneRows];
-    const float unit = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
+        // ---- queries as B fragments: for each step of 16 dims this lane's four of column g
+        uint32_t qf[NT][kSteps][2];
+        float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two (* log2 e without a cap)
+        int qpos[NT][TL::kLaneRows];
+        float slope[NT][TL::kLaneRows];
+        const float unit = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int r = nt * TL::kRowsPer + (HILO ? g >> 1 : g);
-        float q[kSteps][4];
-        float most = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) q[i][e] = 0.0f;
-        if (r < rows) {
-            const int rt = over_g(r0 + r);
-            const int64_t off = int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + r0 + r - rt * G) * a.q_head;
-            auto fetch = [&](auto* p) {
-                const bool vec = (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0;
-#pragma unroll
-                for (int i = 0; i < kSteps; i++) {
-                    // one word of an 8-bit row, two words of an f16 row
-                    const int d = Q8 ? (W::kK >= 4 ? 64 * (i / 4) + 16 * t + 4 * (i % 4) : 8 * t + 4 * i) : 32 * (i / 2) + 8 * t + 4 * (i % 2);
-                    load_row<4>(p + d, vec, q[i]);
-                }
-            };
-            if constexpr (HILO) fetch(static_cast<const float*>(a.q) + off);
-            else if (a.type == kTF16) fetch(static_cast<const __half*>(a.q) + off);
-            else fetch(static_cast<const __nv_bfloat16*>(a.q) + off);
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = nt * TL::kRowsPer + (HILO ? g >> 1 : g);
+            float q[kSteps][4];
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) most = fmaxf(most, finite_abs(q[i][e]));
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const float up = row_up(most);
+                for (int e = 0; e < 4; e++) q[i][e] = 0.0f;
+            if (r < rows) {
+                const int rt = over_g(r0 + r);
+                const int64_t off = int64_t(row0 + rt) * a.q_token + int64_t(kvh * G + r0 + r - rt * G) * a.q_head;
+                auto fetch = [&](auto* p) {
+                    const bool vec = (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0;
 #pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t hi2 = h2u(__floats2half2_rn(q[i][2 * h] * up, q[i][2 * h + 1] * up)), lo2 = 0;
-                if constexpr (HILO) split_hilo(q[i][2 * h] * up, q[i][2 * h + 1] * up, hi2, lo2);
-                qf[nt][i][h] = HILO && (g & 1) ? lo2 : hi2;
-            }
-        const float down = unit / up;
-#pragma unroll
-        for (int y = 0; y < TL::kLaneRows; y++) {
-            const int rr = HILO ? t : 2 * t + y, r2 = nt * TL::kRowsPer + rr, rt = over_g(r0 + r2);
-            qscale[nt][y] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
-            qpos[nt][y] = r2 < rows ? held - n + rt : kNoRow;
-            slope[nt][y] = a.slopes && r2 < rows ? a.slopes[kvh * G + r0 + r2 - rt * G] * kLog2e : 0.0f;
-        }
-    }
-
-    float acc[NT][kSteps][4];
-    float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];
-    float vref = 0.0f;  // the value scale that the accumulators are in units of
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
-#pragma unroll
-        for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = -INFINITY, l[nt][r] = 0.0f;
-    }
-    const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
-
-#pragma unroll 1
-    for (; k < k_end; k++) {
-        const int j0 = key_of(k), j1 = key_of(k + 1);
-        const int after = page_of(k + 2);
-        if (page < 0) {
-            page = next_page, next_page = after;
-            if (page >= 0) {
-                load_k(page, j1);
-                load_v(page, j1);
-            }
-            continue;
-        }
-        // ---- scores
-        float sc[NT][4];
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            uint32_t f[4];
-            if constexpr (Q8) {
-                f[0] = e4m3x2_to_f16x2(uint16_t(kw[0][i])), f[1] = e4m3x2_to_f16x2(uint16_t(kw[1][i]));
-                f[2] = e4m3x2_to_f16x2(uint16_t(kw[0][i] >> 16)), f[3] = e4m3x2_to_f16x2(uint16_t(kw[1][i] >> 16));
-            } else {
-                f[0] = kw[0][2 * i], f[1] = kw[1][2 * i], f[2] = kw[0][2 * i + 1], f[3] = kw[1][2 * i + 1];
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (i == 0) mma16816_z(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
-                else mma16816(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
-            }
-        }
-        const float ks_now = ks;
-        page = next_page, next_page = after;
-        if (page >= 0) load_k(page, j1);
-        // ---- scale, cap, bias, masks
-        // open: every key of the group is seen by every row of the tile
-        const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= pos_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
-        uint32_t seen_bits = 0;  // per lane: (nt, row, key) -> seen
-        float z[NT][TL::kLaneRows][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int r = 0; r < TL::kLaneRows; r++) {
-                const float f = qscale[nt][r] * ks_now;
-#pragma unroll
-                for (int h = 0; h < 2; h++) z[nt][r][h] = (HILO ? sc[nt][2 * h] + sc[nt][2 * h + 1] : sc[nt][2 * h + r]) * f;
-            }
-        if (a.softcap > 0.0f) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int r = 0; r < TL::kLaneRows; r++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) z[nt][r][h] = a.softcap * kLog2e * tanh_abs(z[nt][r][h] * inv_cap);
-        }
-        if (a.slopes) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int r = 0; r < TL::kLaneRows; r++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) z[nt][r][h] = fmaf(slope[nt][r], float(j0 + g + 8 * h - qpos[nt][r]), z[nt][r][h]);
-        }
-        if (!open) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int r = 0; r < TL::kLaneRows; r++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int j = j0 + g + 8 * h, at = qpos[nt][r];
-                        const bool see = (j < len && j <= at && (!a.window || at - j < a.window)) || (j < prefix && at != kNoRow);
-                        if (see) seen_bits |= 1u << (nt * 4 + r * 2 + h);
-                        else z[nt][r][h] = -INFINITY;
+                    for (int i = 0; i < kSteps; i++) {
+                        // one word of an 8-bit row, two words of an f16 row
+                        const int d = Q8 ? (W::kK >= 4 ? 64 * (i / 4) + 16 * t + 4 * (i % 4) : 8 * t + 4 * i) : 32 * (i / 2) + 8 * t + 4 * (i % 2);
+                        load_row<4>(p + d, vec, q[i]);
                     }
-        }
-        // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact) and value scale
-        const float vs_now = vs;
-        bool up = false;
-        float top[NT][TL::kLaneRows];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int r = 0; r < TL::kLaneRows; r++) {
-                float x = fmaxf(z[nt][r][0], z[nt][r][1]);
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                top[nt][r] = x;
-                up |= x > m[nt][r] + kLazy;
-            }
-        const bool v_up = Q8 && vs_now > kVLazy * vref;
-        if (__any_sync(0xffffffffu, up) || v_up) {
-            float fv = 1.0f;
-            if (v_up) {
-                fv = __fdividef(vref, vs_now);
-                vref = vs_now;
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float f[TL::kLaneRows];
-#pragma unroll
-                for (int r = 0; r < TL::kLaneRows; r++) {
-                    f[r] = 1.0f;
-                    if (top[nt][r] > m[nt][r] + kLazy) {
-                        f[r] = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
-                        m[nt][r] = top[nt][r];
-                        l[nt][r] *= f[r];
-                    }
-                    f[r] *= fv;
-                }
+                };
+                if constexpr (HILO) fetch(static_cast<const float*>(a.q) + off);
+                else if (a.type == kTF16) fetch(static_cast<const __half*>(a.q) + off);
+                else fetch(static_cast<const __nv_bfloat16*>(a.q) + off);
 #pragma unroll
                 for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[nt][i][e] *= f[HILO ? 0 : e & 1];
+                    for (int e = 0; e < 4; e++) most = fmaxf(most, finite_abs(q[i][e]));
+            }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const float up = row_up(most);
+#pragma unroll
+            for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t hi2 = h2u(__floats2half2_rn(q[i][2 * h] * up, q[i][2 * h + 1] * up)), lo2 = 0;
+                    if constexpr (HILO) split_hilo(q[i][2 * h] * up, q[i][2 * h + 1] * up, hi2, lo2);
+                    qf[nt][i][h] = HILO && (g & 1) ? lo2 : hi2;
+                }
+            const float down = unit / up;
+#pragma unroll
+            for (int y = 0; y < TL::kLaneRows; y++) {
+                const int rr = HILO ? t : 2 * t + y, r2 = nt * TL::kRowsPer + rr, rt = over_g(r0 + r2);
+                qscale[nt][y] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
+                qpos[nt][y] = r2 < rows ? held - n + rt : kNoRow;
+                slope[nt][y] = a.slopes && r2 < rows ? a.slopes[kvh * G + r0 + r2 - rt * G] * kLog2e : 0.0f;
             }
         }
-        // ---- weights as B fragments, in units of the reference scale
-        uint32_t pf[NT][2];
-        const float ratio = Q8 ? (vref > 0.0f ? __fdividef(vs_now, vref) : 0.0f) : 1.0f;
+
+        float acc[NT][kSteps][4];
+        float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];
+        float vref = 0.0f;  // the value scale that the accumulators are in units of
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float p[2][TL::kLaneRows];
 #pragma unroll
-            for (int r = 0; r < TL::kLaneRows; r++) {
-                const float ref = (m[nt][r] == -INFINITY ? 0.0f : m[nt][r]) - kLift;
-                p[0][r] = ex2(z[nt][r][0] - ref), p[1][r] = ex2(z[nt][r][1] - ref);
-                l[nt][r] += p[0][r] + p[1][r];
-            }
+            for (int i = 0; i < kSteps; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t hl;
-                if constexpr (HILO) {
-                    const float x = p[h][0] * ratio;
-                    const __half hi1 = __float2half_rn(x);
-                    hl = h2u(__halves2half2(hi1, __float2half_rn(x - __half2float(hi1))));
-                } else {
-                    hl = h2u(__floats2half2_rn(p[h][0] * ratio, p[h][1] * ratio));
-                }
-                pf[nt][h] = movmatrix(hl);
-            }
+                for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = -INFINITY, l[nt][r] = 0.0f;
         }
-        // ---- P V
-        if (!open) {
-            // Values that no row of the tile sees are zeroed (they may hold anything); values that only some rows see
-            // and that are not finite join the accumulators of the rows that see them, key by key.
-            bool odd = false;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int j = j0 + 2 * t + (x & 1) + 8 * (x >> 1);
-                const bool dead = !((j < hi && j >= lo) || j < prefix);
-#pragma unroll
-                for (int w = 0; w < W::kV; w++) {
-                    if (dead) vw[x][w] = 0;
-                    odd |= odd_lanes<Q8>(vw[x][w]) != 0;
-                }
-            }
-            if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-                for (int key = 0; key < 16; key++) {
-                    // who sees this key: the lanes that hold its scores say so
-                    const uint32_t bits = __shfl_sync(0xffffffffu, seen_bits, (key & 7) * 4 + t) >> (key >> 3);
-                    const int mine = (key >> 3) * 2 + (key & 1);
-                    const bool here = (key & 7) >> 1 == t;
-                    uint32_t keep[4][W::kV];
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-#pragma unroll
-                        for (int w = 0; w < W::kV; w++) {
-                            keep[x][w] = vw[x][w];
-                            const uint32_t mask = here && x == mine ? odd_lanes<Q8>(vw[x][w]) : 0u;
-                            vw[x][w] &= mask;
-                            keep[x][w] &= ~mask;
-                        }
-#pragma unroll
-                    for (int i = 0; i < kSteps; i++) {
-                        uint32_t f[4];
-                        v_frag(i, f);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            float d[4];
-                            mma16816_z(d, f, pf[nt][0], pf[nt][1]);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int r = HILO ? 0 : e & 1;
-                                if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e];
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-#pragma unroll
-                        for (int w = 0; w < W::kV; w++) vw[x][w] = keep[x][w];
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) {
-            uint32_t f[4];
-            v_frag(i, f);
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if constexpr (HILO) {
-                    // added outside the MMA, which truncates: on the accumulator itself every group took 3e-8 off it
-                    // (an error of 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time; 16-bit results do not see it)
-                    float d[4];
-                    mma16816_z(d, f, pf[nt][0], pf[nt][1]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[nt][i][e] += d[e];
-                } else {
-                    mma16816(acc[nt][i], f, pf[nt][0], pf[nt][1]);
-                }
-            }
-        }
-        if (page >= 0) load_v(page, j1);
-    }
+        const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
-    // ---- an item of this warp's own to the output, a part of one to shared memory
-    const bool first = k_begin == 0, ends = k_end == cnt;
-    float* st0 = sm + (2 * warp + first) * TL::kState;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int r = 0; r < TL::kLaneRows; r++) {
-            float sum = l[nt][r];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
-            float* st = st0 + row * TL::kPitch;
-            if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum;
+#pragma unroll 1
+        for (; k < k_end; k++) {
+            const int j0 = key_of(k), j1 = key_of(k + 1);
+            const int after = page_of(k + 2);
+            if (page < 0) {
+                page = next_page, next_page = after;
+                if (page >= 0) {
+                    load_k(page, j1);
+                    load_v(page, j1);
+                }
+                continue;
+            }
+            // ---- scores
+            float sc[NT][4];
 #pragma unroll
             for (int i = 0; i < kSteps; i++) {
-                float2 v;
-                v.x = HILO ? acc[nt][i][0] + acc[nt][i][1] : acc[nt][i][r];
-                v.y = HILO ? acc[nt][i][2] + acc[nt][i][3] : acc[nt][i][2 + r];
-                if (Q8) v.x *= vref, v.y *= vref;
-                const int d = Q8 ? (HD / 8) * g + 2 * i : W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : 4 * g + 2 * i;
-                *reinterpret_cast<float2*>(st + d) = v;
+                uint32_t f[4];
+                if constexpr (Q8) {
+                    f[0] = e4m3x2_to_f16x2(uint16_t(kw[0][i])), f[1] = e4m3x2_to_f16x2(uint16_t(kw[1][i]));
+                    f[2] = e4m3x2_to_f16x2(uint16_t(kw[0][i] >> 16)), f[3] = e4m3x2_to_f16x2(uint16_t(kw[1][i] >> 16));
+                } else {
+                    f[0] = kw[0][2 * i], f[1] = kw[1][2 * i], f[2] = kw[0][2 * i + 1], f[3] = kw[1][2 * i + 1];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (i == 0) mma16816_z(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
+                    else mma16816(sc[nt], f, qf[nt][i][0], qf[nt][i][1]);
+                }
+            }
+            const float ks_now = ks;
+            page = next_page, next_page = after;
+            if (page >= 0) load_k(page, j1);
+            // ---- scale, cap, bias, masks
+            // open: every key of the group is seen by every row of the tile
+            const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= pos_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
+            uint32_t seen_bits = 0;  // per lane: (nt, row, key) -> seen
+            float z[NT][TL::kLaneRows][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++) {
+                    const float f = qscale[nt][r] * ks_now;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) z[nt][r][h] = (HILO ? sc[nt][2 * h] + sc[nt][2 * h + 1] : sc[nt][2 * h + r]) * f;
+                }
+            if (a.softcap > 0.0f) {
+                float most = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) most = fmaxf(most, fabsf(z[nt][r][h] *= inv_cap));
+                const bool small = __all_sync(0xffffffffu, most <= 0.5f);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float y = z[nt][r][h];
+                            z[nt][r][h] = a.softcap * kLog2e * (small || fabsf(y) <= 0.5f ? tanh_small(y) : tanh_abs(y));
+                        }
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) z[nt][r][h] = fmaf(slope[nt][r], float(j0 + g + 8 * h - qpos[nt][r]), z[nt][r][h]);
+            }
+            if (!open) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int r = 0; r < TL::kLaneRows; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int j = j0 + g + 8 * h, at = qpos[nt][r];
+                            const bool see = (j < len && j <= at && (!a.window || at - j < a.window)) || (j < prefix && at != kNoRow);
+                            if (see) seen_bits |= 1u << (nt * 4 + r * 2 + h);
+                            else z[nt][r][h] = -INFINITY;
+                        }
+            }
+            // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact) and value scale
+            const float vs_now = vs;
+            bool up = false;
+            float top[NT][TL::kLaneRows];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++) {
+                    float x = fmaxf(z[nt][r][0], z[nt][r][1]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    top[nt][r] = x;
+                    up |= x > m[nt][r] + kLazy;
+                }
+            const bool v_up = Q8 && vs_now > kVLazy * vref;
+            if (__any_sync(0xffffffffu, up) || v_up) {
+                float fv = 1.0f;
+                if (v_up) {
+                    fv = __fdividef(vref, vs_now);
+                    vref = vs_now;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float f[TL::kLaneRows];
+#pragma unroll
+                    for (int r = 0; r < TL::kLaneRows; r++) {
+                        f[r] = 1.0f;
+                        if (top[nt][r] > m[nt][r] + kLazy) {
+                            f[r] = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
+                            m[nt][r] = top[nt][r];
+                            l[nt][r] *= f[r];
+                        }
+                        f[r] *= fv;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[nt][i][e] *= f[HILO ? 0 : e & 1];
+                }
+            }
+            // ---- weights as B fragments, in units of the reference scale
+            uint32_t pf[NT][2];
+            const float ratio = Q8 ? (vref > 0.0f ? __fdividef(vs_now, vref) : 0.0f) : 1.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float p[2][TL::kLaneRows];
+#pragma unroll
+                for (int r = 0; r < TL::kLaneRows; r++) {
+                    const float ref = (m[nt][r] == -INFINITY ? 0.0f : m[nt][r]) - kLift;
+                    p[0][r] = ex2(z[nt][r][0] - ref), p[1][r] = ex2(z[nt][r][1] - ref);
+                    l[nt][r] += p[0][r] + p[1][r];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t hl;
+                    if constexpr (HILO) {
+                        const float x = p[h][0] * ratio;
+                        const __half hi1 = __float2half_rn(x);
+                        hl = h2u(__halves2half2(hi1, __float2half_rn(x - __half2float(hi1))));
+                    } else {
+                        hl = h2u(__floats2half2_rn(p[h][0] * ratio, p[h][1] * ratio));
+                    }
+                    pf[nt][h] = movmatrix(hl);
+                }
+            }
+            // ---- P V
+            if (!open) {
+                // Values that no row of the tile sees are zeroed (they may hold anything); values that only some rows see
+                // and that are not finite join the accumulators of the rows that see them, key by key.
+                bool odd = false;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int j = j0 + 2 * t + (x & 1) + 8 * (x >> 1);
+                    const bool dead = !((j < hi && j >= lo) || j < prefix);
+#pragma unroll
+                    for (int w = 0; w < W::kV; w++) {
+                        if (dead) vw[x][w] = 0;
+                        odd |= odd_lanes<Q8>(vw[x][w]) != 0;
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                    for (int key = 0; key < 16; key++) {
+                        // who sees this key: the lanes that hold its scores say so
+                        const uint32_t bits = __shfl_sync(0xffffffffu, seen_bits, (key & 7) * 4 + t) >> (key >> 3);
+                        const int mine = (key >> 3) * 2 + (key & 1);
+                        const bool here = (key & 7) >> 1 == t;
+                        uint32_t keep[4][W::kV];
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll
+                            for (int w = 0; w < W::kV; w++) {
+                                keep[x][w] = vw[x][w];
+                                const uint32_t mask = here && x == mine ? odd_lanes<Q8>(vw[x][w]) : 0u;
+                                vw[x][w] &= mask;
+                                keep[x][w] &= ~mask;
+                            }
+#pragma unroll
+                        for (int i = 0; i < kSteps; i++) {
+                            uint32_t f[4];
+                            v_frag(i, f);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                float d[4];
+                                mma16816_z(d, f, pf[nt][0], pf[nt][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const int r = HILO ? 0 : e & 1;
+                                    if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e];
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll
+                            for (int w = 0; w < W::kV; w++) vw[x][w] = keep[x][w];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; i++) {
+                uint32_t f[4];
+                v_frag(i, f);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if constexpr (HILO) {
+                        // added outside the MMA, which truncates: on the accumulator itself every group took 3e-8 off it
+                        // (an error of 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time; 16-bit results do not see it)
+                        float d[4];
+                        mma16816_z(d, f, pf[nt][0], pf[nt][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[nt][i][e] += d[e];
+                    } else {
+                        mma16816(acc[nt][i], f, pf[nt][0], pf[nt][1]);
+                    }
+                }
+            }
+            if (page >= 0) load_v(page, j1);
+        }
+
+        // ---- an item of this warp's own to the output, a part of one to shared memory
+        const bool first = k_begin == 0, ends = k_end == cnt;
+        float* st0 = sm + (2 * warp + first) * TL::kState;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int r = 0; r < TL::kLaneRows; r++) {
+                float sum = l[nt][r];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
+                float* st = st0 + row * TL::kPitch;
+                if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum;
+#pragma unroll
+                for (int i = 0; i < kSteps; i++) {
+                    float2 v;
+                    v.x = HILO ? acc[nt][i][0] + acc[nt][i][1] : acc[nt][i][r];
+                    v.y = HILO ? acc[nt][i][2] + acc[nt][i][3] : acc[nt][i][2 + r];
+                    if (Q8) v.x *= vref, v.y *= vref;
+                    const int d = Q8 ? (HD / 8) * g + 2 * i : W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : 4 * g + 2 * i;
+                    *reinterpret_cast<float2*>(st + d) = v;
+                }
             }
         }
-    }
-    __syncwarp();
-    if (!CL && first && ends) {
-        for (int y = lane; y < rows * (HD / 4); y += 32) {
-            const int row = y / (HD / 4), d = y % (HD / 4) * 4;
-            const float* st = st0 + row * TL::kPitch;
-            put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d), st[HD + 1]);
-        }
         __syncwarp();
-    } else if (lane == 0) {
-        meta[2 * warp + first] = make_int4(s * n_kv + kvh, (first ? 1 : 0) | (ends ? 2 : 0), row0, rows);
-    }
-    if (first && !ends) starts_last = int((((item + cnt) * warps - 1) / total) / kWarps);
-    x = item + k_end;
-    if (!CL && x < x_end && ++kvh == n_kv) {
-        kvh = 0;
-        do s++;
-        while (pre[s + 1] == pre[s]);
-        cnt = pre[s + 1] - pre[s];
-    }
+        if (!CL && first && ends) {
+            for (int y = lane; y < rows * (HD / 4); y += 32) {
+                const int row = y / (HD / 4), d = y % (HD / 4) * 4;
+                const float* st = st0 + row * TL::kPitch;
+                put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d), st[HD + 1]);
+            }
+            __syncwarp();
+        } else if (lane == 0) {
+            meta[2 * warp + first] = make_int4(s * n_kv + kvh, (first ? 1 : 0) | (ends ? 2 : 0), row0, rows);
+        }
+        if (first && !ends) starts_last = int((((item + cnt) * warps - 1) / total) / kWarps);
+        x = item + k_end;
+        if (!CL && x < x_end && ++kvh == n_kv) {
+            kvh = 0;
+            do s++;
+            while (pre[s + 1] == pre[s]);
+            cnt = pre[s + 1] - pre[s];
+        }
     }
     __syncthreads();
     if constexpr (CL) {
@@ -769,6 +780,16 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const neko_paged_attent
     }
 }
 
+// Few items of few keys: a cluster of CTAs each, about two groups of 16 keys for every warp, which need neither scratch memory
+// nor the second kernel (one chat, 777 keys: 12 us a call, 8.4 on the GPU, against 16 and 10.4). 0: not that few, else the CTAs
+// of a cluster. Where an SM holds one CTA, clusters of 8 find no room side by side (4: 13.8 us, 8: 23.3).
+int small_ranks(int64_t items, int64_t per_item, int64_t room) {
+    const int most = room > num_sms() ? 8 : 4;
+    int ranks = 1;
+    while (ranks < most && per_item > 16 * ranks && items * ranks * 2 <= room) ranks *= 2;
+    return items * ranks <= room && per_item <= 64 * ranks ? ranks : 0;
+}
+
 template <int HD, bool Q8, bool HILO, int NT>
 cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     using TL = Tile<HD, HILO, NT>;
@@ -786,13 +807,8 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t items = int64_t(c.n_kv) * c.n_seq;
     const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(num_sms()) * kCtas<HD, Q8, NT>, std::max(groups, items) / kWarps)));
     const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
-    // Few items of few keys: a cluster of CTAs each, two groups for every warp, which need neither scratch memory nor the
-    // second kernel (one chat, 777 keys: 12 us a call, 8.4 on
-    // the GPU, against 16 and 10.4 of the variant below)
     const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, room = int64_t(num_sms()) * kCtas<HD, Q8, NT>;
-    int ranks = 1;
-    while (ranks < 8 && per_item > 16 * ranks && items * row_tiles * ranks * 2 <= room) ranks *= 2;
-    if (items * row_tiles * ranks <= room && per_item <= 64 * ranks && c.n_kv <= 65535) {
+    if (const int ranks = c.n_kv <= 65535 ? small_ranks(items * row_tiles, per_item, room) : 0) {
         auto* small = paged_decode_kernel<HD, Q8, HILO, NT, true>;
         if (cudaError_t e = ensure_dyn_smem(small, TL::smem_small()); e != cudaSuccess) return e;
         p.ranks_log = 31 - __builtin_clz(ranks);
@@ -835,8 +851,17 @@ cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st) {
-    const int64_t rows = int64_t(a.max_new) * (a.n_head / a.cache.n_kv);
-    if (rows > kPromptRows && a.cache.head_dim >= 64) return launch_paged_prompt(a, st);
+    // Rows past 16 go to the tensor cores' kernel (8 x 4,000 f16 keys, f32 rows: 16 rows 61 us each way, 20 rows 62 against 90),
+    // but not where this one's small variant takes them (64 rows on 600 keys: 12 us against 22) nor up to 32 rows on many 8-bit
+    // keys, which that one would convert for few rows (48 x 2,000 keys: 252 us against 316, 16-bit rows 139 against 277; of fewer
+    // than 8,192 groups of 16 keys, 5,000 keys: 43 against 35). Head dim 32 stays here.
+    const neko_paged_cache& c = a.cache;
+    const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv), items = int64_t(c.n_seq) * c.n_kv;
+    if (rows > kPromptRows && c.head_dim >= 64) {
+        const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, tile = a.type == NEKO_T_F32 ? 8 : 16;
+        const bool many = c.type == NEKO_T_E4M3 && rows <= 2 * kPromptRows && items * per_item >= 8192;
+        if (!many && !small_ranks(items * ((rows + tile - 1) / tile), per_item, num_sms())) return launch_paged_prompt(a, st);
+    }
     const bool q8 = a.cache.type == NEKO_T_E4M3;
     switch (a.cache.head_dim) {
         case 32: return q8 ? by_rows<32, true>(a, st) : by_rows<32, false>(a, st);

@@ -753,7 +753,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             }
                         } else {
 #pragma unroll
-                            for (int x = 0; x < 32; x++) u[x] = __float_as_uint(cap * tanh_abs(__uint_as_float(u[x])));
+                            for (int x = 0; x < 32; x++) {
+                                const float y = __uint_as_float(u[x]);
+                                u[x] = __float_as_uint(cap * (fabsf(y) <= 0.5f ? tanh_small(y) : tanh_abs(y)));
+                            }
                         }
                     }
                     if (a.slopes) {

@@ -14,7 +14,7 @@ constexpr int kScaleMinExp = -100;  // scale of a block of zeros: 2^-100
 
 cudaError_t launch_paged_append(const neko_paged_append_args& a, cudaStream_t st);
 cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st);
-// The tcgen05 kernel for more than kPromptRows packed rows (new tokens x query heads per KV head), head dim 64 or 128.
+// The tcgen05 kernel, head dim 64 or 128; launch_paged_attention says when (packed rows: new tokens x query heads per KV head).
 cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st);
 constexpr int kPromptRows = 16;
 

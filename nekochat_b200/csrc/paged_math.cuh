@@ -16,6 +16,16 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float tanh_abs(float x) {
     return 1.0f - __fdividef(2.0f, 1.0f + ex2(fminf(x * (2.0f * kLog2e), 64.0f)));
 }
+// tanh of |x| <= 1/2 as an odd polynomial of degree 9 (least maximum error there: 3e-9): no special functions, and exact to the
+// last places where tanh_abs is off by a few 2^-23, which a cap of 50 makes 1e-5 of a score.
+__device__ __forceinline__ float tanh_small(float x) {
+    const float y = x * x;
+    float p = fmaf(y, 0.016737453639507294f, -0.05276207625865936f);
+    p = fmaf(p, y, 0.13320569694042206f);
+    p = fmaf(p, y, -0.3333277702331543f);
+    p = fmaf(p, y, 0.9999999403953552f);
+    return p * x;
+}
 __device__ __forceinline__ float finite_abs(float x) {
     const float m = fabsf(x);
     return m <= 3.402823466e38f ? m : 0.0f;

@@ -500,3 +500,16 @@ def test_long_steps_keep_f32_precision(torch, n, L, heads, n_kv, hd):
         for h in range(heads):
             want = torch.softmax(kk[h * n_kv // heads] @ q[s, h].double() * hd ** -0.5, -1) @ vv[h * n_kv // heads]
             assert (got[s, h] - want).norm() <= 1.5e-6 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_prompts_whose_keys_are_split(torch, dtype, e4m3):
+    """Few row tiles on thousands of keys: the keys of a row tile go to several CTAs, which join."""
+    rng = np.random.default_rng(61)
+    cache = Cache(torch, rng, [1900], 2, 32, 128, e4m3)
+    cache.fill(rng, [1900])
+    if e4m3:
+        cache.vs.copy_(torch.from_numpy((2.0 ** rng.integers(-8, 5, tuple(cache.vs.shape))).astype(np.float32)).cuda())
+    attend(torch, cache, [1900], [150], 8, dtype, 62)
+    attend(torch, cache, [1900], [150], 8, dtype, 62, window=700, softcap=20.0, prefix=[100])

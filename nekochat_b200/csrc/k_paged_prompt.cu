@@ -1,6 +1,11 @@
 // Attention of many query rows over a paged cache (neko_op_paged_attention): prompts and long continuations, on
 // tcgen05.
 //
+// A prompt of 8,192 bf16 tokens, 16 heads on 8: 320 us, 860 TFLOP/s of the causal half's products (51 % of the measured rate).
+// Per pair of row tiles and 128 keys about 4,080 cycles against 2,048 of the UMMAs: each row tile's chain is S, softmax (2,010
+// cycles: TMEM reads 330, maximum and meeting 500, exponentials 1,110), P V and S again (1,190), and the two tiles take
+// turns. f32 rows take twice the UMMAs (5,900 cycles).
+//
 // The packed rows of a (sequence, KV head) are its new tokens times the G query heads that share the KV head. A CTA
 // takes two tiles of 128 rows (one when there are no more) and walks the keys in tiles of 128:
 //   S = Q K^T in TMEM, weights P back into TMEM over S (f16), O += P V in TMEM, all accumulation f32.
@@ -23,6 +28,8 @@
 // order. Every wait is bounded and gives up once another role has failed.
 #include <cooperative_groups.h>
 
+#include <array>
+
 #include "paged.cuh"
 #include "paged_math.cuh"
 #include "tc5_core.cuh"
@@ -37,7 +44,7 @@ namespace {
 constexpr int kRows = 128, kKeys = 128;  // of a tile
 constexpr int kSoftWarps = 16, kLoadWarp = 16, kMmaWarp = 19, kThreads = 20 * 32;  // 96 registers a thread
 constexpr int kLoaders = 96;
-constexpr int kCopyTiles = 3;
+constexpr int kCopyTiles = 2;
 constexpr int64_t kCopyBytes = int64_t(1) << 31;
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
@@ -53,7 +60,7 @@ constexpr float kLift = 15.0f - kLazy - kVLazy;
 // tiles, 2.4e-6 every 16; ragged prompts on 3,000 keys: 669 and 646 us).
 constexpr float kDrop = 3.2e-8f;
 constexpr int kFlush = 8;
-constexpr int64_t kFlushBytes = int64_t(1) << 30;
+constexpr int64_t kFlushBytes = int64_t(1) << 30;  // sums of more CTAs stay in TMEM (batches padded to their longest prompt can be large)
 constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
 constexpr float kVNone = -126.0f;
 constexpr float kGone = -1.0f;
@@ -1001,9 +1008,11 @@ cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, in
     const neko_paged_cache& c = a.cache;
     if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, p, items, nullptr, st);
     // Each CTA would convert its keys again: from kCopyTiles CTAs per (sequence, KV head) on, they are converted once,
-    // if the copies stay below kCopyBytes.
+    // if the copies stay below kCopyBytes. Not copied and copied, f32 rows: 2 CTAs each (8 x 2,048 keys, 256 tokens) 128 and
+    // 113 us, (4 x 8,192) 238 and 201; 6 each (1 x 8,192, 768 tokens) 349 and 239. One each gains less (16 x 4,096 keys,
+    // 128 tokens: 256 and 238), for copies that are twice the cache.
     const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
-    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes || c.n_seq > 65535) return by_type<HD, kCodes>(a, p, items, nullptr, st);
+    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes) return by_type<HD, kCodes>(a, p, items, nullptr, st);
     void* mem = nullptr;
     if (cudaError_t e = scratch_alloc(&mem, size_t(bytes), st); e != cudaSuccess) return e;
     cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
@@ -1013,20 +1022,68 @@ cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, in
     return e;
 }
 
+// How many clusters of 1 << log CTAs run at once (a CTA fills an SM; an SM left over in its GPC stays idle).
+template <int HD>
+int clusters_at_once(int log) {
+    static const std::array<int, 4> fits = [] {
+        std::array<int, 4> out = {};
+        auto* fn = paged_prompt_kernel<HD, kCodes, true>;
+        const size_t smem = PL<HD, true>::kSmem;
+        const bool ready = ensure_dyn_smem(fn, smem) == cudaSuccess;
+        for (int i = 0; i < 4; i++) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1u << i;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(1u << i);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (!ready || cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) {
+                cudaGetLastError();
+                n = std::max(1, num_sms() >> (i + 1));
+            }
+            out[size_t(i)] = i ? n : num_sms();
+        }
+        return out;
+    }();
+    return fits[size_t(log)];
+}
+
+// Row tiles of a CTA and CTAs of a cluster: what takes the least time by the measured cost of 128 keys (one and two row
+// tiles, in tenths of a microsecond), of a CTA's start and of the join. Two row tiles share a CTA's keys and its tensor core
+// (one prompt of 768 f32 tokens on 8,192 keys, 8 KV heads: one row tile each 239 us, two in clusters of 2 159); one is
+// better where that fills SMs (512 bf16 tokens on 2,048 keys: 30.4 us, two in clusters of 4 33.7). Without clusters 64 f32 tokens
+// on 8,192 keys take 207 us, with clusters of 8 39; 16 clusters of 8 do not run at once and 90 us become 62 with 8 of them.
+template <int HD>
+int64_t split(PromptPlan& p, int64_t tiles, int64_t heads, int64_t key_tiles, bool f32) {
+    const int64_t step[2] = {f32 ? 34 : 23, f32 ? 41 : 26}, start = 80, join[2] = {50, 150};
+    int64_t best = INT64_MAX, items = 0;
+    for (int two = 0; two < (tiles > 1 ? 2 : 1); two++) {
+        const int64_t row_tiles = (tiles + two) / (1 + two), n = heads * row_tiles;
+        for (int log = 0; log < 4 && (log == 0 || key_tiles >= (1 << log)); log++) {
+            const int64_t at_once = clusters_at_once<HD>(log), rounds = (n + at_once - 1) / at_once;
+            const int64_t time = rounds * (start + ((key_tiles + (1 << log) - 1) >> log) * step[two] + (log ? join[two] : 0));
+            if (time >= best) continue;
+            best = time, items = n;
+            p.tiles_per = 1 + two, p.row_tiles = int(row_tiles), p.ranks = 1 << log;
+        }
+    }
+    return items;
+}
+
 template <int HD>
 cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
     const neko_paged_cache& c = a.cache;
     const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
     PromptPlan p;
-    // two row tiles per CTA unless that leaves SMs without work
-    const int64_t tiles = (rows + kRows - 1) / kRows, heads = int64_t(c.n_seq) * c.n_kv;
-    p.tiles_per = tiles > 1 && heads * ((tiles + 1) / 2) * 2 > num_sms() ? 2 : 1;
-    p.row_tiles = int((tiles + p.tiles_per - 1) / p.tiles_per);
-    const int64_t items = heads * p.row_tiles, key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
     p.group = a.n_head / c.n_kv;
     p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
-    p.ranks = 1;
-    while (p.ranks < 8 && items * p.ranks * 2 <= num_sms() && key_tiles >= 2 * p.ranks) p.ranks *= 2;
+    const int64_t key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
+    const int64_t items = split<HD>(p, (rows + kRows - 1) / kRows, int64_t(c.n_seq) * c.n_kv, key_tiles, a.type == NEKO_T_F32);
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     p.flush = nullptr;
     void* flush = nullptr;

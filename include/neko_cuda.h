@@ -208,7 +208,8 @@ typedef struct neko_paged_cache {
  * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
  * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new
  * (exact, but for codes that become subnormal). Infinities are stored as +-448 * scale, NaN as NaN.
- * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous. */
+ * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous; token strides
+ * below 2^24 (else NEKO_ERR_UNSUPPORTED). */
 typedef struct neko_paged_append_args {
     neko_paged_cache cache;
     const void *q, *k, *v;
@@ -233,7 +234,8 @@ int neko_op_paged_append(const neko_paged_append_args* args, void* stream);
  * or pos - j < window), or j < prefix[s] (prefix NULL: none). out = sum_j softmax(z)_j v_j over the keys seen, zeros
  * when there are none. A value that is not seen has no effect, whatever it holds. Sums, maxima and accumulators are f32;
  * NEKO_T_F32 queries and weights enter the tensor cores as f16 hi + lo (22 bits), 16-bit ones as one f16.
- * n_head a multiple of n_kv. out rows have type `type` and strides o_token, o_head. */
+ * n_head a multiple of n_kv, at most 16384 sequences (else NEKO_ERR_UNSUPPORTED). out rows have type `type` and strides
+ * o_token, o_head. */
 typedef struct neko_paged_attention_args {
     neko_paged_cache cache;
     const void* q;

@@ -80,6 +80,12 @@ def test_refused_attentions(over):
     assert call("neko_op_paged_attention", ATTEND, ops._ATTEND, tokens=2, n_seq=20000) == -6
 
 
+@pytest.mark.parametrize("over", [dict(k_token=1 << 24), dict(v_token=-(1 << 24)), dict(q_token=1 << 40), dict(o_token=1 << 24)])
+def test_refused_token_strides(over):
+    assert call("neko_op_paged_append", APPEND, ops._APPEND, **dict(dict(tokens=2), **over)) == -6
+    assert b"token strides" in nb.lib().neko_last_error()
+
+
 def test_null_arguments():
     assert nb.lib().neko_op_paged_append(None, None) == -1
     assert nb.lib().neko_op_paged_attention(None, None) == -1

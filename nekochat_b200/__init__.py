@@ -8,6 +8,7 @@ engine binds. It mirrors the engine's interfaces:
   ``begin``/``dispatch``/``flush``/``submit_and_wait`` of the nine :class:`Kernel` ids with the shaders' parameter
   blocks.
 * :mod:`nekochat_b200.ops` - single operators on torch CUDA tensors (device pointers).
+* :mod:`nekochat_b200.paged` - Qwen3 on a paged (f16 or 8-bit) key/value cache, from those operators.
 * :class:`Model` - the native GPT-2 / Qwen3 runner (``Model::forward`` semantics plus batched decode).
 
 There is no CPU fallback: importing works without a GPU, but every call needs the compiled library and a CUDA

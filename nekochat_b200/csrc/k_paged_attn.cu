@@ -1,5 +1,8 @@
-// Attention of few query rows over a paged cache (neko_op_paged_attention): decode steps, short continuations and,
-// one tile of rows after the other, anything else.
+// Attention of few query rows over a paged cache (neko_op_paged_attention): decode steps, short continuations, small
+// prompts, and every head dim of 32.
+//
+// Bound by memory: on contexts of one length 5.9 TB/s from 8-bit pages and 6.4 TB/s from f16 ones (74 x 8,192 tokens, 91 and
+// 99 % of the measured copy rate), 5.3 TB/s on 128 ragged contexts up to 8,192 tokens (227 us); small calls by latency.
 //
 // The packed rows of a (sequence, KV head) are its new tokens times the G query heads that share the KV head, so a key
 // is read once for all of them. Every warp owns groups of 16 keys and works alone (no barrier until the end): scores
@@ -7,8 +10,8 @@
 // its 8 columns. The order of the summed index is free as long as both operands agree, so the fragments come straight
 // from global memory: lane (g, t) holds, for K, 16-byte pieces t, t + 4, .. of key rows g and g + 8, and for V the
 // pieces g, g + 8, .. of key rows 2t, 2t + 1, 2t + 8, 2t + 9; neither K nor V passes through shared memory. 8-bit codes
-// become f16 in registers (exact), keys' scales multiply the scores, values' scales the group's P V before it joins
-// the f32 accumulator. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
+// become f16 in registers (exact), keys' scales multiply the scores, values' scales the weights, relative to a reference
+// that the accumulators are in units of. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
 // 16-bit queries one exact f16 column, weights one f16. Rows are scaled by a power of two into f16's range first.
 // All groups of all items, in order, are dealt out in equal shares to the warps that the GPU holds at a time, whatever
@@ -29,7 +32,6 @@ namespace cg = cooperative_groups;
 namespace neko {
 
 namespace {
-
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;

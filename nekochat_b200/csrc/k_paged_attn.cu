@@ -850,19 +850,34 @@ cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
     return rows <= 8 ? go<HD, Q8, false, 1>(a, st) : go<HD, Q8, false, 2>(a, st);
 }
 
+// Whether a row tile each of more items than SMs costs the tensor cores' kernel, which runs one CTA per SM, more in CTA starts
+// than this kernel takes in all: both by measured costs in nanoseconds (a CTA's start, 128 keys; a row tile's pass, an item and its
+// groups of 16 keys). f32 rows, 448 items: 32 rows on 24 keys 55 us there, 44 here, on 128 keys 57 and 64; 2,048 items:
+// 20 rows on 64 keys 196 and 85, on 512 keys 301 and 315. Of 304 measured shapes the rule makes 79 faster, up to 2.9 times, and 6 of
+// 160 items up to 17 % slower.
+bool starts(int64_t items, int64_t rows, int64_t per_item, bool f32) {
+    const int64_t rounds = (items + num_sms() - 1) / num_sms(), tile = f32 ? 8 : 16, tiles = (rows + tile - 1) / tile;
+    if (rounds == 1 || rows > 128) return false;
+    const int64_t there = 5000 + rounds * (8000 + (per_item + 7) / 8 * (f32 ? 3400 : 2300));
+    const int64_t here = 12000 + tiles * ((f32 ? 3000 : 2000) + items * (per_item + 5) * (f32 ? 13 : 18) / 10);
+    return here < there;
+}
+
 }  // namespace
 
 cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st) {
     // Rows past 16 go to the tensor cores' kernel (8 x 4,000 f16 keys, f32 rows: 16 rows 61 us each way, 20 rows 62 against 90),
     // but not where this one's small variant takes them (64 rows on 600 keys: 12 us against 22) nor up to 32 rows on many 8-bit
     // keys, which that one would convert for few rows (48 x 2,000 keys: 252 us against 316, 16-bit rows 139 against 277; of fewer
-    // than 8,192 groups of 16 keys, 5,000 keys: 43 against 35). Head dim 32 stays here.
+    // than 8,192 groups of 16 keys, 5,000 keys: 43 against 35), nor many short contexts: starts() below. Head dim 32 stays here.
     const neko_paged_cache& c = a.cache;
     const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv), items = int64_t(c.n_seq) * c.n_kv;
     if (rows > kPromptRows && c.head_dim >= 64) {
         const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, tile = a.type == NEKO_T_F32 ? 8 : 16;
         const bool many = c.type == NEKO_T_E4M3 && rows <= 2 * kPromptRows && items * per_item >= 8192;
-        if (!many && !small_ranks(items * ((rows + tile - 1) / tile), per_item, num_sms())) return launch_paged_prompt(a, st);
+        if (!many && !small_ranks(items * ((rows + tile - 1) / tile), per_item, num_sms()) &&
+            !starts(items, rows, per_item, a.type == NEKO_T_F32))
+            return launch_paged_prompt(a, st);
     }
     const bool q8 = a.cache.type == NEKO_T_E4M3;
     switch (a.cache.head_dim) {

@@ -513,3 +513,15 @@ def test_prompts_whose_keys_are_split(torch, dtype, e4m3):
         cache.vs.copy_(torch.from_numpy((2.0 ** rng.integers(-8, 5, tuple(cache.vs.shape))).astype(np.float32)).cuda())
     attend(torch, cache, [1900], [150], 8, dtype, 62)
     attend(torch, cache, [1900], [150], 8, dtype, 62, window=700, softcap=20.0, prefix=[100])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_a_few_tokens_of_many_short_contexts(torch, dtype, e4m3):
+    """More row tiles than SMs on a page or two each, of ragged lengths."""
+    rng = np.random.default_rng(63)
+    new = [int(x) for x in rng.integers(0, 10, 112)]
+    lens = [n + int(x) for n, x in zip(new, rng.integers(0, 60, 112))]
+    cache = Cache(torch, rng, lens, 4, 64, 128, e4m3)
+    cache.fill(rng, lens)
+    attend(torch, cache, lens, new, 12, dtype, 64, softcap=30.0, alibi=True)

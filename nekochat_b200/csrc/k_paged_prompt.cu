@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             };
             for (int i = 0; i < nt && ok; i++) {
                 ok = wait_on(&ms.full[sv], pv, fail);
+                ok = __all_sync(0xffffffffu, ok);
                 for (int h = 0; h < mt && ok; h++) {
                     ok = ok && wait_on(&ms.p_full[h], i & 1, fail);
                     ok = __all_sync(0xffffffffu, ok);

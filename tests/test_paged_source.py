@@ -1,0 +1,21 @@
+"""What running the paged kernels cannot show, because it only matters once a bounded wait has given up: read from the
+source. A wait may end differently in the lanes of a warp (one sees the barrier complete, another that a role has failed),
+so its result is voted on before any lane goes by it."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nekochat_b200", "csrc")
+
+
+def lines(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return [re.sub(r"//.*", "", x).strip() for x in f]
+
+
+def test_waits_of_a_role_are_voted_on():
+    src = lines("k_paged_prompt.cu")
+    at = [i for i, x in enumerate(src) if re.search(r"\bok = .*wait_on\(", x)]
+    assert len(at) >= 6
+    for i in at:
+        after = src[i + 1]
+        assert after.startswith("ok = __all_sync(0xffffffffu, ok);"), f"line {i + 1}: {src[i]} / {after}"

@@ -411,6 +411,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const uint32_t box_bytes = uint32_t(c.page_size) * 128;
             const bool carrier = box < per_page;  // at most 16 lanes (8 pages of 16 tokens, two halves)
             int scans = 0;
+            int begun = 0;             // items whose copies have been started;
+            uint32_t by_land = 0;      // bit x % 32: they complete on `land`, not on `full`;
+            bool landing = false;      // `land` has not been seen complete since
             float ks = 0.0f, vs = 0.0f;
             auto scales = [&]() {
                 if (SRC == kCopies && warp == kLoadWarp && pages >= 0) {
@@ -446,6 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     uint64_t* bar = scan ? &ms.land : &ms.full[st];
                     if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_bytes);
                     __syncwarp();
+                    begun = x + 1, landing = scan;
+                    by_land = (by_land & ~(1u << (x & 31))) | uint32_t(scan) << (x & 31);
                     if (page >= 0)
                         copy_box(base + half * L::kHalf + box * box_bytes, v ? &maps.v : &maps.k, half * 64, kvh * c.page_size, page, bar);
                 }
@@ -453,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     ok = wait_on(&ms.land, scans & 1, fail);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                    landing = false;
                     // rows that nobody holds are zeroed, values that are not finite taken out
                     uint32_t held_rows = 0;  // lane x < 8: rows of block x that are held
                     if (lane < 8 && pages >= 0) held_rows = uint32_t(min(max(len - j0 - 16 * lane, 0), 16));
@@ -484,6 +490,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     pages = pages_next;
                     scales();
                 }
+            }
+            // Given up: the copies that are still in flight land (again with a limit) before their place is used otherwise or the
+            // CTA leaves.
+            if (!ok && warp == kLoadWarp) {
+                for (int x = max(begun - L::kStages, 0); x < begun; x++)
+                    if (!(by_land >> (x & 31) & 1)) mbar_wait(&ms.full[x % L::kStages], (x / L::kStages) & 1);
+                if (landing) mbar_wait(&ms.land, scans & 1);
+                __syncwarp();
             }
         }
     } else if (warp == kMmaWarp) {

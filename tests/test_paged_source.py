@@ -19,3 +19,13 @@ def test_waits_of_a_role_are_voted_on():
     for i in at:
         after = src[i + 1]
         assert after.startswith("ok = __all_sync(0xffffffffu, ok);"), f"line {i + 1}: {src[i]} / {after}"
+
+
+def test_a_loader_that_gives_up_waits_for_its_copies():
+    """After the loop that starts tensor copies, the warp that started them waits, with a limit, for those in flight."""
+    src = lines("k_paged_prompt.cu")
+    start = next(i for i, x in enumerate(src) if "copy_box(base" in x)
+    end = next(i for i, x in enumerate(src) if i > start and "} else if (warp == kMmaWarp)" in x)
+    rest = " ".join(src[start:end])
+    given_up = rest.partition("if (!ok && warp == kLoadWarp)")[2]
+    assert "mbar_wait(&ms.full[" in given_up and "mbar_wait(&ms.land" in given_up

@@ -109,14 +109,17 @@ class PagedDecoder:
         T = sum(news)
         if not batch or min(news) <= 0 or T > MAX_ROWS or len(set(seqs)) != len(seqs):
             raise NekoError(f"forward: 1 to {MAX_ROWS} tokens, some for each of different sequences")
+        tokens = np.concatenate([np.asarray(t, np.int64) for _, t in batch])
+        if tokens.min() < 0 or tokens.max() >= s["vocab"]:  # the embedding is gathered by them on the device
+            raise NekoError(f"forward: a token is not in the vocabulary of {s['vocab']}")
         c.grow(list(zip(seqs, news)))
         begin = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
         start = np.array([c.length[x] for x in seqs], np.int32)
         table = c.rows(seqs)
         n = len(seqs)
         # one copy for all the integers
-        ints = np.concatenate([np.concatenate([np.asarray(t, np.int32) for _, t in batch]), begin, start,
-                               start + np.asarray(news, np.int32), table.ravel()])
+        ints = np.concatenate([tokens.astype(np.int32), begin, start, start + np.asarray(news, np.int32),
+                               table.ravel()])
         d = torch.from_numpy(ints).cuda()
         tokens, q_start, at, held, table_d = d.split([T, n + 1, n, n, table.size])
         table_d = table_d.view(table.shape)

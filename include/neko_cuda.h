@@ -203,7 +203,7 @@ typedef struct neko_paged_cache {
  * [cs_rows][rot / 2] of (cos, sin) over the first rot of each head's head_dim values: pairs (j, j + rot / 2), or
  * (2j, 2j + 1) when interleaved (rot a multiple of 8; 0: no rotation). k and v are rounded once, from f32.
  * A sequence with start[s] < 0 is inactive: nothing is stored, its q rows come out as zeros. Positions at or past
- * cs_rows are not stored either and report a device error.
+ * cs_rows are not stored either (their q rows are not turned) and neko_op_status reports them.
  * NEKO_T_E4M3: a (page, head) that gets tokens takes as scale the smallest power of two (at least 2^-100) with which
  * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
  * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new
@@ -254,6 +254,12 @@ typedef struct neko_paged_attention_args {
     int32_t reserved;
 } neko_paged_attention_args;
 int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream);
+/* What the two calls above could not do depends on lengths that only the device holds: a sequence with more than max_new
+ * new tokens, or rows outside [0, tokens), is left out whole (its rows of out and q_out keep what they held), positions past the rotation
+ * table are not stored. Waits for the stream's work and returns NEKO_ERR_DEVICE, with the reason in neko_last_error, when that
+ * has happened on the current device since the last call of this function, whatever the stream; NEKO_OK when it has not. Not
+ * while the stream is being captured. A neko_model's steps and a neko_ctx neither see these errors nor clear them. */
+int neko_op_status(void* stream);
 
 /* ------------------------------------------------------------------ 3. native model runner */
 

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
     const int start = a.start[s];
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {  // outside the planned rows
-        if (lane == 0) set_device_error(kErrBadIndex);
+        if (lane == 0) set_op_error(kErrBadIndex);
         return;
     }
     const bool live = start >= 0;
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged
     int i_end = i1;
     if (a.rot > 0 && start + i1 > a.cs_rows) {  // positions past the rotation table are not stored
         i_end = max(i0, a.cs_rows - start);
-        if (lane == 0) set_device_error(kErrBadIndex);
+        if (lane == 0) set_op_error(kErrBadIndex);
     }
     if (i_end <= i0 || !resident) return;
     const int64_t base = int64_t(page) * c.page_stride + int64_t(head) * ps * HD;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
     const int start = a.start[s];
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {  // outside the planned rows
-        if (threadIdx.x == 0) set_device_error(kErrBadIndex);
+        if (threadIdx.x == 0) set_op_error(kErrBadIndex);
         return;
     }
     const bool live = start >= 0;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
     int stored = page >= 0 && page < c.num_pages ? count : 0;  // tokens that are stored: none past the rotation table
     if (live && a.rot > 0 && pos0 + count > a.cs_rows) {
         stored = min(stored, max(0, a.cs_rows - pos0));
-        if (threadIdx.x == 0) set_device_error(kErrBadIndex);
+        if (threadIdx.x == 0) set_op_error(kErrBadIndex);
     }
     const int nh = a.q ? a.n_head : 0;
 

@@ -121,7 +121,7 @@ __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, cons
     v.len = min(v.held, a.cache.max_pages << plan.page_log);
     v.prefix = a.prefix ? min(max(a.prefix[s], 0), v.len) : 0;
     if (v.row0 < 0 || v.n < 0 || v.n > a.max_new || v.row0 + v.n > a.tokens) {
-        set_device_error(kErrBadIndex);
+        set_op_error(kErrBadIndex);
         v.n = 0;
     }
     auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };

@@ -195,8 +195,14 @@ __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile
         if ((i & 7) == 7 && *fail) return false;
     }
     *fail = 1;
-    set_device_error(kErrMbarTimeout);
+    set_op_error(kErrMbarTimeout);
     return false;
+}
+// Bounded wait for what is in flight once a role has given up.
+__device__ __forceinline__ void wait_out(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kMbarMaxTries; i++)
+        if (mbar_try_wait(bar, parity)) return;
+    set_op_error(kErrMbarTimeout);
 }
 // Whether the four 16-byte words hold f16 values that are not finite; those are zeroed.
 __device__ __forceinline__ bool drop_odd(uint4& x) {
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     using L = PL<HD, HILO>;
     extern __shared__ __align__(1024) uint8_t sm[];
     if (smem_u32(sm) & 1023u) {  // the operands' swizzle goes by address bits
-        if (threadIdx.x == 0) set_device_error(kErrMisalignedSmem);
+        if (threadIdx.x == 0) set_op_error(kErrMisalignedSmem);
         return;
     }
     Misc& ms = *reinterpret_cast<Misc*>(sm + L::kMiscOff);
@@ -252,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int held = max(a.kv_len[s], 0);
     const int len = min(held, c.max_pages * c.page_size);
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {
-        if (tid == 0) set_device_error(kErrBadIndex);
+        if (tid == 0) set_op_error(kErrBadIndex);
         return;
     }
     const int r0 = tile * plan.tiles_per * kRows;
@@ -495,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             // CTA leaves.
             if (!ok && warp == kLoadWarp) {
                 for (int x = max(begun - L::kStages, 0); x < begun; x++)
-                    if (!(by_land >> (x & 31) & 1)) mbar_wait(&ms.full[x % L::kStages], (x / L::kStages) & 1);
-                if (landing) mbar_wait(&ms.land, scans & 1);
+                    if (!(by_land >> (x & 31) & 1)) wait_out(&ms.full[x % L::kStages], (x / L::kStages) & 1);
+                if (landing) wait_out(&ms.land, scans & 1);
                 __syncwarp();
             }
         }
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 next(sv, pv), next(sk, pk);
             }
             commit(&ms.drain);  // nothing is in flight when the TMEM is freed, whatever happened
-            mbar_wait(&ms.drain, 0);
+            wait_out(&ms.drain, 0);
         }
         __syncwarp();
     } else {

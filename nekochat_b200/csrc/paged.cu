@@ -3,6 +3,10 @@
 
 using namespace neko;
 
+namespace neko {
+__device__ unsigned g_op_error = 0;
+}
+
 namespace {
 
 int paged_fail(int code, const char* op, const char* why) {
@@ -78,4 +82,22 @@ extern "C" int neko_op_paged_attention(const neko_paged_attention_args* a, void*
     if (a->window < 0 || !(a->softcap >= 0.0f) || !(a->scale == a->scale))
         return paged_fail(NEKO_ERR_ARG, op, "window and softcap are not negative");
     return finish(op, launch_paged_attention(*a, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int neko_op_status(void* stream) {
+    const char* op = "op_status";
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    unsigned code = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&code, g_op_error, sizeof code, 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess || code == kErrNone) return finish(op, e);
+    const unsigned none = kErrNone;
+    e = cudaMemcpyToSymbolAsync(g_op_error, &none, sizeof none, 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return finish(op, e);
+    return paged_fail(NEKO_ERR_DEVICE, op,
+                      code == kErrBadIndex ? "a sequence of a paged call had more new tokens than max_new, rows outside `tokens`, or "
+                                             "positions past the rotation table; those rows were left out"
+                      : code == kErrMbarTimeout ? "a bounded wait of a paged kernel gave up; its output is not valid"
+                                                : "a paged kernel found its shared memory misaligned and did nothing");
 }

@@ -18,6 +18,11 @@ cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStrea
 cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st);
 constexpr int kPromptRows = 16;
 
+// What a kernel of these operators could not do (kErr*) goes to a word of their own, which neko_op_status reads: a model's
+// steps read and clear the other one, and would fail for an operator's arguments.
+extern __device__ unsigned g_op_error;
+__device__ inline void set_op_error(unsigned code) { atomicCAS(&g_op_error, 0u, code); }
+
 // Two e4m3 codes as exact f16 (0x7F / 0xFF: NaN).
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
     uint32_t r;

@@ -316,3 +316,9 @@ def paged_attention(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=No
     if rc:
         check(rc, "paged_attention")
     return out
+
+
+def status():
+    """neko_op_status: waits for the current stream and raises when a paged_append or paged_attention since the last call
+    had a sequence with more new tokens than max_new, rows that are not there, or positions past the rotation table."""
+    check(lib().neko_op_status(_stream()), "paged operators")

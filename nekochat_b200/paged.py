@@ -151,6 +151,7 @@ class PagedDecoder:
             feed = [list(p) for p in prompts]
             while live:
                 nxt = ops.argmax(self.forward([(seqs[i], feed[i]) for i in live])).cpu().numpy()
+                ops.status()
                 still = []
                 for i, t in zip(live, nxt):
                     if int(t) in stop_ids:

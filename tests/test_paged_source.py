@@ -28,4 +28,4 @@ def test_a_loader_that_gives_up_waits_for_its_copies():
     end = next(i for i, x in enumerate(src) if i > start and "} else if (warp == kMmaWarp)" in x)
     rest = " ".join(src[start:end])
     given_up = rest.partition("if (!ok && warp == kLoadWarp)")[2]
-    assert "mbar_wait(&ms.full[" in given_up and "mbar_wait(&ms.land" in given_up
+    assert "wait_out(&ms.full[" in given_up and "wait_out(&ms.land" in given_up

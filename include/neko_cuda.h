@@ -203,7 +203,7 @@ typedef struct neko_paged_cache {
  * [cs_rows][rot / 2] of (cos, sin) over the first rot of each head's head_dim values: pairs (j, j + rot / 2), or
  * (2j, 2j + 1) when interleaved (rot a multiple of 8; 0: no rotation). k and v are rounded once, from f32.
  * A sequence with start[s] < 0 is inactive: nothing is stored, its q rows come out as zeros. Positions at or past
- * cs_rows are not stored either (their q rows are not turned) and neko_op_status reports them.
+ * cs_rows (or 2^30) are not stored either (their q rows are not turned) and neko_op_status reports them.
  * NEKO_T_E4M3: a (page, head) that gets tokens takes as scale the smallest power of two (at least 2^-100) with which
  * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
  * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new

@@ -22,6 +22,10 @@ namespace neko {
 
 namespace {
 
+// Starts count as no more than this: no page and no row of the rotation table is there, and positions stay within 31 bits (the
+// new tokens of a call are fewer than 2^24, 65,535 pages).
+constexpr int kFarthest = 1 << 30;
+
 constexpr int kFewTokens = 4;  // tokens of a unit in the step kernel
 
 constexpr int kSlots = 4;  // tokens of a lane in the prompt kernel (2: 32 warps per SM instead of 16, 115 us against 92 on ragged prompts)
@@ -61,7 +65,7 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged
     const neko_paged_cache& c = a.cache;
     const int row0 = a.q_start ? a.q_start[s] : s;
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
-    const int start = a.start[s];
+    const int start = min(a.start[s], kFarthest);
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {  // outside the planned rows
         if (lane == 0) set_op_error(kErrBadIndex);
         return;
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
     const neko_paged_cache& c = a.cache;
     const int row0 = a.q_start ? a.q_start[s] : s;
     const int n = a.q_start ? a.q_start[s + 1] - row0 : 1;
-    const int start = a.start[s];
+    const int start = min(a.start[s], kFarthest);
     if (row0 < 0 || n < 0 || n > a.max_new || row0 + n > a.tokens) {  // outside the planned rows
         if (threadIdx.x == 0) set_op_error(kErrBadIndex);
         return;
@@ -522,7 +526,9 @@ cudaError_t by_shape(const neko_paged_append_args& a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_paged_append(const neko_paged_append_args& a, cudaStream_t st) {
+cudaError_t launch_paged_append(const neko_paged_append_args& args, cudaStream_t st) {
+    neko_paged_append_args a = args;
+    a.cs_rows = std::min(a.cs_rows, kFarthest);
     return a.type == NEKO_T_F32   ? by_shape<float>(a, st)
            : a.type == NEKO_T_F16 ? by_shape<__half>(a, st)
                                   : by_shape<__nv_bfloat16>(a, st);

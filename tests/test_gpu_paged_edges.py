@@ -52,3 +52,30 @@ def test_rows_left_out_are_reported_to_who_asks(torch, native, rows):
         with pytest.raises(NekoError, match="max_new"):
             ops.status()
         ops.status()
+
+
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("at", [2 ** 31 - 2, 2 ** 31 - 40, 2 ** 30, 2 ** 30 + 1])
+def test_starts_past_every_table(torch, at, e4m3, n):
+    """Positions that do not fit 31 bits: nothing is read from before the rotation table, nothing is stored, the queries are
+    what they are without a rotation, and the status says so."""
+    from nekochat_b200 import NekoError, ops
+    rng = np.random.default_rng(122)
+    cache = Cache(torch, rng, [9, 50], 2, 16, 64, e4m3)
+    cache.fill(rng, [9, 50])
+    q, k, v = fresh_rows(torch, rng, n, 4, 2, 64, torch.float32)
+    gain = torch.rand(64, device="cuda") + 0.5
+    args = dict(k_scale=cache.ks, v_scale=cache.vs, q_start=ints(torch, 0, n, n), max_new=n, q=q, q_gain=gain, k_gain=gain)
+    table, start = torch.from_numpy(cache.table).cuda(), ints(torch, at, 50)
+    before = [x.clone() for x in (cache.k, cache.v) + ((cache.ks, cache.vs) if e4m3 else ())]
+    plain = ops.paged_append(k, v, cache.k, cache.v, table, start, **args)
+    ops.status()
+    turned = ops.paged_append(k, v, cache.k, cache.v, table, start, cs=ops.rope_table(600, 64, 1e4), **args)
+    with pytest.raises(NekoError, match="positions past the rotation table"):
+        ops.status()
+    want = q * torch.rsqrt(q.square().mean(-1, keepdim=True) + 1e-6) * gain
+    for got in (plain, turned):
+        assert ((got - want).abs() <= 2e-6 * want.abs().amax(-1, keepdim=True)).all()
+    for x, y in zip(before, (cache.k, cache.v, cache.ks, cache.vs)):
+        assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))

@@ -1,6 +1,8 @@
 // C entries of the paged key/value cache (neko_op_paged_* in include/neko_cuda.h): the checks of the arguments.
 #include "paged.cuh"
 
+#include <algorithm>
+
 using namespace neko;
 
 namespace neko {
@@ -79,9 +81,17 @@ extern "C" int neko_op_paged_attention(const neko_paged_attention_args* a, void*
     if (!a->q_start && a->tokens != a->cache.n_seq)
         return paged_fail(NEKO_ERR_ARG, op, "without q_start there is one token per sequence");
     if (a->cache.n_seq > 16384) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 16384 sequences");
+    // A sequence has no more rows than there are: a loose max_new costs nothing. The kernels count a KV head's rows (tokens x heads per KV
+    // head) with 31 bits and divide them by the heads with a 32-bit reciprocal, exact below 2^32 / its excess over 1 / group.
+    neko_paged_attention_args own = *a;
+    own.max_new = std::min(a->max_new, a->tokens);
+    const int64_t group = a->n_head / a->cache.n_kv, rows = own.max_new * group;
+    const int64_t excess = ((int64_t(1) << 32) + group - 1) / group * group - (int64_t(1) << 32);
+    if (rows > INT32_MAX - 1024 || rows * excess >= (int64_t(1) << 32))
+        return paged_fail(NEKO_ERR_UNSUPPORTED, op, "2^31 rows (new tokens times heads per KV head) or more; fewer where those heads are no power of two");
     if (a->window < 0 || !(a->softcap >= 0.0f) || !(a->scale == a->scale))
         return paged_fail(NEKO_ERR_ARG, op, "window and softcap are not negative");
-    return finish(op, launch_paged_attention(*a, static_cast<cudaStream_t>(stream)));
+    return finish(op, launch_paged_attention(own, static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int neko_op_status(void* stream) {

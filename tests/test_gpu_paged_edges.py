@@ -79,3 +79,96 @@ def test_starts_past_every_table(torch, at, e4m3, n):
         assert ((got - want).abs() <= 2e-6 * want.abs().amax(-1, keepdim=True)).all()
     for x, y in zip(before, (cache.k, cache.v, cache.ks, cache.vs)):
         assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+def exact(torch, cache, q, lens, new, scale, softcap=0.0, window=0, slopes=None, prefix=None):
+    """The definition in 64 bits, and for each row and head what its rounding errors are measured by: mass = sum_j p_j |v_j| per value
+    and reach = max_j sum_d |q_d k_jd| scale."""
+    pages, n_kv, ps, hd = cache.k.shape
+    if cache.e4m3:
+        code = torch.from_numpy(ref.E4M3).cuda()
+        k, v = (code[x.view(torch.uint8).long()] * s[:, :, None, None].double() for x, s in ((cache.k, cache.ks), (cache.v, cache.vs)))
+    else:
+        k, v = cache.k.double(), cache.v.double()
+    table = torch.from_numpy(cache.table).cuda().long()
+    out, mass = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    reach = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda")
+    G = q.shape[1] // n_kv
+    at = 0
+    for s, (L, n) in enumerate(zip(lens, new)):
+        rows, at = slice(at, at + n), at + n
+        L_ = min(L, table.shape[1] * ps)
+        if n == 0 or L_ <= 0:
+            continue
+        t = table[s, :-(-L_ // ps)]
+        held = ((t >= 0) & (t < pages)).repeat_interleave(ps)[:L_]
+        j, pos = torch.arange(L_, device="cuda")[None], (L - n + torch.arange(n, device="cuda"))[:, None]
+        see = (j <= pos) & ((pos - j < window) if window else True)
+        if prefix is not None:
+            see = see | (j < prefix[s])
+        see = see & held[None]
+        for h in range(q.shape[1]):
+            kk, vv = (x[t.clamp(0, pages - 1), h // G].reshape(-1, hd)[:L_] for x in (k, v))
+            kk, vv = (torch.where(see.any(0)[:, None], x, 0.0) for x in (kk, vv))
+            qq = q[rows, h].double()
+            z = qq @ kk.T * scale
+            reach[rows, h] = torch.where(see, qq.abs() @ kk.abs().T * abs(scale), 0).amax(1)
+            if softcap:
+                z = softcap * torch.tanh(z / softcap)
+            if slopes is not None:
+                z = z + slopes[h].double() * (j - pos)
+            z = torch.where(see, z, -torch.inf)
+            p = torch.softmax(z, 1).nan_to_num(0.0)
+            out[rows, h], mass[rows, h] = p @ vv, p @ vv.abs()
+    return out, mass, reach
+
+
+def bound(dtype, want, mass, reach, softcap=0.0):
+    """What a row's arithmetic may be off by. Scores: 22 bits of q, sums of hd / 16 steps, together 2^-20 of reach; a cap 2^-21 of
+    itself; exponentials, hi + lo weights and the sums 2^-18 of mass (16-bit rows: weights to f16, 2^-11). The output's rounding
+    2^-11 (f16) or 2^-8 (bf16) of itself, f16 subnormals 2^-25."""
+    rel = 2.0 ** -20 * reach[..., None] + 2.0 ** -21 * softcap + (2.0 ** -18 if dtype == "float32" else 2.0 ** -11 + 2.0 ** -16)
+    return rel * mass + ROUND[dtype] * want.abs() + (2.0 ** -25 if dtype == "float16" else 0.0)
+
+
+def held_to(torch, cache, lens, new, heads, dtype, seed, q_scale=1.0, q=None, softcap=0.0, window=0, alibi=False, prefix=None, max_new=None,
+            scale=None):
+    """One call, every value within bound()."""
+    from nekochat_b200 import ops
+    g = torch.Generator("cuda").manual_seed(seed)
+    hd = cache.k.shape[3]
+    if q is None:
+        q = torch.randn((int(sum(new)), heads, hd), device="cuda", generator=g) * q_scale
+    q = q.to(getattr(torch, dtype))
+    slopes = (2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)) if alibi else None
+    got = ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, *lens), k_scale=cache.ks,
+                              v_scale=cache.vs, q_start=ints(torch, *starts(new).tolist()), max_new=max_new or max(new), softcap=softcap,
+                              window=window, slopes=slopes, prefix=None if prefix is None else ints(torch, *prefix), scale=scale)
+    ops.status()
+    want, mass, reach = exact(torch, cache, q, lens, new, hd ** -0.5 if scale is None else scale, softcap, window, slopes, prefix)
+    off = (got.double() - want).abs()
+    far = ~(off <= bound(dtype, want, mass, reach, softcap))
+    assert not far.any(), f"{int(far.sum())} of {far.numel()} values, the worst off by {off[far].max().item():.3g} at {far.nonzero()[0].tolist()}"
+    return got, want
+
+
+def quantize(torch, cache, k, v):
+    """Normal values into the cache's pages ([pages][n_kv][ps][hd] f32): f16, or codes with the append's scales."""
+    if not cache.e4m3:
+        cache.k.copy_(k), cache.v.copy_(v)
+        return
+    for x, pool, sc in ((k, cache.k, cache.ks), (v, cache.v, cache.vs)):
+        e = torch.ceil(torch.log2(x.abs().amax((2, 3)).double() / 448)).clamp(min=-100)
+        sc.copy_(torch.exp2(e).float())
+        pool.copy_((x / sc[:, :, None, None]).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+@pytest.mark.parametrize("max_new", [1000, 1 << 24, 2 ** 31 - 1])
+def test_a_loose_limit_of_new_tokens(torch, hd, max_new):
+    """max_new far above what any sequence has: the same results."""
+    rng = np.random.default_rng(116)
+    new, lens = [40, 1, 7], [60, 200, 7]
+    cache = Cache(torch, rng, lens, 2, 16, hd, False)
+    cache.fill(rng, lens)
+    held_to(torch, cache, lens, new, 8, "float32", 117, max_new=max_new)

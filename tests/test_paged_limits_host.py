@@ -1,0 +1,27 @@
+"""Limits of the paged entries that come before any CUDA call."""
+import numpy as np
+import pytest
+
+import nekochat_b200 as nb
+from nekochat_b200 import ops
+from tests.test_paged_host import APPEND, ATTEND, call  # noqa: F401
+
+
+@pytest.mark.parametrize("over", [dict(tokens=1 << 30, max_new=1 << 30, n_head=16), dict(tokens=(1 << 31) - 1, max_new=(1 << 31) - 1, n_head=8),
+                                  dict(tokens=1 << 28, max_new=1 << 28, n_head=8 * 48), dict(tokens=1 << 24, max_new=1 << 24, n_head=8 * 100)])
+def test_refused_rows(over):
+    """Rows of a KV head that 31 bits or the reciprocal of the group do not hold (the second is a whole call's of one head)."""
+    assert call("neko_op_paged_attention", ATTEND, ops._ATTEND, **over) == -6
+    assert b"rows" in nb.lib().neko_last_error()
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 12, 24, 48, 100, 127])
+def test_rows_are_divided_exactly(group):
+    """x * ceil(2^32 / group) >> 32 is x / group for every x that is not refused: where it first is not, the call is refused."""
+    inv = -(-(1 << 32) // group)
+    excess = inv * group - (1 << 32)
+    top = min((1 << 31) - 1025, ((1 << 32) - 1) // excess if excess else 1 << 40)
+    rng = np.random.default_rng(group)
+    xs = np.unique(np.concatenate([rng.integers(0, top + 1, 200000), np.arange(top - 3 * group, top + 1), np.arange(3 * group)]))
+    for near in (xs, np.minimum(xs // group * group + group - 1, top)):
+        assert all(int(x) * inv >> 32 == int(x) // group for x in near)

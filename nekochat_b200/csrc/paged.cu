@@ -66,7 +66,11 @@ extern "C" int neko_op_paged_append(const neko_paged_append_args* a, void* strea
     for (const int64_t step : {a->q ? a->q_token : 0, a->k_token, a->v_token, a->q ? a->o_token : 0})  // the rows of a page are addressed with 32 bits
         if (step >= (1 << 24) || step <= -(1 << 24)) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "token strides of 2^24 elements or more");
     if (a->q && !a->q_gain != !a->k_gain) return paged_fail(NEKO_ERR_ARG, op, "both gains or neither");
-    return finish(op, launch_paged_append(*a, static_cast<cudaStream_t>(stream)));
+    neko_paged_append_args own = *a;
+    own.max_new = std::min(a->max_new, a->tokens);  // a sequence has no more than there are: a loose max_new costs nothing
+    if (own.max_new / a->cache.page_size > 65530 || a->n_head > 65535 || a->cache.n_kv > 65535)  // the grid's second and third dimension
+        return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 65,530 pages of new tokens per sequence, or 65,535 heads");
+    return finish(op, launch_paged_append(own, static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int neko_op_paged_attention(const neko_paged_attention_args* a, void* stream) {

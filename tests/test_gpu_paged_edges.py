@@ -172,3 +172,19 @@ def test_a_loose_limit_of_new_tokens(torch, hd, max_new):
     cache = Cache(torch, rng, lens, 2, 16, hd, False)
     cache.fill(rng, lens)
     held_to(torch, cache, lens, new, 8, "float32", 117, max_new=max_new)
+
+
+@pytest.mark.parametrize("max_new", [1 << 24, 2 ** 31 - 1])
+def test_a_loose_limit_of_appended_tokens(torch, max_new):
+    """max_new far above what any sequence has: the pages and queries of a tight one, to the last bit."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(123)
+    new, at = [40, 1, 7], [20, 199, 0]
+    q, k, v = fresh_rows(torch, rng, sum(new), 4, 2, 64, torch.float32)
+    cs, outs = ops.rope_table(300, 64, 1e4), []
+    for limit in (40, max_new):
+        cache = Cache(torch, np.random.default_rng(1), [a + n for a, n in zip(at, new)], 2, 16, 64, False)
+        outs.append((ops.paged_append(k, v, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, *at),
+                                      q_start=ints(torch, *starts(new).tolist()), max_new=limit, q=q, cs=cs), cache.k.nan_to_num(9), cache.v.nan_to_num(9)))
+        ops.status()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

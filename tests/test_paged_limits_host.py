@@ -25,3 +25,11 @@ def test_rows_are_divided_exactly(group):
     xs = np.unique(np.concatenate([rng.integers(0, top + 1, 200000), np.arange(top - 3 * group, top + 1), np.arange(3 * group)]))
     for near in (xs, np.minimum(xs // group * group + group - 1, top)):
         assert all(int(x) * inv >> 32 == int(x) // group for x in near)
+
+
+def test_refused_lengths_of_an_append():
+    """New tokens that take more pages than a grid counts; a max_new that is only loose is not refused (it fails later, without
+    a GPU)."""
+    assert call("neko_op_paged_append", APPEND, ops._APPEND, tokens=1 << 21, max_new=1 << 21) == -6
+    assert b"pages of new tokens" in nb.lib().neko_last_error()
+    assert call("neko_op_paged_append", APPEND, ops._APPEND, tokens=0, max_new=1 << 30) == 0

@@ -208,7 +208,7 @@ typedef struct neko_paged_cache {
  * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
  * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new
  * (exact, but for codes that become subnormal). Infinities are stored as +-448 * scale, NaN as NaN.
- * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous; token strides
+ * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous; token strides (of several rows)
  * below 2^24 and at most 65,530 pages of new tokens per sequence (else NEKO_ERR_UNSUPPORTED). */
 typedef struct neko_paged_append_args {
     neko_paged_cache cache;

@@ -63,8 +63,10 @@ extern "C" int neko_op_paged_append(const neko_paged_append_args* a, void* strea
         return paged_fail(NEKO_ERR_ARG, op, "rot is a multiple of 8 up to the head dim");
     if (a->rot && (!a->cs || a->cs_rows <= 0 || !aligned(a->cs, 16)))
         return paged_fail(NEKO_ERR_ARG, op, "a rotation needs its table (16-byte aligned)");
-    for (const int64_t step : {a->q ? a->q_token : 0, a->k_token, a->v_token, a->q ? a->o_token : 0})  // the rows of a page are addressed with 32 bits
-        if (step >= (1 << 24) || step <= -(1 << 24)) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "token strides of 2^24 elements or more");
+    // the rows of a page are addressed with 32 bits; the stride of a single row says nothing (a dimension of one may have any)
+    for (const int64_t step : {a->q ? a->q_token : 0, a->k_token, a->v_token, a->q ? a->o_token : 0})
+        if (a->tokens > 1 && (step >= (1 << 24) || step <= -(1 << 24)))
+            return paged_fail(NEKO_ERR_UNSUPPORTED, op, "token strides of 2^24 elements or more");
     if (a->q && !a->q_gain != !a->k_gain) return paged_fail(NEKO_ERR_ARG, op, "both gains or neither");
     neko_paged_append_args own = *a;
     own.max_new = std::min(a->max_new, a->tokens);  // a sequence has no more than there are: a loose max_new costs nothing

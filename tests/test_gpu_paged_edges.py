@@ -188,3 +188,18 @@ def test_a_loose_limit_of_appended_tokens(torch, max_new):
                                       q_start=ints(torch, *starts(new).tolist()), max_new=limit, q=q, cs=cs), cache.k.nan_to_num(9), cache.v.nan_to_num(9)))
         ops.status()
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("max_new", [1, 9])
+def test_one_row_with_any_stride(torch, max_new):
+    """The token stride of a single row: 2^24 and more, as a dimension of one may have it."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(124)
+    outs = []
+    q, k, v = fresh_rows(torch, rng, 1, 4, 2, 64, torch.float32)
+    far = lambda x: x.as_strided(x.shape, (1 << 33, x.stride(1), 1))  # noqa: E731
+    for f in (lambda x: x, far):
+        cache = Cache(torch, np.random.default_rng(1), [30], 2, 16, 64, False)
+        outs.append((ops.paged_append(f(k), f(v), cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, 29), q_start=ints(torch, 0, 1),
+                                      max_new=max_new, q=f(q), q_out=f(torch.empty_like(q))).clone(), cache.k.nan_to_num(9), cache.v.nan_to_num(9)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

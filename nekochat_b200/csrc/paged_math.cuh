@@ -12,9 +12,15 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// tanh(x) = 1 - 2 / (1 + e^2x): absolute error of a few 2^-23, which the cap multiplies; large |x| saturate.
+// The smaller of two numbers, NaN where either is one.
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+// tanh(x) = 1 - 2 / (1 + e^2x): absolute error of a few 2^-23, which the cap multiplies; large |x| saturate, NaN stays.
 __device__ __forceinline__ float tanh_abs(float x) {
-    return 1.0f - __fdividef(2.0f, 1.0f + ex2(fminf(x * (2.0f * kLog2e), 64.0f)));
+    return 1.0f - __fdividef(2.0f, 1.0f + ex2(min_nan(x * (2.0f * kLog2e), 64.0f)));
 }
 // tanh of |x| <= 1/2 as an odd polynomial of degree 9 (least maximum error there: 3e-9): no special functions, and exact to the
 // last places where tanh_abs is off by a few 2^-23, which a cap of 50 makes 1e-5 of a score.

@@ -203,3 +203,36 @@ def test_one_row_with_any_stride(torch, max_new):
         outs.append((ops.paged_append(f(k), f(v), cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, 29), q_start=ints(torch, 0, 1),
                                       max_new=max_new, q=f(q), q_out=f(torch.empty_like(q))).clone(), cache.k.nan_to_num(9), cache.v.nan_to_num(9)))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("softcap,q_scale", [(30.0, 1.0), (0.5, 1.0), (2.0, 50.0)])
+@pytest.mark.parametrize("new,lens", [([3, 1, 2], [60, 70, 20]), ([200, 40, 150], [330, 600, 150])])
+def test_scores_that_are_not_numbers_stay_so_under_a_cap(torch, new, lens, softcap, q_scale, e4m3, dtype):
+    """tanh(NaN) is NaN: rows that see such a key give NaN, whatever the other scores are, and no other row does."""
+    rng = np.random.default_rng(81)
+    cache = Cache(torch, rng, lens, 2, 16, 128, e4m3)
+    cache.fill(rng, lens)
+    nan = 0x7F if e4m3 else float("nan")
+    for s, j in ((0, lens[0] - 2), (2, lens[2] - 1)):
+        cache.k[int(cache.table[s, j // 16]), s // 2, j % 16, 5] = nan
+    got, want = attend(torch, cache, lens, new, 4, dtype, 82, softcap=softcap, q_scale=q_scale)
+    assert np.isnan(want).any() and np.isfinite(want).any()
+
+
+@pytest.mark.parametrize("n", [1, 9, 200])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_a_query_that_is_not_a_number(torch, n, softcap):
+    """Its row and head are NaN, with and without a cap; the rows beside it are not."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(83)
+    cache = Cache(torch, rng, [300], 2, 16, 128, False)
+    cache.fill(rng, [300])
+    q = torch.randn((n, 4, 128), device="cuda")
+    q[n // 2, 1, 77] = float("nan")
+    got = ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, 300),
+                              q_start=ints(torch, 0, n), max_new=n, softcap=softcap)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[n // 2, 1] = True
+    assert torch.equal(got.isnan(), bad)

@@ -302,8 +302,8 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
     }
     const int nh = a.q ? a.n_head : 0;
 
-    // this lane's eight values: four at da, four at db. Half layout: pairs (j, j + rot / 2), then the rest of the head as
-    // pairs that do not turn; interleaved: eight in a row.
+    // this lane's eight values: four at da, four at db. Half layout: pairs (j, j + rot / 2), then the rest of the head, whose
+    // values stay as they are (not turned by 0: an infinity or NaN beside would reach them); interleaved: eight in a row.
     const int l = lane % kLanes, half = a.rot >> 1;
     int da = 8 * l, db = 8 * l + 4;
     bool in_rot = 8 * l < a.rot;
@@ -315,16 +315,19 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
     }
     int tok[kSlots];  // this lane's token in each slot, from i0
     uint64_t cs[kSlots][2], sn[kSlots][2];  // cosines and sines of the four pairs, two and two
+    bool turns[kSlots];                     // past the rotation table, and beyond `rot`, nothing does
 #pragma unroll
     for (int z = 0; z < kSlots; z++) {
         tok[z] = (z * warps + warp) * kRowsPer + lane / kLanes;
         const int pos = pos0 + tok[z];
         const bool turn = in_rot && live && tok[z] < count && pos < a.cs_rows;
+        turns[z] = turn;
         const float4* p = reinterpret_cast<const float4*>(a.cs + (turn ? int64_t(pos) * a.rot + 8 * l : 0));
         const float4 t0 = turn ? p[0] : make_float4(1, 0, 1, 0), t1 = turn ? p[1] : make_float4(1, 0, 1, 0);
         cs[z][0] = pack2(t0.x, t0.z), cs[z][1] = pack2(t1.x, t1.z);
         sn[z][0] = pack2(t0.y, t0.w), sn[z][1] = pack2(t1.y, t1.w);
     }
+    const bool all_turn = a.rot == HD && live && pos0 + count <= a.cs_rows;
     if (a.k_gain) {
         for (int d = threadIdx.x; d < HD; d += blockDim.x) {
             if (a.q) gains[0][d] = a.q_gain[d];
@@ -403,27 +406,33 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
             }
         }
         if (kind != 2 && a.rot) {
-            if (a.interleaved) {
+            auto turn = [&](auto all) {
 #pragma unroll
-                for (int z = 0; z < kSlots; z++)
+                for (int z = 0; z < kSlots; z++) {
+                    if (!decltype(all)::value && !turns[z]) continue;
+                    if (a.interleaved) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {  // pair e: its two values are one register pair
-                        float p, q, c0, c1, s0, s1;
-                        unpack2(x[z][e], p, q), unpack2(cs[z][e / 2], c0, c1), unpack2(sn[z][e / 2], s0, s1);
-                        const float co = e & 1 ? c1 : c0, si = e & 1 ? s1 : s0;
-                        x[z][e] = pack2(turned(p, q, co, -si), turned(q, p, co, si));
+                        for (int e = 0; e < 4; e++) {  // pair e: its two values are one register pair
+                            float p, q, c0, c1, s0, s1;
+                            unpack2(x[z][e], p, q), unpack2(cs[z][e / 2], c0, c1), unpack2(sn[z][e / 2], s0, s1);
+                            const float co = e & 1 ? c1 : c0, si = e & 1 ? s1 : s0;
+                            x[z][e] = pack2(turned(p, q, co, -si), turned(q, p, co, si));
+                        }
+                    } else {
+                        const uint64_t minus = pack2(-1.0f, -1.0f);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {  // pairs 2 e and 2 e + 1
+                            const uint64_t p = x[z][e], q = x[z][2 + e];
+                            x[z][e] = fma2(p, cs[z][e], mul2(q, mul2(sn[z][e], minus)));
+                            x[z][2 + e] = fma2(q, cs[z][e], mul2(p, sn[z][e]));
+                        }
                     }
-            } else {
-                const uint64_t minus = pack2(-1.0f, -1.0f);
-#pragma unroll
-                for (int z = 0; z < kSlots; z++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {  // pairs 2 e and 2 e + 1
-                        const uint64_t p = x[z][e], q = x[z][2 + e];
-                        x[z][e] = fma2(p, cs[z][e], mul2(q, mul2(sn[z][e], minus)));
-                        x[z][2 + e] = fma2(q, cs[z][e], mul2(p, sn[z][e]));
-                    }
-            }
+                }
+            };
+            // Where the whole head turns at every position, whatever rows past `count` hold turns too: no predicate a value
+            // (ragged prompts 95.7 us, 97.6 with one).
+            if (all_turn) turn(std::true_type());
+            else turn(std::false_type());
         }
         if (kind == 0) {
             T* dst = static_cast<T*>(a.q_out) + head * a.o_head + (row0 + i0) * a.o_token;

@@ -236,3 +236,40 @@ def test_a_query_that_is_not_a_number(torch, n, softcap):
     bad = torch.zeros_like(got, dtype=torch.bool)
     bad[n // 2, 1] = True
     assert torch.equal(got.isnan(), bad)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_values_that_do_not_turn_stay_apart(torch, dtype, interleaved, e4m3, n):
+    """Infinities and NaN in the part of a head that a rotation leaves alone change no other value, in the steps' kernel and
+    the prompts', and those in a pair reach that pair alone. f32 arithmetic, one rounding: 2e-6 of the row's largest finite
+    value and half a unit of the type; 8-bit codes are as the definition's but for ties within that (none at these values)."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(84)
+    hd, rot, start = 64, 32, 5
+    cache = Cache(torch, rng, [start + n], 2, 16, hd, e4m3)
+    cache.fill(rng, [start])
+    q, k, v = fresh_rows(torch, rng, n, 4, 2, hd, getattr(torch, dtype))
+    for x in (q, k, v):
+        x[1, 0, 40], x[1, 1, 50], x[2, 0, 63] = float("nan"), float("inf"), float("-inf")
+        x[2, 1, 3] = float("inf")
+        x[0, 1, 33] = float("inf")
+    cs = ops.rope_table(100, rot, 1e4)
+    f64 = lambda t: t.float().cpu().numpy().astype(np.float64)  # noqa: E731
+    before, scales = cache.values(scaled=False), [f64(cache.ks), f64(cache.vs)] if e4m3 else [None, None]
+    got = ops.paged_append(k, v, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, start), k_scale=cache.ks,
+                           v_scale=cache.vs, q_start=ints(torch, 0, n), max_new=n, q=q, cs=cs, interleaved=interleaved)
+    want = ref.append(f64(k), f64(v), *before, cache.table, [start], [0, n], *scales, f64(q), cs.cpu().numpy(), interleaved)
+
+    def same(g, w, near):
+        assert np.array_equal(np.isnan(g), np.isnan(w))
+        assert np.array_equal(np.where(np.isinf(g), g, 0), np.where(np.isinf(w), w, 0))
+        f = np.isfinite(w)
+        top = np.where(f, np.abs(w), 0).max(-1, keepdims=True)
+        assert (np.abs(g - w)[f] <= (2e-6 * top + near * np.abs(w))[f]).all()
+
+    same(f64(got), want, 0 if dtype == "float32" else 2.0 ** -8)
+    for g, w in zip(cache.values(scaled=False), before):
+        same(g, w, 2.0 ** -3 if e4m3 else 2.0 ** -11)

@@ -220,7 +220,8 @@ def rope_table(positions, rot, theta, scaling="none", factor=1.0, original=0, be
       "linear" positions divided by factor;
       "ntk"    theta raised to theta * factor^(rot / (rot - 2)), so the slowest pair is slowed by factor;
       "yarn"   pairs that turn more than beta_fast times over `original` positions keep their speed, those below
-               beta_slow turns are slowed by factor, a linear ramp between, and cos and sin are multiplied by
+               beta_slow turns are slowed by factor, a linear ramp between (its ends in whole pairs, in [0, rot - 1]; the
+               upper one may lie past the last pair, which then is slowed in part), and cos and sin are multiplied by
                0.1 ln(factor) + 1 (YaRN, Peng et al. 2023)."""
     import math
 
@@ -240,7 +241,7 @@ def rope_table(positions, rot, theta, scaling="none", factor=1.0, original=0, be
         if original <= 0:
             raise NekoError("rope_table: yarn needs the original context length")
         pair = lambda turns: half * math.log(original / (turns * 2 * math.pi)) / math.log(theta)  # noqa: E731
-        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), half - 1)
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rot - 1)
         slow = np.clip((j - low) / max(high - low, 1e-3), 0, 1)
         freq = freq * (1 - slow) + freq / factor * slow
         gain = 0.1 * math.log(factor) + 1.0

@@ -145,9 +145,13 @@ class PagedDecoder:
 
     def generate(self, prompts, max_new, stop_ids=()):
         """Greedy tokens after each prompt (lists of ids), stopped at a stop id or max_new tokens."""
-        seqs = [self.cache.open() for _ in prompts]
+        if not all(len(p) for p in prompts):
+            raise NekoError("generate: an empty prompt")
         out, live = [[] for _ in prompts], list(range(len(prompts)))
+        seqs = []
         try:
+            for _ in prompts:
+                seqs.append(self.cache.open())
             feed = [list(p) for p in prompts]
             while live:
                 nxt = ops.argmax(self.forward([(seqs[i], feed[i]) for i in live])).cpu().numpy()
@@ -167,9 +171,10 @@ class PagedDecoder:
         return out
 
 
-def build(shape_name, fmt=1, kind="f16", pages=256, page=64, max_len=4096, seed=0, perturb=False, **rope):
+def build(shape_name, fmt=1, kind="f16", pages=256, page=64, max_len=4096, seed=0, perturb=False, max_seqs=64,
+          **rope):
     s = workload.shape(shape_name)
-    cache = PagedCache(s["layers"], s["kv_heads"], s["head_dim"], pages, page, kind, max_len=max_len)
+    cache = PagedCache(s["layers"], s["kv_heads"], s["head_dim"], pages, page, kind, max_seqs, max_len)
     return PagedDecoder(s, fmt, cache, **rope).load(workload.weights(s, seed, perturb))
 
 

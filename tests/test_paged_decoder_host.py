@@ -23,3 +23,42 @@ def test_tokens_outside_the_vocabulary_are_refused(ids):
     with pytest.raises(nb.NekoError, match="vocabulary"):
         m.forward([(s, [m.s["vocab"] if t == "vocab" else t for t in ids])])
     assert m.cache.length[s] == 0 and not m.cache.held[s]  # nothing was taken
+
+
+class Fake:
+    """Stands in for the device: a step's "logits" are the next tokens themselves, the sum of all that a sequence has taken in."""
+
+    def __init__(self, monkeypatch, m, vocab=1000):
+        self.calls, self.m, self.seen, self.vocab = [], m, {}, vocab
+        monkeypatch.setattr(paged, "ops", types.SimpleNamespace(argmax=lambda x: x, status=lambda: None))
+        monkeypatch.setattr(m, "forward", self.forward, raising=False)
+
+    def forward(self, batch):
+        import torch
+        rows = sum(len(t) for _, t in batch)
+        assert 0 < rows <= paged.MAX_ROWS and all(len(t) for _, t in batch)
+        self.calls.append([(s, len(t)) for s, t in batch])
+        self.m.cache.grow([(s, len(t)) for s, t in batch])
+        for s, t in batch:
+            self.m.cache.length[s] += len(t)
+            self.seen[s] = (self.seen.get(s, 0) + sum(t)) % self.vocab
+        return torch.tensor([self.seen[s] for s, _ in batch])
+
+    def want(self, prompt, max_new, stop=()):
+        out, total = [], sum(prompt) % self.vocab
+        while len(out) < max_new and total not in stop:
+            out.append(total)
+            total = 2 * total % self.vocab
+        return out
+
+
+def test_generate_gives_back_what_it_opened(monkeypatch):
+    m = decoder(max_seqs=3)
+    Fake(monkeypatch, m)
+    with pytest.raises(nb.NekoError, match="in use"):
+        m.generate([[1]] * 4, 2)
+    assert len(m.cache.ids) == 3 and not m.cache.held
+    assert [len(o) for o in m.generate([[1]] * 3, 2)] == [2, 2, 2]
+    with pytest.raises(nb.NekoError, match="empty prompt"):
+        m.generate([[1], []], 2)
+    assert len(m.cache.ids) == 3 and len(m.cache.free) == 8

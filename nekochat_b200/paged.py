@@ -148,6 +148,8 @@ class PagedDecoder:
         if not all(len(p) for p in prompts):
             raise NekoError("generate: an empty prompt")
         out, live = [[] for _ in prompts], list(range(len(prompts)))
+        if max_new <= 0:
+            return out
         seqs = []
         try:
             for _ in prompts:

@@ -62,3 +62,12 @@ def test_generate_gives_back_what_it_opened(monkeypatch):
     with pytest.raises(nb.NekoError, match="empty prompt"):
         m.generate([[1], []], 2)
     assert len(m.cache.ids) == 3 and len(m.cache.free) == 8
+
+
+def test_generate_makes_as_many_tokens_as_asked(monkeypatch):
+    m = decoder()
+    f = Fake(monkeypatch, m)
+    assert m.generate([[1], [2]], 0) == [[], []] and not f.calls
+    assert m.generate([], 3) == []
+    f.seen.clear()
+    assert m.generate([[5], [7]], 3) == [f.want([5], 3), f.want([7], 3)]

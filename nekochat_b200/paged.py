@@ -144,29 +144,41 @@ class PagedDecoder:
         return ops.matmul(self.fmt, ops.norm(x[last], self.norm, eps=eps), self.embed, C)
 
     def generate(self, prompts, max_new, stop_ids=()):
-        """Greedy tokens after each prompt (lists of ids), stopped at a stop id or max_new tokens."""
+        """Greedy tokens after each prompt (lists of ids), stopped at a stop id or max_new tokens. Prompts may be longer than
+        one forward takes: they go through in pieces."""
         if not all(len(p) for p in prompts):
             raise NekoError("generate: an empty prompt")
-        out, live = [[] for _ in prompts], list(range(len(prompts)))
+        out = [[] for _ in prompts]
         if max_new <= 0:
             return out
         seqs = []
         try:
             for _ in prompts:
                 seqs.append(self.cache.open())
-            feed = [list(p) for p in prompts]
+            feed = [list(p) for p in prompts]  # what each sequence has still to take in
+            live = list(range(len(prompts)))
             while live:
-                nxt = ops.argmax(self.forward([(seqs[i], feed[i]) for i in live])).cpu().numpy()
+                room, batch = MAX_ROWS, []
+                for i in live[:MAX_ROWS]:
+                    batch.append((i, feed[i][:room]))
+                    room -= len(batch[-1][1])
+                    if not room:
+                        break
+                nxt = ops.argmax(self.forward([(seqs[i], t) for i, t in batch])).cpu().numpy()
                 ops.status()
-                still = []
-                for i, t in zip(live, nxt):
+                done = set()
+                for (i, taken), t in zip(batch, nxt):
+                    feed[i] = feed[i][len(taken):]
+                    if feed[i]:
+                        continue
                     if int(t) in stop_ids:
+                        done.add(i)
                         continue
                     out[i].append(int(t))
-                    if len(out[i]) < max_new:
-                        feed[i] = [int(t)]
-                        still.append(i)
-                live = still
+                    feed[i] = [int(t)]
+                    if len(out[i]) == max_new:
+                        done.add(i)
+                live = [i for i in live if i not in done]
         finally:
             for sq in seqs:
                 self.cache.close(sq)

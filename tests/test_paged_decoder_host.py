@@ -71,3 +71,15 @@ def test_generate_makes_as_many_tokens_as_asked(monkeypatch):
     assert m.generate([], 3) == []
     f.seen.clear()
     assert m.generate([[5], [7]], 3) == [f.want([5], 3), f.want([7], 3)]
+
+
+def test_generate_takes_long_prompts_in_pieces(monkeypatch):
+    m = decoder(pages=2000, max_len=20000)
+    f = Fake(monkeypatch, m)
+    prompts = [[3] * 5000, [1] * 10, [2] * 9001, [4]]
+    assert m.generate(prompts, 4) == [f.want(p, 4) for p in prompts]
+    assert max(sum(n for _, n in c) for c in f.calls) == paged.MAX_ROWS
+    assert len(m.cache.free) == 2000
+    f.seen.clear()
+    stop = f.want([3], 3)[2]
+    assert m.generate([[3], [1] * 4500], 6, {stop}) == [f.want([3], 6, {stop}), f.want([1] * 4500, 6, {stop})]

@@ -130,7 +130,7 @@ __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, cons
     v.pos_lo = v.held - v.n + over_g(r0), v.pos_hi = v.held - v.n + over_g(r0 + max(v.rows, 1) - 1);
     // keys some row of the tile sees: [0, pre) and [lo, hi), as groups of 16
     v.hi = max(min(v.len, v.pos_hi + 1), 0);
-    v.lo = a.window ? min(max(v.pos_lo - a.window + 1, 0), v.hi) : 0;
+    v.lo = a.window && v.pos_lo >= a.window ? min(v.pos_lo - a.window + 1, v.hi) : 0;
     const int g_hi = (max(v.hi, v.prefix > v.lo ? v.prefix : 0) + 15) / 16;
     v.g_lo = v.lo / 16;
     v.g_pre = min((v.prefix + 15) / 16, v.g_lo);  // prefix groups before g_lo

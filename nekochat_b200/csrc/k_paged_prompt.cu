@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int pos_lo = held - n + over_g(r0), pos_hi = held - n + over_g(r0 + rows - 1);
     const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
     const int hi = max(min(len, pos_hi + 1), 0);
-    const int lo = a.window ? min(max(pos_lo - a.window + 1, 0), hi) : 0;
+    const int lo = a.window && pos_lo >= a.window ? min(pos_lo - a.window + 1, hi) : 0;
     const int t_lo = lo / kKeys, t_hi = (max(hi, prefix > lo ? prefix : 0) + kKeys - 1) / kKeys;
     const int t_pre = min((prefix + kKeys - 1) / kKeys, t_lo);
     const int nt_all = t_pre + max(t_hi - t_lo, 0);
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     if (!plain_mask) {
                         // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
-                        const int see_hi = min(len, qpos + 1) - jq, see_lo = (a.window ? qpos - a.window + 1 : 0) - jq;
+                        const int see_hi = min(len, qpos + 1) - jq, see_lo = (a.window && qpos >= a.window ? qpos - a.window + 1 : 0) - jq;
                         const int pre = (real ? prefix : 0) - jq;
                         const bool gone0 = kb[2 * q] == kGone, gone1 = kb[2 * q + 1] == kGone;
 #pragma unroll

@@ -273,3 +273,14 @@ def test_values_that_do_not_turn_stay_apart(torch, dtype, interleaved, e4m3, n):
     same(f64(got), want, 0 if dtype == "float32" else 2.0 ** -8)
     for g, w in zip(cache.values(scaled=False), before):
         same(g, w, 2.0 ** -3 if e4m3 else 2.0 ** -11)
+
+
+@pytest.mark.parametrize("new,lens", [([6, 1], [3, 40]), ([100, 1], [60, 300])])
+def test_a_window_that_leaves_nothing_out(torch, new, lens):
+    """The largest window there is gives what no window gives, also where positions are negative."""
+    rng = np.random.default_rng(110)
+    cache = Cache(torch, rng, lens, 2, 16, 128, False)
+    cache.fill(rng, lens)
+    a, _ = held_to(torch, cache, lens, new, 4, "float32", 111)
+    b, _ = held_to(torch, cache, lens, new, 4, "float32", 111, window=2 ** 31 - 1)
+    assert (a - b).abs().max() <= 1e-5 * a.abs().max()

@@ -229,7 +229,7 @@ typedef struct neko_paged_append_args {
 int neko_op_paged_append(const neko_paged_append_args* args, void* stream);
 /* Attention over the cache. Row q_start[s] + i of q is at position pos = kv_len[s] - n + i of its sequence, n its
  * new tokens (q_start NULL: one per sequence; they are in the cache already). Per query head h (KV head
- * h / (n_head / n_kv)) and key j: z = scale * q . k_j; with softcap > 0, z = softcap * tanh(z / softcap); with slopes,
+ * h / (n_head / n_kv)) and key j: z = scale * q . k_j; with softcap > 0 (finite), z = softcap * tanh(z / softcap); with slopes,
  * z += slopes[h] * (j - pos). Key j is seen when its page is resident, j < kv_len[s], and j <= pos with (window == 0
  * or pos - j < window), or j < prefix[s] (prefix NULL: none). out = sum_j softmax(z)_j v_j over the keys seen, zeros
  * when there are none. A value that is not seen has no effect, whatever it holds. Sums, maxima and accumulators are f32;

@@ -2,6 +2,7 @@
 #include "paged.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace neko;
 
@@ -95,6 +96,7 @@ extern "C" int neko_op_paged_attention(const neko_paged_attention_args* a, void*
     const int64_t excess = ((int64_t(1) << 32) + group - 1) / group * group - (int64_t(1) << 32);
     if (rows > INT32_MAX - 1024 || rows * excess >= (int64_t(1) << 32))
         return paged_fail(NEKO_ERR_UNSUPPORTED, op, "2^31 rows (new tokens times heads per KV head) or more; fewer where those heads are no power of two");
+    if (a->softcap == INFINITY) return paged_fail(NEKO_ERR_ARG, op, "softcap is finite (0: no cap)");
     if (a->window < 0 || !(a->softcap >= 0.0f) || !(a->scale == a->scale))
         return paged_fail(NEKO_ERR_ARG, op, "window and softcap are not negative");
     return finish(op, launch_paged_attention(own, static_cast<cudaStream_t>(stream)));

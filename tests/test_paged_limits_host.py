@@ -57,3 +57,9 @@ def test_yarn_ramps_between_its_two_speeds(theta, rot, original, factor, fast, s
         for pos in range(7):
             assert abs(table[pos, j, 0] - gain * math.cos(pos * w)) <= 1.2e-7 * gain
             assert abs(table[pos, j, 1] - gain * math.sin(pos * w)) <= 1.2e-7 * gain
+
+
+def test_an_infinite_cap_is_refused():
+    """cap tanh(z / cap) has no value there (no cap is 0)."""
+    assert call("neko_op_paged_attention", ATTEND, ops._ATTEND, tokens=2, softcap=float("inf")) == -1
+    assert b"softcap" in nb.lib().neko_last_error()

@@ -453,6 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     if (SRC == kCopies && page >= 0) page = s * c.max_pages + (j0 >> ps_log) + box;
                     const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
                     uint64_t* bar = scan ? &ms.land : &ms.full[st];
+                    __syncwarp();  // lane 0's arrival publishes what the other lanes have written above
                     if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box_bytes);
                     __syncwarp();
                     begun = x + 1, landing = scan;

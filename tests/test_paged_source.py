@@ -29,3 +29,15 @@ def test_a_loader_that_gives_up_waits_for_its_copies():
     rest = " ".join(src[start:end])
     given_up = rest.partition("if (!ok && warp == kLoadWarp)")[2]
     assert "wait_out(&ms.full[" in given_up and "wait_out(&ms.land" in given_up
+
+
+def test_what_lanes_write_is_ordered_before_the_arrival_that_publishes_it():
+    """Several lanes of the loader store a tile's scales and lane 0 arrives: a warp barrier stands between."""
+    src = lines("k_paged_prompt.cu")
+    stores = [i for i, x in enumerate(src) if "ms.ks[i % kRing][lane] =" in x]
+    assert len(stores) == 2
+    for i in stores:
+        rest = src[i:]
+        one = next(j for j, x in enumerate(rest) if re.search(r"mbar_arrive(_expect_tx)?\(", x))
+        alone = "lane == 0" in rest[one]
+        assert not alone or any("__syncwarp()" in x for x in rest[:one])

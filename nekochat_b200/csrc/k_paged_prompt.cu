@@ -28,7 +28,8 @@
 // order. Every wait is bounded and gives up once another role has failed.
 #include <cooperative_groups.h>
 
-#include <array>
+#include <algorithm>
+#include <atomic>
 
 #include "paged.cuh"
 #include "paged_math.cuh"
@@ -1044,35 +1045,35 @@ cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, in
     return e;
 }
 
-// How many clusters of 1 << log CTAs run at once (a CTA fills an SM; an SM left over in its GPC stays idle).
+// How many clusters of 1 << log CTAs run at once on the current device (a CTA fills an SM; an SM left over in its GPC stays
+// idle). Asked once per device; threads that ask at the same time get the same answer.
 template <int HD>
 int clusters_at_once(int log) {
-    static const std::array<int, 4> fits = [] {
-        std::array<int, 4> out = {};
+    static std::atomic<int> known[64][4];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::atomic<int>& slot = known[dev & 63][log];
+    if (const int n = slot.load(std::memory_order_relaxed)) return n;
+    int n = num_sms();
+    if (log > 0) {
         auto* fn = paged_prompt_kernel<HD, kCodes, true>;
-        const size_t smem = PL<HD, true>::kSmem;
-        const bool ready = ensure_dyn_smem(fn, smem) == cudaSuccess;
-        for (int i = 0; i < 4; i++) {
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 1u << i;
-            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-            cfg.gridDim = dim3(1u << i);
-            cfg.blockDim = dim3(kThreads);
-            cfg.dynamicSmemBytes = smem;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int n = 0;
-            if (!ready || cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) {
-                cudaGetLastError();
-                n = std::max(1, num_sms() >> (i + 1));
-            }
-            out[size_t(i)] = i ? n : num_sms();
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1u << log;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(1u << log);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = PL<HD, true>::kSmem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (ensure_dyn_smem(fn, PL<HD, true>::kSmem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = std::max(1, num_sms() >> (log + 1));
         }
-        return out;
-    }();
-    return fits[size_t(log)];
+    }
+    slot.store(n, std::memory_order_relaxed);
+    return n;
 }
 
 // Row tiles of a CTA and CTAs of a cluster: what takes the least time by the measured cost of 128 keys (one and two row

@@ -41,3 +41,10 @@ def test_what_lanes_write_is_ordered_before_the_arrival_that_publishes_it():
         one = next(j for j, x in enumerate(rest) if re.search(r"mbar_arrive(_expect_tx)?\(", x))
         alone = "lane == 0" in rest[one]
         assert not alone or any("__syncwarp()" in x for x in rest[:one])
+
+
+def test_what_is_asked_once_is_asked_once_per_device():
+    """Clusters that run at once: kept by device, like the number of SMs beside it (one GPU cannot show the difference)."""
+    src = " ".join(lines("k_paged_prompt.cu"))
+    body = src[src.index("int clusters_at_once(int log) {"):]
+    assert "cudaGetDevice(&dev)" in body[:300] and "[dev & 63]" in body[:400]

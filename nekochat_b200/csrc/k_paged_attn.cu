@@ -87,8 +87,9 @@ struct DecodePlan {
     uint64_t group_inv;   // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
     uint32_t page_16;     // page stride in 16-byte units
     int page_log;
-    float* part;          // [row tile][2 * CTAs][rows][HD + 4]: values, maximum, sum
+    float* part;          // [row tile][2 * CTAs][rows][HD + 4]: values, maximum, sum (NULL where a row tile has one CTA)
     int4* desc;           // [row tile][CTAs]: an item that starts in the CTA and ends in a later one
+    int tile0;            // first row tile of the launch
     int ranks_log;        // of the clusters of the small variant
 };
 
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
-    const int tile = blockIdx.y, G = plan.group, n_kv = c.n_kv;
+    const int tile = plan.tile0 + blockIdx.y, G = plan.group, n_kv = c.n_kv;
     uint8_t* smb = reinterpret_cast<uint8_t*>(sm);
     int4* meta = reinterpret_cast<int4*>(smb + TL::kMetaOff);  // item, 1 starts | 2 ends, row0, rows; item -1: none
     int* totals = reinterpret_cast<int*>(smb + TL::kScanOff);
@@ -731,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             }
         }
     }
-    if (!open_item && tid == 0) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(-1, 0, 0, 0);
+    if (!open_item && tid == 0 && plan.desc) plan.desc[int64_t(tile) * gridDim.x + cta] = make_int4(-1, 0, 0, 0);
     pdl_trigger();
 }
 
@@ -802,14 +803,16 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     p.page_16 = uint32_t(c.page_stride * (Q8 ? 1 : 2) / 16);
     p.page_log = 31 - __builtin_clz(c.page_size);
     p.ranks_log = 0;
+    p.tile0 = 0;
     const int64_t row_tiles = (int64_t(a.max_new) * p.group + TL::kRows - 1) / TL::kRows;
-    if (row_tiles > 65535) return cudaErrorInvalidConfiguration;
-    // as many CTAs as the GPU holds at a time, or a group of 16 keys for each warp where the cache has room for fewer
+    // as many CTAs for each row tile as the GPU holds at a time, or a group of 16 keys for each warp where the cache has room for
+    // fewer. Prompts on heads of 32 have thousands of row tiles: no more than 16 times what the GPU holds in all, which bounds the
+    // parts (80 MB, two states a CTA), and none where that is one CTA each.
     const int64_t groups = int64_t(c.max_pages) * c.page_size / 16 * c.n_kv * c.n_seq;
     const int64_t items = int64_t(c.n_kv) * c.n_seq;
-    const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(int64_t(num_sms()) * kCtas<HD, Q8, NT>, std::max(groups, items) / kWarps)));
-    const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
     const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, room = int64_t(num_sms()) * kCtas<HD, Q8, NT>;
+    const int ctas = int(std::max<int64_t>(1, std::min({room, std::max(groups, items) / kWarps, 16 * room / row_tiles})));
+    const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
     if (const int ranks = c.n_kv <= 65535 ? small_ranks(items * row_tiles, per_item, room) : 0) {
         auto* small = paged_decode_kernel<HD, Q8, HILO, NT, true>;
         if (cudaError_t e = ensure_dyn_smem(small, TL::smem_small()); e != cudaSuccess) return e;
@@ -832,6 +835,12 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     const size_t smem = TL::smem(c.n_seq);
     cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;
+    if (ctas == 1) {  // nothing is shared
+        p.part = nullptr, p.desc = nullptr;
+        for (int64_t left = row_tiles; left > 0 && e == cudaSuccess; left -= 65535, p.tile0 += 65535)
+            e = launch_ex(fn, dim3(1, unsigned(std::min<int64_t>(left, 65535))), dim3(kThreads), smem, st, false, a, p);
+        return e;
+    }
     void* mem = nullptr;
     if ((e = scratch_alloc(&mem, part_bytes + desc_bytes, st)) != cudaSuccess) return e;
     p.part = static_cast<float*>(mem);

@@ -10,8 +10,8 @@
 // its 8 columns. The order of the summed index is free as long as both operands agree, so the fragments come straight
 // from global memory: lane (g, t) holds, for K, 16-byte pieces t, t + 4, .. of key rows g and g + 8, and for V the
 // pieces g, g + 8, .. of key rows 2t, 2t + 1, 2t + 8, 2t + 9; neither K nor V passes through shared memory. 8-bit codes
-// become f16 in registers (exact), keys' scales multiply the scores, values' scales the weights, relative to a reference
-// that the accumulators are in units of. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
+// become f16 in registers (exact), keys' scales multiply the scores, values' scales the products of 16 keys on their way to
+// the accumulators. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
 // 16-bit queries one exact f16 column, weights one f16. Rows are scaled by a power of two into f16's range first.
 // All groups of all items, in order, are dealt out in equal shares to the warps that the GPU holds at a time, whatever
@@ -160,8 +160,11 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
-    // Weights are 2^(score - maximum + kLift) times a ratio of value scales up to kVLazy: at most 2^15, clear of f16's subnormals.
-    constexpr float kLazy = 8.0f, kVLazy = 16.0f, kLift = 3.0f;
+    // Weights are 2^(score - maximum + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with hi + lo, is 2^-32 of the
+    // largest weight; the maximum lags by 2^kLazy at most. 8-bit values' scales are outside the products (times 2^-15, which
+    // the sum of the weights takes too: an accumulator is no larger than the values).
+    constexpr float kLazy = 8.0f, kLift = 7.0f;
+    constexpr float kUnit = Q8 ? 1.0f / 32768.0f : 1.0f;
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
@@ -348,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 
         float acc[NT][kSteps][4];
         float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];
-        float vref = 0.0f;  // the value scale that the accumulators are in units of
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -445,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                             else z[nt][r][h] = -INFINITY;
                         }
             }
-            // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact) and value scale
-            const float vs_now = vs;
+            // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact)
+            const float vs_now = vs * kUnit;
             bool up = false;
             float top[NT][TL::kLaneRows];
 #pragma unroll
@@ -460,13 +462,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                     top[nt][r] = x;
                     up |= x > m[nt][r] + kLazy;
                 }
-            const bool v_up = Q8 && vs_now > kVLazy * vref;
-            if (__any_sync(0xffffffffu, up) || v_up) {
-                float fv = 1.0f;
-                if (v_up) {
-                    fv = __fdividef(vref, vs_now);
-                    vref = vs_now;
-                }
+            if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float f[TL::kLaneRows];
@@ -478,7 +474,6 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                             m[nt][r] = top[nt][r];
                             l[nt][r] *= f[r];
                         }
-                        f[r] *= fv;
                     }
 #pragma unroll
                     for (int i = 0; i < kSteps; i++)
@@ -486,9 +481,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                         for (int e = 0; e < 4; e++) acc[nt][i][e] *= f[HILO ? 0 : e & 1];
                 }
             }
-            // ---- weights as B fragments, in units of the reference scale
+            // ---- weights as B fragments
             uint32_t pf[NT][2];
-            const float ratio = Q8 ? (vref > 0.0f ? __fdividef(vs_now, vref) : 0.0f) : 1.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float p[2][TL::kLaneRows];
@@ -502,11 +496,11 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 for (int h = 0; h < 2; h++) {
                     uint32_t hl;
                     if constexpr (HILO) {
-                        const float x = p[h][0] * ratio;
+                        const float x = p[h][0];
                         const __half hi1 = __float2half_rn(x);
                         hl = h2u(__halves2half2(hi1, __float2half_rn(x - __half2float(hi1))));
                     } else {
-                        hl = h2u(__floats2half2_rn(p[h][0] * ratio, p[h][1] * ratio));
+                        hl = h2u(__floats2half2_rn(p[h][0], p[h][1]));
                     }
                     pf[nt][h] = movmatrix(hl);
                 }
@@ -554,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
                                     const int r = HILO ? 0 : e & 1;
-                                    if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e];
+                                    if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] = fmaf(d[e], vs_now, acc[nt][i][e]);
                                 }
                             }
                         }
@@ -571,13 +565,14 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 v_frag(i, f);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    if constexpr (HILO) {
-                        // added outside the MMA, which truncates: on the accumulator itself every group took 3e-8 off it
-                        // (an error of 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time; 16-bit results do not see it)
+                    if constexpr (HILO || Q8) {
+                        // Added outside the MMA: it truncates (on the accumulator itself every group took 3e-8 off it, an error of
+                        // 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time), and 8-bit values' scales come
+                        // in here, in f32, so that small blocks keep their bits beside large ones.
                         float d[4];
                         mma16816_z(d, f, pf[nt][0], pf[nt][1]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[nt][i][e] += d[e];
+                        for (int e = 0; e < 4; e++) acc[nt][i][e] = Q8 ? fmaf(d[e], vs_now, acc[nt][i][e]) : acc[nt][i][e] + d[e];
                     } else {
                         mma16816(acc[nt][i], f, pf[nt][0], pf[nt][1]);
                     }
@@ -599,13 +594,12 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
                 float* st = st0 + row * TL::kPitch;
-                if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum;
+                if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum * kUnit;
 #pragma unroll
                 for (int i = 0; i < kSteps; i++) {
                     float2 v;
                     v.x = HILO ? acc[nt][i][0] + acc[nt][i][1] : acc[nt][i][r];
                     v.y = HILO ? acc[nt][i][2] + acc[nt][i][3] : acc[nt][i][2 + r];
-                    if (Q8) v.x *= vref, v.y *= vref;
                     const int d = Q8 ? (HD / 8) * g + 2 * i : W::kV >= 4 ? 64 * (i / 4) + 8 * g + 2 * (i % 4) : 4 * g + 2 * i;
                     *reinterpret_cast<float2*>(st + d) = v;
                 }

@@ -326,3 +326,58 @@ def test_long_prompts_on_heads_of_32_take_little_scratch_memory(torch, n, dtype)
         want, mass = (p.T @ x[lo:i + 1] for x in (vv, vv.abs()))
         reach = (kk[lo:i + 1].abs() @ q[i].double().abs().T * 32 ** -0.5).amax(0)
         assert ((out[i].double() - want).abs() <= bound(dtype, want, mass, reach)).all()
+
+
+FORMS = {  # new tokens, length, query heads, KV heads, head dim
+    "step": (1, 300, 4, 2, 128), "step, many keys": (1, 6000, 8, 2, 64), "verify": (7, 300, 8, 2, 128), "head dim 32": (30, 200, 4, 2, 32),
+    "rows of a few tiles": (200, 300, 4, 2, 128),
+}
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_small_blocks_keep_their_bits_beside_large_ones(torch, form, dtype):
+    """Blocks of values 2^-30 the size of their neighbours', which the softmax prefers by 2^-90: the result is theirs, in
+    all its bits."""
+    new, L, heads, n_kv, hd = FORMS[form]
+    rng = np.random.default_rng(94)
+    cache = Cache(torch, rng, [L], n_kv, 16, hd, True)
+    g = torch.Generator("cuda").manual_seed(95)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+    k[..., 0] = 0
+    order = torch.from_numpy(cache.table[0]).cuda().long()
+    k[order[1::2], :, :, 0] = -31.25  # times 2 of q: 62.5 less
+    v[order[0::2]] *= 2.0 ** -30
+    quantize(torch, cache, k, v)
+    q = torch.randn((new, heads, hd), device="cuda", generator=g) * 0.1
+    q[..., 0] = 2.0
+    held_to(torch, cache, [L], [new], heads, dtype, 96, q=q, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,L,window", [(200, 330, 24), (9, 60, 5)])
+def test_blocks_that_a_row_does_not_see_take_none_of_its_bits(torch, new, L, window, dtype):
+    """Values 2^40 larger in every fourth block: rows whose window or place leaves those out are exact in their own size."""
+    rng = np.random.default_rng(97)
+    cache = Cache(torch, rng, [L], 2, 16, 128, True)
+    g = torch.Generator("cuda").manual_seed(98)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+    v[torch.from_numpy(cache.table[0]).cuda().long()[3::4]] *= 2.0 ** 40
+    quantize(torch, cache, k, v)
+    held_to(torch, cache, [L], [new], 4, dtype, 99, window=window)
+
+
+@pytest.mark.parametrize("new,L", [(1, 200), (100, 200)])
+def test_values_at_the_ends_of_the_scales(torch, new, L):
+    """All values about 2^-95, about 2^100, and blocks of zeros (scale 2^-100) beside others: relative to their own size."""
+    rng = np.random.default_rng(100)
+    for size in (2.0 ** -95, 2.0 ** 100, 0.0):
+        cache = Cache(torch, rng, [L], 2, 16, 128, True)
+        g = torch.Generator("cuda").manual_seed(101)
+        k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+        if size:
+            v *= size
+        else:
+            v[torch.from_numpy(cache.table[0]).cuda().long()[::2]] = 0
+        quantize(torch, cache, k, v)
+        held_to(torch, cache, [L], [new], 4, "float32", 102)

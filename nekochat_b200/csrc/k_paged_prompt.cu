@@ -20,7 +20,9 @@
 //  * warps 16..18: the loader. K and V tiles go to a ring of shared-memory stages in the 128-byte-swizzled layout that
 //    serves K as a K-major and V as an MN-major operand: tensor copies for f16 pages, registers and an exact conversion to
 //    f16 for 8-bit ones (fetched one tile ahead). Scales stay out of the operands: a block's key scale multiplies its
-//    scores and its value scale enters the weights' exponent (the sum takes it out again), 16 columns at a time.
+//    scores and its value scale enters the weights' exponent (the sum takes it out again), 16 columns at a time. A row's
+//    reference is then the largest score plus log2 of the value scale that it sees: what is rounded off a weight is small beside
+//    what the largest of its products adds, not beside the largest scale.
 //  * warp 19, an elected lane: issues the UMMAs; PV of one tile and S of its next key tile go back to back.
 // Masks only touch the key tiles that need them. Values that no row sees are zeroed by the loader; values that are not
 // finite in a tile that some row does not see whole are zeroed too and added by the threads of the rows that see them.
@@ -49,10 +51,10 @@ constexpr int kCopyTiles = 2;
 constexpr int64_t kCopyBytes = int64_t(1) << 31;
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
-// Weights are 2^(score - reference + kLift), in units of the reference value scale: at most 2^15, clear of f16's subnormals.
+// Weights are 2^(score (+ log2 of the value scale) - reference + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with
+// hi + lo, is 2^-32 of the largest.
 constexpr float kLazy = 8.0f;   // log2 of how far a score may exceed the reference maximum
-constexpr float kVLazy = 4.0f;  // and a block's value scale the reference scale
-constexpr float kLift = 15.0f - kLazy - kVLazy;
+constexpr float kLift = 15.0f - kLazy;
 // An UMMA's f32 accumulation truncates: each step takes a share off the sum, 3.2e-8 on average (measured on sums of 2,500
 // steps, whose common factor was 1 - 2.1e-5; half a unit in the last of 24 places is 4.3e-8 of a mantissa spread evenly over
 // the logarithm). What O held before a step loses as a whole, so the sum of the weights, which is rounded to nearest, is made
@@ -62,7 +64,7 @@ constexpr float kLift = 15.0f - kLazy - kVLazy;
 constexpr float kDrop = 3.2e-8f;
 constexpr int kFlush = 8;
 constexpr int64_t kFlushBytes = int64_t(1) << 30;  // sums of more CTAs stay in TMEM (batches padded to their longest prompt can be large)
-constexpr float kVMin = -64.0f; // a block's scale counts as no less than 2^-64 of the reference
+constexpr float kVMin = -60.0f; // the product of a row's likeliest key with a block's scale counts as no less than 2^-60 of the reference
 constexpr float kVNone = -126.0f;
 constexpr float kGone = -1.0f;
 
@@ -88,7 +90,7 @@ struct PL {
     static constexpr int kStages = HD == 64 ? 5 : HILO ? 3 : 5;
     static constexpr int kStageOff = kQBytes;
     static constexpr int kMiscOff = kStageOff + kStages * kStage;
-    static constexpr int kJoinPitch = HD + 4;             // floats of a row's state: values, maximum, sum
+    static constexpr int kJoinPitch = HD + 4;             // floats of a row's state: values, their unit, sum, its unit
     static constexpr int kSmem = kMiscOff + 3072 - 128;
     static_assert(kSmem <= 227 * 1024, "shared memory");
     static_assert(2 * kRows * kJoinPitch * 4 <= kMiscOff, "the joined states take the operands' place");
@@ -101,11 +103,11 @@ struct Misc {
     uint32_t tmem, fail;
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
-    float vtop[kRing];                 // the largest of vs
     uint32_t whole[kRing];             // every block is resident
     uint32_t odd[kOddRing][4];         // of a key tile that needs masks: keys with values that are not finite
-    float most[2][2 * kRows];          // by half of the key tile: the rows' largest scores, at the end their sums; before
-                                       // the first tile most[0] is scale / the row's power of two
+    float most[2][2 * kRows];          // by half of the key tile: the rows' largest scores (with value scales), at the end their
+                                       // largest scores without and their sums; before the first tile most[0] is scale / the
+                                       // row's power of two
 };
 static_assert(sizeof(Misc) <= 3072 - 128, "misc");
 
@@ -300,9 +302,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const uint32_t tmem = ms.tmem;
     volatile uint32_t* fail = &ms.fail;
 
-    float row_max = -INFINITY, row_sum = 0.0f, vref = 0.0f;  // of a softmax thread's row; vref: log2 of O's unit
-    // f32 queries: this thread's first kept sum (256 floats between columns), and log2 of their unit, the reference maximum and
-    // value scale, which only grow
+    // Of a softmax thread's row: log2 of O's unit (the reference), and the sum of the weights with log2 of its unit. Without
+    // value scales the two are one; with them the sum's is the largest score of this thread's half of the keys.
+    float row_max = -INFINITY, row_sum = 0.0f, sum_max = -INFINITY;
+    // f32 queries: this thread's first kept sum (256 floats between columns), and log2 of their unit, which only grows
     float* kept = nullptr;
     float kept_ref = 0.0f, sum_kept = 0.0f;  // and the weights' sum that goes with them
     if (warp >= kLoadWarp && warp < kMmaWarp) {
@@ -365,10 +368,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 uint8_t* base = sm + L::kStageOff + st * L::kStage + place;
                 if (!v) {
                     if (warp == kLoadWarp) {
-                        const float vl = lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone, vt = warp_max(vl);
+                        const float vl = lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone;
                         const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0);
                         if (lane < 8) ms.ks[i % kRing][lane] = pages >= 0 ? fabsf(ks) : kGone, ms.vs[i % kRing][lane] = vl;
-                        if (lane == 0) ms.vtop[i % kRing] = vt, ms.whole[i % kRing] = whole;
+                        if (lane == 0) ms.whole[i % kRing] = whole;
                     }
                     // every loader thread is past item x - kStages (the wait above), so none has touched tile i + 2's yet
                     if (lt >= 32 && lt < 36) ms.odd[(i + 2) % kOddRing][lt - 32] = 0;
@@ -444,9 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     if (!v) {
                         const float vl = SRC == kCopies && lane < 8 && pages >= 0 ? fmaxf(log2f(vs), kVNone) : kVNone;
-                        const float vt = SRC == kCopies ? warp_max(vl) : 0.0f;
                         if (lane < 8) ms.ks[i % kRing][lane] = pages < 0 ? kGone : SRC == kCopies ? fabsf(ks) : 1.0f, ms.vs[i % kRing][lane] = vl;
-                        if (lane == 0) ms.vtop[i % kRing] = vt;
                     }
                     if (!v && lane < 4) ms.odd[(i + 2) % kOddRing][lane] = 0;
                     if (!v && lane == 0) ms.whole[i % kRing] = whole;
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     tc_fence_after();
                     const bool again = kept != nullptr;
                     kept = plan.flush + (int64_t(blockIdx.x) * HD + col_w * (HD / 2)) * (2 * kRows) + r;
-                    const float now = (row_max == -INFINITY ? 0.0f : row_max) + vref, f = ex2(fminf(kept_ref - now, 0.0f));
+                    const float now = row_max == -INFINITY ? 0.0f : row_max, f = ex2(fminf(kept_ref - now, 0.0f));
                     kept_ref = now;
                     sum_kept += row_sum;
                     row_sum = 0.0f;
@@ -740,12 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 st_wait();
             };
-            if (kScaled || odd_tile) {
-                const float vnow = kScaled ? ms.vtop[i % kRing] : 0.0f;
-                const bool v_up = kScaled && (i == 0 || vnow > vref + kVLazy);
-                if (odd_tile || (v_up && i > 0)) fix_o(v_up && i > 0 ? ex2(vref - vnow) : 1.0f, odd_tile);
-                if (v_up) vref = vnow;
-            }
+            if (odd_tile) fix_o(1.0f, true);
             // ---- tiles that need more than the scale: a cap, a bias, masks; 32 scores at a time in a rolled loop, in log2 units
             // back into TMEM
             const float *kb = ksp + 4 * col_w, *vb = vsp + 4 * col_w;  // of this thread's blocks of 16 keys
@@ -806,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
                 st_wait();
             }
-            // ---- this thread's 64 scores and the largest of them
+            // ---- this thread's 64 scores and the largest of them, with their blocks' value scales and without
             uint32_t u[2][32];
             ld32(tc, u[0]);
             ld32(tc + 32, u[1]);
@@ -814,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
 #pragma unroll
             for (int b = 0; b < 4; b++) fb[b] = shaped ? 1.0f : kScaled ? factor * kb[b] : factor;
             ld_wait(u[0]), ld_wait(u[1]);
-            float top = -INFINITY;
+            float top = -INFINITY, top_score = -INFINITY;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 float m[4];
@@ -823,34 +819,45 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     const float v = __uint_as_float(u[b / 2][16 * (b & 1) + x]);
                     m[x & 3] = x < 4 ? v : max_nan(m[x & 3], v);
                 }
-                top = max_nan(top, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * fb[b]);
+                const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * fb[b];
+                top = max_nan(top, kScaled ? most + vb[b] : most);
+                if (kScaled) top_score = max_nan(top_score, most);
+            }
+            if (kScaled && top_score > sum_max && top_score < INFINITY) {
+                top_score = ceilf(top_score);
+                const float f = ex2(sum_max - top_score);  // from -inf: 0
+                sum_max = top_score, row_sum *= f;
+                if (HILO) sum_kept *= f;
             }
             // One buffer: this tile's scores exist, so the other thread has handed in its last weights and read this one's.
             ms.most[col_w][r] = top;
             meet();
             top = max_nan(top, ms.most[col_w ^ 1][r]);
             if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
-            // the reference moves only when a score exceeds it by more than 2^kLazy (the same decision in both warps of a row)
+            // The reference moves only when a score exceeds it by more than 2^kLazy (the same decision in both warps of a row). Units are
+            // whole powers of two, as the append's scales are: what goes from one to another is exact.
             const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
             if (__any_sync(0xffffffffu, up)) {
                 float f = 1.0f;
                 if (up) {
-                    f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
-                    row_max = top;
-                    row_sum *= f;
-                    if (HILO) sum_kept *= f;
+                    const float next = ceilf(top);
+                    f = ex2(row_max - next);  // row_max = -inf: nothing there yet, 0
+                    row_max = next;
+                    if (!kScaled) row_sum *= f;
+                    if (!kScaled && HILO) sum_kept *= f;
                 }
                 if (i > 0) fix_o(f, false);
             }
             // ---- weights, their sum; P over this thread's scores
-            const float ref = (row_max == -INFINITY ? 0.0f : row_max) - kLift;
+            const float ref = row_max == -INFINITY ? 0.0f : row_max, sum_ref = sum_max == -INFINITY ? 0.0f : sum_max;
             float sum = 0.0f;
             uint64_t sums[2] = {0, 0};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 const int q = b / 2, g = b & 1;
-                const float vr = kScaled ? fmaxf(vb[b] - vref, kVMin) : 0.0f;
-                const uint64_t ff = pack2(fb[b], fb[b]), off = pack2(vr - ref, vr - ref);
+                // weights of score and scale against the reference: 2^vr times what they add to the sum
+                const float vr = kScaled ? fmaxf(vb[b] + (sum_ref - ref), kVMin) : 0.0f, o = (kScaled ? vr - sum_ref : -ref) + kLift;
+                const uint64_t ff = pack2(fb[b], fb[b]), off = pack2(o, o);
                 if (kScaled) sums[0] = sums[1] = 0;
                 [[maybe_unused]] uint32_t lo8[8];
 #pragma unroll
@@ -887,6 +894,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             __syncwarp();
             tc_fence_after();
         }
+        if constexpr (kScaled) {  // the two halves' sums in one unit
+            ms.most[col_w][r] = sum_max;
+            meet();
+            const float both = fmaxf(sum_max, ms.most[col_w ^ 1][r]);
+            meet();  // both are read before the sums take their place
+            if (sum_max > -INFINITY) {
+                const float f = ex2(sum_max - both);
+                row_sum *= f;
+                if (HILO) sum_kept *= f;
+            }
+            sum_max = both;
+        }
     }
     // ---- the outputs. Alone: through shared memory, once the operands are used up. In a cluster each CTA owns a share of
     // the rows: every CTA pushes its states of them into the owner's shared memory.
@@ -903,9 +922,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         const int r = row_w;
         const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + half_w * 128 + col_w * (HD / 2);
         row_sum += ms.most[col_w ^ 1][r];
-        float f = kScaled ? exp2f(vref) : 1.0f;
-        if (alone) f = row_sum == 0.0f ? 0.0f : f / row_sum;
-        const float f_kept = ex2(fminf(kept_ref - (row_max == -INFINITY ? 0.0f : row_max) - vref, 0.0f));
+        float f = 1.0f;
+        if (alone) f = row_sum == 0.0f ? 0.0f : (kScaled && row_max > -INFINITY ? exp2f(row_max - sum_max) : 1.0f) / row_sum;
+        const float f_kept = ex2(fminf(kept_ref - (row_max == -INFINITY ? 0.0f : row_max), 0.0f));
         float* mine = (alone ? state : cluster.map_shared_rank(state, r / share)) + (rank * share + r % share) * L::kJoinPitch;
 #pragma unroll
         for (int x = 0; x < HD / 2; x += 32) {
@@ -924,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 *reinterpret_cast<float4*>(mine + col_w * (HD / 2) + x + y) = v;
             }
         }
-        if (!col_w) mine[HD] = row_max, mine[HD + 1] = row_sum;
+        if (!col_w) mine[HD] = row_max, mine[HD + 1] = row_sum, mine[HD + 2] = kScaled ? sum_max : row_max;
     }
     tc_fence_before();
     if (alone) __syncthreads();
@@ -950,17 +969,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int mine = min(max(rows - rank * share, 0), share);  // rows that this CTA owns
     for (int x = tid; x < mine * (HD / 4); x += kThreads) {
         const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-        float top = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < plan.ranks; w++) top = fmaxf(top, state[(w * share + r) * L::kJoinPitch + HD]);
-        const float ref = top == -INFINITY ? 0.0f : top;
+        float top = -INFINITY, top_sum = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < plan.ranks; w++) {
+            const float* st = state + (w * share + r) * L::kJoinPitch;
+            top = fmaxf(top, st[HD]), top_sum = fmaxf(top_sum, st[HD + 2]);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top, sum_ref = top_sum == -INFINITY ? 0.0f : top_sum;
         float4 v = make_float4(0, 0, 0, 0);
         for (int w = 0; w < plan.ranks; w++) {
             const float* st = state + (w * share + r) * L::kJoinPitch;
             const float f = ex2(st[HD] - ref);
             const float4 o = *reinterpret_cast<const float4*>(st + d);
-            sum = fmaf(f, st[HD + 1], sum), v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
+            sum = fmaf(kScaled ? ex2(st[HD + 2] - sum_ref) : f, st[HD + 1], sum), v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
         }
-        const float f = 1.0f / sum;
+        const float f = (kScaled ? exp2f(ref - sum_ref) : 1.0f) / sum;
         put(rank * share + r, d, sum == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
     }
 }

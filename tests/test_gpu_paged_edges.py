@@ -331,6 +331,7 @@ def test_long_prompts_on_heads_of_32_take_little_scratch_memory(torch, n, dtype)
 FORMS = {  # new tokens, length, query heads, KV heads, head dim
     "step": (1, 300, 4, 2, 128), "step, many keys": (1, 6000, 8, 2, 64), "verify": (7, 300, 8, 2, 128), "head dim 32": (30, 200, 4, 2, 32),
     "rows of a few tiles": (200, 300, 4, 2, 128),
+    "prompt on keys": (60, 2500, 8, 2, 64), "prompt": (700, 800, 4, 2, 128), "prompt, heads of 64": (900, 1000, 4, 2, 64),
 }
 
 
@@ -355,7 +356,7 @@ def test_small_blocks_keep_their_bits_beside_large_ones(torch, form, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("new,L,window", [(200, 330, 24), (9, 60, 5)])
+@pytest.mark.parametrize("new,L,window", [(200, 330, 24), (9, 60, 5), (300, 300, 0), (700, 900, 24), (700, 700, 0)])
 def test_blocks_that_a_row_does_not_see_take_none_of_its_bits(torch, new, L, window, dtype):
     """Values 2^40 larger in every fourth block: rows whose window or place leaves those out are exact in their own size."""
     rng = np.random.default_rng(97)
@@ -367,7 +368,7 @@ def test_blocks_that_a_row_does_not_see_take_none_of_its_bits(torch, new, L, win
     held_to(torch, cache, [L], [new], 4, dtype, 99, window=window)
 
 
-@pytest.mark.parametrize("new,L", [(1, 200), (100, 200)])
+@pytest.mark.parametrize("new,L", [(1, 200), (100, 200), (700, 800)])
 def test_values_at_the_ends_of_the_scales(torch, new, L):
     """All values about 2^-95, about 2^100, and blocks of zeros (scale 2^-100) beside others: relative to their own size."""
     rng = np.random.default_rng(100)

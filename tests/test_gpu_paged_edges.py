@@ -382,3 +382,36 @@ def test_values_at_the_ends_of_the_scales(torch, new, L):
             v[torch.from_numpy(cache.table[0]).cuda().long()[::2]] = 0
         quantize(torch, cache, k, v)
         held_to(torch, cache, [L], [new], 4, "float32", 102)
+
+
+SHAPES = {  # what takes the call: new tokens, lengths, query heads, KV heads, head dim, page
+    "one token, short": ([1] * 4, [1, 17, 500, 777], 16, 8, 128, 16),
+    "one token, long": ([1] * 9, [9000, 1, 5000, 33, 700, 8191, 64, 4097, 128], 16, 2, 128, 64),
+    "one token, wide heads": ([1] * 40, [300 + 41 * i for i in range(40)], 12, 12, 64, 32),
+    "verify": ([5, 3, 9, 1], [2000, 3, 4100, 900], 8, 4, 128, 64),
+    "head dim 32": ([7, 130, 1], [300, 130, 900], 8, 2, 32, 16),
+    "chunk": ([64], [576], 16, 8, 128, 16),
+    "prompts": ([300, 41, 257, 1], [300, 900, 800, 650], 12, 4, 128, 64),
+    "prompts, narrow heads": ([200, 129], [1500, 129], 6, 2, 64, 128),
+    "a prompt among steps": ([500] + [1] * 12, [900] + [50 + 97 * i for i in range(12)], 8, 2, 128, 64),
+}
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=20.0, window=150, alibi=True), dict(window=70, prefix=True)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_every_value_within_its_own_bound(torch, shape, opts, e4m3, dtype):
+    """Normal keys and values, 8-bit ones quantized as the append does: a wrong head, key range, window's edge or scale moves an
+    output by its own size, and the bounds are 2 to 3 orders below that."""
+    new, lens, heads, n_kv, hd, ps = SHAPES[shape]
+    opts = dict(opts)
+    if opts.pop("prefix", False):
+        opts["prefix"] = [max(0, x // 2 - 5) for x in lens]
+    rng = np.random.default_rng(91)
+    cache = Cache(torch, rng, lens, n_kv, ps, hd, e4m3)
+    g = torch.Generator("cuda").manual_seed(92)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) * torch.exp(0.5 * torch.randn((cache.k.shape[0], n_kv, ps, 1), device="cuda", generator=g))
+            for _ in range(2))
+    quantize(torch, cache, k, v)
+    held_to(torch, cache, lens, new, heads, dtype, 93, **opts)

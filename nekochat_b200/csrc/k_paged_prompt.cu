@@ -922,8 +922,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         const int r = row_w;
         const uint32_t to = tmem + (uint32_t(32 * (warp & 3)) << 16) + 256 + half_w * 128 + col_w * (HD / 2);
         row_sum += ms.most[col_w ^ 1][r];
+        // A row without keys goes by its reference: its sum holds the 2^-126 that exp2_poly gives a masked score (NaN stays).
+        const bool none = row_max == -INFINITY && row_sum == row_sum;
         float f = 1.0f;
-        if (alone) f = row_sum == 0.0f ? 0.0f : (kScaled && row_max > -INFINITY ? exp2f(row_max - sum_max) : 1.0f) / row_sum;
+        if (alone) f = none ? 0.0f : (kScaled && row_max > -INFINITY ? exp2f(row_max - sum_max) : 1.0f) / row_sum;
         const float f_kept = ex2(fminf(kept_ref - (row_max == -INFINITY ? 0.0f : row_max), 0.0f));
         float* mine = (alone ? state : cluster.map_shared_rank(state, r / share)) + (rank * share + r % share) * L::kJoinPitch;
 #pragma unroll
@@ -939,7 +941,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             for (int y = 0; y < 32; y += 4) {
                 float4 v = make_float4(__uint_as_float(w[y]) * f, __uint_as_float(w[y + 1]) * f, __uint_as_float(w[y + 2]) * f,
                                        __uint_as_float(w[y + 3]) * f);
-                if (alone && row_sum == 0.0f) v = make_float4(0, 0, 0, 0);
+                if (alone && none) v = make_float4(0, 0, 0, 0);
                 *reinterpret_cast<float4*>(mine + col_w * (HD / 2) + x + y) = v;
             }
         }

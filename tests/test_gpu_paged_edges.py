@@ -415,3 +415,20 @@ def test_every_value_within_its_own_bound(torch, shape, opts, e4m3, dtype):
             for _ in range(2))
     quantize(torch, cache, k, v)
     held_to(torch, cache, lens, new, heads, dtype, 93, **opts)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new,L,page_gone", [(700, 128, False), (700, 100, False), (100, 60, False), (7, 3, False), (150, 150, True), (1, 40, True)])
+def test_rows_that_see_nothing_beside_rows_that_do(torch, new, L, page_gone, e4m3, dtype):
+    """Zeros, not NaN, whatever the values' scale: positions before the first token, and pages that are gone."""
+    rng = np.random.default_rng(107)
+    cache = Cache(torch, rng, [L], 2, 16, 128, e4m3)
+    g = torch.Generator("cuda").manual_seed(108)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+    quantize(torch, cache, k, v if not e4m3 else v * 2.0 ** 17)
+    if page_gone:
+        cache.table[0, :3] = -1
+    got, want = held_to(torch, cache, [L], [new], 4, dtype, 109)
+    none = (want == 0).all(-1)
+    assert none.any() and (got[none] == 0).all()

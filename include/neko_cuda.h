@@ -233,7 +233,8 @@ int neko_op_paged_append(const neko_paged_append_args* args, void* stream);
  * z += slopes[h] * (j - pos). Key j is seen when its page is resident, j < kv_len[s], and j <= pos with (window == 0
  * or pos - j < window), or j < prefix[s] (prefix NULL: none). out = sum_j softmax(z)_j v_j over the keys seen, zeros
  * when there are none. A value that is not seen has no effect, whatever it holds. Sums, maxima and accumulators are f32;
- * NEKO_T_F32 queries and weights enter the tensor cores as f16 hi + lo (22 bits), 16-bit ones as one f16.
+ * NEKO_T_F32 queries and weights enter the tensor cores as f16 hi + lo (22 bits, and what is rounded off a weight is at most 2^-32
+ * of the row's largest), 16-bit ones as one f16 (11 bits; bf16 queries below 2^-17 of their row's largest fewer). E4M3 pages with tokens have finite scales.
  * n_head a multiple of n_kv, at most 16384 sequences and 2^31 rows (max_new or tokens, times n_head / n_kv; fewer where that
  * quotient is no power of two), else NEKO_ERR_UNSUPPORTED. out rows have type `type` and strides
  * o_token, o_head. */

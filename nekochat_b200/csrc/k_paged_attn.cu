@@ -160,10 +160,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
-    // Weights are 2^(score - maximum + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with hi + lo, is 2^-32 of the
+    // Weights are 2^(score - maximum + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with hi + lo, is 2^-36 of the
     // largest weight; the maximum lags by 2^kLazy at most. 8-bit values' scales are outside the products (times 2^-15, which
     // the sum of the weights takes too: an accumulator is no larger than the values).
-    constexpr float kLazy = 8.0f, kLift = 7.0f;
+    constexpr float kLazy = 4.0f, kLift = 11.0f;
     constexpr float kUnit = Q8 ? 1.0f / 32768.0f : 1.0f;
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;

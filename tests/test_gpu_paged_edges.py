@@ -432,3 +432,18 @@ def test_rows_that_see_nothing_beside_rows_that_do(torch, new, L, page_gone, e4m
     got, want = held_to(torch, cache, [L], [new], 4, dtype, 109)
     none = (want == 0).all(-1)
     assert none.any() and (got[none] == 0).all()
+
+
+@pytest.mark.parametrize("new,heads,n_kv", [(1, 2, 1), (40, 2, 2)])
+def test_many_small_weights_count(torch, new, heads, n_kv):
+    """40,000 keys whose weights are 2^-29 of one key's: together 7.5e-5 of the result, which is within 2.5e-5 of the
+    definition's."""
+    L = 40000
+    rng = np.random.default_rng(103)
+    cache = Cache(torch, rng, [L], n_kv, 64, 128, False)
+    k, v = torch.zeros(cache.k.shape, device="cuda"), torch.ones(cache.k.shape, device="cuda")
+    k[int(cache.table[0, 0]), :, 0, 0] = 1.0
+    quantize(torch, cache, k, v)
+    q = torch.zeros((new, heads, 128), device="cuda")
+    q[..., 0] = 29 * np.log(2.0)
+    held_to(torch, cache, [L], [new], heads, "float32", 104, q=q, scale=1.0)

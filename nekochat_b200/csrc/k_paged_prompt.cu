@@ -59,7 +59,8 @@ constexpr float kLift = 15.0f - kLazy;
 // An UMMA's f32 accumulation truncates: each step takes a share off the sum, 3.2e-8 on average (measured on sums of 2,500
 // steps, whose common factor was 1 - 2.1e-5; half a unit in the last of 24 places is 4.3e-8 of a mantissa spread evenly over
 // the logarithm). What O held before a step loses as a whole, so the sum of the weights, which is rounded to nearest, is made
-// to lose as much and the quotient does not keep it. What is left differs from value to value, about 6e-9 a step: for f32
+// to lose as much and the quotient does not keep it - but no more than a key tile adds, since a step that adds nothing truncates
+// nothing (one key with all the weight, 262,144 keys: 5e-4 too large otherwise). What is left differs from value to value, about 6e-9 a step: for f32
 // queries O leaves TMEM every kFlush key tiles for sums that are rounded to nearest (20,000 keys: an error of 1.3e-6 every 8
 // tiles, 2.4e-6 every 16; ragged prompts on 3,000 keys: 669 and 646 us).
 constexpr float kDrop = 3.2e-8f;
@@ -885,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 }
             }
             constexpr float kSteps = kKeys / 16 * L::kParts;
-            row_sum = fmaf(row_sum, -kSteps * kDrop, row_sum) + fmaf(sum, -(kSteps + 1) / 2 * kDrop, sum);
+            row_sum = row_sum - fminf(kSteps * kDrop * row_sum, sum) + fmaf(sum, -(kSteps + 1) / 2 * kDrop, sum);
             st_wait();
             tc_fence_before();
             mbar_arrive(&ms.p_full[h]);

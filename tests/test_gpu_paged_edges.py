@@ -447,3 +447,23 @@ def test_many_small_weights_count(torch, new, heads, n_kv):
     q = torch.zeros((new, heads, 128), device="cuda")
     q[..., 0] = 29 * np.log(2.0)
     held_to(torch, cache, [L], [new], heads, "float32", 104, q=q, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,L,hd,near", [("float32", 16384, 128, 1.5e-6), ("float32", 1100, 64, 1.5e-6), ("float16", 262144, 64, 0.0)])
+def test_a_first_key_that_takes_all_weight(torch, dtype, L, hd, near):
+    """The result is that key's value however many keys of no weight follow: for f32 within the two roundings of a weight's
+    f16 halves, of the sum and of the quotient (together 1.5e-6), for f16, which that error does not reach, exactly."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(105)
+    n = 64
+    cache = Cache(torch, rng, [L], 1, 128, hd, False)
+    g = torch.Generator("cuda").manual_seed(106)
+    k, v = torch.zeros(cache.k.shape, device="cuda"), torch.randn(cache.k.shape, device="cuda", generator=g)
+    first = int(cache.table[0, 0])
+    k[first, :, 0, 0] = 8.0
+    quantize(torch, cache, k, v)
+    q = torch.zeros((n, 2, hd), device="cuda", dtype=getattr(torch, dtype))
+    q[..., 0] = 16.0  # the others' weights are e^-128 of the first's
+    got = ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, L), q_start=ints(torch, 0, n), max_new=n, scale=1.0)
+    want = cache.v[first, 0, 0].double().expand(n, 2, hd)
+    assert ((got.double() - want).abs() <= near * want.abs()).all(), ((got.double() - want) / want).abs().max()

@@ -65,7 +65,6 @@ constexpr float kLift = 15.0f - kLazy;
 // tiles, 2.4e-6 every 16; ragged prompts on 3,000 keys: 669 and 646 us).
 constexpr float kDrop = 3.2e-8f;
 constexpr int kFlush = 8;
-constexpr int64_t kFlushBytes = int64_t(1) << 30;  // sums of more CTAs stay in TMEM (batches padded to their longest prompt can be large)
 constexpr float kVMin = -60.0f; // the product of a row's likeliest key with a block's scale counts as no less than 2^-60 of the reference
 constexpr float kVNone = -126.0f;
 constexpr float kGone = -1.0f;
@@ -79,7 +78,9 @@ struct PromptPlan {
     int tiles_per;  // row tiles of a CTA: 1 or 2
     int group;      // query heads per KV head
     uint64_t group_inv;  // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
-    float* flush;        // [CTA][HD][256 rows]: sums that have left TMEM (f32 queries; NULL: none do)
+    float* flush;        // [slot][HD][256 rows]: sums that have left TMEM (f32 queries; NULL: none do)
+    uint32_t* taken;     // [slot]: 1 while a CTA has it
+    int slots;           // as many as CTAs run at once
 };
 
 template <int HD, bool HILO>
@@ -103,6 +104,7 @@ struct PL {
 struct Misc {
     uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done[2], drain, land, scanned, q_full;
     uint32_t tmem, fail;
+    int slot;                          // of plan.flush; -1: none
     float ks[kRing][8];                // scales of a key tile's blocks of 16 keys; kGone: not resident
     float vs[kRing][8];                // log2 of theirs of the values
     uint32_t whole[kRing];             // every block is resident
@@ -292,6 +294,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         ms.fail = 0;
         for (int i = 0; i < 8; i++) ms.odd[i / 4][i % 4] = 0;  // tiles 0 and 1
         fence_barrier_init();
+    }
+    if constexpr (HILO) {
+        // There is a free slot for every CTA that runs; the search is bounded all the same. It begins at the SM's number, where the
+        // SM's CTA before this one had its slot (from the block's number on it took 90 us of 770 in all).
+        if (tid == 32 * kLoadWarp) {
+            int slot = -1;
+            unsigned sm_id;
+            asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
+            if (plan.flush && nt > kFlush)
+                for (int x = 0; x < 2 * plan.slots && slot < 0; x++) {
+                    const int y = int((sm_id + unsigned(x)) % unsigned(plan.slots));
+                    if (atomicCAS(&plan.taken[y], 0u, 1u) == 0u) slot = y;
+                }
+            ms.slot = slot;
+        }
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(512u)
@@ -666,12 +683,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             __syncwarp();
             tc_fence_after();
             if constexpr (HILO) {
-                if (i > 0 && i % kFlush == 0 && plan.flush) {
+                if (i > 0 && i % kFlush == 0 && ms.slot >= 0) {
                     wait_on(&ms.pv_done[h], (i - 1) & 1, fail);
                     __syncwarp();
                     tc_fence_after();
                     const bool again = kept != nullptr;
-                    kept = plan.flush + (int64_t(blockIdx.x) * HD + col_w * (HD / 2)) * (2 * kRows) + r;
+                    kept = plan.flush + (int64_t(ms.slot) * HD + col_w * (HD / 2)) * (2 * kRows) + r;
                     const float now = row_max == -INFINITY ? 0.0f : row_max, f = ex2(fminf(kept_ref - now, 0.0f));
                     kept_ref = now;
                     sum_kept += row_sum;
@@ -952,6 +969,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     tc_fence_before();
     if (alone) __syncthreads();
     else cluster.sync();
+    if (HILO && tid == 32 * kLoadWarp && ms.slot >= 0) {  // every thread has read its sums
+        __threadfence();
+        atomicExch(&plan.taken[ms.slot], 0u);
+    }
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     auto put = [&](int r, int d, float4 v) {
         const int pr = r0 + r;
@@ -1134,12 +1155,18 @@ cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
     const int64_t items = split<HD>(p, (rows + kRows - 1) / kRows, int64_t(c.n_seq) * c.n_kv, key_tiles, a.type == NEKO_T_F32);
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    p.flush = nullptr;
+    p.flush = nullptr, p.taken = nullptr;
+    p.slots = int(std::min<int64_t>(items * p.ranks, num_sms()));
     void* flush = nullptr;
-    const int64_t flush_bytes = items * p.ranks * 2 * kRows * HD * 4;
-    if (a.type == NEKO_T_F32 && key_tiles > int64_t(p.ranks) * kFlush && flush_bytes <= kFlushBytes) {
-        if (cudaError_t e = scratch_alloc(&flush, size_t(flush_bytes), st); e != cudaSuccess) return e;
+    if (a.type == NEKO_T_F32 && key_tiles > int64_t(p.ranks) * kFlush) {
+        const size_t bytes = size_t(p.slots) * 2 * kRows * HD * 4;  // at most 19 MB
+        if (cudaError_t e = scratch_alloc(&flush, bytes + size_t(p.slots) * 4, st); e != cudaSuccess) return e;
         p.flush = static_cast<float*>(flush);
+        p.taken = reinterpret_cast<uint32_t*>(static_cast<char*>(flush) + bytes);
+        if (cudaError_t e = cudaMemsetAsync(p.taken, 0, size_t(p.slots) * 4, st); e != cudaSuccess) {
+            cudaFreeAsync(flush, st);
+            return e;
+        }
     }
     const cudaError_t e = by_pages<HD>(a, p, items, st);
     if (flush) cudaFreeAsync(flush, st);

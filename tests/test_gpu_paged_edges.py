@@ -467,3 +467,27 @@ def test_a_first_key_that_takes_all_weight(torch, dtype, L, hd, near):
     got = ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, L), q_start=ints(torch, 0, n), max_new=n, scale=1.0)
     want = cache.v[first, 0, 0].double().expand(n, 2, hd)
     assert ((got.double() - want).abs() <= near * want.abs()).all(), ((got.double() - want) / want).abs().max()
+
+
+def test_f32_precision_of_more_prompts_than_run_at_once(torch):
+    """8,800 row tiles of 16,384 keys (one sequence's pages, shared): sums kept outside the tensor cores for those that run, at
+    most 64 MiB in all, and the error of every row as small as for few (2-norm, 3e-6)."""
+    from nekochat_b200 import ops
+    n_seq, n, L, n_kv, ps = 1100, 32, 16384, 8, 128
+    g = torch.Generator("cuda").manual_seed(125)
+    k, v = (torch.randn((L // ps, n_kv, ps, 128), device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn((n_seq * n, n_kv, 128), device="cuda", generator=g)
+    table = torch.randperm(L // ps, device="cuda", generator=g).int().repeat(n_seq, 1)
+    out = torch.empty_like(q)
+    before = free(torch)
+    ops.paged_attention(q, k, v, table, torch.full((n_seq,), L, dtype=torch.int32, device="cuda"),
+                        q_start=torch.arange(0, n_seq * n + 1, n, dtype=torch.int32, device="cuda"), max_new=n, out=out)
+    ops.status()
+    assert before - free(torch) <= 64 << 20
+    see = torch.arange(L, device="cuda")[None] <= (L - n + torch.arange(n, device="cuda"))[:, None]
+    for h in (0, 5):
+        kk, vv = (x[table[0].long(), h].reshape(L, 128).double() for x in (k, v))
+        for s in (0, 1, 147, 148, 600, n_seq - 1):
+            rows = slice(s * n, s * n + n)
+            want = torch.softmax(torch.where(see, q[rows, h].double() @ kk.T * 128 ** -0.5, -torch.inf), -1) @ vv
+            assert (out[rows, h] - want).norm() <= 3e-6 * want.norm()

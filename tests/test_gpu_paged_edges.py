@@ -491,3 +491,40 @@ def test_f32_precision_of_more_prompts_than_run_at_once(torch):
             rows = slice(s * n, s * n + n)
             want = torch.softmax(torch.where(see, q[rows, h].double() @ kk.T * 128 ** -0.5, -torch.inf), -1) @ vv
             assert (out[rows, h] - want).norm() <= 3e-6 * want.norm()
+
+
+@pytest.mark.parametrize("new,lens", [([1] * 3, [700, 3000, 65]), ([300, 5], [2000, 900])])
+def test_calls_in_a_graph(torch, new, lens):
+    """Append and attention captured once and replayed on other inputs: the bits of the calls themselves."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(118)
+    cache, other = (Cache(torch, np.random.default_rng(119), lens, 2, 64, 128, True, width=80) for _ in range(2))
+    g = torch.Generator("cuda").manual_seed(120)
+    for c in (cache, other):
+        g.manual_seed(121)
+        quantize(torch, c, *(torch.randn(c.k.shape, device="cuda", generator=g) for _ in range(2)))
+    T = sum(new)
+    q, k, v = fresh_rows(torch, rng, T, 8, 2, 128, torch.float32)
+    cs = ops.rope_table(4000, 128, 1e6)
+    at, n, qs, table = ints(torch, *[a - b for a, b in zip(lens, new)]), ints(torch, *lens), ints(torch, *starts(new).tolist()), torch.from_numpy(cache.table).cuda()
+
+    def both(c):
+        turned = ops.paged_append(k, v, c.k, c.v, table, at, k_scale=c.ks, v_scale=c.vs, q_start=qs, max_new=max(new), q=q, cs=cs)
+        return ops.paged_attention(turned, c.k, c.v, table, n, k_scale=c.ks, v_scale=c.vs, q_start=qs, max_new=max(new))
+
+    both(other)
+    for x, y in ((other.k, cache.k), (other.v, cache.v), (other.ks, cache.ks), (other.vs, cache.vs)):
+        x.copy_(y)  # scales and codes go by what a page has held
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = both(cache)
+    for turn in range(3):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device="cuda", generator=g))
+        graph.replay()
+        want = both(other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(cache.k, other.k) and torch.equal(cache.vs, other.vs)
+    ops.status()

@@ -36,10 +36,10 @@ __device__ __forceinline__ float finite_abs(float x) {
     const float m = fabsf(x);
     return m <= 3.402823466e38f ? m : 0.0f;
 }
-// The power of two that brings a row's largest magnitude to [1, 2).
+// The power of two that brings a row's largest magnitude to [1, 2), or to [2, 4) where that power would be subnormal.
 __device__ __forceinline__ float row_up(float most) {
     const int ex = most > 0.0f ? max(int(__float_as_uint(most) >> 23) - 127, -126) : 0;
-    return __uint_as_float(uint32_t(min(127 - ex, 253)) << 23);
+    return __uint_as_float(uint32_t(min(max(127 - ex, 1), 253)) << 23);
 }
 
 // Two f32 operations in one instruction.

@@ -528,3 +528,17 @@ def test_calls_in_a_graph(torch, new, lens):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(cache.k, other.k) and torch.equal(cache.vs, other.vs)
     ops.status()
+
+
+@pytest.mark.parametrize("new,L", [(1, 50), (700, 800)])
+@pytest.mark.parametrize("size,scale", [(2.0 ** 125, 2.0 ** -125), (2.0 ** -135, 2.0 ** 125)])
+def test_queries_at_the_ends_of_f32(torch, size, scale, new, L):
+    """Rows whose largest magnitude is above 2^127 or subnormal, brought back by the scale."""
+    rng = np.random.default_rng(126)
+    cache = Cache(torch, rng, [L], 2, 16, 128, False)
+    g = torch.Generator("cuda").manual_seed(127)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+    quantize(torch, cache, k * 0.05, v)
+    q = torch.randn((new, 4, 128), device="cuda", generator=g).clamp(-7, 7)
+    q[..., 3] = 7.5
+    held_to(torch, cache, [L], [new], 4, "float32", 128, q=(q.double() * size).float(), scale=scale)

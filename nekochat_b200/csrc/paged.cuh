@@ -9,7 +9,6 @@
 namespace neko {
 
 enum PagedType : int { kTF32 = NEKO_T_F32, kTF16 = NEKO_T_F16, kTBF16 = NEKO_T_BF16, kTE4M3 = NEKO_T_E4M3 };
-constexpr float kE4m3Max = 448.0f;
 constexpr int kScaleMinExp = -100;  // scale of a block of zeros: 2^-100
 
 cudaError_t launch_paged_append(const neko_paged_append_args& a, cudaStream_t st);

@@ -8,15 +8,12 @@
 
 namespace neko {
 
-// A [rows] x [cols] f16 matrix (row stride row_stride_bytes) read in boxes of box_rows x box_cols elements with
-// the 128-byte swizzle (box_cols * 2 <= 128); elements past the matrix read as zeros. False when the driver entry
-// point is unavailable or the map is invalid (alignment, strides).
-inline bool encode_f16_2d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
-                                uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows) {
-    using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Fn fn = []() -> Fn {
+using TensorMapEncoder = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                     const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                     CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// The driver's encoder, resolved once; NULL where there is none.
+inline TensorMapEncoder tensor_map_encoder() {
+    static const TensorMapEncoder fn = []() -> TensorMapEncoder {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q{};
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
@@ -24,8 +21,17 @@ inline bool encode_f16_2d_sw128(CUtensorMap* map, const void* base, uint64_t col
             cudaGetLastError();
             return nullptr;
         }
-        return reinterpret_cast<Fn>(p);
+        return reinterpret_cast<TensorMapEncoder>(p);
     }();
+    return fn;
+}
+
+// A [rows] x [cols] f16 matrix (row stride row_stride_bytes) read in boxes of box_rows x box_cols elements with
+// the 128-byte swizzle (box_cols * 2 <= 128); elements past the matrix read as zeros. False when the driver entry
+// point is unavailable or the map is invalid (alignment, strides).
+inline bool encode_f16_2d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
+                                uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows) {
+    const TensorMapEncoder fn = tensor_map_encoder();
     if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || row_stride_bytes % 16 || box_cols * 2 > 128) return false;
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {row_stride_bytes};
@@ -41,19 +47,7 @@ inline bool encode_f16_2d_sw128(CUtensorMap* map, const void* base, uint64_t col
 // row r lands at chunk c ^ (r % 8)); bytes past the matrix read as zeros. box_cols a multiple of 16.
 inline bool encode_u8_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
                          uint32_t box_cols, uint32_t box_rows, bool swizzle128 = false) {
-    using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Fn fn = []() -> Fn {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            return nullptr;
-        }
-        return reinterpret_cast<Fn>(p);
-    }();
+    const TensorMapEncoder fn = tensor_map_encoder();
     if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || row_stride_bytes % 16 || box_cols % 16 || box_cols > 256 ||
         box_rows > 256 || (swizzle128 && box_cols > 128))
         return false;
@@ -70,19 +64,7 @@ inline bool encode_u8_2d(CUtensorMap* map, const void* base, uint64_t cols, uint
 // columns of one page, with the 128-byte swizzle. False as encode_f16_2d_sw128.
 inline bool encode_f16_pages(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pages,
                              uint64_t page_bytes, uint32_t box_rows) {
-    using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                            const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Fn fn = []() -> Fn {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            return nullptr;
-        }
-        return reinterpret_cast<Fn>(p);
-    }();
+    const TensorMapEncoder fn = tensor_map_encoder();
     if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || page_bytes % 16 || box_rows > 256) return false;
     const cuuint64_t dims[3] = {cols, rows, pages};
     const cuuint64_t strides[2] = {cols * 2, page_bytes};

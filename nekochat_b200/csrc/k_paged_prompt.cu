@@ -853,15 +853,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             meet();
             top = max_nan(top, ms.most[col_w ^ 1][r]);
             if (!(top < INFINITY)) row_sum = NAN;  // as exp(inf - inf) and exp(NaN) give, whatever computes the weights
-            // The reference moves only when a score exceeds it by more than 2^kLazy (the same decision in both warps of a row). Units are
-            // whole powers of two, as the append's scales are: what goes from one to another is exact.
+            // The reference moves only when a score exceeds it by more than 2^kLazy (the same decision in both warps of a row), and then to
+            // that score itself: its weight, often most of the row, is a power of two and f16 takes nothing off it (whole
+            // powers of two as references: f16 rows' error 2.9e-4 instead of 2.6e-4).
             const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
             if (__any_sync(0xffffffffu, up)) {
                 float f = 1.0f;
                 if (up) {
-                    const float next = ceilf(top);
-                    f = ex2(row_max - next);  // row_max = -inf: nothing there yet, 0
-                    row_max = next;
+                    f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
+                    row_max = top;
                     if (!kScaled) row_sum *= f;
                     if (!kScaled && HILO) sum_kept *= f;
                 }

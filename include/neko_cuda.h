@@ -262,6 +262,11 @@ int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream)
  * has happened on the current device since the last call of this function, whatever the stream; NEKO_OK when it has not. Not
  * while the stream is being captured. A neko_model's steps and a neko_ctx neither see these errors nor clear them. */
 int neko_op_status(void* stream);
+/* The single operators (neko_op_*) take stream-ordered scratch memory from a pool of the library's, which keeps what it has grown
+ * to: prompts over long E4M3 caches as f16 copies of the pages (up to 2 GiB), f32 rows over more than 1,024 keys up to 19 MB,
+ * decode steps over shared keys up to 80 MB. Gives what is not in use on the current device beyond keep_bytes back to the system
+ * (memory whose last use has been synchronised with). */
+int neko_op_trim(size_t keep_bytes);
 
 /* ------------------------------------------------------------------ 3. native model runner */
 

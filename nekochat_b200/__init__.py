@@ -99,6 +99,7 @@ _SIGS = {
     "neko_op_paged_append": (C.c_int, [_vp, _vp]),
     "neko_op_paged_attention": (C.c_int, [_vp, _vp]),
     "neko_op_status": (C.c_int, [_vp]),
+    "neko_op_trim": (C.c_int, [C.c_size_t]),
     "neko_model_create": (_vp, [C.c_int, C.POINTER(ModelConfig), C.c_char_p, C.c_size_t]),
     "neko_model_destroy": (None, [_vp]),
     "neko_model_last_error": (C.c_char_p, [_vp]),

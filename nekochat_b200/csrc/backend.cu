@@ -60,29 +60,37 @@ int num_sms() {
 // Stream-ordered scratch for operators called outside a model comes from the library's own memory pool on the
 // current device: it keeps what it has grown to (release threshold at its maximum), so after the first calls an
 // allocation maps no memory, and the default pool's settings stay the caller's.
-cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st) {
+static cudaError_t scratch_pool(cudaMemPool_t* pool, bool create) {
     static std::mutex mu;
     static cudaMemPool_t pools[64] = {};
+    *pool = nullptr;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaMallocAsync(p, bytes, st);
-    cudaMemPool_t pool;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (!pools[dev]) {
-            cudaMemPoolProps props = {};
-            props.allocType = cudaMemAllocationTypePinned;
-            props.handleTypes = cudaMemHandleTypeNone;
-            props.location.type = cudaMemLocationTypeDevice;
-            props.location.id = dev;
-            if ((e = cudaMemPoolCreate(&pools[dev], &props)) != cudaSuccess) return e;
-            uint64_t keep = UINT64_MAX;
-            cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
-        }
-        pool = pools[dev];
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!pools[dev] && create) {
+        cudaMemPoolProps props = {};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.handleTypes = cudaMemHandleTypeNone;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = dev;
+        if ((e = cudaMemPoolCreate(&pools[dev], &props)) != cudaSuccess) return e;
+        uint64_t keep = UINT64_MAX;
+        cudaMemPoolSetAttribute(pools[dev], cudaMemPoolAttrReleaseThreshold, &keep);
     }
-    return cudaMallocFromPoolAsync(p, bytes, pool, st);
+    *pool = pools[dev];
+    return cudaSuccess;
+}
+cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st) {
+    cudaMemPool_t pool;
+    const cudaError_t e = scratch_pool(&pool, true);
+    if (e != cudaSuccess) return e;
+    return pool ? cudaMallocFromPoolAsync(p, bytes, pool, st) : cudaMallocAsync(p, bytes, st);
+}
+cudaError_t scratch_trim(size_t keep) {
+    cudaMemPool_t pool;
+    const cudaError_t e = scratch_pool(&pool, false);
+    return e == cudaSuccess && pool ? cudaMemPoolTrimTo(pool, keep) : e;
 }
 
 namespace {

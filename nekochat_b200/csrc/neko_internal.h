@@ -45,6 +45,7 @@ inline cudaError_t ensure_dyn_smem(F* fn, size_t bytes) { return ensure_dyn_smem
 
 // Stream-ordered scratch from the library's own pool of the current device (backend.cu); freed with cudaFreeAsync.
 cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st);
+cudaError_t scratch_trim(size_t keep);  // gives back what is not in use beyond `keep` bytes
 
 // ------------------------------------------------------------------ weight codec (k_quant.cu)
 cudaError_t launch_quantize(int fmt, const float* w, int rows, int cols, int64_t ld, int transpose, uint8_t* out,

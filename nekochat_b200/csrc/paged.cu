@@ -119,3 +119,5 @@ extern "C" int neko_op_status(void* stream) {
                       : code == kErrMbarTimeout ? "a bounded wait of a paged kernel gave up; its output is not valid"
                                                 : "a paged kernel found its shared memory misaligned and did nothing");
 }
+
+extern "C" int neko_op_trim(size_t keep_bytes) { return finish("op_trim", scratch_trim(keep_bytes)); }

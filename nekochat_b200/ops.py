@@ -323,3 +323,9 @@ def status():
     """neko_op_status: waits for the current stream and raises when a paged_append or paged_attention since the last call
     had a sequence with more new tokens than max_new, rows that are not there, or positions past the rotation table."""
     check(lib().neko_op_status(_stream()), "paged operators")
+
+
+def trim(keep_bytes=0):
+    """neko_op_trim: gives the operators' idle scratch memory on the current device back, beyond keep_bytes. Work that used it
+    has to be synchronised with."""
+    check(lib().neko_op_trim(keep_bytes), "trim")

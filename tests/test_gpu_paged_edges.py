@@ -542,3 +542,27 @@ def test_queries_at_the_ends_of_f32(torch, size, scale, new, L):
     q = torch.randn((new, 4, 128), device="cuda", generator=g).clamp(-7, 7)
     q[..., 3] = 7.5
     held_to(torch, cache, [L], [new], 4, "float32", 128, q=(q.double() * size).float(), scale=scale)
+
+
+def test_scratch_memory_is_given_back_when_asked(torch):
+    """f16 copies of a long 8-bit cache's pages (491 MB) stay with the library until trim; calls after it work as before."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(129)
+    lens, new = [120000], [300]
+    cache = Cache(torch, rng, lens, 8, 128, 128, True)
+    g = torch.Generator("cuda").manual_seed(130)
+    cache.k.copy_(torch.randint(0, 100, cache.k.shape, device="cuda", generator=g, dtype=torch.uint8))
+    cache.v.copy_(cache.k)
+    cache.ks.fill_(0.01), cache.vs.fill_(0.01)
+    q = torch.randn((300, 16, 128), device="cuda", generator=g)
+    call = lambda: ops.paged_attention(q, cache.k, cache.v, torch.from_numpy(cache.table).cuda(), ints(torch, *lens), k_scale=cache.ks,  # noqa: E731
+                                       v_scale=cache.vs, q_start=ints(torch, 0, 300), max_new=300, out=out)
+    out = torch.empty_like(q)
+    ops.trim()
+    call()
+    held, first = free(torch), out.clone()
+    ops.trim()
+    assert free(torch) - held >= 450 << 20
+    call()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)

@@ -264,7 +264,7 @@ int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream)
 int neko_op_status(void* stream);
 /* The single operators (neko_op_*) take stream-ordered scratch memory from a pool of the library's, which keeps what it has grown
  * to: prompts over long E4M3 caches as f16 copies of the pages (up to 2 GiB), f32 rows over more than 1,024 keys up to 19 MB,
- * decode steps over shared keys up to 80 MB. Gives what is not in use on the current device beyond keep_bytes back to the system
+ * decode steps over shared keys up to 40 MB. Gives what is not in use on the current device beyond keep_bytes back to the system
  * (memory whose last use has been synchronised with). */
 int neko_op_trim(size_t keep_bytes);
 

@@ -801,7 +801,7 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     const int64_t row_tiles = (int64_t(a.max_new) * p.group + TL::kRows - 1) / TL::kRows;
     // as many CTAs for each row tile as the GPU holds at a time, or a group of 16 keys for each warp where the cache has room for
     // fewer. Prompts on heads of 32 have thousands of row tiles: no more than 16 times what the GPU holds in all, which bounds the
-    // parts (80 MB, two states a CTA), and none where that is one CTA each.
+    // parts (40 MB, two states a CTA), and none where that is one CTA each.
     const int64_t groups = int64_t(c.max_pages) * c.page_size / 16 * c.n_kv * c.n_seq;
     const int64_t items = int64_t(c.n_kv) * c.n_seq;
     const int64_t per_item = int64_t(c.max_pages) * c.page_size / 16, room = int64_t(num_sms()) * kCtas<HD, Q8, NT>;

@@ -10,8 +10,9 @@
 // its 8 columns. The order of the summed index is free as long as both operands agree, so the fragments come straight
 // from global memory: lane (g, t) holds, for K, 16-byte pieces t, t + 4, .. of key rows g and g + 8, and for V the
 // pieces g, g + 8, .. of key rows 2t, 2t + 1, 2t + 8, 2t + 9; neither K nor V passes through shared memory. 8-bit codes
-// become f16 in registers (exact), keys' scales multiply the scores, values' scales the products of 16 keys on their way to
-// the accumulators. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
+// become f16 in registers (exact), keys' scales multiply the scores, values' scales enter the weights' exponent: a row's
+// reference is the largest score plus log2 of the value scale that it sees, and the sum of its weights has the largest score
+// as a unit of its own, so what f16 rounds off a weight is small beside the largest of the row's products. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
 // 16-bit queries one exact f16 column, weights one f16. Rows are scaled by a power of two into f16's range first.
 // All groups of all items, in order, are dealt out in equal shares to the warps that the GPU holds at a time, whatever
@@ -87,7 +88,7 @@ struct DecodePlan {
     uint64_t group_inv;   // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
     uint32_t page_16;     // page stride in 16-byte units
     int page_log;
-    float* part;          // [row tile][2 * CTAs][rows][HD + 4]: values, maximum, sum (NULL where a row tile has one CTA)
+    float* part;          // [row tile][2 * CTAs][rows][HD + 4]: rows' states (NULL where a row tile has one CTA)
     int4* desc;           // [row tile][CTAs]: an item that starts in the CTA and ends in a later one
     int tile0;            // first row tile of the launch
     int ranks_log;        // of the clusters of the small variant
@@ -99,7 +100,7 @@ struct Tile {
     static constexpr int kRowsPer = HILO ? 4 : 8;
     static constexpr int kRows = NT * kRowsPer;
     static constexpr int kLaneRows = HILO ? 1 : 2;  // rows per lane and column tile
-    static constexpr int kPitch = HD + 4;           // floats of a row's state: values, maximum, sum
+    static constexpr int kPitch = HD + 4;           // floats of a row's state: values, log2 of their unit, sum, log2 of its unit
     static constexpr int kState = kRows * kPitch;
     // dynamic shared memory: the warps' two states, what they are, warp totals, groups before each sequence
     static constexpr int kMetaOff = 2 * kWarps * kState * 4;
@@ -140,13 +141,21 @@ __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, cons
     return v;
 }
 
-// v / sum to four values of a packed row of the output.
+// log2 of a code's value where the scale is x: exact for powers of two, which the append writes.
+__device__ __forceinline__ float log2_scale(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return fmaxf((b & 0x7fffffu) == 0 ? float(int(b >> 23) - 127) : log2f(x), -126.0f);
+}
+// What turns values in units of 2^top over a sum in units of 2^top_sum into the quotient (nothing seen: there are no values).
+__device__ __forceinline__ float over_sum(float top, float sum, float top_sum) {
+    return sum == 0.0f ? 0.0f : (top > -INFINITY ? exp2f(top - top_sum) : 1.0f) / sum;
+}
+// v * f to four values of a packed row of the output.
 template <bool HILO>
 __device__ __forceinline__ void put_row(const neko_paged_attention_args& a, const DecodePlan& plan, int row0, int kvh, int pr, int d,
-                                        float4 v, float sum) {
+                                        float4 v, float f) {
     const int rt = int(uint64_t(uint32_t(pr)) * plan.group_inv >> 32);
     const int64_t off = int64_t(row0 + rt) * a.o_token + int64_t(kvh * plan.group + pr - rt * plan.group) * a.o_head + d;
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     const float x[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
     auto store = [&](auto* p) { store_row<4>(p, (reinterpret_cast<uintptr_t>(p) & (sizeof(*p) * 4 - 1)) == 0, x); };
     if constexpr (HILO) store(static_cast<float*>(a.out) + off);
@@ -160,11 +169,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
-    // Weights are 2^(score - maximum + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with hi + lo, is 2^-36 of the
-    // largest weight; the maximum lags by 2^kLazy at most. 8-bit values' scales are outside the products (times 2^-15, which
-    // the sum of the weights takes too: an accumulator is no larger than the values).
-    constexpr float kLazy = 4.0f, kLift = 11.0f;
-    constexpr float kUnit = Q8 ? 1.0f / 32768.0f : 1.0f;
+    // Weights are 2^(score + log2 of the value scale - reference + kLift), at most 2^15. What f16 rounds off them, half of 2^-24
+    // with hi + lo, is 2^-36 of the largest; the reference lags by 2^kLazy at most. A row's likeliest key times a block's scale
+    // counts as no less than 2^kLeast of the reference.
+    constexpr float kLazy = 4.0f, kLift = 11.0f, kLeast = -60.0f;
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
@@ -350,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         }
 
         float acc[NT][kSteps][4];
-        float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];
+        float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];  // largest score and sum of the weights against it
+        float u[NT][TL::kLaneRows];                        // reference: the accumulators' unit (8-bit values; else m)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -358,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = -INFINITY, l[nt][r] = 0.0f;
+            for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = u[nt][r] = -INFINITY, l[nt][r] = 0.0f;
         }
         const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
@@ -447,8 +456,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                             else z[nt][r][h] = -INFINITY;
                         }
             }
-            // ---- running maximum (moved only by more than 2^kLazy: weights above 1 are as exact)
-            const float vs_now = vs * kUnit;
+            // ---- running maxima (moved only by more than 2^kLazy: weights above 1 are as exact)
+            const float lv = Q8 ? log2_scale(vs) : 0.0f;
             bool up = false;
             float top[NT][TL::kLaneRows];
 #pragma unroll
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     top[nt][r] = x;
-                    up |= x > m[nt][r] + kLazy;
+                    up |= x > m[nt][r] + kLazy || (Q8 && x + lv > u[nt][r] + kLazy);
                 }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -470,9 +479,14 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                     for (int r = 0; r < TL::kLaneRows; r++) {
                         f[r] = 1.0f;
                         if (top[nt][r] > m[nt][r] + kLazy) {
-                            f[r] = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
+                            const float fm = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
                             m[nt][r] = top[nt][r];
-                            l[nt][r] *= f[r];
+                            l[nt][r] *= fm;
+                            if (!Q8) f[r] = fm;
+                        }
+                        if (Q8 && top[nt][r] + lv > u[nt][r] + kLazy) {
+                            f[r] = ex2(u[nt][r] - (top[nt][r] + lv));
+                            u[nt][r] = top[nt][r] + lv;
                         }
                     }
 #pragma unroll
@@ -488,9 +502,12 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 float p[2][TL::kLaneRows];
 #pragma unroll
                 for (int r = 0; r < TL::kLaneRows; r++) {
-                    const float ref = (m[nt][r] == -INFINITY ? 0.0f : m[nt][r]) - kLift;
-                    p[0][r] = ex2(z[nt][r][0] - ref), p[1][r] = ex2(z[nt][r][1] - ref);
-                    l[nt][r] += p[0][r] + p[1][r];
+                    // 2^vr: what a weight against the reference is of what it adds to the sum
+                    const float ref = m[nt][r] == -INFINITY ? 0.0f : m[nt][r];
+                    const float vr = Q8 ? fmaxf(lv + (ref - (u[nt][r] == -INFINITY ? 0.0f : u[nt][r])), kLeast) : 0.0f;
+                    const float off = (Q8 ? vr - ref : -ref) + kLift;
+                    p[0][r] = ex2(z[nt][r][0] + off), p[1][r] = ex2(z[nt][r][1] + off);
+                    l[nt][r] = Q8 ? fmaf(p[0][r] + p[1][r], ex2(-vr), l[nt][r]) : l[nt][r] + (p[0][r] + p[1][r]);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -548,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
                                     const int r = HILO ? 0 : e & 1;
-                                    if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] = fmaf(d[e], vs_now, acc[nt][i][e]);
+                                    if (bits >> (nt * 4 + r * 2) & 1u) acc[nt][i][e] += d[e];
                                 }
                             }
                         }
@@ -565,14 +582,13 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 v_frag(i, f);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    if constexpr (HILO || Q8) {
-                        // Added outside the MMA: it truncates (on the accumulator itself every group took 3e-8 off it, an error of
-                        // 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time), and 8-bit values' scales come
-                        // in here, in f32, so that small blocks keep their bits beside large ones.
+                    if constexpr (HILO) {
+                        // added outside the MMA, which truncates: on the accumulator itself every group took 3e-8 off it
+                        // (an error of 1.6e-5 on 150 x 18,000 keys, 6.4e-7 this way in the same time; 16-bit results do not see it)
                         float d[4];
                         mma16816_z(d, f, pf[nt][0], pf[nt][1]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[nt][i][e] = Q8 ? fmaf(d[e], vs_now, acc[nt][i][e]) : acc[nt][i][e] + d[e];
+                        for (int e = 0; e < 4; e++) acc[nt][i][e] += d[e];
                     } else {
                         mma16816(acc[nt][i], f, pf[nt][0], pf[nt][1]);
                     }
@@ -594,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
                 float* st = st0 + row * TL::kPitch;
-                if (g == 0) st[HD] = m[nt][r], st[HD + 1] = sum * kUnit;
+                if (g == 0) st[HD] = Q8 ? u[nt][r] : m[nt][r], st[HD + 1] = sum, st[HD + 2] = m[nt][r];
 #pragma unroll
                 for (int i = 0; i < kSteps; i++) {
                     float2 v;
@@ -610,7 +626,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             for (int y = lane; y < rows * (HD / 4); y += 32) {
                 const int row = y / (HD / 4), d = y % (HD / 4) * 4;
                 const float* st = st0 + row * TL::kPitch;
-                put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d), st[HD + 1]);
+                put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d),
+                              over_sum(st[HD], st[HD + 1], st[HD + 2]));
             }
             __syncwarp();
         } else if (lane == 0) {
@@ -632,11 +649,11 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         const Span sp = span_of<TL::kRows>(a, plan, s, tile);
         const int ranks = 1 << plan.ranks_log, rank = blockIdx.x & (ranks - 1);
         float* mine = reinterpret_cast<float*>(smb + TL::kPreOff);
-        auto join = [&](int row, int d, int parts, auto part, float& top, float& sum) {
-            top = -INFINITY, sum = 0.0f;
+        auto join = [&](int row, int d, int parts, auto part, float& top, float& sum, float& top_sum) {
+            top = top_sum = -INFINITY, sum = 0.0f;
             for (int i = 0; i < parts; i++)
-                if (const float* st = part(i)) top = fmaxf(top, st[row * TL::kPitch + HD]);
-            const float ref = top == -INFINITY ? 0.0f : top;
+                if (const float* st = part(i)) top = fmaxf(top, st[row * TL::kPitch + HD]), top_sum = fmaxf(top_sum, st[row * TL::kPitch + HD + 2]);
+            const float ref = top == -INFINITY ? 0.0f : top, sum_ref = top_sum == -INFINITY ? 0.0f : top_sum;
             float4 v = make_float4(0, 0, 0, 0);
             for (int i = 0; i < parts; i++) {
                 const float* st = part(i);
@@ -644,29 +661,29 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 st += row * TL::kPitch;
                 const float f = ex2(st[HD] - ref);
                 const float4 o = *reinterpret_cast<const float4*>(st + d);
-                sum = fmaf(f, st[HD + 1], sum);
+                sum = fmaf(ex2(st[HD + 2] - sum_ref), st[HD + 1], sum);
                 v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
             }
             return v;
         };
         for (int y = tid; y < sp.rows * (HD / 4); y += kThreads) {
             const int row = y / (HD / 4), d = y % (HD / 4) * 4;
-            float top, sum;
-            const float4 v = join(row, d, 2 * kWarps, [&](int i) { return meta[i].x >= 0 ? sm + i * TL::kState : nullptr; }, top, sum);
+            float top, sum, top_sum;
+            const float4 v = join(row, d, 2 * kWarps, [&](int i) { return meta[i].x >= 0 ? sm + i * TL::kState : nullptr; }, top, sum, top_sum);
             if (ranks == 1) {
-                put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, sum);
+                put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
             } else {
                 *reinterpret_cast<float4*>(mine + row * TL::kPitch + d) = v;
-                if (d == 0) mine[row * TL::kPitch + HD] = top, mine[row * TL::kPitch + HD + 1] = sum;
+                if (d == 0) mine[row * TL::kPitch + HD] = top, mine[row * TL::kPitch + HD + 1] = sum, mine[row * TL::kPitch + HD + 2] = top_sum;
             }
         }
         if (ranks == 1) return;
         cluster.sync();
         for (int y = rank * kThreads + tid; y < sp.rows * (HD / 4); y += kThreads * ranks) {
             const int row = y / (HD / 4), d = y % (HD / 4) * 4;
-            float top, sum;
-            const float4 v = join(row, d, ranks, [&](int i) -> const float* { return cluster.map_shared_rank(mine, i); }, top, sum);
-            put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, sum);
+            float top, sum, top_sum;
+            const float4 v = join(row, d, ranks, [&](int i) -> const float* { return cluster.map_shared_rank(mine, i); }, top, sum, top_sum);
+            put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
         }
         cluster.sync();  // no CTA leaves while another reads its part
         return;
@@ -695,34 +712,35 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             const int y = y0 + lane;
             if (turn++ % kWarps != warp || y >= rows * (HD / 4)) continue;
             const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
-            float top = -INFINITY, sum = 0.0f;
+            float top = -INFINITY, top_sum = -INFINITY, sum = 0.0f;
             float4 v = make_float4(0, 0, 0, 0);
             for (uint32_t w = in; w;) {  // four parts at a time
-                float mw[4], lw[4];
+                float uw[4], lw[4], mw[4];
                 float4 o[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float* st = sm + (w ? __ffs(w) - 1 : b) * TL::kState + at;
-                    mw[i] = w ? st[HD] : -INFINITY, lw[i] = st[HD + 1];
+                    uw[i] = w ? st[HD] : -INFINITY, lw[i] = st[HD + 1], mw[i] = w ? st[HD + 2] : -INFINITY;
                     o[i] = *reinterpret_cast<const float4*>(st + d);
                     w &= w - 1;
                 }
-                const float now = fmaxf(top, fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3])));
-                const float ref = now == -INFINITY ? 0.0f : now, was = ex2(top - ref);
-                top = now;
-                sum *= was, v.x *= was, v.y *= was, v.z *= was, v.w *= was;
+                const float now = fmaxf(top, fmaxf(fmaxf(uw[0], uw[1]), fmaxf(uw[2], uw[3])));
+                const float now_sum = fmaxf(top_sum, fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3])));
+                const float ref = now == -INFINITY ? 0.0f : now, sum_ref = now_sum == -INFINITY ? 0.0f : now_sum, was = ex2(top - ref);
+                sum *= ex2(top_sum - sum_ref), v.x *= was, v.y *= was, v.z *= was, v.w *= was;
+                top = now, top_sum = now_sum;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float f = ex2(mw[i] - ref);
-                    sum = fmaf(f, lw[i], sum);
+                    const float f = ex2(uw[i] - ref);
+                    sum = fmaf(ex2(mw[i] - sum_ref), lw[i], sum);
                     v.x = fmaf(f, o[i].x, v.x), v.y = fmaf(f, o[i].y, v.y), v.z = fmaf(f, o[i].z, v.z), v.w = fmaf(f, o[i].w, v.w);
                 }
             }
             if (flags == 3) {
-                put_row<HILO>(a, plan, row0, item_id % n_kv, tile * TL::kRows + row, d, v, sum);
+                put_row<HILO>(a, plan, row0, item_id % n_kv, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
             } else {
                 *reinterpret_cast<float4*>(part + at + d) = v;
-                if (d == 0) part[at + HD] = top, part[at + HD + 1] = sum;
+                if (d == 0) part[at + HD] = top, part[at + HD + 1] = sum, part[at + HD + 2] = top_sum;
             }
         }
     }
@@ -748,32 +766,32 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const neko_paged_attent
     const int parts = last - cta + 1;
     for (int y = threadIdx.x; y < rows * (HD / 4); y += 128) {
         const int row = y / (HD / 4), d = y % (HD / 4) * 4, at = row * TL::kPitch;
-        float top = -INFINITY, sum = 0.0f;
+        float top = -INFINITY, top_sum = -INFINITY, sum = 0.0f;
         float4 v = make_float4(0, 0, 0, 0);
         for (int i0 = 0; i0 < parts; i0 += 8) {  // eight parts' loads in flight
-            float mw[8], lw[8];
+            float uw[8], lw[8], mw[8];
             float4 o[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const bool in = i0 + i < parts;
                 const float* p = part(in ? i0 + i : 0) + at;
-                mw[i] = in ? p[HD] : -INFINITY, lw[i] = in ? p[HD + 1] : 0.0f;
+                uw[i] = in ? p[HD] : -INFINITY, lw[i] = in ? p[HD + 1] : 0.0f, mw[i] = in ? p[HD + 2] : -INFINITY;
                 o[i] = in ? *reinterpret_cast<const float4*>(p + d) : make_float4(0, 0, 0, 0);
             }
-            float now = top;
+            float now = top, now_sum = top_sum;
 #pragma unroll
-            for (int i = 0; i < 8; i++) now = fmaxf(now, mw[i]);
-            const float ref = now == -INFINITY ? 0.0f : now, old = ex2(top - ref);
-            top = now;
-            sum *= old, v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+            for (int i = 0; i < 8; i++) now = fmaxf(now, uw[i]), now_sum = fmaxf(now_sum, mw[i]);
+            const float ref = now == -INFINITY ? 0.0f : now, sum_ref = now_sum == -INFINITY ? 0.0f : now_sum, old = ex2(top - ref);
+            sum *= ex2(top_sum - sum_ref), top = now, top_sum = now_sum;
+            v.x *= old, v.y *= old, v.z *= old, v.w *= old;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float f = ex2(mw[i] - ref);
-                sum = fmaf(f, lw[i], sum);
+                const float f = ex2(uw[i] - ref);
+                sum = fmaf(ex2(mw[i] - sum_ref), lw[i], sum);
                 v.x = fmaf(f, o[i].x, v.x), v.y = fmaf(f, o[i].y, v.y), v.z = fmaf(f, o[i].z, v.z), v.w = fmaf(f, o[i].w, v.w);
             }
         }
-        put_row<HILO>(a, plan, row0, kvh, tile * TL::kRows + row, d, v, sum);
+        put_row<HILO>(a, plan, row0, kvh, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
     }
 }
 

@@ -566,3 +566,22 @@ def test_scratch_memory_is_given_back_when_asked(torch):
     call()
     torch.cuda.synchronize()
     assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_large_values_of_small_weight_count(torch, form, dtype):
+    """Blocks of values 2^45 the size of their neighbours', whose keys' weights are 2^-43 of theirs: both make up the result."""
+    new, L, heads, n_kv, hd = FORMS[form]
+    rng = np.random.default_rng(131)
+    cache = Cache(torch, rng, [L], n_kv, 16, hd, True)
+    g = torch.Generator("cuda").manual_seed(132)
+    k, v = (torch.randn(cache.k.shape, device="cuda", generator=g) for _ in range(2))
+    k[..., 0] = 0
+    order = torch.from_numpy(cache.table[0]).cuda().long()
+    k[order[1::2], :, :, 0] = -15.0  # times 2 of q: 30 less
+    v[order[1::2]] *= 2.0 ** 45
+    quantize(torch, cache, k, v)
+    q = torch.randn((new, heads, hd), device="cuda", generator=g) * 0.1
+    q[..., 0] = 2.0
+    held_to(torch, cache, [L], [new], heads, dtype, 133, q=q, scale=1.0)

@@ -144,7 +144,9 @@ __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, cons
 // log2 of a code's value where the scale is x: exact for powers of two, which the append writes.
 __device__ __forceinline__ float log2_scale(float x) {
     const uint32_t b = __float_as_uint(x);
-    return fmaxf((b & 0x7fffffu) == 0 ? float(int(b >> 23) - 127) : log2f(x), -126.0f);
+    float e = __uint_as_float(0x4b000000u | b >> 23) - (8388608.0f + 127.0f);  // 2^23 + the exponent's field
+    if (b & 0x7fffffu) e = log2f(x);
+    return fmaxf(e, -126.0f);
 }
 // What turns values in units of 2^top over a sum in units of 2^top_sum into the quotient (nothing seen: there are no values).
 __device__ __forceinline__ float over_sum(float top, float sum, float top_sum) {
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     // with hi + lo, is 2^-36 of the largest; the reference lags by 2^kLazy at most. A row's likeliest key times a block's scale
     // counts as no less than 2^kLeast of the reference.
     constexpr float kLazy = 4.0f, kLift = 11.0f, kLeast = -60.0f;
+    constexpr float kNone = -3.0e38f;  // of what has seen nothing: a number, so that differences need no questions
     extern __shared__ __align__(16) float sm[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const neko_paged_cache& c = a.cache;
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 
         float acc[NT][kSteps][4];
         float m[NT][TL::kLaneRows], l[NT][TL::kLaneRows];  // largest score and sum of the weights against it
-        float u[NT][TL::kLaneRows];                        // reference: the accumulators' unit (8-bit values; else m)
+        float u[NT][TL::kLaneRows];                        // reference less kLift: the accumulators' unit (8-bit values)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[nt][i][e] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = u[nt][r] = -INFINITY, l[nt][r] = 0.0f;
+            for (int r = 0; r < TL::kLaneRows; r++) m[nt][r] = u[nt][r] = kNone, l[nt][r] = 0.0f;
         }
         const float inv_cap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     top[nt][r] = x;
-                    up |= x > m[nt][r] + kLazy || (Q8 && x + lv > u[nt][r] + kLazy);
+                    up |= x > m[nt][r] + kLazy || (Q8 && x + lv > u[nt][r] + (kLift + kLazy));
                 }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -479,14 +482,15 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                     for (int r = 0; r < TL::kLaneRows; r++) {
                         f[r] = 1.0f;
                         if (top[nt][r] > m[nt][r] + kLazy) {
-                            const float fm = ex2(m[nt][r] - top[nt][r]);  // from -inf: 0
+                            const float fm = ex2(m[nt][r] - top[nt][r]);  // from kNone: 0
                             m[nt][r] = top[nt][r];
                             l[nt][r] *= fm;
                             if (!Q8) f[r] = fm;
                         }
-                        if (Q8 && top[nt][r] + lv > u[nt][r] + kLazy) {
-                            f[r] = ex2(u[nt][r] - (top[nt][r] + lv));
-                            u[nt][r] = top[nt][r] + lv;
+                        if (Q8 && top[nt][r] + lv > u[nt][r] + (kLift + kLazy)) {
+                            const float next = top[nt][r] + lv - kLift;
+                            f[r] = ex2(u[nt][r] - next);
+                            u[nt][r] = next;
                         }
                     }
 #pragma unroll
@@ -503,9 +507,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                 for (int r = 0; r < TL::kLaneRows; r++) {
                     // 2^vr: what a weight against the reference is of what it adds to the sum
-                    const float ref = m[nt][r] == -INFINITY ? 0.0f : m[nt][r];
-                    const float vr = Q8 ? fmaxf(lv + (ref - (u[nt][r] == -INFINITY ? 0.0f : u[nt][r])), kLeast) : 0.0f;
-                    const float off = (Q8 ? vr - ref : -ref) + kLift;
+                    const float vr = Q8 ? fmaxf(lv + (m[nt][r] - u[nt][r]), kLeast + kLift) : kLift, off = vr - m[nt][r];
                     p[0][r] = ex2(z[nt][r][0] + off), p[1][r] = ex2(z[nt][r][1] + off);
                     l[nt][r] = Q8 ? fmaf(p[0][r] + p[1][r], ex2(-vr), l[nt][r]) : l[nt][r] + (p[0][r] + p[1][r]);
                 }
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int row = nt * TL::kRowsPer + (HILO ? t : 2 * t + r);
                 float* st = st0 + row * TL::kPitch;
-                if (g == 0) st[HD] = Q8 ? u[nt][r] : m[nt][r], st[HD + 1] = sum, st[HD + 2] = m[nt][r];
+                if (g == 0) *reinterpret_cast<float4*>(st + HD) = make_float4(Q8 ? u[nt][r] : m[nt][r], sum, m[nt][r], 0.0f);
 #pragma unroll
                 for (int i = 0; i < kSteps; i++) {
                     float2 v;
@@ -626,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             for (int y = lane; y < rows * (HD / 4); y += 32) {
                 const int row = y / (HD / 4), d = y % (HD / 4) * 4;
                 const float* st = st0 + row * TL::kPitch;
-                put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d),
-                              over_sum(st[HD], st[HD + 1], st[HD + 2]));
+                const float4 of = *reinterpret_cast<const float4*>(st + HD);
+                put_row<HILO>(a, plan, row0, kvh, r0 + row, d, *reinterpret_cast<const float4*>(st + d), over_sum(of.x, of.y, of.z));
             }
             __syncwarp();
         } else if (lane == 0) {
@@ -652,16 +654,19 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         auto join = [&](int row, int d, int parts, auto part, float& top, float& sum, float& top_sum) {
             top = top_sum = -INFINITY, sum = 0.0f;
             for (int i = 0; i < parts; i++)
-                if (const float* st = part(i)) top = fmaxf(top, st[row * TL::kPitch + HD]), top_sum = fmaxf(top_sum, st[row * TL::kPitch + HD + 2]);
+                if (const float* st = part(i)) {
+                    const float4 of = *reinterpret_cast<const float4*>(st + row * TL::kPitch + HD);
+                    top = fmaxf(top, of.x), top_sum = fmaxf(top_sum, of.z);
+                }
             const float ref = top == -INFINITY ? 0.0f : top, sum_ref = top_sum == -INFINITY ? 0.0f : top_sum;
             float4 v = make_float4(0, 0, 0, 0);
             for (int i = 0; i < parts; i++) {
                 const float* st = part(i);
                 if (!st) continue;
                 st += row * TL::kPitch;
-                const float f = ex2(st[HD] - ref);
-                const float4 o = *reinterpret_cast<const float4*>(st + d);
-                sum = fmaf(ex2(st[HD + 2] - sum_ref), st[HD + 1], sum);
+                const float4 o = *reinterpret_cast<const float4*>(st + d), of = *reinterpret_cast<const float4*>(st + HD);
+                const float f = ex2(of.x - ref);
+                sum = fmaf(ex2(of.z - sum_ref), of.y, sum);
                 v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
             }
             return v;
@@ -674,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 put_row<HILO>(a, plan, sp.row0, kvh, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
             } else {
                 *reinterpret_cast<float4*>(mine + row * TL::kPitch + d) = v;
-                if (d == 0) mine[row * TL::kPitch + HD] = top, mine[row * TL::kPitch + HD + 1] = sum, mine[row * TL::kPitch + HD + 2] = top_sum;
+                if (d == 0) *reinterpret_cast<float4*>(mine + row * TL::kPitch + HD) = make_float4(top, sum, top_sum, 0.0f);
             }
         }
         if (ranks == 1) return;
@@ -720,7 +725,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float* st = sm + (w ? __ffs(w) - 1 : b) * TL::kState + at;
-                    uw[i] = w ? st[HD] : -INFINITY, lw[i] = st[HD + 1], mw[i] = w ? st[HD + 2] : -INFINITY;
+                    const float4 of = *reinterpret_cast<const float4*>(st + HD);
+                    uw[i] = w ? of.x : -INFINITY, lw[i] = of.y, mw[i] = w ? of.z : -INFINITY;
                     o[i] = *reinterpret_cast<const float4*>(st + d);
                     w &= w - 1;
                 }
@@ -740,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                 put_row<HILO>(a, plan, row0, item_id % n_kv, tile * TL::kRows + row, d, v, over_sum(top, sum, top_sum));
             } else {
                 *reinterpret_cast<float4*>(part + at + d) = v;
-                if (d == 0) part[at + HD] = top, part[at + HD + 1] = sum, part[at + HD + 2] = top_sum;
+                if (d == 0) *reinterpret_cast<float4*>(part + at + HD) = make_float4(top, sum, top_sum, 0.0f);
             }
         }
     }
@@ -775,7 +781,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const neko_paged_attent
             for (int i = 0; i < 8; i++) {
                 const bool in = i0 + i < parts;
                 const float* p = part(in ? i0 + i : 0) + at;
-                uw[i] = in ? p[HD] : -INFINITY, lw[i] = in ? p[HD + 1] : 0.0f, mw[i] = in ? p[HD + 2] : -INFINITY;
+                const float4 of = in ? *reinterpret_cast<const float4*>(p + HD) : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+                uw[i] = of.x, lw[i] = of.y, mw[i] = of.z;
                 o[i] = in ? *reinterpret_cast<const float4*>(p + d) : make_float4(0, 0, 0, 0);
             }
             float now = top, now_sum = top_sum;

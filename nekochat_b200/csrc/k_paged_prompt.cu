@@ -79,8 +79,8 @@ struct PromptPlan {
     int group;      // query heads per KV head
     uint64_t group_inv;  // ceil(2^32 / group): x / group = x * group_inv >> 32 for x below 2^32 / group
     float* flush;        // [slot][HD][256 rows]: sums that have left TMEM (f32 queries; NULL: none do)
-    uint32_t* taken;     // [slot]: 1 while a CTA has it
-    int slots;           // as many as CTAs run at once
+    uint32_t* taken;     // [slot]: 1 while a CTA has it (NULL: every CTA has one of its own)
+    int slots;           // as many as CTAs run at once, or as there are
 };
 
 template <int HD, bool HILO>
@@ -296,17 +296,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         fence_barrier_init();
     }
     if constexpr (HILO) {
-        // There is a free slot for every CTA that runs; the search is bounded all the same. It begins at the SM's number, where the
-        // SM's CTA before this one had its slot (from the block's number on it took 90 us of 770 in all).
+        // A slot for this CTA: its own number's in a grid of no more CTAs than slots, else one that is free. There is one for every
+        // CTA that runs (the search is bounded all the same), and it begins at the SM's number, where the SM's CTA before this
+        // one had its slot: from the block's number on it took 90 us of 770 in all, and with fewer slots than SMs 50 of 165.
         if (tid == 32 * kLoadWarp) {
             int slot = -1;
-            unsigned sm_id;
-            asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
-            if (plan.flush && nt > kFlush)
+            if (plan.flush && nt > kFlush) {
+                unsigned sm_id;
+                asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
+                if (!plan.taken) slot = int(blockIdx.x);
                 for (int x = 0; x < 2 * plan.slots && slot < 0; x++) {
                     const int y = int((sm_id + unsigned(x)) % unsigned(plan.slots));
                     if (atomicCAS(&plan.taken[y], 0u, 1u) == 0u) slot = y;
                 }
+            }
             ms.slot = slot;
         }
     }
@@ -969,7 +972,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     tc_fence_before();
     if (alone) __syncthreads();
     else cluster.sync();
-    if (HILO && tid == 32 * kLoadWarp && ms.slot >= 0) {  // every thread has read its sums
+    if (HILO && tid == 32 * kLoadWarp && plan.taken && ms.slot >= 0) {  // every thread has read its sums
         __threadfence();
         atomicExch(&plan.taken[ms.slot], 0u);
     }
@@ -1159,13 +1162,16 @@ cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
     p.slots = int(std::min<int64_t>(items * p.ranks, num_sms()));
     void* flush = nullptr;
     if (a.type == NEKO_T_F32 && key_tiles > int64_t(p.ranks) * kFlush) {
+        const bool shared = items * p.ranks > p.slots;
         const size_t bytes = size_t(p.slots) * 2 * kRows * HD * 4;  // at most 19 MB
         if (cudaError_t e = scratch_alloc(&flush, bytes + size_t(p.slots) * 4, st); e != cudaSuccess) return e;
         p.flush = static_cast<float*>(flush);
-        p.taken = reinterpret_cast<uint32_t*>(static_cast<char*>(flush) + bytes);
-        if (cudaError_t e = cudaMemsetAsync(p.taken, 0, size_t(p.slots) * 4, st); e != cudaSuccess) {
-            cudaFreeAsync(flush, st);
-            return e;
+        if (shared) {
+            p.taken = reinterpret_cast<uint32_t*>(static_cast<char*>(flush) + bytes);
+            if (cudaError_t e = cudaMemsetAsync(p.taken, 0, size_t(p.slots) * 4, st); e != cudaSuccess) {
+                cudaFreeAsync(flush, st);
+                return e;
+            }
         }
     }
     const cudaError_t e = by_pages<HD>(a, p, items, st);

@@ -9,9 +9,9 @@
 //  * Steps (a few new tokens per sequence): a warp per unit, head_dim / 32 consecutive values a lane; latency is all.
 //  * Prompts: a CTA per (sequence, page) and group of heads. A lane holds eight values of a token, both members of four
 //    rotation pairs, so the rotation needs no exchange and its cosines stay in registers from head to head; the next
-//    head's values fly while this one's are worked on. Ragged prompts of 12,700 bf16 tokens, 32 + 16 heads of 128, 8-bit
-//    cache: 92 us, 3.6 TB/s (56 % of the measured copy rate; issue slots bound it: 136 warp instructions a row at first,
-//    packed f32 pairs and eight values a lane since); 4,001 f32 tokens, f16 cache: 14 us, 4.4 TB/s.
+//    head's values fly while this one's are worked on. Ragged prompts of 14,364 bf16 tokens, 32 + 16 heads of 128, 8-bit
+//    cache: 94 us, 3.5 TB/s (55 % of the measured copy rate; issue slots bound it: 136 warp instructions a row at first,
+//    packed f32 pairs and eight values a lane since); 4,001 f32 tokens, f16 cache: 15 us, 4.1 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -514,7 +514,7 @@ cudaError_t go(const neko_paged_append_args& a, cudaStream_t st) {
                          dim3(128), 0, st, false, a, p);
     }
     const int warps = std::max(1, ps * (HD / 8) / (32 * kSlots));
-    // heads per CTA: up to 8, which share the loads of the cosines (ragged prompts of 12,700 tokens: 92 us, with 4 heads
+    // heads per CTA: up to 8, which share the loads of the cosines (ragged prompts of 14,364 tokens: 92 us, with 4 heads
     // 97), as long as every SM gets 24 warps (a prompt of 4,001 tokens on 12 heads: 4 heads 12.5 us, 8 heads 14.8)
     while (p.per_cta < 8 && a.cache.n_seq * chunks * ((p.units + 2 * p.per_cta - 1) / (2 * p.per_cta)) * warps >= 24 * num_sms()) p.per_cta *= 2;
     const int groups = (p.units + p.per_cta - 1) / p.per_cta;

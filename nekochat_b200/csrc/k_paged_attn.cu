@@ -1,8 +1,9 @@
 // Attention of few query rows over a paged cache (neko_op_paged_attention): decode steps, short continuations, small
 // prompts, and every head dim of 32.
 //
-// Bound by memory: on contexts of one length 5.9 TB/s from 8-bit pages and 6.4 TB/s from f16 ones (74 x 8,192 tokens, 91 and
-// 99 % of the measured copy rate), 5.3 TB/s on 128 ragged contexts up to 8,192 tokens (227 us); small calls by latency.
+// Bound by memory: on contexts of one length 5.6 TB/s from 8-bit pages and 6.5 TB/s from f16 ones (74 x 8,192 tokens, 87 and
+// 101 % of the measured copy rate; the value scales' exponents cost the former 5 %), 5.2 TB/s on 128 ragged contexts up to
+// 8,192 tokens (232 us); small calls by latency.
 //
 // The packed rows of a (sequence, KV head) are its new tokens times the G query heads that share the KV head, so a key
 // is read once for all of them. Every warp owns groups of 16 keys and works alone (no barrier until the end): scores

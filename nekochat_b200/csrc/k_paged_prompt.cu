@@ -1,7 +1,8 @@
 // Attention of many query rows over a paged cache (neko_op_paged_attention): prompts and long continuations, on
 // tcgen05.
 //
-// A prompt of 8,192 bf16 tokens, 16 heads on 8: 320 us, 860 TFLOP/s of the causal half's products (51 % of the measured rate).
+// A prompt of 8,192 bf16 tokens, 16 heads on 8: 320 to 337 us, 816 to 860 TFLOP/s of the causal half's products (50 % of the measured
+// rate); 350 us and more in a second of such calls, under the power cap.
 // Per pair of row tiles and 128 keys about 4,080 cycles against 2,048 of the UMMAs: each row tile's chain is S, softmax (2,010
 // cycles: TMEM reads 330, maximum and meeting 500, exponentials 1,110), P V and S again (1,190), and the two tiles take
 // turns. f32 rows take twice the UMMAs (5,900 cycles).
@@ -785,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     if (a.softcap > 0.0f) {  // of score / cap
                         if (__all_sync(0xffffffffu, most <= 0.5f)) {
-                            // an odd polynomial of degree 9 (least maximum error on [-1/2, 1/2]: 3e-9): two units of the
+                            // an odd polynomial of degree 9 (largest error on [-1/2, 1/2]: 6.3e-9): two units of the
                             // special functions less than below
 #pragma unroll
                             for (int x = 0; x < 32; x += 2) {

@@ -15,7 +15,8 @@
 // reference is the largest score plus log2 of the value scale that it sees, and the sum of its weights has the largest score
 // as a unit of its own, so what f16 rounds off a weight is small beside the largest of the row's products. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
-// 16-bit queries one exact f16 column, weights one f16. Rows are scaled by a power of two into f16's range first.
+// 16-bit queries one f16 column, weights one f16. Rows are scaled by a power of two into f16's range first (exact, but for
+// bf16 values below 2^-17 of their row's largest, which lose bits).
 // All groups of all items, in order, are dealt out in equal shares to the warps that the GPU holds at a time, whatever
 // the lengths; each CTA adds up the sequences' groups itself (the lengths are on the device only). A warp goes through
 // its share item by item, its start-up hidden behind the other warps of its SM: nothing waits for a CTA's other warps

@@ -11,8 +11,8 @@
 // takes two tiles of 128 rows (one when there are no more) and walks the keys in tiles of 128:
 //   S = Q K^T in TMEM, weights P back into TMEM over S (f16), O += P V in TMEM, all accumulation f32.
 // f32 queries are f16 hi + lo in shared memory (S = Qhi K^T + Qlo K^T) and their weights hi + lo in TMEM (P takes
-// exactly the 128 columns of its S); 16-bit queries are one exact f16 and their weights one f16. Rows are scaled by a
-// power of two into f16's range first. Roles:
+// exactly the 128 columns of its S); 16-bit queries are one f16 and their weights one f16. Rows are scaled by a
+// power of two into f16's range first (exact, but for bf16 values below 2^-17 of their row's largest, which lose bits). Roles:
 //  * warps 0..7 and 8..15: softmax of one row tile each, two threads per row (64 keys each; two warps more per scheduler
 //    hide each other's latencies), which tell each other their largest scores. The reference maximum moves only
 //    when a score exceeds it by a factor of 2^8 (weights above 1 are as exact as any in f16), so O is hardly ever rescaled, and

@@ -208,8 +208,10 @@ typedef struct neko_paged_cache {
  * the largest finite magnitude of the new tokens is at most 448, or its old scale when it already held tokens of the
  * sequence and that is larger; when the scale grows, the codes of the tokens held before are multiplied by old / new
  * (exact, but for codes that become subnormal). Infinities are stored as +-448 * scale, NaN as NaN.
- * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous; token strides (of several rows)
- * below 2^24 and at most 65,530 pages of new tokens per sequence (else NEKO_ERR_UNSUPPORTED). */
+ * A page that gets tokens is in one sequence's table only, once (pages that are only read may be shared).
+ * q may be NULL (keys and values only); q_out may equal q. Row strides in elements, head_dim contiguous; token strides
+ * (of several rows) below 2^24 and at most 65,530 pages of new tokens per sequence (else NEKO_ERR_UNSUPPORTED). max_new
+ * may be larger than any sequence needs; the call is planned for it. */
 typedef struct neko_paged_append_args {
     neko_paged_cache cache;
     const void *q, *k, *v;
@@ -232,12 +234,13 @@ int neko_op_paged_append(const neko_paged_append_args* args, void* stream);
  * h / (n_head / n_kv)) and key j: z = scale * q . k_j; with softcap > 0 (finite), z = softcap * tanh(z / softcap); with slopes,
  * z += slopes[h] * (j - pos). Key j is seen when its page is resident, j < kv_len[s], and j <= pos with (window == 0
  * or pos - j < window), or j < prefix[s] (prefix NULL: none). out = sum_j softmax(z)_j v_j over the keys seen, zeros
- * when there are none. A value that is not seen has no effect, whatever it holds. Sums, maxima and accumulators are f32;
- * NEKO_T_F32 queries and weights enter the tensor cores as f16 hi + lo (22 bits, and what is rounded off a weight is at most 2^-32
- * of the row's largest), 16-bit ones as one f16 (11 bits; bf16 queries below 2^-17 of their row's largest fewer). E4M3 pages with tokens have finite scales.
- * n_head a multiple of n_kv, at most 16384 sequences and 2^31 rows (max_new or tokens, times n_head / n_kv; fewer where that
- * quotient is no power of two), else NEKO_ERR_UNSUPPORTED. out rows have type `type` and strides
- * o_token, o_head. */
+ * when there are none; rows of no sequence keep what they held. A value that is not seen has no effect, whatever it holds
+ * (E4M3 pages with tokens have finite scales). Sums, maxima and accumulators are f32; NEKO_T_F32 queries and weights enter
+ * the tensor cores as f16 hi + lo (22 bits; what is rounded off a weight is at most 2^-32 of the row's largest, E4M3 values'
+ * scales counted in), 16-bit ones as one f16 (11 bits; bf16 queries below 2^-17 of their row's largest fewer).
+ * n_head a multiple of n_kv; at most 16384 sequences, and 2^31 rows of a KV head (the smaller of max_new and tokens, times
+ * n_head / n_kv; fewer where that quotient is no power of two), else NEKO_ERR_UNSUPPORTED. Which kernel takes a call goes by
+ * max_new and cache.max_pages. out rows have type `type` and strides o_token, o_head. */
 typedef struct neko_paged_attention_args {
     neko_paged_cache cache;
     const void* q;
@@ -256,11 +259,12 @@ typedef struct neko_paged_attention_args {
     int32_t reserved;
 } neko_paged_attention_args;
 int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream);
-/* What the two calls above could not do depends on lengths that only the device holds: a sequence with more than max_new
- * new tokens, or rows outside [0, tokens), is left out whole (its rows of out and q_out keep what they held), positions past the rotation
- * table are not stored. Waits for the stream's work and returns NEKO_ERR_DEVICE, with the reason in neko_last_error, when that
- * has happened on the current device since the last call of this function, whatever the stream; NEKO_OK when it has not. Not
- * while the stream is being captured. A neko_model's steps and a neko_ctx neither see these errors nor clear them. */
+/* What the two calls above cannot do depends on lengths that only the device holds: a sequence with more than max_new new
+ * tokens, or with rows outside [0, tokens), is left out whole (its rows of out and q_out keep what they held), positions past
+ * the rotation table are not stored. Waits for the stream's work and returns NEKO_ERR_DEVICE, with the reason in
+ * neko_last_error, when that has happened on the current device since the last call of this function, whatever the stream;
+ * NEKO_OK when it has not. Not while the stream is being captured. A neko_model's steps and a neko_ctx neither see these
+ * errors nor clear them. */
 int neko_op_status(void* stream);
 /* The single operators (neko_op_*) take stream-ordered scratch memory from a pool of the library's, which keeps what it has grown
  * to: prompts over long E4M3 caches as f16 copies of the pages (up to 2 GiB), f32 rows over more than 1,024 keys up to 19 MB,

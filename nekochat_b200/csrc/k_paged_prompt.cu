@@ -1088,7 +1088,10 @@ cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, in
     const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
     if (p.row_tiles < kCopyTiles || bytes > kCopyBytes) return by_type<HD, kCodes>(a, p, items, nullptr, st);
     void* mem = nullptr;
-    if (cudaError_t e = scratch_alloc(&mem, size_t(bytes), st); e != cudaSuccess) return e;
+    if (scratch_alloc(&mem, size_t(bytes), st) != cudaSuccess) {  // a cache that fills the GPU: every CTA converts its own
+        cudaGetLastError();
+        return by_type<HD, kCodes>(a, p, items, nullptr, st);
+    }
     cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
                               static_cast<uint4*>(mem));
     if (e == cudaSuccess) e = by_type<HD, kCopies>(a, p, items, static_cast<const __half*>(mem), st);

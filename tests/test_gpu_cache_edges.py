@@ -585,3 +585,35 @@ def test_large_values_of_small_weight_count(torch, form, dtype):
     q = torch.randn((new, heads, hd), device="cuda", generator=g) * 0.1
     q[..., 0] = 2.0
     held_to(torch, cache, [L], [new], heads, dtype, 133, q=q, scale=1.0)
+
+
+def test_a_prompt_on_a_gpu_that_the_cache_fills(torch):
+    """Where there is no room for f16 copies of an 8-bit cache's pages (491 MB here), the call does without."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(134)
+    lens, new = [120000], [300]
+    cache = Cache(torch, rng, lens, 8, 128, 128, True)
+    g = torch.Generator("cuda").manual_seed(135)
+    cache.k.copy_(torch.randint(0, 100, cache.k.shape, device="cuda", generator=g, dtype=torch.uint8))
+    cache.v.copy_(cache.k)
+    cache.ks.fill_(0.01), cache.vs.fill_(0.01)
+    q = torch.randn((300, 16, 128), device="cuda", generator=g)
+    table, out = torch.from_numpy(cache.table).cuda(), torch.empty_like(q)
+
+    def call(n, L):
+        ops.paged_attention(q[:n], cache.k, cache.v, table[:, :-(-L // 128)], ints(torch, L), k_scale=cache.ks, v_scale=cache.vs,
+                            q_start=ints(torch, 0, n), max_new=n, out=out[:n])
+
+    call(60, 4000)  # one row tile: the kernel without copies is loaded
+    call(300, lens[0])
+    want = out.clone()
+    torch.cuda.synchronize()
+    ops.trim()
+    torch.cuda.empty_cache()
+    full = torch.empty(torch.cuda.mem_get_info()[0] - (300 << 20), dtype=torch.uint8, device="cuda")
+    out.zero_()
+    call(300, lens[0])
+    torch.cuda.synchronize()
+    del full
+    torch.cuda.empty_cache()
+    assert (out - want).abs().max() <= 2e-6 * want.abs().max()

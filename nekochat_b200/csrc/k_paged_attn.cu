@@ -13,7 +13,8 @@
 // pieces g, g + 8, .. of key rows 2t, 2t + 1, 2t + 8, 2t + 9; neither K nor V passes through shared memory. 8-bit codes
 // become f16 in registers (exact), keys' scales multiply the scores, values' scales enter the weights' exponent: a row's
 // reference is the largest score plus log2 of the value scale that it sees, and the sum of its weights has the largest score
-// as a unit of its own, so what f16 rounds off a weight is small beside the largest of the row's products. P reaches the second product by transposing 8 x 8 tiles in registers (movmatrix).
+// as a unit of its own, so what f16 rounds off a weight is small beside the largest of the row's products. P reaches the
+// second product by transposing 8 x 8 tiles in registers (movmatrix).
 // f32 queries are two columns each, f16 hi and lo (22 bits; scores are the columns' sum), and so are their weights P;
 // 16-bit queries one f16 column, weights one f16. Rows are scaled by a power of two into f16's range first (exact, but for
 // bf16 values below 2^-17 of their row's largest, which lose bits).

@@ -259,9 +259,96 @@ typedef struct neko_paged_attention_args {
     int32_t reserved;
 } neko_paged_attention_args;
 int neko_op_paged_attention(const neko_paged_attention_args* args, void* stream);
-/* What the two calls above cannot do depends on lengths that only the device holds: a sequence with more than max_new new
- * tokens, or with rows outside [0, tokens), is left out whole (its rows of out and q_out keep what they held), positions past
- * the rotation table are not stored. Waits for the stream's work and returns NEKO_ERR_DEVICE, with the reason in
+
+/* ---- drafted tokens: several guesses at what comes next go through the model in one step, as a tree behind the newest token
+ * (node 0 of a sequence, the root; node i's parent is an earlier node of its sequence). Node i of sequence s is row q_start[s] + i
+ * and goes to slot start[s] + i of the cache; its position is start[s] + depth[i], depth the number of its ancestors. */
+typedef struct neko_tree {
+    const uint64_t* mask;   /* device [tokens][words]: bit j of a row's words: the row sees node j of its sequence */
+    const int32_t* depth;   /* device [tokens], counted as within [0, n), n the sequence's nodes; NULL: only where neither window nor
+                               slopes ask for positions */
+    int32_t words;          /* at least max_new / 64, rounded up */
+    int32_t reserved;
+} neko_tree;
+/* neko_op_paged_append for nodes: q and k are turned by start[s] + depth[i] (depth within [0, i]; NULL: as neko_op_paged_append)
+ * and stored to slot start[s] + i. Slots at or past cs_rows are not stored, as there. */
+int neko_op_paged_tree_append(const neko_paged_append_args* args, const int32_t* depth, void* stream);
+/* neko_op_paged_attention for nodes, which are in the cache already (the last n of kv_len[s]): a row sees the keys before them
+ * (with a window those less than `window` positions back) and the nodes of its mask (the same); whether it sees itself is up to
+ * the mask. Positions (window, slopes) go by depth, of keys too. No prefix. A row that sees nothing comes out as zeros. */
+int neko_op_paged_tree_attention(const neko_paged_attention_args* args, const neko_tree* tree, void* stream);
+/* The masks and depths of trees given by parents: parent[q_start[s] + i] in [0, i) is node i's parent, counted from the
+ * sequence's first node; anything else makes node i a root. Bit j of row i: j is i or an ancestor of i. Any of mask and depth may
+ * be NULL. Rows of no sequence keep what they held. At most NEKO_MAX_NODES nodes a sequence. */
+#define NEKO_MAX_NODES 4096
+int neko_op_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
+                       int32_t* depth, void* stream);
+/* Walks each sequence's tree along the tokens chosen at its nodes: from node 0 to the lowest child whose draft is the token
+ * chosen at the node, and so on. path [n_seq][max_new]: the nodes walked through, 0 first, zeros behind them; count [n_seq]: how
+ * many; token [n_seq]: the one chosen at the last of them. A sequence without nodes has count 0 and token -1. */
+int neko_op_tree_accept(const int32_t* chosen, const int32_t* draft, const int32_t* parent, const int32_t* q_start, int n_seq,
+                        int tokens, int max_new, int32_t* path, int32_t* count, int32_t* token, void* stream);
+
+/* ---- moving what a cache holds. `planes` pools of pages (keys and values of every layer, say) alike but for their place, plane p
+ * plane_stride elements after plane 0 (scales: scale_plane floats), each as neko_paged_cache describes a pool. */
+typedef struct neko_paged_planes {
+    void* pages;            /* device; NEKO_T_F16 or NEKO_T_E4M3, 16-byte aligned as are the strides */
+    float* scale;           /* device; NEKO_T_E4M3 only */
+    const int32_t* table;   /* device [n_seq][table_stride]; not read by neko_op_paged_copy */
+    int64_t plane_stride, page_stride, scale_plane, scale_stride, table_stride;
+    int32_t type;
+    int32_t planes;
+    int32_t n_seq;
+    int32_t max_pages;
+    int32_t num_pages;
+    int32_t n_kv;
+    int32_t page_size;
+    int32_t head_dim;
+} neko_paged_planes;
+/* In every plane, token start[s] + path[s][k] of sequence s becomes token start[s] + k, k < count[s] (at most max_count), as if all
+ * were read before any is written: what tree_accept leaves of a tree, brought together. Rows of path are path_stride apart. Tokens
+ * from or to pages that are not resident stay away; tokens at or past start[s] + count[s] are no longer the sequence's (what their
+ * places hold is not said). start[s] < 0: inactive.
+ * NEKO_T_E4M3: a page that gets tokens takes as scale the largest of its own (where tokens before start[s] are in it) and of the
+ * pages that its tokens come from; codes are multiplied by old / new scale (exact, but for codes that become subnormal). A page
+ * that gets tokens is in one sequence's table only, once. */
+int neko_op_paged_compact(const neko_paged_planes* planes, const int32_t* start, const int32_t* path, int64_t path_stride,
+                          const int32_t* count, int max_count, void* stream);
+/* In every plane, page dst[i] becomes a copy of page src[i] (its scales too), i < n (device arrays). A pair with an entry outside
+ * [0, num_pages) is skipped. A page is in dst once, and not in src if it is in dst of another pair. Forks of sequences share
+ * their full pages and copy the one that is partly filled. */
+int neko_op_paged_copy(const neko_paged_planes* planes, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* A token for each row of logits [rows][vocab] (row stride row_stride elements; not changed), from the row's number u in [0, 1):
+ * weights w_i = exp((x_i - max x) / temperature); of the tokens in descending order of x (equal ones by index) the first top_k
+ * (0 or less: all), of those the shortest beginning whose weights add up to top_p times all of theirs (1 or more: all; at least
+ * one), of those the ones with w_i >= min_p (values above 1 count as 1). Among what is left, in the order of the vocabulary, the
+ * first token at which the sum of the weights exceeds u times their total. temperature 0 or less: the first maximum. NaN and
+ * -infinity are never taken; +infinities share the weight. A row with nothing to take gives token -1, probability 0.
+ * Weights are held to 2^-45 of the largest and added as integers: the result depends on no order.
+ * Each parameter is one number, or an array [rows] where its pointer is not NULL. prob (or NULL): w_token / total, 1 for
+ * temperature 0. vocab at most NEKO_MAX_VOCAB. */
+#define NEKO_MAX_VOCAB 393216
+typedef struct neko_sample_rows_args {
+    const void* logits;     /* device; NEKO_T_F32, NEKO_T_F16, NEKO_T_BF16, aligned to its type */
+    const double* u;        /* device [rows]; NULL: every row greedy */
+    const float *temperatures, *top_ps, *min_ps; /* device [rows] or NULL */
+    const int32_t* top_ks;  /* device [rows] or NULL */
+    int32_t* token;         /* device [rows] */
+    float* prob;            /* device [rows] or NULL */
+    int64_t row_stride;
+    int32_t type;
+    int32_t rows;
+    int32_t vocab;
+    int32_t top_k;
+    float temperature, top_p, min_p;
+    int32_t reserved;
+} neko_sample_rows_args;
+int neko_op_sample_rows(const neko_sample_rows_args* args, void* stream);
+
+/* What the paged and tree calls above cannot do depends on lengths that only the device holds: a sequence with more than max_new new
+ * tokens (max_count), or with rows outside [0, tokens), is left out whole (its rows of out and q_out keep what they held), positions
+ * past the rotation table are not stored. Waits for the stream's work and returns NEKO_ERR_DEVICE, with the reason in
  * neko_last_error, when that has happened on the current device since the last call of this function, whatever the stream;
  * NEKO_OK when it has not. Not while the stream is being captured. A neko_model's steps and a neko_ctx neither see these
  * errors nor clear them. */

@@ -98,6 +98,13 @@ _SIGS = {
                                             _vp]),
     "neko_op_paged_append": (C.c_int, [_vp, _vp]),
     "neko_op_paged_attention": (C.c_int, [_vp, _vp]),
+    "neko_op_paged_tree_append": (C.c_int, [_vp, _vp, _vp]),
+    "neko_op_paged_tree_attention": (C.c_int, [_vp, _vp, _vp]),
+    "neko_op_tree_masks": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp]),
+    "neko_op_tree_accept": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp]),
+    "neko_op_paged_compact": (C.c_int, [_vp, _vp, _vp, C.c_int64, _vp, C.c_int, _vp]),
+    "neko_op_paged_copy": (C.c_int, [_vp, _vp, _vp, C.c_int, _vp]),
+    "neko_op_sample_rows": (C.c_int, [_vp, _vp]),
     "neko_op_status": (C.c_int, [_vp]),
     "neko_op_trim": (C.c_int, [C.c_size_t]),
     "neko_model_create": (_vp, [C.c_int, C.POINTER(ModelConfig), C.c_char_p, C.c_size_t]),

@@ -36,6 +36,9 @@ struct AppendPlan {
     int page_log;
 };
 
+// Positions after `start` by which a node of a tree is turned: its depth, no more than its place.
+__device__ __forceinline__ int depth_of(const int32_t* depth, int row0, int i) { return min(max(depth[row0 + i], 0), i); }
+
 // x c + y s, the same bits in both kernels.
 __device__ __forceinline__ float turned(float x, float y, float c, float s) { return __fmaf_rn(x, c, __fmul_rn(y, s)); }
 
@@ -56,7 +59,8 @@ __device__ __forceinline__ void recode(uint8_t* blk, int count, float ratio, int
 }
 
 template <typename T, int HD, bool Q8>
-__global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged_append_args a, const AppendPlan plan) {
+__global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged_append_args a, const AppendPlan plan,
+                                                                const int32_t* depth) {
     constexpr int E = HD / 32;  // values per lane and token
     const int lane = threadIdx.x & 31;
     const int unit = blockIdx.y * 4 + (threadIdx.x >> 5), s = blockIdx.x, chunk = blockIdx.z;
@@ -135,7 +139,8 @@ __global__ void __launch_bounds__(128) paged_append_step_kernel(const neko_paged
 #pragma unroll
             for (int e = 0; e < E; e++) y[e] = __shfl_sync(0xffffffffu, x[r][e], partner);
             if (in_rot && live && pos < a.cs_rows) {
-                const float2* cs = reinterpret_cast<const float2*>(a.cs) + int64_t(pos) * half + j0;
+                const int at = depth ? start + depth_of(depth, row0, i) : pos;
+                const float2* cs = reinterpret_cast<const float2*>(a.cs) + int64_t(at) * half + j0;
                 if (a.interleaved && E > 1) {
 #pragma unroll
                     for (int e = 0; e < E / 2; e++) {
@@ -270,7 +275,7 @@ __device__ __forceinline__ void put4(T* p, bool vec, uint64_t x, uint64_t y) {
 }
 
 template <typename T, int HD, bool Q8>
-__global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_append_args a, const AppendPlan plan) {
+__global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_append_args a, const AppendPlan plan, const int32_t* depth) {
     constexpr int kLanes = HD / 8, kRowsPer = 32 / kLanes;  // lanes per token, tokens per warp and slot
     __shared__ uint32_t red[2][32];
     __shared__ __align__(16) float gains[2][HD];
@@ -322,7 +327,8 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
         const int pos = pos0 + tok[z];
         const bool turn = in_rot && live && tok[z] < count && pos < a.cs_rows;
         turns[z] = turn;
-        const float4* p = reinterpret_cast<const float4*>(a.cs + (turn ? int64_t(pos) * a.rot + 8 * l : 0));
+        const int at = depth && turn ? start + depth_of(depth, row0, i0 + tok[z]) : pos;
+        const float4* p = reinterpret_cast<const float4*>(a.cs + (turn ? int64_t(at) * a.rot + 8 * l : 0));
         const float4 t0 = turn ? p[0] : make_float4(1, 0, 1, 0), t1 = turn ? p[1] : make_float4(1, 0, 1, 0);
         cs[z][0] = pack2(t0.x, t0.z), cs[z][1] = pack2(t1.x, t1.z);
         sn[z][0] = pack2(t0.y, t0.w), sn[z][1] = pack2(t1.y, t1.w);
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const neko_paged_appe
 }
 
 template <typename T, int HD, bool Q8>
-cudaError_t go(const neko_paged_append_args& a, cudaStream_t st) {
+cudaError_t go(const neko_paged_append_args& a, const int32_t* depth, cudaStream_t st) {
     AppendPlan p;
     const int ps = a.cache.page_size;
     p.page_log = 31 - __builtin_clz(ps);
@@ -511,7 +517,7 @@ cudaError_t go(const neko_paged_append_args& a, cudaStream_t st) {
     if (a.max_new <= kFewTokens) {
         if (chunks > 65535 || (p.units + 3) / 4 > 65535) return cudaErrorInvalidConfiguration;
         return launch_ex(paged_append_step_kernel<T, HD, Q8>, dim3(unsigned(a.cache.n_seq), unsigned(p.units + 3) / 4, unsigned(chunks)),
-                         dim3(128), 0, st, false, a, p);
+                         dim3(128), 0, st, false, a, p, depth);
     }
     const int warps = std::max(1, ps * (HD / 8) / (32 * kSlots));
     // heads per CTA: up to 8, which share the loads of the cosines (ragged prompts of 14,364 tokens: 92 us, with 4 heads
@@ -520,27 +526,27 @@ cudaError_t go(const neko_paged_append_args& a, cudaStream_t st) {
     const int groups = (p.units + p.per_cta - 1) / p.per_cta;
     if (chunks > 65535 || groups > 65535) return cudaErrorInvalidConfiguration;
     return launch_ex(paged_append_kernel<T, HD, Q8>, dim3(unsigned(a.cache.n_seq), unsigned(groups), unsigned(chunks)), dim3(32 * warps), 0,
-                     st, false, a, p);
+                     st, false, a, p, depth);
 }
 
 template <typename T>
-cudaError_t by_shape(const neko_paged_append_args& a, cudaStream_t st) {
+cudaError_t by_shape(const neko_paged_append_args& a, const int32_t* depth, cudaStream_t st) {
     const bool q8 = a.cache.type == NEKO_T_E4M3;
     switch (a.cache.head_dim) {
-        case 32: return q8 ? go<T, 32, true>(a, st) : go<T, 32, false>(a, st);
-        case 64: return q8 ? go<T, 64, true>(a, st) : go<T, 64, false>(a, st);
-        default: return q8 ? go<T, 128, true>(a, st) : go<T, 128, false>(a, st);
+        case 32: return q8 ? go<T, 32, true>(a, depth, st) : go<T, 32, false>(a, depth, st);
+        case 64: return q8 ? go<T, 64, true>(a, depth, st) : go<T, 64, false>(a, depth, st);
+        default: return q8 ? go<T, 128, true>(a, depth, st) : go<T, 128, false>(a, depth, st);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_append(const neko_paged_append_args& args, cudaStream_t st) {
+cudaError_t launch_paged_append(const neko_paged_append_args& args, const int32_t* depth, cudaStream_t st) {
     neko_paged_append_args a = args;
     a.cs_rows = std::min(a.cs_rows, kFarthest);
-    return a.type == NEKO_T_F32   ? by_shape<float>(a, st)
-           : a.type == NEKO_T_F16 ? by_shape<__half>(a, st)
-                                  : by_shape<__nv_bfloat16>(a, st);
+    return a.type == NEKO_T_F32   ? by_shape<float>(a, depth, st)
+           : a.type == NEKO_T_F16 ? by_shape<__half>(a, depth, st)
+                                  : by_shape<__nv_bfloat16>(a, depth, st);
 }
 
 }  // namespace neko

@@ -117,7 +117,7 @@ struct Tile {
 struct Span {
     int row0, n, held, len, prefix, rows, pos_lo, pos_hi, hi, lo, g_lo, g_pre, ng;
 };
-template <int kRows>
+template <int kRows, bool TREE>
 __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, const DecodePlan& plan, int s, int tile) {
     Span v;
     v.row0 = a.q_start ? a.q_start[s] : s;
@@ -133,6 +133,7 @@ __device__ __forceinline__ Span span_of(const neko_paged_attention_args& a, cons
     const int r0 = tile * kRows;
     v.rows = max(min(v.n * plan.group - r0, kRows), 0);
     v.pos_lo = v.held - v.n + over_g(r0), v.pos_hi = v.held - v.n + over_g(r0 + max(v.rows, 1) - 1);
+    if constexpr (TREE) v.pos_lo = v.held - v.n, v.pos_hi = v.held - 1;  // whatever the depths
     // keys some row of the tile sees: [0, pre) and [lo, hi), as groups of 16
     v.hi = max(min(v.len, v.pos_hi + 1), 0);
     v.lo = a.window && v.pos_lo >= a.window ? min(v.pos_lo - a.window + 1, v.hi) : 0;
@@ -168,9 +169,9 @@ __device__ __forceinline__ void put_row(const neko_paged_attention_args& a, cons
     else store(static_cast<__nv_bfloat16*>(a.out) + off);
 }
 
-template <int HD, bool Q8, bool HILO, int NT, bool CL>
+template <int HD, bool Q8, bool HILO, int NT, bool CL, bool TREE>
 __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kernel(const neko_paged_attention_args a,
-                                                                                const DecodePlan plan) {
+                                                                                const DecodePlan plan, const neko_tree tr) {
     using TL = Tile<HD, HILO, NT>;
     using W = Words<HD, Q8>;
     constexpr int kSteps = HD / 16;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     if constexpr (CL) {
         // of one item: the cluster's
         s = blockIdx.x >> plan.ranks_log, kvh = blockIdx.z;
-        cnt = span_of<TL::kRows>(a, plan, s, tile).ng;
+        cnt = span_of<TL::kRows, TREE>(a, plan, s, tile).ng;
         total = cnt, warps = min(int64_t(kWarps) << plan.ranks_log, total);
         const int gw = (blockIdx.x & ((1 << plan.ranks_log) - 1)) * kWarps + warp;
         if (gw < warps) x = total * gw / warps, x_end = total * (gw + 1) / warps;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         int carry = 0;
         for (int base = 0; base < c.n_seq; base += kThreads) {
             const int sq = base + tid;
-            int y = sq < c.n_seq ? span_of<TL::kRows>(a, plan, sq, tile).ng : 0;
+            int y = sq < c.n_seq ? span_of<TL::kRows, TREE>(a, plan, sq, tile).ng : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int z = __shfl_up_sync(0xffffffffu, y, o);
@@ -247,10 +248,12 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     while (x < x_end) {
         const int64_t item = CL ? 0 : int64_t(pre[s]) * n_kv + int64_t(kvh) * cnt;  // its first group
         const int k_begin = int(x - item), k_end = int(min(int64_t(cnt), x_end - item));
-        const Span sp = span_of<TL::kRows>(a, plan, s, tile);
+        const Span sp = span_of<TL::kRows, TREE>(a, plan, s, tile);
         const int row0 = sp.row0, n = sp.n, held = sp.held, len = sp.len, prefix = sp.prefix, rows = sp.rows;
         const int pos_lo = sp.pos_lo, pos_hi = sp.pos_hi, hi = sp.hi, lo = sp.lo, g_lo = sp.g_lo, g_pre = sp.g_pre;
         const int r0 = tile * TL::kRows;
+        const int base = held - n;                            // TREE: keys from here on are nodes
+        const int all_lo = TREE ? base - 1 : pos_lo;          // keys up to here are seen by every row, but for a window
 
         // ---- keys and values: fragments straight from the pages
         const int32_t* table = c.table + int64_t(s) * c.table_stride;
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
         uint32_t qf[NT][kSteps][2];
         float qscale[NT][TL::kLaneRows];  // of this lane's score columns: scale * the row's power of two (* log2 e without a cap)
         int qpos[NT][TL::kLaneRows];
+        [[maybe_unused]] int qrow[TREE ? NT : 1][TL::kLaneRows];  // TREE: their rows of the masks
         float slope[NT][TL::kLaneRows];
         const float unit = a.softcap > 0.0f ? a.scale : a.scale * kLog2e;
 #pragma unroll
@@ -358,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             for (int y = 0; y < TL::kLaneRows; y++) {
                 const int rr = HILO ? t : 2 * t + y, r2 = nt * TL::kRowsPer + rr, rt = over_g(r0 + r2);
                 qscale[nt][y] = __shfl_sync(0xffffffffu, down, (HILO ? 2 * rr : rr) * 4);
-                qpos[nt][y] = r2 < rows ? held - n + rt : kNoRow;
+                qpos[nt][y] = r2 < rows ? base + (TREE ? tree_depth(tr, row0, rt, n) : rt) : kNoRow;
+                if constexpr (TREE) qrow[nt][y] = row0 + rt;
                 slope[nt][y] = a.slopes && r2 < rows ? a.slopes[kvh * G + r0 + r2 - rt * G] * kLog2e : 0.0f;
             }
         }
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
             if (page >= 0) load_k(page, j1);
             // ---- scale, cap, bias, masks
             // open: every key of the group is seen by every row of the tile
-            const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= pos_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
+            const bool open = (j0 + 16 <= prefix) || (j0 + 15 <= all_lo && j0 + 16 <= len && (!a.window || pos_hi - j0 < a.window));
             uint32_t seen_bits = 0;  // per lane: (nt, row, key) -> seen
             float z[NT][TL::kLaneRows][2];
 #pragma unroll
@@ -441,26 +446,41 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
                             z[nt][r][h] = a.softcap * kLog2e * (small || fabsf(y) <= 0.5f ? tanh_small(y) : tanh_abs(y));
                         }
             }
+            int kpos[2] = {j0 + g, j0 + g + 8};  // positions of this lane's keys
+            if constexpr (TREE) {
+                if (tr.depth && j0 + 16 > base) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (kpos[h] >= base && kpos[h] < len) kpos[h] = base + tree_depth(tr, row0, kpos[h] - base, n);
+                }
+            }
             if (a.slopes) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int r = 0; r < TL::kLaneRows; r++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) z[nt][r][h] = fmaf(slope[nt][r], float(j0 + g + 8 * h - qpos[nt][r]), z[nt][r][h]);
+                        for (int h = 0; h < 2; h++) z[nt][r][h] = fmaf(slope[nt][r], float(kpos[h] - qpos[nt][r]), z[nt][r][h]);
             }
             if (!open) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int r = 0; r < TL::kLaneRows; r++)
+                    for (int r = 0; r < TL::kLaneRows; r++) {
+                        // of the masks: bit g + 8 h says whether key j0 + g + 8 h is seen
+                        [[maybe_unused]] uint32_t nodes = 0;
+                        if constexpr (TREE)
+                            if (qpos[nt][r] != kNoRow && j0 + 16 > base) nodes = tree_bits(tr, qrow[nt][r], j0 - base);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const int j = j0 + g + 8 * h, at = qpos[nt][r];
-                            const bool see = (j < len && j <= at && (!a.window || at - j < a.window)) || (j < prefix && at != kNoRow);
+                            bool see = (j < len && j <= at && (!a.window || at - j < a.window)) || (j < prefix && at != kNoRow);
+                            if constexpr (TREE)
+                                see = at != kNoRow && j < len && (j < base || (nodes >> (g + 8 * h) & 1u)) && (!a.window || at - kpos[h] < a.window);
                             if (see) seen_bits |= 1u << (nt * 4 + r * 2 + h);
                             else z[nt][r][h] = -INFINITY;
                         }
+                    }
             }
             // ---- running maxima (moved only by more than 2^kLazy: weights above 1 are as exact)
             const float lv = Q8 ? log2_scale(vs) : 0.0f;
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<HD, Q8, NT>) paged_decode_kern
     if constexpr (CL) {
         // ---- the warps' parts joined in each CTA, the CTAs' over distributed shared memory, in order
         cg::cluster_group cluster = cg::this_cluster();
-        const Span sp = span_of<TL::kRows>(a, plan, s, tile);
+        const Span sp = span_of<TL::kRows, TREE>(a, plan, s, tile);
         const int ranks = 1 << plan.ranks_log, rank = blockIdx.x & (ranks - 1);
         float* mine = reinterpret_cast<float*>(smb + TL::kPreOff);
         auto join = [&](int row, int d, int parts, auto part, float& top, float& sum, float& top_sum) {
@@ -815,8 +835,8 @@ int small_ranks(int64_t items, int64_t per_item, int64_t room) {
     return items * ranks <= room && per_item <= 64 * ranks ? ranks : 0;
 }
 
-template <int HD, bool Q8, bool HILO, int NT>
-cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
+template <int HD, bool Q8, bool HILO, int NT, bool TREE>
+cudaError_t go(const neko_paged_attention_args& a, const neko_tree& tr, cudaStream_t st) {
     using TL = Tile<HD, HILO, NT>;
     const neko_paged_cache& c = a.cache;
     DecodePlan p;
@@ -836,7 +856,7 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
     const int ctas = int(std::max<int64_t>(1, std::min({room, std::max(groups, items) / kWarps, 16 * room / row_tiles})));
     const size_t part_bytes = size_t(row_tiles) * ctas * 2 * TL::kState * 4, desc_bytes = size_t(row_tiles) * ctas * sizeof(int4);
     if (const int ranks = c.n_kv <= 65535 ? small_ranks(items * row_tiles, per_item, room) : 0) {
-        auto* small = paged_decode_kernel<HD, Q8, HILO, NT, true>;
+        auto* small = paged_decode_kernel<HD, Q8, HILO, NT, true, TREE>;
         if (cudaError_t e = ensure_dyn_smem(small, TL::smem_small()); e != cudaSuccess) return e;
         p.ranks_log = 31 - __builtin_clz(ranks);
         p.part = nullptr, p.desc = nullptr;
@@ -851,34 +871,44 @@ cudaError_t go(const neko_paged_attention_args& a, cudaStream_t st) {
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = ranks > 1 ? 1 : 0;
-        return cudaLaunchKernelEx(&cfg, small, a, p);
+        return cudaLaunchKernelEx(&cfg, small, a, p, tr);
     }
-    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, false>;
+    auto* fn = paged_decode_kernel<HD, Q8, HILO, NT, false, TREE>;
     const size_t smem = TL::smem(c.n_seq);
     cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;
     if (ctas == 1) {  // nothing is shared
         p.part = nullptr, p.desc = nullptr;
         for (int64_t left = row_tiles; left > 0 && e == cudaSuccess; left -= 65535, p.tile0 += 65535)
-            e = launch_ex(fn, dim3(1, unsigned(std::min<int64_t>(left, 65535))), dim3(kThreads), smem, st, false, a, p);
+            e = launch_ex(fn, dim3(1, unsigned(std::min<int64_t>(left, 65535))), dim3(kThreads), smem, st, false, a, p, tr);
         return e;
     }
     void* mem = nullptr;
     if ((e = scratch_alloc(&mem, part_bytes + desc_bytes, st)) != cudaSuccess) return e;
     p.part = static_cast<float*>(mem);
     p.desc = reinterpret_cast<int4*>(static_cast<char*>(mem) + part_bytes);
-    e = launch_ex(fn, dim3(unsigned(ctas), unsigned(row_tiles)), dim3(kThreads), smem, st, false, a, p);
+    e = launch_ex(fn, dim3(unsigned(ctas), unsigned(row_tiles)), dim3(kThreads), smem, st, false, a, p, tr);
     if (e == cudaSuccess)
         e = launch_ex(paged_join_kernel<HD, HILO, NT>, dim3(unsigned(ctas), unsigned(row_tiles)), dim3(128), 0, st, true, a, p, ctas);
     cudaFreeAsync(mem, st);
     return e;
 }
 
-template <int HD, bool Q8>
-cudaError_t by_rows(const neko_paged_attention_args& a, cudaStream_t st) {
+template <int HD, bool Q8, bool TREE>
+cudaError_t by_rows(const neko_paged_attention_args& a, const neko_tree& tr, cudaStream_t st) {
     const int64_t rows = int64_t(a.max_new) * (a.n_head / a.cache.n_kv);
-    if (a.type == NEKO_T_F32) return rows <= 4 ? go<HD, Q8, true, 1>(a, st) : go<HD, Q8, true, 2>(a, st);
-    return rows <= 8 ? go<HD, Q8, false, 1>(a, st) : go<HD, Q8, false, 2>(a, st);
+    if (a.type == NEKO_T_F32) return rows <= 4 ? go<HD, Q8, true, 1, TREE>(a, tr, st) : go<HD, Q8, true, 2, TREE>(a, tr, st);
+    return rows <= 8 ? go<HD, Q8, false, 1, TREE>(a, tr, st) : go<HD, Q8, false, 2, TREE>(a, tr, st);
+}
+
+template <bool TREE>
+cudaError_t by_cache(const neko_paged_attention_args& a, const neko_tree& tr, cudaStream_t st) {
+    const bool q8 = a.cache.type == NEKO_T_E4M3;
+    switch (a.cache.head_dim) {
+        case 32: return q8 ? by_rows<32, true, TREE>(a, tr, st) : by_rows<32, false, TREE>(a, tr, st);
+        case 64: return q8 ? by_rows<64, true, TREE>(a, tr, st) : by_rows<64, false, TREE>(a, tr, st);
+        default: return q8 ? by_rows<128, true, TREE>(a, tr, st) : by_rows<128, false, TREE>(a, tr, st);
+    }
 }
 
 // Whether a row tile each of more items than SMs costs the tensor cores' kernel, which runs one CTA per SM, more in CTA starts
@@ -896,7 +926,7 @@ bool starts(int64_t items, int64_t rows, int64_t per_item, bool f32) {
 
 }  // namespace
 
-cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStream_t st) {
+cudaError_t launch_paged_attention(const neko_paged_attention_args& a, const neko_tree* tree, cudaStream_t st) {
     // Rows past 16 go to the tensor cores' kernel (8 x 4,000 f16 keys, f32 rows: 16 rows 61 us each way, 20 rows 62 against 90),
     // but not where this one's small variant takes them (64 rows on 600 keys: 12 us against 22) nor up to 32 rows on many 8-bit
     // keys, which that one would convert for few rows (48 x 2,000 keys: 252 us against 316, 16-bit rows 139 against 277; of fewer
@@ -908,14 +938,9 @@ cudaError_t launch_paged_attention(const neko_paged_attention_args& a, cudaStrea
         const bool many = c.type == NEKO_T_E4M3 && rows <= 2 * kPromptRows && items * per_item >= 8192;
         if (!many && !small_ranks(items * ((rows + tile - 1) / tile), per_item, num_sms()) &&
             !starts(items, rows, per_item, a.type == NEKO_T_F32))
-            return launch_paged_prompt(a, st);
+            return launch_paged_prompt(a, tree, st);
     }
-    const bool q8 = a.cache.type == NEKO_T_E4M3;
-    switch (a.cache.head_dim) {
-        case 32: return q8 ? by_rows<32, true>(a, st) : by_rows<32, false>(a, st);
-        case 64: return q8 ? by_rows<64, true>(a, st) : by_rows<64, false>(a, st);
-        default: return q8 ? by_rows<128, true>(a, st) : by_rows<128, false>(a, st);
-    }
+    return tree ? by_cache<true>(a, *tree, st) : by_cache<false>(a, neko_tree{}, st);
 }
 
 }  // namespace neko

@@ -1,0 +1,169 @@
+// Moving what a paged cache holds, in all its planes (keys and values of every layer) by one launch: whole pages
+// (neko_op_paged_copy) and tokens of a sequence (neko_op_paged_compact).
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace neko {
+
+namespace {
+
+constexpr int kCopyThreads = 256, kPieces = 4;  // 16-byte pieces that a thread has in flight
+
+// A CTA for each 16 KB of a page and plane: bound by memory, every thread's loads come before its stores.
+__global__ void __launch_bounds__(kCopyThreads) paged_copy_kernel(const neko_paged_planes c, const int32_t* __restrict__ src,
+                                                                 const int32_t* __restrict__ dst, int chunks, int pieces, int size) {
+    const int pair = blockIdx.x / chunks, chunk = blockIdx.x % chunks, plane = blockIdx.y;
+    const int from = src[pair], to = dst[pair];
+    if (from < 0 || from >= c.num_pages || to < 0 || to >= c.num_pages || from == to) return;
+    uint8_t* base = static_cast<uint8_t*>(c.pages) + plane * c.plane_stride * size;
+    const uint4* s = reinterpret_cast<const uint4*>(base + from * c.page_stride * size);
+    uint4* d = reinterpret_cast<uint4*>(base + to * c.page_stride * size);
+    const int i0 = chunk * kCopyThreads * kPieces + threadIdx.x;
+    uint4 v[kPieces];
+#pragma unroll
+    for (int k = 0; k < kPieces; k++)
+        if (i0 + k * kCopyThreads < pieces) v[k] = s[i0 + k * kCopyThreads];
+#pragma unroll
+    for (int k = 0; k < kPieces; k++)
+        if (i0 + k * kCopyThreads < pieces) d[i0 + k * kCopyThreads] = v[k];
+    if (c.type == kTE4M3 && chunk == 0) {
+        float* scale = c.scale + plane * c.scale_plane;
+        for (int h = threadIdx.x; h < c.n_kv; h += kCopyThreads) scale[to * c.scale_stride + h] = scale[from * c.scale_stride + h];
+    }
+}
+
+// Codes times a ratio of scales, four at a time.
+__device__ __forceinline__ uint32_t recode4(uint32_t v, float ratio) {
+    const uint32_t f0 = e4m3x2_to_f16x2(uint16_t(v)), f1 = e4m3x2_to_f16x2(uint16_t(v >> 16));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f0)), b = __half22float2(*reinterpret_cast<const __half2*>(&f1));
+    return uint32_t(f32x2_to_e4m3x2(a.x * ratio, a.y * ratio)) | uint32_t(f32x2_to_e4m3x2(b.x * ratio, b.y * ratio)) << 16;
+}
+__device__ __forceinline__ uint4 recode16(uint4 v, float ratio) {
+    if (ratio == 1.0f) return v;
+    return make_uint4(recode4(v.x, ratio), recode4(v.y, ratio), recode4(v.z, ratio), recode4(v.w, ratio));
+}
+
+// A warp for each (sequence, head, plane). Paths ascend, so no token goes to a later place than it comes from, and none that is
+// still to be read has been written over: a group of tokens is read into registers, then written, then the next. 8-bit: one
+// target page after the other, for its scale is that of all the tokens that end in it; those come from it or from later pages, whose
+// scales are still the old ones.
+constexpr int kWarps = 4, kBatch = 4;
+template <int HD, bool Q8>
+__global__ void __launch_bounds__(32 * kWarps) paged_compact_kernel(const neko_paged_planes c, const int32_t* __restrict__ start_of,
+                                                                  const int32_t* __restrict__ path_of, int64_t path_stride,
+                                                                  const int32_t* __restrict__ count_of, int max_count, int page_log) {
+    constexpr int kRow = HD * (Q8 ? 1 : 2), kLanes = kRow / 16, kPer = 32 / kLanes;  // bytes of a token, lanes, tokens of a group's step
+    const int lane = threadIdx.x & 31, head = blockIdx.y * kWarps + (threadIdx.x >> 5), s = blockIdx.x, plane = blockIdx.z;
+    if (head >= c.n_kv) return;
+    const int32_t* path = path_of + int64_t(s) * path_stride;
+    const int start = min(start_of[s], 1 << 30), count = count_of[s];
+    if (count > max_count) {
+        if (lane == 0) set_op_error(kErrBadIndex);
+        return;
+    }
+    if (start < 0 || count <= 0) return;
+    const int32_t* table = c.table + int64_t(s) * c.table_stride;
+    const int in_page = (1 << page_log) - 1;
+    uint8_t* pool = static_cast<uint8_t*>(c.pages) + (plane * c.plane_stride + (int64_t(head) << page_log) * HD) * (Q8 ? 1 : 2);
+    float* scales = Q8 ? c.scale + plane * c.scale_plane + head : nullptr;
+    auto page_at = [&](int pos) {
+        const int slot = pos >> page_log;
+        const int p = pos >= 0 && slot < c.max_pages ? table[slot] : -1;
+        return p < c.num_pages ? p : -1;
+    };
+    auto row_at = [&](int page, int pos) { return pool + page * c.page_stride * (Q8 ? 1 : 2) + (pos & in_page) * kRow; };
+    // where token k comes from; -1: nowhere
+    auto source_of = [&](int k) {
+        const int x = path[k];
+        return x >= 0 && x <= (1 << 30) ? start + x : -1;
+    };
+    for (int k0 = 0; k0 < count;) {
+        // tokens of one target page
+        const int k1 = min(count, k0 + (in_page + 1) - ((start + k0) & in_page));
+        const int to_page = page_at(start + k0);
+        [[maybe_unused]] float scale = 0.0f;
+        if constexpr (Q8) {
+            if (to_page >= 0) {
+                const int stay = k0 == 0 ? start & in_page : 0;  // tokens of this page before the moved ones
+                const float old = scales[to_page * c.scale_stride];
+                if (stay) scale = old;
+                bool any = stay;
+                for (int k = k0 + lane; k < k1; k += 32) {
+                    const int page = page_at(source_of(k));
+                    if (page >= 0) scale = fmaxf(scale, scales[page * c.scale_stride]), any = true;
+                }
+                scale = warp_max(scale);
+                any = __any_sync(0xffffffffu, any);
+                if (any && stay && scale > old) {
+                    uint4* w = reinterpret_cast<uint4*>(row_at(to_page, 0));
+                    for (int i = lane; i < stay * kLanes; i += 32) w[i] = recode16(w[i], old / scale);
+                }
+                if (!any) scale = old;
+            }
+        }
+        if (to_page >= 0) {
+            for (int k = k0; k < k1; k += kPer * kBatch) {
+                uint4 v[kBatch];
+                uint8_t* to[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; b++) {
+                    const int kk = k + b * kPer + lane / kLanes;
+                    to[b] = nullptr;
+                    if (kk >= k1) continue;
+                    const int from = source_of(kk), page = page_at(from);
+                    if (page < 0) continue;
+                    float ratio = 1.0f;
+                    if constexpr (Q8) {
+                        const float x = scales[page * c.scale_stride];
+                        if (x < scale) ratio = x / scale;
+                    }
+                    if (from == start + kk && ratio == 1.0f) continue;
+                    v[b] = *reinterpret_cast<const uint4*>(row_at(page, from) + lane % kLanes * 16);
+                    if constexpr (Q8) v[b] = recode16(v[b], ratio);
+                    to[b] = row_at(to_page, start + kk) + lane % kLanes * 16;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int b = 0; b < kBatch; b++)
+                    if (to[b]) *reinterpret_cast<uint4*>(to[b]) = v[b];
+                __syncwarp();
+            }
+            if constexpr (Q8) {
+                __syncwarp();
+                if (lane == 0) scales[to_page * c.scale_stride] = scale;
+                __syncwarp();
+            }
+        }
+        k0 = k1;
+    }
+}
+
+template <int HD>
+cudaError_t go(const neko_paged_planes& c, const int32_t* start, const int32_t* path, int64_t path_stride, const int32_t* count, int max_count,
+               cudaStream_t st) {
+    const dim3 grid(unsigned(c.n_seq), unsigned(c.n_kv + kWarps - 1) / kWarps, unsigned(c.planes));
+    auto* fn = c.type == NEKO_T_E4M3 ? paged_compact_kernel<HD, true> : paged_compact_kernel<HD, false>;
+    return launch_ex(fn, grid, dim3(32 * kWarps), 0, st, false, c, start, path, path_stride, count, max_count, 31 - __builtin_clz(c.page_size));
+}
+
+}  // namespace
+
+cudaError_t launch_paged_copy(const neko_paged_planes& c, const int32_t* src, const int32_t* dst, int n, cudaStream_t st) {
+    const int size = c.type == NEKO_T_E4M3 ? 1 : 2;
+    const int64_t pieces = int64_t(c.n_kv) * c.page_size * c.head_dim * size / 16, chunks = (pieces + kCopyThreads * kPieces - 1) / (kCopyThreads * kPieces);
+    if (chunks * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    return launch_ex(paged_copy_kernel, dim3(unsigned(chunks * n), unsigned(c.planes)), dim3(kCopyThreads), 0, st, false, c, src, dst, int(chunks),
+                     int(pieces), size);
+}
+
+cudaError_t launch_paged_compact(const neko_paged_planes& c, const int32_t* start, const int32_t* path, int64_t path_stride,
+                                 const int32_t* count, int max_count, cudaStream_t st) {
+    switch (c.head_dim) {
+        case 32: return go<32>(c, start, path, path_stride, count, max_count, st);
+        case 64: return go<64>(c, start, path, path_stride, count, max_count, st);
+        default: return go<128>(c, start, path, path_stride, count, max_count, st);
+    }
+}
+
+}  // namespace neko

@@ -236,10 +236,10 @@ __device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-template <int HD, int SRC, bool HILO>
+template <int HD, int SRC, bool HILO, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_paged_attention_args a,
                                                                   const PromptPlan plan,
-                                                                  const __grid_constant__ PromptMaps maps) {
+                                                                  const __grid_constant__ PromptMaps maps, const neko_tree tr) {
     constexpr bool kScaled = SRC != kF16Pages, kConvert = SRC == kCodes;
     using L = PL<HD, HILO>;
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -273,7 +273,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     const int rows = min(n * G - r0, plan.tiles_per * kRows);
     if (rows <= 0) return;
     const int mt = rows > kRows ? 2 : 1;
-    const int pos_lo = held - n + over_g(r0), pos_hi = held - n + over_g(r0 + rows - 1);
+    const int base = held - n;  // TREE: keys from here on are nodes
+    const int pos_lo = TREE ? base : base + over_g(r0), pos_hi = TREE ? held - 1 : base + over_g(r0 + rows - 1);
+    const int all_lo = TREE ? base - 1 : pos_lo;  // keys up to here are seen by every row, but for a window
     const int prefix = a.prefix ? min(max(a.prefix[s], 0), len) : 0;
     const int hi = max(min(len, pos_hi + 1), 0);
     const int lo = a.window && pos_lo >= a.window ? min(pos_lo - a.window + 1, hi) : 0;
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     // every loader thread is past item x - kStages (the wait above), so none has touched tile i + 2's yet
                     if (lt >= 32 && lt < 36) ms.odd[(i + 2) % kOddRing][lt - 32] = 0;
                     if (i + 1 < nt) pages_next = pages_of(key_of(i + 1));
-                } else if (!open(key_of(i), pos_lo, pos_hi)) {  // values that are not numbers leave the operand
+                } else if (!open(key_of(i), all_lo, pos_hi)) {  // values that are not numbers leave the operand
 #pragma unroll
                     for (int y = 0; y < kPer; y++) {
                         uint32_t* w = reinterpret_cast<uint32_t*>(&got[y]);
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                 const bool v = x & 1;
                 const int j0 = key_of(i);
                 uint8_t* base = sm + L::kStageOff + st * L::kStage;
-                const bool strict = !open(j0, pos_lo, pos_hi);
+                const bool strict = !open(j0, all_lo, pos_hi);
                 const bool whole = __all_sync(0xffffffffu, lane >= 8 || pages >= 0), scan = v && (strict || !whole);
                 if (warp == kLoadWarp) {
                     if (x >= L::kStages) {
@@ -656,9 +658,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + h * 128, to = tmem + lanes + 256 + h * 128 + col_w * (HD / 2);
         const bool real = r < rows;
-        const int rt = over_g(pr), qpos = real ? held - n + rt : kNoRow;
+        const int rt = over_g(pr), qpos = real ? base + (TREE ? tree_depth(tr, row0, rt, n) : rt) : kNoRow;
         const float slope = a.slopes && real ? a.slopes[kvh * G + pr - rt * G] * kLog2e : 0.0f;
-        const int h_lo = held - n + over_g(r0 + h * kRows), h_hi = held - n + over_g(r0 + min(rows, (h + 1) * kRows) - 1);
+        const int h_lo = TREE ? all_lo : base + over_g(r0 + h * kRows), h_hi = TREE ? pos_hi : base + over_g(r0 + min(rows, (h + 1) * kRows) - 1);
+        // position of a key
+        auto pos_of = [&](int j) { return TREE && tr.depth && j >= base && j < len ? base + tree_depth(tr, row0, j - base, n) : j; };
         const float cap = a.softcap * kLog2e;
         {
             uint32_t z[32];
@@ -680,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
         meet();  // both threads of a row have read its factor before either writes
         for (int i = 0; i < nt; i++) {
             const int j0 = key_of(i);
-            const bool open_rows = open(j0, h_lo, h_hi), open_cta = open(j0, pos_lo, pos_hi);
+            const bool open_rows = open(j0, h_lo, h_hi), open_cta = open(j0, all_lo, pos_hi);
             const float* ksp = ms.ks[i % kRing];
             const float* vsp = ms.vs[i % kRing];
             wait_on(&ms.s_full[h], i & 1, fail);
@@ -744,7 +748,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                             if (!(ms.odd[i % kOddRing][key >> 5] >> (key & 31) & 1)) continue;
                             const int j = j0 + key, slot = j / c.page_size;
                             if (j >= len || ksp[key >> 4] == kGone) continue;
-                            const bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
+                            bool see = (j <= qpos && (!a.window || qpos - j < a.window)) || (j < prefix && qpos != kNoRow);
+                            if constexpr (TREE)
+                                see = real && (j < base || (tree_bits(tr, row0 + rt, j - base) & 1u)) && (!a.window || qpos - pos_of(j) < a.window);
                             const int64_t at = int64_t(c.table[int64_t(s) * c.table_stride + slot]) * c.page_stride +
                                                (int64_t(kvh) * c.page_size + j % c.page_size) * HD + col_w * (HD / 2) + x;
 #pragma unroll
@@ -810,16 +816,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
                     }
                     if (a.slopes) {
 #pragma unroll
-                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(fmaf(slope, float(jq + x - qpos), __uint_as_float(u[x])));
+                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(fmaf(slope, float((TREE ? pos_of(jq + x) : jq + x) - qpos), __uint_as_float(u[x])));
                     }
                     if (!plain_mask) {
                         // seen: j in [see_lo, see_hi) or j < pre, and the block is resident
                         const int see_hi = min(len, qpos + 1) - jq, see_lo = (a.window && qpos >= a.window ? qpos - a.window + 1 : 0) - jq;
                         const int pre = (real ? prefix : 0) - jq;
                         const bool gone0 = kb[2 * q] == kGone, gone1 = kb[2 * q + 1] == kGone;
+                        if constexpr (TREE) {
+                            // seen: the cached keys in the window, the nodes of this row's mask in it, if the block is resident
+                            const int nodes_at = base - jq, end = len - jq;
+                            uint32_t bits = real && nodes_at < 32 ? tree_bits(tr, row0 + rt, -nodes_at) : 0u;
+                            if (real && nodes_at > 0) bits |= nodes_at >= 32 ? 0xffffffffu : (1u << nodes_at) - 1u;
+                            if (end < 32) bits &= end > 0 ? (1u << end) - 1u : 0u;
+                            if (gone0) bits &= 0xffff0000u;
+                            if (gone1) bits &= 0xffffu;
 #pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (!((x < see_hi && x >= see_lo) || x < pre) || (x < 16 ? gone0 : gone1)) u[x] = 0xff800000u;
+                            for (int x = 0; x < 32; x++)
+                                if (!(bits >> x & 1u) || (a.window && qpos - pos_of(jq + x) >= a.window)) u[x] = 0xff800000u;
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 32; x++)
+                                if (!((x < see_hi && x >= see_lo) || x < pre) || (x < 16 ? gone0 : gone1)) u[x] = 0xff800000u;
+                        }
                     }
                     st32(tc + 32 * q, u);
                 }
@@ -1044,11 +1063,11 @@ __global__ void __launch_bounds__(256) paged_copies_kernel(const neko_paged_atte
     }
 }
 
-template <int HD, int SRC, bool HILO>
-cudaError_t go(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, const __half* copies, cudaStream_t st) {
+template <int HD, int SRC, bool HILO, bool TREE>
+cudaError_t go(const neko_paged_attention_args& a, const neko_tree& tr, const PromptPlan& p, int64_t items, const __half* copies, cudaStream_t st) {
     using L = PL<HD, HILO>;
     const neko_paged_cache& c = a.cache;
-    auto* fn = paged_prompt_kernel<HD, SRC, HILO>;
+    auto* fn = paged_prompt_kernel<HD, SRC, HILO, TREE>;
     if (cudaError_t e = ensure_dyn_smem(fn, L::kSmem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(items * p.ranks));
@@ -1069,32 +1088,35 @@ cudaError_t go(const neko_paged_attention_args& a, const PromptPlan& p, int64_t 
             !encode_f16_pages(&maps.v, copy ? copies + pages * own : c.v_pages, HD, rows, copy ? pages : c.num_pages, (copy ? own : c.page_stride) * 2, c.page_size))
             return cudaErrorNotSupported;
     }
-    return cudaLaunchKernelEx(&cfg, fn, a, p, maps);
+    return cudaLaunchKernelEx(&cfg, fn, a, p, maps, tr);
 }
 
 template <int HD, int SRC>
-cudaError_t by_type(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, const __half* copies, cudaStream_t st) {
-    return a.type == NEKO_T_F32 ? go<HD, SRC, true>(a, p, items, copies, st) : go<HD, SRC, false>(a, p, items, copies, st);
+cudaError_t by_type(const neko_paged_attention_args& a, const neko_tree* tree, const PromptPlan& p, int64_t items, const __half* copies,
+                    cudaStream_t st) {
+    const bool f32 = a.type == NEKO_T_F32;
+    if (tree) return f32 ? go<HD, SRC, true, true>(a, *tree, p, items, copies, st) : go<HD, SRC, false, true>(a, *tree, p, items, copies, st);
+    return f32 ? go<HD, SRC, true, false>(a, {}, p, items, copies, st) : go<HD, SRC, false, false>(a, {}, p, items, copies, st);
 }
 
 template <int HD>
-cudaError_t by_pages(const neko_paged_attention_args& a, const PromptPlan& p, int64_t items, cudaStream_t st) {
+cudaError_t by_pages(const neko_paged_attention_args& a, const neko_tree* tree, const PromptPlan& p, int64_t items, cudaStream_t st) {
     const neko_paged_cache& c = a.cache;
-    if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, p, items, nullptr, st);
+    if (c.type != NEKO_T_E4M3) return by_type<HD, kF16Pages>(a, tree, p, items, nullptr, st);
     // Each CTA would convert its keys again: from kCopyTiles CTAs per (sequence, KV head) on, they are converted once,
     // if the copies stay below kCopyBytes. Not copied and copied, f32 rows: 2 CTAs each (8 x 2,048 keys, 256 tokens) 128 and
     // 113 us, (4 x 8,192) 238 and 201; 6 each (1 x 8,192, 768 tokens) 349 and 239. One each gains less (16 x 4,096 keys,
     // 128 tokens: 256 and 238), for copies that are twice the cache.
     const int64_t bytes = 2 * int64_t(c.n_seq) * c.max_pages * c.n_kv * c.page_size * HD * 2;
-    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes) return by_type<HD, kCodes>(a, p, items, nullptr, st);
+    if (p.row_tiles < kCopyTiles || bytes > kCopyBytes) return by_type<HD, kCodes>(a, tree, p, items, nullptr, st);
     void* mem = nullptr;
     if (scratch_alloc(&mem, size_t(bytes), st) != cudaSuccess) {  // a cache that fills the GPU: every CTA converts its own
         cudaGetLastError();
-        return by_type<HD, kCodes>(a, p, items, nullptr, st);
+        return by_type<HD, kCodes>(a, tree, p, items, nullptr, st);
     }
     cudaError_t e = launch_ex(paged_copies_kernel, dim3(unsigned(c.max_pages), unsigned(c.n_seq), 2), dim3(256), 0, st, false, a,
                               static_cast<uint4*>(mem));
-    if (e == cudaSuccess) e = by_type<HD, kCopies>(a, p, items, static_cast<const __half*>(mem), st);
+    if (e == cudaSuccess) e = by_type<HD, kCopies>(a, tree, p, items, static_cast<const __half*>(mem), st);
     cudaFreeAsync(mem, st);
     return e;
 }
@@ -1110,7 +1132,7 @@ int clusters_at_once(int log) {
     if (const int n = slot.load(std::memory_order_relaxed)) return n;
     int n = num_sms();
     if (log > 0) {
-        auto* fn = paged_prompt_kernel<HD, kCodes, true>;
+        auto* fn = paged_prompt_kernel<HD, kCodes, true, false>;
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1153,7 +1175,7 @@ int64_t split(PromptPlan& p, int64_t tiles, int64_t heads, int64_t key_tiles, bo
 }
 
 template <int HD>
-cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
+cudaError_t by_source(const neko_paged_attention_args& a, const neko_tree* tree, cudaStream_t st) {
     const neko_paged_cache& c = a.cache;
     const int64_t rows = int64_t(a.max_new) * (a.n_head / c.n_kv);
     PromptPlan p;
@@ -1178,15 +1200,15 @@ cudaError_t by_source(const neko_paged_attention_args& a, cudaStream_t st) {
             }
         }
     }
-    const cudaError_t e = by_pages<HD>(a, p, items, st);
+    const cudaError_t e = by_pages<HD>(a, tree, p, items, st);
     if (flush) cudaFreeAsync(flush, st);
     return e;
 }
 
 }  // namespace
 
-cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, cudaStream_t st) {
-    return a.cache.head_dim == 64 ? by_source<64>(a, st) : by_source<128>(a, st);
+cudaError_t launch_paged_prompt(const neko_paged_attention_args& a, const neko_tree* tree, cudaStream_t st) {
+    return a.cache.head_dim == 64 ? by_source<64>(a, tree, st) : by_source<128>(a, tree, st);
 }
 
 }  // namespace neko

@@ -1,0 +1,97 @@
+// Bookkeeping of trees of drafted tokens (neko_op_tree_masks, neko_op_tree_accept): a CTA for each sequence, its nodes in shared
+// memory. Both are bound by latency: a chain of dependent reads as long as the tree is deep, in shared memory instead of L2.
+#include "paged.cuh"
+
+namespace neko {
+
+namespace {
+
+constexpr int kThreads = 128;
+
+// The sequence's nodes: its first row and how many; false: none, or rows that are not there (reported).
+__device__ __forceinline__ bool nodes_of(const int32_t* q_start, int s, int tokens, int max_new, int& row0, int& n) {
+    row0 = q_start[s], n = q_start[s + 1] - row0;
+    if (row0 < 0 || n < 0 || n > max_new || row0 > tokens - n) {
+        if (threadIdx.x == 0) set_op_error(kErrBadIndex);
+        n = -1;
+    }
+    return n > 0;
+}
+
+// A thread for each node walks up to the root. Parents come before their children, so the bits of the node's words come from the
+// last to the first: each word is written once, from a register.
+__global__ void __launch_bounds__(kThreads) tree_masks_kernel(const int32_t* __restrict__ parent, const int32_t* __restrict__ q_start, int tokens,
+                                                             int max_new, uint64_t* __restrict__ mask, int words, int32_t* __restrict__ depth) {
+    extern __shared__ int32_t up[];
+    int row0, n;
+    if (!nodes_of(q_start, blockIdx.x, tokens, max_new, row0, n)) return;
+    for (int i = threadIdx.x; i < n; i += kThreads) up[i] = parent[row0 + i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        uint64_t* out = mask ? mask + int64_t(row0 + i) * words : nullptr;
+        int w = words - 1, deep = -1;
+        uint64_t bits = 0;
+        for (int at = i;;) {
+            if (out)
+                for (; w > at >> 6; w--) out[w] = bits, bits = 0;
+            bits |= uint64_t(1) << (at & 63);
+            deep++;
+            const int p = up[at];
+            if (p < 0 || p >= at) break;
+            at = p;
+        }
+        if (out)
+            for (; w >= 0; w--) out[w] = bits, bits = 0;
+        if (depth) depth[row0 + i] = deep;
+    }
+}
+
+// Where each node leads is found for all nodes at once (the lowest child whose draft is the token chosen here); one thread walks.
+__global__ void __launch_bounds__(kThreads) tree_accept_kernel(const int32_t* __restrict__ chosen, const int32_t* __restrict__ draft,
+                                                              const int32_t* __restrict__ parent, const int32_t* __restrict__ q_start,
+                                                              int tokens, int max_new, int32_t* __restrict__ path, int32_t* __restrict__ count,
+                                                              int32_t* __restrict__ token) {
+    extern __shared__ int32_t next[];  // [max_new], then the path
+    int32_t* walk = next + max_new;
+    __shared__ int steps;
+    const int s = blockIdx.x;
+    int row0, n;
+    const bool any = nodes_of(q_start, s, tokens, max_new, row0, n);
+    if (n < 0) return;
+    for (int i = threadIdx.x; i < n; i += kThreads) next[i] = 0x7fffffff;
+    if (threadIdx.x == 0) steps = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int p = parent[row0 + i];
+        if (p >= 0 && p < i && draft[row0 + i] == chosen[row0 + p]) atomicMin(&next[p], i);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && any) {
+        int k = 0;
+        for (int at = 0; at < n; at = next[at]) walk[k++] = at;  // ascending: ends
+        steps = k;
+        token[s] = chosen[row0 + walk[k - 1]];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        count[s] = steps;
+        if (!any) token[s] = -1;
+    }
+    for (int k = threadIdx.x; k < max_new; k += kThreads) path[int64_t(s) * max_new + k] = k < steps ? walk[k] : 0;
+}
+
+}  // namespace
+
+cudaError_t launch_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
+                              int32_t* depth, cudaStream_t st) {
+    return launch_ex(tree_masks_kernel, dim3(n_seq), dim3(kThreads), size_t(max_new) * 4, st, false, parent, q_start, tokens, max_new, mask, words,
+                     depth);
+}
+
+cudaError_t launch_tree_accept(const int32_t* chosen, const int32_t* draft, const int32_t* parent, const int32_t* q_start, int n_seq,
+                               int tokens, int max_new, int32_t* path, int32_t* count, int32_t* token, cudaStream_t st) {
+    return launch_ex(tree_accept_kernel, dim3(n_seq), dim3(kThreads), size_t(max_new) * 8, st, false, chosen, draft, parent, q_start, tokens, max_new,
+                     path, count, token);
+}
+
+}  // namespace neko

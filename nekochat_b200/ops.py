@@ -146,6 +146,9 @@ def attention(q, q_stride, k_cache, v_cache, T, n_head, n_kv, hd, pos0):
 _CACHE = "5P3q8i"
 _APPEND = struct.Struct("@" + _CACHE + "4P8q5P7if")
 _ATTEND = struct.Struct("@" + _CACHE + "2P4q4P5i2fi")
+_TREE = struct.Struct("@2P2i")
+_PLANES = struct.Struct("@3P5q8i")
+_SAMPLE = struct.Struct("@8Pq4i3fi")
 _types = {}
 
 
@@ -155,7 +158,10 @@ def _setup():
     l = lib()
     _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3, torch.uint8: 3,
                    "f32": torch.float32, "i32": torch.int32, "append": l.neko_op_paged_append,
-                   "attend": l.neko_op_paged_attention, "device": torch.cuda.current_device,
+                   "attend": l.neko_op_paged_attention, "i64": torch.int64, "f64": torch.float64,
+                   "tree_append": l.neko_op_paged_tree_append, "tree_attend": l.neko_op_paged_tree_attention,
+                   "masks": l.neko_op_tree_masks, "accept": l.neko_op_tree_accept, "compact": l.neko_op_paged_compact,
+                   "copy": l.neko_op_paged_copy, "sample": l.neko_op_sample_rows, "device": torch.cuda.current_device,
                    "stream": getattr(torch._C, "_cuda_getCurrentRawStream", None) or
                    (lambda i: torch.cuda.current_stream(i).cuda_stream)})
     return _types
@@ -252,11 +258,12 @@ def rope_table(positions, rot, theta, scaling="none", factor=1.0, original=0, be
 
 
 def paged_append(k, v, k_pages, v_pages, table, start, k_scale=None, v_scale=None, q_start=None, max_new=1, q=None,
-                 cs=None, interleaved=False, q_gain=None, k_gain=None, eps=1e-6, q_out=None):
+                 cs=None, interleaved=False, q_gain=None, k_gain=None, eps=1e-6, q_out=None, depth=None):
     """neko_op_paged_append: k, v [tokens][kv heads][hd] (any token and head stride) go to the pages, after the
     per-head norm (k_gain) and the rotation by cs (rope_table) of k. Sequence s's rows are q_start[s] ..
     q_start[s + 1] - 1 (q_start None: row s) and go to positions start[s], start[s] + 1, ..; at most max_new per
-    sequence. Returns q with its norm (q_gain) and rotation applied (into q_out, which may be q; a new tensor when
+    sequence. depth [tokens] (neko_op_paged_tree_append): the new tokens are nodes of a tree, turned by start[s] + depth
+    instead of their places. Returns q with its norm (q_gain) and rotation applied (into q_out, which may be q; a new tensor when
     None), or None without q."""
     types = _types or _setup()
     fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table, types)
@@ -287,7 +294,10 @@ def paged_append(k, v, k_pages, v_pages, table, start, k_scale=None, v_scale=Non
                         _vector(q_gain, "paged_append q_gain", f32, hd, dev),
                         _vector(k_gain, "paged_append k_gain", f32, hd, dev),
                         types.get(dt, -1), tokens, heads, max_new, rot, rows, 1 if interleaved else 0, eps)
-    rc = types["append"](args, types["stream"](dev))
+    if depth is None:
+        rc = types["append"](args, types["stream"](dev))
+    else:
+        rc = types["tree_append"](args, _vector(depth, "paged_append depth", i32, tokens, dev), types["stream"](dev))
     if rc:
         check(rc, "paged_append")
     return q_out if q is not None else None
@@ -298,25 +308,185 @@ def paged_attention(q, k_pages, v_pages, table, kv_len, k_scale=None, v_scale=No
     """neko_op_paged_attention: q [tokens][heads][hd] over the cached keys and values; kv_len [sequences] counts the
     new tokens, which are in the cache already. scale: 1 / sqrt(hd) when None; softcap, window, slopes [heads] and
     prefix [sequences] as the header defines them. Returns out (shaped and typed like q)."""
+    return _attend("paged_attention", q, k_pages, v_pages, table, kv_len, k_scale, v_scale, q_start, max_new, scale, softcap,
+                   window, slopes, prefix, out)
+
+
+def _attend(what, q, k_pages, v_pages, table, kv_len, k_scale, v_scale, q_start, max_new, scale, softcap, window, slopes, prefix,
+            out, mask=None, depth=None):
     types = _types or _setup()
     fields, n_seq, n_kv, hd, dev = _cache(k_pages, v_pages, k_scale, v_scale, table, types)
     dt, shape = q.dtype, q.shape
     if len(shape) != 3 or shape[2] != hd:
-        raise NekoError("paged_attention q: [tokens][heads][head_dim] rows")
-    qp = _rows(q, "paged_attention q", dt, shape, dev)
+        raise NekoError(f"{what} q: [tokens][heads][head_dim] rows")
+    qp = _rows(q, what + " q", dt, shape, dev)
     if out is None:
         out = q.new_empty(shape)
-    op = _rows(out, "paged_attention out", dt, shape, dev)
+    op = _rows(out, what + " out", dt, shape, dev)
     i32 = types["i32"]
-    args = _ATTEND.pack(*fields, qp[0], op[0], *qp[1:], *op[1:], _vector(kv_len, "paged_attention kv_len", i32, n_seq, dev),
-                        _vector(q_start, "paged_attention q_start", i32, n_seq + 1, dev),
-                        _vector(slopes, "paged_attention slopes", types["f32"], shape[1], dev),
-                        _vector(prefix, "paged_attention prefix", i32, n_seq, dev), types.get(dt, -1), shape[0], shape[1],
+    args = _ATTEND.pack(*fields, qp[0], op[0], *qp[1:], *op[1:], _vector(kv_len, what + " kv_len", i32, n_seq, dev),
+                        _vector(q_start, what + " q_start", i32, n_seq + 1, dev),
+                        _vector(slopes, what + " slopes", types["f32"], shape[1], dev),
+                        _vector(prefix, what + " prefix", i32, n_seq, dev), types.get(dt, -1), shape[0], shape[1],
                         max_new, window, hd ** -0.5 if scale is None else scale, softcap, 0)
-    rc = types["attend"](args, types["stream"](dev))
+    if mask is None:
+        rc = types["attend"](args, types["stream"](dev))
+    else:
+        words = mask.shape[1] if mask.dim() == 2 else -1
+        tree = _TREE.pack(_vector(mask, what + " mask", types["i64"], shape[0] * words, dev),
+                          _vector(depth, what + " depth", i32, shape[0], dev), words, 0)
+        rc = types["tree_attend"](args, tree, types["stream"](dev))
     if rc:
-        check(rc, "paged_attention")
+        check(rc, what)
     return out
+
+
+# ------------------------------------------------------------------ drafted tokens
+def paged_tree_attention(q, k_pages, v_pages, table, kv_len, mask, depth=None, k_scale=None, v_scale=None, q_start=None,
+                         max_new=1, scale=None, softcap=0.0, window=0, slopes=None, out=None):
+    """neko_op_paged_tree_attention: paged_attention for the nodes of trees of drafted tokens, which are in the cache already:
+    each sees the keys before the tree and the nodes of its mask (int64 [tokens][words], 64 nodes a word, as tree_masks
+    gives it); positions (window, slopes) go by depth [tokens]. Returns out (shaped and typed like q)."""
+    return _attend("paged_tree_attention", q, k_pages, v_pages, table, kv_len, k_scale, v_scale, q_start, max_new, scale, softcap,
+                   window, slopes, None, out, mask, depth)
+
+
+def _on_device(t, what, types):
+    dev = t.get_device()
+    if dev < 0 or types["device"]() != dev:
+        raise NekoError(f"{what}: CUDA tensors on the current device")
+    return dev
+
+
+def tree_masks(parent, q_start, max_new):
+    """neko_op_tree_masks: parent int32 [tokens] (each node's parent, counted from its sequence's first node; no earlier node: a
+    root), sequence s's nodes at q_start[s] .. q_start[s + 1] - 1, at most max_new. Returns mask int64
+    [tokens][ceil(max_new / 64)] (bit j: node j is the node itself or an ancestor) and depth int32 [tokens]. Rows of no
+    sequence are zeros."""
+    import torch
+    types = _types or _setup()
+    dev, tokens, i32 = _on_device(parent, "tree_masks", types), parent.numel(), types["i32"]
+    n_seq, words = q_start.numel() - 1, max((max_new + 63) // 64, 1)
+    mask = torch.zeros((tokens, words), dtype=types["i64"], device=parent.device)
+    depth = torch.zeros(tokens, dtype=i32, device=parent.device)
+    rc = types["masks"](_vector(parent, "tree_masks parent", i32, tokens, dev), _vector(q_start, "tree_masks q_start", i32, n_seq + 1, dev),
+                        n_seq, tokens, max_new, mask.data_ptr(), words, depth.data_ptr(), types["stream"](dev))
+    if rc:
+        check(rc, "tree_masks")
+    return mask, depth
+
+
+def tree_accept(chosen, draft, parent, q_start, max_new):
+    """neko_op_tree_accept: walks each sequence's tree (parent, q_start, max_new as in tree_masks) from its node 0 to the lowest
+    child whose draft is the token chosen at the node, and so on; chosen, draft int32 [tokens]. Returns path int32
+    [sequences][max_new] (the nodes, then zeros), count int32 [sequences] and token int32 [sequences], the one chosen at the
+    last of them (a sequence without nodes: 0 and -1)."""
+    types = _types or _setup()
+    dev, tokens, i32 = _on_device(parent, "tree_accept", types), parent.numel(), types["i32"]
+    n_seq = q_start.numel() - 1
+    path, count, token = parent.new_empty((n_seq, max_new)), parent.new_empty(n_seq), parent.new_empty(n_seq)
+    rc = types["accept"](*(_vector(x, "tree_accept " + w, i32, tokens, dev) for x, w in ((chosen, "chosen"), (draft, "draft"), (parent, "parent"))),
+                         _vector(q_start, "tree_accept q_start", i32, n_seq + 1, dev), n_seq, tokens, max_new, path.data_ptr(),
+                         count.data_ptr(), token.data_ptr(), types["stream"](dev))
+    if rc:
+        check(rc, "tree_accept")
+    return path, count, token
+
+
+def _planes(pool, scale, table, what, types):
+    """The fields of neko_paged_planes and the device index; pool [..][pages][kv heads][page][hd], any uniform planes."""
+    dev, sh, st = _on_device(pool, what, types), pool.shape, pool.stride()
+    type_ = types.get(pool.dtype, -1)
+    if len(sh) < 4:
+        raise NekoError(f"{what}: the pool is [planes ..][pages][kv heads][page][head_dim]")
+    pages, n_kv, ps, hd = sh[-4:]
+    if st[-1] != 1 or st[-2] != hd or (st[-3] != ps * hd and n_kv > 1):
+        raise NekoError(f"{what}: a page is contiguous")
+
+    def uniform(shape, stride, name):
+        """Planes and their stride, leading dimensions taken together."""
+        n, step = 1, 0
+        for s, d in zip(reversed(shape), reversed(stride)):
+            if s == 1:
+                continue
+            if n > 1 and d != n * step:
+                raise NekoError(f"{what}: the {name}'s planes are not a constant step apart")
+            if n == 1:
+                step = d
+            n *= s
+        return n, step
+
+    planes, step = uniform(sh[:-4], st[:-4], "pool")
+    sp = plane = page = 0
+    if type_ == 3:
+        if scale is None or scale.dtype is not types["f32"] or scale.get_device() != dev or scale.shape != sh[:-2] or \
+                (n_kv > 1 and scale.stride(-1) != 1):
+            raise NekoError(f"{what}: 8-bit pages need scales float32 [planes ..][pages][kv heads]")
+        plane, page = uniform(sh[:-4], scale.stride()[:-2], "scales")[1], scale.stride(-2) if pages > 1 else n_kv
+        sp = scale.data_ptr()
+    n_seq = width = tp = ts = 0
+    if table is not None:
+        tsh, tst = table.shape, table.stride()
+        if len(tsh) != 2 or table.dtype is not types["i32"] or table.get_device() != dev or (tsh[1] > 1 and tst[1] != 1):
+            raise NekoError(f"{what}: the table is [sequences][pages] int32")
+        (n_seq, width), tp = tsh, table.data_ptr()
+        ts = tst[0] if n_seq > 1 else width
+    return _PLANES.pack(pool.data_ptr(), sp, tp, step, st[-4] if pages > 1 else n_kv * ps * hd, plane, page, ts, type_, planes,
+                        n_seq, width, pages, n_kv, ps, hd), n_seq, dev
+
+
+def paged_compact(pool, table, start, path, count, scale=None):
+    """neko_op_paged_compact: in every plane of pool [planes ..][pages][kv heads][page][hd] (scale [planes ..][pages][kv heads] with
+    8-bit pages), token start[s] + path[s][k] becomes token start[s] + k, k < count[s]: what tree_accept leaves of a tree. Paths
+    [sequences][width] int32 ascend."""
+    types = _types or _setup()
+    args, n_seq, dev = _planes(pool, scale, table, "paged_compact", types)
+    i32 = types["i32"]
+    if path.dtype is not i32 or path.dim() != 2 or path.shape[0] != n_seq or path.get_device() != dev or \
+            (path.shape[1] > 1 and path.stride(1) != 1):
+        raise NekoError("paged_compact path: int32 [sequences][width]")
+    width = path.shape[1]
+    rc = types["compact"](args, _vector(start, "paged_compact start", i32, n_seq, dev), path.data_ptr(),
+                          path.stride(0) if n_seq > 1 else width, _vector(count, "paged_compact count", i32, n_seq, dev), width,
+                          types["stream"](dev))
+    if rc:
+        check(rc, "paged_compact")
+
+
+def paged_copy(pool, src, dst, scale=None):
+    """neko_op_paged_copy: in every plane of pool (as in paged_compact), page dst[i] becomes a copy of page src[i] (int32)."""
+    types = _types or _setup()
+    args, _, dev = _planes(pool, scale, None, "paged_copy", types)
+    n = src.numel()
+    rc = types["copy"](args, _vector(src, "paged_copy src", types["i32"], n, dev), _vector(dst, "paged_copy dst", types["i32"], n, dev), n,
+                       types["stream"](dev))
+    if rc:
+        check(rc, "paged_copy")
+
+
+def sample_rows(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """neko_op_sample_rows: a token for each row of logits [rows][vocab] (float32, float16, bfloat16; any row stride; unchanged)
+    from u float64 [rows] in [0, 1) (None: greedy). temperature, top_k, top_p and min_p are numbers or tensors [rows] (float32,
+    top_k int32). Returns token int32 [rows] (-1: nothing to take) and prob float32 [rows], the one with which it was taken."""
+    import torch
+    types = _types or _setup()
+    dev = _on_device(logits, "sample_rows", types)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise NekoError("sample_rows: logits are [rows][vocab], the vocabulary contiguous")
+    (rows, vocab), is_tensor, each, one = logits.shape, torch.is_tensor, [], []
+    for v, what, dt in ((temperature, "temperature", "f32"), (top_p, "top_p", "f32"), (min_p, "min_p", "f32"), (top_k, "top_k", "i32")):
+        each.append(_vector(v, "sample_rows " + what, types[dt], rows, dev) if is_tensor(v) else 0)
+        one.append(0 if is_tensor(v) else v)
+    token, prob = logits.new_empty(rows, dtype=types["i32"]), logits.new_empty(rows, dtype=types["f32"])
+    if u is None and not each[0] and one[0] > 0:
+        raise NekoError("sample_rows: a positive temperature needs the rows' numbers u")
+    args = _SAMPLE.pack(logits.data_ptr(), _vector(u, "sample_rows u", types["f64"], rows, dev), *each, token.data_ptr(), prob.data_ptr(),
+                        logits.stride(0) if rows > 1 else vocab, types.get(logits.dtype, -1), rows, vocab, int(one[3]), one[0], one[1],
+                        one[2], 0)
+    rc = types["sample"](args, types["stream"](dev))
+    if rc:
+        check(rc, "sample_rows")
+    return token, prob
 
 
 def status():

@@ -319,7 +319,7 @@ int neko_op_paged_compact(const neko_paged_planes* planes, const int32_t* start,
  * their full pages and copy the one that is partly filled. */
 int neko_op_paged_copy(const neko_paged_planes* planes, const int32_t* src, const int32_t* dst, int n, void* stream);
 
-/* A token for each row of logits [rows][vocab] (row stride row_stride elements; not changed), from the row's number u in [0, 1):
+/* A token for each row of logits [rows][vocab] (rows row_stride elements apart, any number; not changed), from the row's number u in [0, 1):
  * weights w_i = exp((x_i - max x) / temperature); of the tokens in descending order of x (equal ones by index) the first top_k
  * (0 or less: all), of those the shortest beginning whose weights add up to top_p times all of theirs (1 or more: all; at least
  * one), of those the ones with w_i >= min_p (values above 1 count as 1). Among what is left, in the order of the vocabulary, the
@@ -328,7 +328,7 @@ int neko_op_paged_copy(const neko_paged_planes* planes, const int32_t* src, cons
  * Weights are held to 2^-45 of the largest and added as integers: the result depends on no order.
  * Each parameter is one number, or an array [rows] where its pointer is not NULL. prob (or NULL): w_token / total, 1 for
  * temperature 0. vocab at most NEKO_MAX_VOCAB. */
-#define NEKO_MAX_VOCAB 393216
+#define NEKO_MAX_VOCAB 262144
 typedef struct neko_sample_rows_args {
     const void* logits;     /* device; NEKO_T_F32, NEKO_T_F16, NEKO_T_BF16, aligned to its type */
     const double* u;        /* device [rows]; NULL: every row greedy */

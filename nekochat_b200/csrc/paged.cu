@@ -195,8 +195,7 @@ extern "C" int neko_op_sample_rows(const neko_sample_rows_args* a, void* stream)
     if (a->rows == 0) return NEKO_OK;
     if (!a->logits || !a->token) return paged_fail(NEKO_ERR_ARG, op, "null pointer");
     if (!aligned(a->logits, a->type == NEKO_T_F32 ? 4 : 2)) return paged_fail(NEKO_ERR_ARG, op, "logits must be aligned to their type");
-    if (a->rows > 1 && a->row_stride < a->vocab) return paged_fail(NEKO_ERR_ARG, op, "rows of logits overlap");
-    if (a->vocab > NEKO_MAX_VOCAB) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "a vocabulary of more than 393,216 tokens");
+    if (a->vocab > NEKO_MAX_VOCAB) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "a vocabulary of more than 262,144 tokens");
     if (a->rows > (1 << 24)) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 2^24 rows");
     if (!a->u && (a->temperatures || a->temperature > 0.0f)) return paged_fail(NEKO_ERR_ARG, op, "sampling needs its numbers");
     return finish(op, launch_sample_rows(*a, static_cast<cudaStream_t>(stream)));

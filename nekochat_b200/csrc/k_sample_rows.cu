@@ -2,15 +2,18 @@
 //
 // A cluster of CTAs takes a row: each holds its slice in shared memory, so the logits are read from memory once whatever follows.
 // Weights 2^(44 - y), y = (max - x) log2(e) / temperature, are rounded to integers and added as integers: sums do not depend on an
-// order, and any split of a row gives the same token. They are computed in 64 bits (a table of 512 powers and a cubic): with V
-// tokens of about equal weight a row's number falls within 2^-24 of a border once in 2^24 / V rows, so f32 sums would choose
-// otherwise than the definition now and then.
+// order, and any split of a row gives the same token. They are computed in 64 bits (a table of 32 powers, 16 copies of it so that no
+// two lanes of a half warp meet in a bank, and a polynomial of degree 5): with V tokens of about equal weight a row's number falls
+// within 2^-24 of a border once in 2^24 / V rows, so f32 sums would choose otherwise than the definition now and then.
 //
 // What is kept is a beginning of the row in descending order, found without sorting the row:
 //  * the largest values of 64 groups of threads a CTA bound the r-th largest of the row from below (the r-th largest of them), and few
 //    more than r tokens reach that bound: they are collected in one CTA, ranked by counting and cut there. Enough for top-k up to
 //    three quarters of the groups, and for top-p where the collected tokens hold that much of the sum.
-//  * else a histogram over equal steps of max - x, of counts or of weights in three pieces of 15 bits (32-bit additions in shared memory),
+//  * top-p else: the pass that adds up the weights has counted the tokens in 4,096 equal steps of max - x, which say in which step
+//    the cut must lie, but for a few steps about an edge. One more pass over the weights adds up what lies before it and
+//    collects the step's tokens, which are ranked; the exact sums confirm the step (or the next way is taken).
+//  * else a histogram over equal steps, of counts or of weights in three pieces of 15 bits (32-bit additions in shared memory),
 //    added up over the cluster, gives the step that the cut falls into; its tokens are collected and ranked, or where they are
 //    too many the key's digits (11, 11 and 10 bits) lead to the cut's value, whose equals are cut by index.
 // The draw goes through the slices in the order of the vocabulary: sums of CTAs, of warps' segments, of lanes.
@@ -30,12 +33,17 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kGroups = kThreads / 8;  // groups of threads whose largest values are known
 constexpr int kCand = 1024;            // tokens that are ranked by counting
+constexpr int kMine = 512;             // of them those of one CTA of several
 constexpr int kBins = 2048;
-constexpr int kTable = 512;
+constexpr int kSteps = 4096;           // steps of max - x that tokens are counted in, two 16-bit counts a word
+constexpr int kPowers = 32, kCopies = 16;
 constexpr int kMaxCluster = 8;
 constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest
-constexpr int kSmemAux = 4 * kBins * 4;    // histograms, or the lists
-static_assert(4 * kCand * 8 <= kSmemAux, "the lists take the histograms' place");
+// lists of CTA 0 (as collected, then the sums; in order), the CTA's own list, the counts; histograms take all of it
+constexpr int kSortedOff = kCand * 8, kMineOff = 2 * kCand * 8;
+__host__ __device__ constexpr int counts_off(int ctas) { return kMineOff + (ctas > 1 ? kMine : kCand) * 8; }
+__host__ __device__ constexpr int aux_bytes(int ctas) { return counts_off(ctas) + kSteps * 2; }
+static_assert(aux_bytes(kMaxCluster) >= 3 * kBins * 4, "the histograms");
 
 // The order of values as unsigned numbers; zeros are alike.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -44,46 +52,49 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
 
-template <typename T>
-__device__ __forceinline__ float value_of(T v) {
-    return float(v);
-}
-
 // What the threads of a row share. Lists are ordered by key (value, then lower index): (order_key << 32) | ~index.
 struct Shared {
-    double table[kTable];            // 2^(i / 512)
+    double table[kPowers * kCopies];      // 2^(i / 32) at [i][copy]
     float gmax[kMaxCluster * kGroups];
     unsigned long long sum[kMaxCluster];  // by CTA: of weights or counts
     unsigned long long warp_sum[kWarps];
-    unsigned long long cut;          // tokens from here up (in the lists' order) are kept
+    unsigned long long seg[kWarps];       // what is kept in each warp's segment
+    unsigned long long cut;               // tokens from here up (in the lists' order) are kept
     unsigned long long before, total;
-    unsigned best, found;            // lowest index
-    unsigned n_list, n_all, at_list; // tokens in this CTA's list, in the owner's, and where this CTA's begin there
-    int bin, done;
+    long long more;                       // what the collected tokens weigh more than their steps say
+    unsigned best, found;                 // lowest index
+    unsigned n_list, n_all, at_list;      // tokens in this CTA's list, in CTA 0's, and where this CTA's begin there
+    int bin, bin_end, done;
     float pick;
     uint64_t bar;
 };
 
 struct Row {
     float m;        // largest value
-    double c;       // log2(e) / temperature
+    float c32;      // log2(e) / temperature
+    double c;
     double lim;     // y up to this is kept (min-p)
 };
 
-// 2^(44 - y) to the nearest integer.
-__device__ __forceinline__ double weight(const Row& r, const double* table, float x) {
-    const double d = x == r.m ? 0.0 : double(r.m) - double(x);
-    const double v = fma(-d, r.c, 44.0);
-    if (!(v >= -1.0)) return 0.0;
-    const double t = fma(v, double(kTable), 6755399441055744.0);  // + 1.5 * 2^52: the integer in the low word
+// 2^(44 - y) to the nearest integer, as the bits of 2^52 plus it (kBits: of 2^52 alone).
+constexpr unsigned long long kBits = 0x4330000000000000ull;
+__device__ __forceinline__ unsigned long long weight_bits(const Row& r, const double* table, float x) {
+    if (!((r.m - x) * r.c32 < 45.5f) && x != r.m) return kBits;
+    const double d = x == r.m ? 0.0 : double(x) - double(r.m), c = r.c * kPowers;
+    constexpr double kMagic = 6755399441055744.0 + 44 * kPowers;  // 1.5 * 2^52: the integer in the low word
+    const double t = fma(d, c, kMagic);
     const int n = __double2loint(t);
-    const double f = fma(t - 6755399441055744.0, -1.0 / kTable, v);
-    double p = fma(f, 0.05550410866482158, 0.2402265069591007);  // ln2^3 / 6, ln2^2 / 2
-    p = fma(p, f, 0.6931471805599453);
-    const double w = table[n & (kTable - 1)];
-    const double s = __hiloint2double(__double2hiint(w) + ((n >> 9) << 20), __double2loint(w));
-    return (fma(p * f, s, s) + 4503599627370496.0) - 4503599627370496.0;  // 2^52
+    const double f = fma(d, c, kMagic - t);
+    // 2^(f / 32), |f| <= 1/2: (ln2 / 32)^k / k!
+    double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
+    p = fma(p, f, 1.6938509724371819e-06);
+    p = fma(p, f, 0.00023459619820224677);
+    p = fma(p, f, 0.02166084939249829);
+    const double w = table[(n & (kPowers - 1)) * kCopies + (threadIdx.x & (kCopies - 1))];
+    const double s = __hiloint2double(__double2hiint(w) + ((n >> 5) << 20), __double2loint(w));
+    return __double_as_longlong(fma(p * f, s, s) + 4503599627370496.0);
 }
+__device__ __forceinline__ unsigned long long weight(const Row& r, const double* table, float x) { return weight_bits(r, table, x) - kBits; }
 __device__ __forceinline__ bool within(const Row& r, float x) { return (x == r.m ? 0.0 : double(r.m) - double(x)) * r.c <= r.lim; }
 
 __device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
@@ -99,9 +110,9 @@ __device__ __forceinline__ unsigned long long warp_upto(unsigned long long v, in
     }
     return v;
 }
-// Sums up to and with each of `per` consecutive values a thread, in place.
+// Sums up to and with each of `per` consecutive values a thread, in place; the sum of all is returned.
 template <int kPer>
-__device__ __forceinline__ void cta_upto(Shared& sh, unsigned long long (&v)[kPer]) {
+__device__ __forceinline__ unsigned long long cta_upto(Shared& sh, unsigned long long (&v)[kPer]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 1; i < kPer; i++) v[i] += v[i - 1];
@@ -109,15 +120,21 @@ __device__ __forceinline__ void cta_upto(Shared& sh, unsigned long long (&v)[kPe
     __syncthreads();
     if (lane == 31) sh.warp_sum[warp] = upto;
     __syncthreads();
-    unsigned long long before = upto - v[kPer - 1];
-    for (int w = 0; w < warp; w++) before += sh.warp_sum[w];
+    unsigned long long before = upto - v[kPer - 1], all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        const unsigned long long x = sh.warp_sum[w];
+        before += w < warp ? x : 0ull, all += x;
+    }
 #pragma unroll
     for (int i = 0; i < kPer; i++) v[i] += before;
+    return all;
 }
 
 template <typename T>
 struct Sampler {
     static constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte vector
+    using u64 = unsigned long long;
     const neko_sample_rows_args& a;
     cg::cluster_group cluster;
     Shared& sh;
@@ -128,160 +145,161 @@ struct Sampler {
 
     __device__ Sampler(const neko_sample_rows_args& a_, Shared& s, uint8_t* x) : a(a_), cluster(cg::this_cluster()), sh(s), aux(x) {}
 
-    // f(value, index) of every value of the slice, by vectors of this thread. Places outside the row hold -infinity.
+    __device__ u64* list() const { return reinterpret_cast<u64*>(aux); }
+    __device__ u64* sorted() const { return reinterpret_cast<u64*>(aux + kSortedOff); }
+    __device__ u64* mine() const { return reinterpret_cast<u64*>(aux + kMineOff); }
+    __device__ uint32_t* counts() const { return reinterpret_cast<uint32_t*>(aux + counts_off(ctas)); }
+    __device__ unsigned mine_room() const { return ctas > 1 ? kMine : kCand; }
+    __device__ int segment() const { return (nv + kWarps - 1) / kWarps; }  // vectors of a warp's segment
+
+    // f(value, index) of a vector's values. Places outside the row hold -infinity.
+    template <typename F>
+    __device__ __forceinline__ void of_vector(int v, F f) const {
+        const uint4 w = data[v];
+        const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) f(float(x[j]), first + v * kPer + j);
+    }
+    // Of every value of the slice, vectors spread over the threads, or over the lanes of the segment's warp.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        for (int v = threadIdx.x; v < nv; v += kThreads) {
-            const uint4 w = data[v];
-            const T* x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int j = 0; j < kPer; j++) f(value_of(x[j]), first + v * kPer + j);
-        }
+        for (int v = threadIdx.x; v < nv; v += kThreads) of_vector(v, f);
     }
-    __device__ __forceinline__ static unsigned long long entry(float x, int i) {
-        return (static_cast<unsigned long long>(order_key(x)) << 32) | (0xFFFFFFFFu - unsigned(i));
+    template <typename F>
+    __device__ __forceinline__ void each_of_segment(F f) const {
+        const int v0 = int(threadIdx.x >> 5) * segment(), v1 = min(v0 + segment(), nv);
+        for (int v = v0 + int(threadIdx.x & 31); v < v1; v += 32) of_vector(v, f);
     }
+    __device__ __forceinline__ static u64 entry(float x, int i) { return (static_cast<u64>(order_key(x)) << 32) | (0xFFFFFFFFu - unsigned(i)); }
+    __device__ __forceinline__ static float value(u64 e) { return key_value(uint32_t(e >> 32)); }
     // Values that can be taken at all: not NaN, not -infinity.
     __device__ __forceinline__ static bool real(float x) { return x > -INFINITY; }
+    __device__ __forceinline__ u64 weight_of(float x) const { return weight(row, sh.table, x); }
 
-    // The slices' sums meet: sum[i] of every CTA.
-    __device__ void share_sum(unsigned long long v) {
+    // The CTAs' sums meet: sum[i] of every CTA.
+    __device__ void share_sum(u64 v) {
         if (threadIdx.x < ctas) *cluster.map_shared_rank(&sh.sum[rank], threadIdx.x) = v;
         cluster.sync();
     }
 
-    // The tokens for which take(value, index) holds come together in CTA 0's list (aux); n_all says how many there are, the
-    // first kCand of them are in it.
-    template <typename F, typename G>
-    __device__ void collect(F take, G then) {
-        unsigned long long* mine = reinterpret_cast<unsigned long long*>(aux) + kCand;
-        unsigned long long* list = cluster.map_shared_rank(reinterpret_cast<unsigned long long*>(aux), 0);
-        if (threadIdx.x == 0) sh.n_list = 0;
-        __syncthreads();
-        each([&](float x, int i) {
-            if (take(x, i)) {
-                const unsigned at = atomicAdd(&sh.n_list, 1u);
-                if (at < kCand) mine[at] = entry(x, i);
-            }
-        });
+    // A token that take() has chosen goes to this CTA's list.
+    __device__ __forceinline__ void put(float x, int i) {
+        const unsigned at = atomicAdd(&sh.n_list, 1u);
+        if (at < mine_room()) mine()[at] = entry(x, i);
+    }
+    // The CTAs' lists come together in CTA 0's: n_all says how many tokens there are, if more than kCand they are not all there.
+    // then() before the CTAs meet.
+    template <typename G>
+    __device__ void gather(G then) {
         __syncthreads();
         const unsigned n = sh.n_list;
-        if (threadIdx.x == 0) sh.at_list = atomicAdd(cluster.map_shared_rank(&sh.n_all, 0), n);
+        u64* to = cluster.map_shared_rank(list(), 0);
+        if (threadIdx.x == 0) sh.at_list = atomicAdd(cluster.map_shared_rank(&sh.n_all, 0), n > mine_room() ? kCand + 1 : n);
         __syncthreads();
-        for (unsigned i = threadIdx.x; i < min(n, unsigned(kCand)); i += kThreads)
-            if (sh.at_list + i < kCand) list[sh.at_list + i] = mine[i];
+        for (unsigned i = threadIdx.x; i < min(n, mine_room()); i += kThreads)
+            if (sh.at_list + i < kCand) to[sh.at_list + i] = mine()[i];
         then();
         cluster.sync();
     }
 
-    // CTA 0's list in descending order (into the second list), and sums of measure(entry) up to and with each (the third).
+    // CTA 0's list in descending order (sorted()), and in its place the sums of measure(entry) up to and with each.
     template <typename F>
     __device__ void rank_list(int n, F measure) {
-        unsigned long long* list = reinterpret_cast<unsigned long long*>(aux);
-        unsigned long long *sorted = list + kCand, *upto = list + 2 * kCand;
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            const unsigned long long e = list[i];
-            int r = 0;
-            for (int j = 0; j < n; j++) r += list[j] > e;
-            sorted[r] = e;
+            const u64 e = list()[i];
+            int r = 0, j = 0;
+            for (; j + 4 <= n; j += 4) {
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list() + j), y = *reinterpret_cast<const ulonglong2*>(list() + j + 2);
+                r += (x.x > e) + (x.y > e) + (y.x > e) + (y.y > e);
+            }
+            for (; j < n; j++) r += list()[j] > e;
+            sorted()[r] = e;
         }
         __syncthreads();
-        unsigned long long v[2];
+        u64 v[kCand / kThreads];
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = 2 * threadIdx.x + k;
-            v[k] = i < n ? measure(sorted[i]) : 0ull;
+        for (int k = 0; k < kCand / kThreads; k++) {
+            const int i = kCand / kThreads * threadIdx.x + k;
+            v[k] = i < n ? measure(sorted()[i]) : 0ull;
         }
         cta_upto(sh, v);
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (2 * threadIdx.x + k < n) upto[2 * threadIdx.x + k] = v[k];
+        for (int k = 0; k < kCand / kThreads; k++)
+            if (int(kCand / kThreads * threadIdx.x) + k < n) list()[kCand / kThreads * threadIdx.x + k] = v[k];
         __syncthreads();
     }
-    __device__ __forceinline__ unsigned long long weight_of(unsigned long long e) const {
-        return static_cast<unsigned long long>(weight(row, sh.table, key_value(uint32_t(e >> 32))));
-    }
-    // How many of the n sums, each with what lies ahead, are below target.
-    __device__ int below(const unsigned long long* upto, int n, double target, unsigned long long ahead) {
+    // How many of CTA 0's n sums, each with what lies ahead, are below target.
+    __device__ int below(int n, double target, u64 ahead) {
         int c = 0;
         for (int base = 0; base < n; base += kThreads)
-            c += __syncthreads_count(base + threadIdx.x < n && double(ahead + upto[base + threadIdx.x]) < target);
+            c += __syncthreads_count(base + threadIdx.x < n && double(ahead + list()[base + threadIdx.x]) < target);
         return c;
     }
 
-    __device__ void answer(int r, int token, float x, unsigned long long total) {
+    __device__ void answer(int r, int token, float x, u64 total) {
         a.token[r] = token;
         if (a.prob) a.prob[r] = token < 0 ? 0.0f : float(exp2(-(x == row.m ? 0.0 : (double(row.m) - double(x)) * row.c)) * (kOne / double(total)));
     }
     // floor(u * total), below total.
-    __device__ unsigned long long place(int r, unsigned long long total) {
+    __device__ u64 place(int r, u64 total) {
         const double x = a.u[r] * double(total);
-        const unsigned long long p = x > 0.0 ? static_cast<unsigned long long>(x) : 0ull;
-        return min(p, total - 1);
+        return min(x > 0.0 ? static_cast<u64>(x) : 0ull, total - 1);
     }
 
-    // The first index, in the order of the vocabulary, at which the sum of measure(value, index) exceeds where(total): its CTA
-    // gets found = index, pick = value; total to all. Sums of warps' segments of the slice, then of 32 vectors at a time.
+    // The first index, in the order of the vocabulary, at which the sum of measure(value, index) exceeds where(sum of all): its CTA
+    // gets found = index, pick = value. seg[] holds the segments' sums. The sum of all is returned.
     template <typename M, typename P>
-    __device__ unsigned long long find(M measure, P where) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seg = (nv + kWarps - 1) / kWarps;
-        const int v0 = min(warp * seg, nv), v1 = min(v0 + seg, nv);
-        double part = 0.0;  // of integers, exact
-        for (int v = v0 + lane; v < v1; v += 32) {
-            const uint4 w = data[v];
-            const T* x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int j = 0; j < kPer; j++) part += measure(value_of(x[j]), first + v * kPer + j);
-        }
-        const unsigned long long of_warp = warp_total(static_cast<unsigned long long>(part));
+    __device__ u64 locate(M measure, P where) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (threadIdx.x == 0) sh.found = 0xFFFFFFFFu;
         __syncthreads();
-        if (lane == 0) sh.warp_sum[warp] = of_warp;
-        __syncthreads();
-        unsigned long long mine = 0, before = 0, total = 0;
-        for (int w = 0; w < kWarps; w++) mine += sh.warp_sum[w];
-        share_sum(mine);
-        for (int i = 0; i < ctas; i++) {
-            if (i < rank) before += sh.sum[i];
-            total += sh.sum[i];
+        u64 of_cta = 0, before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const u64 x = sh.seg[w];
+            of_cta += x, before += w < warp ? x : 0ull;
         }
-        const unsigned long long at = where(total);
-        for (int w = 0; w < warp; w++) before += sh.warp_sum[w];
-        if (total && at >= before && at < before + of_warp) {  // one warp of the cluster
+        share_sum(of_cta);
+        for (int i = 0; i < ctas; i++) {
+            const u64 x = sh.sum[i];
+            before += i < rank ? x : 0ull, total += x;
+        }
+        const u64 at = where(total);
+        if (total && at >= before && at - before < sh.seg[warp]) {  // one warp of the cluster
+            const int v0 = warp * segment(), v1 = min(v0 + segment(), nv);
             for (int base = v0; base < v1; base += 32) {
                 const int v = base + lane;
-                unsigned long long s = 0;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                const T* x = reinterpret_cast<const T*>(&w);
-                if (v < v1) {
-                    w = data[v];
-#pragma unroll
-                    for (int j = 0; j < kPer; j++) s += static_cast<unsigned long long>(measure(value_of(x[j]), first + v * kPer + j));
+                u64 s = 0;
+                if (v < v1) of_vector(v, [&](float x, int i) { s += measure(x, i); });
+                const u64 upto = before + warp_upto(s, lane);
+                if (upto > at && upto - s <= at) {  // one lane
+                    u64 sum = upto - s;
+                    bool there = false;
+                    of_vector(v, [&](float x, int i) {
+                        sum += measure(x, i);
+                        if (sum > at && !there) sh.found = unsigned(i), sh.pick = x, there = true;
+                    });
                 }
-                const unsigned long long upto = warp_upto(s, lane);
-                if (before + upto > at && before + upto - s <= at) {  // one lane
-                    unsigned long long sum = before + upto - s;
-                    for (int j = 0; j < kPer; j++) {
-                        sum += static_cast<unsigned long long>(measure(value_of(x[j]), first + v * kPer + j));
-                        if (sum > at) {
-                            sh.found = unsigned(first + v * kPer + j);
-                            sh.pick = value_of(x[j]);
-                            break;
-                        }
-                    }
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
+                before = __shfl_sync(0xffffffffu, upto, 31);
                 if (before > at) break;
             }
         }
         __syncthreads();
         return total;
     }
+    template <typename M, typename P>
+    __device__ u64 find(M measure, P where) {
+        u64 part = 0;
+        each_of_segment([&](float x, int i) { part += measure(x, i); });
+        part = warp_total(part);
+        if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
+        return locate(measure, where);
+    }
 
     // Adds up a histogram over the cluster and finds the bin at which the sum reaches target(total of all bins, with what lies
-    // before them): bin (-1: none does), before (without the bin), total to every CTA.
+    // ahead of them): bin (-1: none does), before (the sum without the bin), total to every CTA.
     template <bool MASS, typename F, typename G>
-    __device__ void histogram(F bin_of, unsigned long long ahead, G target) {
+    __device__ void histogram(F bin_of, u64 ahead, G target) {
         uint32_t* h = reinterpret_cast<uint32_t*>(aux);
         for (int i = threadIdx.x; i < (MASS ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
         __syncthreads();
@@ -289,7 +307,7 @@ struct Sampler {
             const int b = bin_of(x, i);
             if (b < 0) return;
             if constexpr (MASS) {
-                const unsigned long long w = static_cast<unsigned long long>(weight(row, sh.table, x));
+                const u64 w = weight_of(x);
                 const uint32_t p0 = uint32_t(w) & 0x7fffu, p1 = uint32_t(w >> 15) & 0x7fffu, p2 = uint32_t(w >> 30);
                 if (p0) atomicAdd(&h[b], p0);
                 if (p1) atomicAdd(&h[kBins + b], p1);
@@ -300,28 +318,25 @@ struct Sampler {
         });
         cluster.sync();
         // this CTA's share of the bins, kBins / ctas of them: four at most a thread
+        constexpr int kMost = kBins / kThreads;
         const int share = kBins / ctas, per = (share + kThreads - 1) / kThreads;
-        unsigned long long v[4] = {0, 0, 0, 0};
+        u64 v[kMost] = {}, own[kMost];
         for (int c = 0; c < ctas; c++) {
             const uint32_t* o = cluster.map_shared_rank(h, c) + rank * share;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < kMost; k++) {
                 const int b = threadIdx.x * per + k;
                 if (k >= per || b >= share) continue;
                 v[k] += o[b];
-                if (MASS) v[k] += (static_cast<unsigned long long>(o[kBins + b]) << 15) + (static_cast<unsigned long long>(o[2 * kBins + b]) << 30);
+                if (MASS) v[k] += (static_cast<u64>(o[kBins + b]) << 15) + (static_cast<u64>(o[2 * kBins + b]) << 30);
             }
         }
-        unsigned long long own[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) own[k] = v[k];
-        cta_upto(sh, v);
-        __syncthreads();
-        unsigned long long all = 0;
-        for (int w = 0; w < kWarps; w++) all += sh.warp_sum[w];
+        for (int k = 0; k < kMost; k++) own[k] = v[k];
+        const u64 all = cta_upto(sh, v);
         if (threadIdx.x == 0) sh.bin = -1;
         share_sum(all);
-        unsigned long long before = ahead, total = ahead;
+        u64 before = ahead, total = ahead;
         for (int i = 0; i < ctas; i++) {
             if (i < rank) before += sh.sum[i];
             total += sh.sum[i];
@@ -329,8 +344,8 @@ struct Sampler {
         const double want = target(total);
         // one thread of the cluster has the bin that reaches it
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const unsigned long long upto = before + v[k], less = upto - own[k];
+        for (int k = 0; k < kMost; k++) {
+            const u64 upto = before + v[k], less = upto - own[k];
             if (own[k] && double(upto) >= want && double(less) < want) {
                 for (int c = 0; c < ctas; c++) {
                     Shared* o = cluster.map_shared_rank(&sh, c);
@@ -344,29 +359,29 @@ struct Sampler {
     }
 
     // Moves the cut (among what the present one keeps) to the first token, in descending order, at which the sum of the counts
-    // (COUNT) or weights reaches want(total).
+    // or weights (MASS) reaches want_of(total).
     template <bool MASS, typename G>
     __device__ void select(G want_of) {
-        const unsigned long long cut = sh.cut;
-        const float scale = fminf(64.0f * fmaxf(float(fmin(row.c, 1e30)), 1.0f), 1e30f);
+        const u64 cut = sh.cut;
+        const float scale = fminf(64.0f * fmaxf(row.c32, 1.0f), 1e30f);
         auto step_of = [&](float x, int i) {
             if (!real(x) || entry(x, i) < cut) return -1;
             return x == row.m ? 0 : int(fminf((row.m - x) * scale, float(kBins - 1)));
         };
-        if (threadIdx.x == 0) sh.n_all = 0;
+        if (threadIdx.x == 0) sh.n_all = sh.n_list = 0;
         histogram<MASS>(step_of, 0, want_of);
         const int step = sh.bin;
         if (step < 0) return;  // fewer than that many
-        unsigned long long before = sh.before;
+        u64 before = sh.before;
         const double want = want_of(sh.total);
-        collect([&](float x, int i) { return step_of(x, i) == step; }, []() {});
+        each([&](float x, int i) { if (step_of(x, i) == step) put(x, i); });
+        gather([]() {});
         if (rank == 0) {
-            const int n = int(min(sh.n_all, unsigned(kCand) + 1u));
-            unsigned long long next = 0;
-            if (n <= kCand) {
-                unsigned long long* list = reinterpret_cast<unsigned long long*>(aux);
-                rank_list(n, [&](unsigned long long e) { return MASS ? weight_of(e) : 1ull; });
-                next = list[kCand + min(below(list + 2 * kCand, n, want, before), n - 1)];
+            u64 next = 0;
+            if (sh.n_all <= kCand) {
+                const int n = int(sh.n_all);
+                rank_list(n, [&](u64 e) { return MASS ? weight_of(value(e)) : 1ull; });
+                next = sorted()[min(below(n, want, before), n - 1)];
             }
             if (threadIdx.x < ctas) {
                 Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
@@ -384,66 +399,190 @@ struct Sampler {
             histogram<MASS>([&](float x, int i) {
                 const uint32_t k = order_key(x);
                 return step_of(x, i) == step && (k & known) == key ? int(most - (k >> shift & most)) : -1;
-            }, before, [&](unsigned long long) { return want; });
+            }, before, [&](u64) { return want; });
             before = sh.before;
             key |= (most - uint32_t(max(sh.bin, 0))) << shift;
             known |= most << shift;
         }
-        const double each_one = MASS ? weight(row, sh.table, key_value(key)) : 1.0;
+        const double each_one = MASS ? double(weight_of(key_value(key))) : 1.0;
         const double more = ceil((want - double(before)) / each_one);
-        find([&](float x, int i) { return step_of(x, i) == step && order_key(x) == key ? 1.0 : 0.0; },
-             [&](unsigned long long total) { return more > 1.0 ? min(static_cast<unsigned long long>(more) - 1, total - 1) : 0ull; });
+        find([&](float x, int i) { return step_of(x, i) == step && order_key(x) == key ? 1ull : 0ull; },
+             [&](u64 total) { return more > 1.0 ? min(static_cast<u64>(more) - 1, total - 1) : 0ull; });
         if (threadIdx.x == 0 && sh.found != 0xFFFFFFFFu) {
-            const unsigned long long next = (static_cast<unsigned long long>(key) << 32) | (0xFFFFFFFFu - sh.found);
+            const u64 next = (static_cast<u64>(key) << 32) | (0xFFFFFFFFu - sh.found);
             for (int c = 0; c < ctas; c++) cluster.map_shared_rank(&sh, c)->cut = next;
         }
         cluster.sync();
     }
 
-    // The cut by the largest values alone (see above); true: the row is answered.
+    // The steps that few() counts in, and what a step's tokens weigh by its middle.
+    __device__ __forceinline__ float count_scale() const { return fminf(128.0f * fmaxf(row.c32, 1.0f), 1e30f); }
+    __device__ __forceinline__ int count_step(float x, float scale) const { return x == row.m ? 0 : int(fminf((row.m - x) * scale, float(kSteps - 1))); }
+    __device__ __forceinline__ float middle(int step, float scale) const {
+        return step == kSteps - 1 ? 0.0f : exp2f(44.0f - (float(step) + 0.5f) / scale * row.c32);
+    }
+
+    // The cut by the largest values alone; true: the row is answered. Without top_k the weights are added up and the tokens
+    // counted in steps, for what comes next.
     __device__ bool few(int r, float t, int top_k, bool use_p, float top_p) {
-        double part = 0.0;
-        if (threadIdx.x == 0) sh.done = 0;
-        collect([&](float x, int) {
-            if (!top_k && real(x)) part += weight(row, sh.table, x);
-            return x >= t && real(x);
-        }, [&]() {
-            if (top_k) return;
-            const unsigned long long s = warp_total(static_cast<unsigned long long>(part));
-            if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.total, 0), s);
-        });
-        if (rank == 0 && sh.n_all <= kCand) {
-            unsigned long long *sorted = reinterpret_cast<unsigned long long*>(aux) + kCand, *upto = sorted + kCand, *w = upto + kCand;
-            const int n = int(sh.n_all), n_k = top_k ? min(top_k, n) : n;
-            rank_list(n, [&](unsigned long long e) { return weight_of(e); });
-            int n_p = n_k;
-            bool sure = top_k != 0;
-            if (use_p) {
-                const unsigned long long total = top_k ? upto[n_k - 1] : sh.total;
-                const int less = below(upto, n_k, fmax(double(top_p) * double(total), 0.5), 0);
-                if (less < n_k) n_p = less + 1, sure = true;
-            }
-            int n_m = 0;
-            for (int base = 0; base < n_p; base += kThreads) {
-                const int i = base + threadIdx.x;
-                n_m += __syncthreads_count(i < n_p && within(row, key_value(uint32_t(sorted[i < n_p ? i : 0] >> 32))));
-            }
-            sure |= n_m < n_p;
-            if (sure) {
-                const unsigned long long total = upto[n_m - 1], at = place(r, total);
-                for (int i = threadIdx.x; i < n_m; i += kThreads) w[i] = upto[i] - (i ? upto[i - 1] : 0ull);
-                __syncthreads();
-                for (int i = threadIdx.x; i < n_m; i += kThreads) {
-                    const uint32_t low = uint32_t(sorted[i]);  // ~index
-                    unsigned long long before = 0;
-                    for (int j = 0; j < n_m; j++) before += uint32_t(sorted[j]) > low ? w[j] : 0ull;
-                    if (at >= before && at < before + w[i]) answer(r, int(0xFFFFFFFFu - low), key_value(uint32_t(sorted[i] >> 32)), total);
+        const float scale = count_scale();
+        if (!top_k)
+            for (int i = threadIdx.x; i < kSteps / 2; i += kThreads) counts()[i] = 0;
+        if (threadIdx.x == 0) sh.done = 0, sh.n_list = 0;
+        __syncthreads();
+        if (top_k) {
+            each([&](float x, int i) { if (x >= t && real(x)) put(x, i); });
+            gather([]() {});
+        } else {
+            u64 part = 0;
+            each([&](float x, int i) {
+                if (!real(x)) return;
+                part += weight_of(x);
+                const int step = count_step(x, scale);
+                atomicAdd(&counts()[step >> 1], 1u << (16 * (step & 1)));
+                if (x >= t) put(x, i);
+            });
+            gather([&]() {
+                part = warp_total(part);
+                if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.total, 0), part);
+            });
+        }
+        if (rank == 0) {
+            bool sure = false;
+            long long more = 0;
+            const unsigned n_all = sh.n_all;
+            __syncthreads();  // read by all before it is set again below
+            if (n_all <= kCand) {
+                const int n = int(n_all), n_k = top_k ? min(top_k, n) : n;
+                rank_list(n, [&](u64 e) { return weight_of(value(e)); });
+                const u64* upto = list();
+                int n_p = n_k;
+                sure = top_k != 0;
+                if (use_p) {
+                    const u64 total = top_k ? upto[n_k - 1] : sh.total;
+                    const int less = below(n_k, fmax(double(top_p) * double(total), 0.5), 0);
+                    if (less < n_k) n_p = less + 1, sure = true;
                 }
-                if (threadIdx.x < ctas) cluster.map_shared_rank(&sh, threadIdx.x)->done = 1;
+                int n_m = n_p;
+                if (row.lim < INFINITY) {
+                    n_m = 0;
+                    for (int base = 0; base < n_p; base += kThreads) {
+                        const int i = base + threadIdx.x;
+                        n_m += __syncthreads_count(i < n_p && within(row, value(sorted()[i < n_p ? i : 0])));
+                    }
+                    sure |= n_m < n_p;
+                }
+                if (sure) {
+                    const u64 total = upto[n_m - 1], at = place(r, total);
+                    for (int i = threadIdx.x; i < n_m; i += kThreads) {
+                        const uint32_t low = uint32_t(sorted()[i]);  // ~index
+                        u64 before = 0, last = 0;
+                        for (int j = 0; j < n_m; j++) {
+                            const u64 u = upto[j];
+                            before += uint32_t(sorted()[j]) > low ? u - last : 0ull;
+                            last = u;
+                        }
+                        if (at >= before && at - before < upto[i] - (i ? upto[i - 1] : 0ull))
+                            answer(r, int(0xFFFFFFFFu - low), value(sorted()[i]), total);
+                    }
+                } else {
+                    u64 by_step = 0;
+                    for (int i = threadIdx.x; i < n; i += kThreads) by_step += static_cast<u64>(middle(count_step(value(sorted()[i]), scale), scale));
+                    u64 v[1] = {by_step};
+                    more = static_cast<long long>(upto[n - 1]) - static_cast<long long>(cta_upto(sh, v));
+                }
             }
+            if (threadIdx.x < ctas) {
+                Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
+                o->done = sure, o->more = more;
+                if (rank != int(threadIdx.x)) o->total = sh.total;
+            }
+            if (threadIdx.x == 0) sh.n_all = 0, sh.before = 0;
         }
         cluster.sync();
         return sh.done != 0;
+    }
+
+    // Top-p by the counts of few(): true: the cut is set, and seg[] holds what is kept.
+    __device__ bool near_cut(float top_p) {
+        const float scale = count_scale();
+        // this CTA's share of the steps: what their tokens weigh, by the middles
+        constexpr int kMost = kSteps / kThreads;
+        const int share = kSteps / ctas, per = share / kThreads;
+        u64 v[kMost] = {}, own[kMost];
+        {
+            uint32_t n[kMost] = {};
+            for (int c = 0; c < ctas; c++) {
+                const uint16_t* o = reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c)) + rank * share + threadIdx.x * per;
+#pragma unroll
+                for (int k = 0; k < kMost; k++)
+                    if (k < per) n[k] += o[k];
+            }
+#pragma unroll
+            for (int k = 0; k < kMost; k++)
+                if (k < per) v[k] = static_cast<u64>(n[k]) * static_cast<u64>(middle(rank * share + threadIdx.x * per + k, scale));
+        }
+#pragma unroll
+        for (int k = 0; k < kMost; k++) own[k] = v[k];
+        const u64 all = cta_upto(sh, v);
+        const double sum = double(sh.total), want = fmax(double(top_p) * sum, 0.5);
+        if (threadIdx.x == 0) sh.bin = sh.bin_end = kSteps - 1, sh.n_list = 0;
+        share_sum(all);
+        double before = double(sh.more);
+        for (int i = 0; i < rank; i++) before += double(sh.sum[i]);
+        // the first steps at which the sum may and must have reached it
+        const double margin = sum * 0x1p-13;
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            const double upto = before + double(v[k]), less = upto - double(own[k]);
+            const int step = rank * share + int(threadIdx.x) * per + k;
+            if (k >= per || !own[k]) continue;
+            const bool may = upto >= want - margin && less < want - margin, must = upto >= want + margin && less < want + margin;
+            if (may || must)
+                for (int c = 0; c < ctas; c++) {
+                    Shared* o = cluster.map_shared_rank(&sh, c);
+                    if (may) o->bin = step;
+                    if (must) o->bin_end = step;
+                }
+        }
+        cluster.sync();
+        const int lo = sh.bin, hi = sh.bin_end;
+        u64 part = 0;
+        each_of_segment([&](float x, int i) {
+            if (!real(x)) return;
+            const int step = count_step(x, scale);
+            if (step < lo) part += weight_of(x);
+            else if (step <= hi) put(x, i);
+        });
+        part = warp_total(part);
+        if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
+        gather([&]() {
+            if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.before, 0), part);
+        });
+        if (rank == 0) {
+            u64 next = 0;
+            const u64 ahead = sh.before;
+            if (sh.n_all <= kCand && double(ahead) < want) {
+                const int n = int(sh.n_all);
+                rank_list(n, [&](u64 e) { return weight_of(value(e)); });
+                const int less = below(n, want, ahead);
+                if (less < n) next = sorted()[less];
+            }
+            if (threadIdx.x < ctas) {
+                Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
+                o->done = next != 0;
+                if (next) o->cut = next;
+            }
+        }
+        cluster.sync();
+        if (!sh.done) return false;
+        const unsigned n = sh.n_list;
+        for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+            const u64 e = mine()[i];
+            if (e >= sh.cut) atomicAdd(&sh.seg[(int(0xFFFFFFFFu - uint32_t(e)) - first) / kPer / segment()], weight_of(value(e)));
+        }
+        __syncthreads();
+        return true;
     }
 };
 
@@ -454,10 +593,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     Shared& sh = *reinterpret_cast<Shared*>(sm);
     constexpr int kAuxOff = (sizeof(Shared) + 127) / 128 * 128;
     S s(a, sh, sm + kAuxOff);
-    uint8_t* buf = sm + kAuxOff + kSmemAux;
-    const int tid = threadIdx.x, lane = tid & 31;
     s.ctas = int(s.cluster.num_blocks()), s.rank = int(s.cluster.block_rank());
-    const int r = blockIdx.x / s.ctas, ctas = s.ctas;
+    const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.x / s.ctas, ctas = s.ctas;
+    uint8_t* buf = sm + kAuxOff + aux_bytes(ctas);
     const int b = min(s.rank * slice, a.vocab), n = min(slice, a.vocab - b);
     const T* src = static_cast<const T*>(a.logits) + r * a.row_stride + b;
     const int ph = int(reinterpret_cast<uintptr_t>(src) & 15) / int(sizeof(T));  // places before the slice in its first vector
@@ -474,6 +612,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
             bulk_g2s(buf + (ph + head) * sizeof(T) + o, reinterpret_cast<const uint8_t*>(src + head) + o, min(bytes - o, 16384u), &sh.bar);
         sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
     }
+    // while the copies fly: the row's parameters, the table, the ends that are not whole vectors
+    const float temperature = !a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature;
+    const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+    int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+    if (top_k < 0 || top_k >= a.vocab) top_k = 0;
     {
         T* x = reinterpret_cast<T*>(buf);
         const T none = T(-INFINITY);
@@ -482,7 +625,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         const int at = head + body + tid;  // the last, partly filled vector
         if (tid < S::kPer && ph + at < s.nv * S::kPer) x[ph + at] = at < n ? src[at] : none;
     }
-    sh.table[tid] = exp2(double(tid) / kTable);
+    if (temperature > 0.0f) {
+        for (int i = tid; i < kPowers * kCopies; i += kThreads) sh.table[i] = exp2(double(i / kCopies) / kPowers);
+        s.row.c = 1.4426950408889634 / double(temperature);
+        s.row.c32 = float(s.row.c);
+        s.row.lim = min_p > 0.0f ? fmax(-log2(double(min_p)), 0.0) : INFINITY;
+    }
     s.cluster.barrier_arrive();
     __syncthreads();
     bool ok = false;
@@ -504,6 +652,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     float m = warp_max(g);
     if (lane == 0) reinterpret_cast<float*>(sh.warp_sum)[tid >> 5] = m;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < kWarps; w++) m = fmaxf(m, reinterpret_cast<float*>(sh.warp_sum)[w]);
     s.row.m = m;
     if (!(m > -INFINITY)) {  // nothing to take
@@ -512,7 +661,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     }
 
     // ---- greedy: the first maximum
-    const float temperature = !a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature;
     if (!(temperature > 0.0f)) {
         unsigned best = 0xFFFFFFFFu;
         s.each([&](float x, int i) { if (x == m) best = min(best, unsigned(i)); });
@@ -526,29 +674,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         return;
     }
 
-    const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-    int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-    if (top_k < 0 || top_k >= a.vocab) top_k = 0;
     const bool use_p = top_p < 1.0f;
-    s.row.c = 1.4426950408889634 / double(temperature);
-    s.row.lim = min_p > 0.0f ? fmax(-log2(double(min_p)), 0.0) : INFINITY;
+    bool ready = false;  // seg[] holds what is kept
     if (top_k || use_p) {
-        const int want = top_k ? top_k : groups / 2;
-        if (4 * want <= 3 * groups) {
-            if (tid < groups) {
-                int above = 0;
-                for (int j = 0; j < groups; j++) above += sh.gmax[j] > g || (sh.gmax[j] == g && j < tid);
-                if (above == want - 1) sh.pick = g;
+        // for top-p alone a sixth of the groups: 94 tokens of 8 CTAs hold most nuclei
+        const int want = top_k ? top_k : max(groups / 6, 1);
+        const bool bounded = 4 * want <= 3 * groups;
+        if (bounded || !top_k) {
+            // the bound: a key that `want` groups reach, to 16 of its bits (one more halving a bit)
+            uint32_t bound = 0;
+            const uint32_t key = tid < groups ? order_key(g) : 0u;
+            for (int bit = 31; bit >= 16; bit--) {
+                const uint32_t next = bound | 1u << bit;
+                if (__syncthreads_count(tid < groups && key >= next) >= want) bound = next;
             }
-            __syncthreads();
-            if (s.few(r, sh.pick, top_k, use_p, top_p)) return;
+            if (s.few(r, bound >= 0x00800000u ? key_value(bound) : -INFINITY, top_k, use_p, top_p)) return;  // below: no finite value
         }
         if (top_k) s.template select<false>([&](unsigned long long) { return double(top_k); });
-        if (use_p) s.template select<true>([&](unsigned long long total) { return fmax(double(top_p) * double(total), 0.5); });
+        if (use_p) {
+            if (!top_k) ready = s.near_cut(top_p);
+            if (!ready) {
+                s.template select<true>([&](unsigned long long total) { return fmax(double(top_p) * double(total), 0.5); });
+            } else if (s.row.lim < INFINITY) {
+                ready = false;
+            }
+        }
     }
     const unsigned long long cut = sh.cut;
-    const unsigned long long total = s.find([&](float x, int i) { return S::real(x) && S::entry(x, i) >= cut && within(s.row, x) ? weight(s.row, sh.table, x) : 0.0; },
-                                            [&](unsigned long long all) { return s.place(r, all); });
+    const bool all_p = !(s.row.lim < INFINITY);
+    auto kept = [&](float x, int i) { return S::real(x) && S::entry(x, i) >= cut && (all_p || within(s.row, x)) ? s.weight_of(x) : 0ull; };
+    auto where = [&](unsigned long long all) { return s.place(r, all); };
+    const unsigned long long total = ready ? s.locate(kept, where) : s.find(kept, where);
     if (tid == 0 && sh.found != 0xFFFFFFFFu) s.answer(r, int(sh.found), sh.pick, total);
 }
 
@@ -558,7 +714,7 @@ cudaError_t go(const neko_sample_rows_args& a, cudaStream_t st) {
     int ctas = 1;
     while (ctas < kMaxCluster && a.vocab > 4096 * ctas) ctas *= 2;
     const int slice = ((a.vocab + ctas - 1) / ctas + kPer - 1) / kPer * kPer;
-    const size_t smem = (sizeof(Shared) + 127) / 128 * 128 + kSmemAux + size_t(slice + kPer) * sizeof(T);
+    const size_t smem = (sizeof(Shared) + 127) / 128 * 128 + aux_bytes(ctas) + size_t(slice + kPer) * sizeof(T);
     auto* fn = sample_rows_kernel<T>;
     if (cudaError_t e = ensure_dyn_smem(fn, smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -69,22 +69,26 @@ struct Shared {
     uint64_t bar;
 };
 
+// Of a row with finite values only, or -infinity (what is infinite, or where the next value below the largest weighs nothing, becomes
+// zeros and -infinity first): y = (m - x) c.
 struct Row {
     float m;        // largest value
-    float c32;      // log2(e) / temperature
-    double c;
+    float low;      // values count as no less than this: they weigh nothing there
+    float c32;
+    double m64, c, c_powers;  // c = log2(e) / temperature, times the table's powers
     double lim;     // y up to this is kept (min-p)
+    float cut;      // kept: larger values, and this one up to an index
+    unsigned cut_at;
 };
 
-// 2^(44 - y) to the nearest integer, as the bits of 2^52 plus it (kBits: of 2^52 alone).
-constexpr unsigned long long kBits = 0x4330000000000000ull;
+// 2^(44 - y) to the nearest integer, as the bits of 2^52 plus it. No branch, so that several values' chains run side by side.
+constexpr unsigned long long kBits = 0x4330000000000000ull;  // of 2^52
 __device__ __forceinline__ unsigned long long weight_bits(const Row& r, const double* table, float x) {
-    if (!((r.m - x) * r.c32 < 45.5f) && x != r.m) return kBits;
-    const double d = x == r.m ? 0.0 : double(x) - double(r.m), c = r.c * kPowers;
+    const double d = double(fmaxf(x, r.low)) - r.m64;  // NaN: low
     constexpr double kMagic = 6755399441055744.0 + 44 * kPowers;  // 1.5 * 2^52: the integer in the low word
-    const double t = fma(d, c, kMagic);
+    const double t = fma(d, r.c_powers, kMagic);
     const int n = __double2loint(t);
-    const double f = fma(d, c, kMagic - t);
+    const double f = fma(d, r.c_powers, kMagic - t);
     // 2^(f / 32), |f| <= 1/2: (ln2 / 32)^k / k!
     double p = fma(f, 3.9737099845494154e-11, 9.172562701824643e-09);
     p = fma(p, f, 1.6938509724371819e-06);
@@ -95,7 +99,15 @@ __device__ __forceinline__ unsigned long long weight_bits(const Row& r, const do
     return __double_as_longlong(fma(p * f, s, s) + 4503599627370496.0);
 }
 __device__ __forceinline__ unsigned long long weight(const Row& r, const double* table, float x) { return weight_bits(r, table, x) - kBits; }
-__device__ __forceinline__ bool within(const Row& r, float x) { return (x == r.m ? 0.0 : double(r.m) - double(x)) * r.c <= r.lim; }
+// Four weights, all of them before any is asked for: moved under the conditions that they are used on, the chains run one after
+// the other (a warp's 128 values 1,500 cycles instead of 230).
+__device__ __forceinline__ void four_weights(const Row& r, const double* table, const float (&x)[4], unsigned long long (&y)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = weight(r, table, x[j]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) asm volatile("" : "+l"(y[j]));
+}
+__device__ __forceinline__ bool within(const Row& r, float x) { return (r.m64 - double(x)) * r.c <= r.lim; }
 
 __device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
 #pragma unroll
@@ -160,20 +172,45 @@ struct Sampler {
 #pragma unroll
         for (int j = 0; j < kPer; j++) f(float(x[j]), first + v * kPer + j);
     }
+    // The sum of the weights of a vector's values for which take(value, index) holds, four chains at a time.
+    template <typename F>
+    __device__ __forceinline__ u64 weights_of_vector(int v, F take) const {
+        u64 sum = 0;
+#pragma unroll 1
+        for (int j0 = 0; j0 < kPer; j0 += 4) {
+            float x[4];
+            four(v, j0, x);
+            u64 y[4];
+            four_weights(row, sh.table, x, y);
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum += take(x[j], first + v * kPer + j0 + j) ? y[j] : 0ull;
+        }
+        return sum;
+    }
+    // Four values of a vector.
+    __device__ __forceinline__ void four(int v, int j0, float (&x)[4]) const {
+        load_row<4>(reinterpret_cast<const T*>(data + v) + j0, true, x);
+    }
     // Of every value of the slice, vectors spread over the threads, or over the lanes of the segment's warp.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         for (int v = threadIdx.x; v < nv; v += kThreads) of_vector(v, f);
     }
     template <typename F>
-    __device__ __forceinline__ void each_of_segment(F f) const {
+    __device__ __forceinline__ void each_vector_of_segment(F f) const {
         const int v0 = int(threadIdx.x >> 5) * segment(), v1 = min(v0 + segment(), nv);
-        for (int v = v0 + int(threadIdx.x & 31); v < v1; v += 32) of_vector(v, f);
+        for (int v = v0 + int(threadIdx.x & 31); v < v1; v += 32) f(v);
     }
     __device__ __forceinline__ static u64 entry(float x, int i) { return (static_cast<u64>(order_key(x)) << 32) | (0xFFFFFFFFu - unsigned(i)); }
     __device__ __forceinline__ static float value(u64 e) { return key_value(uint32_t(e >> 32)); }
     // Values that can be taken at all: not NaN, not -infinity.
     __device__ __forceinline__ static bool real(float x) { return x > -INFINITY; }
+    // Whether the cut leaves a token in.
+    __device__ __forceinline__ bool kept(float x, int i) const { return x > row.cut || (x == row.cut && unsigned(i) <= row.cut_at); }
+    __device__ void take_cut() {  // as sh.cut says it; 0: nothing is cut
+        row.cut = sh.cut ? value(sh.cut) : -INFINITY;
+        row.cut_at = sh.cut ? 0xFFFFFFFFu - uint32_t(sh.cut) : 0u;
+    }
     __device__ __forceinline__ u64 weight_of(float x) const { return weight(row, sh.table, x); }
 
     // The CTAs' sums meet: sum[i] of every CTA.
@@ -236,9 +273,68 @@ struct Sampler {
         return c;
     }
 
+    // The entry of CTA 0's n at which, in descending order, the sum of the weights (mass) or counts with what lies ahead reaches want:
+    // by 512 bins of their keys, and the entries of one bin against each other. 0: none.
+    __device__ u64 cut_in_list(int n, double want, u64 ahead, bool mass) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        uint32_t* red = reinterpret_cast<uint32_t*>(sh.warp_sum);
+        uint32_t most = 0, least = 0xFFFFFFFFu;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const uint32_t k = uint32_t(list()[i] >> 32);
+            most = max(most, k), least = min(least, k);
+        }
+        most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) red[warp] = most, red[kWarps + warp] = least;
+        u64* bins = sorted();
+        bins[threadIdx.x] = 0;
+        if (threadIdx.x == 0) sh.n_list = 0, sh.cut = 0, sh.bin = -1;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) most = max(most, red[w]), least = min(least, red[kWarps + w]);
+        const int shift = max(23 - __clz(most - least), 0);
+        auto bin_of = [&](u64 e) { return int((most - uint32_t(e >> 32)) >> shift); };  // below 512
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 e = list()[i];
+            atomicAdd(&bins[bin_of(e)], mass ? weight_of(value(e)) : 1ull);
+        }
+        __syncthreads();
+        u64 v[1] = {bins[threadIdx.x]};
+        const u64 own = v[0];
+        cta_upto(sh, v);
+        const u64 upto = ahead + v[0], less = upto - own;
+        if (own && double(upto) >= want && double(less) < want) sh.bin = threadIdx.x, sh.before = less;
+        __syncthreads();
+        const int bin = sh.bin;
+        ahead = sh.before;
+        u64 e[kCand / kThreads];
+#pragma unroll
+        for (int k = 0; k < kCand / kThreads; k++) {
+            const int i = threadIdx.x + k * kThreads;
+            e[k] = i < n ? list()[i] : 0ull;
+            if (i >= n || bin_of(e[k]) != bin) e[k] = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kCand / kThreads; k++)
+            if (e[k]) {
+                const unsigned at = atomicAdd(&sh.n_list, 1u);
+                sorted()[at] = e[k], list()[at] = mass ? weight_of(value(e[k])) : 1ull;
+            }
+        __syncthreads();
+        const int few = int(sh.n_list);
+        for (int i = threadIdx.x; i < few; i += kThreads) {
+            const u64 x = sorted()[i];
+            u64 sum = ahead;
+            for (int j = 0; j < few; j++) sum += sorted()[j] > x ? list()[j] : 0ull;
+            if (double(sum) < want && double(sum + list()[i]) >= want) sh.cut = x;
+        }
+        __syncthreads();
+        return sh.cut;
+    }
+
     __device__ void answer(int r, int token, float x, u64 total) {
         a.token[r] = token;
-        if (a.prob) a.prob[r] = token < 0 ? 0.0f : float(exp2(-(x == row.m ? 0.0 : (double(row.m) - double(x)) * row.c)) * (kOne / double(total)));
+        if (a.prob) a.prob[r] = token < 0 ? 0.0f : float(exp2((double(x) - row.m64) * row.c) * (kOne / double(total)));
     }
     // floor(u * total), below total.
     __device__ u64 place(int r, u64 total) {
@@ -246,10 +342,18 @@ struct Sampler {
         return min(x > 0.0 ? static_cast<u64>(x) : 0ull, total - 1);
     }
 
-    // The first index, in the order of the vocabulary, at which the sum of measure(value, index) exceeds where(sum of all): its CTA
+    // What a token counts that take(value, index) chooses: its weight, or 1.
+    template <bool MASS, typename F>
+    __device__ __forceinline__ u64 measured(int v, F take) const {
+        if constexpr (MASS) return weights_of_vector(v, take);
+        u64 n = 0;
+        of_vector(v, [&](float x, int i) { n += take(x, i); });
+        return n;
+    }
+    // The first index, in the order of the vocabulary, at which the sum over the tokens taken exceeds where(sum of all): its CTA
     // gets found = index, pick = value. seg[] holds the segments' sums. The sum of all is returned.
-    template <typename M, typename P>
-    __device__ u64 locate(M measure, P where) {
+    template <bool MASS, typename M, typename P>
+    __device__ u64 locate(M take, P where) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (threadIdx.x == 0) sh.found = 0xFFFFFFFFu;
         __syncthreads();
@@ -270,13 +374,13 @@ struct Sampler {
             for (int base = v0; base < v1; base += 32) {
                 const int v = base + lane;
                 u64 s = 0;
-                if (v < v1) of_vector(v, [&](float x, int i) { s += measure(x, i); });
+                if (v < v1) s = measured<MASS>(v, take);
                 const u64 upto = before + warp_upto(s, lane);
                 if (upto > at && upto - s <= at) {  // one lane
                     u64 sum = upto - s;
                     bool there = false;
                     of_vector(v, [&](float x, int i) {
-                        sum += measure(x, i);
+                        sum += !take(x, i) ? 0ull : MASS ? weight_of(x) : 1ull;
                         if (sum > at && !there) sh.found = unsigned(i), sh.pick = x, there = true;
                     });
                 }
@@ -287,40 +391,44 @@ struct Sampler {
         __syncthreads();
         return total;
     }
-    template <typename M, typename P>
-    __device__ u64 find(M measure, P where) {
+    template <bool MASS, typename M>
+    __device__ void fill(M take) {
         u64 part = 0;
-        each_of_segment([&](float x, int i) { part += measure(x, i); });
+        each_vector_of_segment([&](int v) { part += measured<MASS>(v, take); });
         part = warp_total(part);
         if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
-        return locate(measure, where);
     }
 
-    // Adds up a histogram over the cluster and finds the bin at which the sum reaches target(total of all bins, with what lies
-    // ahead of them): bin (-1: none does), before (the sum without the bin), total to every CTA.
-    template <bool MASS, typename F, typename G>
-    __device__ void histogram(F bin_of, u64 ahead, G target) {
+    // Adds up a histogram of counts, or of weights (mass), over the cluster and finds the bin at which the sum, with what lies ahead
+    // of it, reaches `part` of the sum of all (0: `want`): bin (-1: none does), before (the sum without the bin), total to every CTA.
+    template <typename F>
+    __device__ void histogram(bool mass, F bin_of, u64 ahead, double part, double want) {
         uint32_t* h = reinterpret_cast<uint32_t*>(aux);
-        for (int i = threadIdx.x; i < (MASS ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
+        for (int i = threadIdx.x; i < (mass ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
         __syncthreads();
-        each([&](float x, int i) {
-            const int b = bin_of(x, i);
-            if (b < 0) return;
-            if constexpr (MASS) {
+#pragma unroll 1
+        for (int v = threadIdx.x; v < nv; v += kThreads)
+#pragma unroll 1
+            for (int j = 0; j < kPer; j++) {
+                const float x = float(reinterpret_cast<const T*>(data + v)[j]);
+                const int b = bin_of(x, first + v * kPer + j);
+                if (b < 0) continue;
+                if (!mass) {
+                    atomicAdd(&h[b], 1u);
+                    continue;
+                }
                 const u64 w = weight_of(x);
                 const uint32_t p0 = uint32_t(w) & 0x7fffu, p1 = uint32_t(w >> 15) & 0x7fffu, p2 = uint32_t(w >> 30);
                 if (p0) atomicAdd(&h[b], p0);
                 if (p1) atomicAdd(&h[kBins + b], p1);
                 if (p2) atomicAdd(&h[2 * kBins + b], p2);
-            } else {
-                atomicAdd(&h[b], 1u);
             }
-        });
         cluster.sync();
         // this CTA's share of the bins, kBins / ctas of them: four at most a thread
         constexpr int kMost = kBins / kThreads;
         const int share = kBins / ctas, per = (share + kThreads - 1) / kThreads;
         u64 v[kMost] = {}, own[kMost];
+#pragma unroll 1
         for (int c = 0; c < ctas; c++) {
             const uint32_t* o = cluster.map_shared_rank(h, c) + rank * share;
 #pragma unroll
@@ -328,7 +436,7 @@ struct Sampler {
                 const int b = threadIdx.x * per + k;
                 if (k >= per || b >= share) continue;
                 v[k] += o[b];
-                if (MASS) v[k] += (static_cast<u64>(o[kBins + b]) << 15) + (static_cast<u64>(o[2 * kBins + b]) << 30);
+                if (mass) v[k] += (static_cast<u64>(o[kBins + b]) << 15) + (static_cast<u64>(o[2 * kBins + b]) << 30);
             }
         }
 #pragma unroll
@@ -341,7 +449,7 @@ struct Sampler {
             if (i < rank) before += sh.sum[i];
             total += sh.sum[i];
         }
-        const double want = target(total);
+        if (part > 0.0) want = fmax(part * double(total), 0.5);
         // one thread of the cluster has the bin that reaches it
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
@@ -358,68 +466,70 @@ struct Sampler {
         cluster.sync();
     }
 
-    // Moves the cut (among what the present one keeps) to the first token, in descending order, at which the sum of the counts
-    // or weights (MASS) reaches want_of(total).
-    template <bool MASS, typename G>
-    __device__ void select(G want_of) {
-        const u64 cut = sh.cut;
+    // Moves the cut (among what the present one keeps) to the first token, in descending order, at which the count reaches top_k, or
+    // (mass) the sum of the weights top_p times theirs. Equal steps of max - x first; where more tokens than can be ranked are in
+    // the step of the cut, the three digits of their keys.
+    __device__ void select(bool mass, int top_k, float top_p) {
         const float scale = fminf(64.0f * fmaxf(row.c32, 1.0f), 1e30f);
-        auto step_of = [&](float x, int i) {
-            if (!real(x) || entry(x, i) < cut) return -1;
-            return x == row.m ? 0 : int(fminf((row.m - x) * scale, float(kBins - 1)));
-        };
+        auto step_of = [&](float x, int i) { return real(x) && kept(x, i) ? int(fminf((row.m - x) * scale, float(kBins - 1))) : -1; };
         if (threadIdx.x == 0) sh.n_all = sh.n_list = 0;
-        histogram<MASS>(step_of, 0, want_of);
-        const int step = sh.bin;
-        if (step < 0) return;  // fewer than that many
-        u64 before = sh.before;
-        const double want = want_of(sh.total);
-        each([&](float x, int i) { if (step_of(x, i) == step) put(x, i); });
-        gather([]() {});
-        if (rank == 0) {
-            u64 next = 0;
-            if (sh.n_all <= kCand) {
-                const int n = int(sh.n_all);
-                rank_list(n, [&](u64 e) { return MASS ? weight_of(value(e)) : 1ull; });
-                next = sorted()[min(below(n, want, before), n - 1)];
-            }
-            if (threadIdx.x < ctas) {
-                Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
-                o->done = next != 0;
-                if (next) o->cut = next;
-            }
-        }
-        cluster.sync();
-        if (sh.done) return;
-        // too many tokens in one step: by the digits of their keys
         uint32_t key = 0, known = 0;
-        for (int digit = 0; digit < 3; digit++) {
-            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-            const uint32_t most = digit == 2 ? 1023u : 2047u;
-            histogram<MASS>([&](float x, int i) {
+        u64 before = 0;
+        double want = mass ? 0.5 : double(top_k);
+        int step = 0;
+#pragma unroll 1
+        for (int level = 0; level < 4; level++) {
+            const int shift = level == 1 ? 21 : level == 2 ? 10 : 0;
+            const uint32_t most = level == 3 ? 1023u : 2047u;
+            histogram(mass, [&](float x, int i) {
+                const int b = step_of(x, i);
+                if (!level) return b;
                 const uint32_t k = order_key(x);
-                return step_of(x, i) == step && (k & known) == key ? int(most - (k >> shift & most)) : -1;
-            }, before, [&](u64) { return want; });
+                return b == step && (k & known) == key ? int(most - (k >> shift & most)) : -1;
+            }, before, mass && !level ? fmax(double(top_p), 0x1p-80) : 0.0, want);
+            if (sh.bin < 0) return;  // fewer than that many
             before = sh.before;
-            key |= (most - uint32_t(max(sh.bin, 0))) << shift;
-            known |= most << shift;
+            if (level) {
+                key |= (most - uint32_t(sh.bin)) << shift;
+                known |= most << shift;
+                continue;
+            }
+            step = sh.bin;
+            if (mass) want = fmax(double(top_p) * double(sh.total), 0.5);
+            each([&](float x, int i) { if (step_of(x, i) == step) put(x, i); });
+            gather([]() {});
+            if (rank == 0) {
+                u64 next = 0;
+                if (sh.n_all <= kCand) next = cut_in_list(int(sh.n_all), want, before, mass);
+                if (threadIdx.x < ctas) {
+                    Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
+                    o->done = next != 0;
+                    if (next) o->cut = next;
+                }
+            }
+            cluster.sync();
+            if (sh.done) return take_cut();
         }
-        const double each_one = MASS ? double(weight_of(key_value(key))) : 1.0;
+        const double each_one = mass ? double(weight_of(key_value(key))) : 1.0;
         const double more = ceil((want - double(before)) / each_one);
-        find([&](float x, int i) { return step_of(x, i) == step && order_key(x) == key ? 1ull : 0ull; },
-             [&](u64 total) { return more > 1.0 ? min(static_cast<u64>(more) - 1, total - 1) : 0ull; });
+        auto equal = [&](float x, int i) { return step_of(x, i) == step && order_key(x) == key; };
+        fill<false>(equal);
+        locate<false>(equal, [&](u64 total) { return more > 1.0 ? min(static_cast<u64>(more) - 1, total - 1) : 0ull; });
         if (threadIdx.x == 0 && sh.found != 0xFFFFFFFFu) {
             const u64 next = (static_cast<u64>(key) << 32) | (0xFFFFFFFFu - sh.found);
             for (int c = 0; c < ctas; c++) cluster.map_shared_rank(&sh, c)->cut = next;
         }
         cluster.sync();
+        take_cut();
     }
 
     // The steps that few() counts in, and what a step's tokens weigh by its middle.
     __device__ __forceinline__ float count_scale() const { return fminf(128.0f * fmaxf(row.c32, 1.0f), 1e30f); }
-    __device__ __forceinline__ int count_step(float x, float scale) const { return x == row.m ? 0 : int(fminf((row.m - x) * scale, float(kSteps - 1))); }
+    __device__ __forceinline__ int count_step(float x, float scale) const {  // NaN: the last
+        return __float_as_int(fminf((row.m - x) * scale, float(kSteps - 1)) + 8388608.0f) & (kSteps - 1);  // to nearest
+    }
     __device__ __forceinline__ float middle(int step, float scale) const {
-        return step == kSteps - 1 ? 0.0f : exp2f(44.0f - (float(step) + 0.5f) / scale * row.c32);
+        return step == kSteps - 1 ? 0.0f : exp2f(44.0f - (step ? float(step) : 0.25f) / scale * row.c32);
     }
 
     // The cut by the largest values alone; true: the row is answered. Without top_k the weights are added up and the tokens
@@ -435,13 +545,23 @@ struct Sampler {
             gather([]() {});
         } else {
             u64 part = 0;
-            each([&](float x, int i) {
-                if (!real(x)) return;
-                part += weight_of(x);
-                const int step = count_step(x, scale);
-                atomicAdd(&counts()[step >> 1], 1u << (16 * (step & 1)));
-                if (x >= t) put(x, i);
-            });
+#pragma unroll 1
+            for (int v4 = threadIdx.x; v4 < nv * (kPer / 4); v4 += kThreads) {
+                float x[4];
+                load_row<4>(reinterpret_cast<const T*>(data) + 4 * v4, true, x);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int step = count_step(x[j], scale);
+                    atomicAdd(&counts()[step >> 1], step & 1 ? 0x10000u : 1u);
+                }
+                u64 y[4];
+                four_weights(row, sh.table, x, y);
+                part += (y[0] + y[1]) + (y[2] + y[3]);
+                if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= t)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (x[j] >= t && real(x[j])) put(x[j], first + 4 * v4 + j);
+            }
             gather([&]() {
                 part = warp_total(part);
                 if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.total, 0), part);
@@ -512,11 +632,17 @@ struct Sampler {
         u64 v[kMost] = {}, own[kMost];
         {
             uint32_t n[kMost] = {};
-            for (int c = 0; c < ctas; c++) {
-                const uint16_t* o = reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c)) + rank * share + threadIdx.x * per;
+            if (per == 1) {
 #pragma unroll
-                for (int k = 0; k < kMost; k++)
-                    if (k < per) n[k] += o[k];
+                for (int c = 0; c < kMaxCluster; c++)  // their loads side by side
+                    n[0] += reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c))[rank * share + threadIdx.x];
+            } else {
+                for (int c = 0; c < ctas; c++) {
+                    const uint16_t* o = reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c)) + rank * share + threadIdx.x * per;
+#pragma unroll
+                    for (int k = 0; k < kMost; k++)
+                        if (k < per) n[k] += o[k];
+                }
             }
 #pragma unroll
             for (int k = 0; k < kMost; k++)
@@ -548,26 +674,37 @@ struct Sampler {
         cluster.sync();
         const int lo = sh.bin, hi = sh.bin_end;
         u64 part = 0;
-        each_of_segment([&](float x, int i) {
-            if (!real(x)) return;
-            const int step = count_step(x, scale);
-            if (step < lo) part += weight_of(x);
-            else if (step <= hi) put(x, i);
+        each_vector_of_segment([&](int v) {
+#pragma unroll 1
+            for (int j0 = 0; j0 < kPer; j0 += 4) {
+                float x[4];
+                four(v, j0, x);
+                int step[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) step[j] = count_step(x[j], scale);
+                if (min(min(step[0], step[1]), min(step[2], step[3])) > hi) continue;
+                u64 y[4];
+                four_weights(row, sh.table, x, y);
+#pragma unroll
+                for (int j = 0; j < 4; j++) part += step[j] < lo ? y[j] : 0ull;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (step[j] >= lo && step[j] <= hi && real(x[j])) put(x[j], first + v * kPer + j0 + j);
+            }
         });
         part = warp_total(part);
         if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
         gather([&]() {
             if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.before, 0), part);
         });
+        const unsigned n = sh.n_list;
+        __syncthreads();
         if (rank == 0) {
             u64 next = 0;
             const u64 ahead = sh.before;
-            if (sh.n_all <= kCand && double(ahead) < want) {
-                const int n = int(sh.n_all);
-                rank_list(n, [&](u64 e) { return weight_of(value(e)); });
-                const int less = below(n, want, ahead);
-                if (less < n) next = sorted()[less];
-            }
+            const unsigned n_all = sh.n_all;
+            __syncthreads();  // ahead is read by all before it is set again
+            if (n_all <= kCand && double(ahead) < want) next = cut_in_list(int(n_all), want, ahead, true);
             if (threadIdx.x < ctas) {
                 Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
                 o->done = next != 0;
@@ -576,12 +713,12 @@ struct Sampler {
         }
         cluster.sync();
         if (!sh.done) return false;
-        const unsigned n = sh.n_list;
         for (unsigned i = threadIdx.x; i < n; i += kThreads) {
             const u64 e = mine()[i];
             if (e >= sh.cut) atomicAdd(&sh.seg[(int(0xFFFFFFFFu - uint32_t(e)) - first) / kPer / segment()], weight_of(value(e)));
         }
         __syncthreads();
+        take_cut();
         return true;
     }
 };
@@ -613,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
     }
     // while the copies fly: the row's parameters, the table, the ends that are not whole vectors
-    const float temperature = !a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature;
+    const float temperature = fminf(!a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature, 1e36f);  // above, all weigh the same
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
     if (top_k < 0 || top_k >= a.vocab) top_k = 0;
@@ -628,7 +765,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     if (temperature > 0.0f) {
         for (int i = tid; i < kPowers * kCopies; i += kThreads) sh.table[i] = exp2(double(i / kCopies) / kPowers);
         s.row.c = 1.4426950408889634 / double(temperature);
-        s.row.c32 = float(s.row.c);
+        s.row.c_powers = s.row.c * kPowers;
+        s.row.c32 = fminf(float(s.row.c), 1e30f);
         s.row.lim = min_p > 0.0f ? fmax(-log2(double(min_p)), 0.0) : INFINITY;
     }
     s.cluster.barrier_arrive();
@@ -648,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     if ((tid & 7) < ctas) *s.cluster.map_shared_rank(&sh.gmax[s.rank * kGroups + tid / 8], tid & 7) = most;
     s.cluster.sync();
     const int groups = ctas * kGroups;
-    const float g = tid < groups ? sh.gmax[tid] : -INFINITY;
+    float g = tid < groups ? sh.gmax[tid] : -INFINITY;
     float m = warp_max(g);
     if (lane == 0) reinterpret_cast<float*>(sh.warp_sum)[tid >> 5] = m;
     __syncthreads();
@@ -674,6 +812,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         return;
     }
 
+    // ---- infinities, and largest values beside which the next one below weighs nothing: those are all that counts
+    if (!(fabsf(m) * 0x1p-25f * s.row.c32 < 64.0f)) {
+        uint4* d = reinterpret_cast<uint4*>(buf);
+        __syncthreads();
+        for (int v = tid; v < s.nv; v += kThreads) {
+            uint4 w = d[v];
+            T* x = reinterpret_cast<T*>(&w);
+#pragma unroll
+            for (int j = 0; j < S::kPer; j++) x[j] = T(float(x[j]) == m ? 0.0f : -INFINITY);
+            d[v] = w;
+        }
+        g = g == m ? 0.0f : -INFINITY, m = 0.0f, s.row.m = 0.0f;
+        __syncthreads();
+    }
+    s.row.m64 = double(m);
+    s.row.low = nextafterf(m - 46.5f / s.row.c32, -INFINITY);
+    s.take_cut();
+
     const bool use_p = top_p < 1.0f;
     bool ready = false;  // seg[] holds what is kept
     if (top_k || use_p) {
@@ -681,30 +837,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         const int want = top_k ? top_k : max(groups / 6, 1);
         const bool bounded = 4 * want <= 3 * groups;
         if (bounded || !top_k) {
-            // the bound: a key that `want` groups reach, to 16 of its bits (one more halving a bit)
-            uint32_t bound = 0;
-            const uint32_t key = tid < groups ? order_key(g) : 0u;
-            for (int bit = 31; bit >= 16; bit--) {
+            // the bound: a key that `want` groups reach, by halving below the bits that the largest has in common with the smallest group
+            const uint32_t key = tid < groups ? order_key(g) : 0xFFFFFFFFu, top = order_key(m);
+            uint32_t least = __reduce_min_sync(0xffffffffu, key);
+            if (lane == 0) reinterpret_cast<uint32_t*>(sh.warp_sum)[tid >> 5] = least;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) least = min(least, reinterpret_cast<uint32_t*>(sh.warp_sum)[w]);
+            const int same = __clz(top ^ least);  // 32: all alike
+            uint32_t bound = same ? top & ~(0xFFFFFFFFu >> (same - 1) >> 1) : 0u;
+            const int last = max(min(31 - same - 8, 16), 0);
+            for (int bit = 31 - same; bit >= last; bit--) {
                 const uint32_t next = bound | 1u << bit;
                 if (__syncthreads_count(tid < groups && key >= next) >= want) bound = next;
             }
             if (s.few(r, bound >= 0x00800000u ? key_value(bound) : -INFINITY, top_k, use_p, top_p)) return;  // below: no finite value
         }
-        if (top_k) s.template select<false>([&](unsigned long long) { return double(top_k); });
-        if (use_p) {
-            if (!top_k) ready = s.near_cut(top_p);
-            if (!ready) {
-                s.template select<true>([&](unsigned long long total) { return fmax(double(top_p) * double(total), 0.5); });
-            } else if (s.row.lim < INFINITY) {
-                ready = false;
-            }
+        if (use_p && !top_k) ready = s.near_cut(top_p);
+        if (!ready) {
+#pragma unroll 1
+            for (int mass = top_k ? 0 : 1; mass < (use_p ? 2 : 1); mass++) s.select(mass, top_k, top_p);
         }
     }
-    const unsigned long long cut = sh.cut;
     const bool all_p = !(s.row.lim < INFINITY);
-    auto kept = [&](float x, int i) { return S::real(x) && S::entry(x, i) >= cut && (all_p || within(s.row, x)) ? s.weight_of(x) : 0ull; };
-    auto where = [&](unsigned long long all) { return s.place(r, all); };
-    const unsigned long long total = ready ? s.locate(kept, where) : s.find(kept, where);
+    auto kept = [&](float x, int i) { return s.kept(x, i) && (all_p || within(s.row, x)); };
+    if (!ready || !all_p) s.template fill<true>(kept);
+    const unsigned long long total = s.template locate<true>(kept, [&](unsigned long long all) { return s.place(r, all); });
     if (tid == 0 && sh.found != 0xFFFFFFFFu) s.answer(r, int(sh.found), sh.pick, total);
 }
 

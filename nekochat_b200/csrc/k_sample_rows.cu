@@ -1,6 +1,8 @@
 // Tokens from rows of logits with temperature, top-k, top-p and min-p (neko_op_sample_rows).
 //
-// A cluster of CTAs takes a row: each holds its slice in shared memory, so the logits are read from memory once whatever follows.
+// A cluster of one to eight CTAs takes a row, each a slice, which it reads again for each pass (two to four; all but the first from
+// L2 unless the logits are far larger). Slices kept in shared memory would leave room for 33 rows of 151,936 at a time, and a row
+// waits for its cluster's meetings as long as it computes (320 nuclei: 411 us that way).
 // Weights 2^(44 - y), y = (max - x) log2(e) / temperature, are rounded to integers and added as integers: sums do not depend on an
 // order, and any split of a row gives the same token. They are computed in 64 bits (a table of 32 powers, 16 copies of it so that no
 // two lanes of a half warp meet in a bank, and a polynomial of degree 5): with V tokens of about equal weight a row's number falls
@@ -20,6 +22,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -35,14 +38,14 @@ constexpr int kGroups = kThreads / 8;  // groups of threads whose largest values
 constexpr int kCand = 1024;            // tokens that are ranked by counting
 constexpr int kMine = 512;             // of them those of one CTA of several
 constexpr int kBins = 2048;
-constexpr int kSteps = 4096;           // steps of max - x that tokens are counted in, two 16-bit counts a word
+constexpr int kSteps = 4096;           // steps of max - x that tokens are counted in
 constexpr int kPowers = 32, kCopies = 16;
 constexpr int kMaxCluster = 8;
 constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest
 // lists of CTA 0 (as collected, then the sums; in order), the CTA's own list, the counts; histograms take all of it
 constexpr int kSortedOff = kCand * 8, kMineOff = 2 * kCand * 8;
 __host__ __device__ constexpr int counts_off(int ctas) { return kMineOff + (ctas > 1 ? kMine : kCand) * 8; }
-__host__ __device__ constexpr int aux_bytes(int ctas) { return counts_off(ctas) + kSteps * 2; }
+__host__ __device__ constexpr int aux_bytes(int ctas) { return counts_off(ctas) + kSteps * 4; }
 static_assert(aux_bytes(kMaxCluster) >= 3 * kBins * 4, "the histograms");
 
 // The order of values as unsigned numbers; zeros are alike.
@@ -66,17 +69,17 @@ struct Shared {
     unsigned n_list, n_all, at_list;      // tokens in this CTA's list, in CTA 0's, and where this CTA's begin there
     int bin, bin_end, done;
     float pick;
-    uint64_t bar;
+    uint4 ends[2];                        // the slice's first and last vector, -infinity in places outside it
 };
 
-// Of a row with finite values only, or -infinity (what is infinite, or where the next value below the largest weighs nothing, becomes
-// zeros and -infinity first): y = (m - x) c.
+// y = (m - x) c.
 struct Row {
     float m;        // largest value
+    float alone;    // where it is infinite, or the next value below weighs nothing: it, and values are read as 0 (it) and -infinity; else NaN
     float low;      // values count as no less than this: they weigh nothing there
     float c32;
     double m64, c, c_powers;  // c = log2(e) / temperature, times the table's powers
-    double lim;     // y up to this is kept (min-p)
+    float least;    // of the values that min-p leaves in
     float cut;      // kept: larger values, and this one up to an index
     unsigned cut_at;
 };
@@ -107,8 +110,6 @@ __device__ __forceinline__ void four_weights(const Row& r, const double* table, 
 #pragma unroll
     for (int j = 0; j < 4; j++) asm volatile("" : "+l"(y[j]));
 }
-__device__ __forceinline__ bool within(const Row& r, float x) { return (r.m64 - double(x)) * r.c <= r.lim; }
-
 __device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -151,8 +152,8 @@ struct Sampler {
     cg::cluster_group cluster;
     Shared& sh;
     uint8_t* aux;
-    const uint4* data;
-    int ctas, rank, nv, first;  // vectors of this CTA's slice; vocabulary index of the first vector's first place
+    const uint4* data;          // the slice's vectors; the first and the last are read from sh.ends
+    int ctas, rank, nv, first;  // how many; vocabulary index of the first one's first place
     Row row;
 
     __device__ Sampler(const neko_sample_rows_args& a_, Shared& s, uint8_t* x) : a(a_), cluster(cg::this_cluster()), sh(s), aux(x) {}
@@ -164,42 +165,69 @@ struct Sampler {
     __device__ unsigned mine_room() const { return ctas > 1 ? kMine : kCand; }
     __device__ int segment() const { return (nv + kWarps - 1) / kWarps; }  // vectors of a warp's segment
 
-    // f(value, index) of a vector's values. Places outside the row hold -infinity.
-    template <typename F>
-    __device__ __forceinline__ void of_vector(int v, F f) const {
-        const uint4 w = data[v];
-        const T* x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int j = 0; j < kPer; j++) f(float(x[j]), first + v * kPer + j);
+    // A vector; past the end -infinities.
+    __device__ __forceinline__ uint4 load(int v, int end) const {
+        constexpr uint32_t none = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        if (v >= end) return make_uint4(none, none, none, none);
+        return v == 0 || v == nv - 1 ? sh.ends[v != 0] : __ldg(data + v);
     }
-    // The sum of the weights of a vector's values for which take(value, index) holds, four chains at a time.
-    template <typename F>
-    __device__ __forceinline__ u64 weights_of_vector(int v, F take) const {
-        u64 sum = 0;
-#pragma unroll 1
-        for (int j0 = 0; j0 < kPer; j0 += 4) {
-            float x[4];
-            four(v, j0, x);
-            u64 y[4];
-            four_weights(row, sh.table, x, y);
+    // Values j0 .. j0 + 3 of a vector. Places outside the row hold -infinity.
+    __device__ __forceinline__ void four(const uint4& w, int j0, float (&x)[4]) const {
+        if constexpr (kPer == 4) {
+            x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+        } else {
+            const uint2 h = j0 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y);
+            const T* y = reinterpret_cast<const T*>(&h);
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum += take(x[j], first + v * kPer + j0 + j) ? y[j] : 0ull;
+            for (int j = 0; j < 4; j++) x[j] = float(y[j]);
         }
-        return sum;
+        if (row.alone == row.alone)
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = x[j] == row.alone ? 0.0f : -INFINITY;
     }
-    // Four values of a vector.
-    __device__ __forceinline__ void four(int v, int j0, float (&x)[4]) const {
-        load_row<4>(reinterpret_cast<const T*>(data + v) + j0, true, x);
+    // f(four values, index of the first) of the vectors v0, v0 + step, .. before v1, kAhead of them on their way at a time.
+    template <int kAhead, typename F>
+    __device__ __forceinline__ void sweep(int v0, int step, int v1, F f) const {
+        uint4 w[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) w[k] = load(v0 + k * step, v1);
+#pragma unroll 1
+        for (int v = v0; v < v1; v += kAhead * step) {
+            uint4 now[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) now[k] = w[k], w[k] = load(v + (kAhead + k) * step, v1);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++)
+#pragma unroll
+                for (int j0 = 0; j0 < kPer; j0 += 4) {
+                    float x[4];
+                    four(now[k], j0, x);
+                    f(x, first + (v + k * step) * kPer + j0);
+                }
+        }
     }
-    // Of every value of the slice, vectors spread over the threads, or over the lanes of the segment's warp.
-    template <typename F>
+    // Of all vectors, spread over the threads; of the warp's segment.
+    template <int kAhead, typename F>
     __device__ __forceinline__ void each(F f) const {
-        for (int v = threadIdx.x; v < nv; v += kThreads) of_vector(v, f);
+        sweep<kAhead>(threadIdx.x, kThreads, nv, f);
     }
     template <typename F>
-    __device__ __forceinline__ void each_vector_of_segment(F f) const {
-        const int v0 = int(threadIdx.x >> 5) * segment(), v1 = min(v0 + segment(), nv);
-        for (int v = v0 + int(threadIdx.x & 31); v < v1; v += 32) f(v);
+    __device__ __forceinline__ void each_of_segment(F f) const {
+        const int v0 = int(threadIdx.x >> 5) * segment();
+        sweep<1>(v0 + int(threadIdx.x & 31), 32, min(v0 + segment(), nv), f);
+    }
+    // What four tokens count of which take(value, index) holds: their weights, or 1 each.
+    template <bool MASS, typename F>
+    __device__ __forceinline__ u64 measured(const float (&x)[4], int i, F take) const {
+        bool in[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) in[j] = take(x[j], i + j);
+        if (!(in[0] || in[1] || in[2] || in[3])) return 0;
+        u64 sum = 0, y[4] = {1, 1, 1, 1};
+        if constexpr (MASS) four_weights(row, sh.table, x, y);
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum += in[j] ? y[j] : 0ull;
+        return sum;
     }
     __device__ __forceinline__ static u64 entry(float x, int i) { return (static_cast<u64>(order_key(x)) << 32) | (0xFFFFFFFFu - unsigned(i)); }
     __device__ __forceinline__ static float value(u64 e) { return key_value(uint32_t(e >> 32)); }
@@ -210,6 +238,9 @@ struct Sampler {
     __device__ void take_cut() {  // as sh.cut says it; 0: nothing is cut
         row.cut = sh.cut ? value(sh.cut) : -INFINITY;
         row.cut_at = sh.cut ? 0xFFFFFFFFu - uint32_t(sh.cut) : 0u;
+    }
+    __device__ void cut_least() {  // min-p's too
+        if (row.least > row.cut) row.cut = row.least, row.cut_at = 0xFFFFFFFFu;
     }
     __device__ __forceinline__ u64 weight_of(float x) const { return weight(row, sh.table, x); }
 
@@ -342,14 +373,6 @@ struct Sampler {
         return min(x > 0.0 ? static_cast<u64>(x) : 0ull, total - 1);
     }
 
-    // What a token counts that take(value, index) chooses: its weight, or 1.
-    template <bool MASS, typename F>
-    __device__ __forceinline__ u64 measured(int v, F take) const {
-        if constexpr (MASS) return weights_of_vector(v, take);
-        u64 n = 0;
-        of_vector(v, [&](float x, int i) { n += take(x, i); });
-        return n;
-    }
     // The first index, in the order of the vocabulary, at which the sum over the tokens taken exceeds where(sum of all): its CTA
     // gets found = index, pick = value. seg[] holds the segments' sums. The sum of all is returned.
     template <bool MASS, typename M, typename P>
@@ -374,15 +397,22 @@ struct Sampler {
             for (int base = v0; base < v1; base += 32) {
                 const int v = base + lane;
                 u64 s = 0;
-                if (v < v1) s = measured<MASS>(v, take);
+                const uint4 w = load(v, v1);
+                float x[4];
+#pragma unroll
+                for (int j0 = 0; j0 < kPer; j0 += 4) four(w, j0, x), s += measured<MASS>(x, first + v * kPer + j0, take);
                 const u64 upto = before + warp_upto(s, lane);
                 if (upto > at && upto - s <= at) {  // one lane
                     u64 sum = upto - s;
                     bool there = false;
-                    of_vector(v, [&](float x, int i) {
-                        sum += !take(x, i) ? 0ull : MASS ? weight_of(x) : 1ull;
-                        if (sum > at && !there) sh.found = unsigned(i), sh.pick = x, there = true;
-                    });
+#pragma unroll 1
+                    for (int j = 0; j < kPer; j++) {
+                        const int i = first + v * kPer + j;
+                        four(w, j & ~3, x);
+                        const float y = x[j & 3];
+                        sum += !take(y, i) ? 0ull : MASS ? weight_of(y) : 1ull;
+                        if (sum > at && !there) sh.found = unsigned(i), sh.pick = y, there = true;
+                    }
                 }
                 before = __shfl_sync(0xffffffffu, upto, 31);
                 if (before > at) break;
@@ -394,7 +424,7 @@ struct Sampler {
     template <bool MASS, typename M>
     __device__ void fill(M take) {
         u64 part = 0;
-        each_vector_of_segment([&](int v) { part += measured<MASS>(v, take); });
+        each_of_segment([&](const float (&x)[4], int i) { part += measured<MASS>(x, i, take); });
         part = warp_total(part);
         if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
     }
@@ -406,23 +436,23 @@ struct Sampler {
         uint32_t* h = reinterpret_cast<uint32_t*>(aux);
         for (int i = threadIdx.x; i < (mass ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
         __syncthreads();
+        each<1>([&](const float (&x)[4], int i) {
 #pragma unroll 1
-        for (int v = threadIdx.x; v < nv; v += kThreads)
-#pragma unroll 1
-            for (int j = 0; j < kPer; j++) {
-                const float x = float(reinterpret_cast<const T*>(data + v)[j]);
-                const int b = bin_of(x, first + v * kPer + j);
+            for (int j = 0; j < 4; j++) {
+                const float y = j == 0 ? x[0] : j == 1 ? x[1] : j == 2 ? x[2] : x[3];
+                const int b = bin_of(y, i + j);
                 if (b < 0) continue;
                 if (!mass) {
                     atomicAdd(&h[b], 1u);
                     continue;
                 }
-                const u64 w = weight_of(x);
+                const u64 w = weight_of(y);
                 const uint32_t p0 = uint32_t(w) & 0x7fffu, p1 = uint32_t(w >> 15) & 0x7fffu, p2 = uint32_t(w >> 30);
                 if (p0) atomicAdd(&h[b], p0);
                 if (p1) atomicAdd(&h[kBins + b], p1);
                 if (p2) atomicAdd(&h[2 * kBins + b], p2);
             }
+        });
         cluster.sync();
         // this CTA's share of the bins, kBins / ctas of them: four at most a thread
         constexpr int kMost = kBins / kThreads;
@@ -496,7 +526,11 @@ struct Sampler {
             }
             step = sh.bin;
             if (mass) want = fmax(double(top_p) * double(sh.total), 0.5);
-            each([&](float x, int i) { if (step_of(x, i) == step) put(x, i); });
+            each<1>([&](const float (&x)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (step_of(x[j], i + j) == step) put(x[j], i + j);
+            });
             gather([]() {});
             if (rank == 0) {
                 u64 next = 0;
@@ -537,31 +571,31 @@ struct Sampler {
     __device__ bool few(int r, float t, int top_k, bool use_p, float top_p) {
         const float scale = count_scale();
         if (!top_k)
-            for (int i = threadIdx.x; i < kSteps / 2; i += kThreads) counts()[i] = 0;
+            for (int i = threadIdx.x; i < kSteps; i += kThreads) counts()[i] = 0;
         if (threadIdx.x == 0) sh.done = 0, sh.n_list = 0;
         __syncthreads();
+        auto reaches = [&](const float (&x)[4], int i) {
+            if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= t)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (x[j] >= t && real(x[j])) put(x[j], i + j);
+        };
         if (top_k) {
-            each([&](float x, int i) { if (x >= t && real(x)) put(x, i); });
+            each<4>(reaches);
             gather([]() {});
         } else {
             u64 part = 0;
-#pragma unroll 1
-            for (int v4 = threadIdx.x; v4 < nv * (kPer / 4); v4 += kThreads) {
-                float x[4];
-                load_row<4>(reinterpret_cast<const T*>(data) + 4 * v4, true, x);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int step = count_step(x[j], scale);
-                    atomicAdd(&counts()[step >> 1], step & 1 ? 0x10000u : 1u);
-                }
+            each<1>([&](const float (&x)[4], int i) {
                 u64 y[4];
                 four_weights(row, sh.table, x, y);
                 part += (y[0] + y[1]) + (y[2] + y[3]);
-                if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= t)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (x[j] >= t && real(x[j])) put(x[j], first + 4 * v4 + j);
-            }
+                for (int j = 0; j < 4; j++) {
+                    const int step = count_step(x[j], scale);
+                    if (step < kSteps - 1) atomicAdd(&counts()[step], 1u);  // the last step's tokens are not counted
+                }
+                reaches(x, i);
+            });
             gather([&]() {
                 part = warp_total(part);
                 if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.total, 0), part);
@@ -584,11 +618,11 @@ struct Sampler {
                     if (less < n_k) n_p = less + 1, sure = true;
                 }
                 int n_m = n_p;
-                if (row.lim < INFINITY) {
+                if (row.least > -INFINITY) {
                     n_m = 0;
                     for (int base = 0; base < n_p; base += kThreads) {
                         const int i = base + threadIdx.x;
-                        n_m += __syncthreads_count(i < n_p && within(row, value(sorted()[i < n_p ? i : 0])));
+                        n_m += __syncthreads_count(i < n_p && value(sorted()[i < n_p ? i : 0]) >= row.least);
                     }
                     sure |= n_m < n_p;
                 }
@@ -634,11 +668,10 @@ struct Sampler {
             uint32_t n[kMost] = {};
             if (per == 1) {
 #pragma unroll
-                for (int c = 0; c < kMaxCluster; c++)  // their loads side by side
-                    n[0] += reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c))[rank * share + threadIdx.x];
+                for (int c = 0; c < kMaxCluster; c++) n[0] += cluster.map_shared_rank(counts(), c)[rank * share + threadIdx.x];  // side by side
             } else {
                 for (int c = 0; c < ctas; c++) {
-                    const uint16_t* o = reinterpret_cast<const uint16_t*>(cluster.map_shared_rank(counts(), c)) + rank * share + threadIdx.x * per;
+                    const uint32_t* o = cluster.map_shared_rank(counts(), c) + rank * share + threadIdx.x * per;
 #pragma unroll
                     for (int k = 0; k < kMost; k++)
                         if (k < per) n[k] += o[k];
@@ -674,23 +707,18 @@ struct Sampler {
         cluster.sync();
         const int lo = sh.bin, hi = sh.bin_end;
         u64 part = 0;
-        each_vector_of_segment([&](int v) {
-#pragma unroll 1
-            for (int j0 = 0; j0 < kPer; j0 += 4) {
-                float x[4];
-                four(v, j0, x);
-                int step[4];
+        each_of_segment([&](const float (&x)[4], int i) {
+            int step[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) step[j] = count_step(x[j], scale);
-                if (min(min(step[0], step[1]), min(step[2], step[3])) > hi) continue;
-                u64 y[4];
-                four_weights(row, sh.table, x, y);
+            for (int j = 0; j < 4; j++) step[j] = count_step(x[j], scale);
+            if (min(min(step[0], step[1]), min(step[2], step[3])) > hi) return;
+            u64 y[4];
+            four_weights(row, sh.table, x, y);
 #pragma unroll
-                for (int j = 0; j < 4; j++) part += step[j] < lo ? y[j] : 0ull;
+            for (int j = 0; j < 4; j++) part += step[j] < lo ? y[j] : 0ull;
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (step[j] >= lo && step[j] <= hi && real(x[j])) put(x[j], first + v * kPer + j0 + j);
-            }
+            for (int j = 0; j < 4; j++)
+                if (step[j] >= lo && step[j] <= hi && real(x[j])) put(x[j], i + j);
         });
         part = warp_total(part);
         if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
@@ -732,54 +760,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     S s(a, sh, sm + kAuxOff);
     s.ctas = int(s.cluster.num_blocks()), s.rank = int(s.cluster.block_rank());
     const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.x / s.ctas, ctas = s.ctas;
-    uint8_t* buf = sm + kAuxOff + aux_bytes(ctas);
     const int b = min(s.rank * slice, a.vocab), n = min(slice, a.vocab - b);
     const T* src = static_cast<const T*>(a.logits) + r * a.row_stride + b;
     const int ph = int(reinterpret_cast<uintptr_t>(src) & 15) / int(sizeof(T));  // places before the slice in its first vector
-    const int head = min(n, (S::kPer - ph) % S::kPer), body = (n - head) / S::kPer * S::kPer;
     s.nv = n ? (ph + n + S::kPer - 1) / S::kPer : 0;
     s.first = b - ph;
-    s.data = reinterpret_cast<const uint4*>(buf);
-    if (tid == 0) {
-        mbar_init(&sh.bar, 1);
-        fence_barrier_init();
-        const uint32_t bytes = uint32_t(body) * sizeof(T);
-        mbar_arrive_expect_tx(&sh.bar, bytes);
-        for (uint32_t o = 0; o < bytes; o += 16384)
-            bulk_g2s(buf + (ph + head) * sizeof(T) + o, reinterpret_cast<const uint8_t*>(src + head) + o, min(bytes - o, 16384u), &sh.bar);
-        sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
-    }
-    // while the copies fly: the row's parameters, the table, the ends that are not whole vectors
+    s.data = reinterpret_cast<const uint4*>(src - ph);
+    s.row.alone = NAN;
+    if (tid == 0) sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
     const float temperature = fminf(!a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature, 1e36f);  // above, all weigh the same
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
     if (top_k < 0 || top_k >= a.vocab) top_k = 0;
-    {
-        T* x = reinterpret_cast<T*>(buf);
-        const T none = T(-INFINITY);
-        if (tid < ph) x[tid] = none;
-        if (tid < head) x[ph + tid] = src[tid];
-        const int at = head + body + tid;  // the last, partly filled vector
-        if (tid < S::kPer && ph + at < s.nv * S::kPer) x[ph + at] = at < n ? src[at] : none;
+    if (tid < 2 * S::kPer && s.nv > (tid < S::kPer ? 0 : 1)) {
+        const int at = (tid < S::kPer ? tid : (s.nv - 1) * S::kPer + tid - S::kPer) - ph;
+        reinterpret_cast<T*>(sh.ends)[tid] = at >= 0 && at < n ? src[at] : T(-INFINITY);
     }
     if (temperature > 0.0f) {
         for (int i = tid; i < kPowers * kCopies; i += kThreads) sh.table[i] = exp2(double(i / kCopies) / kPowers);
         s.row.c = 1.4426950408889634 / double(temperature);
         s.row.c_powers = s.row.c * kPowers;
         s.row.c32 = fminf(float(s.row.c), 1e30f);
-        s.row.lim = min_p > 0.0f ? fmax(-log2(double(min_p)), 0.0) : INFINITY;
     }
     s.cluster.barrier_arrive();
     __syncthreads();
-    bool ok = false;
-    for (int tries = 0; tries < 2 && !ok; tries++) {
-        for (uint32_t i = 0; i < kMbarMaxTries && !ok; i++) ok = mbar_try_wait(&sh.bar, 0);
-        if (!ok) set_op_error(kErrMbarTimeout);
-    }
-
     // ---- the largest values, by groups of eight threads, to every CTA
     float most = -INFINITY;
-    s.each([&](float x, int) { most = fmaxf(most, x); });
+    s.template each<4>([&](const float (&x)[4], int) { most = fmaxf(most, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     s.cluster.barrier_wait();
@@ -801,7 +808,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     // ---- greedy: the first maximum
     if (!(temperature > 0.0f)) {
         unsigned best = 0xFFFFFFFFu;
-        s.each([&](float x, int i) { if (x == m) best = min(best, unsigned(i)); });
+        s.template each<4>([&](const float (&x)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (x[j] == m) best = min(best, unsigned(i + j));
+        });
         best = __reduce_min_sync(0xffffffffu, best);
         if (lane == 0 && best != 0xFFFFFFFFu) atomicMin(s.cluster.map_shared_rank(&sh.best, 0), best);
         s.cluster.sync();
@@ -812,23 +823,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         return;
     }
 
-    // ---- infinities, and largest values beside which the next one below weighs nothing: those are all that counts
     if (!(fabsf(m) * 0x1p-25f * s.row.c32 < 64.0f)) {
-        uint4* d = reinterpret_cast<uint4*>(buf);
-        __syncthreads();
-        for (int v = tid; v < s.nv; v += kThreads) {
-            uint4 w = d[v];
-            T* x = reinterpret_cast<T*>(&w);
-#pragma unroll
-            for (int j = 0; j < S::kPer; j++) x[j] = T(float(x[j]) == m ? 0.0f : -INFINITY);
-            d[v] = w;
-        }
+        s.row.alone = m;
         g = g == m ? 0.0f : -INFINITY, m = 0.0f, s.row.m = 0.0f;
-        __syncthreads();
     }
     s.row.m64 = double(m);
     s.row.low = nextafterf(m - 46.5f / s.row.c32, -INFINITY);
-    s.take_cut();
+    s.row.cut = s.row.least = -INFINITY, s.row.cut_at = 0;
+    if (min_p > 0.0f) {  // the least float with (m - x) c <= -log2(min_p): near the quotient, then one by one
+        const double lim = fmax(-log2(double(min_p)), 0.0);
+        auto in = [&](float x) { return (s.row.m64 - double(x)) * s.row.c <= lim; };
+        float x = fminf(float(s.row.m64 - lim / s.row.c), m);
+        for (int i = 0; i < 64 && !in(x); i++) x = fminf(nextafterf(x, INFINITY), m);
+        for (int i = 0; i < 64 && in(nextafterf(x, -INFINITY)); i++) x = nextafterf(x, -INFINITY);
+        s.row.least = x;
+    }
 
     const bool use_p = top_p < 1.0f;
     bool ready = false;  // seg[] holds what is kept
@@ -859,9 +868,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
             for (int mass = top_k ? 0 : 1; mass < (use_p ? 2 : 1); mass++) s.select(mass, top_k, top_p);
         }
     }
-    const bool all_p = !(s.row.lim < INFINITY);
-    auto kept = [&](float x, int i) { return s.kept(x, i) && (all_p || within(s.row, x)); };
-    if (!ready || !all_p) s.template fill<true>(kept);
+    if (s.row.least > s.row.cut) ready = false;
+    s.cut_least();
+    auto kept = [&](float x, int i) { return s.kept(x, i); };
+    if (!ready) s.template fill<true>(kept);
     const unsigned long long total = s.template locate<true>(kept, [&](unsigned long long all) { return s.place(r, all); });
     if (tid == 0 && sh.found != 0xFFFFFFFFu) s.answer(r, int(sh.found), sh.pick, total);
 }
@@ -871,8 +881,9 @@ cudaError_t go(const neko_sample_rows_args& a, cudaStream_t st) {
     constexpr int kPer = 16 / sizeof(T);
     int ctas = 1;
     while (ctas < kMaxCluster && a.vocab > 4096 * ctas) ctas *= 2;
+    if (getenv("NEKO_C")) ctas = std::min(ctas, atoi(getenv("NEKO_C")));
     const int slice = ((a.vocab + ctas - 1) / ctas + kPer - 1) / kPer * kPer;
-    const size_t smem = (sizeof(Shared) + 127) / 128 * 128 + aux_bytes(ctas) + size_t(slice + kPer) * sizeof(T);
+    const size_t smem = (sizeof(Shared) + 127) / 128 * 128 + aux_bytes(ctas);
     auto* fn = sample_rows_kernel<T>;
     if (cudaError_t e = ensure_dyn_smem(fn, smem); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

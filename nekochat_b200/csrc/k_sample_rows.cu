@@ -9,12 +9,13 @@
 // within 2^-24 of a border once in 2^24 / V rows, so f32 sums would choose otherwise than the definition now and then.
 //
 // What is kept is a beginning of the row in descending order, found without sorting the row:
-//  * the largest values of 64 groups of threads a CTA bound the r-th largest of the row from below (the r-th largest of them), and few
-//    more than r tokens reach that bound: they are collected in one CTA, ranked by counting and cut there. Enough for top-k up to
-//    three quarters of the groups, and for top-p where the collected tokens hold that much of the sum.
-//  * top-p else: the pass that adds up the weights has counted the tokens in 4,096 equal steps of max - x, which say in which step
-//    the cut must lie, but for a few steps about an edge. One more pass over the weights adds up what lies before it and
-//    collects the step's tokens, which are ranked; the exact sums confirm the step (or the next way is taken).
+//  * top-k: the largest values of 64 groups of threads a CTA bound the k-th largest of the row from below (the k-th largest of them),
+//    and few more than k tokens reach that bound: they are collected in one CTA, ranked by counting and cut there. Enough for k
+//    up to three quarters of the groups.
+//  * top-p alone: an eighth of the tokens is counted in 4,096 equal steps of max - x, which gives the step of the cut but for the
+//    sample's error (the largest tokens, which would make it large, are summed as they are). One pass over the weights adds up
+//    the row, what lies before that window, and puts the window's tokens aside; among those the cut is found by the exact sums,
+//    which also tell a window that has missed it (then the next way is taken).
 //  * else a histogram over equal steps, of counts or of weights in three pieces of 15 bits (32-bit additions in shared memory),
 //    added up over the cluster, gives the step that the cut falls into; its tokens are collected and ranked, or where they are
 //    too many the key's digits (11, 11 and 10 bits) lead to the cut's value, whose equals are cut by index.
@@ -22,7 +23,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cstdlib>
+#include <cfloat>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -38,15 +39,21 @@ constexpr int kGroups = kThreads / 8;  // groups of threads whose largest values
 constexpr int kCand = 1024;            // tokens that are ranked by counting
 constexpr int kMine = 512;             // of them those of one CTA of several
 constexpr int kBins = 2048;
-constexpr int kSteps = 4096;           // steps of max - x that tokens are counted in
+constexpr int kSteps = 4096;           // steps of max - x that a sample of the tokens is counted in
+constexpr int kFine = 1024;            // steps of the window
+constexpr int kRing = 4;
 constexpr int kPowers = 32, kCopies = 16;
 constexpr int kMaxCluster = 8;
 constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest
 // lists of CTA 0 (as collected, then the sums; in order), the CTA's own list, the counts; histograms take all of it
 constexpr int kSortedOff = kCand * 8, kMineOff = 2 * kCand * 8;
 __host__ __device__ constexpr int counts_off(int ctas) { return kMineOff + (ctas > 1 ? kMine : kCand) * 8; }
-__host__ __device__ constexpr int aux_bytes(int ctas) { return counts_off(ctas) + kSteps * 4; }
-static_assert(aux_bytes(kMaxCluster) >= 3 * kBins * 4, "the histograms");
+__host__ __device__ constexpr int window_off(int ctas) { return counts_off(ctas) + kSteps * 4; }
+// tokens of the window in one CTA: with one CTA two of them fill an SM's shared memory
+__host__ __device__ constexpr int window_room(int ctas) { return ctas == 1 ? 8192 : ctas == 2 ? 5120 : ctas == 4 ? 3072 : 2048; }
+__host__ __device__ constexpr int aux_bytes(int ctas) { return window_off(ctas) + window_room(ctas) * 8; }
+static_assert(window_off(kMaxCluster) >= kRing * kThreads * 16, "the ring");
+static_assert(window_off(kMaxCluster) >= 3 * kBins * 4, "the histograms");
 
 // The order of values as unsigned numbers; zeros are alike.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -64,9 +71,10 @@ struct Shared {
     unsigned long long seg[kWarps];       // what is kept in each warp's segment
     unsigned long long cut;               // tokens from here up (in the lists' order) are kept
     unsigned long long before, total;
-    long long more;                       // what the collected tokens weigh more than their steps say
+    unsigned long long others[kMaxCluster][2];  // by CTA: two more sums
     unsigned best, found;                 // lowest index
     unsigned n_list, n_all, at_list;      // tokens in this CTA's list, in CTA 0's, and where this CTA's begin there
+    unsigned n_window;
     int bin, bin_end, done;
     float pick;
     uint4 ends[2];                        // the slice's first and last vector, -infinity in places outside it
@@ -133,12 +141,8 @@ __device__ __forceinline__ unsigned long long cta_upto(Shared& sh, unsigned long
     __syncthreads();
     if (lane == 31) sh.warp_sum[warp] = upto;
     __syncthreads();
-    unsigned long long before = upto - v[kPer - 1], all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        const unsigned long long x = sh.warp_sum[w];
-        before += w < warp ? x : 0ull, all += x;
-    }
+    const unsigned long long x = lane < kWarps ? sh.warp_sum[lane] : 0ull, all = warp_total(x);
+    const unsigned long long before = upto - v[kPer - 1] + warp_total(lane < warp ? x : 0ull);
 #pragma unroll
     for (int i = 0; i < kPer; i++) v[i] += before;
     return all;
@@ -161,6 +165,7 @@ struct Sampler {
     __device__ u64* list() const { return reinterpret_cast<u64*>(aux); }
     __device__ u64* sorted() const { return reinterpret_cast<u64*>(aux + kSortedOff); }
     __device__ u64* mine() const { return reinterpret_cast<u64*>(aux + kMineOff); }
+    __device__ u64* window() const { return reinterpret_cast<u64*>(aux + window_off(ctas)); }
     __device__ uint32_t* counts() const { return reinterpret_cast<uint32_t*>(aux + counts_off(ctas)); }
     __device__ unsigned mine_room() const { return ctas > 1 ? kMine : kCand; }
     __device__ int segment() const { return (nv + kWarps - 1) / kWarps; }  // vectors of a warp's segment
@@ -206,6 +211,36 @@ struct Sampler {
                 }
         }
     }
+    // The same, kRing vectors on their way to shared memory (aux, which holds nothing else then): the passes over the weights have no
+    // registers for them (320 nuclei: 288 us with one ahead in registers).
+    template <typename F>
+    __device__ __forceinline__ void sweep_ring(int v0, int step, int v1, F f) const {
+        uint4* ring = reinterpret_cast<uint4*>(aux) + threadIdx.x;
+        auto fetch = [&](int v, int slot) {
+            if (v < v1) {
+                if (v == 0 || v == nv - 1) ring[slot * kThreads] = sh.ends[v != 0];
+                else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + slot * kThreads)), "l"(data + v) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int k = 0; k < kRing; k++) fetch(v0 + k * step, k);
+        int slot = 0;
+#pragma unroll 1
+        for (int v = v0; v < v1; v += step) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            const uint4 now = ring[slot * kThreads];
+            fetch(v + kRing * step, slot);
+            slot = (slot + 1) & (kRing - 1);
+#pragma unroll
+            for (int j0 = 0; j0 < kPer; j0 += 4) {
+                float x[4];
+                four(now, j0, x);
+                f(x, first + v * kPer + j0);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
     // Of all vectors, spread over the threads; of the warp's segment.
     template <int kAhead, typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -214,7 +249,7 @@ struct Sampler {
     template <typename F>
     __device__ __forceinline__ void each_of_segment(F f) const {
         const int v0 = int(threadIdx.x >> 5) * segment();
-        sweep<1>(v0 + int(threadIdx.x & 31), 32, min(v0 + segment(), nv), f);
+        sweep_ring(v0 + int(threadIdx.x & 31), 32, min(v0 + segment(), nv), f);
     }
     // What four tokens count of which take(value, index) holds: their weights, or 1 each.
     template <bool MASS, typename F>
@@ -308,6 +343,21 @@ struct Sampler {
     // by 512 bins of their keys, and the entries of one bin against each other. 0: none.
     __device__ u64 cut_in_list(int n, double want, u64 ahead, bool mass) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (n <= 32) {  // one warp's
+            if (threadIdx.x == 0) sh.cut = 0;
+            __syncthreads();
+            if (warp == 0) {
+                const u64 x = lane < n ? list()[lane] : 0ull, w = lane >= n ? 0ull : mass ? weight_of(value(x)) : 1ull;
+                u64 sum = ahead;
+                for (int j = 0; j < n; j++) {
+                    const u64 y = __shfl_sync(0xffffffffu, x, j), v = __shfl_sync(0xffffffffu, w, j);
+                    sum += y > x ? v : 0ull;
+                }
+                if (lane < n && double(sum) < want && double(sum + w) >= want) sh.cut = x;
+            }
+            __syncthreads();
+            return sh.cut;
+        }
         uint32_t* red = reinterpret_cast<uint32_t*>(sh.warp_sum);
         uint32_t most = 0, least = 0xFFFFFFFFu;
         for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -382,41 +432,49 @@ struct Sampler {
         __syncthreads();
         u64 of_cta = 0, before = 0, total = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const u64 x = sh.seg[w];
-            of_cta += x, before += w < warp ? x : 0ull;
-        }
+        for (int w = 0; w < kWarps; w++) of_cta += sh.seg[w];
         share_sum(of_cta);
         for (int i = 0; i < ctas; i++) {
             const u64 x = sh.sum[i];
             before += i < rank ? x : 0ull, total += x;
         }
         const u64 at = where(total);
-        if (total && at >= before && at - before < sh.seg[warp]) {  // one warp of the cluster
-            const int v0 = warp * segment(), v1 = min(v0 + segment(), nv);
-            for (int base = v0; base < v1; base += 32) {
-                const int v = base + lane;
-                u64 s = 0;
-                const uint4 w = load(v, v1);
-                float x[4];
+        if (total && at >= before && at - before < of_cta) {  // one CTA of the cluster
+            // its segment that has it, in as many parts as warps
+            int w = 0;
+            while (at - before >= sh.seg[w]) before += sh.seg[w++];
+            const int s0 = w * segment(), s1 = min(s0 + segment(), nv), size = (s1 - s0 + kWarps - 1) / kWarps;
+            const int v0 = min(s0 + warp * size, s1), v1 = min(v0 + size, s1);
+            u64 part = 0;
+            sweep<1>(v0 + lane, 32, v1, [&](const float (&x)[4], int i) { part += measured<MASS>(x, i, take); });
+            part = warp_total(part);
+            if (lane == 0) sh.warp_sum[warp] = part;
+            __syncthreads();
+            for (int i = 0; i < warp; i++) before += sh.warp_sum[i];
+            if (at >= before && at - before < part)  // one warp
+                for (int base = v0; base < v1; base += 32) {
+                    const int v = base + lane;
+                    u64 s = 0;
+                    const uint4 w = load(v, v1);
+                    float x[4];
 #pragma unroll
-                for (int j0 = 0; j0 < kPer; j0 += 4) four(w, j0, x), s += measured<MASS>(x, first + v * kPer + j0, take);
-                const u64 upto = before + warp_upto(s, lane);
-                if (upto > at && upto - s <= at) {  // one lane
-                    u64 sum = upto - s;
-                    bool there = false;
+                    for (int j0 = 0; j0 < kPer; j0 += 4) four(w, j0, x), s += measured<MASS>(x, first + v * kPer + j0, take);
+                    const u64 upto = before + warp_upto(s, lane);
+                    if (upto > at && upto - s <= at) {  // one lane
+                        u64 sum = upto - s;
+                        bool there = false;
 #pragma unroll 1
-                    for (int j = 0; j < kPer; j++) {
-                        const int i = first + v * kPer + j;
-                        four(w, j & ~3, x);
-                        const float y = x[j & 3];
-                        sum += !take(y, i) ? 0ull : MASS ? weight_of(y) : 1ull;
-                        if (sum > at && !there) sh.found = unsigned(i), sh.pick = y, there = true;
+                        for (int j = 0; j < kPer; j++) {
+                            const int i = first + v * kPer + j;
+                            four(w, j & ~3, x);
+                            const float y = (j & 3) == 0 ? x[0] : (j & 3) == 1 ? x[1] : (j & 3) == 2 ? x[2] : x[3];
+                            sum += !take(y, i) ? 0ull : MASS ? weight_of(y) : 1ull;
+                            if (sum > at && !there) sh.found = unsigned(i), sh.pick = y, there = true;
+                        }
                     }
+                    before = __shfl_sync(0xffffffffu, upto, 31);
+                    if (before > at) break;
                 }
-                before = __shfl_sync(0xffffffffu, upto, 31);
-                if (before > at) break;
-            }
         }
         __syncthreads();
         return total;
@@ -424,6 +482,7 @@ struct Sampler {
     template <bool MASS, typename M>
     __device__ void fill(M take) {
         u64 part = 0;
+        __syncthreads();
         each_of_segment([&](const float (&x)[4], int i) { part += measured<MASS>(x, i, take); });
         part = warp_total(part);
         if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
@@ -557,182 +616,262 @@ struct Sampler {
         take_cut();
     }
 
-    // The steps that few() counts in, and what a step's tokens weigh by its middle.
-    __device__ __forceinline__ float count_scale() const { return fminf(128.0f * fmaxf(row.c32, 1.0f), 1e30f); }
-    __device__ __forceinline__ int count_step(float x, float scale) const {  // NaN: the last
-        return __float_as_int(fminf((row.m - x) * scale, float(kSteps - 1)) + 8388608.0f) & (kSteps - 1);  // to nearest
-    }
-    __device__ __forceinline__ float middle(int step, float scale) const {
-        return step == kSteps - 1 ? 0.0f : exp2f(44.0f - (step ? float(step) : 0.25f) / scale * row.c32);
-    }
-
-    // The cut by the largest values alone; true: the row is answered. Without top_k the weights are added up and the tokens
-    // counted in steps, for what comes next.
+    // Top-k by the largest values alone; true: the row is answered.
     __device__ bool few(int r, float t, int top_k, bool use_p, float top_p) {
-        const float scale = count_scale();
-        if (!top_k)
-            for (int i = threadIdx.x; i < kSteps; i += kThreads) counts()[i] = 0;
         if (threadIdx.x == 0) sh.done = 0, sh.n_list = 0;
         __syncthreads();
-        auto reaches = [&](const float (&x)[4], int i) {
+        each<4>([&](const float (&x)[4], int i) {
             if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= t)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (x[j] >= t && real(x[j])) put(x[j], i + j);
-        };
-        if (top_k) {
-            each<4>(reaches);
-            gather([]() {});
-        } else {
-            u64 part = 0;
-            each<1>([&](const float (&x)[4], int i) {
-                u64 y[4];
-                four_weights(row, sh.table, x, y);
-                part += (y[0] + y[1]) + (y[2] + y[3]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int step = count_step(x[j], scale);
-                    if (step < kSteps - 1) atomicAdd(&counts()[step], 1u);  // the last step's tokens are not counted
-                }
-                reaches(x, i);
-            });
-            gather([&]() {
-                part = warp_total(part);
-                if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.total, 0), part);
-            });
-        }
+        });
+        gather([]() {});
         if (rank == 0) {
-            bool sure = false;
-            long long more = 0;
             const unsigned n_all = sh.n_all;
             __syncthreads();  // read by all before it is set again below
             if (n_all <= kCand) {
-                const int n = int(n_all), n_k = top_k ? min(top_k, n) : n;
+                const int n = int(n_all), n_k = min(top_k, n);
                 rank_list(n, [&](u64 e) { return weight_of(value(e)); });
                 const u64* upto = list();
-                int n_p = n_k;
-                sure = top_k != 0;
-                if (use_p) {
-                    const u64 total = top_k ? upto[n_k - 1] : sh.total;
-                    const int less = below(n_k, fmax(double(top_p) * double(total), 0.5), 0);
-                    if (less < n_k) n_p = less + 1, sure = true;
-                }
-                int n_m = n_p;
+                int left = n_k;
+                if (use_p) left = min(below(n_k, fmax(double(top_p) * double(upto[n_k - 1]), 0.5), 0) + 1, n_k);
                 if (row.least > -INFINITY) {
-                    n_m = 0;
-                    for (int base = 0; base < n_p; base += kThreads) {
+                    int n_m = 0;
+                    for (int base = 0; base < left; base += kThreads) {
                         const int i = base + threadIdx.x;
-                        n_m += __syncthreads_count(i < n_p && value(sorted()[i < n_p ? i : 0]) >= row.least);
+                        n_m += __syncthreads_count(i < left && value(sorted()[i < left ? i : 0]) >= row.least);
                     }
-                    sure |= n_m < n_p;
+                    left = n_m;
                 }
-                if (sure) {
-                    const u64 total = upto[n_m - 1], at = place(r, total);
-                    for (int i = threadIdx.x; i < n_m; i += kThreads) {
-                        const uint32_t low = uint32_t(sorted()[i]);  // ~index
-                        u64 before = 0, last = 0;
-                        for (int j = 0; j < n_m; j++) {
-                            const u64 u = upto[j];
-                            before += uint32_t(sorted()[j]) > low ? u - last : 0ull;
-                            last = u;
-                        }
-                        if (at >= before && at - before < upto[i] - (i ? upto[i - 1] : 0ull))
-                            answer(r, int(0xFFFFFFFFu - low), value(sorted()[i]), total);
+                const u64 total = upto[left - 1], at = place(r, total);
+                for (int i = threadIdx.x; i < left; i += kThreads) {
+                    const uint32_t low = uint32_t(sorted()[i]);  // ~index
+                    u64 before = 0, last = 0;
+                    for (int j = 0; j < left; j++) {
+                        const u64 u = upto[j];
+                        before += uint32_t(sorted()[j]) > low ? u - last : 0ull;
+                        last = u;
                     }
-                } else {
-                    u64 by_step = 0;
-                    for (int i = threadIdx.x; i < n; i += kThreads) by_step += static_cast<u64>(middle(count_step(value(sorted()[i]), scale), scale));
-                    u64 v[1] = {by_step};
-                    more = static_cast<long long>(upto[n - 1]) - static_cast<long long>(cta_upto(sh, v));
+                    if (at >= before && at - before < upto[i] - (i ? upto[i - 1] : 0ull))
+                        answer(r, int(0xFFFFFFFFu - low), value(sorted()[i]), total);
                 }
             }
-            if (threadIdx.x < ctas) {
-                Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
-                o->done = sure, o->more = more;
-                if (rank != int(threadIdx.x)) o->total = sh.total;
-            }
-            if (threadIdx.x == 0) sh.n_all = 0, sh.before = 0;
+            if (threadIdx.x < ctas) cluster.map_shared_rank(&sh, threadIdx.x)->done = n_all <= kCand;
+            if (threadIdx.x == 0) sh.n_all = 0;
         }
         cluster.sync();
         return sh.done != 0;
     }
 
-    // Top-p by the counts of few(): true: the cut is set, and seg[] holds what is kept.
-    __device__ bool near_cut(float top_p) {
-        const float scale = count_scale();
-        // this CTA's share of the steps: what their tokens weigh, by the middles
-        constexpr int kMost = kSteps / kThreads;
-        const int share = kSteps / ctas, per = share / kThreads;
-        u64 v[kMost] = {}, own[kMost];
-        {
-            uint32_t n[kMost] = {};
-            if (per == 1) {
-#pragma unroll
-                for (int c = 0; c < kMaxCluster; c++) n[0] += cluster.map_shared_rank(counts(), c)[rank * share + threadIdx.x];  // side by side
-            } else {
-                for (int c = 0; c < ctas; c++) {
-                    const uint32_t* o = cluster.map_shared_rank(counts(), c) + rank * share + threadIdx.x * per;
-#pragma unroll
-                    for (int k = 0; k < kMost; k++)
-                        if (k < per) n[k] += o[k];
+    // Steps of max - x: to nearest, NaN and what is far: the last; and what a step's tokens weigh by its middle.
+    __device__ __forceinline__ int count_step(float x, float scale) const {
+        return __float_as_int(fminf((row.m - x) * scale, float(kSteps - 1)) + 8388608.0f) & (kSteps - 1);
+    }
+    __device__ __forceinline__ float middle(int step, float scale) const {
+        return step == kSteps - 1 ? 0.0f : exp2f(44.0f - (step ? float(step) : 0.25f) / scale * row.c32);
+    }
+
+    // Top-p alone; t: a value that some dozens of tokens reach. True: the cut is set, and seg[] holds what is kept.
+    __device__ bool nucleus(float t, float top_p) {
+        const float scale = fminf(128.0f * fmaxf(row.c32, 1.0f), 1e30f);
+        // ---- a sample by steps: one in `rate` of each warp's turns, not the same ones for neighbours
+        int rate = 1;
+        while (rate < 8 && a.vocab > 16384 * rate) rate *= 2;
+        for (int i = threadIdx.x; i < kSteps; i += kThreads) counts()[i] = 0;
+        if (threadIdx.x == 0) sh.n_list = sh.n_window = 0;
+        __syncthreads();
+        u64 top = 0;
+        int turn = threadIdx.x >> 5;
+        each<4>([&](const float (&x)[4], int) {
+            if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= t)
+#pragma unroll 1
+                for (int j = 0; j < 4; j++) {
+                    const float y = j == 0 ? x[0] : j == 1 ? x[1] : j == 2 ? x[2] : x[3];
+                    if (y >= t) top += weight_of(y);
                 }
-            }
+            if ((turn++ & (rate - 1)) == 0)
 #pragma unroll
-            for (int k = 0; k < kMost; k++)
-                if (k < per) v[k] = static_cast<u64>(n[k]) * static_cast<u64>(middle(rank * share + threadIdx.x * per + k, scale));
+                for (int j = 0; j < 4; j++)
+                    if (!(x[j] >= t)) {
+                        const int step = count_step(x[j], scale);
+                        if (step < kSteps - 1) atomicAdd(&counts()[step], 1u);
+                    }
+        });
+        top = warp_total(top);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = top;
+        __syncthreads();
+        if (threadIdx.x < ctas) {
+            u64 s = 0;
+            for (int w = 0; w < kWarps; w++) s += sh.warp_sum[w];
+            cluster.map_shared_rank(&sh, threadIdx.x)->others[rank][0] = s;
         }
+        cluster.sync();
+        // ---- this CTA's share of the steps: what all their tokens weigh, by the middles, and the squares (in units of 2^-44) that the
+        // sample's error goes by
+        const int share = kSteps / ctas, per = share / kThreads, step0 = rank * share + int(threadIdx.x) * per;
+        uint32_t* merged = reinterpret_cast<uint32_t*>(aux) + threadIdx.x * per;
+        if (per == 1) {
+            uint32_t n = 0;
 #pragma unroll
-        for (int k = 0; k < kMost; k++) own[k] = v[k];
-        const u64 all = cta_upto(sh, v);
-        const double sum = double(sh.total), want = fmax(double(top_p) * sum, 0.5);
-        if (threadIdx.x == 0) sh.bin = sh.bin_end = kSteps - 1, sh.n_list = 0;
+            for (int c = 0; c < kMaxCluster; c++) n += cluster.map_shared_rank(counts(), c)[step0];  // side by side
+            merged[0] = n;
+        } else {
+#pragma unroll 4
+            for (int k = 0; k < per; k++) {
+                uint32_t n = 0;
+                for (int c = 0; c < ctas; c++) n += cluster.map_shared_rank(counts(), c)[step0 + k];
+                merged[k] = n;
+            }
+        }
+        auto weighed = [&](int k, u64& w, u64& q) {
+            const uint32_t n = merged[k];
+            const float one = middle(step0 + k, scale) * float(rate);
+            w = static_cast<u64>(n) * static_cast<u64>(one), q = static_cast<u64>(float(n) * one * (one * float(1.0 / kOne)));
+        };
+        u64 v[1] = {0}, q[1] = {0};
+#pragma unroll 1
+        for (int k = 0; k < per; k++) {
+            u64 w, z;
+            weighed(k, w, z);
+            v[0] += w, q[0] += z;
+        }
+        u64 upto = 0 - v[0], upto_q = 0 - q[0];
+        const u64 all = cta_upto(sh, v), all_q = cta_upto(sh, q);
+        upto += v[0], upto_q += q[0];  // before this thread's steps
+        if (threadIdx.x == 0) sh.bin = -1, sh.bin_end = kSteps - 1;
+        if (threadIdx.x < ctas) cluster.map_shared_rank(&sh, threadIdx.x)->others[rank][1] = all_q;
         share_sum(all);
-        double before = double(sh.more);
-        for (int i = 0; i < rank; i++) before += double(sh.sum[i]);
-        // the first steps at which the sum may and must have reached it
-        const double margin = sum * 0x1p-13;
-#pragma unroll
-        for (int k = 0; k < kMost; k++) {
-            const double upto = before + double(v[k]), less = upto - double(own[k]);
-            const int step = rank * share + int(threadIdx.x) * per + k;
-            if (k >= per || !own[k]) continue;
-            const bool may = upto >= want - margin && less < want - margin, must = upto >= want + margin && less < want + margin;
+        u64 largest = 0, before = 0, sum = 0, before_q = 0, sum_q = 0;
+        for (int i = 0; i < ctas; i++) {
+            const u64 x = sh.sum[i], y = sh.others[i][1];
+            largest += sh.others[i][0];
+            before += i < rank ? x : 0ull, before_q += i < rank ? y : 0ull, sum += x, sum_q += y;
+        }
+        upto += before + largest, upto_q += before_q, sum += largest;
+        // The first steps at which the sum may and must have reached its part. What the sample makes of a beginning less p times all
+        // is off by (1 - p) of what is in it and p of what is not: three standard deviations, and a little for the middles.
+        const long long want_near = static_cast<long long>(double(top_p) * double(sum));
+        const float in = (1 - top_p) * (1 - top_p) * float(kOne), out = top_p * top_p * float(kOne), least = float(sum) * 0x1p-11f;
+        auto margin = [&](u64 upto_q) {
+            return rate > 1 ? static_cast<long long>(3.0f * sqrtf(in * float(upto_q) + out * float(sum_q - upto_q)) + least) : static_cast<long long>(least);
+        };
+        long long e_less = margin(upto_q);
+#pragma unroll 1
+        for (int k = 0; k < per; k++) {
+            u64 w, z;
+            weighed(k, w, z);
+            if (!w) continue;
+            const long long less = static_cast<long long>(upto) - want_near;
+            upto += w, upto_q += z;
+            const long long more = static_cast<long long>(upto) - want_near, e = margin(upto_q);
+            const bool may = more + e >= 0 && less + e_less < 0, must = more - e >= 0 && less - e_less < 0;
+            e_less = e;
             if (may || must)
                 for (int c = 0; c < ctas; c++) {
                     Shared* o = cluster.map_shared_rank(&sh, c);
-                    if (may) o->bin = step;
-                    if (must) o->bin_end = step;
+                    if (may) o->bin = step0 + k;
+                    if (must) o->bin_end = step0 + k;
                 }
         }
         cluster.sync();
-        const int lo = sh.bin, hi = sh.bin_end;
-        u64 part = 0;
+        // none: the cut may be, or is, among the largest, which are not counted
+        const int lo = max(sh.bin - 1, 0), hi = static_cast<long long>(largest) - want_near - margin(0) >= 0 ? min(count_step(t, scale) + 1, kSteps - 1) : sh.bin_end;
+        // ---- one pass over the weights: the row's sum, the sum before the window, the window's tokens by finer steps
+        u64* fine = reinterpret_cast<u64*>(counts());
+        // the window: values from `bottom` to `top_value`; larger ones lie before it
+        const float top_value = lo > 0 ? row.m - (float(lo) - 0.5f) / scale : INFINITY;
+        const float bottom = hi < kSteps - 1 ? fmaxf(row.m - (float(hi) + 0.5f) / scale, -FLT_MAX) : -FLT_MAX;
+        const float fine_scale = scale * (float(kFine) / float(hi - lo + 1)), fine_top = fminf(top_value, row.m);
+        auto fine_step = [&](float x) { return int(fminf((fine_top - x) * fine_scale, float(kFine - 1))); };
+        u64 part = 0, whole = 0;
+        const unsigned room = window_room(ctas);
         each_of_segment([&](const float (&x)[4], int i) {
-            int step[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) step[j] = count_step(x[j], scale);
-            if (min(min(step[0], step[1]), min(step[2], step[3])) > hi) return;
             u64 y[4];
             four_weights(row, sh.table, x, y);
+            whole += (y[0] + y[1]) + (y[2] + y[3]);
+            bool in[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) part += step[j] < lo ? y[j] : 0ull;
+            for (int j = 0; j < 4; j++) {
+                if (x[j] > top_value) part += y[j];
+                in[j] = x[j] >= bottom && x[j] <= top_value;
+            }
+            const int n = in[0] + in[1] + in[2] + in[3];
+            if (n) {
+                unsigned at = atomicAdd(&sh.n_window, unsigned(n));
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (step[j] >= lo && step[j] <= hi && real(x[j])) put(x[j], i + j);
+                for (int j = 0; j < 4; j++) {
+                    if (in[j] && at < room) window()[at] = entry(x[j], i + j);
+                    at += in[j];
+                }
+            }
         });
-        part = warp_total(part);
-        if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part;
-        gather([&]() {
-            if ((threadIdx.x & 31) == 0) atomicAdd(cluster.map_shared_rank(&sh.before, 0), part);
-        });
-        const unsigned n = sh.n_list;
+        part = warp_total(part), whole = warp_total(whole);
         __syncthreads();
+        for (int i = threadIdx.x; i < kFine; i += kThreads) fine[i] = 0;
+        __syncthreads();
+        const int n = int(min(sh.n_window, room));
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const float x = value(window()[i]);
+            atomicAdd(&fine[fine_step(x)], weight_of(x));
+        }
+        if ((threadIdx.x & 31) == 0) sh.seg[threadIdx.x >> 5] = part, sh.warp_sum[threadIdx.x >> 5] = whole;
+        __syncthreads();
+        if (threadIdx.x < ctas) {
+            u64 p = 0, s = 0;
+            for (int w = 0; w < kWarps; w++) p += sh.seg[w], s += sh.warp_sum[w];
+            Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
+            o->others[rank][0] = p, o->others[rank][1] = s + (sh.n_window > room ? 1ull << 63 : 0ull);  // no room: says so
+        }
+        cluster.sync();
+        u64 ahead = 0, total = 0;
+        bool fits = true;
+        for (int i = 0; i < ctas; i++) {
+            ahead += sh.others[i][0], total += sh.others[i][1] & ~(1ull << 63);
+            fits &= !(sh.others[i][1] >> 63);
+        }
+        const double want = fmax(double(top_p) * double(total), 0.5);
+        if (!fits || double(ahead) >= want) return false;
+        // ---- the fine step of the cut, its tokens, the cut
+        constexpr int kMostFine = kFine / kThreads;
+        const int share_fine = kFine / ctas, per_fine = (share_fine + kThreads - 1) / kThreads;
+        u64 f[kMostFine] = {}, own_fine[kMostFine];
+        for (int c = 0; c < ctas; c++) {
+            const u64* o = cluster.map_shared_rank(fine, c) + rank * share_fine;
+#pragma unroll
+            for (int k = 0; k < kMostFine; k++)
+                if (k < per_fine && int(threadIdx.x) * per_fine + k < share_fine) f[k] += o[threadIdx.x * per_fine + k];
+        }
+#pragma unroll
+        for (int k = 0; k < kMostFine; k++) own_fine[k] = f[k];
+        const u64 of_cta = cta_upto(sh, f);
+        if (threadIdx.x == 0) sh.bin = -1;
+        share_sum(of_cta);
+        for (int i = 0; i < rank; i++) ahead += sh.sum[i];
+#pragma unroll
+        for (int k = 0; k < kMostFine; k++) {
+            const u64 upto = ahead + f[k], less = upto - own_fine[k];
+            if (own_fine[k] && double(upto) >= want && double(less) < want)
+                for (int c = 0; c < ctas; c++) {
+                    Shared* o = cluster.map_shared_rank(&sh, c);
+                    o->bin = rank * share_fine + int(threadIdx.x) * per_fine + k, o->before = less;
+                }
+        }
+        cluster.sync();
+        const int step = sh.bin;
+        if (step < 0) return false;  // behind the window
+        const u64 less = sh.before;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 e = window()[i];
+            const float x = value(e);
+            if (fine_step(x) == step) put(x, int(0xFFFFFFFFu - uint32_t(e)));
+        }
+        gather([]() {});
         if (rank == 0) {
             u64 next = 0;
-            const u64 ahead = sh.before;
             const unsigned n_all = sh.n_all;
-            __syncthreads();  // ahead is read by all before it is set again
-            if (n_all <= kCand && double(ahead) < want) next = cut_in_list(int(n_all), want, ahead, true);
+            if (n_all <= kCand) next = cut_in_list(int(n_all), want, less, true);
             if (threadIdx.x < ctas) {
                 Shared* o = cluster.map_shared_rank(&sh, threadIdx.x);
                 o->done = next != 0;
@@ -741,9 +880,10 @@ struct Sampler {
         }
         cluster.sync();
         if (!sh.done) return false;
-        for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-            const u64 e = mine()[i];
-            if (e >= sh.cut) atomicAdd(&sh.seg[(int(0xFFFFFFFFu - uint32_t(e)) - first) / kPer / segment()], weight_of(value(e)));
+        const int seg = segment();
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 e = window()[i];
+            if (e >= sh.cut) atomicAdd(&sh.seg[(int(0xFFFFFFFFu - uint32_t(e)) - first) / kPer / seg], weight_of(value(e)));
         }
         __syncthreads();
         take_cut();
@@ -842,10 +982,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     const bool use_p = top_p < 1.0f;
     bool ready = false;  // seg[] holds what is kept
     if (top_k || use_p) {
-        // for top-p alone a sixth of the groups: 94 tokens of 8 CTAs hold most nuclei
-        const int want = top_k ? top_k : max(groups / 6, 1);
-        const bool bounded = 4 * want <= 3 * groups;
-        if (bounded || !top_k) {
+        const int want = top_k ? top_k : min(3 * groups / 4, 96);
+        if (4 * want <= 3 * groups) {
             // the bound: a key that `want` groups reach, by halving below the bits that the largest has in common with the smallest group
             const uint32_t key = tid < groups ? order_key(g) : 0xFFFFFFFFu, top = order_key(m);
             uint32_t least = __reduce_min_sync(0xffffffffu, key);
@@ -860,9 +998,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
                 const uint32_t next = bound | 1u << bit;
                 if (__syncthreads_count(tid < groups && key >= next) >= want) bound = next;
             }
-            if (s.few(r, bound >= 0x00800000u ? key_value(bound) : -INFINITY, top_k, use_p, top_p)) return;  // below: no finite value
+            const float t = bound >= 0x00800000u ? key_value(bound) : -INFINITY;  // below: no finite value
+            if (top_k) {
+                if (s.few(r, t, top_k, use_p, top_p)) return;
+            } else {
+                ready = s.nucleus(t, top_p);
+            }
         }
-        if (use_p && !top_k) ready = s.near_cut(top_p);
         if (!ready) {
 #pragma unroll 1
             for (int mass = top_k ? 0 : 1; mass < (use_p ? 2 : 1); mass++) s.select(mass, top_k, top_p);
@@ -879,9 +1021,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
 template <typename T>
 cudaError_t go(const neko_sample_rows_args& a, cudaStream_t st) {
     constexpr int kPer = 16 / sizeof(T);
+    // As many CTAs a row as run at once (two an SM), slices of 4,096 tokens at least: 24 rows of 151,936, k = 40: 8 CTAs 15.1 us, 4 14.5,
+    // nuclei 47 and 48; 64 rows 8 CTAs 28.2, 4 18.1, 2 19.3, nuclei 99, 68, 75. More rows than that: one each (320 x 50,257: 31.5 us,
+    // two 40.8), but two where one would leave a wave of large slices nearly empty (320 x 151,936: 83 us, one 107).
+    const int64_t room = 2 * num_sms();
     int ctas = 1;
-    while (ctas < kMaxCluster && a.vocab > 4096 * ctas) ctas *= 2;
-    if (getenv("NEKO_C")) ctas = std::min(ctas, atoi(getenv("NEKO_C")));
+    while (ctas < kMaxCluster && a.vocab > 4096 * ctas && a.rows * ctas * 2 <= room) ctas *= 2;
+    if (a.rows > room && a.vocab > 100000) {
+        auto waste = [&](int64_t n) { return double((a.rows * n + room - 1) / room) / double(a.rows * n); };
+        if (waste(1) > 1.25 * waste(2)) ctas = 2;
+    }
     const int slice = ((a.vocab + ctas - 1) / ctas + kPer - 1) / kPer * kPer;
     const size_t smem = (sizeof(Shared) + 127) / 128 * 128 + aux_bytes(ctas);
     auto* fn = sample_rows_kernel<T>;

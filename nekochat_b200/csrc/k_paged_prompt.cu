@@ -52,6 +52,8 @@ constexpr int kCopyTiles = 2;
 constexpr int64_t kCopyBytes = int64_t(1) << 31;
 constexpr int kRing = 4;        // key tiles whose scales are kept (at most 5 stages are in flight)
 constexpr int kOddRing = 8;     // and their keys with odd values
+constexpr int kSorted = 128;    // so many sequences at most are taken in the order of their lengths (trees)
+static_assert(kSorted < 4 * kRows, "the lengths stand in Misc::most");
 // Weights are 2^(score (+ log2 of the value scale) - reference + kLift), at most 2^15. What f16 rounds off them, half of 2^-24 with
 // hi + lo, is 2^-32 of the largest: little lag of the reference keeps small weights, much saves trips of O through registers (f32
 // ragged prompts at a lag of 2^8 678 us, 2^7 693, 2^6 718, 2^4 806).
@@ -257,7 +259,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     b /= plan.ranks;
     const int kvh = b % c.n_kv;
     b /= c.n_kv;
-    const int s = b % c.n_seq;
+    int s = b % c.n_seq;
+    if constexpr (TREE) {
+        // The longest contexts first: a long one that starts last leaves the other SMs idle (16 trees of 63 bf16 nodes on 8,192
+        // keys: 273 us in the sequences' order, 222 this way). Each CTA ranks the lengths itself, once for all sequences.
+        if (c.n_seq > 1 && c.n_seq <= kSorted) {
+            int* lens = reinterpret_cast<int*>(ms.most);
+            if (tid < c.n_seq) lens[tid] = a.kv_len[tid];
+            __syncthreads();
+            if (tid < c.n_seq) {
+                const int mine = lens[tid];
+                int longer = 0;
+                for (int i = 0; i < c.n_seq; i++) longer += lens[i] > mine || (lens[i] == mine && i < tid);
+                if (longer == s) lens[kSorted] = tid;
+            }
+            __syncthreads();
+            s = lens[kSorted];
+            __syncthreads();
+        }
+    }
     const int tile = plan.row_tiles - 1 - b / c.n_seq;  // the longest rows first
     const int G = plan.group;
     auto over_g = [&](int x) { return int(uint64_t(uint32_t(x)) * plan.group_inv >> 32); };
@@ -775,7 +795,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             // back into TMEM
             const float *kb = ksp + 4 * col_w, *vb = vsp + 4 * col_w;  // of this thread's blocks of 16 keys
             const uint32_t tc = ts + 64 * col_w;
-            const bool shaped = a.softcap > 0.0f || a.slopes || !plain_mask || a.scale < 0.0f;
+            // A cap alone needs no second trip through TMEM: the scores in registers take it (trees only).
+            const bool capped = TREE && a.softcap > 0.0f && !a.slopes && plain_mask && a.scale >= 0.0f;
+            const bool shaped = !capped && (a.softcap > 0.0f || a.slopes || !plain_mask || a.scale < 0.0f);
             if (shaped) {
 #pragma unroll 1
                 for (int q = 0; q < 2; q++) {
@@ -852,6 +874,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
 #pragma unroll
             for (int b = 0; b < 4; b++) fb[b] = shaped ? 1.0f : kScaled ? factor * kb[b] : factor;
             ld_wait(u[0]), ld_wait(u[1]);
+            if constexpr (TREE) {
+                if (capped) {
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        float most = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            u[q][x] = __float_as_uint(__uint_as_float(u[q][x]) * fb[2 * q + x / 16]);
+                            most = max_nan(most, fabsf(__uint_as_float(u[q][x])));
+                        }
+                        if (__all_sync(0xffffffffu, most <= 0.5f)) {
+#pragma unroll
+                            for (int x = 0; x < 32; x += 2) {  // tanh_small of two
+                                const uint64_t y = pack2(__uint_as_float(u[q][x]), __uint_as_float(u[q][x + 1])), y2 = mul2(y, y);
+                                uint64_t p = fma2(y2, pack2(0.016737453639507294f, 0.016737453639507294f), pack2(-0.05276207625865936f, -0.05276207625865936f));
+                                p = fma2(p, y2, pack2(0.13320569694042206f, 0.13320569694042206f));
+                                p = fma2(p, y2, pack2(-0.3333277702331543f, -0.3333277702331543f));
+                                p = fma2(p, y2, pack2(0.9999999403953552f, 0.9999999403953552f));
+                                float p0, p1;
+                                unpack2(mul2(p, y), p0, p1);
+                                u[q][x] = __float_as_uint(p0), u[q][x + 1] = __float_as_uint(p1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 32; x++) {
+                                const float y = __uint_as_float(u[q][x]);
+                                u[q][x] = __float_as_uint(fabsf(y) <= 0.5f ? tanh_small(y) : tanh_abs(y));
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < 4; b++) fb[b] = cap;
+                }
+            }
             float top = -INFINITY, top_score = -INFINITY;
 #pragma unroll
             for (int b = 0; b < 4; b++) {
@@ -1158,14 +1214,24 @@ int clusters_at_once(int log) {
 // better where that fills SMs (512 bf16 tokens on 2,048 keys: 30.4 us, two in clusters of 4 33.7). Without clusters 64 f32 tokens
 // on 8,192 keys take 207 us, with clusters of 8 39; 16 clusters of 8 do not run at once and 90 us become 62 with 8 of them.
 template <int HD>
-int64_t split(PromptPlan& p, int64_t tiles, int64_t heads, int64_t key_tiles, bool f32) {
+int64_t split(PromptPlan& p, int64_t tiles, int64_t heads, int64_t key_tiles, bool f32, bool ragged) {
     const int64_t step[2] = {f32 ? 34 : 23, f32 ? 41 : 26}, start = 80, join[2] = {50, 150};
     int64_t best = INT64_MAX, items = 0;
     for (int two = 0; two < (tiles > 1 ? 2 : 1); two++) {
         const int64_t row_tiles = (tiles + two) / (1 + two), n = heads * row_tiles;
         for (int log = 0; log < 4 && (log == 0 || key_tiles >= (1 << log)); log++) {
             const int64_t at_once = clusters_at_once<HD>(log), rounds = (n + at_once - 1) / at_once;
-            const int64_t time = rounds * (start + ((key_tiles + (1 << log) - 1) >> log) * step[two] + (log ? join[two] : 0));
+            const int64_t most = start + ((key_tiles + (1 << log) - 1) >> log) * step[two] + (log ? join[two] : 0);
+            int64_t time = rounds * most;
+            if (ragged && rounds > 1) {
+                // Several trees stand behind contexts of any length up to the table's, and the longest start first. Lengths that
+                // are all the table's count a third; lengths of half of it on average, the whole work of which stands over the
+                // CTAs that run at once with a part of the longest for the end, two thirds. bf16, 16 trees of 63 on 900 to 8,191
+                // keys: 261 -> 226 us (capped 346 -> 267, f32 369 -> 290), all on 8,191 271 -> 338; of 17 tokens 173 -> 136 and
+                // 178 -> 216; 64 trees of 63 671 -> 608 and 1005 -> 1019.
+                const int64_t work = n * ((start + (log ? join[two] : 0)) * (1 << log) + key_tiles * step[two] / 2);
+                time = (time + 2 * std::max(most, work / (at_once << log) + most / 4)) / 3;
+            }
             if (time >= best) continue;
             best = time, items = n;
             p.tiles_per = 1 + two, p.row_tiles = int(row_tiles), p.ranks = 1 << log;
@@ -1182,7 +1248,7 @@ cudaError_t by_source(const neko_paged_attention_args& a, const neko_tree* tree,
     p.group = a.n_head / c.n_kv;
     p.group_inv = ((uint64_t(1) << 32) + p.group - 1) / p.group;
     const int64_t key_tiles = (int64_t(c.max_pages) * c.page_size + kKeys - 1) / kKeys;
-    const int64_t items = split<HD>(p, (rows + kRows - 1) / kRows, int64_t(c.n_seq) * c.n_kv, key_tiles, a.type == NEKO_T_F32);
+    const int64_t items = split<HD>(p, (rows + kRows - 1) / kRows, int64_t(c.n_seq) * c.n_kv, key_tiles, a.type == NEKO_T_F32, tree && c.n_seq > 1);
     if (items * p.ranks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     p.flush = nullptr, p.taken = nullptr;
     p.slots = int(std::min<int64_t>(items * p.ranks, num_sms()));

@@ -48,12 +48,16 @@ __device__ __forceinline__ uint4 recode16(uint4 v, float ratio) {
 // still to be read has been written over: a group of tokens is read into registers, then written, then the next. 8-bit: one
 // target page after the other, for its scale is that of all the tokens that end in it; those come from it or from later pages, whose
 // scales are still the old ones.
-constexpr int kWarps = 4, kBatch = 4;
+// Bound by latency: path, table, scales and tokens one after the other, with little in each warp (64 sequences of up to 16 nodes,
+// 72 planes of 8 e4m3 heads, memory cold: 50 us; 4 CTAs an SM at 116 registers 63, 8 at 64 registers 54).
+constexpr int kWarps = 4, kBatch = 4, kStay = 4;  // warps of a CTA; pieces of tokens, and of tokens that stay, that a lane has in flight
+constexpr int kAtOnce = 6;                          // CTAs of an SM: 80 registers a thread
 template <int HD, bool Q8>
-__global__ void __launch_bounds__(32 * kWarps) paged_compact_kernel(const neko_paged_planes c, const int32_t* __restrict__ start_of,
+__global__ void __launch_bounds__(32 * kWarps, kAtOnce) paged_compact_kernel(const neko_paged_planes c, const int32_t* __restrict__ start_of,
                                                                   const int32_t* __restrict__ path_of, int64_t path_stride,
                                                                   const int32_t* __restrict__ count_of, int max_count, int page_log) {
-    constexpr int kRow = HD * (Q8 ? 1 : 2), kLanes = kRow / 16, kPer = 32 / kLanes;  // bytes of a token, lanes, tokens of a group's step
+    constexpr int kRow = HD * (Q8 ? 1 : 2), kLanes = kRow / 16, kPer = 32 / kLanes,  // bytes of a token, lanes, tokens of a group's step
+                  kB = kBatch < 32 / kPer ? kBatch : 32 / kPer;
     const int lane = threadIdx.x & 31, head = blockIdx.y * kWarps + (threadIdx.x >> 5), s = blockIdx.x, plane = blockIdx.z;
     if (head >= c.n_kv) return;
     const int32_t* path = path_of + int64_t(s) * path_stride;
@@ -79,58 +83,80 @@ __global__ void __launch_bounds__(32 * kWarps) paged_compact_kernel(const neko_p
         return x >= 0 && x <= (1 << 30) ? start + x : -1;
     };
     for (int k0 = 0; k0 < count;) {
-        // tokens of one target page
+        // Tokens of one target page. What says where they come from is read by a lane for each of 32 tokens, and the tokens of the
+        // first batch before anything waits for the scales.
         const int k1 = min(count, k0 + (in_page + 1) - ((start + k0) & in_page));
         const int to_page = page_at(start + k0);
-        [[maybe_unused]] float scale = 0.0f;
-        if constexpr (Q8) {
-            if (to_page >= 0) {
+        if (to_page >= 0) {
+            int from = -1, page = -1;
+            [[maybe_unused]] float mine = 0.0f;  // the scale of the lane's token's page
+            auto look = [&](int kb) {
+                from = kb + lane < k1 ? source_of(kb + lane) : -1;
+                page = page_at(from);
+                if constexpr (Q8) mine = page >= 0 ? scales[page * c.scale_stride] : 0.0f;
+            };
+            uint4 v[kB];
+            // the batch's tokens kb + kk ..: bits of those that there are
+            auto load = [&](int kb, int kk) {
+                int got = 0;
+#pragma unroll
+                for (int b = 0; b < kB; b++) {
+                    const int i = kk + b * kPer + lane / kLanes, f = __shfl_sync(0xffffffffu, from, i), p = __shfl_sync(0xffffffffu, page, i);
+                    if (p < 0 || (!Q8 && f == start + kb + i)) continue;
+                    if (f == start + kb + i) got |= 256 << b;  // stays where it is
+                    v[b] = *reinterpret_cast<const uint4*>(row_at(p, f) + lane % kLanes * 16), got |= 1 << b;
+                }
+                return got;
+            };
+            look(k0);
+            int got = load(k0, 0);
+            [[maybe_unused]] float scale = 0.0f;
+            if constexpr (Q8) {
                 const int stay = k0 == 0 ? start & in_page : 0;  // tokens of this page before the moved ones
                 const float old = scales[to_page * c.scale_stride];
-                if (stay) scale = old;
-                bool any = stay;
-                for (int k = k0 + lane; k < k1; k += 32) {
-                    const int page = page_at(source_of(k));
-                    if (page >= 0) scale = fmaxf(scale, scales[page * c.scale_stride]), any = true;
+                bool any = stay || page >= 0;
+                scale = stay ? fmaxf(old, mine) : mine;
+                for (int k = k0 + 32 + lane; k < k1; k += 32) {
+                    const int p = page_at(source_of(k));
+                    if (p >= 0) scale = fmaxf(scale, scales[p * c.scale_stride]), any = true;
                 }
                 scale = warp_max(scale);
                 any = __any_sync(0xffffffffu, any);
                 if (any && stay && scale > old) {
                     uint4* w = reinterpret_cast<uint4*>(row_at(to_page, 0));
-                    for (int i = lane; i < stay * kLanes; i += 32) w[i] = recode16(w[i], old / scale);
+                    const float ratio = old / scale;
+                    for (int i = lane; i < stay * kLanes; i += 32 * kStay) {
+                        uint4 x[kStay];
+#pragma unroll
+                        for (int b = 0; b < kStay; b++)
+                            if (i + 32 * b < stay * kLanes) x[b] = w[i + 32 * b];
+#pragma unroll
+                        for (int b = 0; b < kStay; b++)
+                            if (i + 32 * b < stay * kLanes) w[i + 32 * b] = recode16(x[b], ratio);
+                    }
                 }
                 if (!any) scale = old;
             }
-        }
-        if (to_page >= 0) {
-            for (int k = k0; k < k1; k += kPer * kBatch) {
-                uint4 v[kBatch];
-                uint8_t* to[kBatch];
+            for (int kb = k0; kb < k1; kb += 32) {
+                if (kb > k0) look(kb);
+                for (int kk = 0; kk < min(32, k1 - kb); kk += kPer * kB) {
+                    if (kb > k0 || kk) got = load(kb, kk);
+                    __syncwarp();
 #pragma unroll
-                for (int b = 0; b < kBatch; b++) {
-                    const int kk = k + b * kPer + lane / kLanes;
-                    to[b] = nullptr;
-                    if (kk >= k1) continue;
-                    const int from = source_of(kk), page = page_at(from);
-                    if (page < 0) continue;
-                    float ratio = 1.0f;
-                    if constexpr (Q8) {
-                        const float x = scales[page * c.scale_stride];
-                        if (x < scale) ratio = x / scale;
+                    for (int b = 0; b < kB; b++) {
+                        const int i = kk + b * kPer + lane / kLanes;
+                        [[maybe_unused]] const float x = __shfl_sync(0xffffffffu, mine, i);
+                        if (!(got >> b & 1)) continue;
+                        if constexpr (Q8) {
+                            if ((got >> b & 256) && x >= scale) continue;
+                            v[b] = recode16(v[b], x < scale ? x / scale : 1.0f);
+                        }
+                        *reinterpret_cast<uint4*>(row_at(to_page, start + kb + i) + lane % kLanes * 16) = v[b];
                     }
-                    if (from == start + kk && ratio == 1.0f) continue;
-                    v[b] = *reinterpret_cast<const uint4*>(row_at(page, from) + lane % kLanes * 16);
-                    if constexpr (Q8) v[b] = recode16(v[b], ratio);
-                    to[b] = row_at(to_page, start + kk) + lane % kLanes * 16;
+                    __syncwarp();
                 }
-                __syncwarp();
-#pragma unroll
-                for (int b = 0; b < kBatch; b++)
-                    if (to[b]) *reinterpret_cast<uint4*>(to[b]) = v[b];
-                __syncwarp();
             }
             if constexpr (Q8) {
-                __syncwarp();
                 if (lane == 0) scales[to_page * c.scale_stride] = scale;
                 __syncwarp();
             }
@@ -152,7 +178,7 @@ cudaError_t go(const neko_paged_planes& c, const int32_t* start, const int32_t* 
 cudaError_t launch_paged_copy(const neko_paged_planes& c, const int32_t* src, const int32_t* dst, int n, cudaStream_t st) {
     const int size = c.type == NEKO_T_E4M3 ? 1 : 2;
     const int64_t pieces = int64_t(c.n_kv) * c.page_size * c.head_dim * size / 16, chunks = (pieces + kCopyThreads * kPieces - 1) / (kCopyThreads * kPieces);
-    if (chunks * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    if (pieces > 0x7fffffff || chunks * n > 0x7fffffff) return cudaErrorInvalidConfiguration;
     return launch_ex(paged_copy_kernel, dim3(unsigned(chunks * n), unsigned(c.planes)), dim3(kCopyThreads), 0, st, false, c, src, dst, int(chunks),
                      int(pieces), size);
 }

@@ -279,13 +279,15 @@ int neko_op_paged_tree_append(const neko_paged_append_args* args, const int32_t*
 int neko_op_paged_tree_attention(const neko_paged_attention_args* args, const neko_tree* tree, void* stream);
 /* The masks and depths of trees given by parents: parent[q_start[s] + i] in [0, i) is node i's parent, counted from the
  * sequence's first node; anything else makes node i a root. Bit j of row i: j is i or an ancestor of i. Any of mask and depth may
- * be NULL. Rows of no sequence keep what they held. At most NEKO_MAX_NODES nodes a sequence. */
+ * be NULL. Rows of no sequence become zeros (with n_seq or max_new 0 nothing is written). At most NEKO_MAX_NODES nodes a
+ * sequence. */
 #define NEKO_MAX_NODES 4096
 int neko_op_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
                        int32_t* depth, void* stream);
 /* Walks each sequence's tree along the tokens chosen at its nodes: from node 0 to the lowest child whose draft is the token
  * chosen at the node, and so on. path [n_seq][max_new]: the nodes walked through, 0 first, zeros behind them; count [n_seq]: how
- * many; token [n_seq]: the one chosen at the last of them. A sequence without nodes has count 0 and token -1. */
+ * many; token [n_seq]: the one chosen at the last of them. A sequence without nodes (or
+ * left out, with more than max_new or rows outside `tokens`) has count 0 and token -1. */
 int neko_op_tree_accept(const int32_t* chosen, const int32_t* draft, const int32_t* parent, const int32_t* q_start, int n_seq,
                         int tokens, int max_new, int32_t* path, int32_t* count, int32_t* token, void* stream);
 
@@ -306,9 +308,10 @@ typedef struct neko_paged_planes {
     int32_t head_dim;
 } neko_paged_planes;
 /* In every plane, token start[s] + path[s][k] of sequence s becomes token start[s] + k, k < count[s] (at most max_count), as if all
- * were read before any is written: what tree_accept leaves of a tree, brought together. Rows of path are path_stride apart. Tokens
- * from or to pages that are not resident stay away; tokens at or past start[s] + count[s] are no longer the sequence's (what their
- * places hold is not said). start[s] < 0: inactive.
+ * were read before any is written: what tree_accept leaves of a tree, brought together. A path ascends from 0 or more, each entry
+ * larger than the one before, as tree_accept's do; rows of path are path_stride apart. Tokens from or to pages that are not
+ * resident stay away; tokens at or past start[s] + count[s] are no longer the sequence's (what their places hold is not said).
+ * start[s] < 0: inactive.
  * NEKO_T_E4M3: a page that gets tokens takes as scale the largest of its own (where tokens before start[s] are in it) and of the
  * pages that its tokens come from; codes are multiplied by old / new scale (exact, but for codes that become subnormal). A page
  * that gets tokens is in one sequence's table only, once. */

@@ -1,5 +1,7 @@
 // Bookkeeping of trees of drafted tokens (neko_op_tree_masks, neko_op_tree_accept): a CTA for each sequence, its nodes in shared
 // memory. Both are bound by latency: a chain of dependent reads as long as the tree is deep, in shared memory instead of L2.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace neko {
@@ -19,12 +21,32 @@ __device__ __forceinline__ bool nodes_of(const int32_t* q_start, int s, int toke
 }
 
 // A thread for each node walks up to the root. Parents come before their children, so the bits of the node's words come from the
-// last to the first: each word is written once, from a register.
-__global__ void __launch_bounds__(kThreads) tree_masks_kernel(const int32_t* __restrict__ parent, const int32_t* __restrict__ q_start, int tokens,
-                                                             int max_new, uint64_t* __restrict__ mask, int words, int32_t* __restrict__ depth) {
+// last to the first: each word is written once, from a register. The CTAs behind the sequences' set the rows of no sequence to
+// zero, which costs less than a fill before the kernel.
+__global__ void __launch_bounds__(kThreads) tree_masks_kernel(const int32_t* __restrict__ parent, const int32_t* __restrict__ q_start, int n_seq,
+                                                             int tokens, int max_new, uint64_t* __restrict__ mask, int words, int32_t* __restrict__ depth) {
     extern __shared__ int32_t up[];
+    // rows [from, to), by this CTA of `many`
+    auto clear = [&](int from, int to, int cta, int many) {
+        from = max(from, 0), to = min(to, tokens);
+        if (from >= to) return;
+        const int64_t at = int64_t(cta) * kThreads + threadIdx.x, step = int64_t(many) * kThreads;
+        if (mask)
+            for (int64_t i = int64_t(from) * words + at; i < int64_t(to) * words; i += step) mask[i] = 0;
+        if (depth)
+            for (int64_t i = from + at; i < to; i += step) depth[i] = 0;
+    };
+    if (blockIdx.x >= n_seq) {
+        const int cta = blockIdx.x - n_seq, many = gridDim.x - n_seq;
+        clear(0, q_start[0], cta, many);
+        clear(q_start[n_seq], tokens, cta, many);
+        return;
+    }
     int row0, n;
-    if (!nodes_of(q_start, blockIdx.x, tokens, max_new, row0, n)) return;
+    if (!nodes_of(q_start, blockIdx.x, tokens, max_new, row0, n)) {
+        if (n < 0) clear(row0, q_start[blockIdx.x + 1], 0, 1);
+        return;
+    }
     for (int i = threadIdx.x; i < n; i += kThreads) up[i] = parent[row0 + i];
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -57,7 +79,6 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(const int32_t* __
     const int s = blockIdx.x;
     int row0, n;
     const bool any = nodes_of(q_start, s, tokens, max_new, row0, n);
-    if (n < 0) return;
     for (int i = threadIdx.x; i < n; i += kThreads) next[i] = 0x7fffffff;
     if (threadIdx.x == 0) steps = 0;
     __syncthreads();
@@ -84,8 +105,9 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(const int32_t* __
 
 cudaError_t launch_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
                               int32_t* depth, cudaStream_t st) {
-    return launch_ex(tree_masks_kernel, dim3(n_seq), dim3(kThreads), size_t(max_new) * 4, st, false, parent, q_start, tokens, max_new, mask, words,
-                     depth);
+    const int64_t blank = std::min<int64_t>((int64_t(tokens) * words + 4095) / 4096, num_sms());
+    return launch_ex(tree_masks_kernel, dim3(unsigned(n_seq + blank)), dim3(kThreads), size_t(max_new) * 4, st, false, parent, q_start, n_seq, tokens,
+                     max_new, mask, words, depth);
 }
 
 cudaError_t launch_tree_accept(const int32_t* chosen, const int32_t* draft, const int32_t* parent, const int32_t* q_start, int n_seq,

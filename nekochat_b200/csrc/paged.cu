@@ -130,6 +130,7 @@ extern "C" int neko_op_tree_masks(const int32_t* parent, const int32_t* q_start,
     if (!parent || !q_start) return paged_fail(NEKO_ERR_ARG, op, "null pointer");
     max_new = std::min(max_new, tokens);
     if (max_new > NEKO_MAX_NODES) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 4096 nodes a sequence");
+    if (n_seq > (1 << 30)) return paged_fail(NEKO_ERR_UNSUPPORTED, op, "more than 2^30 sequences");
     if (mask && (int64_t(words) * 64 < max_new || !aligned(mask, 8))) return paged_fail(NEKO_ERR_ARG, op, "mask words for max_new nodes, 8-byte aligned");
     return finish(op, launch_tree_masks(parent, q_start, n_seq, tokens, max_new, mask, words, depth, static_cast<cudaStream_t>(stream)));
 }
@@ -213,8 +214,8 @@ extern "C" int neko_op_status(void* stream) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return finish(op, e);
     return paged_fail(NEKO_ERR_DEVICE, op,
-                      code == kErrBadIndex ? "a sequence of a paged call had more new tokens than max_new, rows outside `tokens`, or "
-                                             "positions past the rotation table; those rows were left out"
+                      code == kErrBadIndex ? "a sequence of a paged call had more new tokens than max_new (or a path more than max_count), "
+                                             "rows outside `tokens`, or positions past the rotation table; those rows were left out"
                       : code == kErrMbarTimeout ? "a bounded wait of a paged kernel gave up; its output is not valid"
                                                 : "a paged kernel found its shared memory misaligned and did nothing");
 }

@@ -363,17 +363,15 @@ def tree_masks(parent, q_start, max_new):
     root), sequence s's nodes at q_start[s] .. q_start[s + 1] - 1, at most max_new. Returns mask int64
     [tokens][ceil(max_new / 64)] (bit j: node j is the node itself or an ancestor) and depth int32 [tokens]. Rows of no
     sequence are zeros."""
-    import torch
     types = _types or _setup()
     dev, tokens, i32 = _on_device(parent, "tree_masks", types), parent.numel(), types["i32"]
     n_seq, words = q_start.numel() - 1, max((max_new + 63) // 64, 1)
-    both = torch.zeros(tokens * words + (tokens + 1) // 2, dtype=types["i64"], device=parent.device)  # one fill, not two
-    mask, depth = both.as_strided((tokens, words), (words, 1)), both.view(i32).as_strided((tokens,), (1,), 2 * tokens * words)
+    mask, depth = parent.new_empty((tokens, words), dtype=types["i64"]), parent.new_empty(tokens)
     rc = types["masks"](_vector(parent, "tree_masks parent", i32, tokens, dev), _vector(q_start, "tree_masks q_start", i32, n_seq + 1, dev),
                         n_seq, tokens, max_new, mask.data_ptr(), words, depth.data_ptr(), types["stream"](dev))
     if rc:
         check(rc, "tree_masks")
-    return mask, depth
+    return (mask, depth) if n_seq and max_new else (mask.zero_(), depth.zero_())
 
 
 def tree_accept(chosen, draft, parent, q_start, max_new):
@@ -384,11 +382,12 @@ def tree_accept(chosen, draft, parent, q_start, max_new):
     types = _types or _setup()
     dev, tokens, i32 = _on_device(parent, "tree_accept", types), parent.numel(), types["i32"]
     n_seq = q_start.numel() - 1
-    path, count, token = parent.new_empty(n_seq * (max_new + 2)).split([n_seq * max_new, n_seq, n_seq])
-    path = path.view(n_seq, max_new)
+    if n_seq < 0 or max_new < 0:
+        raise NekoError("tree_accept: q_start [sequences + 1], max_new of zero or more")
+    path, count, token = parent.new_empty((n_seq, max_new)), parent.new_empty(n_seq), parent.new_empty(n_seq)
     rc = types["accept"](_vector(chosen, "tree_accept chosen", i32, tokens, dev), _vector(draft, "tree_accept draft", i32, tokens, dev),
-                         _vector(parent, "tree_accept parent", i32, tokens, dev), _vector(q_start, "tree_accept q_start", i32, n_seq + 1, dev), n_seq, tokens, max_new, path.data_ptr(),
-                         count.data_ptr(), token.data_ptr(), types["stream"](dev))
+                         _vector(parent, "tree_accept parent", i32, tokens, dev), _vector(q_start, "tree_accept q_start", i32, n_seq + 1, dev),
+                         n_seq, tokens, max_new, path.data_ptr(), count.data_ptr(), token.data_ptr(), types["stream"](dev))
     if rc:
         check(rc, "tree_accept")
     return path, count, token

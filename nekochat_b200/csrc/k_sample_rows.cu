@@ -987,10 +987,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
             // the bound: a key that `want` groups reach, by halving below the bits that the largest has in common with the smallest group
             const uint32_t key = tid < groups ? order_key(g) : 0xFFFFFFFFu, top = order_key(m);
             uint32_t least = __reduce_min_sync(0xffffffffu, key);
-            if (lane == 0) reinterpret_cast<uint32_t*>(sh.warp_sum)[tid >> 5] = least;
+            uint32_t* by_warp = reinterpret_cast<uint32_t*>(sh.warp_sum) + kWarps;  // behind the warps' largest, which others may still read
+            if (lane == 0) by_warp[tid >> 5] = least;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) least = min(least, reinterpret_cast<uint32_t*>(sh.warp_sum)[w]);
+            for (int w = 0; w < kWarps; w++) least = min(least, by_warp[w]);
             const int same = __clz(top ^ least);  // 32: all alike
             uint32_t bound = same ? top & ~(0xFFFFFFFFu >> (same - 1) >> 1) : 0u;
             const int last = max(min(31 - same - 8, 16), 0);

@@ -908,7 +908,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     s.data = reinterpret_cast<const uint4*>(src - ph);
     s.row.alone = NAN;
     if (tid == 0) sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
-    const float temperature = fminf(!a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature, 1e36f);  // above, all weigh the same
+    const float asked = !a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature;
+    const float temperature = asked > 0.0f ? fminf(asked, 1e36f) : 0.0f;  // above, all weigh the same; NaN: greedy
     const float min_p = a.min_ps ? a.min_ps[r] : a.min_p, top_p = a.top_ps ? a.top_ps[r] : a.top_p;
     int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
     if (top_k < 0 || top_k >= a.vocab) top_k = 0;

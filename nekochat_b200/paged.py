@@ -244,11 +244,11 @@ class PagedDecoder:
         each sequence, the tokens gained: the drafts walked through and the one chosen at the last of them."""
         import torch
         c = self.cache
+        if any(len(t) != len(p) for _, t, p in batch):
+            raise NekoError("verify: a parent for each token")
         seqs, news, tokens, begin = self._batch(batch)
         T, n = len(tokens), len(seqs)
         parents = np.concatenate([np.asarray(p, np.int32) for _, _, p in batch])
-        if len(parents) != T:
-            raise NekoError("verify: a parent for each token")
         start = np.array([c.length[x] for x in seqs], np.int32)
         table = c.rows(seqs)
         ints = np.concatenate([tokens, parents, begin, start, start + np.asarray(news, np.int32), table.ravel()])
@@ -366,6 +366,8 @@ class Drafts:
     tokens ended, or where there are none the same one."""
 
     def __init__(self, tokens, gram=2, looks=4):
+        if gram < 1 or looks < 1:
+            raise NekoError("Drafts: gram and looks are 1 or more")
         self.gram, self.looks, self.tokens, self.ends = gram, looks, [], {}
         for t in tokens:
             self.add(t)
@@ -378,6 +380,8 @@ class Drafts:
 
     def tree(self, nodes):
         """Up to `nodes` tokens and their parents: the newest, and behind it the guesses, shared beginnings once."""
+        if not self.tokens:
+            return [], []
         tree, parents, follow = self.tokens[-1:], [-1], {}
         for g in range(min(self.gram, len(self.tokens)), 0, -1):
             ends = self.ends.get(tuple(self.tokens[-g:]), ())[-self.looks:]

@@ -294,3 +294,19 @@ def test_the_sampling_reference():
         assert want_of.sample([-math.inf, math.nan], 0.5, 1.0, 0, 1.0, 0.0, held) == (-1, 0.0)
         assert want_of.sample([5.0, math.inf, math.inf], 0.7, 1.0, 0, 1.0, 0.0, held)[0] == 2
     assert struct.calcsize("@2P2i") == C.sizeof(C.c_void_p) * 3
+
+
+def test_parents_of_another_number_change_nothing(monkeypatch):
+    m = decoder(pages=4)
+    s, t = m.cache.open(), m.cache.open()
+    with pytest.raises(nb.NekoError, match="a parent for each token"):
+        m.verify([(s, [1, 2], [-1]), (t, [1], [-1, 0])], None)
+    assert len(m.cache.free) == 4
+
+
+def test_drafts_of_nothing():
+    from nekochat_b200.paged import Drafts
+    assert Drafts([]).tree(5) == ([], [])
+    for kw in (dict(gram=0), dict(looks=0)):
+        with pytest.raises(nb.NekoError, match="1 or more"):
+            Drafts([1, 2], **kw)

@@ -3,6 +3,8 @@ sampling, masks and walks, moving tokens and pages, and all of them together.
 
 Whole numbers are equal. Attention: the bound of test_gpu_cache_edges (scores 2^-20 of their reach, weights 2^-18 or f16's 2^-11,
 the output's rounding). Probabilities: sums and exponentials in 64 bits, weights to 2^-45 of the largest, one rounding to f32: 2^-23."""
+import math
+
 import numpy as np
 import pytest
 
@@ -575,3 +577,95 @@ def test_command_samples_and_drafts():
     r = subprocess.run([sys.executable, "-m", "nekochat_b200.paged", "--max-new", "4", "--temperature", "0.8", "--top-k", "40", "--draft", "6", "--copies", "2"],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "tokens/s" in r.stdout and r.stdout.count("prompt tokens") == 6, r.stderr
+
+
+# ------------------------------------------------------------------------------------------------ rows and sequences that are left out
+def test_rows_of_no_sequence_are_zeros(torch):
+    """Before the first sequence, behind the last and of a sequence that is left out, in memory that held other things; as many as
+    several CTAs clear."""
+    from nekochat_b200 import NekoError, ops
+    for starts, tokens, n, bad in (([2, 5, 5, 9], 12, 70, ()), ([0, 1], 3000, 900, ()), ([7, 7], 40, 64, ()), ([0, 3, 9, 12], 12, 4, (3, 9))):
+        parent = torch.arange(-1, tokens - 1, dtype=torch.int32, device="cuda")
+        parent[[s for s in starts[:-1] if s < tokens]] = -1
+        for a, b in zip(starts, starts[1:]):
+            parent[a:b] = torch.arange(-1, b - a - 1, dtype=torch.int32)
+        words = -(-n // 64)
+        for shape in ((tokens, words * 2), (tokens,)):  # the allocator hands these out again
+            torch.full(shape, -1, dtype=torch.int32, device="cuda")
+        mask, depth = ops.tree_masks(parent, ints(torch, *starts), n)
+        want_mask, want_depth = np.zeros((tokens, words), np.uint64), np.zeros(tokens, np.int32)
+        for a, b in zip(starts, starts[1:]):
+            if (a, b) == bad:
+                continue
+            for i in range(b - a):  # lines
+                want_depth[a + i] = i
+                for j in range(i + 1):
+                    want_mask[a + i, j // 64] |= np.uint64(1) << np.uint64(j % 64)
+        assert np.array_equal(mask.cpu().numpy().view(np.uint64), want_mask) and np.array_equal(depth.cpu().numpy(), want_depth)
+        if bad:
+            with pytest.raises(NekoError, match="max_new"):
+                ops.status()
+        ops.status()
+    mask, depth = ops.tree_masks(parent, ints(torch, 0), 5)
+    assert not mask.any() and not depth.any() and mask.shape == (12, 1)
+
+
+def test_a_sequence_left_out_walks_nowhere(torch):
+    from nekochat_b200 import NekoError, ops
+    parent, draft = ints(torch, -1, 0, 1, 2, -1, 0), ints(torch, 1, 2, 3, 4, 5, 6)
+    torch.full((2, 3), 7, dtype=torch.int32, device="cuda")
+    path, count, token = ops.tree_accept(ints(torch, 2, 3, 4, 5, 6, 8), draft, parent, ints(torch, 0, 4, 6), 3)
+    assert path.tolist() == [[0, 0, 0], [0, 1, 0]] and count.tolist() == [0, 2] and token.tolist() == [-1, 8]
+    with pytest.raises(NekoError, match="max_new"):
+        ops.status()
+
+
+@pytest.mark.parametrize("n_seq", [2, 128, 129, 300])
+def test_trees_of_many_sequences(torch, n_seq):
+    """Sequences in any order of their lengths, alike and empty ones, up to and past the number that is ordered by them."""
+    from nekochat_b200 import ops
+    H, KV, hd, ps, new = 8, 2, 64, 32, 9  # 36 rows of a KV head: the kernel for many rows
+    rng = np.random.default_rng(n_seq)
+    ctx = rng.choice([0, 1, 31, 150, 150, 300], n_seq)
+    sizes = np.where(rng.random(n_seq) < 0.1, 0, rng.integers(1, new + 1, n_seq))
+    kv_len, at = ctx + sizes, np.concatenate([[0], np.cumsum(sizes)])
+    width = -(-int(kv_len.max()) // ps)
+    table = rng.permutation(n_seq * width).reshape(n_seq, width).astype(np.int32)
+    k, v = (torch.randn((n_seq * width, KV, ps, hd), device="cuda").half() for _ in range(2))
+    parent = np.concatenate([[-1] + [int(rng.integers(0, i)) for i in range(1, m)] if m else [] for m in sizes]).astype(np.int32)
+    q = torch.randn((len(parent), H, hd), device="cuda")
+    mask, depth = ops.tree_masks(ints(torch, *parent), ints(torch, *at), new)
+    whole = ops.paged_tree_attention(q, k, v, torch.from_numpy(table).cuda(), ints(torch, *kv_len), mask, depth, q_start=ints(torch, *at), max_new=new)
+    ops.status()
+    for s in range(n_seq):  # each by the definition
+        a, b = int(at[s]), int(at[s + 1])
+        if a == b:
+            continue
+        n = int(kv_len[s])
+        kk, vv = (x[torch.from_numpy(table[s]).long().cuda()].transpose(0, 1).reshape(KV, -1, hd)[:, :n].double() for x in (k, v))
+        z = torch.einsum("tghd,gjd->ghtj", q[a:b].double().view(b - a, KV, H // KV, hd), kk) / hd ** 0.5
+        seen = torch.ones((b - a, n), dtype=torch.bool, device="cuda")
+        bits = mask[a:b, 0, None] >> torch.arange(b - a, device="cuda") & 1
+        seen[:, n - (b - a):] = bits.bool()
+        w = torch.softmax(z.masked_fill(~seen, -float("inf")), -1)
+        want = torch.einsum("ghtj,gjd->tghd", w, vv).reshape(b - a, H, hd)
+        # |values| < 6. Queries and weights enter as two f16 (22 bits); scores, of 64 products of sizes up to 16 and divided by 8, are
+        # off by less than 64 * 16 / 8 * 2^-21 = 2^-14 even if all errors agree, a softmax by as much times |value|
+        assert (whole[a:b].double() - want).abs().max() < 6 * 2.0 ** -14, s
+
+
+def test_numbers_of_a_call_out_of_range(torch):
+    """A temperature that is no number is greedy; numbers beyond f32 and 32 bits count as the ends of the range."""
+    from nekochat_b200 import ops
+    x = torch.randn((4, 500), device="cuda")
+    u = torch.rand(4, dtype=torch.float64, device="cuda")
+    greedy = x.argmax(1).int()
+    assert torch.equal(ops.sample_rows(x, u, math.nan)[0], greedy)
+    t = torch.tensor([math.nan, -1.0, 0.0, -math.inf], device="cuda")
+    assert torch.equal(ops.sample_rows(x, u, t)[0], greedy)
+    flat = (u * 500).floor().int()
+    for hot in (1e300, math.inf, 1e36):
+        assert torch.equal(ops.sample_rows(x, u, hot)[0], flat)
+    for k in (2 ** 40, -2 ** 40, 0):
+        assert torch.equal(ops.sample_rows(x, u, 0.9, k, 1e300, -1e300)[0], ops.sample_rows(x, u, 0.9)[0])
+    assert torch.equal(ops.sample_rows(x, u, 0.9, 0, -1e300)[0], greedy) and torch.equal(ops.sample_rows(x, u, 0.9, 0, 1.0, 1e300)[0], greedy)

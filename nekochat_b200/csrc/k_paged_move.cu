@@ -10,7 +10,8 @@ namespace {
 
 constexpr int kCopyThreads = 256, kPieces = 4;  // 16-byte pieces that a thread has in flight
 
-// A CTA for each 16 KB of a page and plane: bound by memory, every thread's loads come before its stores.
+// A CTA for each 16 KB of a page and plane: bound by memory, every thread's loads come before its stores. 301 pages of 64 tokens, 8 e4m3
+// heads of 128, 72 planes: 427 us, 6.65 TB/s of reads and writes, the measured copy rate; 3 f16 pages in 56 planes 6 us.
 __global__ void __launch_bounds__(kCopyThreads) paged_copy_kernel(const neko_paged_planes c, const int32_t* __restrict__ src,
                                                                  const int32_t* __restrict__ dst, int chunks, int pieces, int size) {
     const int pair = blockIdx.x / chunks, chunk = blockIdx.x % chunks, plane = blockIdx.y;

@@ -29,6 +29,11 @@
 // finite in a tile that some row does not see whole are zeroed too and added by the threads of the rows that see them.
 // A cluster of CTAs splits the keys when there are few row tiles and joins over distributed shared memory in rank
 // order. Every wait is bounded and gives up once another role has failed.
+//
+// Trees of drafted tokens (neko_op_paged_tree_attention): every row's keys end with the tree, the masks are read in the key tiles
+// that hold nodes, and positions go by depth there. 16 trees of 21 to 63 bf16 nodes, 32 heads on 8, capped, on 900 to 8,191 f16
+// keys: 223 us (338 MB, 52 us at the measured copy rate; 58 GFLOP, 259 TFLOP/s; 31 % of the SMs' issue): the chain of a key tile
+// with a tanh in it, clusters whose CTAs have few tiles each, and the ends of ragged lengths.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -20,6 +20,10 @@
 //    added up over the cluster, gives the step that the cut falls into; its tokens are collected and ranked, or where they are
 //    too many the key's digits (11, 11 and 10 bits) lead to the cut's value, whose equals are cut by index.
 // The draw goes through the slices in the order of the vocabulary: sums of CTAs, of warps' segments, of lanes.
+//
+// From a graph: 1 x 151,936 f32, k = 40, p = 0.95: 11.5 us (launch, two passes, the cluster's meetings); 64 x 50,257 bf16 with mixed
+// parameters 57 us, the time of the slowest rows (k = 1000, some 40 us alone; nuclei 35; k = 40 10); 320 x 151,936 nuclei 271 us
+// beside 30 for reading them once: 49 M weights in 64 bits, about 35 cycles a warp's 32, and the meetings.
 #include <cooperative_groups.h>
 
 #include <algorithm>

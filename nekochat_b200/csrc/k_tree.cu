@@ -1,5 +1,6 @@
 // Bookkeeping of trees of drafted tokens (neko_op_tree_masks, neko_op_tree_accept): a CTA for each sequence, its nodes in shared
-// memory. Both are bound by latency: a chain of dependent reads as long as the tree is deep, in shared memory instead of L2.
+// memory. Both are bound by latency: a chain of dependent reads as long as the tree is deep, in shared memory instead of L2 (12 nodes:
+// 4.8 us for both kernels from a graph; 128 trees of 17 to 64: 6.1).
 #include <algorithm>
 
 #include "paged.cuh"

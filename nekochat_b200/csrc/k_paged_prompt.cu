@@ -943,7 +943,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
             if (__any_sync(0xffffffffu, up)) {
                 float f = 1.0f;
-                if (up) {
+                // Trees' other rows move along, for the trip is made anyway: they will not ask for one of their own so soon.
+                if (TREE ? top > row_max && top < INFINITY : up) {
                     f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
                     row_max = top;
                     if (!kScaled) row_sum *= f;

@@ -54,7 +54,7 @@ constexpr int kSortedOff = kCand * 8, kMineOff = 2 * kCand * 8;
 __host__ __device__ constexpr int counts_off(int ctas) { return kMineOff + (ctas > 1 ? kMine : kCand) * 8; }
 __host__ __device__ constexpr int window_off(int ctas) { return counts_off(ctas) + kSteps * 4; }
 // tokens of the window in one CTA: with one CTA two of them fill an SM's shared memory
-__host__ __device__ constexpr int window_room(int ctas) { return ctas == 1 ? 8192 : ctas == 2 ? 5120 : ctas == 4 ? 3072 : 2048; }
+__host__ __device__ constexpr int window_room(int ctas) { return ctas == 1 ? 8192 : ctas == 2 ? 5120 : ctas == 4 ? 3584 : 2048; }
 __host__ __device__ constexpr int aux_bytes(int ctas) { return window_off(ctas) + window_room(ctas) * 8; }
 static_assert(window_off(kMaxCluster) >= kRing * kThreads * 16, "the ring");
 static_assert(window_off(kMaxCluster) >= 3 * kBins * 4, "the histograms");

@@ -32,7 +32,7 @@
 //
 // Trees of drafted tokens (neko_op_paged_tree_attention): every row's keys end with the tree, the masks are read in the key tiles
 // that hold nodes, and positions go by depth there. 16 trees of 21 to 63 bf16 nodes, 32 heads on 8, capped, on 900 to 8,191 f16
-// keys: 223 us (338 MB, 52 us at the measured copy rate; 58 GFLOP, 259 TFLOP/s; 31 % of the SMs' issue): the chain of a key tile
+// keys: 208 us (338 MB, 52 us at the measured copy rate; 58 GFLOP, 278 TFLOP/s; 31 % of the SMs' issue): the chain of a key tile
 // with a tanh in it, clusters whose CTAs have few tiles each, and the ends of ragged lengths.
 #include <cooperative_groups.h>
 
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
     int s = b % c.n_seq;
     if constexpr (TREE) {
         // The longest contexts first: a long one that starts last leaves the other SMs idle (16 trees of 63 bf16 nodes on 8,192
-        // keys: 273 us in the sequences' order, 222 this way). Each CTA ranks the lengths itself, once for all sequences.
+        // keys, capped: 252 us in the sequences' order, 208 this way). Each CTA ranks the lengths itself, once for all sequences.
         if (c.n_seq > 1 && c.n_seq <= kSorted) {
             int* lens = reinterpret_cast<int*>(ms.most);
             if (tid < c.n_seq) lens[tid] = a.kv_len[tid];
@@ -943,7 +943,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const neko_pa
             const bool up = top > row_max + kLazy && top < INFINITY;  // also from -inf
             if (__any_sync(0xffffffffu, up)) {
                 float f = 1.0f;
-                // Trees' other rows move along, for the trip is made anyway: they will not ask for one of their own so soon.
+                // Trees' other rows move along, for the trip is made anyway: they will not ask for one of their own so
+                // soon (keys whose sizes differ: 16 of 63 on 8,191 337 -> 308 us, 18 of 64 on 4,095 183 -> 154).
                 if (TREE ? top > row_max && top < INFINITY : up) {
                     f = ex2(row_max - top);  // row_max = -inf: nothing there yet, 0
                     row_max = top;
@@ -1233,8 +1234,8 @@ int64_t split(PromptPlan& p, int64_t tiles, int64_t heads, int64_t key_tiles, bo
                 // Several trees stand behind contexts of any length up to the table's, and the longest start first. Lengths that
                 // are all the table's count a third; lengths of half of it on average, the whole work of which stands over the
                 // CTAs that run at once with a part of the longest for the end, two thirds. bf16, 16 trees of 63 on 900 to 8,191
-                // keys: 261 -> 226 us (capped 346 -> 267, f32 369 -> 290), all on 8,191 271 -> 338; of 17 tokens 173 -> 136 and
-                // 178 -> 216; 64 trees of 63 671 -> 608 and 1005 -> 1019.
+                // keys: 239 -> 202 us (capped 319 -> 250, f32 349 -> 270, 8-bit 445 -> 306), all on 8,191 251 -> 308; of 17 tokens
+                // 168 -> 129 and 172 -> 203; 64 trees of 17 436 -> 359 and 702 -> 656.
                 const int64_t work = n * ((start + (log ? join[two] : 0)) * (1 << log) + key_tiles * step[two] / 2);
                 time = (time + 2 * std::max(most, work / (at_once << log) + most / 4)) / 3;
             }

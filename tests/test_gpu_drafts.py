@@ -669,3 +669,44 @@ def test_numbers_of_a_call_out_of_range(torch):
     for k in (2 ** 40, -2 ** 40, 0):
         assert torch.equal(ops.sample_rows(x, u, 0.9, k, 1e300, -1e300)[0], ops.sample_rows(x, u, 0.9)[0])
     assert torch.equal(ops.sample_rows(x, u, 0.9, 0, -1e300)[0], greedy) and torch.equal(ops.sample_rows(x, u, 0.9, 0, 1.0, 1e300)[0], greedy)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_two_streams_at_once(torch, e4m3):
+    """Calls that run beside each other, each on inputs of its own, give what they give alone."""
+    from nekochat_b200 import ops
+    rng = np.random.default_rng(3)
+    sets = []
+    for n_seq, new in ((5, 40), (40, 3)):
+        ps, KV, hd, ctx = 64, 4, 128, 1500
+        width = -(-(ctx + new) // ps)
+        k, v = (torch.randn((n_seq * width, KV, ps, hd), device="cuda").half() for _ in range(2))
+        scales = {}
+        if e4m3:
+            k, v = (x.to(torch.float8_e4m3fn) for x in (k, v))
+            scales = dict(k_scale=torch.ones((n_seq * width, KV), device="cuda"), v_scale=torch.ones((n_seq * width, KV), device="cuda"))
+        table = torch.randperm(n_seq * width, device="cuda").int().view(n_seq, width)
+        at = torch.arange(n_seq + 1, device="cuda").int() * new
+        parent = ints(torch, *[int(rng.integers(0, i)) if i else -1 for _ in range(n_seq) for i in range(new)])
+        q, x = torch.randn((n_seq * new, 8, hd), device="cuda"), torch.randn((n_seq * new, 20000), device="cuda")
+        u = torch.rand(n_seq * new, dtype=torch.float64, device="cuda")
+        kv_len = torch.full((n_seq,), ctx + new, dtype=torch.int32, device="cuda")
+
+        def call(q=q, k=k, v=v, table=table, kv_len=kv_len, parent=parent, at=at, new=new, scales=scales, x=x, u=u):
+            mask, depth = ops.tree_masks(parent, at, new)
+            out = ops.paged_tree_attention(q, k, v, table, kv_len, mask, depth, q_start=at, max_new=new, **scales)
+            token, prob = ops.sample_rows(x, u, 0.9, 0, 0.9)
+            return (out, token, prob, *ops.tree_accept(token, token, parent, at, new))
+        sets.append(call)
+    alone = [call() for call in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(10):
+        for i, (stream, call) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for want, runs in zip(alone, got):
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(run, want))
+    ops.status()

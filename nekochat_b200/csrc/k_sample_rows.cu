@@ -16,7 +16,7 @@
 //    sample's error (the largest tokens, which would make it large, are summed as they are). One pass over the weights adds up
 //    the row, what lies before that window, and puts the window's tokens aside; among those the cut is found by the exact sums,
 //    which also tell a window that has missed it (then the next way is taken).
-//  * else a histogram over equal steps, of counts or of weights in three pieces of 15 bits (32-bit additions in shared memory),
+//  * else a histogram over equal steps, of counts or of weights in four pieces of 14 bits (32-bit additions in shared memory),
 //    added up over the cluster, gives the step that the cut falls into; its tokens are collected and ranked, or where they are
 //    too many the key's digits (11, 11 and 10 bits) lead to the cut's value, whose equals are cut by index.
 // The draw goes through the slices in the order of the vocabulary: sums of CTAs, of warps' segments, of lanes.
@@ -43,6 +43,7 @@ constexpr int kGroups = kThreads / 8;  // groups of threads whose largest values
 constexpr int kCand = 1024;            // tokens that are ranked by counting
 constexpr int kMine = 512;             // of them those of one CTA of several
 constexpr int kBins = 2048;
+constexpr int kPiece = 14, kPieces = 4;  // bits of a weight's pieces in the histograms, and how many: 2^44 takes 45
 constexpr int kSteps = 4096;           // steps of max - x that a sample of the tokens is counted in
 constexpr int kFine = 1024;            // steps of the window
 constexpr int kRing = 4;
@@ -57,7 +58,9 @@ __host__ __device__ constexpr int window_off(int ctas) { return counts_off(ctas)
 __host__ __device__ constexpr int window_room(int ctas) { return ctas == 1 ? 8192 : ctas == 2 ? 5120 : ctas == 4 ? 3584 : 2048; }
 __host__ __device__ constexpr int aux_bytes(int ctas) { return window_off(ctas) + window_room(ctas) * 8; }
 static_assert(window_off(kMaxCluster) >= kRing * kThreads * 16, "the ring");
-static_assert(window_off(kMaxCluster) >= 3 * kBins * 4, "the histograms");
+static_assert(window_off(kMaxCluster) >= kPieces * kBins * 4, "the histograms");
+// a CTA may hold a whole row, and all its tokens may be in one bin
+static_assert((1ull << kPiece) * NEKO_MAX_VOCAB <= 1ull << 32 && kPiece * kPieces > 44, "a bin holds a row's pieces in 32 bits");
 
 // The order of values as unsigned numbers; zeros are alike.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -497,7 +500,7 @@ struct Sampler {
     template <typename F>
     __device__ void histogram(bool mass, F bin_of, u64 ahead, double part, double want) {
         uint32_t* h = reinterpret_cast<uint32_t*>(aux);
-        for (int i = threadIdx.x; i < (mass ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
+        for (int i = threadIdx.x; i < (mass ? kPieces : 1) * kBins; i += kThreads) h[i] = 0;
         __syncthreads();
         each<1>([&](const float (&x)[4], int i) {
 #pragma unroll 1
@@ -510,10 +513,11 @@ struct Sampler {
                     continue;
                 }
                 const u64 w = weight_of(y);
-                const uint32_t p0 = uint32_t(w) & 0x7fffu, p1 = uint32_t(w >> 15) & 0x7fffu, p2 = uint32_t(w >> 30);
-                if (p0) atomicAdd(&h[b], p0);
-                if (p1) atomicAdd(&h[kBins + b], p1);
-                if (p2) atomicAdd(&h[2 * kBins + b], p2);
+#pragma unroll
+                for (int p = 0; p < kPieces; p++) {
+                    const uint32_t piece = uint32_t(w >> kPiece * p) & ((1u << kPiece) - 1);
+                    if (piece) atomicAdd(&h[p * kBins + b], piece);
+                }
             }
         });
         cluster.sync();
@@ -529,7 +533,9 @@ struct Sampler {
                 const int b = threadIdx.x * per + k;
                 if (k >= per || b >= share) continue;
                 v[k] += o[b];
-                if (mass) v[k] += (static_cast<u64>(o[kBins + b]) << 15) + (static_cast<u64>(o[2 * kBins + b]) << 30);
+                if (mass)
+#pragma unroll
+                    for (int p = 1; p < kPieces; p++) v[k] += static_cast<u64>(o[p * kBins + b]) << kPiece * p;
             }
         }
 #pragma unroll

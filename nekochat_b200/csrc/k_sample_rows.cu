@@ -90,8 +90,9 @@ struct Shared {
 // y = (m - x) c.
 struct Row {
     float m;        // largest value
-    float alone;    // where it is infinite, or the next value below weighs nothing: it, and values are read as 0 (it) and -infinity; else NaN
-    float low;      // values count as no less than this: they weigh nothing there
+    float from;     // NaN, or: values are read as their differences from it, the largest one
+    bool alone;     // the others then as -infinity: it is infinite, or the next value below weighs nothing
+    float low;      // values count as no less than this, 46.5 to 303 powers of two below: they weigh nothing there
     float c32;
     double m64, c, c_powers;  // c = log2(e) / temperature, times the table's powers
     float least;    // of the values that min-p leaves in
@@ -183,6 +184,8 @@ struct Sampler {
         if (v >= end) return make_uint4(none, none, none, none);
         return v == 0 || v == nv - 1 ? sh.ends[v != 0] : __ldg(data + v);
     }
+    // What a value is read as: see Row::from.
+    __device__ __forceinline__ float read(float x) const { return x == row.from ? 0.0f : row.alone ? -INFINITY : x - row.from; }
     // Values j0 .. j0 + 3 of a vector. Places outside the row hold -infinity.
     __device__ __forceinline__ void four(const uint4& w, int j0, float (&x)[4]) const {
         if constexpr (kPer == 4) {
@@ -193,9 +196,9 @@ struct Sampler {
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = float(y[j]);
         }
-        if (row.alone == row.alone)
+        if (row.from == row.from)
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = x[j] == row.alone ? 0.0f : -INFINITY;
+            for (int j = 0; j < 4; j++) x[j] = read(x[j]);
     }
     // f(four values, index of the first) of the vectors v0, v0 + step, .. before v1, kAhead of them on their way at a time.
     template <int kAhead, typename F>
@@ -916,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
     s.nv = n ? (ph + n + S::kPer - 1) / S::kPer : 0;
     s.first = b - ph;
     s.data = reinterpret_cast<const uint4*>(src - ph);
-    s.row.alone = NAN;
+    s.row.from = NAN;
     if (tid == 0) sh.best = 0xFFFFFFFFu, sh.n_all = 0, sh.total = 0, sh.cut = 0;
     const float asked = !a.u ? 0.0f : a.temperatures ? a.temperatures[r] : a.temperature;
     const float temperature = asked > 0.0f ? fminf(asked, 1e36f) : 0.0f;  // above, all weigh the same; NaN: greedy
@@ -974,12 +977,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const neko_sam
         return;
     }
 
-    if (!(fabsf(m) * 0x1p-25f * s.row.c32 < 64.0f)) {
-        s.row.alone = m;
-        g = g == m ? 0.0f : -INFINITY, m = 0.0f, s.row.m = 0.0f;
+    // Where the next value below m weighs 2^-128 of it or less, m is alone; else steps of the values near m are 256 powers of two at most,
+    // which bounds what low adds to 46.5. Where low would lie below the lowest finite value, all finite values are within a factor of
+    // 2 of m, so that differences from it are exact, and -infinity and places outside the row still weigh nothing.
+    s.row.alone = !(double(fabsf(m)) * 0x1p-25 * s.row.c < 64.0);
+    const double far = double(temperature) * (46.5 / 1.4426950408889634);
+    if (s.row.alone || double(m) - far < -double(FLT_MAX)) {
+        s.row.from = m;
+        g = s.read(g), m = 0.0f, s.row.m = 0.0f;
     }
     s.row.m64 = double(m);
-    s.row.low = nextafterf(m - 46.5f / s.row.c32, -INFINITY);
+    s.row.low = __double2float_rd(s.row.m64 - far);
     s.row.cut = s.row.least = -INFINITY, s.row.cut_at = 0;
     if (min_p > 0.0f) {  // the least float with (m - x) c <= -log2(min_p): near the quotient, then one by one
         const double lim = fmax(-log2(double(min_p)), 0.0);

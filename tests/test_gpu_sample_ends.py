@@ -1,12 +1,13 @@
 """neko_op_sample_rows where its ranges end: batches of every size (one to eight CTAs a row), the largest vocabularies with weights that
-are all alike. Tokens are equal to the definition's (drafts_reference.py), probabilities within one rounding to f32 and what 64 bits
-leave: 2^-23."""
+are all alike, temperatures down to the least f32, the lowest finite logits. Tokens are equal to the definition's
+(drafts_reference.py), probabilities within one rounding to f32 and what 64 bits leave: 2^-23."""
 import numpy as np
 import pytest
 
 from tests import drafts_reference as want_of
 
 pytestmark = pytest.mark.gpu
+LOWEST = -np.finfo(np.float32).max
 
 
 @pytest.fixture(scope="module")
@@ -56,6 +57,40 @@ def test_a_row_in_batches_of_every_size(torch, kind, V):
     u = np.array([0.0, 0.37, 0.5, 0.93, 1 - 2.0 ** -20])
     for params in ((0.8, 0, 0.9, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 5000, 0.9, 0.0), (0.8, 40, 0.95, 0.0), (1.0, 0, 1.0, 0.3)):
         check(torch, x, u, params, (1, 5, 40, 120, 200, 320))
+
+
+@pytest.mark.parametrize("T", [1e30, 100.0, 1e-30, 6e-32, 1.9e-32, 1e-33, 1e-35, 1e-38, 1e-45])
+@pytest.mark.parametrize("top", [0.0, 1e-25, -3e-22, 5.0])
+def test_temperatures_at_the_ends(torch, T, top):
+    """Tokens within some temperatures of the largest, and others far from it. The temperature is that of f32."""
+    rng = np.random.default_rng(5)
+    t = float(np.float32(T))
+    for V in (7, 3000, 40000):
+        x = np.float64(top) - np.minimum(t * rng.random((5, V)) * 60, 1e30) * (rng.random((5, V)) < 0.9)
+        x[rng.random((5, V)) < 0.3] = -5.0 if T < 1 else -np.inf
+        x[2:, 0] = top
+        x = x.astype(np.float32)
+        u = np.array([0.0, 0.37, 0.5, 0.93, 1 - 2.0 ** -20])
+        for params in ((t, 0, 1.0, 0.0), (t, 0, 0.9, 0.0), (t, 5, 0.9, 0.0), (t, 0, 1.0, 0.05), (t, 2000, 0.8, 0.0)):
+            check(torch, x, u, params, (5, 200))
+
+
+@pytest.mark.parametrize("T", [1.0, 1e29, 1e30, 3e34, 1e36])
+def test_the_lowest_values(torch, T):
+    """Rows just above the lowest finite value, beside tokens that cannot be taken and places outside the row."""
+    rng = np.random.default_rng(6)
+    t = float(np.float32(T))
+    for V in (1, 13, 3001, 30005):
+        x = LOWEST + np.abs(rng.standard_normal((5, V))) * np.array([t, 2 * t, 2e31, 2e31, 1e36])[:, None]
+        x[3] = LOWEST
+        x[4] = LOWEST + 3 * t
+        x[:3][rng.random((3, V)) < 0.5] = -np.inf
+        x[2][rng.random(V) < 0.2] = np.nan
+        x[:, V // 2] = LOWEST
+        x = x.astype(np.float32)
+        u = np.array([0.0, 0.37, 0.5, 0.93, 1 - 2.0 ** -20])
+        for params in ((t, 0, 1.0, 0.0), (t, 0, 0.9, 0.0), (t, 5, 0.9, 0.0), (t, 0, 1.0, 0.05), (t, 2000, 0.8, 0.0)):
+            check(torch, x, u, params, (5, 200))
 
 
 def unrounded(x, u, t, top_p):

@@ -50,6 +50,8 @@ constexpr int kRing = 4;
 constexpr int kPowers = 32, kCopies = 16;
 constexpr int kMaxCluster = 8;
 constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest
+constexpr double kSquare = 4503599627370496.0;  // 2^52: a sample's squares are added up in units of it
+static_assert(NEKO_MAX_VOCAB / 8 * (8 * kOne) * (8 * kOne) / kSquare < 0x1p63, "one token in 8, each for 8 of the largest weight");
 // lists of CTA 0 (as collected, then the sums; in order), the CTA's own list, the counts; histograms take all of it
 constexpr int kSortedOff = kCand * 8, kMineOff = 2 * kCand * 8;
 __host__ __device__ constexpr int counts_off(int ctas) { return kMineOff + (ctas > 1 ? kMine : kCand) * 8; }
@@ -721,7 +723,7 @@ struct Sampler {
             cluster.map_shared_rank(&sh, threadIdx.x)->others[rank][0] = s;
         }
         cluster.sync();
-        // ---- this CTA's share of the steps: what all their tokens weigh, by the middles, and the squares (in units of 2^-44) that the
+        // ---- this CTA's share of the steps: what all their tokens weigh, by the middles, and the squares that the
         // sample's error goes by
         const int share = kSteps / ctas, per = share / kThreads, step0 = rank * share + int(threadIdx.x) * per;
         uint32_t* merged = reinterpret_cast<uint32_t*>(aux) + threadIdx.x * per;
@@ -741,7 +743,7 @@ struct Sampler {
         auto weighed = [&](int k, u64& w, u64& q) {
             const uint32_t n = merged[k];
             const float one = middle(step0 + k, scale) * float(rate);
-            w = static_cast<u64>(n) * static_cast<u64>(one), q = static_cast<u64>(float(n) * one * (one * float(1.0 / kOne)));
+            w = static_cast<u64>(n) * static_cast<u64>(one), q = static_cast<u64>(float(n) * one * (one * float(1.0 / kSquare)));
         };
         u64 v[1] = {0}, q[1] = {0};
 #pragma unroll 1
@@ -766,7 +768,7 @@ struct Sampler {
         // The first steps at which the sum may and must have reached its part. What the sample makes of a beginning less p times all
         // is off by (1 - p) of what is in it and p of what is not: three standard deviations, and a little for the middles.
         const long long want_near = static_cast<long long>(double(top_p) * double(sum));
-        const float in = (1 - top_p) * (1 - top_p) * float(kOne), out = top_p * top_p * float(kOne), least = float(sum) * 0x1p-11f;
+        const float in = (1 - top_p) * (1 - top_p) * float(kSquare), out = top_p * top_p * float(kSquare), least = float(sum) * 0x1p-11f;
         auto margin = [&](u64 upto_q) {
             return rate > 1 ? static_cast<long long>(3.0f * sqrtf(in * float(upto_q) + out * float(sum_q - upto_q)) + least) : static_cast<long long>(least);
         };

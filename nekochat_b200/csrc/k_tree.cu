@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) tree_accept_kernel(const int32_t* __
 
 cudaError_t launch_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
                               int32_t* depth, cudaStream_t st) {
-    const int64_t blank = std::min<int64_t>((int64_t(tokens) * words + 4095) / 4096, num_sms());
+    const int64_t blank = std::min<int64_t>((int64_t(tokens) * (mask ? words : 1) + 4095) / 4096, num_sms());  // words counts with a mask only
     return launch_ex(tree_masks_kernel, dim3(unsigned(n_seq + blank)), dim3(kThreads), size_t(max_new) * 4, st, false, parent, q_start, n_seq, tokens,
                      max_new, mask, words, depth);
 }

@@ -11,10 +11,14 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// The sequence's nodes: its first row and how many; false: none, or rows that are not there (reported).
-__device__ __forceinline__ bool nodes_of(const int32_t* q_start, int s, int tokens, int max_new, int& row0, int& n) {
+// The sequence's first row and its number of nodes; false: it is left out, with more than max_new or rows that are not there.
+__device__ __forceinline__ bool rows_of(const int32_t* q_start, int s, int tokens, int max_new, int& row0, int& n) {
     row0 = q_start[s], n = q_start[s + 1] - row0;
-    if (row0 < 0 || n < 0 || n > max_new || row0 > tokens - n) {
+    return row0 >= 0 && n >= 0 && n <= max_new && row0 <= tokens - n;
+}
+// The same; false: none, or left out (reported, n < 0).
+__device__ __forceinline__ bool nodes_of(const int32_t* q_start, int s, int tokens, int max_new, int& row0, int& n) {
+    if (!rows_of(q_start, s, tokens, max_new, row0, n)) {
         if (threadIdx.x == 0) set_op_error(kErrBadIndex);
         n = -1;
     }
@@ -23,15 +27,35 @@ __device__ __forceinline__ bool nodes_of(const int32_t* q_start, int s, int toke
 
 // A thread for each node walks up to the root. Parents come before their children, so the bits of the node's words come from the
 // last to the first: each word is written once, from a register. The CTAs behind the sequences' set the rows of no sequence to
-// zero, which costs less than a fill before the kernel.
+// zero, which costs less than a fill before the kernel. Where the starts go down somewhere, sequences that are there may lie among the
+// rows that are to be cleared: each row is looked for in all of them then.
 __global__ void __launch_bounds__(kThreads) tree_masks_kernel(const int32_t* __restrict__ parent, const int32_t* __restrict__ q_start, int n_seq,
                                                              int tokens, int max_new, uint64_t* __restrict__ mask, int words, int32_t* __restrict__ depth) {
     extern __shared__ int32_t up[];
+    // whether the starts go down anywhere
+    auto unordered = [&]() {
+        int down = 0;
+        for (int i = threadIdx.x; i < n_seq; i += kThreads) down |= q_start[i + 1] < q_start[i];
+        return __syncthreads_or(down) != 0;
+    };
     // rows [from, to), by this CTA of `many`
-    auto clear = [&](int from, int to, int cta, int many) {
+    auto clear = [&](int from, int to, int cta, int many, bool mixed) {
         from = max(from, 0), to = min(to, tokens);
         if (from >= to) return;
         const int64_t at = int64_t(cta) * kThreads + threadIdx.x, step = int64_t(many) * kThreads;
+        if (mixed) {
+            for (int64_t row = from + at; row < to; row += step) {
+                bool free = true;
+                for (int s = 0; s < n_seq && free; s++) {
+                    int first, count;
+                    free = !rows_of(q_start, s, tokens, max_new, first, count) || row < first || row >= first + count;
+                }
+                if (free && mask)
+                    for (int w = 0; w < words; w++) mask[row * words + w] = 0;
+                if (free && depth) depth[row] = 0;
+            }
+            return;
+        }
         if (mask)
             for (int64_t i = int64_t(from) * words + at; i < int64_t(to) * words; i += step) mask[i] = 0;
         if (depth)
@@ -39,13 +63,17 @@ __global__ void __launch_bounds__(kThreads) tree_masks_kernel(const int32_t* __r
     };
     if (blockIdx.x >= n_seq) {
         const int cta = blockIdx.x - n_seq, many = gridDim.x - n_seq;
-        clear(0, q_start[0], cta, many);
-        clear(q_start[n_seq], tokens, cta, many);
+        const bool mixed = unordered();
+        clear(0, q_start[0], cta, many, mixed);
+        clear(q_start[n_seq], tokens, cta, many, mixed);
         return;
     }
     int row0, n;
     if (!nodes_of(q_start, blockIdx.x, tokens, max_new, row0, n)) {
-        if (n < 0) clear(row0, q_start[blockIdx.x + 1], 0, 1);
+        if (n < 0) {
+            const bool mixed = unordered();
+            clear(row0, q_start[blockIdx.x + 1], 0, 1, mixed);
+        }
         return;
     }
     for (int i = threadIdx.x; i < n; i += kThreads) up[i] = parent[row0 + i];

@@ -1,4 +1,4 @@
-"""neko_op_tree_masks with one of its outputs only."""
+"""neko_op_tree_masks with one of its outputs only, and with row starts that are out of order."""
 import numpy as np
 import pytest
 
@@ -41,3 +41,23 @@ def test_either_output_alone(torch, starts, tokens):
     got = torch.full((tokens, words), -7, dtype=torch.int64, device="cuda")
     call(torch, parent, at, n, got, words, None)
     assert np.array_equal(got.cpu().numpy().view(np.uint64), mask)
+
+
+@pytest.mark.parametrize("starts,good", [([0, 100, 300, 400], [(0, 100), (300, 400)]), ([100, 200, 150], [(100, 200)]),
+                                         ([0, 64, -1], [(0, 64)]), ([0, 64, 2000, 64, 128], [(0, 64), (64, 128)]),
+                                         ([0, 900, 10, 74], [(10, 74)]), ([500, 600, 0], [(500, 600)])])
+def test_a_sequence_left_out_leaves_the_others(torch, starts, good):
+    """Starts out of order: sequences that are there (and lie apart) have their masks and depths, all other rows are zeros."""
+    from nekochat_b200 import NekoError, ops
+    tokens, n = 700, 100
+    parent = np.full(tokens, -1, np.int32)
+    mask, depth = np.zeros((tokens, 2), np.uint64), np.zeros(tokens, np.int32)
+    for a, b in good:
+        parent[a:b] = np.arange(-1, b - a - 1)
+        mask[a:b], depth[a:b] = want_of.masks([parent[a:b].tolist()], 2)
+    d, at = torch.from_numpy(parent).cuda(), ints(torch, *starts)
+    for _ in range(20):
+        m, p = ops.tree_masks(d, at, n)
+        assert np.array_equal(m.cpu().numpy().view(np.uint64), mask) and np.array_equal(p.cpu().numpy(), depth)
+    with pytest.raises(NekoError, match="max_new"):
+        ops.status()

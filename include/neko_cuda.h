@@ -324,8 +324,8 @@ int neko_op_paged_copy(const neko_paged_planes* planes, const int32_t* src, cons
 
 /* A token for each row of logits [rows][vocab] (rows row_stride elements apart, any number; not changed), from the row's number u in [0, 1):
  * weights w_i = exp((x_i - max x) / temperature); of the tokens in descending order of x (equal ones by index) the first top_k
- * (0 or less: all), of those the shortest beginning whose weights add up to top_p times all of theirs (1 or more: all; at least
- * one), of those the ones with w_i >= min_p (values above 1 count as 1). Among what is left, in the order of the vocabulary, the
+ * (0 or less: all), of those the shortest beginning whose weights add up to top_p times all of theirs (1 or more, or NaN: all; at
+ * least one), of those the ones with w_i >= min_p (values above 1 count as 1, NaN as 0). Among what is left, in the order of the vocabulary, the
  * first token at which the sum of the weights exceeds u times their total. temperature not above 0, or NaN: the first maximum;
  * above 1e36: as 1e36. NaN and -infinity are never taken; +infinities share the weight. A row with nothing to take gives token -1, probability 0.
  * Weights are held to 2^-45 of the largest and added as integers: the result depends on no order.

@@ -482,7 +482,7 @@ def sample_rows(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         raise NekoError("sample_rows: a positive temperature needs the rows' numbers u")
     args = _SAMPLE.pack(logits.data_ptr(), _vector(u, "sample_rows u", types["f64"], rows, dev), *each, token.data_ptr(), prob.data_ptr(),
                         logits.stride(0) if rows > 1 else vocab, types.get(logits.dtype, -1), rows, vocab, max(-1, min(int(one[3]), 0x7fffffff)),
-                        *(max(-3e38, min(x, 3e38)) for x in one[:3]), 0)
+                        *(max(-3e38, min(x, 3e38)) if x == x else x for x in one[:3]), 0)
     rc = types["sample"](args, types["stream"](dev))
     if rc:
         check(rc, "sample_rows")

@@ -1,6 +1,8 @@
 """neko_op_sample_rows where its ranges end: batches of every size (one to eight CTAs a row), the largest vocabularies with weights that
-are all alike, temperatures down to the least f32, the lowest finite logits. Tokens are equal to the definition's
-(drafts_reference.py), probabilities within one rounding to f32 and what 64 bits leave: 2^-23."""
+are all alike, temperatures down to the least f32, the lowest finite logits, shares that are no numbers. Tokens are equal to the
+definition's (drafts_reference.py), probabilities within one rounding to f32 and what 64 bits leave: 2^-23."""
+import math
+
 import numpy as np
 import pytest
 
@@ -91,6 +93,19 @@ def test_the_lowest_values(torch, T):
         u = np.array([0.0, 0.37, 0.5, 0.93, 1 - 2.0 ** -20])
         for params in ((t, 0, 1.0, 0.0), (t, 0, 0.9, 0.0), (t, 5, 0.9, 0.0), (t, 0, 1.0, 0.05), (t, 2000, 0.8, 0.0)):
             check(torch, x, u, params, (5, 200))
+
+
+def test_shares_that_are_no_numbers(torch):
+    """top_p and min_p that are no numbers leave all tokens, as a number and as a row's."""
+    from nekochat_b200 import ops
+    x = torch.randn((64, 900), device="cuda")
+    u = torch.rand(64, dtype=torch.float64, device="cuda")
+    nan = torch.full((64,), math.nan, device="cuda")
+    for k in (0, 40):
+        token, prob = ops.sample_rows(x, u, 0.9, k)
+        for p, m in ((nan, 0.0), (1.0, nan), (math.nan, 0.0), (1.0, math.nan), (math.nan, math.nan)):
+            got = ops.sample_rows(x, u, 0.9, k, p, m)
+            assert torch.equal(got[0], token) and torch.equal(got[1], prob)
 
 
 def unrounded(x, u, t, top_p):

@@ -332,7 +332,7 @@ def _attend(what, q, k_pages, v_pages, table, kv_len, k_scale, v_scale, q_start,
     if mask is None:
         rc = types["attend"](args, types["stream"](dev))
     else:
-        words = mask.shape[1] if mask.dim() == 2 else -1
+        words = mask.shape[1]
         tree = _TREE.pack(_vector(mask, what + " mask", types["i64"], shape[0] * words, dev),
                           _vector(depth, what + " depth", i32, shape[0], dev), words, 0)
         rc = types["tree_attend"](args, tree, types["stream"](dev))
@@ -347,6 +347,8 @@ def paged_tree_attention(q, k_pages, v_pages, table, kv_len, mask, depth=None, k
     """neko_op_paged_tree_attention: paged_attention for the nodes of trees of drafted tokens, which are in the cache already:
     each sees the keys before the tree and the nodes of its mask (int64 [tokens][words], 64 nodes a word, as tree_masks
     gives it); positions (window, slopes) go by depth [tokens]. Returns out (shaped and typed like q)."""
+    if getattr(mask, "ndim", 0) != 2:
+        raise NekoError("paged_tree_attention: a mask [tokens][words]")
     return _attend("paged_tree_attention", q, k_pages, v_pages, table, kv_len, k_scale, v_scale, q_start, max_new, scale, softcap,
                    window, slopes, None, out, mask, depth)
 

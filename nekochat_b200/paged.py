@@ -129,7 +129,7 @@ class PagedCache:
         for s, n in news:
             if self.length[s] + n > self.max_len:
                 raise NekoError(f"PagedCache: sequence {s} would hold more than {self.max_len} tokens")
-            want.append(-(-(self.length[s] + n) // self.page) - len(self.held[s]))
+            want.append(max(-(-(self.length[s] + n) // self.page) - len(self.held[s]), 0))
         if sum(want) > len(self.free):
             raise NekoError(f"PagedCache: {sum(want)} pages wanted, {len(self.free)} free")
         for (s, _), w in zip(news, want):

@@ -313,8 +313,9 @@ typedef struct neko_paged_planes {
  * resident stay away; tokens at or past start[s] + count[s] are no longer the sequence's (what their places hold is not said).
  * start[s] < 0: inactive.
  * NEKO_T_E4M3: a page that gets tokens takes as scale the largest of its own (where tokens before start[s] are in it) and of the
- * pages that its tokens come from; codes are multiplied by old / new scale (exact, but for codes that become subnormal). A page
- * that gets tokens is in one sequence's table only, once. */
+ * pages that its tokens come from; codes are multiplied by old / new scale (exact, but for codes that become subnormal). A scale that
+ * a node raised when it was appended stays when the node is not kept: the page's other tokens were rounded for it then. A page that
+ * gets tokens is in one sequence's table only, once. */
 int neko_op_paged_compact(const neko_paged_planes* planes, const int32_t* start, const int32_t* path, int64_t path_stride,
                           const int32_t* count, int max_count, void* stream);
 /* In every plane, page dst[i] becomes a copy of page src[i] (its scales too), i < n (device arrays). A pair with an entry outside

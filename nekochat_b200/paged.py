@@ -273,7 +273,8 @@ class PagedDecoder:
         (ops.sample_rows) from numbers that seed, the answer's place and the token's decide. copies answers a prompt, one after
         the other in the result; the prompt goes through the model once. draft > 0: up to that many tokens are guessed
         each step from what the answer and its prompt hold (Drafts) and checked at once, which changes how fast the answers come and not
-        what they are, but for rounding. Prompts may be longer than one forward takes: they go through in pieces."""
+        what they are, but for rounding (with 8-bit pages a guess with large keys or values raises its page's scale, which stays when the
+        guess does not come true). Prompts may be longer than one forward takes: they go through in pieces."""
         import torch
         if not all(len(p) for p in prompts):
             raise NekoError("generate: an empty prompt")

@@ -1,4 +1,5 @@
-"""neko_op_tree_masks with one of its outputs only, and with row starts that are out of order."""
+"""neko_op_tree_masks with one of its outputs only, and with row starts that are out of order; what drafts that were not kept leave
+of an 8-bit page."""
 import numpy as np
 import pytest
 
@@ -61,3 +62,52 @@ def test_a_sequence_left_out_leaves_the_others(torch, starts, good):
         assert np.array_equal(m.cpu().numpy().view(np.uint64), mask) and np.array_equal(p.cpu().numpy(), depth)
     with pytest.raises(NekoError, match="max_new"):
         ops.status()
+
+
+def test_what_is_not_kept_leaves_its_scale(torch):
+    """8-bit pages: a node's values may raise its page's scale for the tokens before it and beside it, and the scale stays when the node is
+    not kept. The tokens that are kept stand within half a step of the page's scale: 2^-4 of themselves, or half the least step,
+    2^-10, of the scale; both once for each time that they are rounded (twice: as they come, and when the scale grows)."""
+    from nekochat_b200 import ops
+    ps, hd, ctx = 16, 64, 5
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn((ctx + 4, 1, hd), device="cuda", generator=g) for _ in range(2))
+    big = 300.0
+    k[ctx + 2] *= big  # node 2, a brother of node 3
+    pool = torch.zeros((2, 2, 1, ps, hd), dtype=torch.float8_e4m3fn, device="cuda")
+    scale, table = torch.ones((2, 2, 1), device="cuda"), ints(torch, 1, 0)[None]
+    put = lambda rows, at, **how: ops.paged_append(k[rows], v[rows], pool[0], pool[1], table, ints(torch, at), k_scale=scale[0], v_scale=scale[1],  # noqa: E731
+                                                   q_start=ints(torch, 0, k[rows].shape[0]), max_new=8, **how)
+    put(slice(0, ctx), 0)
+    before = scale.clone()
+    parent = ints(torch, -1, 0, 0, 0)
+    _, depth = ops.tree_masks(parent, ints(torch, 0, 4), 4)
+    put(slice(ctx, ctx + 4), ctx, depth=depth)
+    path, count, token = ops.tree_accept(ints(torch, 9, 1, 1, 8), ints(torch, 0, 3, 4, 9), parent, ints(torch, 0, 4), 4)
+    assert path.tolist() == [[0, 3, 0, 0]] and count.tolist() == [2] and token.tolist() == [8]
+    ops.paged_compact(pool, table, ints(torch, ctx), path, count, scale=scale)
+    ops.status()
+    assert scale[0, 1, 0] > 64 * before[0, 1, 0] and scale[1, 1, 0] <= 4 * before[1, 1, 0]
+    keep = [*range(ctx + 1), ctx + 3]
+    for i, x in enumerate((k, v)):
+        got = pool[i, 1, 0, :len(keep)].double() * scale[i, 1, 0].double()
+        want = x[keep, 0].double()
+        assert ((got - want).abs() <= 2 * (2.0 ** -4 * want.abs() * 1.0625 + 2.0 ** -10 * scale[i, 1, 0])).all()
+
+
+def test_drafts_on_8_bit_pages(torch):
+    """The answers' lengths, their first tokens (before any guess) and the pages are those of one token at a time."""
+    from nekochat_b200 import paged, workload
+    m = paged.build("qwen3-tiny", kind="e4m3", page=16, pages=60, max_len=256, perturb=True, max_seqs=12)
+    prompts = [workload.prompt(m.s, n, seed=i + 5).tolist() for i, n in enumerate((40, 1, 37))]
+    plain, steps, verify = m.generate(prompts, 40), [], m.verify
+    for draft in (1, 7, 70):
+        del steps[:]
+        m.verify = lambda *a: steps.append(1) or verify(*a)
+        try:
+            got = m.generate(prompts, 40, draft=draft)
+        finally:
+            del m.verify
+        assert [len(x) for x in got] == [40] * 3 and [x[0] for x in got] == [x[0] for x in plain]
+        assert all(0 <= t < m.s["vocab"] for x in got for t in x) and 0 < len(steps) < 40
+        assert len(m.cache.free) == 60 and not m.cache.held

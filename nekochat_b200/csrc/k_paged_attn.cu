@@ -26,9 +26,10 @@
 //
 // Trees of drafted tokens (neko_op_paged_tree_attention) differ in the groups that reach past the context: a lane reads the
 // 16 bits of its row's mask that the group's keys have, and where a window or a bias asks for positions, those go by depth. 12 f32
-// nodes on 777 f16 keys (16 heads on 8) take 12.8 us; 64 trees of up to 8 on 300 to 1,100 8-bit keys 74 us, where 16 f32 rows an item
-// (two columns each) are bound by instruction issue: 255 registers, one CTA an SM, 29 % of the SMs' issue and 19 % of the
-// memory rate; 16 rows in one pass, 4 warps in three CTAs or 6 in two: 73 to 102 us.
+// nodes on 777 f16 keys (16 heads on 8) take 12.5 us; 64 trees of up to 8 on 300 to 1,100 8-bit keys 72 us, where 16 f32 rows an item
+// (two columns each) are bound by latency: 255 registers leave two warps a scheduler, each of which issues every 5.9 cycles (1.6 of them
+// waiting for loads, 1.5 for the instruction before), 29 % of the SMs' issue and 19 % of the memory rate; 16 rows in one pass, 4 warps
+// in three CTAs or 6 in two: 73 to 102 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -21,9 +21,10 @@
 //    too many the key's digits (11, 11 and 10 bits) lead to the cut's value, whose equals are cut by index.
 // The draw goes through the slices in the order of the vocabulary: sums of CTAs, of warps' segments, of lanes.
 //
-// From a graph: 1 x 151,936 f32, k = 40, p = 0.95: 11.5 us (launch, two passes, the cluster's meetings); 64 x 50,257 bf16 with mixed
-// parameters 57 us, the time of the slowest rows (k = 1000, some 40 us alone; nuclei 35; k = 40 10); 320 x 151,936 nuclei 271 us
-// beside 30 for reading them once: 49 M weights in 64 bits, about 35 cycles a warp's 32, and the meetings.
+// From a graph: 1 x 151,936 f32, k = 40, p = 0.95: 11.2 us (launch, two passes, the cluster's meetings); 64 x 50,257 bf16 with mixed
+// parameters 59 us, the time of the slowest rows (k = 1000, some 40 us alone; nuclei 35; k = 40 10); 320 x 151,936 nuclei 261 us
+// beside 30 for reading them once: 49 M weights in 64 bits, about 35 cycles a warp's 32, and the meetings. Rows whose tokens are all
+// in one bin of a histogram wait for its additions, one after the other (200 flat rows of 262,144, a nucleus: 2.6 ms).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -279,8 +279,8 @@ int neko_op_paged_tree_append(const neko_paged_append_args* args, const int32_t*
 int neko_op_paged_tree_attention(const neko_paged_attention_args* args, const neko_tree* tree, void* stream);
 /* The masks and depths of trees given by parents: parent[q_start[s] + i] in [0, i) is node i's parent, counted from the
  * sequence's first node; anything else makes node i a root. Bit j of row i: j is i or an ancestor of i. Any of mask and depth may
- * be NULL. Rows of no sequence become zeros (with n_seq or max_new 0 nothing is written). At most NEKO_MAX_NODES nodes a
- * sequence. */
+ * be NULL; words counts where there is a mask. Rows of no sequence, and of those left out, become zeros (with n_seq or max_new 0
+ * nothing is written). At most NEKO_MAX_NODES nodes a sequence. */
 #define NEKO_MAX_NODES 4096
 int neko_op_tree_masks(const int32_t* parent, const int32_t* q_start, int n_seq, int tokens, int max_new, uint64_t* mask, int words,
                        int32_t* depth, void* stream);
